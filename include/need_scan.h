@@ -234,6 +234,80 @@ typedef struct {
     double eps;             /* denominator floor (the reference's 1e-6) */
 } need_assoc_step_args;
 
+/* need_scan_train_forward / need_scan_train_backward: the GATED and SSD scans
+ * with what their gradient needs. */
+typedef struct {
+    int32_t form;           /* NEED_FORM_GATED or NEED_FORM_SSD */
+    int32_t dtype;          /* need_dtype of in[], out, gout and grad[] */
+    int32_t checkpoint;     /* 0: the backward reads in[]; 1: it reads the 8-bit copies */
+    int64_t nb, T, C;       /* C a multiple of 16 bytes' worth of elements */
+    need_view in[5];        /* as need_scan_args.in (stride_h unused); backward: unused with checkpoint */
+    const float* d_skip;    /* SSD: [C] fp32 */
+    double dt_min, dt_max;  /* SSD: 0 <= dt_min <= dt_max */
+    const float* h0;        /* forward: optional [nb, C] fp32 initial state */
+    const uint8_t* seg_start; /* optional reset mask [nb, T] */
+    int64_t seg_stride_b, seg_stride_t;
+    float* states;          /* [nb, ceil(T / need_scan_train_chunk_len()), C] fp32: the state entering
+                               each chunk; written by the forward, read by the backward */
+    uint8_t* ckpt_values;   /* checkpoint: [nin][nb][T][G * 64] e4m3, G = ceil(C / 64), nin = 3 (GATED)
+                               or 5 (SSD), in in[] order; 16-byte aligned */
+    uint8_t* ckpt_scales;   /* checkpoint: [nin][nb][T][G], exponent + 127 (255: not finite) */
+    void* out;              /* forward: [nb, T, C], 16-byte aligned rows */
+    int64_t out_stride_b, out_stride_t;
+    float* h_final;         /* forward: optional [nb, C] fp32 state after the last token */
+    need_view gout;         /* backward: gradient of out */
+    const float* g_final;   /* backward: optional [nb, C] gradient of h_final */
+    void* grad[5];          /* backward: gradients of in[], [nb, T, C] contiguous */
+    float* grad_h0;         /* backward: optional [nb, C] gradient of the initial state */
+    float* grad_d;          /* backward, SSD: [C] gradient of d_skip */
+    void* workspace;        /* >= need_scan_train_workspace_size(...) bytes, 16-byte aligned; the call
+                               clears what it needs, nothing in it outlives the call */
+    size_t workspace_bytes;
+} need_scan_train_args;
+
+/* need_conv_silu_train_forward / _backward: the SSD block's conv + SiLU. */
+typedef struct {
+    int32_t dtype;          /* u, out, gout and grad_u */
+    int32_t K;              /* taps, 1..4 */
+    int64_t nb, T, C;       /* C a multiple of 4 */
+    const void* u;          /* [nb, T, C], channel stride 1, rows aligned to 4 elements */
+    int64_t u_stride_b, u_stride_t;
+    const float* weight;    /* [C, K] contiguous fp32 taps, oldest first */
+    const float* bias;      /* optional [C] fp32 */
+    const uint8_t* seg_start; /* optional reset mask [nb, T] */
+    int64_t seg_stride_b, seg_stride_t;
+    void* out;              /* forward: [nb, T, C] contiguous */
+    const void* gout;       /* backward: [nb, T, C], as u */
+    int64_t gout_stride_b, gout_stride_t;
+    void* grad_u;           /* backward: [nb, T, C] contiguous */
+    float* grad_wb;         /* backward: [C, K + 1] fp32: the taps' gradients, then the bias's */
+    void* workspace;        /* backward: >= need_conv_silu_train_workspace_size(...) bytes */
+    size_t workspace_bytes;
+} need_conv_train_args;
+
+/* need_rms_norm_train_forward / _backward: RMSNorm over rows of C channels. */
+typedef struct {
+    int32_t dtype;          /* x, out, gout and grad_x */
+    int32_t checkpoint;     /* 0: the backward reads x; 1: it reads the 8-bit copy */
+    int64_t rows, C;        /* C a multiple of 16 bytes' worth of elements, rows of at most 32 KB */
+    int64_t C_mean;         /* channels the mean is taken over (<= C; those past it hold zeros) */
+    const void* x;          /* [rows, C], channel stride 1, 16-byte aligned rows; backward: unused
+                               with checkpoint */
+    int64_t x_stride;
+    const float* weight;    /* [C] fp32, 16-byte aligned */
+    double eps;
+    void* out;              /* forward: [rows, C] contiguous */
+    float* rstd;            /* [rows] fp32: written by the forward, read by the backward */
+    uint8_t* ckpt_values;   /* checkpoint: [rows, C] e4m3, 8-byte aligned */
+    uint8_t* ckpt_scales;   /* checkpoint: [rows, ceil(C / 64)] */
+    const void* gout;       /* backward: [rows, C] */
+    int64_t gout_stride;
+    void* grad_x;           /* backward: [rows, C] contiguous */
+    float* grad_weight;     /* backward: [C] fp32 */
+    void* workspace;        /* backward: >= need_rms_norm_train_workspace_size(...) bytes */
+    size_t workspace_bytes;
+} need_norm_train_args;
+
 /* Version of this header the library was built from. */
 NEED_API int need_abi_version(void);
 
@@ -406,6 +480,61 @@ NEED_API int need_assoc_memory(const need_assoc_args* args, need_stream_t stream
  * order.  state and denom are read and written in place (one sequence per
  * row, or per slot[i]); sequences must not share a slot within one call. */
 NEED_API int need_assoc_memory_step(const need_assoc_step_args* args, need_stream_t stream);
+
+/* ------------------------------------------------------------------------ */
+/* Training: forward and backward                                            */
+/* ------------------------------------------------------------------------ */
+
+/* Tokens from one kept state to the next (the training scans' chunk length). */
+NEED_API int64_t need_scan_train_chunk_len(void);
+
+/* Channels of one token that share a scale in an 8-bit checkpoint. */
+NEED_API int64_t need_scan_train_group(void);
+
+/* Workspace bytes of a training scan of this shape (0 for sizes it does not take). */
+NEED_API size_t need_scan_train_workspace_size(int32_t form, int32_t backward, int64_t nb, int64_t T, int64_t C);
+
+/* The GATED or SSD scan for training (need_core.py:1630-1642 computes it with
+ * torch ops under grad).  Gates, states and epilogue are fp32, rounded once to
+ * `dtype`: the reference's GPU kernel's precision (need_kernels.py:119-144), not
+ * need_gated_scan's and need_ssd_scan's 16-bit gates.  Writes out, states,
+ * optionally h_final and (checkpoint) the 8-bit copies of in[]: per token and 64
+ * channels, value = e4m3(x / 2^e) with e the least exponent >= -126 that fits
+ * every |x| under 448 * 2^e.  A reset drops the state before it whatever it
+ * holds (an infinity or NaN included). */
+NEED_API int need_scan_train_forward(const need_scan_train_args* args, need_stream_t stream);
+
+/* Its gradient: from gout (and g_final) the gradients of in[], h0 and d_skip.
+ * The states are run again inside each chunk from `states`.  With checkpoint,
+ * every gate and gradient is taken at the stored 8-bit values (a group that
+ * held an infinity or NaN reads as NaN).  form, sizes, d_skip, dt_min / dt_max,
+ * seg_start, states and the checkpoint as the forward's.  Results do not
+ * depend on the order in which blocks run. */
+NEED_API int need_scan_train_backward(const need_scan_train_args* args, need_stream_t stream);
+
+/* Workspace bytes of need_conv_silu_train_backward. */
+NEED_API size_t need_conv_silu_train_workspace_size(int32_t K, int64_t nb, int64_t T, int64_t C);
+
+/* out = silu(bias + causal depthwise conv_K(u)) (need_core.py:1620-1622) in fp32,
+ * rounded once to `dtype`.  With seg_start, inputs before a token's segment
+ * start count as 0. */
+NEED_API int need_conv_silu_train_forward(const need_conv_train_args* args, need_stream_t stream);
+
+/* Its gradient: grad_u, and the taps' and the bias's sums over all tokens. */
+NEED_API int need_conv_silu_train_backward(const need_conv_train_args* args, need_stream_t stream);
+
+/* Workspace bytes of need_rms_norm_train_backward. */
+NEED_API size_t need_rms_norm_train_workspace_size(int64_t rows, int64_t C);
+
+/* out = x * rstd * weight, rstd = 1 / sqrt(sum(x^2) / C_mean + eps), per row in
+ * fp32, rounded once (need_kernels.py:99-107); optionally keeps x in 8 bits as
+ * need_scan_train_forward does. */
+NEED_API int need_rms_norm_train_forward(const need_norm_train_args* args, need_stream_t stream);
+
+/* Its gradient: with n = x rstd and g = weight gout,
+ * grad_x = rstd (g - n sum(g n) / C_mean), grad_weight = sum over rows of gout n.
+ * With checkpoint, x is the stored 8-bit values and rstd the true row's. */
+NEED_API int need_rms_norm_train_backward(const need_norm_train_args* args, need_stream_t stream);
 
 /* ------------------------------------------------------------------------ */
 /* Ragged decode / speculative verify                                        */

@@ -113,6 +113,40 @@ class NeedAssocStepArgs(Structure):
     ]
 
 
+class NeedScanTrainArgs(Structure):
+    _fields_ = [
+        ("form", c_int32), ("dtype", c_int32), ("checkpoint", c_int32),
+        ("nb", c_int64), ("T", c_int64), ("C", c_int64),
+        ("in_", NeedView * 5), ("d_skip", c_void_p), ("dt_min", c_double), ("dt_max", c_double),
+        ("h0", c_void_p), ("seg_start", c_void_p), ("seg_stride_b", c_int64), ("seg_stride_t", c_int64),
+        ("states", c_void_p), ("ckpt_values", c_void_p), ("ckpt_scales", c_void_p),
+        ("out", c_void_p), ("out_stride_b", c_int64), ("out_stride_t", c_int64), ("h_final", c_void_p),
+        ("gout", NeedView), ("g_final", c_void_p), ("grad", c_void_p * 5), ("grad_h0", c_void_p),
+        ("grad_d", c_void_p), ("workspace", c_void_p), ("workspace_bytes", c_size_t),
+    ]
+
+
+class NeedConvTrainArgs(Structure):
+    _fields_ = [
+        ("dtype", c_int32), ("K", c_int32), ("nb", c_int64), ("T", c_int64), ("C", c_int64),
+        ("u", c_void_p), ("u_stride_b", c_int64), ("u_stride_t", c_int64),
+        ("weight", c_void_p), ("bias", c_void_p),
+        ("seg_start", c_void_p), ("seg_stride_b", c_int64), ("seg_stride_t", c_int64),
+        ("out", c_void_p), ("gout", c_void_p), ("gout_stride_b", c_int64), ("gout_stride_t", c_int64),
+        ("grad_u", c_void_p), ("grad_wb", c_void_p), ("workspace", c_void_p), ("workspace_bytes", c_size_t),
+    ]
+
+
+class NeedNormTrainArgs(Structure):
+    _fields_ = [
+        ("dtype", c_int32), ("checkpoint", c_int32), ("rows", c_int64), ("C", c_int64), ("C_mean", c_int64),
+        ("x", c_void_p), ("x_stride", c_int64), ("weight", c_void_p), ("eps", c_double),
+        ("out", c_void_p), ("rstd", c_void_p), ("ckpt_values", c_void_p), ("ckpt_scales", c_void_p),
+        ("gout", c_void_p), ("gout_stride", c_int64), ("grad_x", c_void_p), ("grad_weight", c_void_p),
+        ("workspace", c_void_p), ("workspace_bytes", c_size_t),
+    ]
+
+
 # every symbol the header declares, with (restype, argtypes)
 SIGNATURES = {
     "need_abi_version": (c_int32, []),
@@ -138,6 +172,17 @@ SIGNATURES = {
     "need_ragged_verify": (c_int32, [POINTER(NeedVerifyArgs), c_void_p]),
     "need_segment_starts": (c_int32, [POINTER(NeedSegmentArgs), c_void_p]),
     "need_ssd_conv_silu": (c_int32, [POINTER(NeedConvArgs), c_void_p]),
+    "need_scan_train_chunk_len": (c_int64, []),
+    "need_scan_train_group": (c_int64, []),
+    "need_scan_train_workspace_size": (c_size_t, [c_int32, c_int32, c_int64, c_int64, c_int64]),
+    "need_scan_train_forward": (c_int32, [POINTER(NeedScanTrainArgs), c_void_p]),
+    "need_scan_train_backward": (c_int32, [POINTER(NeedScanTrainArgs), c_void_p]),
+    "need_conv_silu_train_workspace_size": (c_size_t, [c_int32, c_int64, c_int64, c_int64]),
+    "need_conv_silu_train_forward": (c_int32, [POINTER(NeedConvTrainArgs), c_void_p]),
+    "need_conv_silu_train_backward": (c_int32, [POINTER(NeedConvTrainArgs), c_void_p]),
+    "need_rms_norm_train_workspace_size": (c_size_t, [c_int64, c_int64]),
+    "need_rms_norm_train_forward": (c_int32, [POINTER(NeedNormTrainArgs), c_void_p]),
+    "need_rms_norm_train_backward": (c_int32, [POINTER(NeedNormTrainArgs), c_void_p]),
     "need_commit_states": (c_int32, [c_int32, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p,
                                      c_void_p, c_void_p]),
     "need_sp_local_scan": (c_int32, [POINTER(NeedScanArgs), c_int32, c_void_p]),

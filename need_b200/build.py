@@ -21,8 +21,9 @@ CSRC = os.path.join(HERE, "csrc")
 INCLUDE = os.path.join(ROOT, "include")
 LIBDIR = os.path.join(HERE, "_lib")
 LIB = os.path.join(LIBDIR, "libneed_scan.so")
-SOURCES = ["need_scan.cu", "decode.cu", "sp.cu", "noalloc.cu", "segments.cu", "prologue.cu", "epilogue.cu", "assoc.cu"]
-HEADERS = ["ptx.cuh", "scan_kernel.cuh", "host_common.h"]
+SOURCES = ["need_scan.cu", "decode.cu", "sp.cu", "noalloc.cu", "segments.cu", "prologue.cu", "epilogue.cu", "assoc.cu",
+           "train_scan.cu", "train_conv.cu", "train_norm.cu"]
+HEADERS = ["ptx.cuh", "scan_kernel.cuh", "host_common.h", "umma.cuh", "train_common.cuh"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 

@@ -100,6 +100,9 @@ int rms_norm_rows(int32_t dtype, const void* x, int64_t xsb, int64_t xst, void* 
                   int64_t nb, int64_t T, int64_t C, const void* weight, int32_t weight_dtype, double eps,
                   cudaStream_t stream);
 
+// Look-back polls before a wait gives up (need_scan.cu; need_test_set_lookback_polls lowers it).
+uint32_t lookback_polls();
+
 inline int dtype_bytes(int dt) { return dt == NEED_F32 ? 4 : 2; }
 inline bool dtype_ok(int dt) { return dt == NEED_F32 || dt == NEED_BF16 || dt == NEED_F16; }
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }

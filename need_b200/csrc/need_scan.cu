@@ -363,8 +363,7 @@ int prepare(const need_scan_args* a, int expect_form, Plan* pl, ScanParams* P, b
     P->tile_carry = a->tile_carry;
     unsigned char* ws = static_cast<unsigned char*>(a->workspace);
     P->hdr = reinterpret_cast<uint32_t*>(ws);
-    const uint32_t polls = g_lookback_polls.load(std::memory_order_relaxed);
-    P->lb_polls = polls != 0 ? polls : kLookbackPolls;
+    P->lb_polls = need::lookback_polls();
     P->agg = reinterpret_cast<ulonglong2*>(ws + WS_HDR_WORDS * 4);
     P->incl = P->agg + size_t(g.ntiles) * pl->CB;
     return NEED_OK;
@@ -398,6 +397,11 @@ int sp_list_of(const need_scan_args* a, ScanParams* P) {
 }  // namespace
 
 namespace need {
+uint32_t lookback_polls() {
+    const uint32_t polls = g_lookback_polls.load(std::memory_order_relaxed);
+    return polls != 0 ? polls : kLookbackPolls;
+}
+
 // The gated scan kernel in fix-up mode over the slice described by `a`: it
 // rewrites the tiles that the deferring local scan listed in a->sp_list (and
 // whose rounded updates b it left in their output rows), entering each from the local scan's tile_prod / tile_carry and

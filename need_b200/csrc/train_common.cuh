@@ -1,0 +1,88 @@
+// train_common.cuh -- what the training kernels share: gates with both
+// halves of a sigmoid, the 8-bit checkpoint format, a fixed-order column sum.
+#pragma once
+
+#include <cuda_fp8.h>
+
+#include "scan_kernel.cuh"
+
+namespace need {
+
+// ------------------------------------------------------------------ gates
+// s = sigmoid(x) and n = 1 - s = sigmoid(-x) of a pair, both with full relative
+// precision: t = e^-x, s = 1 / (1 + t), n = t s.  16-bit streams use the
+// hardware exp2 and reciprocal (about 1e-7 relative, against the 2^-9 and 2^-12
+// of the rounding that follows); fp32 streams the library exp and IEEE division.
+template <typename T>
+__device__ __forceinline__ void sig_pair(float2 x, float2& s, float2& n) {
+    if constexpr (Ops<T>::BYTES == 4) {
+        const float t0 = expf(-fabsf(x.x)), t1 = expf(-fabsf(x.y));
+        const float r0 = __fdiv_rn(1.0f, 1.0f + t0), r1 = __fdiv_rn(1.0f, 1.0f + t1);
+        const float m0 = t0 * r0, m1 = t1 * r1;
+        s = make_float2(x.x < 0.0f ? m0 : r0, x.y < 0.0f ? m1 : r1);
+        n = make_float2(x.x < 0.0f ? r0 : m0, x.y < 0.0f ? r1 : m1);
+    } else {
+        // the exponent is capped at 2^126, so that t s stays a number; a NaN passes through
+        const float2 k = fmul2(x, splat2(-1.4426950408889634f));
+        float e0, e1, t0, t1;
+        asm("min.NaN.f32 %0, %1, 0f42FC0000;" : "=f"(e0) : "f"(k.x));
+        asm("min.NaN.f32 %0, %1, 0f42FC0000;" : "=f"(e1) : "f"(k.y));
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(t0) : "f"(e0));
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(t1) : "f"(e1));
+        const float2 d = fadd2(make_float2(t0, t1), splat2(1.0f));
+        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s.x) : "f"(d.x));
+        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s.y) : "f"(d.y));
+        n = fmul2(make_float2(t0, t1), s);
+    }
+}
+
+// a = e^-r and n = 1 - a of a pair, r >= 0.  fp32: expm1.  16 bit: below 2^-4
+// the first five terms of the series of 1 - e^-r (the next is r^5 / 720 of it,
+// 1.3e-9), above it the difference (2^-24 / 2^-4 relative).
+template <typename T>
+__device__ __forceinline__ void exp_neg(float2 r, float2& a, float2& n) {
+    if constexpr (Ops<T>::BYTES == 4) {
+        a = make_float2(expf(-r.x), expf(-r.y));
+        n = make_float2(-expm1f(-r.x), -expm1f(-r.y));
+    } else {
+        a = make_float2(exp_approx(-r.x), exp_approx(-r.y));
+        float2 q = ffma2(r, splat2(1.0f / 120.0f), splat2(-1.0f / 24.0f));
+        q = ffma2(r, q, splat2(1.0f / 6.0f));
+        q = ffma2(r, q, splat2(-0.5f));
+        q = ffma2(r, q, splat2(1.0f));
+        q = fmul2(r, q);
+        n = make_float2(r.x < 0.0625f ? q.x : 1.0f - a.x, r.y < 0.0625f ? q.y : 1.0f - a.y);
+    }
+}
+
+// ------------------------------------------------------------------ 8 bits
+// A group's scale is 2^e, e the least exponent >= -126 with every |value| <=
+// 448 * 2^e (448: e4m3's largest), kept as the byte e + 127; 255 marks a group
+// that holds an infinity or NaN and reads back as NaN.  `top` is the bit
+// pattern of the group's largest magnitude.  A power of two scales without
+// rounding, so a value is rounded once, by the conversion.
+__device__ __forceinline__ uint32_t e4m3_scale_byte(uint32_t top) {
+    const int b = static_cast<int>(top >> 23) - 8 + ((top & 0x7fffffu) > 0x600000u ? 1 : 0);
+    return top >= 0x7f800000u ? 255u : static_cast<uint32_t>(b < 1 ? 1 : b);
+}
+__device__ __forceinline__ float e4m3_scale(uint32_t byte) {
+    return __uint_as_float(byte == 255u ? 0x7fc00000u : byte << 23);
+}
+__device__ __forceinline__ uint16_t e4m3_pair(float2 x, uint32_t byte) {
+    const float inv = __uint_as_float((254u - min(byte, 253u)) << 23);  // 2^-e
+    return __nv_cvt_float2_to_fp8x2(make_float2(x.x * inv, x.y * inv), __NV_SATFINITE, __NV_E4M3);
+}
+
+// ------------------------------------------------------------------ TMA
+__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* tm, int c0, int c1, int c2, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(smem_addr(dst)),
+        "l"(tm), "r"(c0), "r"(c1), "r"(c2), "r"(smem_addr(bar))
+        : "memory");
+}
+
+// out[c] = sum over rows of part[row][c], in a fixed order (train_norm.cu).
+int column_sums(const float* part, int64_t rows, int64_t C, float* out, cudaStream_t stream);
+
+}  // namespace need

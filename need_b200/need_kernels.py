@@ -26,8 +26,10 @@ New entry points (no ``need_kernels`` counterpart): ``gated_scan``
 ``segment_starts`` (reset mask of packed token windows), ``ssd_conv_silu`` and
 ``ssd_scan_rms_norm`` (the SSD block's prologue, and its scan with the
 out_norm fused), ``linear_associative_memory`` (HierarchicalMemory's
-matrix-state memory, need_core.py:1960-2001), and the pieces of the
-sequence-parallel scan used by ``need_b200.sp``.
+matrix-state memory, need_core.py:1960-2001), the pieces of the
+sequence-parallel scan used by ``need_b200.sp``, and the block's operators for
+training, with gradients (``need_b200.train``): ``gated_scan_train``,
+``ssd_scan_train``, ``ssd_conv_silu_train`` and ``rms_norm_train``.
 """
 from __future__ import annotations
 
@@ -40,6 +42,7 @@ import torch
 import torch.nn.functional as F
 
 from . import abi
+from .train import gated_scan_train, rms_norm_train, ssd_conv_silu_train, ssd_scan_train  # noqa: F401
 
 HAS_TRITON = False  # the reference's flag: this module uses no Triton
 
