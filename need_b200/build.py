@@ -1,11 +1,14 @@
-"""Builds need_b200/_lib/libneed_scan.so from need_b200/csrc with nvcc for sm_100a.
+"""Builds need_b200/_lib/libneed_scan.so from need_b200/csrc with nvcc for sm_100a,
+and need_b200/_lib/_train.so, the autograd nodes of need_b200.train over it, with
+the host compiler against torch's headers.
 
     python -m need_b200.build            # build if sources changed
     python -m need_b200.build --force
 
 The library is built in-tree so it travels with the repository; there is no
 JIT path.  Flags: -gencode arch=compute_100a,code=sm_100a (B200 only), -O3,
--lineinfo (source-level ncu attribution), static cudart.
+-lineinfo (source-level ncu attribution), static cudart.  libneed_scan.so does
+not depend on torch.
 """
 from __future__ import annotations
 
@@ -21,6 +24,8 @@ CSRC = os.path.join(HERE, "csrc")
 INCLUDE = os.path.join(ROOT, "include")
 LIBDIR = os.path.join(HERE, "_lib")
 LIB = os.path.join(LIBDIR, "libneed_scan.so")
+EXT = os.path.join(LIBDIR, "_train.so")
+EXT_SOURCE = "train_autograd.cpp"
 SOURCES = ["need_scan.cu", "decode.cu", "sp.cu", "noalloc.cu", "segments.cu", "prologue.cu", "epilogue.cu", "assoc.cu",
            "train_scan.cu", "train_conv.cu", "train_norm.cu"]
 HEADERS = ["ptx.cuh", "scan_kernel.cuh", "host_common.h", "umma.cuh", "train_common.cuh"]
@@ -34,19 +39,52 @@ def nvcc() -> str:
     raise RuntimeError("nvcc not found (set NVCC)")
 
 
-def _stale() -> bool:
-    if not os.path.exists(LIB):
+def _older(target: str, deps) -> bool:
+    if not os.path.exists(target):
         return True
-    t = os.path.getmtime(LIB)
-    deps = [os.path.join(CSRC, f) for f in SOURCES + HEADERS] + [os.path.join(INCLUDE, "need_scan.h")]
+    t = os.path.getmtime(target)
     return any(os.path.getmtime(d) > t for d in deps)
 
 
+def _stale() -> bool:
+    return _older(LIB, [os.path.join(CSRC, f) for f in SOURCES + HEADERS] + [os.path.join(INCLUDE, "need_scan.h")])
+
+
+def _ext_stale() -> bool:
+    return _older(EXT, [os.path.join(CSRC, EXT_SOURCE), os.path.join(INCLUDE, "need_scan.h")])
+
+
+def _ext_command() -> list:
+    """The host compile of the autograd module (no torch import: its headers are found by path)."""
+    import importlib.util
+    import sysconfig
+    torch_dir = os.path.dirname(importlib.util.find_spec("torch").origin)
+    inc = [os.path.join(torch_dir, "include"), os.path.join(torch_dir, "include", "torch", "csrc", "api", "include"),
+           sysconfig.get_path("include"), os.path.join(os.path.dirname(os.path.dirname(nvcc())), "include")]
+    return [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-shared",
+            "-DTORCH_EXTENSION_NAME=_train", "-DTORCH_API_INCLUDE_EXTENSION_H", f"-I{INCLUDE}",
+            *[x for d in inc for x in ("-isystem", d)], os.path.join(CSRC, EXT_SOURCE), "-o", EXT + ".tmp",
+            "-L" + os.path.join(torch_dir, "lib"), "-L" + LIBDIR, "-l:libneed_scan.so", "-lc10", "-lc10_cuda", "-ltorch",
+            "-ltorch_cpu", "-ltorch_python", "-Wl,-rpath,$ORIGIN"]
+
+
 def build(force: bool = False, verbose: bool = False) -> str:
-    """Compiles the shared library if needed; returns its path."""
-    if not force and not _stale():
-        return LIB
+    """Compiles the shared library and the autograd module if needed; returns the library's path."""
     os.makedirs(LIBDIR, exist_ok=True)
+    if force or _stale():
+        _build_lib(verbose)
+    if force or _ext_stale():
+        cmd = _ext_command()
+        if verbose:
+            print(" ".join(cmd), file=sys.stderr)
+        p = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT)
+        if p.returncode != 0:
+            raise RuntimeError(f"--- {EXT_SOURCE}\n{p.stdout.decode(errors='replace')}")
+        os.replace(EXT + ".tmp", EXT)
+    return LIB
+
+
+def _build_lib(verbose: bool) -> None:
     objdir = os.path.join(LIBDIR, "obj")
     os.makedirs(objdir, exist_ok=True)
     common = [nvcc(), *ARCH, "-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC,-fvisibility=hidden",
@@ -72,7 +110,6 @@ def build(force: bool = False, verbose: bool = False) -> str:
            "-Xlinker", "--exclude-libs,ALL"]
     subprocess.run(cmd, check=True)
     os.replace(tmp, LIB)
-    return LIB
 
 
 def main() -> None:

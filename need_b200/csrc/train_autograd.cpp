@@ -1,0 +1,315 @@
+// train_autograd.cpp -- the autograd nodes of need_b200.train, over the C ABI
+// of libneed_scan.so (module need_b200._lib._train).
+//
+// A training pass of a small call is bound by the host, not the GPU: as Python
+// autograd functions over ctypes these operators took 160 to 390 us a pass
+// where their kernels took 20 to 60.  The nodes, their argument structs and
+// their allocations are therefore here; need_b200/train.py checks the arguments
+// and documents the operators.
+//
+// Nothing is kept between calls: outputs, saved tensors and scratch come from
+// torch's allocator on the current stream, so a call can be captured into a
+// graph and run on any stream.
+#include <c10/cuda/CUDAGuard.h>
+#include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
+#include <torch/extension.h>
+
+#include <string>
+
+#include "need_scan.h"
+
+using at::Tensor;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+namespace {
+
+constexpr int64_t kSpan = 64, kGroup = 64;  // need_scan_train_chunk_len(), need_scan_train_group()
+
+void check(const char* fn, int rc) {
+    TORCH_CHECK(rc == NEED_OK, fn, " failed (status ", rc, "): ", need_last_error());
+}
+
+int32_t dtype_of(const Tensor& t) {
+    switch (t.scalar_type()) {
+        case at::kFloat: return NEED_F32;
+        case at::kBFloat16: return NEED_BF16;
+        case at::kHalf: return NEED_F16;
+        default: TORCH_CHECK_TYPE(false, "fp32, bf16 or f16 expected; got ", t.scalar_type());
+    }
+}
+
+// `t` with channel stride 1, a 16-byte aligned base and positive row strides of
+// whole 16 bytes (dims of size 1 excepted); a copy if it is laid out otherwise.
+Tensor rows(const Tensor& t) {
+    const int64_t es = t.element_size(), d = t.dim();
+    bool ok = reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0 && (t.stride(d - 1) == 1 || t.size(d - 1) == 1);
+    for (int64_t i = 0; i + 1 < d; ++i) ok = ok && (t.size(i) == 1 || (t.stride(i) > 0 && t.stride(i) * es % 16 == 0));
+    return ok ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+
+Tensor scratch(const Tensor& like, size_t bytes) {
+    return at::empty({static_cast<int64_t>(bytes)}, like.options().dtype(at::kByte));
+}
+Tensor floats(const Tensor& like, at::IntArrayRef shape) { return at::empty(shape, like.options().dtype(at::kFloat)); }
+template <typename T = void>
+T* ptr(const Tensor& t) {
+    return t.defined() ? static_cast<T*>(t.data_ptr()) : nullptr;
+}
+need_view view(const Tensor& t) { return need_view{t.const_data_ptr(), t.stride(0), 0, t.stride(1)}; }
+
+using OptTensor = std::optional<Tensor>;
+Tensor or_none(const OptTensor& t) { return t.has_value() ? *t : Tensor(); }
+OptTensor opt(const Tensor& t) { return t.defined() ? OptTensor(t) : std::nullopt; }
+
+// The current stream of t's device, which is made current for the guard's life.
+struct On {
+    explicit On(const Tensor& t) : guard(t.device()), stream(c10::cuda::getCurrentCUDAStream(t.device().index())) {}
+    c10::cuda::CUDAGuard guard;
+    c10::cuda::CUDAStream stream;
+};
+
+bool wants_grad(std::initializer_list<const Tensor*> ts) {
+    if (!at::GradMode::is_enabled()) return false;
+    for (const Tensor* t : ts)
+        if (t->defined() && t->requires_grad()) return true;
+    return false;
+}
+
+// Under create_graph: gradients of these gradients raise instead of being left out.
+variable_list once(variable_list g) {
+    if (!at::GradMode::is_enabled()) return g;
+    auto node = std::make_shared<torch::autograd::DelayedError>(
+        "need_b200: the training operators have no second derivative", static_cast<int>(g.size()));
+    variable_list in;
+    for (Tensor& t : g) in.push_back(t.defined() ? t.detach().requires_grad_() : t);
+    return (*node)(std::move(in));
+}
+
+// ------------------------------------------------------------------ the recurrences
+struct ScanShape {
+    int64_t form, B, T, C;
+    double dt_min, dt_max;
+    bool ckpt;
+};
+
+need_scan_train_args scan_args(const ScanShape& s, int32_t dtype, const Tensor& seg, const Tensor& d_skip,
+                               const Tensor& states) {
+    need_scan_train_args a{};
+    a.form = static_cast<int32_t>(s.form), a.dtype = dtype, a.checkpoint = s.ckpt ? 1 : 0;
+    a.nb = s.B, a.T = s.T, a.C = s.C, a.dt_min = s.dt_min, a.dt_max = s.dt_max;
+    a.d_skip = ptr<float>(d_skip), a.states = ptr<float>(states);
+    if (seg.defined()) a.seg_start = ptr<uint8_t>(seg), a.seg_stride_b = seg.stride(0), a.seg_stride_t = seg.stride(1);
+    return a;
+}
+
+struct ScanOut {
+    Tensor out, final, states, q, qs;
+};
+
+// Runs the forward; x: the streams in in[] order, each as rows() gives it.
+ScanOut scan_forward(const ScanShape& s, const variable_list& x, const Tensor& seg, const Tensor& h0,
+                     const Tensor& d_skip) {
+    On on(x[0]);
+    ScanOut r;
+    const int64_t nin = static_cast<int64_t>(x.size());
+    r.out = at::empty({s.B, s.T, s.C}, x[0].options());
+    r.final = floats(x[0], {s.B, s.C});
+    r.states = floats(x[0], {s.B, (s.T + kSpan - 1) / kSpan, s.C});
+    need_scan_train_args a = scan_args(s, dtype_of(x[0]), seg, d_skip, r.states);
+    for (int64_t k = 0; k < nin; ++k) a.in[k] = view(x[k]);
+    if (s.ckpt) {
+        const int64_t groups = (s.C + kGroup - 1) / kGroup;
+        r.q = scratch(x[0], nin * s.B * s.T * groups * kGroup);
+        r.qs = scratch(x[0], nin * s.B * s.T * groups);
+        a.ckpt_values = ptr<uint8_t>(r.q), a.ckpt_scales = ptr<uint8_t>(r.qs);
+    }
+    a.h0 = ptr<float>(h0);
+    a.out = r.out.data_ptr(), a.out_stride_b = s.T * s.C, a.out_stride_t = s.C;
+    a.h_final = ptr<float>(r.final);
+    const Tensor ws = scratch(x[0], need_scan_train_workspace_size(a.form, 0, s.B, s.T, s.C));
+    a.workspace = ws.data_ptr(), a.workspace_bytes = ws.numel();
+    check("need_scan_train_forward", need_scan_train_forward(&a, on.stream));
+    return r;
+}
+
+struct ScanTrain : torch::autograd::Function<ScanTrain> {
+    static variable_list forward(AutogradContext* ctx, int64_t form, bool ckpt, double dt_min, double dt_max,
+                                 const OptTensor& seg_, const OptTensor& h0_, const OptTensor& d_skip_,
+                                 const Tensor& x0, const Tensor& x1, const Tensor& x2, const OptTensor& x3_,
+                                 const OptTensor& x4_) {
+        const Tensor seg = or_none(seg_), h0 = or_none(h0_), d_skip = or_none(d_skip_);
+        const Tensor x3 = or_none(x3_), x4 = or_none(x4_);  // none for the GATED form
+        variable_list x{rows(x0), rows(x1), rows(x2)};
+        if (x3.defined()) x.insert(x.end(), {rows(x3), rows(x4)});
+        const ScanShape s{form, x0.size(0), x0.size(1), x0.size(2), dt_min, dt_max, ckpt};
+        ScanOut r = scan_forward(s, x, seg, h0, d_skip);
+        variable_list saved{r.states, seg, d_skip};
+        if (ckpt) saved.insert(saved.end(), {r.q, r.qs});
+        else saved.insert(saved.end(), x.begin(), x.end());
+        ctx->save_for_backward(std::move(saved));
+        auto& d = ctx->saved_data;
+        d["form"] = form, d["ckpt"] = ckpt, d["lo"] = dt_min, d["hi"] = dt_max, d["h0"] = h0.defined();
+        d["B"] = s.B, d["T"] = s.T, d["C"] = s.C, d["dtype"] = static_cast<int64_t>(x0.scalar_type());
+        ctx->set_materialize_grads(false);
+        return {r.out, r.final};
+    }
+
+    static variable_list backward(AutogradContext* ctx, variable_list go) {
+        auto& d = ctx->saved_data;
+        const ScanShape s{d["form"].toInt(),    d["B"].toInt(),     d["T"].toInt(), d["C"].toInt(),
+                          d["lo"].toDouble(), d["hi"].toDouble(), d["ckpt"].toBool()};
+        variable_list saved = ctx->get_saved_variables();
+        const Tensor &states = saved[0], &seg = saved[1], &d_skip = saved[2];
+        On on(states);
+        const auto opts = states.options().dtype(static_cast<at::ScalarType>(d["dtype"].toInt()));
+        const int nin = s.form == NEED_FORM_GATED ? 3 : 5;
+        const Tensor gout = go[0].defined() ? rows(go[0]) : at::zeros({s.B, s.T, s.C}, opts);
+        const Tensor gfin = go[1].defined() ? go[1].contiguous() : Tensor();
+        need_scan_train_args a = scan_args(s, dtype_of(gout), seg, d_skip, states);
+        if (s.ckpt) a.ckpt_values = ptr<uint8_t>(saved[3]), a.ckpt_scales = ptr<uint8_t>(saved[4]);
+        else
+            for (int k = 0; k < nin; ++k) a.in[k] = view(saved[3 + k]);
+        a.gout = view(gout), a.g_final = ptr<float>(gfin);
+        variable_list g(12);  // as forward's arguments
+        for (int k = 0; k < nin; ++k) {
+            g[7 + k] = at::empty({s.B, s.T, s.C}, opts);
+            a.grad[k] = g[7 + k].data_ptr();
+        }
+        if (d["h0"].toBool()) g[5] = floats(states, {s.B, s.C}), a.grad_h0 = ptr<float>(g[5]);
+        if (d_skip.defined()) g[6] = floats(states, {s.C}), a.grad_d = ptr<float>(g[6]);
+        const Tensor ws = scratch(states, need_scan_train_workspace_size(a.form, 1, s.B, s.T, s.C));
+        a.workspace = ws.data_ptr(), a.workspace_bytes = ws.numel();
+        check("need_scan_train_backward", need_scan_train_backward(&a, on.stream));
+        return once(std::move(g));
+    }
+};
+
+std::tuple<Tensor, Tensor> scan_train(int64_t form, bool ckpt, double dt_min, double dt_max, const OptTensor& seg_,
+                                      const OptTensor& h0_, const OptTensor& d_skip_, const Tensor& x0, const Tensor& x1,
+                                      const Tensor& x2, const OptTensor& x3_, const OptTensor& x4_) {
+    const Tensor seg = or_none(seg_), x3 = or_none(x3_), x4 = or_none(x4_);
+    Tensor h0 = or_none(h0_), d_skip = or_none(d_skip_);
+    if (h0.defined()) h0 = h0.contiguous();
+    if (d_skip.defined()) d_skip = d_skip.contiguous();
+    if (!wants_grad({&h0, &d_skip, &x0, &x1, &x2, &x3, &x4})) {  // nothing to keep
+        at::NoGradGuard no_grad;
+        variable_list x{rows(x0), rows(x1), rows(x2)};
+        if (x3.defined()) x.insert(x.end(), {rows(x3), rows(x4)});
+        ScanOut r = scan_forward({form, x0.size(0), x0.size(1), x0.size(2), dt_min, dt_max, false}, x, seg, h0, d_skip);
+        return {r.out, r.final};
+    }
+    variable_list r = ScanTrain::apply(form, ckpt, dt_min, dt_max, seg_, opt(h0), opt(d_skip), x0, x1, x2, x3_, x4_);
+    return {r[0], r[1]};
+}
+
+// ------------------------------------------------------------------ the conv
+need_conv_train_args conv_args(const Tensor& u, const Tensor& w, const Tensor& b, const Tensor& seg) {
+    need_conv_train_args a{};
+    a.dtype = dtype_of(u), a.K = static_cast<int32_t>(w.size(1));
+    a.nb = u.size(0), a.T = u.size(1), a.C = u.size(2);
+    a.u = u.const_data_ptr(), a.u_stride_b = u.stride(0), a.u_stride_t = u.stride(1);
+    a.weight = ptr<float>(w), a.bias = ptr<float>(b);
+    if (seg.defined()) a.seg_start = ptr<uint8_t>(seg), a.seg_stride_b = seg.stride(0), a.seg_stride_t = seg.stride(1);
+    return a;
+}
+
+struct ConvTrain : torch::autograd::Function<ConvTrain> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& u_, const Tensor& w_, const OptTensor& b_,
+                          const OptTensor& seg_) {
+        const Tensor u = rows(u_), w = w_.contiguous(), seg = or_none(seg_);
+        const Tensor b = b_.has_value() ? b_->contiguous() : Tensor();
+        On on(u);
+        Tensor out = at::empty(u.sizes(), u.options());
+        need_conv_train_args a = conv_args(u, w, b, seg);
+        a.out = out.data_ptr();
+        check("need_conv_silu_train_forward", need_conv_silu_train_forward(&a, on.stream));
+        ctx->save_for_backward({u, w, b, seg});
+        return out;
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list go) {
+        variable_list s = ctx->get_saved_variables();
+        const Tensor &u = s[0], &w = s[1], &b = s[2], &seg = s[3];
+        On on(u);
+        const Tensor gout = rows(go[0]);
+        need_conv_train_args a = conv_args(u, w, b, seg);
+        a.gout = gout.const_data_ptr(), a.gout_stride_b = gout.stride(0), a.gout_stride_t = gout.stride(1);
+        Tensor gu = at::empty(u.sizes(), u.options()), gwb = floats(u, {a.C, a.K + 1});
+        const Tensor ws = scratch(u, need_conv_silu_train_workspace_size(a.K, a.nb, a.T, a.C));
+        a.grad_u = gu.data_ptr(), a.grad_wb = ptr<float>(gwb);
+        a.workspace = ws.data_ptr(), a.workspace_bytes = ws.numel();
+        check("need_conv_silu_train_backward", need_conv_silu_train_backward(&a, on.stream));
+        return once({gu, gwb.narrow(1, 0, a.K), b.defined() ? gwb.select(1, a.K) : Tensor(), Tensor()});
+    }
+};
+
+Tensor conv_train(const Tensor& u, const Tensor& w, const OptTensor& b, const OptTensor& seg) {
+    return ConvTrain::apply(u, w, b, seg);
+}
+
+// ------------------------------------------------------------------ the norm
+need_norm_train_args norm_args(int32_t dtype, int64_t n, int64_t C, int64_t c_mean, const Tensor& w, const Tensor& rstd,
+                               double eps, bool ckpt) {
+    need_norm_train_args a{};
+    a.dtype = dtype, a.checkpoint = ckpt ? 1 : 0, a.rows = n, a.C = C, a.C_mean = c_mean;
+    a.weight = ptr<float>(w), a.rstd = ptr<float>(rstd), a.eps = eps;
+    return a;
+}
+
+struct NormTrain : torch::autograd::Function<NormTrain> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& x_, const Tensor& w_, double eps, bool ckpt, int64_t c_mean) {
+        const Tensor x = rows(x_);
+        const Tensor w = w_.is_contiguous() && reinterpret_cast<uintptr_t>(w_.const_data_ptr()) % 16 == 0
+                             ? w_
+                             : w_.clone(at::MemoryFormat::Contiguous);
+        const int64_t n = x.size(0), C = x.size(1);
+        On on(x);
+        Tensor out = at::empty({n, C}, x.options()), rstd = floats(x, {n}), q, qs;
+        need_norm_train_args a = norm_args(dtype_of(x), n, C, c_mean, w, rstd, eps, ckpt);
+        a.x = x.const_data_ptr(), a.x_stride = x.stride(0), a.out = out.data_ptr();
+        if (ckpt) {
+            q = scratch(x, n * C), qs = scratch(x, n * ((C + kGroup - 1) / kGroup));
+            a.ckpt_values = ptr<uint8_t>(q), a.ckpt_scales = ptr<uint8_t>(qs);
+        }
+        check("need_rms_norm_train_forward", need_rms_norm_train_forward(&a, on.stream));
+        if (ckpt) ctx->save_for_backward({w, rstd, q, qs});
+        else ctx->save_for_backward({w, rstd, x});
+        auto& d = ctx->saved_data;
+        d["n"] = n, d["C"] = C, d["mean"] = c_mean, d["eps"] = eps, d["ckpt"] = ckpt;
+        return out;
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list go) {
+        auto& d = ctx->saved_data;
+        const bool ckpt = d["ckpt"].toBool();
+        const int64_t n = d["n"].toInt(), C = d["C"].toInt();
+        variable_list s = ctx->get_saved_variables();
+        On on(s[0]);
+        const Tensor gout = rows(go[0]);
+        need_norm_train_args a = norm_args(dtype_of(gout), n, C, d["mean"].toInt(), s[0], s[1], d["eps"].toDouble(), ckpt);
+        if (ckpt) a.ckpt_values = ptr<uint8_t>(s[2]), a.ckpt_scales = ptr<uint8_t>(s[3]);
+        else a.x = s[2].const_data_ptr(), a.x_stride = s[2].stride(0);
+        a.gout = gout.const_data_ptr(), a.gout_stride = gout.stride(0);
+        Tensor gx = at::empty({n, C}, gout.options()), gw = floats(gout, {C});
+        const Tensor ws = scratch(gout, need_rms_norm_train_workspace_size(n, C));
+        a.grad_x = gx.data_ptr(), a.grad_weight = ptr<float>(gw);
+        a.workspace = ws.data_ptr(), a.workspace_bytes = ws.numel();
+        check("need_rms_norm_train_backward", need_rms_norm_train_backward(&a, on.stream));
+        return once({gx, gw, Tensor(), Tensor(), Tensor()});
+    }
+};
+
+Tensor norm_train(const Tensor& x, const Tensor& w, double eps, bool ckpt, int64_t c_mean) {
+    return NormTrain::apply(x, w, eps, ckpt && wants_grad({&x, &w}), c_mean);
+}
+
+}  // namespace
+
+PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
+    const auto nogil = py::call_guard<py::gil_scoped_release>();
+    m.def("scan_train", &scan_train, nogil);
+    m.def("conv_train", &conv_train, nogil);
+    m.def("norm_train", &norm_train, nogil);
+}
