@@ -240,8 +240,9 @@ typedef struct {
     int32_t form;           /* NEED_FORM_GATED or NEED_FORM_SSD */
     int32_t dtype;          /* need_dtype of in[], out, gout and grad[] */
     int32_t checkpoint;     /* 0: the backward reads in[]; 1: it reads the 8-bit copies */
-    int64_t nb, T, C;       /* C a multiple of 16 bytes' worth of elements */
-    need_view in[5];        /* as need_scan_args.in (stride_h unused); backward: unused with checkpoint */
+    int64_t nb, T, C;
+    need_view in[5];        /* as need_scan_args.in (stride_h unused), but any alignment and strides will do;
+                               backward: unused with checkpoint */
     const float* d_skip;    /* SSD: [C] fp32 */
     double dt_min, dt_max;  /* SSD: 0 <= dt_min <= dt_max */
     const float* h0;        /* forward: optional [nb, C] fp32 initial state */
@@ -252,12 +253,14 @@ typedef struct {
     uint8_t* ckpt_values;   /* checkpoint: [nin][nb][T][G * 64] e4m3, G = ceil(C / 64), nin = 3 (GATED)
                                or 5 (SSD), in in[] order; 16-byte aligned */
     uint8_t* ckpt_scales;   /* checkpoint: [nin][nb][T][G], exponent + 127 (255: not finite) */
-    void* out;              /* forward: [nb, T, C], 16-byte aligned rows */
+    void* out;              /* forward: [nb, T, C], 16-byte aligned rows (so with strides of C rounded up
+                               where C is odd); bytes past a row's C channels are left alone */
     int64_t out_stride_b, out_stride_t;
     float* h_final;         /* forward: optional [nb, C] fp32 state after the last token */
-    need_view gout;         /* backward: gradient of out */
+    need_view gout;         /* backward: gradient of out, any alignment and strides */
     const float* g_final;   /* backward: optional [nb, C] gradient of h_final */
-    void* grad[5];          /* backward: gradients of in[], [nb, T, C] contiguous */
+    void* grad[5];          /* backward: gradients of in[], [nb, T, C], as out */
+    int64_t grad_stride_b, grad_stride_t;
     float* grad_h0;         /* backward: optional [nb, C] gradient of the initial state */
     float* grad_d;          /* backward, SSD: [C] gradient of d_skip */
     void* workspace;        /* >= need_scan_train_workspace_size(...) bytes, 16-byte aligned; the call
@@ -491,8 +494,9 @@ NEED_API int64_t need_scan_train_chunk_len(void);
 /* Channels of one token that share a scale in an 8-bit checkpoint. */
 NEED_API int64_t need_scan_train_group(void);
 
-/* Workspace bytes of a training scan of this shape (0 for sizes it does not take). */
-NEED_API size_t need_scan_train_workspace_size(int32_t form, int32_t backward, int64_t nb, int64_t T, int64_t C);
+/* Workspace bytes of a training scan of this form, dtype and shape. */
+NEED_API size_t need_scan_train_workspace_size(int32_t form, int32_t dtype, int32_t checkpoint, int32_t backward,
+                                               int64_t nb, int64_t T, int64_t C);
 
 /* The GATED or SSD scan for training (need_core.py:1630-1642 computes it with
  * torch ops under grad).  Gates, states and epilogue are fp32, rounded once to

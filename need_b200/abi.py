@@ -121,7 +121,8 @@ class NeedScanTrainArgs(Structure):
         ("h0", c_void_p), ("seg_start", c_void_p), ("seg_stride_b", c_int64), ("seg_stride_t", c_int64),
         ("states", c_void_p), ("ckpt_values", c_void_p), ("ckpt_scales", c_void_p),
         ("out", c_void_p), ("out_stride_b", c_int64), ("out_stride_t", c_int64), ("h_final", c_void_p),
-        ("gout", NeedView), ("g_final", c_void_p), ("grad", c_void_p * 5), ("grad_h0", c_void_p),
+        ("gout", NeedView), ("g_final", c_void_p), ("grad", c_void_p * 5),
+        ("grad_stride_b", c_int64), ("grad_stride_t", c_int64), ("grad_h0", c_void_p),
         ("grad_d", c_void_p), ("workspace", c_void_p), ("workspace_bytes", c_size_t),
     ]
 
@@ -174,7 +175,7 @@ SIGNATURES = {
     "need_ssd_conv_silu": (c_int32, [POINTER(NeedConvArgs), c_void_p]),
     "need_scan_train_chunk_len": (c_int64, []),
     "need_scan_train_group": (c_int64, []),
-    "need_scan_train_workspace_size": (c_size_t, [c_int32, c_int32, c_int64, c_int64, c_int64]),
+    "need_scan_train_workspace_size": (c_size_t, [c_int32, c_int32, c_int32, c_int32, c_int64, c_int64, c_int64]),
     "need_scan_train_forward": (c_int32, [POINTER(NeedScanTrainArgs), c_void_p]),
     "need_scan_train_backward": (c_int32, [POINTER(NeedScanTrainArgs), c_void_p]),
     "need_conv_silu_train_workspace_size": (c_size_t, [c_int32, c_int64, c_int64, c_int64]),

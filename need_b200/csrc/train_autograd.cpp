@@ -42,6 +42,17 @@ int32_t dtype_of(const Tensor& t) {
     }
 }
 
+// `t` with channel stride 1; a copy if its channels are apart.
+Tensor channels(const Tensor& t) {
+    return t.stride(-1) == 1 || t.size(-1) <= 1 ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+// A new [B, T, C] tensor whose rows start 16-byte aligned: contiguous, or with
+// rows apart by C rounded up.
+Tensor rows_like(const at::TensorOptions& opts, int64_t B, int64_t T, int64_t C) {
+    const int64_t n = 16 / static_cast<int64_t>(opts.dtype().itemsize()), pitch = (C + n - 1) / n * n;
+    return pitch == C ? at::empty({B, T, C}, opts) : at::empty_strided({B, T, C}, {T * pitch, pitch, 1}, opts);
+}
+
 // `t` with channel stride 1, a 16-byte aligned base and positive row strides of
 // whole 16 bytes (dims of size 1 excepted); a copy if it is laid out otherwise.
 Tensor rows(const Tensor& t) {
@@ -110,13 +121,13 @@ struct ScanOut {
     Tensor out, final, states, q, qs;
 };
 
-// Runs the forward; x: the streams in in[] order, each as rows() gives it.
+// Runs the forward; x: the streams in in[] order, each as channels() gives it.
 ScanOut scan_forward(const ScanShape& s, const variable_list& x, const Tensor& seg, const Tensor& h0,
                      const Tensor& d_skip) {
     On on(x[0]);
     ScanOut r;
     const int64_t nin = static_cast<int64_t>(x.size());
-    r.out = at::empty({s.B, s.T, s.C}, x[0].options());
+    r.out = rows_like(x[0].options(), s.B, s.T, s.C);
     r.final = floats(x[0], {s.B, s.C});
     r.states = floats(x[0], {s.B, (s.T + kSpan - 1) / kSpan, s.C});
     need_scan_train_args a = scan_args(s, dtype_of(x[0]), seg, d_skip, r.states);
@@ -128,9 +139,9 @@ ScanOut scan_forward(const ScanShape& s, const variable_list& x, const Tensor& s
         a.ckpt_values = ptr<uint8_t>(r.q), a.ckpt_scales = ptr<uint8_t>(r.qs);
     }
     a.h0 = ptr<float>(h0);
-    a.out = r.out.data_ptr(), a.out_stride_b = s.T * s.C, a.out_stride_t = s.C;
+    a.out = r.out.data_ptr(), a.out_stride_b = r.out.stride(0), a.out_stride_t = r.out.stride(1);
     a.h_final = ptr<float>(r.final);
-    const Tensor ws = scratch(x[0], need_scan_train_workspace_size(a.form, 0, s.B, s.T, s.C));
+    const Tensor ws = scratch(x[0], need_scan_train_workspace_size(a.form, a.dtype, a.checkpoint, 0, s.B, s.T, s.C));
     a.workspace = ws.data_ptr(), a.workspace_bytes = ws.numel();
     check("need_scan_train_forward", need_scan_train_forward(&a, on.stream));
     return r;
@@ -143,8 +154,8 @@ struct ScanTrain : torch::autograd::Function<ScanTrain> {
                                  const OptTensor& x4_) {
         const Tensor seg = or_none(seg_), h0 = or_none(h0_), d_skip = or_none(d_skip_);
         const Tensor x3 = or_none(x3_), x4 = or_none(x4_);  // none for the GATED form
-        variable_list x{rows(x0), rows(x1), rows(x2)};
-        if (x3.defined()) x.insert(x.end(), {rows(x3), rows(x4)});
+        variable_list x{channels(x0), channels(x1), channels(x2)};
+        if (x3.defined()) x.insert(x.end(), {channels(x3), channels(x4)});
         const ScanShape s{form, x0.size(0), x0.size(1), x0.size(2), dt_min, dt_max, ckpt};
         ScanOut r = scan_forward(s, x, seg, h0, d_skip);
         variable_list saved{r.states, seg, d_skip};
@@ -167,7 +178,7 @@ struct ScanTrain : torch::autograd::Function<ScanTrain> {
         On on(states);
         const auto opts = states.options().dtype(static_cast<at::ScalarType>(d["dtype"].toInt()));
         const int nin = s.form == NEED_FORM_GATED ? 3 : 5;
-        const Tensor gout = go[0].defined() ? rows(go[0]) : at::zeros({s.B, s.T, s.C}, opts);
+        const Tensor gout = go[0].defined() ? channels(go[0]) : at::zeros({s.B, s.T, s.C}, opts);
         const Tensor gfin = go[1].defined() ? go[1].contiguous() : Tensor();
         need_scan_train_args a = scan_args(s, dtype_of(gout), seg, d_skip, states);
         if (s.ckpt) a.ckpt_values = ptr<uint8_t>(saved[3]), a.ckpt_scales = ptr<uint8_t>(saved[4]);
@@ -176,12 +187,13 @@ struct ScanTrain : torch::autograd::Function<ScanTrain> {
         a.gout = view(gout), a.g_final = ptr<float>(gfin);
         variable_list g(12);  // as forward's arguments
         for (int k = 0; k < nin; ++k) {
-            g[7 + k] = at::empty({s.B, s.T, s.C}, opts);
+            g[7 + k] = rows_like(opts, s.B, s.T, s.C);
             a.grad[k] = g[7 + k].data_ptr();
         }
+        a.grad_stride_b = g[7].stride(0), a.grad_stride_t = g[7].stride(1);
         if (d["h0"].toBool()) g[5] = floats(states, {s.B, s.C}), a.grad_h0 = ptr<float>(g[5]);
         if (d_skip.defined()) g[6] = floats(states, {s.C}), a.grad_d = ptr<float>(g[6]);
-        const Tensor ws = scratch(states, need_scan_train_workspace_size(a.form, 1, s.B, s.T, s.C));
+        const Tensor ws = scratch(states, need_scan_train_workspace_size(a.form, a.dtype, a.checkpoint, 1, s.B, s.T, s.C));
         a.workspace = ws.data_ptr(), a.workspace_bytes = ws.numel();
         check("need_scan_train_backward", need_scan_train_backward(&a, on.stream));
         return once(std::move(g));
@@ -197,8 +209,8 @@ std::tuple<Tensor, Tensor> scan_train(int64_t form, bool ckpt, double dt_min, do
     if (d_skip.defined()) d_skip = d_skip.contiguous();
     if (!wants_grad({&h0, &d_skip, &x0, &x1, &x2, &x3, &x4})) {  // nothing to keep
         at::NoGradGuard no_grad;
-        variable_list x{rows(x0), rows(x1), rows(x2)};
-        if (x3.defined()) x.insert(x.end(), {rows(x3), rows(x4)});
+        variable_list x{channels(x0), channels(x1), channels(x2)};
+        if (x3.defined()) x.insert(x.end(), {channels(x3), channels(x4)});
         ScanOut r = scan_forward({form, x0.size(0), x0.size(1), x0.size(2), dt_min, dt_max, false}, x, seg, h0, d_skip);
         return {r.out, r.final};
     }

@@ -36,7 +36,29 @@ __device__ __forceinline__ void sig_pair(float2 x, float2& s, float2& n) {
     }
 }
 
-// a = e^-r and n = 1 - a of a pair, r >= 0.  fp32: expm1.  16 bit: below 2^-4
+// s alone (e^-x may overflow: s is then 0)
+template <typename T>
+__device__ __forceinline__ float2 sig_only(float2 x) {
+    if constexpr (Ops<T>::BYTES == 4) {
+        return make_float2(sigmoid_exact(x.x), sigmoid_exact(x.y));
+    } else {
+        return sig2<T>(x);
+    }
+}
+
+// a = e^-r and n = 1 - a of a pair, 0 <= r <= 1/4: six terms of the series of
+// 1 - e^-r (the seventh is r^6 / 5040 of it, 4.8e-8).
+__device__ __forceinline__ void exp_neg_small(float2 r, float2& a, float2& n) {
+    float2 q = ffma2(r, splat2(-1.0f / 720.0f), splat2(1.0f / 120.0f));
+    q = ffma2(r, q, splat2(-1.0f / 24.0f));
+    q = ffma2(r, q, splat2(1.0f / 6.0f));
+    q = ffma2(r, q, splat2(-0.5f));
+    q = ffma2(r, q, splat2(1.0f));
+    n = fmul2(r, q);
+    a = fadd2(splat2(1.0f), make_float2(-n.x, -n.y));
+}
+
+// The same for any r >= 0.  fp32: expm1.  16 bit: below 2^-4
 // the first five terms of the series of 1 - e^-r (the next is r^5 / 720 of it,
 // 1.3e-9), above it the difference (2^-24 / 2^-4 relative).
 template <typename T>
@@ -68,9 +90,14 @@ __device__ __forceinline__ uint32_t e4m3_scale_byte(uint32_t top) {
 __device__ __forceinline__ float e4m3_scale(uint32_t byte) {
     return __uint_as_float(byte == 255u ? 0x7fc00000u : byte << 23);
 }
+__device__ __forceinline__ float e4m3_inverse(uint32_t byte) {  // 2^-e
+    return __uint_as_float((254u - min(byte, 253u)) << 23);
+}
+__device__ __forceinline__ uint16_t e4m3_round(float2 x) {
+    return __nv_cvt_float2_to_fp8x2(x, __NV_SATFINITE, __NV_E4M3);
+}
 __device__ __forceinline__ uint16_t e4m3_pair(float2 x, uint32_t byte) {
-    const float inv = __uint_as_float((254u - min(byte, 253u)) << 23);  // 2^-e
-    return __nv_cvt_float2_to_fp8x2(make_float2(x.x * inv, x.y * inv), __NV_SATFINITE, __NV_E4M3);
+    return e4m3_round(fmul2(x, splat2(e4m3_inverse(byte))));
 }
 
 // ------------------------------------------------------------------ TMA
@@ -81,6 +108,17 @@ __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* tm, in
         "l"(tm), "r"(c0), "r"(c1), "r"(c2), "r"(smem_addr(bar))
         : "memory");
 }
+
+// Its counterpart: shared -> global, rows and channels outside the tensor left
+// out.  The shared bytes must have been fenced for the async proxy.
+__device__ __forceinline__ void tma_store_3d(const CUtensorMap* tm, const void* src, int c0, int c1, int c2) {
+    asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3}], [%4];" ::"l"(tm),
+                 "r"(c0), "r"(c1), "r"(c2), "r"(smem_addr(src))
+                 : "memory");
+}
+__device__ __forceinline__ void tma_store_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+// This thread's committed stores have read their shared memory (which the CTA may then give up).
+__device__ __forceinline__ void tma_store_drain() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
 
 // out[c] = sum over rows of part[row][c], in a fixed order (train_norm.cu).
 int column_sums(const float* part, int64_t rows, int64_t C, float* out, cudaStream_t stream);

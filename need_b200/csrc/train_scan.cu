@@ -25,13 +25,15 @@
 // segment reaches neither the next segment's states nor the gradients of the
 // one before.
 //
-// Tiles are 64 tokens x 64 channels, one CTA each: 8 row warps of 8 rows, a
-// lane owning one pair of channels (packed fp32 arithmetic), and a look-back
-// warp.  The forward writes the fp32 state entering each tile ([nb, chunks,
-// C], 1/32 of one 16-bit stream); the backward runs its tile's states again
-// from there, so it reads neither h nor any gate from memory, and both
+// Tiles are 64 tokens x 64 channels, one CTA each: 8 row warps of 8 rows and a
+// look-back warp.  A lane owns 4 channels (two packed fp32 pairs) of 4 rows, half
+// a warp a row.  The forward writes the fp32 state entering each tile ([nb,
+// chunks, C], 1/32 of one 16-bit stream); the backward runs its tile's states
+// again from there, so it reads neither h nor any gate from memory, and both
 // directions stream their algorithmic bytes once: 8 and 14 B per element
-// (GATED, 16 bit), 12 and 22 B (SSD).
+// (GATED, 16 bit), 12 and 22 B (SSD).  Tiles come by TMA (streams whose rows
+// are not 16-byte aligned by plain loads into the same slots), results leave by
+// TMA from the slots they were computed in.
 //
 // Across tiles the carry travels as in scan_kernel.cuh (single pass, decoupled
 // look-back over the kTrainDepth tiles before and the inclusive carry of the
@@ -51,6 +53,7 @@
 #include <string.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "host_common.h"
 #include "need_scan.h"
@@ -61,31 +64,45 @@ using namespace need;
 
 namespace {
 
-constexpr int kL = 64, kCB = 64;      // tokens and channels per tile
-constexpr int kNW = 8, kR = kL / kNW;  // row warps and rows per warp
+constexpr int kCB = 64;                // channels per tile
+constexpr int kSpan = 64;              // tokens between kept states
+constexpr int kNW = 8;                 // row warps
 constexpr int kNT = (kNW + 1) * 32;    // threads: the row warps and the look-back warp
-constexpr int kTrainDepth = 3;         // tile maps composed before an inclusive carry
+#ifndef K_FWD_MINB
+#define K_FWD_MINB 4
+#endif
+#ifndef K_BWD_MINB
+#define K_BWD_MINB 3
+#endif
+#ifndef K_DEEP
+#define K_DEEP 7
+#endif
+constexpr int kDeep = K_DEEP;              // most tile maps composed before an inclusive carry
 constexpr int kHdrBytes = WS_HDR_WORDS * 4;
 constexpr int kTileRecBytes = kCB * 12;  // per tile: (A, B) and the inclusive carry of each channel
 
 struct TrainParams {
-    CUtensorMap tm[6];  // the streamed inputs, and gout (backward, last)
-    int32_t nb, T, C, ncb, nchains, nchunks;
+    CUtensorMap tm[6];   // the streamed inputs, and gout (backward, last)
+    CUtensorMap tmo[5];  // the streamed outputs: out, or grad[]
+    uint32_t plain;      // bit k: stream k is read with plain loads, from
+    const void* src[6];
+    int64_t ssb[6], sst[6];
+    int32_t nb, T, C, ncb, nchains, nchunks;  // tiles along T
+    int32_t nspans, depth;                    // kept states along T; look-back depth
     const float* dskip;
     float dt_min, dt_scale;
     const float* h0;       // forward: initial state; backward: unused (the states hold it)
     float* h_final;        // forward
     const uint8_t* seg;
     int64_t sgb, sgt;
-    float* states;         // [nb, nchunks, C] the state entering each tile
-    void* out;             // forward
-    int64_t osb, ost;
+    float* states;         // [nb, nspans, C] the state entering each span
     uint8_t* q;            // 8-bit values [nin][nb][T][ncb * 64]
     uint8_t* qs;           // their scales [nin][nb][T][ncb]
-    void* grad[5];         // backward: [nb, T, C] each, in in[] order
     const float* g_final;  // backward: gradient of the final state or null
     float* grad_h0;        // backward, optional
-    float* dpart;          // backward SSD: [nb * nchunks, C] partial sums of the gradient of D
+    float* dpart;          // backward SSD: [nb * nchunks, C] partial sums of the gradient of D,
+    uint32_t* dcount;      // [ncb] tiles of each channel block that have written theirs,
+    float* grad_d;         // and [C] their sum
     uint32_t* hdr;
     ulonglong2* agg;           // [ntiles][32] (A, B) of the lane's two channels
     unsigned long long* incl;  // [ntiles][32] the carry past the tile, two channels
@@ -93,14 +110,17 @@ struct TrainParams {
 };
 
 // ------------------------------------------------------------------ maps
-// Affine maps c -> A c + B with A == 0 meaning "drops c", whatever c holds.
-__device__ __forceinline__ float2 apply(float2 A, float2 c, float2 B) {
-    const float2 r = ffma2(A, c, B);
-    return make_float2(A.x == 0.0f ? B.x : r.x, A.y == 0.0f ? B.y : r.y);
+// Affine maps c -> A c + B.  With segments in the call (`seg`), A == 0 means
+// "drops c", whatever c holds.
+__device__ __forceinline__ float2 apply(float2 A, float2 c, float2 B, bool seg) {
+    float2 r = ffma2(A, c, B);
+    if (seg) r = make_float2(A.x == 0.0f ? B.x : r.x, A.y == 0.0f ? B.y : r.y);
+    return r;
 }
-__device__ __forceinline__ float2 mulz(float2 a, float2 b) {
-    const float2 r = fmul2(a, b);
-    return make_float2(a.x == 0.0f || b.x == 0.0f ? 0.0f : r.x, a.y == 0.0f || b.y == 0.0f ? 0.0f : r.y);
+__device__ __forceinline__ float2 mulz(float2 a, float2 b, bool seg) {
+    float2 r = fmul2(a, b);
+    if (seg) r = make_float2(a.x == 0.0f || b.x == 0.0f ? 0.0f : r.x, a.y == 0.0f || b.y == 0.0f ? 0.0f : r.y);
+    return r;
 }
 
 // ------------------------------------------------------------------ records
@@ -130,31 +150,117 @@ __device__ __forceinline__ unsigned long long ld_relaxed_u64(const unsigned long
 }
 
 // ------------------------------------------------------------------ inputs
-// A lane's channel pair of row r of a 16- or 32-bit slot.
+struct F4 {  // four channels
+    float2 p[2];
+};
+// Channels 4 v .. 4 v + 3 of row r of a slot.
 template <typename T>
-__device__ __forceinline__ float2 pair_at(const unsigned char* slot, int r, int lane) {
-    return widen(reinterpret_cast<const typename Ops<T>::P*>(slot)[r * (kCB / 2) + lane]);
+__device__ __forceinline__ F4 row4(const unsigned char* slot, int r, int v) {
+    F4 f;
+    if constexpr (Ops<T>::BYTES == 4) {
+        const float4 x = reinterpret_cast<const float4*>(slot)[r * (kCB / 4) + v];
+        f.p[0] = make_float2(x.x, x.y);
+        f.p[1] = make_float2(x.z, x.w);
+    } else {
+        const uint2 x = reinterpret_cast<const uint2*>(slot)[r * (kCB / 4) + v];
+        f.p[0] = widen(*reinterpret_cast<const typename Ops<T>::P*>(&x.x));
+        f.p[1] = widen(*reinterpret_cast<const typename Ops<T>::P*>(&x.y));
+    }
+    return f;
+}
+template <typename T>
+__device__ __forceinline__ void put4(unsigned char* slot, int r, int v, const F4& f) {
+    const typename Ops<T>::P h[2] = {Ops<T>::pack(f.p[0].x, f.p[0].y), Ops<T>::pack(f.p[1].x, f.p[1].y)};
+    if constexpr (Ops<T>::BYTES == 4)
+        reinterpret_cast<float4*>(slot)[r * (kCB / 4) + v] = *reinterpret_cast<const float4*>(h);
+    else reinterpret_cast<uint2*>(slot)[r * (kCB / 4) + v] = *reinterpret_cast<const uint2*>(h);
 }
 // The same of an 8-bit slot, times its row's scale.
-__device__ __forceinline__ float2 pair8_at(const unsigned char* slot, int r, int lane, float scale) {
-    const __nv_fp8x2_storage_t q = reinterpret_cast<const __nv_fp8x2_storage_t*>(slot)[r * (kCB / 2) + lane];
-    const float2 f = __half22float2(static_cast<__half2>(__nv_cvt_fp8x2_to_halfraw2(q, __NV_E4M3)));
-    return make_float2(f.x * scale, f.y * scale);
+__device__ __forceinline__ F4 row4_8(const unsigned char* slot, int r, int v, float scale) {
+    const uint32_t q = reinterpret_cast<const uint32_t*>(slot)[r * (kCB / 4) + v];
+    F4 f;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const __nv_fp8x2_storage_t h = static_cast<__nv_fp8x2_storage_t>(q >> (16 * i));
+        f.p[i] = fmul2(__half22float2(static_cast<__half2>(__nv_cvt_fp8x2_to_halfraw2(h, __NV_E4M3))), splat2(scale));
+    }
+    return f;
 }
 
-template <int FORM, typename T, bool CK, bool BWD>
+// What a sigmoid computed in phase 1 leaves in its stream's slot for phase 2,
+// in place of the logit: fp32 s itself; bf16 the nearer of s and s - 1 to 0 as
+// f16 (2^-12 relative against the 2^-9 the gradient is rounded to, of whichever
+// of s and 1 - s is small; below 6e-5 a fixed 3e-8), which saves the second
+// round of exponentials and reciprocals.  f16 gradients are rounded to 2^-12
+// themselves: there the logit stays and the sigmoid is computed again.
+template <typename T>
+constexpr bool kKeep = !std::is_same<T, __half>::value;
+template <typename T>
+__device__ __forceinline__ void keep4(unsigned char* slot, int r, int v, const F4& s) {
+    if constexpr (Ops<T>::BYTES == 4) {
+        put4<float>(slot, r, v, s);
+    } else if constexpr (kKeep<T>) {
+        F4 y;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {  // s = 1 is kept as -0
+            const float2 n = fadd2(splat2(1.0f), make_float2(-s.p[i].x, -s.p[i].y));
+            y.p[i] = make_float2(s.p[i].x >= 0.5f ? -n.x : s.p[i].x, s.p[i].y >= 0.5f ? -n.y : s.p[i].y);
+        }
+        put4<__half>(slot, r, v, y);
+    }
+}
+__device__ __forceinline__ float one_if_negative(float y) {  // by the sign bit: -0 too
+    return __int_as_float((__float_as_int(y) >> 31) & 0x3f800000);
+}
+// s and s (1 - s) from a kept slot.
+template <typename T>
+__device__ __forceinline__ void kept4(const unsigned char* slot, int r, int v, F4& s, F4& slope) {
+    static_assert(kKeep<T>, "kept as fp32 or f16");
+    if constexpr (Ops<T>::BYTES == 4) {
+        s = row4<float>(slot, r, v);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) slope.p[i] = fmul2(s.p[i], fadd2(splat2(1.0f), make_float2(-s.p[i].x, -s.p[i].y)));
+    } else {
+        const F4 y = row4<__half>(slot, r, v);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            s.p[i] = fadd2(y.p[i], make_float2(one_if_negative(y.p[i].x), one_if_negative(y.p[i].y)));
+            slope.p[i] = make_float2(fmaf(-y.p[i].x, y.p[i].x, fabsf(y.p[i].x)), fmaf(-y.p[i].y, y.p[i].y, fabsf(y.p[i].y)));
+        }
+    }
+}
+template <typename T>
+__device__ __forceinline__ F4 sig4(const F4& x) {
+    F4 s;
+    s.p[0] = sig_only<T>(x.p[0]);
+    s.p[1] = sig_only<T>(x.p[1]);
+    return s;
+}
+
+// Tokens per tile.
+__host__ __device__ constexpr int tile_tokens(int bytes, bool ck, bool bwd) {
+    return 64;
+}
+
+// DT: how the SSD form gets a = e^-r (r <= dt_max): 0 any range, 1 dt_max <= 1/4.
+template <int FORM, typename T, bool CK, int DT, bool BWD>
 struct TrainCfg {
     static constexpr int NIN = FORM == FORM_GATED ? 3 : 5;
-    static constexpr int IN_BYTES = (BWD && CK) ? 1 : Ops<T>::BYTES;     // per streamed input element
-    static constexpr int IN_SLOT = kL * kCB * IN_BYTES;
+    static constexpr int IN_BYTES = (BWD && CK) ? 1 : Ops<T>::BYTES;  // per streamed input element
+    static constexpr int L = tile_tokens(Ops<T>::BYTES, CK, BWD), R = L / kNW, RT = R / 2;  // rows per warp, thread
+    static constexpr int IN_SLOT = L * kCB * IN_BYTES;
+    static constexpr int SLOT = L * kCB * Ops<T>::BYTES;
     static constexpr int OFF_GOUT = NIN * IN_SLOT;
-    static constexpr int OFF_MAP = OFF_GOUT + (BWD ? kL * kCB * Ops<T>::BYTES : 0);  // [NW][32] (A, B) float4
-    static constexpr int OFF_FWD = OFF_MAP + kNW * 32 * 16;                // BWD: [NW][32] forward B, float2
+    // where kept sigmoids and results go: the input slots, or (8-bit inputs) slots of their own
+    static constexpr bool STAGED = BWD && CK;
+    static constexpr int OFF_STAGE = STAGED ? OFF_GOUT + SLOT : 0;
+    static constexpr int OFF_MAP = OFF_GOUT + (BWD ? SLOT : 0) + (STAGED ? NIN * SLOT : 0);  // [NW][32] (A, B)
+    static constexpr int OFF_FWD = OFF_MAP + kNW * 32 * 16;                // BWD: [NW][32] forward B
     static constexpr int OFF_IN = OFF_FWD + (BWD ? kNW * 32 * 8 : 0);      // [NW][32] carry entering each warp
     static constexpr int OFF_HIN = OFF_IN + kNW * 32 * 8;                  // BWD: [NW][32] state entering each warp
     static constexpr int OFF_SCALE = OFF_HIN + (BWD ? kNW * 32 * 8 : 0);   // BWD CK: [NW][NIN][R] fp32 scales
-    static constexpr int OFF_BAR = OFF_SCALE + (BWD && CK ? kNW * NIN * kR * 4 : 0);
-    static constexpr int SMEM = OFF_BAR + (kNW + 1) * 8 + 128;
+    static constexpr int OFF_BAR = OFF_SCALE + (BWD && CK ? kNW * NIN * R * 4 : 0);
+    static constexpr int SMEM = OFF_BAR + (kNW + 1) * 8 + 8;
 };
 
 // ------------------------------------------------------------------ look-back
@@ -166,24 +272,26 @@ struct TrainCfg {
 template <bool REV, class Wait>
 __device__ __forceinline__ float2 look_back(const TrainParams& p, int64_t tile, int pos, bool last, int lane,
                                             float2& carry, const float4* s_map, float2* s_in, Wait maps_ready) {
-    const int nagg = min(pos - 1, kTrainDepth);
+    const int nagg = min(pos - 1, p.depth);
+    const bool seg = p.seg != nullptr;
     bool have = pos == 0, mapped = false;
     float2 A, B;
+    const int64_t step = int64_t(p.nchains) * 32;
     for (uint32_t it = 0;; ++it) {
         bool progressed = false;
         if (!have) {
-            bool valid = true;
-            float2 accA = splat2(1.0f), accB = splat2(0.0f);
-            for (int j = 0; j < nagg; ++j) {
-                const ulonglong2 m = ld_relaxed_v2u64(p.agg + (tile - int64_t(j + 1) * p.nchains) * 32 + lane);
-                valid &= rec_set(m.x) & rec_set(m.y);  // (A0, B0), (A1, B1)
-                accB = apply(accA, make_float2(rec_hi(m.x), rec_hi(m.y)), accB);
-                accA = mulz(accA, make_float2(rec_lo(m.x), rec_lo(m.y)));
-            }
+            const ulonglong2* src = p.agg + (tile - p.nchains) * 32 + lane;
             const unsigned long long c = ld_relaxed_u64(p.incl + (tile - int64_t(nagg + 1) * p.nchains) * 32 + lane);
-            valid &= rec_set(c);
+            bool valid = rec_set(c);
+            float2 accA = splat2(1.0f), accB = splat2(0.0f);
+            for (int j = 0; j < nagg; ++j, src -= step) {
+                const ulonglong2 m = ld_relaxed_v2u64(src);
+                valid &= rec_set(m.x) & rec_set(m.y);  // (A0, B0), (A1, B1)
+                accB = apply(accA, make_float2(rec_hi(m.x), rec_hi(m.y)), accB, seg);
+                accA = mulz(accA, make_float2(rec_lo(m.x), rec_lo(m.y)), seg);
+            }
             if (__all_sync(0xffffffffu, valid)) {
-                carry = apply(accA, make_float2(rec_lo(c), rec_hi(c)), accB);
+                carry = apply(accA, make_float2(rec_lo(c), rec_hi(c)), accB, seg);
                 have = progressed = true;
             }
         }
@@ -194,8 +302,8 @@ __device__ __forceinline__ float2 look_back(const TrainParams& p, int64_t tile, 
 #pragma unroll
             for (int k = 0; k < kNW; ++k) {  // in the order the carry meets the warps
                 const float4 m = s_map[(REV ? kNW - 1 - k : k) * 32 + lane];
-                B = apply(make_float2(m.x, m.y), B, make_float2(m.z, m.w));
-                A = mulz(make_float2(m.x, m.y), A);
+                B = apply(make_float2(m.x, m.y), B, make_float2(m.z, m.w), seg);
+                A = mulz(make_float2(m.x, m.y), A, seg);
             }
             if (!last && pos > 0)  // the first tile's map is never composed: its carry is known
                 st_relaxed_v2u64(p.agg + tile * 32 + lane, rec_pair(A.x, B.x), rec_pair(A.y, B.y));
@@ -214,7 +322,7 @@ __device__ __forceinline__ float2 look_back(const TrainParams& p, int64_t tile, 
         }
         if (!progressed && !have && it >= 2) __nanosleep(64);
     }
-    const float2 past = apply(A, carry, B);
+    const float2 past = apply(A, carry, B, seg);
     if (!last) {
         st_relaxed_u64(p.incl + tile * 32 + lane, rec_pair(past.x, past.y));
     }
@@ -224,7 +332,7 @@ __device__ __forceinline__ float2 look_back(const TrainParams& p, int64_t tile, 
         const int w = REV ? kNW - 1 - k : k;
         s_in[w * 32 + lane] = c;
         const float4 m = s_map[w * 32 + lane];
-        c = apply(make_float2(m.x, m.y), c, make_float2(m.z, m.w));
+        c = apply(make_float2(m.x, m.y), c, make_float2(m.z, m.w), seg);
     }
     return past;
 }
@@ -232,6 +340,12 @@ __device__ __forceinline__ float2 look_back(const TrainParams& p, int64_t tile, 
 // This lane's two channels of a [.., C] fp32 row (0 past C).
 __device__ __forceinline__ float2 ld_pair(const float* row, int c, int C) {
     return make_float2(c < C ? row[c] : 0.0f, c + 1 < C ? row[c + 1] : 0.0f);
+}
+__device__ __forceinline__ float2 ld_pair_cg(const float* row, int c, int C) {  // another block's writes: from L2
+    return make_float2(c < C ? __ldcg(row + c) : 0.0f, c + 1 < C ? __ldcg(row + c + 1) : 0.0f);
+}
+__device__ __forceinline__ float2 shfl2(float2 x, int m) {
+    return make_float2(__shfl_xor_sync(0xffffffffu, x.x, m), __shfl_xor_sync(0xffffffffu, x.y, m));
 }
 __device__ __forceinline__ void st_pair(float* row, int c, int C, float2 v) {
     if (c < C) row[c] = v.x;
@@ -242,65 +356,161 @@ struct Tile {
     int pos, chunk, cblk, b, t0, c0, nvalid;
     int64_t tile;
 };
+template <int L>
 __device__ __forceinline__ Tile tile_of(const TrainParams& p, bool rev) {
     Tile t;
-    t.tile = blockIdx.x;
-    t.pos = static_cast<int>(blockIdx.x) / p.nchains;  // in the order the carry meets the tiles
-    const int chain = static_cast<int>(blockIdx.x) - t.pos * p.nchains;
+    // chains along x, then positions along them (y, then z): blocks start in that
+    // order, so the tiles a block waits for are resident or finished
+    const int chain = static_cast<int>(blockIdx.x);
+    t.pos = static_cast<int>(blockIdx.y + blockIdx.z * gridDim.y);  // in the order the carry meets the tiles
+    t.tile = int64_t(t.pos) * p.nchains + chain;
     t.chunk = rev ? p.nchunks - 1 - t.pos : t.pos;
     t.b = chain / p.ncb;
     t.cblk = chain - t.b * p.ncb;
-    t.t0 = t.chunk * kL;
+    t.t0 = t.chunk * L;
     t.c0 = t.cblk * kCB;
-    t.nvalid = min(kL, p.T - t.t0);
+    t.nvalid = min(L, p.T - t.t0);
     return t;
 }
 
 // Bit j: row wr0 + j of the tile starts a segment (rows past T: clear).
+template <int R>
 __device__ __forceinline__ uint32_t reset_bits(const TrainParams& p, const Tile& tl, int wr0, int lane) {
     bool r = false;
     const int t = tl.t0 + wr0 + lane;
-    if (p.seg != nullptr && lane < kR && t < p.T) r = p.seg[tl.b * p.sgb + int64_t(t) * p.sgt] != 0;
+    if (p.seg != nullptr && lane < R && t < p.T) r = p.seg[tl.b * p.sgb + int64_t(t) * p.sgt] != 0;
     return __ballot_sync(0xffffffffu, r);
 }
 
-// ------------------------------------------------------------------ gates
-// a, 1 - a and w = s(gate) * value from a row's streams.
-template <int FORM, typename T>
-__device__ __forceinline__ void decay(const TrainParams& p, float2 x0, float2& a, float2& na) {
-    if constexpr (FORM == FORM_GATED) {
-        sig_pair<T>(x0, a, na);
-    } else {
-        float2 s, n;
-        sig_pair<T>(x0, s, n);
-        const float2 rate = ffma2(s, splat2(p.dt_scale), splat2(p.dt_min));
-        exp_neg<T>(rate, a, na);
+// A warp's rows of stream k with plain loads, as TMA would leave them (zeros past C and T).
+template <typename T, int R>
+__device__ __forceinline__ void plain_rows(const TrainParams& p, const Tile& tl, int k, unsigned char* slot, int wr0,
+                                           int rows, int lane) {
+    const T* src = static_cast<const T*>(p.src[k]) + tl.b * p.ssb[k] + int64_t(tl.t0 + wr0) * p.sst[k];
+    const int c = tl.c0 + 2 * lane;
+    for (int r = 0; r < R; ++r) {
+        const float x = r < rows && c < p.C ? to_f(src[r * p.sst[k] + c]) : 0.0f;
+        const float y = r < rows && c + 1 < p.C ? to_f(src[r * p.sst[k] + c + 1]) : 0.0f;
+        reinterpret_cast<typename Ops<T>::P*>(slot)[r * (kCB / 2) + lane] = Ops<T>::pack(x, y);
+    }
+    __syncwarp();
+}
+
+// Starts the loads of a warp's rows: n streams, of `bytes` per element (gout,
+// stream n - 1 of the backward, of sizeof(T)), into slot(k).
+template <typename T, int N, int NIN, int IN_BYTES, int R, class Slot>
+__device__ __forceinline__ void load_rows(const TrainParams& p, const Tile& tl, int wr0, int rows, int lane,
+                                          uint64_t* bar, bool stacked, Slot slot) {
+    if (rows > 0) {
+        if (lane == 0) {
+            uint32_t tx = 0;
+#pragma unroll
+            for (int k = 0; k < N; ++k)
+                if (!((p.plain >> k) & 1u)) tx += R * kCB * (k < NIN ? IN_BYTES : Ops<T>::BYTES);
+            mbar_arrive_expect_tx(bar, tx);
+#pragma unroll
+            for (int k = 0; k < N; ++k)
+                if (!((p.plain >> k) & 1u))
+                    tma_load_3d(slot(k), &p.tm[k], tl.c0, tl.t0 + wr0, stacked && k < NIN ? k * p.nb + tl.b : tl.b, bar);
+        }
+        if (p.plain != 0)
+            for (int k = 0; k < N; ++k)
+                if ((p.plain >> k) & 1u) plain_rows<T, R>(p, tl, k, slot(k), wr0, rows, lane);
+    }
+}
+
+// a and 1 - a of the decay stream's four channels.
+template <int FORM, typename T, int DT>
+__device__ __forceinline__ void decay4(const TrainParams& p, const F4& x, F4& a, F4& na, F4& s) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        if constexpr (FORM == FORM_GATED) {
+            sig_pair<T>(x.p[i], a.p[i], na.p[i]);
+        } else {
+            s.p[i] = sig_only<T>(x.p[i]);
+            const float2 r = ffma2(s.p[i], splat2(p.dt_scale), splat2(p.dt_min));
+            if constexpr (DT == 1) exp_neg_small(r, a.p[i], na.p[i]);
+            else exp_neg<T>(r, a.p[i], na.p[i]);
+        }
+    }
+}
+
+// The 8-bit copies of a warp's rows: a lane takes 16 bytes, 64 channels lie in
+// 64 / N neighbouring lanes.
+template <typename T, int NIN, int R>
+__device__ __forceinline__ void write_e4m3(const TrainParams& p, const Tile& tl, const unsigned char* base, int slot_bytes,
+                                           int wr0, int rows, int lane) {
+    constexpr int N = 16 / Ops<T>::BYTES, LPR = kCB / N, RP = 32 / LPR;  // elements, lanes per row, rows at once
+    const int v = lane % LPR;
+    const int64_t pitch = int64_t(p.ncb) * kCB;
+#pragma unroll
+    for (int k = 0; k < NIN; ++k) {
+        const unsigned char* slot = base + k * slot_bytes;
+        const int64_t first = (int64_t(k) * p.nb + tl.b) * p.T + tl.t0 + wr0;
+#pragma unroll
+        for (int r0 = 0; r0 < R; r0 += RP) {
+            const int r = r0 + lane / LPR;
+            const uint4 raw = reinterpret_cast<const uint4*>(slot)[r * LPR + v];
+            const typename Ops<T>::P* h = reinterpret_cast<const typename Ops<T>::P*>(&raw);
+            float2 f[N / 2];
+            uint32_t top;
+#pragma unroll
+            for (int e = 0; e < N / 2; ++e) f[e] = widen(h[e]);
+            if constexpr (Ops<T>::BYTES == 2) {
+                // magnitudes of 16-bit floats order as their bits do
+                const uint32_t w[4] = {raw.x & 0x7fff7fffu, raw.y & 0x7fff7fffu, raw.z & 0x7fff7fffu, raw.w & 0x7fff7fffu};
+                uint32_t m = __vmaxu2(__vmaxu2(w[0], w[1]), __vmaxu2(w[2], w[3]));
+#pragma unroll
+                for (int d = LPR / 2; d >= 1; d >>= 1) m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, d));
+                const uint16_t b = static_cast<uint16_t>(max(m & 0xffffu, m >> 16));
+                if constexpr (std::is_same<T, __half>::value) top = __float_as_uint(__half2float(__ushort_as_half(b)));
+                else top = static_cast<uint32_t>(b) << 16;
+            } else {
+                top = 0;
+#pragma unroll
+                for (int e = 0; e < N / 2; ++e)
+                    top = max(top, max(__float_as_uint(f[e].x) & 0x7fffffffu, __float_as_uint(f[e].y) & 0x7fffffffu));
+#pragma unroll
+                for (int d = LPR / 2; d >= 1; d >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
+            }
+            const uint32_t sc = e4m3_scale_byte(top);
+            const float inv = e4m3_inverse(sc);
+            uint32_t q[N / 4];
+#pragma unroll
+            for (int e = 0; e < N / 4; ++e)
+                q[e] = e4m3_round(fmul2(f[2 * e], splat2(inv))) | uint32_t(e4m3_round(fmul2(f[2 * e + 1], splat2(inv)))) << 16;
+            if (r < rows) {
+                uint8_t* dst = p.q + (first + r) * pitch + tl.c0 + v * N;
+                if constexpr (N == 8) *reinterpret_cast<uint2*>(dst) = make_uint2(q[0], q[1]);
+                else *reinterpret_cast<uint32_t*>(dst) = q[0];
+                if (v == 0) p.qs[(first + r) * p.ncb + tl.cblk] = static_cast<uint8_t>(sc);
+            }
+        }
     }
 }
 
 // ------------------------------------------------------------------ forward
-template <int FORM, typename T, bool CK>
-__global__ void __launch_bounds__(kNT) train_fwd_kernel(const __grid_constant__ TrainParams p) {
-    using K = TrainCfg<FORM, T, CK, false>;
-    using O = Ops<T>;
-    extern __shared__ unsigned char smem_raw[];
-    unsigned char* base =
-        reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 127) & ~uintptr_t(127));
+template <int FORM, typename T, bool CK, int DT>
+__global__ void __launch_bounds__(kNT, K_FWD_MINB) train_fwd_kernel(const __grid_constant__ TrainParams p) {
+    using K = TrainCfg<FORM, T, CK, DT, false>;
+    extern __shared__ __align__(128) unsigned char base[];
     float4* s_map = reinterpret_cast<float4*>(base + K::OFF_MAP);
     float2* s_in = reinterpret_cast<float2*>(base + K::OFF_IN);
     uint64_t* s_bar = reinterpret_cast<uint64_t*>(base + K::OFF_BAR);
     uint64_t* s_maps = s_bar + kNW;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const Tile tl = tile_of(p, false);
+    const bool seg = p.seg != nullptr;
+    const Tile tl = tile_of<K::L>(p, false);
+    if (tl.pos >= p.nchunks) return;
     if (threadIdx.x == 0) {
         for (int w = 0; w < kNW; ++w) mbar_init(&s_bar[w], 1);
         mbar_init(s_maps, kNW * 32);
         fence_barrier_init();
     }
     __syncthreads();
-    const int c = tl.c0 + 2 * lane;  // this lane's channels c, c + 1
 
     if (warp == kNW) {
+        const int c = tl.c0 + 2 * lane;
         const bool last = tl.chunk + 1 == p.nchunks;
         float2 carry = splat2(0.0f);
         if (tl.pos == 0 && p.h0 != nullptr) carry = ld_pair(p.h0 + int64_t(tl.b) * p.C, c, p.C);
@@ -309,104 +519,128 @@ __global__ void __launch_bounds__(kNT) train_fwd_kernel(const __grid_constant__ 
         });
         __syncwarp();
         named_arrive(1, kNT);
-        st_pair(p.states + (int64_t(tl.b) * p.nchunks + tl.chunk) * p.C, c, p.C, carry);
+        float* st = p.states + (int64_t(tl.b) * p.nspans + tl.t0 / kSpan) * p.C;
+        st_pair(st, c, p.C, carry);
+        if (K::L > kSpan && tl.nvalid > kSpan) st_pair(st + p.C, c, p.C, s_in[kSpan / K::R * 32 + lane]);
         if (last && p.h_final != nullptr) st_pair(p.h_final + int64_t(tl.b) * p.C, c, p.C, past);
         return;
     }
 
-    const int wr0 = warp * kR;
-    const int rows = max(0, min(kR, tl.nvalid - wr0));
-    if (lane == 0 && rows > 0) {
-        mbar_arrive_expect_tx(&s_bar[warp], K::NIN * K::IN_SLOT / kNW);
-#pragma unroll
-        for (int k = 0; k < K::NIN; ++k)
-            tma_load_3d(base + k * K::IN_SLOT + wr0 * kCB * K::IN_BYTES, &p.tm[k], tl.c0, tl.t0 + wr0, tl.b,
-                        &s_bar[warp]);
+    constexpr int RT = K::RT;
+    const int wr0 = warp * K::R;
+    const int rows = max(0, min(K::R, tl.nvalid - wr0));
+    unsigned char* slots = base + wr0 * kCB * K::IN_BYTES;  // this warp's rows of stream 0
+    auto slot = [&](int k) { return slots + k * K::IN_SLOT; };
+    load_rows<T, K::NIN, K::NIN, K::IN_BYTES, K::R>(p, tl, wr0, rows, lane, &s_bar[warp], false, slot);
+    const uint32_t wresets = reset_bits<K::R>(p, tl, wr0, lane);
+    const int q = lane >> 4, v = lane & 15;          // row group (half the warp's rows) and four channels
+    const int c = tl.c0 + 4 * v;
+    const uint32_t resets = (wresets >> (RT * q)) & ((1u << RT) - 1u);
+    F4 D;
+    if constexpr (FORM == FORM_SSD) {
+        D.p[0] = ld_pair(p.dskip, c, p.C);
+        D.p[1] = ld_pair(p.dskip, c + 2, p.C);
     }
-    const uint32_t resets = reset_bits(p, tl, wr0, lane);
-    float2 D = splat2(0.0f);
-    if constexpr (FORM == FORM_SSD) D = ld_pair(p.dskip, c, p.C);
     if (rows > 0 && !mbar_wait_bounded(&s_bar[warp], 0, kTmaPolls)) {
         atomicOr(&p.hdr[WS_ERROR], ERR_TMA);
         mbar_wait_bounded(&s_bar[warp], 0, kTmaPolls);
     }
-    const unsigned char* in[K::NIN];
-#pragma unroll
-    for (int k = 0; k < K::NIN; ++k) in[k] = base + k * K::IN_SLOT + wr0 * kCB * K::IN_BYTES;
 
     // phase 1: each row's state from a zero entering state (H) and the product
-    // of a up to it (P); the last is the warp's map
-    float2 P[kR], H[kR];
-    float2 A = splat2(1.0f), B = splat2(0.0f);
-    if (rows > 0) {
+    // of a up to it (P); the last are the thread's map.  Rows past T pass the
+    // state on; a reset drops it.
+    F4 P[RT], H[RT], A, B;
 #pragma unroll
-        for (int j = 0; j < kR; ++j) {
-            float2 a, na, s, n;
-            decay<FORM, T>(p, pair_at<T>(in[0], j, lane), a, na);
-            sig_pair<T>(pair_at<T>(in[1], j, lane), s, n);
-            const float2 b = fmul2(na, fmul2(s, pair_at<T>(in[2], j, lane)));
-            if ((resets >> j) & 1u) {
-                A = splat2(0.0f);
-                B = b;
-            } else if (j < rows) {
-                B = ffma2(a, B, b);
-                A = (resets & ((1u << j) - 1u)) ? A : fmul2(a, A);  // stays 0 after a reset
-            }
-            P[j] = A;
-            H[j] = B;
-        }
-    }
-    s_map[warp * 32 + lane] = make_float4(A.x, A.y, B.x, B.y);
-    mbar_arrive(s_maps);
-
-    if constexpr (CK) {  // the 8-bit copies, while the carry comes in
-        const int64_t pitch = int64_t(p.ncb) * kCB;
+    for (int i = 0; i < 2; ++i) A.p[i] = splat2(1.0f), B.p[i] = splat2(0.0f);
+    auto phase1 = [&](auto whole) {
 #pragma unroll
-        for (int k = 0; k < K::NIN; ++k) {
+        for (int j = 0; j < RT; ++j) {
+            const int r = q * RT + j;
+            F4 a, na, s;
+            decay4<FORM, T, DT>(p, row4<T>(slot(0), r, v), a, na, s);
+            const F4 g = sig4<T>(row4<T>(slot(1), r, v)), x = row4<T>(slot(2), r, v);
 #pragma unroll
-            for (int j = 0; j < kR; ++j) {
-                if (j < rows) {
-                    const float2 x = pair_at<T>(in[k], j, lane);
-                    const uint32_t top =
-                        __reduce_max_sync(0xffffffffu, max(__float_as_uint(x.x) & 0x7fffffffu,
-                                                           __float_as_uint(x.y) & 0x7fffffffu));
-                    const uint32_t sc = e4m3_scale_byte(top);
-                    const int64_t row = (int64_t(k) * p.nb + tl.b) * p.T + tl.t0 + wr0 + j;
-                    *reinterpret_cast<uint16_t*>(p.q + row * pitch + c) = e4m3_pair(x, sc);
-                    if (lane == 0) p.qs[row * p.ncb + tl.cblk] = static_cast<uint8_t>(sc);
+            for (int i = 0; i < 2; ++i) {
+                const float2 b = fmul2(na.p[i], fmul2(g.p[i], x.p[i]));
+                if constexpr (decltype(whole)::value) {
+                    B.p[i] = j == 0 ? b : ffma2(a.p[i], B.p[i], b);
+                    A.p[i] = j == 0 ? a.p[i] : fmul2(a.p[i], A.p[i]);
+                } else if (r < rows) {
+                    const bool cut = ((resets >> j) & 1u) != 0u;
+                    B.p[i] = cut ? b : ffma2(a.p[i], B.p[i], b);
+                    A.p[i] = (resets & ((2u << j) - 1u)) != 0u ? splat2(0.0f) : fmul2(a.p[i], A.p[i]);
                 }
+                P[j].p[i] = A.p[i];
+                H[j].p[i] = B.p[i];
             }
         }
+    };
+    const bool whole = rows == K::R && wresets == 0u;
+    if (whole) phase1(std::true_type{});
+    else if (rows > 0) phase1(std::false_type{});
+    // the two groups of a warp: EA, EB the map of the rows before this thread's,
+    // and the warp's map from the second group
+    F4 EA, EB;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const float2 oA = shfl2(A.p[i], 16), oB = shfl2(B.p[i], 16);
+        EA.p[i] = q == 0 ? splat2(1.0f) : oA;
+        EB.p[i] = q == 0 ? splat2(0.0f) : oB;
+        if (q == 1) {
+            const float2 tB = apply(A.p[i], oB, B.p[i], seg), tA = mulz(A.p[i], oA, seg);
+            s_map[warp * 32 + 2 * v + i] = make_float4(tA.x, tA.y, tB.x, tB.y);
+        }
     }
+    mbar_arrive(s_maps);
+    if constexpr (CK)  // while the carry comes in
+        if (rows > 0) write_e4m3<T, K::NIN, K::R>(p, tl, slots, K::IN_SLOT, wr0, rows, lane);
     named_sync(1, kNT);
+    if (rows == 0) return;
 
     // phase 2: the states from the entering one, and the outputs
-    const float2 hin = s_in[warp * 32 + lane];
-    T* orow = static_cast<T*>(p.out) + tl.b * p.osb + int64_t(tl.t0 + wr0) * p.ost + c;
+    const float4 in4 = reinterpret_cast<const float4*>(s_in)[warp * 16 + v];
+    F4 h0;
+    h0.p[0] = apply(EA.p[0], make_float2(in4.x, in4.y), EB.p[0], seg);
+    h0.p[1] = apply(EA.p[1], make_float2(in4.z, in4.w), EB.p[1], seg);
+    constexpr int OUT = K::NIN - 1;  // results replace the last stream
+    auto phase2 = [&](auto whole) {
 #pragma unroll
-    for (int j = 0; j < kR; ++j) {
-        if (j < rows) {
-            const bool cut = (resets & ((2u << j) - 1u)) != 0u;
-            float2 o = cut ? H[j] : ffma2(P[j], hin, H[j]);
+        for (int j = 0; j < RT; ++j) {
+            const int r = q * RT + j;
+            F4 o, sc, so, u;
             if constexpr (FORM == FORM_SSD) {
-                float2 s, n, g;
-                sig_pair<T>(pair_at<T>(in[3], j, lane), s, n);
-                sig_pair<T>(pair_at<T>(in[4], j, lane), g, n);
-                o = fmul2(ffma2(s, o, fmul2(D, pair_at<T>(in[2], j, lane))), g);
+                sc = sig4<T>(row4<T>(slot(3), r, v));
+                so = sig4<T>(row4<T>(slot(4), r, v));
+                u = row4<T>(slot(2), r, v);
             }
-            if (c < p.C) *reinterpret_cast<typename O::P*>(orow + j * p.ost) = O::pack(o.x, o.y);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                o.p[i] = ffma2(P[j].p[i], h0.p[i], H[j].p[i]);
+                if constexpr (!decltype(whole)::value)
+                    if ((resets & ((2u << j) - 1u)) != 0u) o.p[i] = H[j].p[i];
+                if constexpr (FORM == FORM_SSD)
+                    o.p[i] = fmul2(ffma2(sc.p[i], o.p[i], fmul2(D.p[i], u.p[i])), so.p[i]);
+            }
+            put4<T>(slot(OUT), r, v, o);
         }
+    };
+    if (whole) phase2(std::true_type{});
+    else phase2(std::false_type{});
+    fence_proxy_async_shared();
+    __syncwarp();
+    if (lane == 0) {
+        tma_store_3d(&p.tmo[0], slot(OUT), tl.c0, tl.t0 + wr0, tl.b);
+        tma_store_commit();
+        tma_store_drain();
     }
 }
 
 // ------------------------------------------------------------------ backward
-template <int FORM, typename T, bool CK>
-__global__ void __launch_bounds__(kNT) train_bwd_kernel(const __grid_constant__ TrainParams p) {
-    using K = TrainCfg<FORM, T, CK, true>;
+template <int FORM, typename T, bool CK, int DT>
+__global__ void __launch_bounds__(kNT, K_BWD_MINB) train_bwd_kernel(const __grid_constant__ TrainParams p) {
+    using K = TrainCfg<FORM, T, CK, DT, true>;
     using O = Ops<T>;
-    extern __shared__ unsigned char smem_raw[];
-    unsigned char* base =
-        reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 127) & ~uintptr_t(127));
+    extern __shared__ __align__(128) unsigned char base[];
     float4* s_map = reinterpret_cast<float4*>(base + K::OFF_MAP);
     float2* s_fwd = reinterpret_cast<float2*>(base + K::OFF_FWD);
     float2* s_in = reinterpret_cast<float2*>(base + K::OFF_IN);
@@ -414,19 +648,24 @@ __global__ void __launch_bounds__(kNT) train_bwd_kernel(const __grid_constant__ 
     float* s_scale = reinterpret_cast<float*>(base + K::OFF_SCALE);
     uint64_t* s_bar = reinterpret_cast<uint64_t*>(base + K::OFF_BAR);
     uint64_t* s_maps = s_bar + kNW;
+    uint32_t* s_last = reinterpret_cast<uint32_t*>(s_maps + 1);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const Tile tl = tile_of(p, true);
+    const bool seg = p.seg != nullptr;
+    const Tile tl = tile_of<K::L>(p, true);
+    if (tl.pos >= p.nchunks) return;
     if (threadIdx.x == 0) {
         for (int w = 0; w < kNW; ++w) mbar_init(&s_bar[w], 1);
         mbar_init(s_maps, kNW * 32);
         fence_barrier_init();
     }
     __syncthreads();
-    const int c = tl.c0 + 2 * lane;
 
     if (warp == kNW) {
+        const int c = tl.c0 + 2 * lane;
         const bool last = tl.chunk == 0;
-        float2 h = ld_pair(p.states + (int64_t(tl.b) * p.nchunks + tl.chunk) * p.C, c, p.C);
+        const float* st = p.states + (int64_t(tl.b) * p.nspans + tl.t0 / kSpan) * p.C;
+        float2 h = ld_pair(st, c, p.C), hmid = splat2(0.0f);
+        if (K::L > kSpan && tl.nvalid > kSpan) hmid = ld_pair(st + p.C, c, p.C);
         float2 carry = splat2(0.0f);
         if (tl.pos == 0 && p.g_final != nullptr) carry = ld_pair(p.g_final + int64_t(tl.b) * p.C, c, p.C);
         bool handed = false;
@@ -437,9 +676,10 @@ __global__ void __launch_bounds__(kNT) train_bwd_kernel(const __grid_constant__ 
                 handed = true;
 #pragma unroll
                 for (int w = 0; w < kNW; ++w) {
+                    if (K::L > kSpan && w == kSpan / K::R) h = hmid;
                     s_hin[w * 32 + lane] = h;
                     const float4 m = s_map[w * 32 + lane];
-                    h = apply(make_float2(m.x, m.y), h, s_fwd[w * 32 + lane]);
+                    h = apply(make_float2(m.x, m.y), h, s_fwd[w * 32 + lane], seg);
                 }
                 __syncwarp();
                 named_arrive(1, kNT);
@@ -453,181 +693,294 @@ __global__ void __launch_bounds__(kNT) train_bwd_kernel(const __grid_constant__ 
         return;
     }
 
-    const int wr0 = warp * kR;
-    const int rows = max(0, min(kR, tl.nvalid - wr0));
-    if (lane == 0 && rows > 0) {
-        mbar_arrive_expect_tx(&s_bar[warp], (K::NIN * K::IN_SLOT + kL * kCB * O::BYTES) / kNW);
-#pragma unroll
-        for (int k = 0; k < K::NIN; ++k)
-            tma_load_3d(base + k * K::IN_SLOT + wr0 * kCB * K::IN_BYTES, &p.tm[k], tl.c0, tl.t0 + wr0,
-                        CK ? k * p.nb + tl.b : tl.b, &s_bar[warp]);
-        tma_load_3d(base + K::OFF_GOUT + wr0 * kCB * O::BYTES, &p.tm[K::NIN], tl.c0, tl.t0 + wr0, tl.b,
-                    &s_bar[warp]);
-    }
-    const uint32_t resets = reset_bits(p, tl, wr0, lane);
+    constexpr int RT = K::RT;
+    const int wr0 = warp * K::R;
+    const int rows = max(0, min(K::R, tl.nvalid - wr0));
+    auto slot = [&](int k) {
+        return k < K::NIN ? base + k * K::IN_SLOT + wr0 * kCB * K::IN_BYTES : base + K::OFF_GOUT + wr0 * kCB * O::BYTES;
+    };
+    auto stage = [&](int k) {  // kept sigmoids, then gradients
+        return K::STAGED ? base + K::OFF_STAGE + k * K::SLOT + wr0 * kCB * O::BYTES : slot(k);
+    };
+    load_rows<T, K::NIN + 1, K::NIN, K::IN_BYTES, K::R>(p, tl, wr0, rows, lane, &s_bar[warp], CK, slot);
+    const uint32_t wresets = reset_bits<K::R>(p, tl, wr0, lane);
     if constexpr (CK) {
-        for (int i = lane; i < K::NIN * kR; i += 32) {
-            const int k = i / kR, j = i - k * kR;
+        for (int i = lane; i < K::NIN * K::R; i += 32) {
+            const int k = i / K::R, j = i - k * K::R;
             float f = 0.0f;
             if (j < rows)
                 f = e4m3_scale(p.qs[((int64_t(k) * p.nb + tl.b) * p.T + tl.t0 + wr0 + j) * p.ncb + tl.cblk]);
-            s_scale[warp * K::NIN * kR + i] = f;
+            s_scale[warp * K::NIN * K::R + i] = f;
         }
         __syncwarp();
     }
-    float2 D = splat2(0.0f);
-    if constexpr (FORM == FORM_SSD) D = ld_pair(p.dskip, c, p.C);
+    const int q = lane >> 4, v = lane & 15;
+    const int c = tl.c0 + 4 * v;
+    const uint32_t resets = (wresets >> (RT * q)) & ((1u << RT) - 1u);
+    F4 D;
+    if constexpr (FORM == FORM_SSD) {
+        D.p[0] = ld_pair(p.dskip, c, p.C);
+        D.p[1] = ld_pair(p.dskip, c + 2, p.C);
+    }
     if (rows > 0 && !mbar_wait_bounded(&s_bar[warp], 0, kTmaPolls)) {
         atomicOr(&p.hdr[WS_ERROR], ERR_TMA);
         mbar_wait_bounded(&s_bar[warp], 0, kTmaPolls);
     }
-    auto input = [&](int k, int j) {
-        const unsigned char* slot = base + k * K::IN_SLOT + wr0 * kCB * K::IN_BYTES;
-        if constexpr (CK) return pair8_at(slot, j, lane, s_scale[(warp * K::NIN + k) * kR + j]);
-        else return pair_at<T>(slot, j, lane);
+    auto input = [&](int k, int r) {
+        if constexpr (CK) return row4_8(slot(k), r, v, s_scale[(warp * K::NIN + k) * K::R + r]);
+        else return row4<T>(slot(k), r, v);
     };
-    auto gout = [&](int j) { return pair_at<T>(base + K::OFF_GOUT + wr0 * kCB * O::BYTES, j, lane); };
-
-    // phase 1: the warp's maps.  Forward: h_out = A h_in + B.  Backward, over
-    // the same a: mu_first = A mu_in + M, M = sum over rows of (product of a up
-    // to the row) e.
-    float2 a[kR], h[kR];
-    float2 A = splat2(1.0f), B = splat2(0.0f), M = splat2(0.0f);
-    if (rows > 0) {
+    auto gout = [&](int r) { return row4<T>(slot(K::NIN), r, v); };
+    // sigmoid of logit stream k again (or as kept), and its slope
+    auto gate = [&](int k, int r, F4& s, F4& slope) {
+        if constexpr (kKeep<T>) {
+            kept4<T>(stage(k), r, v, s, slope);
+        } else {
+            const F4 x = input(k, r);
 #pragma unroll
-        for (int j = 0; j < kR; ++j) {
-            float2 na, s, n;
-            decay<FORM, T>(p, input(0, j), a[j], na);
-            sig_pair<T>(input(1, j), s, n);
-            const float2 b = fmul2(na, fmul2(s, input(2, j)));
-            float2 e = gout(j);
-            if constexpr (FORM == FORM_SSD) {
-                float2 sc, so;
-                sig_pair<T>(input(3, j), sc, n);
-                sig_pair<T>(input(4, j), so, n);
-                e = fmul2(e, fmul2(so, sc));
+            for (int i = 0; i < 2; ++i) {
+                float2 n;
+                sig_pair<T>(x.p[i], s.p[i], n);
+                slope.p[i] = fmul2(s.p[i], n);
             }
-            h[j] = b;
-            if ((resets >> j) & 1u) {
-                A = splat2(0.0f);
-                B = b;
-            } else if (j < rows) {
-                B = ffma2(a[j], B, b);
-                if ((resets & ((1u << j) - 1u)) == 0u) {
-                    A = fmul2(a[j], A);
-                    M = ffma2(A, e, M);
+        }
+    };
+
+    // phase 1: the thread's maps.  Forward: h_out = A h_in + B.  Backward, over
+    // the same a: mu_first = A mu_in + M, M = sum over rows of (product of a up
+    // to the row) e.  1 - a stays in registers (and a = 1 - (1 - a): of the two
+    // the small one is the one whose relative error matters), b too, where the
+    // states then take its place.
+    F4 na[RT], h[RT], A, B, M, dD;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) A.p[i] = splat2(1.0f), B.p[i] = M.p[i] = dD.p[i] = splat2(0.0f);
+    auto one_minus = [](float2 x) { return fadd2(splat2(1.0f), make_float2(-x.x, -x.y)); };
+    auto phase1 = [&](auto whole) {
+#pragma unroll
+        for (int j = 0; j < RT; ++j) {
+            const int r = q * RT + j;
+            F4 a, sd;
+            decay4<FORM, T, DT>(p, input(0, r), a, na[j], sd);
+            const F4 g = sig4<T>(input(1, r)), x = input(2, r);
+            F4 e = gout(r);
+            keep4<T>(stage(1), r, v, g);
+            if constexpr (FORM == FORM_SSD) {
+                const F4 sc = sig4<T>(input(3, r)), so = sig4<T>(input(4, r));
+                keep4<T>(stage(0), r, v, sd);
+                keep4<T>(stage(3), r, v, sc);
+                keep4<T>(stage(4), r, v, so);
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const float2 gs = fmul2(e.p[i], so.p[i]);
+                    dD.p[i] = ffma2(gs, x.p[i], dD.p[i]);  // fp32 results come from the sigmoids as computed
+                    e.p[i] = fmul2(gs, sc.p[i]);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const float2 b = fmul2(na[j].p[i], fmul2(g.p[i], x.p[i]));
+                h[j].p[i] = b;
+                if constexpr (decltype(whole)::value) {
+                    B.p[i] = j == 0 ? b : ffma2(a.p[i], B.p[i], b);
+                    A.p[i] = j == 0 ? a.p[i] : fmul2(a.p[i], A.p[i]);
+                    M.p[i] = j == 0 ? fmul2(A.p[i], e.p[i]) : ffma2(A.p[i], e.p[i], M.p[i]);
+                } else if (r < rows) {
+                    B.p[i] = ((resets >> j) & 1u) != 0u ? b : ffma2(a.p[i], B.p[i], b);
+                    if ((resets & ((2u << j) - 1u)) != 0u) {
+                        A.p[i] = splat2(0.0f);
+                    } else {
+                        A.p[i] = fmul2(a.p[i], A.p[i]);
+                        M.p[i] = ffma2(A.p[i], e.p[i], M.p[i]);
+                    }
                 }
             }
         }
+    };
+    const bool whole = rows == K::R && wresets == 0u;
+    if (whole) phase1(std::true_type{});
+    else if (rows > 0) phase1(std::false_type{});
+    // the other row group's maps: the state enters the second group through the
+    // first's (fA, fB), mu enters the first through the second's (fA, fM)
+    F4 fA, fC;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const float2 oA = shfl2(A.p[i], 16), oB = shfl2(B.p[i], 16), oM = shfl2(M.p[i], 16);
+        fA.p[i] = oA;
+        fC.p[i] = q == 1 ? oB : oM;
+        if (q == 1) {
+            const float2 tA = mulz(A.p[i], oA, seg), tB = apply(A.p[i], oB, B.p[i], seg);
+            const float2 tM = apply(oA, M.p[i], oM, seg);
+            s_map[warp * 32 + 2 * v + i] = make_float4(tA.x, tA.y, tM.x, tM.y);
+            s_fwd[warp * 32 + 2 * v + i] = tB;
+        }
     }
-    s_map[warp * 32 + lane] = make_float4(A.x, A.y, M.x, M.y);
-    s_fwd[warp * 32 + lane] = B;
     mbar_arrive(s_maps);
     named_sync(1, kNT);
 
-    // the states of the warp's rows, from the one entering them
-    const float2 hin = s_hin[warp * 32 + lane];
-    if (rows > 0) {
-        float2 hp = hin;
+    // the states of the thread's rows, from the one entering them
+    F4 hin;
+    {
+        const float4 in4 = reinterpret_cast<const float4*>(s_hin)[warp * 16 + v];
+        hin.p[0] = make_float2(in4.x, in4.y);
+        hin.p[1] = make_float2(in4.z, in4.w);
 #pragma unroll
-        for (int j = 0; j < kR; ++j) {
-            h[j] = ((resets >> j) & 1u) ? h[j] : ffma2(a[j], hp, h[j]);
-            hp = h[j];
+        for (int i = 0; i < 2; ++i) {
+            if (q == 1) hin.p[i] = apply(fA.p[i], hin.p[i], fC.p[i], seg);
+            float2 hp = hin.p[i];
+            if (rows > 0) {
+#pragma unroll
+                for (int j = 0; j < RT; ++j) {
+                    const bool cut = ((resets >> j) & 1u) != 0u;
+                    h[j].p[i] = cut ? h[j].p[i] : ffma2(one_minus(na[j].p[i]), hp, h[j].p[i]);
+                    hp = h[j].p[i];
+                }
+            }
         }
     }
     named_sync(2, kNT);
 
     // phase 2: the rows from last to first
-    float2 mu = s_in[warp * 32 + lane];
-    float2 dD = splat2(0.0f);
-    const int64_t row0 = (int64_t(tl.b) * p.T + tl.t0 + wr0) * p.C + c;
-    auto put = [&](int k, int j, float2 v) {
-        if (c < p.C)
-            *reinterpret_cast<typename O::P*>(static_cast<T*>(p.grad[k]) + row0 + int64_t(j) * p.C) =
-                O::pack(v.x, v.y);
-    };
+    F4 mu;
+    {
+        const float4 in4 = reinterpret_cast<const float4*>(s_in)[warp * 16 + v];
+        mu.p[0] = make_float2(in4.x, in4.y);
+        mu.p[1] = make_float2(in4.z, in4.w);
 #pragma unroll
-    for (int j = kR - 1; j >= 0; --j) {
-        if (j < rows) {
-            const bool reset = ((resets >> j) & 1u) != 0u;
-            const float2 prev = reset ? splat2(0.0f) : (j > 0 ? h[j > 0 ? j - 1 : 0] : hin);
-            float2 s0, n0, aj, na, sg, ng;
-            const float2 x0 = input(0, j), val = input(2, j);
-            if constexpr (FORM == FORM_GATED) {
-                sig_pair<T>(x0, aj, na);
-            } else {
-                sig_pair<T>(x0, s0, n0);
-                exp_neg<T>(ffma2(s0, splat2(p.dt_scale), splat2(p.dt_min)), aj, na);
-            }
-            sig_pair<T>(input(1, j), sg, ng);
-            const float2 go = gout(j);
-            float2 e = go, gs = go;
-            if constexpr (FORM == FORM_SSD) {
-                float2 sc, nc, so, no;
-                sig_pair<T>(input(3, j), sc, nc);
-                sig_pair<T>(input(4, j), so, no);
-                gs = fmul2(go, so);
-                e = fmul2(gs, sc);
-                put(3, j, fmul2(fmul2(gs, h[j]), fmul2(sc, nc)));
-                const float2 v = ffma2(sc, h[j], fmul2(D, val));
-                put(4, j, fmul2(fmul2(gs, v), no));
-                dD = ffma2(gs, val, dD);
-            }
-            const float2 lam = fadd2(e, mu);
-            mu = reset ? splat2(0.0f) : fmul2(aj, lam);
-            const float2 w = fmul2(sg, val);
-            const float2 da = fmul2(lam, fadd2(prev, make_float2(-w.x, -w.y)));
-            const float2 dw = fmul2(lam, na);
-            if constexpr (FORM == FORM_GATED) {
-                put(0, j, fmul2(da, fmul2(aj, na)));
-                put(2, j, fmul2(dw, sg));
-            } else {
-                const float2 slope = fmul2(fmul2(s0, n0), splat2(-p.dt_scale));
-                put(0, j, fmul2(fmul2(da, aj), slope));
-                put(2, j, ffma2(dw, sg, fmul2(D, gs)));
-            }
-            put(1, j, fmul2(fmul2(dw, val), fmul2(sg, ng)));
+        for (int i = 0; i < 2; ++i) {
+            if (q == 0) mu.p[i] = apply(fA.p[i], mu.p[i], fC.p[i], seg);
         }
     }
+    auto phase2 = [&](auto whole) {
+#pragma unroll
+        for (int j = RT - 1; j >= 0; --j) {
+            const int r = q * RT + j;
+            if (!decltype(whole)::value && r >= rows) continue;
+            const bool reset = !decltype(whole)::value && ((resets >> j) & 1u) != 0u;
+            F4 sg, lg, val = input(2, r), e = gout(r), gs, d[5];
+            gate(1, r, sg, lg);
+            if constexpr (FORM == FORM_SSD) {
+                F4 sc, lc, so, lo;
+                gate(3, r, sc, lc);
+                gate(4, r, so, lo);
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const float2 go = e.p[i];
+                    gs.p[i] = fmul2(go, so.p[i]);
+                    e.p[i] = fmul2(gs.p[i], sc.p[i]);
+                    d[3].p[i] = fmul2(fmul2(gs.p[i], h[j].p[i]), lc.p[i]);
+                    d[4].p[i] = fmul2(fmul2(go, ffma2(sc.p[i], h[j].p[i], fmul2(D.p[i], val.p[i]))), lo.p[i]);
+                }
+                put4<T>(stage(3), r, v, d[3]);
+                put4<T>(stage(4), r, v, d[4]);
+            }
+            F4 sd, ld;
+            if constexpr (FORM == FORM_SSD) gate(0, r, sd, ld);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const float2 a = one_minus(na[j].p[i]), n = na[j].p[i];
+                const float2 prev = reset ? splat2(0.0f) : (j > 0 ? h[j > 0 ? j - 1 : 0].p[i] : hin.p[i]);
+                const float2 lam = fadd2(e.p[i], mu.p[i]);
+                mu.p[i] = reset ? splat2(0.0f) : fmul2(a, lam);
+                const float2 w = fmul2(sg.p[i], val.p[i]);
+                const float2 da = fmul2(fmul2(lam, a), fadd2(prev, make_float2(-w.x, -w.y)));
+                const float2 dw = fmul2(lam, n);
+                d[1].p[i] = fmul2(fmul2(dw, val.p[i]), lg.p[i]);
+                if constexpr (FORM == FORM_GATED) {
+                    d[0].p[i] = fmul2(da, n);
+                    d[2].p[i] = fmul2(dw, sg.p[i]);
+                } else {
+                    d[0].p[i] = fmul2(da, fmul2(ld.p[i], splat2(-p.dt_scale)));
+                    d[2].p[i] = ffma2(dw, sg.p[i], fmul2(D.p[i], gs.p[i]));
+                }
+            }
+            put4<T>(stage(0), r, v, d[0]);
+            put4<T>(stage(1), r, v, d[1]);
+            put4<T>(stage(2), r, v, d[2]);
+        }
+    };
+    if (whole) phase2(std::true_type{});
+    else if (rows > 0) phase2(std::false_type{});
+    fence_proxy_async_shared();
+    __syncwarp();
+    if (lane == 0 && rows > 0) {
+#pragma unroll
+        for (int k = 0; k < K::NIN; ++k) tma_store_3d(&p.tmo[k], stage(k), tl.c0, tl.t0 + wr0, tl.b);
+        tma_store_commit();
+    }
     if constexpr (FORM == FORM_SSD) {
-        // the tile's sum for the gradient of D: the warps' sums in a fixed order
-        s_fwd[warp * 32 + lane] = dD;  // the look-back warp is done with it
+        // The gradient of D: the tile's sum over its rows, then, by the last tile
+        // of the channel block to come here, the sum over the block's tiles --
+        // each in a fixed order, whichever tile is last.
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            dD.p[i] = fadd2(dD.p[i], shfl2(dD.p[i], 16));
+            if (q == 0) s_fwd[warp * 32 + 2 * v + i] = dD.p[i];  // the look-back warp is done with it
+        }
         named_sync(3, kNW * 32);
+        const int ntile = p.nb * p.nchunks;
         if (warp == 0) {
             float2 sum = splat2(0.0f);
 #pragma unroll
             for (int w = 0; w < kNW; ++w) sum = fadd2(sum, s_fwd[w * 32 + lane]);
-            st_pair(p.dpart + (int64_t(tl.b) * p.nchunks + tl.chunk) * p.C, c, p.C, sum);
+            st_pair(p.dpart + (int64_t(tl.b) * p.nchunks + tl.chunk) * p.C, tl.c0 + 2 * lane, p.C, sum);
+            __threadfence();
+            __syncwarp();
+            if (lane == 0) *s_last = atomicAdd(&p.dcount[tl.cblk], 1u) == static_cast<uint32_t>(ntile) - 1u;
+        }
+        named_sync(3, kNW * 32);
+        if (*s_last != 0u) {
+            __threadfence();
+            const int ch = tl.c0 + 2 * lane;
+            float2 sum = splat2(0.0f);
+#pragma unroll 8
+            for (int i = warp; i < ntile; i += kNW) sum = fadd2(sum, ld_pair_cg(p.dpart + int64_t(i) * p.C, ch, p.C));
+            s_hin[warp * 32 + lane] = sum;
+            named_sync(3, kNW * 32);
+            if (warp == 0) {
+                sum = splat2(0.0f);
+#pragma unroll
+                for (int w = 0; w < kNW; ++w) sum = fadd2(sum, s_hin[w * 32 + lane]);
+                st_pair(p.grad_d, ch, p.C, sum);
+            }
         }
     }
+    if (lane == 0 && rows > 0) tma_store_drain();
 }
 
 // ------------------------------------------------------------------ launch
+constexpr unsigned kMaxGridY = 65535;
+
 template <class Kern>
-int launch(Kern kern, int smem, std::atomic<uint64_t>& done, const TrainParams& P, int64_t ntiles, cudaStream_t s) {
+int launch(Kern kern, int smem, std::atomic<uint64_t>& done, const TrainParams& P, cudaStream_t s) {
     cudaError_t e = ensure_smem(kern, smem, done);
     if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(training scan)");
-    kern<<<static_cast<unsigned>(ntiles), kNT, smem, s>>>(P);
+    const unsigned z = (static_cast<unsigned>(P.nchunks) + kMaxGridY - 1) / kMaxGridY;
+    const unsigned y = (static_cast<unsigned>(P.nchunks) + z - 1) / z;
+    kern<<<dim3(static_cast<unsigned>(P.nchains), y, z), kNT, smem, s>>>(P);
     e = cudaGetLastError();
     return e == cudaSuccess ? NEED_OK : cuda_fail(e, "training scan launch");
 }
 
-template <int FORM, typename T, bool CK, bool BWD>
-int run_cfg(const TrainParams& P, int64_t ntiles, cudaStream_t s) {
+template <int FORM, typename T, bool CK, int DT, bool BWD>
+int run_cfg(const TrainParams& P, cudaStream_t s) {
     static std::atomic<uint64_t> done{0};
-    constexpr int smem = TrainCfg<FORM, T, CK, BWD>::SMEM;
-    if constexpr (BWD) return launch(train_bwd_kernel<FORM, T, CK>, smem, done, P, ntiles, s);
-    else return launch(train_fwd_kernel<FORM, T, CK>, smem, done, P, ntiles, s);
+    constexpr int smem = TrainCfg<FORM, T, CK, DT, BWD>::SMEM;
+    if constexpr (BWD) return launch(train_bwd_kernel<FORM, T, CK, DT>, smem, done, P, s);
+    else return launch(train_fwd_kernel<FORM, T, CK, DT>, smem, done, P, s);
 }
 
 template <bool BWD>
-int run(const need_scan_train_args* a, const TrainParams& P, int64_t ntiles, cudaStream_t s) {
+int run(const need_scan_train_args* a, const TrainParams& P, cudaStream_t s) {
     auto form = [&](auto tag) {
         using T = decltype(tag);
-        const bool ck = a->checkpoint != 0;
-        if (a->form == NEED_FORM_GATED)
-            return ck ? run_cfg<FORM_GATED, T, true, BWD>(P, ntiles, s) : run_cfg<FORM_GATED, T, false, BWD>(P, ntiles, s);
-        return ck ? run_cfg<FORM_SSD, T, true, BWD>(P, ntiles, s) : run_cfg<FORM_SSD, T, false, BWD>(P, ntiles, s);
+        auto go = [&](auto ck) {
+            constexpr bool CK = decltype(ck)::value;
+            if (a->form == NEED_FORM_GATED) return run_cfg<FORM_GATED, T, CK, 0, BWD>(P, s);
+            // steps of at most 1/4 (the block's are at most 0.2): e^-r by its series, see exp_neg_small
+            if (a->dt_max <= 0.25) return run_cfg<FORM_SSD, T, CK, 1, BWD>(P, s);
+            return run_cfg<FORM_SSD, T, CK, 0, BWD>(P, s);
+        };
+        return a->checkpoint != 0 ? go(std::true_type{}) : go(std::false_type{});
     };
     if (a->dtype == NEED_F32) return form(float{});
     if (a->dtype == NEED_BF16) return form(__nv_bfloat16{});
@@ -635,44 +988,40 @@ int run(const need_scan_train_args* a, const TrainParams& P, int64_t ntiles, cud
 }
 
 struct Geom {
-    int64_t ncb, nchains, nchunks, ntiles;
+    int64_t L, ncb, nchains, nchunks, ntiles;
 };
-Geom geom(int64_t nb, int64_t T, int64_t C) {
+Geom geom(int dtype, bool ck, bool bwd, int64_t nb, int64_t T, int64_t C) {
     Geom g;
+    g.L = tile_tokens(dtype_bytes(dtype), ck, bwd);
     g.ncb = (C + kCB - 1) / kCB;
     g.nchains = nb * g.ncb;
-    g.nchunks = (T + kL - 1) / kL;
+    g.nchunks = (T + g.L - 1) / g.L;
     g.ntiles = g.nchains * g.nchunks;
     return g;
 }
+// The workspace: header, look-back records and (SSD backward) the counters,
+// which the call clears, then the partial sums of the gradient of D.
 size_t rec_bytes(const Geom& g) { return g.nchunks > 1 ? size_t(g.ntiles) * kTileRecBytes : 0; }
+size_t clear_bytes(const Geom& g, bool dpart) {
+    return kHdrBytes + rec_bytes(g) + (dpart ? (size_t(g.ncb) * 4 + 15) / 16 * 16 : 0);
+}
 size_t ws_size(const Geom& g, int64_t nb, int64_t C, bool dpart) {
-    return kHdrBytes + rec_bytes(g) + (dpart ? size_t(nb) * size_t(g.nchunks) * size_t(C) * 4 : 0);
+    return clear_bytes(g, dpart) + (dpart ? size_t(nb) * size_t(g.nchunks) * size_t(C) * 4 : 0);
 }
 
-// A [nb, T, C] tensor (element strides) as a 3-D tensor map with boxes of one
-// warp's rows.
+// Whether a [nb, T, C] tensor's rows can be read or written by TMA.
+bool tma_rows(const void* ptr, int64_t sb, int64_t st, int es, int64_t nb, int64_t T) {
+    auto ok = [&](int64_t n, int64_t s) { return n == 1 || (s > 0 && s * es % 16 == 0 && s * es < (int64_t(1) << 40)); };
+    return aligned16(ptr) && ok(T, st) && ok(nb, sb);
+}
+
+// Such a tensor (element strides) as a 3-D tensor map with boxes of one warp's rows.
 int encode(CUtensorMap* tm, const void* ptr, int64_t sb, int64_t st, int es, CUtensorMapDataType ty, int64_t nb,
-           int64_t T, int64_t C, const char* what) {
-    if (ptr == nullptr) return fail(NEED_ERR_INVALID, "%s is null", what);
-    if (!aligned16(ptr)) return fail(NEED_ERR_UNSUPPORTED, "%s is not 16-byte aligned", what);
-    const int64_t sizes[2] = {T, nb}, strides[2] = {st, sb};
-    cuuint64_t gs[2];
-    int64_t prev = ((C * es + 15) / 16) * 16;  // a size-1 dim's stride is not used
-    for (int i = 0; i < 2; ++i) {
-        int64_t by = prev;
-        if (sizes[i] > 1) {
-            by = strides[i] * es;
-            if (strides[i] <= 0 || by % 16 != 0 || by >= (int64_t(1) << 40))
-                return fail(NEED_ERR_UNSUPPORTED, "%s: stride %lld must be positive and a multiple of 16 bytes", what,
-                            (long long)strides[i]);
-        }
-        gs[i] = static_cast<cuuint64_t>(by);
-        prev = by * sizes[i];
-        if (prev >= (int64_t(1) << 40)) prev = 16;
-    }
+           int64_t T, int64_t C, int64_t L, const char* what) {
+    const cuuint64_t row = (C * es + 15) / 16 * 16;  // a size-1 dim's stride is not used
+    const cuuint64_t gs[2] = {T > 1 ? cuuint64_t(st * es) : row, nb > 1 ? cuuint64_t(sb * es) : row};
     const cuuint64_t dims[3] = {cuuint64_t(C), cuuint64_t(T), cuuint64_t(nb)};
-    const cuuint32_t box[3] = {kCB, kR, 1}, estr[3] = {1, 1, 1};
+    const cuuint32_t box[3] = {kCB, cuuint32_t(L / kNW), 1}, estr[3] = {1, 1, 1};
     auto fn = encode_fn();
     if (fn == nullptr) return fail(NEED_ERR_CUDA, "cuTensorMapEncodeTiled entry point unavailable");
     const CUresult r = fn(tm, ty, 3, const_cast<void*>(ptr), dims, gs, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
@@ -697,12 +1046,10 @@ int prepare(const need_scan_train_args* a, bool bwd, TrainParams* P, Geom* g) {
     if (a->nb < 1 || a->T < 1 || a->C < 1)
         return fail(NEED_ERR_INVALID, "sizes must be >= 1 (nb=%lld T=%lld C=%lld)", (long long)a->nb, (long long)a->T,
                     (long long)a->C);
-    const int es = dtype_bytes(a->dtype), group = 16 / es;
-    if (a->C % group != 0)
-        return fail(NEED_ERR_UNSUPPORTED, "C=%lld must be a multiple of %d for this dtype", (long long)a->C, group);
-    if (a->nb > INT32_MAX / 8 || a->T > INT32_MAX / 2 || a->C > INT32_MAX / 2)
+    const int es = dtype_bytes(a->dtype);
+    if (a->nb > INT32_MAX / 8 || a->nb * ((a->T + kSpan - 1) / kSpan) > INT32_MAX / 2 || a->T > INT32_MAX / 2 || a->C > INT32_MAX / 2)
         return fail(NEED_ERR_UNSUPPORTED, "sizes exceed the 32-bit index range");
-    *g = geom(a->nb, a->T, a->C);
+    *g = geom(a->dtype, a->checkpoint != 0, bwd, a->nb, a->T, a->C);
     if (g->nchains > INT32_MAX || g->ntiles > INT32_MAX)
         return fail(NEED_ERR_UNSUPPORTED, "too many tiles (%lld)", (long long)g->ntiles);
     const int nin = a->form == NEED_FORM_GATED ? 3 : 5;
@@ -722,37 +1069,48 @@ int prepare(const need_scan_train_args* a, bool bwd, TrainParams* P, Geom* g) {
     if (a->workspace_bytes < ws_size(*g, a->nb, a->C, dpart))
         return fail(NEED_ERR_WORKSPACE, "workspace has %zu bytes, needs %zu", a->workspace_bytes,
                     ws_size(*g, a->nb, a->C, dpart));
+    // outputs: rows that TMA can write, at least C long
+    auto writable = [&](const void* ptr, int64_t sb, int64_t st) {
+        return ptr != nullptr && tma_rows(ptr, sb, st, es, a->nb, a->T) && (a->T == 1 || st >= a->C);
+    };
     if (bwd) {
         for (int k = 0; k < nin; ++k)
-            if (a->grad[k] == nullptr || !aligned16(a->grad[k]))
-                return fail(NEED_ERR_INVALID, "grad[%d] is null or not 16-byte aligned", k);
+            if (!writable(a->grad[k], a->grad_stride_b, a->grad_stride_t))
+                return fail(NEED_ERR_INVALID, "grad[%d] is null or its rows are not 16-byte aligned, C or more long", k);
         if (a->form == NEED_FORM_SSD && a->grad_d == nullptr) return fail(NEED_ERR_INVALID, "grad_d is null");
-    } else {
-        if (a->out == nullptr || !aligned16(a->out)) return fail(NEED_ERR_INVALID, "out is null or not 16-byte aligned");
-        if ((a->T > 1 && (a->out_stride_t < a->C || a->out_stride_t % group != 0)) ||
-            (a->nb > 1 && (a->out_stride_b <= 0 || a->out_stride_b % group != 0)))
-            return fail(NEED_ERR_UNSUPPORTED, "out strides must be positive multiples of %d elements", group);
+    } else if (!writable(a->out, a->out_stride_b, a->out_stride_t)) {
+        return fail(NEED_ERR_INVALID, "out is null or its rows are not 16-byte aligned, C or more long");
     }
+    const bool stored = bwd && a->checkpoint != 0;
+    for (int k = 0; k < nin && !stored; ++k)
+        if (a->in[k].ptr == nullptr) return fail(NEED_ERR_INVALID, "in[%d] is null", k);
+    if (bwd && a->gout.ptr == nullptr) return fail(NEED_ERR_INVALID, "gout is null");
     if (int rc = ensure_context()) return rc;
     memset(P, 0, sizeof(*P));
-    static const char* const names[5] = {"in[0]", "in[1]", "in[2]", "in[3]", "in[4]"};
-    if (bwd && a->checkpoint != 0) {
-        // every stream's 8-bit values as one [nin * nb, T, ncb * 64] tensor: the
-        // kernel adds its stream's first row of sequences to b
+    static const char* const names[6] = {"in[0]", "in[1]", "in[2]", "in[3]", "in[4]", "gout"};
+    const auto ty = map_type(a->dtype);
+    auto stream = [&](int k, const need_view& v, const char* name) {
+        if (tma_rows(v.ptr, v.stride_b, v.stride_t, es, a->nb, a->T))
+            return encode(&P->tm[k], v.ptr, v.stride_b, v.stride_t, es, ty, a->nb, a->T, a->C, g->L, name);
+        P->plain |= 1u << k;
+        P->src[k] = v.ptr, P->ssb[k] = v.stride_b, P->sst[k] = v.stride_t;
+        return int(NEED_OK);
+    };
+    for (int k = 0; k < nin; ++k) {
         const int64_t pitch = g->ncb * kCB;
-        for (int k = 0; k < nin; ++k)
-            if (int rc = encode(&P->tm[k], a->ckpt_values, a->T * pitch, pitch, 1, CU_TENSOR_MAP_DATA_TYPE_UINT8,
-                                nin * a->nb, a->T, pitch, "ckpt_values"))
-                return rc;
-    } else {
-        for (int k = 0; k < nin; ++k)
-            if (int rc = encode(&P->tm[k], a->in[k].ptr, a->in[k].stride_b, a->in[k].stride_t, es, map_type(a->dtype),
-                                a->nb, a->T, a->C, names[k]))
-                return rc;
+        // the 8-bit values of every stream as one [nin * nb, T, ncb * 64] tensor: the
+        // kernel adds its stream's first sequence to b
+        const int rc = stored ? encode(&P->tm[k], a->ckpt_values, a->T * pitch, pitch, 1, CU_TENSOR_MAP_DATA_TYPE_UINT8,
+                                       nin * a->nb, a->T, pitch, g->L, "ckpt_values")
+                              : stream(k, a->in[k], names[k]);
+        if (rc) return rc;
     }
     if (bwd)
-        if (int rc = encode(&P->tm[nin], a->gout.ptr, a->gout.stride_b, a->gout.stride_t, es, map_type(a->dtype), a->nb,
-                            a->T, a->C, "gout"))
+        if (int rc = stream(nin, a->gout, names[5])) return rc;
+    for (int k = 0; k < (bwd ? nin : 1); ++k)
+        if (int rc = bwd ? encode(&P->tmo[k], a->grad[k], a->grad_stride_b, a->grad_stride_t, es, ty, a->nb, a->T, a->C,
+                                  g->L, "grad")
+                         : encode(&P->tmo[0], a->out, a->out_stride_b, a->out_stride_t, es, ty, a->nb, a->T, a->C, g->L, "out"))
             return rc;
     P->nb = int32_t(a->nb);
     P->T = int32_t(a->T);
@@ -760,6 +1118,9 @@ int prepare(const need_scan_train_args* a, bool bwd, TrainParams* P, Geom* g) {
     P->ncb = int32_t(g->ncb);
     P->nchains = int32_t(g->nchains);
     P->nchunks = int32_t(g->nchunks);
+    P->nspans = int32_t((a->T + kSpan - 1) / kSpan);
+    // few chains have many of their tiles in flight at once: look further back
+    P->depth = g->nchains < 148 ? kDeep : 3;
     P->dskip = a->d_skip;
     P->dt_min = static_cast<float>(a->dt_min);
     P->dt_scale = static_cast<float>(a->dt_max - a->dt_min);
@@ -769,25 +1130,23 @@ int prepare(const need_scan_train_args* a, bool bwd, TrainParams* P, Geom* g) {
     P->sgb = a->seg_stride_b;
     P->sgt = a->seg_stride_t;
     P->states = a->states;
-    P->out = a->out;
-    P->osb = a->out_stride_b;
-    P->ost = a->out_stride_t;
     P->q = a->ckpt_values;
     P->qs = a->ckpt_scales;
-    for (int k = 0; k < nin; ++k) P->grad[k] = a->grad[k];
     P->g_final = a->g_final;
     P->grad_h0 = a->grad_h0;
     unsigned char* ws = static_cast<unsigned char*>(a->workspace);
     P->hdr = reinterpret_cast<uint32_t*>(ws);
     P->agg = reinterpret_cast<ulonglong2*>(ws + kHdrBytes);
     P->incl = reinterpret_cast<unsigned long long*>(ws + kHdrBytes + size_t(g->ntiles) * kCB * 8);
-    P->dpart = reinterpret_cast<float*>(ws + kHdrBytes + rec_bytes(*g));
+    P->dcount = reinterpret_cast<uint32_t*>(ws + kHdrBytes + rec_bytes(*g));
+    P->dpart = reinterpret_cast<float*>(ws + clear_bytes(*g, dpart));
+    P->grad_d = a->grad_d;
     P->polls = lookback_polls();
     return NEED_OK;
 }
 
-int clear_records(const need_scan_train_args* a, const Geom& g, cudaStream_t s) {
-    const cudaError_t e = cudaMemsetAsync(a->workspace, 0, kHdrBytes + rec_bytes(g), s);
+int clear_records(const need_scan_train_args* a, const Geom& g, bool dpart, cudaStream_t s) {
+    const cudaError_t e = cudaMemsetAsync(a->workspace, 0, clear_bytes(g, dpart), s);
     return e == cudaSuccess ? NEED_OK : cuda_fail(e, "cudaMemsetAsync(training scan records)");
 }
 
@@ -795,21 +1154,22 @@ int clear_records(const need_scan_train_args* a, const Geom& g, cudaStream_t s) 
 
 extern "C" {
 
-int64_t need_scan_train_chunk_len(void) { return kL; }
+int64_t need_scan_train_chunk_len(void) { return kSpan; }
 
 int64_t need_scan_train_group(void) { return kCB; }
 
-size_t need_scan_train_workspace_size(int32_t form, int32_t backward, int64_t nb, int64_t T, int64_t C) {
-    if (nb < 1 || T < 1 || C < 1) return kHdrBytes;
-    return ws_size(geom(nb, T, C), nb, C, backward != 0 && form == NEED_FORM_SSD);
+size_t need_scan_train_workspace_size(int32_t form, int32_t dtype, int32_t checkpoint, int32_t backward, int64_t nb,
+                                      int64_t T, int64_t C) {
+    if (nb < 1 || T < 1 || C < 1 || !dtype_ok(dtype)) return kHdrBytes;
+    return ws_size(geom(dtype, checkpoint != 0, backward != 0, nb, T, C), nb, C, backward != 0 && form == NEED_FORM_SSD);
 }
 
 int need_scan_train_forward(const need_scan_train_args* args, need_stream_t stream) {
     TrainParams P;
     Geom g;
     if (int rc = prepare(args, false, &P, &g)) return rc;
-    if (int rc = clear_records(args, g, stream)) return rc;
-    if (int rc = run<false>(args, P, g.ntiles, stream)) return rc;
+    if (int rc = clear_records(args, g, false, stream)) return rc;
+    if (int rc = run<false>(args, P, stream)) return rc;
     return ok();
 }
 
@@ -817,10 +1177,8 @@ int need_scan_train_backward(const need_scan_train_args* args, need_stream_t str
     TrainParams P;
     Geom g;
     if (int rc = prepare(args, true, &P, &g)) return rc;
-    if (int rc = clear_records(args, g, stream)) return rc;
-    if (int rc = run<true>(args, P, g.ntiles, stream)) return rc;
-    if (args->form == NEED_FORM_SSD)
-        if (int rc = column_sums(P.dpart, args->nb * g.nchunks, args->C, args->grad_d, stream)) return rc;
+    if (int rc = clear_records(args, g, args->form == NEED_FORM_SSD, stream)) return rc;
+    if (int rc = run<true>(args, P, stream)) return rc;
     return ok();
 }
 

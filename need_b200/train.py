@@ -96,16 +96,9 @@ def _scan_train(form, streams, seg_start, h0, checkpoint, return_final_state, d_
             out = (out * d_skip).to(x.dtype)
         final = h0 if h0 is not None else torch.zeros((B, C), device=x.device)
         return (out, final) if return_final_state else out
-    pad = -C % (4 if x.dtype == torch.float32 else 8)
-    if pad:
-        streams = [F.pad(s, (0, pad)) for s in streams]
-        h0 = None if h0 is None else F.pad(h0, (0, pad))
-        d_skip = None if d_skip is None else F.pad(d_skip, (0, pad))
     if form == abi.FORM_GATED:
         streams = (*streams, None, None)
     out, final = _ext().scan_train(form, ckpt, dt_min, dt_max, seg, h0, d_skip, *streams)
-    if pad:
-        out, final = out[..., :C], final[:, :C]
     return (out, final) if return_final_state else out
 
 
@@ -143,8 +136,8 @@ def ssd_scan_train(u: torch.Tensor, b_gate: torch.Tensor, c_gate: torch.Tensor, 
 
     Differentiable in the five streams, ``d_skip`` and ``h0``, through ``y`` and the
     final state.  ``seg_start`` as for :func:`gated_scan_train`; ``checkpoint``: see
-    the module.  The streams may be chunks of one in-projection (no copy is made
-    of views whose rows are 16-byte aligned).
+    the module.  The streams may be chunks of one in-projection: no copy is made of
+    views with channel stride 1.
     """
     streams = (u, b_gate, c_gate, dt_raw, out_gate)
     _check("ssd_scan_train", *streams, d_skip, seg_start, h0)
@@ -156,7 +149,7 @@ def ssd_scan_train(u: torch.Tensor, b_gate: torch.Tensor, c_gate: torch.Tensor, 
         raise ValueError(f"0 <= dt_min <= dt_max expected; got {dt_min}, {dt_max}")
     order = [s.to(u.dtype) for s in (dt_raw, b_gate, u, c_gate, out_gate)]
     return _scan_train(abi.FORM_SSD, order, seg_start, h0, checkpoint, return_final_state,
-                       d_skip.reshape(-1).float(), float(dt_min), float(dt_max))
+                       (d_skip if d_skip.dim() == 1 else d_skip.reshape(-1)).float(), float(dt_min), float(dt_max))
 
 
 # --------------------------------------------------------------------------

@@ -44,10 +44,12 @@ def test_sizes(lib):
     assert lib.need_scan_train_chunk_len() == ref.SPAN
     assert lib.need_scan_train_group() == ref.GROUP
     ws = lib.need_scan_train_workspace_size
-    assert ws(abi.FORM_GATED, 0, 2, 64, 64) == 128                      # one chunk: no records
-    assert ws(abi.FORM_GATED, 1, 2, 65, 65) == 128 + 2 * 2 * 2 * 64 * 12
-    assert ws(abi.FORM_SSD, 1, 2, 65, 65) == 128 + 2 * 2 * 2 * 64 * 12 + 2 * 2 * 65 * 4
-    assert ws(abi.FORM_SSD, 1, 0, 65, 65) == 128
+    assert ws(abi.FORM_GATED, abi.BF16, 0, 0, 2, 128, 64) == 128        # one tile: no records
+    assert ws(abi.FORM_GATED, abi.BF16, 0, 1, 2, 129, 65) == 128 + 2 * 2 * 2 * 64 * 12
+    assert ws(abi.FORM_SSD, abi.BF16, 0, 1, 2, 129, 65) == 128 + 2 * 2 * 2 * 64 * 12 + 16 + 2 * 2 * 65 * 4
+    for dtype, ckpt in ((abi.F32, 0), (abi.BF16, 1)):                   # 64-token tiles
+        assert ws(abi.FORM_SSD, dtype, ckpt, 1, 2, 65, 65) == 128 + 2 * 2 * 2 * 64 * 12 + 16 + 2 * 2 * 65 * 4
+    assert ws(abi.FORM_SSD, abi.BF16, 0, 1, 0, 65, 65) == 128
     assert lib.need_conv_silu_train_workspace_size(3, 2, 129, 8) == 2 * 2 * 8 * 4 * 4
     assert lib.need_rms_norm_train_workspace_size(3, 8) == 3 * 8 * 4
 
@@ -65,6 +67,7 @@ def scan_args(form=abi.FORM_SSD, **kw):
     a.gout = abi.NeedView(P, 6400, 0, 64)
     a.d_skip = a.states = a.out = a.workspace = a.grad_d = P
     a.out_stride_b, a.out_stride_t, a.workspace_bytes = 6400, 64, 1 << 30
+    a.grad_stride_b, a.grad_stride_t = 6400, 64
     for k, v in kw.items():
         setattr(a, k, v)
     return a
@@ -74,7 +77,7 @@ def scan_args(form=abi.FORM_SSD, **kw):
 @pytest.mark.parametrize("change,code", [
     ({"form": abi.FORM_AFFINE}, abi.ERR_INVALID), ({"dtype": 7}, abi.ERR_UNSUPPORTED),
     ({"checkpoint": 2}, abi.ERR_INVALID), ({"T": 0}, abi.ERR_INVALID), ({"nb": -1}, abi.ERR_INVALID),
-    ({"C": 60}, abi.ERR_UNSUPPORTED), ({"C": 1 << 32}, abi.ERR_UNSUPPORTED),
+    ({"C": 1 << 32}, abi.ERR_UNSUPPORTED),
     ({"nb": 1 << 27, "T": 1 << 29}, abi.ERR_UNSUPPORTED),
     ({"states": None}, abi.ERR_INVALID), ({"d_skip": None}, abi.ERR_INVALID),
     ({"dt_min": -0.1}, abi.ERR_INVALID), ({"dt_max": 0.0}, abi.ERR_INVALID),
@@ -93,11 +96,19 @@ def test_scan_refuses_outputs(lib):
     assert fwd(None, None) == bwd(None, None) == abi.ERR_INVALID
     assert fwd(ctypes.byref(scan_args(out=None)), None) == abi.ERR_INVALID
     assert fwd(ctypes.byref(scan_args(out=P + 2)), None) == abi.ERR_INVALID
-    assert fwd(ctypes.byref(scan_args(out_stride_t=60)), None) == abi.ERR_UNSUPPORTED
-    assert fwd(ctypes.byref(scan_args(out_stride_b=0)), None) == abi.ERR_UNSUPPORTED
+    for bad in (60, 56, 63):  # not 16 bytes apart, or shorter than C
+        assert fwd(ctypes.byref(scan_args(out_stride_t=bad)), None) == abi.ERR_INVALID
+        assert bwd(ctypes.byref(scan_args(grad_stride_t=bad)), None) == abi.ERR_INVALID
+    assert fwd(ctypes.byref(scan_args(out_stride_b=0)), None) == abi.ERR_INVALID
     assert bwd(ctypes.byref(scan_args(grad_d=None)), None) == abi.ERR_INVALID
     a = scan_args()
     a.grad[3] = None
+    assert bwd(ctypes.byref(a), None) == abi.ERR_INVALID
+    a = scan_args()
+    a.in_[2].ptr = None
+    assert fwd(ctypes.byref(a), None) == bwd(ctypes.byref(a), None) == abi.ERR_INVALID
+    a = scan_args()
+    a.gout.ptr = None
     assert bwd(ctypes.byref(a), None) == abi.ERR_INVALID
 
 

@@ -106,7 +106,11 @@ def close(got, want, dtype, reach, what=""):
     products of the two by both.  Differences (h - w) and slopes (s (1 - s) <= 1/4)
     put the operands at up to 4 times the largest result.  Sums over all tokens
     are trees whose steps round by 2^-24, less than this.
-    In the 2-norm the steps' errors have independent signs: sqrt(reach) for reach."""
+    In the 2-norm the steps' errors have independent signs: sqrt(reach) for reach.
+    Kept sigmoids: a bf16 gradient of the scans is a product of at most four that the
+    kernel holds in f16 from its first pass to its second, 2^-12 off each (of the
+    value, and in the difference h - w of the larger operand): 4 * 2^-12, half of
+    bf16's own half step."""
     d = 2.0 ** -22 if dtype == torch.float32 else 2.0 ** -21
     eps = torch.finfo(got.dtype).eps
     reach = max(reach, 4)
@@ -117,10 +121,11 @@ def close(got, want, dtype, reach, what=""):
     err = (got.detach().cpu().to(torch.float64) - w).abs()
     top = float(w.abs().max())
     tiny = float(torch.finfo(got.dtype).smallest_normal) * eps  # a step of the subnormals
-    bound = 1.125 * eps / 2 * w.abs() + 2 * 4 * reach * d * top + tiny
+    kept = 4 * 2.0 ** -12 if got.dtype == torch.bfloat16 else 0.0
+    bound = 1.125 * (eps / 2 + kept) * w.abs() + (2 * 4 * reach * d + kept) * top + tiny
     assert bool((err <= bound).all()), (f"{what}: {int((~(err <= bound)).sum())} of {err.numel()} beyond; worst "
                                         f"{float((err / bound).max()):.2f} of the bound, error {float(err.max()):.3e}, "
                                         f"largest {top:.3e}")
     norm = float(torch.linalg.norm(w))
-    assert float(torch.linalg.norm(err)) <= (eps / 2 + 2 * 4 * reach ** 0.5 * d) * norm + tiny * w.numel() ** 0.5, (
+    assert float(torch.linalg.norm(err)) <= (eps / 2 + kept + 2 * 4 * reach ** 0.5 * d) * norm + tiny * w.numel() ** 0.5, (
         f"{what}: 2-norm off by {float(torch.linalg.norm(err)) / norm:.3e}")
