@@ -272,17 +272,18 @@ typedef struct {
 typedef struct {
     int32_t dtype;          /* u, out, gout and grad_u */
     int32_t K;              /* taps, 1..4 */
-    int64_t nb, T, C;       /* C a multiple of 4 */
-    const void* u;          /* [nb, T, C], channel stride 1, rows aligned to 4 elements */
+    int64_t nb, T, C;
+    const void* u;          /* [nb, T, C], channel stride 1 (rows aligned to 4 elements are read fastest) */
     int64_t u_stride_b, u_stride_t;
     const float* weight;    /* [C, K] contiguous fp32 taps, oldest first */
     const float* bias;      /* optional [C] fp32 */
     const uint8_t* seg_start; /* optional reset mask [nb, T] */
     int64_t seg_stride_b, seg_stride_t;
-    void* out;              /* forward: [nb, T, C] contiguous */
+    void* out;              /* forward: [nb, T, C], channel stride 1 */
     const void* gout;       /* backward: [nb, T, C], as u */
     int64_t gout_stride_b, gout_stride_t;
-    void* grad_u;           /* backward: [nb, T, C] contiguous */
+    void* grad_u;           /* backward: [nb, T, C], channel stride 1 */
+    int64_t out_stride_b, out_stride_t; /* of out (forward) or grad_u (backward) */
     float* grad_wb;         /* backward: [C, K + 1] fp32: the taps' gradients, then the bias's */
     void* workspace;        /* backward: >= need_conv_silu_train_workspace_size(...) bytes */
     size_t workspace_bytes;
@@ -292,20 +293,20 @@ typedef struct {
 typedef struct {
     int32_t dtype;          /* x, out, gout and grad_x */
     int32_t checkpoint;     /* 0: the backward reads x; 1: it reads the 8-bit copy */
-    int64_t rows, C;        /* C a multiple of 16 bytes' worth of elements, rows of at most 32 KB */
-    int64_t C_mean;         /* channels the mean is taken over (<= C; those past it hold zeros) */
-    const void* x;          /* [rows, C], channel stride 1, 16-byte aligned rows; backward: unused
-                               with checkpoint */
+    int64_t rows, C;        /* rows of at most 32 KB */
+    const void* x;          /* [rows, C], channel stride 1 (16-byte aligned rows are read fastest);
+                               backward: unused with checkpoint */
     int64_t x_stride;
-    const float* weight;    /* [C] fp32, 16-byte aligned */
+    const float* weight;    /* [C] fp32 */
     double eps;
-    void* out;              /* forward: [rows, C] contiguous */
+    void* out;              /* forward: [rows, C], channel stride 1 */
     float* rstd;            /* [rows] fp32: written by the forward, read by the backward */
-    uint8_t* ckpt_values;   /* checkpoint: [rows, C] e4m3, 8-byte aligned */
+    uint8_t* ckpt_values;   /* checkpoint: [rows, ceil(C / 64) * 64] e4m3, 8-byte aligned */
     uint8_t* ckpt_scales;   /* checkpoint: [rows, ceil(C / 64)] */
-    const void* gout;       /* backward: [rows, C] */
+    const void* gout;       /* backward: [rows, C], as x */
     int64_t gout_stride;
-    void* grad_x;           /* backward: [rows, C] contiguous */
+    void* grad_x;           /* backward: [rows, C], channel stride 1 */
+    int64_t out_stride;     /* of out (forward) or grad_x (backward) */
     float* grad_weight;     /* backward: [C] fp32 */
     void* workspace;        /* backward: >= need_rms_norm_train_workspace_size(...) bytes */
     size_t workspace_bytes;
@@ -530,13 +531,13 @@ NEED_API int need_conv_silu_train_backward(const need_conv_train_args* args, nee
 /* Workspace bytes of need_rms_norm_train_backward. */
 NEED_API size_t need_rms_norm_train_workspace_size(int64_t rows, int64_t C);
 
-/* out = x * rstd * weight, rstd = 1 / sqrt(sum(x^2) / C_mean + eps), per row in
+/* out = x * rstd * weight, rstd = 1 / sqrt(sum(x^2) / C + eps), per row in
  * fp32, rounded once (need_kernels.py:99-107); optionally keeps x in 8 bits as
  * need_scan_train_forward does. */
 NEED_API int need_rms_norm_train_forward(const need_norm_train_args* args, need_stream_t stream);
 
 /* Its gradient: with n = x rstd and g = weight gout,
- * grad_x = rstd (g - n sum(g n) / C_mean), grad_weight = sum over rows of gout n.
+ * grad_x = rstd (g - n sum(g n) / C), grad_weight = sum over rows of gout n.
  * With checkpoint, x is the stored 8-bit values and rstd the true row's. */
 NEED_API int need_rms_norm_train_backward(const need_norm_train_args* args, need_stream_t stream);
 

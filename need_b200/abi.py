@@ -134,16 +134,16 @@ class NeedConvTrainArgs(Structure):
         ("weight", c_void_p), ("bias", c_void_p),
         ("seg_start", c_void_p), ("seg_stride_b", c_int64), ("seg_stride_t", c_int64),
         ("out", c_void_p), ("gout", c_void_p), ("gout_stride_b", c_int64), ("gout_stride_t", c_int64),
-        ("grad_u", c_void_p), ("grad_wb", c_void_p), ("workspace", c_void_p), ("workspace_bytes", c_size_t),
+        ("grad_u", c_void_p), ("out_stride_b", c_int64), ("out_stride_t", c_int64), ("grad_wb", c_void_p), ("workspace", c_void_p), ("workspace_bytes", c_size_t),
     ]
 
 
 class NeedNormTrainArgs(Structure):
     _fields_ = [
-        ("dtype", c_int32), ("checkpoint", c_int32), ("rows", c_int64), ("C", c_int64), ("C_mean", c_int64),
+        ("dtype", c_int32), ("checkpoint", c_int32), ("rows", c_int64), ("C", c_int64),
         ("x", c_void_p), ("x_stride", c_int64), ("weight", c_void_p), ("eps", c_double),
         ("out", c_void_p), ("rstd", c_void_p), ("ckpt_values", c_void_p), ("ckpt_scales", c_void_p),
-        ("gout", c_void_p), ("gout_stride", c_int64), ("grad_x", c_void_p), ("grad_weight", c_void_p),
+        ("gout", c_void_p), ("gout_stride", c_int64), ("grad_x", c_void_p), ("out_stride", c_int64), ("grad_weight", c_void_p),
         ("workspace", c_void_p), ("workspace_bytes", c_size_t),
     ]
 

@@ -53,15 +53,6 @@ Tensor rows_like(const at::TensorOptions& opts, int64_t B, int64_t T, int64_t C)
     return pitch == C ? at::empty({B, T, C}, opts) : at::empty_strided({B, T, C}, {T * pitch, pitch, 1}, opts);
 }
 
-// `t` with channel stride 1, a 16-byte aligned base and positive row strides of
-// whole 16 bytes (dims of size 1 excepted); a copy if it is laid out otherwise.
-Tensor rows(const Tensor& t) {
-    const int64_t es = t.element_size(), d = t.dim();
-    bool ok = reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0 && (t.stride(d - 1) == 1 || t.size(d - 1) == 1);
-    for (int64_t i = 0; i + 1 < d; ++i) ok = ok && (t.size(i) == 1 || (t.stride(i) > 0 && t.stride(i) * es % 16 == 0));
-    return ok ? t : t.clone(at::MemoryFormat::Contiguous);
-}
-
 Tensor scratch(const Tensor& like, size_t bytes) {
     return at::empty({static_cast<int64_t>(bytes)}, like.options().dtype(at::kByte));
 }
@@ -221,7 +212,7 @@ std::tuple<Tensor, Tensor> scan_train(int64_t form, bool ckpt, double dt_min, do
 // ------------------------------------------------------------------ the conv
 need_conv_train_args conv_args(const Tensor& u, const Tensor& w, const Tensor& b, const Tensor& seg) {
     need_conv_train_args a{};
-    a.dtype = dtype_of(u), a.K = static_cast<int32_t>(w.size(1));
+    a.dtype = dtype_of(u), a.K = static_cast<int32_t>(w.size(-1));
     a.nb = u.size(0), a.T = u.size(1), a.C = u.size(2);
     a.u = u.const_data_ptr(), a.u_stride_b = u.stride(0), a.u_stride_t = u.stride(1);
     a.weight = ptr<float>(w), a.bias = ptr<float>(b);
@@ -232,12 +223,13 @@ need_conv_train_args conv_args(const Tensor& u, const Tensor& w, const Tensor& b
 struct ConvTrain : torch::autograd::Function<ConvTrain> {
     static Tensor forward(AutogradContext* ctx, const Tensor& u_, const Tensor& w_, const OptTensor& b_,
                           const OptTensor& seg_) {
-        const Tensor u = rows(u_), w = w_.contiguous(), seg = or_none(seg_);
+        // the weight [C, K] or [C, 1, K], as it is
+        const Tensor u = channels(u_), w = w_.contiguous(), seg = or_none(seg_);
         const Tensor b = b_.has_value() ? b_->contiguous() : Tensor();
         On on(u);
-        Tensor out = at::empty(u.sizes(), u.options());
+        Tensor out = rows_like(u.options(), u.size(0), u.size(1), u.size(2));
         need_conv_train_args a = conv_args(u, w, b, seg);
-        a.out = out.data_ptr();
+        a.out = out.data_ptr(), a.out_stride_b = out.stride(0), a.out_stride_t = out.stride(1);
         check("need_conv_silu_train_forward", need_conv_silu_train_forward(&a, on.stream));
         ctx->save_for_backward({u, w, b, seg});
         return out;
@@ -246,15 +238,17 @@ struct ConvTrain : torch::autograd::Function<ConvTrain> {
         variable_list s = ctx->get_saved_variables();
         const Tensor &u = s[0], &w = s[1], &b = s[2], &seg = s[3];
         On on(u);
-        const Tensor gout = rows(go[0]);
+        const Tensor gout = channels(go[0]);
         need_conv_train_args a = conv_args(u, w, b, seg);
         a.gout = gout.const_data_ptr(), a.gout_stride_b = gout.stride(0), a.gout_stride_t = gout.stride(1);
-        Tensor gu = at::empty(u.sizes(), u.options()), gwb = floats(u, {a.C, a.K + 1});
+        Tensor gu = rows_like(u.options(), a.nb, a.T, a.C), gwb = floats(u, {a.C, a.K + 1});
         const Tensor ws = scratch(u, need_conv_silu_train_workspace_size(a.K, a.nb, a.T, a.C));
-        a.grad_u = gu.data_ptr(), a.grad_wb = ptr<float>(gwb);
+        a.grad_u = gu.data_ptr(), a.out_stride_b = gu.stride(0), a.out_stride_t = gu.stride(1);
+        a.grad_wb = ptr<float>(gwb);
         a.workspace = ws.data_ptr(), a.workspace_bytes = ws.numel();
         check("need_conv_silu_train_backward", need_conv_silu_train_backward(&a, on.stream));
-        return once({gu, gwb.narrow(1, 0, a.K), b.defined() ? gwb.select(1, a.K) : Tensor(), Tensor()});
+        const Tensor gw = w.dim() == 3 ? gwb.unsqueeze(1).narrow(2, 0, a.K) : gwb.narrow(1, 0, a.K);
+        return once({gu, gw, b.defined() ? gwb.select(1, a.K) : Tensor(), Tensor()});
     }
 };
 
@@ -263,58 +257,69 @@ Tensor conv_train(const Tensor& u, const Tensor& w, const OptTensor& b, const Op
 }
 
 // ------------------------------------------------------------------ the norm
-need_norm_train_args norm_args(int32_t dtype, int64_t n, int64_t C, int64_t c_mean, const Tensor& w, const Tensor& rstd,
-                               double eps, bool ckpt) {
+need_norm_train_args norm_args(int32_t dtype, int64_t n, int64_t C, const Tensor& w, const Tensor& rstd, double eps,
+                               bool ckpt) {
     need_norm_train_args a{};
-    a.dtype = dtype, a.checkpoint = ckpt ? 1 : 0, a.rows = n, a.C = C, a.C_mean = c_mean;
+    a.dtype = dtype, a.checkpoint = ckpt ? 1 : 0, a.rows = n, a.C = C;
     a.weight = ptr<float>(w), a.rstd = ptr<float>(rstd), a.eps = eps;
     return a;
 }
+// The distance of t's rows (all dims but the last, as one) where they are evenly
+// apart with channel stride 1; else 0.
+int64_t row_stride(const Tensor& t) {
+    if (t.stride(-1) != 1 && t.size(-1) > 1) return 0;
+    int64_t step = 0, next = 0;  // of the innermost dim of more than one, and what the next must be
+    for (int64_t d = t.dim() - 2; d >= 0; --d) {
+        if (t.size(d) == 1) continue;
+        if (step == 0) step = t.stride(d);
+        else if (t.stride(d) != next) return 0;
+        if (step <= 0) return 0;
+        next = t.stride(d) * t.size(d);
+    }
+    return step == 0 ? t.size(-1) : step;
+}
+Tensor even_rows(const Tensor& t) { return row_stride(t) != 0 ? t : t.clone(at::MemoryFormat::Contiguous); }
 
 struct NormTrain : torch::autograd::Function<NormTrain> {
-    static Tensor forward(AutogradContext* ctx, const Tensor& x_, const Tensor& w_, double eps, bool ckpt, int64_t c_mean) {
-        const Tensor x = rows(x_);
-        const Tensor w = w_.is_contiguous() && reinterpret_cast<uintptr_t>(w_.const_data_ptr()) % 16 == 0
-                             ? w_
-                             : w_.clone(at::MemoryFormat::Contiguous);
-        const int64_t n = x.size(0), C = x.size(1);
+    static Tensor forward(AutogradContext* ctx, const Tensor& x_, const Tensor& w_, double eps, bool ckpt) {
+        const Tensor x = even_rows(x_), w = w_.contiguous();
+        const int64_t C = x.size(-1), n = x.numel() / C;
         On on(x);
-        Tensor out = at::empty({n, C}, x.options()), rstd = floats(x, {n}), q, qs;
-        need_norm_train_args a = norm_args(dtype_of(x), n, C, c_mean, w, rstd, eps, ckpt);
-        a.x = x.const_data_ptr(), a.x_stride = x.stride(0), a.out = out.data_ptr();
+        Tensor out = at::empty(x.sizes(), x.options()), rstd = floats(x, {n}), q, qs;
+        need_norm_train_args a = norm_args(dtype_of(x), n, C, w, rstd, eps, ckpt);
+        a.x = x.const_data_ptr(), a.x_stride = row_stride(x), a.out = out.data_ptr(), a.out_stride = C;
         if (ckpt) {
-            q = scratch(x, n * C), qs = scratch(x, n * ((C + kGroup - 1) / kGroup));
+            const int64_t groups = (C + kGroup - 1) / kGroup;
+            q = scratch(x, n * groups * kGroup), qs = scratch(x, n * groups);
             a.ckpt_values = ptr<uint8_t>(q), a.ckpt_scales = ptr<uint8_t>(qs);
         }
         check("need_rms_norm_train_forward", need_rms_norm_train_forward(&a, on.stream));
         if (ckpt) ctx->save_for_backward({w, rstd, q, qs});
         else ctx->save_for_backward({w, rstd, x});
-        auto& d = ctx->saved_data;
-        d["n"] = n, d["C"] = C, d["mean"] = c_mean, d["eps"] = eps, d["ckpt"] = ckpt;
+        ctx->saved_data["eps"] = eps;
         return out;
     }
     static variable_list backward(AutogradContext* ctx, variable_list go) {
-        auto& d = ctx->saved_data;
-        const bool ckpt = d["ckpt"].toBool();
-        const int64_t n = d["n"].toInt(), C = d["C"].toInt();
         variable_list s = ctx->get_saved_variables();
+        const bool ckpt = s.size() == 4;
         On on(s[0]);
-        const Tensor gout = rows(go[0]);
-        need_norm_train_args a = norm_args(dtype_of(gout), n, C, d["mean"].toInt(), s[0], s[1], d["eps"].toDouble(), ckpt);
+        const Tensor gout = even_rows(go[0]);
+        const int64_t C = gout.size(-1), n = s[1].numel();
+        need_norm_train_args a = norm_args(dtype_of(gout), n, C, s[0], s[1], ctx->saved_data["eps"].toDouble(), ckpt);
         if (ckpt) a.ckpt_values = ptr<uint8_t>(s[2]), a.ckpt_scales = ptr<uint8_t>(s[3]);
-        else a.x = s[2].const_data_ptr(), a.x_stride = s[2].stride(0);
-        a.gout = gout.const_data_ptr(), a.gout_stride = gout.stride(0);
-        Tensor gx = at::empty({n, C}, gout.options()), gw = floats(gout, {C});
+        else a.x = s[2].const_data_ptr(), a.x_stride = row_stride(s[2]);
+        a.gout = gout.const_data_ptr(), a.gout_stride = row_stride(gout);
+        Tensor gx = at::empty(gout.sizes(), gout.options()), gw = floats(gout, s[0].sizes());
         const Tensor ws = scratch(gout, need_rms_norm_train_workspace_size(n, C));
-        a.grad_x = gx.data_ptr(), a.grad_weight = ptr<float>(gw);
+        a.grad_x = gx.data_ptr(), a.out_stride = C, a.grad_weight = ptr<float>(gw);
         a.workspace = ws.data_ptr(), a.workspace_bytes = ws.numel();
         check("need_rms_norm_train_backward", need_rms_norm_train_backward(&a, on.stream));
-        return once({gx, gw, Tensor(), Tensor(), Tensor()});
+        return once({gx, gw, Tensor(), Tensor()});
     }
 };
 
-Tensor norm_train(const Tensor& x, const Tensor& w, double eps, bool ckpt, int64_t c_mean) {
-    return NormTrain::apply(x, w, eps, ckpt && wants_grad({&x, &w}), c_mean);
+Tensor norm_train(const Tensor& x, const Tensor& w, double eps, bool ckpt) {
+    return NormTrain::apply(x, w, eps, ckpt && wants_grad({&x, &w}));
 }
 
 }  // namespace

@@ -10,11 +10,13 @@
 // the fewest that leave a lane at most 4 16-byte pieces -- and the two sums of
 // the backward are reduced together.  The backward's blocks stride over the
 // rows, so that a lane's channels stay the same and their share of dw stays in
-// its registers; each block ends with one row of partial sums, and
-// column_sums adds those rows in a fixed order.
+// its registers, the next row's loads in flight while one is worked on; each
+// block ends with one row of partial sums, and column_sums adds those rows in a
+// fixed order.
 #include <cuda_fp8.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "host_common.h"
 #include "need_scan.h"
@@ -40,88 +42,100 @@ struct NormTrainParams {
     uint8_t* q;
     uint8_t* qs;
     float* part;  // [gridDim.x, C]
+    int64_t os;
     int64_t rows;
-    int32_t C, ngroups, wpr;  // warps per row
+    int32_t C, ngroups, wpr;     // warps per row
     float inv_c, eps;
 };
 
-// Sums a and b over the warps of a row (all of them call it).
-__device__ __forceinline__ void row_sums(float& a, float& b, int wpr, float2* s_red) {
+// Sums a over the warps of a row (all of them call it).
+__device__ __forceinline__ float row_sum(float a, int wpr, float* s_red) {
 #pragma unroll
-    for (int m = 16; m >= 1; m >>= 1) {
-        a += __shfl_xor_sync(0xffffffffu, a, m);
-        b += __shfl_xor_sync(0xffffffffu, b, m);
-    }
+    for (int m = 16; m >= 1; m >>= 1) a += __shfl_xor_sync(0xffffffffu, a, m);
     if (wpr > 1) {
         const int warp = threadIdx.x >> 5;
         __syncthreads();  // the previous row's sums have been read
-        if ((threadIdx.x & 31) == 0) s_red[warp] = make_float2(a, b);
+        if ((threadIdx.x & 31) == 0) s_red[warp] = a;
         __syncthreads();
         const int w0 = warp / wpr * wpr;
-        a = b = 0.0f;
-        for (int w = 0; w < wpr; ++w) {
-            a += s_red[w0 + w].x;
-            b += s_red[w0 + w].y;
-        }
+        a = 0.0f;
+        for (int w = 0; w < wpr; ++w) a += s_red[w0 + w];
     }
+    return a;
 }
 
-template <typename T>
-struct Piece {  // a 16-byte piece of a row
+// A 16-byte piece of a row, as loaded.  VEC: rows are 16-byte aligned and C whole
+// pieces; else element by element, n of the piece's N elements inside C.
+template <typename T, bool VEC>
+struct Piece {
+    using P = typename Ops<T>::P;
     static constexpr int N = 16 / Ops<T>::BYTES;
-    static __device__ __forceinline__ void load(const T* p, float2 (&f)[N / 2]) {
-        const uint4 u = *reinterpret_cast<const uint4*>(p);
-        const typename Ops<T>::P* h = reinterpret_cast<const typename Ops<T>::P*>(&u);
+    static __device__ __forceinline__ uint4 load(const T* p, int n) {
+        if constexpr (VEC) {
+            return *reinterpret_cast<const uint4*>(p);
+        } else {
+            uint4 u;
+            P* h = reinterpret_cast<P*>(&u);
 #pragma unroll
-        for (int e = 0; e < N / 2; ++e) f[e] = widen(h[e]);
-    }
-    static __device__ __forceinline__ void store(T* p, const float2 (&f)[N / 2]) {
-        uint4 u;
-        typename Ops<T>::P* h = reinterpret_cast<typename Ops<T>::P*>(&u);
-#pragma unroll
-        for (int e = 0; e < N / 2; ++e) h[e] = Ops<T>::pack(f[e].x, f[e].y);
-        *reinterpret_cast<uint4*>(p) = u;
-    }
-    static __device__ __forceinline__ void load_w(const float* w, float2 (&f)[N / 2]) {
-#pragma unroll
-        for (int e = 0; e < N / 4; ++e) {
-            const float4 v = __ldg(reinterpret_cast<const float4*>(w) + e);
-            f[2 * e] = make_float2(v.x, v.y);
-            f[2 * e + 1] = make_float2(v.z, v.w);
+            for (int e = 0; e < N / 2; ++e)
+                h[e] = Ops<T>::pack(2 * e < n ? to_f(p[2 * e]) : 0.0f, 2 * e + 1 < n ? to_f(p[2 * e + 1]) : 0.0f);
+            return u;
         }
     }
+    static __device__ __forceinline__ void store(T* p, int n, const uint4& u) {
+        if constexpr (VEC) {
+            *reinterpret_cast<uint4*>(p) = u;
+        } else {
+            const T* q = reinterpret_cast<const T*>(&u);
+            for (int e = 0; e < N && e < n; ++e) p[e] = q[e];
+        }
+    }
+    static __device__ __forceinline__ float2 weight(const float* w, int e, int n) {  // of elements 2 e, 2 e + 1
+        if constexpr (VEC) return __ldg(reinterpret_cast<const float2*>(w) + e);
+        else return make_float2(2 * e < n ? w[2 * e] : 0.0f, 2 * e + 1 < n ? w[2 * e + 1] : 0.0f);
+    }
 };
+template <typename T>
+__device__ __forceinline__ float2 pair_of(const uint4& u, int e) {
+    return widen(reinterpret_cast<const typename Ops<T>::P*>(&u)[e]);
+}
+template <typename T>
+__device__ __forceinline__ void set_pair(uint4& u, int e, float2 f) {
+    reinterpret_cast<typename Ops<T>::P*>(&u)[e] = Ops<T>::pack(f.x, f.y);
+}
 
 // blockDim = 32 * wpr * (rows per block); a row is handled by wpr warps, lane l
 // of its warp w holding pieces (w * 32 + l) + k * 32 * wpr.
-template <typename T, bool CK, int NP>
+template <typename T, bool CK, int NP, bool VEC>
 __global__ void __launch_bounds__(512) norm_train_fwd(const NormTrainParams p) {
-    using Pc = Piece<T>;
+    using Pc = Piece<T, VEC>;
     constexpr int N = Pc::N;
-    __shared__ float2 s_red[kMaxWarps];
+    __shared__ float s_red[kMaxWarps];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rpb = (blockDim.x >> 5) / p.wpr;
     const int64_t row = int64_t(blockIdx.x) * rpb + warp / p.wpr;
     const bool live = row < p.rows;
-    const int l0 = (warp % p.wpr) * 32 + lane, step = 32 * p.wpr, nvec = p.C / N;
+    const int l0 = (warp % p.wpr) * 32 + lane, step = 32 * p.wpr, nvec = (p.C + N - 1) / N;
     const T* x = static_cast<const T*>(p.x) + (live ? row : 0) * p.xs;
-    float2 f[NP][N / 2];
-    float ss = 0.0f, none = 0.0f;
+    uint4 u[NP];
 #pragma unroll
     for (int k = 0; k < NP; ++k) {
         const int v = l0 + k * step;
-#pragma unroll
-        for (int e = 0; e < N / 2; ++e) f[k][e] = splat2(0.0f);
-        if (live && v < nvec) Pc::load(x + v * N, f[k]);
+        u[k] = make_uint4(0, 0, 0, 0);
+        if (live && v < nvec) u[k] = Pc::load(x + v * N, p.C - v * N);
     }
+    float ss = 0.0f;
 #pragma unroll
     for (int k = 0; k < NP; ++k)
 #pragma unroll
-        for (int e = 0; e < N / 2; ++e) ss = fmaf(f[k][e].x, f[k][e].x, fmaf(f[k][e].y, f[k][e].y, ss));
-    row_sums(ss, none, p.wpr, s_red);
+        for (int e = 0; e < N / 2; ++e) {
+            const float2 f = pair_of<T>(u[k], e);
+            ss = fmaf(f.x, f.x, fmaf(f.y, f.y, ss));
+        }
+    ss = row_sum(ss, p.wpr, s_red);
     const float r = 1.0f / sqrtf(fmaf(ss, p.inv_c, p.eps));
     if (live && l0 == 0) p.rstd[row] = r;
-    T* out = static_cast<T*>(p.out) + row * p.C;
+    T* out = static_cast<T*>(p.out) + row * p.os;
 #pragma unroll
     for (int k = 0; k < NP; ++k) {
         const int v = l0 + k * step;
@@ -130,109 +144,126 @@ __global__ void __launch_bounds__(512) norm_train_fwd(const NormTrainParams p) {
             // 64 channels lie in 64 / N neighbouring lanes
             uint32_t top = 0;
 #pragma unroll
-            for (int e = 0; e < N / 2; ++e)
-                top = max(top, max(__float_as_uint(f[k][e].x) & 0x7fffffffu, __float_as_uint(f[k][e].y) & 0x7fffffffu));
+            for (int e = 0; e < N / 2; ++e) {
+                const float2 f = pair_of<T>(u[k], e);
+                top = max(top, max(__float_as_uint(f.x) & 0x7fffffffu, __float_as_uint(f.y) & 0x7fffffffu));
+            }
 #pragma unroll
             for (int m = kGroup / N / 2; m >= 1; m >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, m));
             if (in) {
                 const uint32_t sc = e4m3_scale_byte(top);
-                uint16_t q[N / 2];
+                uint32_t q[N / 4];
 #pragma unroll
-                for (int e = 0; e < N / 2; ++e) q[e] = e4m3_pair(f[k][e], sc);
-                uint8_t* dst = p.q + row * p.C + int64_t(v) * N;
-                if constexpr (N == 8)
-                    *reinterpret_cast<uint2*>(dst) = make_uint2(q[0] | uint32_t(q[1]) << 16, q[2] | uint32_t(q[3]) << 16);
-                else
-                    *reinterpret_cast<uint32_t*>(dst) = q[0] | uint32_t(q[1]) << 16;
+                for (int e = 0; e < N / 4; ++e)
+                    q[e] = e4m3_pair(pair_of<T>(u[k], 2 * e), sc) | uint32_t(e4m3_pair(pair_of<T>(u[k], 2 * e + 1), sc)) << 16;
+                uint8_t* dst = p.q + row * p.ngroups * kGroup + v * N;
+                if constexpr (N == 8) *reinterpret_cast<uint2*>(dst) = make_uint2(q[0], q[1]);
+                else *reinterpret_cast<uint32_t*>(dst) = q[0];
                 if (v % (kGroup / N) == 0) p.qs[row * p.ngroups + v * N / kGroup] = static_cast<uint8_t>(sc);
             }
         }
         if (in) {
-            float2 w[N / 2], o[N / 2];
-            Pc::load_w(p.w + v * N, w);
+            uint4 o;
 #pragma unroll
-            for (int e = 0; e < N / 2; ++e) o[e] = fmul2(fmul2(f[k][e], splat2(r)), w[e]);
-            Pc::store(out + v * N, o);
+            for (int e = 0; e < N / 2; ++e)
+                set_pair<T>(o, e, fmul2(fmul2(pair_of<T>(u[k], e), splat2(r)), Pc::weight(p.w + v * N, e, p.C - v * N)));
+            Pc::store(out + v * N, p.C - v * N, o);
         }
     }
 }
 
-template <typename T, bool CK, int NP>
+// A row's pieces on their way: x (or its 8-bit values and scale) and gout.
+template <int NP, bool CK>
+struct RowIn {
+    uint4 g[NP];
+    uint4 x[CK ? 1 : NP];
+    uint2 q[CK ? NP : 1];
+    uint32_t sc[CK ? NP : 1];
+    float r;
+};
+
+template <typename T, bool CK, int NP, bool VEC>
 __global__ void __launch_bounds__(512) norm_train_bwd(const NormTrainParams p) {
-    using Pc = Piece<T>;
+    using Pc = Piece<T, VEC>;
     constexpr int N = Pc::N;
-    __shared__ float2 s_red[kMaxWarps];
-    extern __shared__ float s_dw[];  // [C]
+    __shared__ float s_red[kMaxWarps];
+    extern __shared__ __align__(16) float s_dw[];  // [C rounded up to a piece]
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rpb = (blockDim.x >> 5) / p.wpr, sub = warp / p.wpr;
-    const int l0 = (warp % p.wpr) * 32 + lane, step = 32 * p.wpr, nvec = p.C / N;
+    const int l0 = (warp % p.wpr) * 32 + lane, step = 32 * p.wpr, nvec = (p.C + N - 1) / N;
     float2 dw[NP][N / 2];
 #pragma unroll
     for (int k = 0; k < NP; ++k)
 #pragma unroll
         for (int e = 0; e < N / 2; ++e) dw[k][e] = splat2(0.0f);
-    for (int64_t base = int64_t(blockIdx.x) * rpb; base < p.rows; base += int64_t(gridDim.x) * rpb) {
-        const int64_t row = base + sub;
+    RowIn<NP, CK> in;
+    auto fetch = [&](int64_t row) {
         const bool live = row < p.rows;
-        const int64_t rr = live ? row : 0;
-        const T* go = static_cast<const T*>(p.gout) + rr * p.gs;
-        float2 x[NP][N / 2], g[NP][N / 2];
+        const T* go = static_cast<const T*>(p.gout) + row * p.gs;
+        in.r = live ? p.rstd[row] : 0.0f;
 #pragma unroll
         for (int k = 0; k < NP; ++k) {
             const int v = l0 + k * step;
-#pragma unroll
-            for (int e = 0; e < N / 2; ++e) x[k][e] = g[k][e] = splat2(0.0f);
+            in.g[k] = make_uint4(0, 0, 0, 0);
+            if constexpr (CK) in.q[k] = make_uint2(0, 0), in.sc[k] = 1;
+            else in.x[k] = make_uint4(0, 0, 0, 0);
             if (live && v < nvec) {
-                Pc::load(go + v * N, g[k]);
+                in.g[k] = Pc::load(go + v * N, p.C - v * N);
                 if constexpr (CK) {
-                    const uint8_t* src = p.q + rr * p.C + int64_t(v) * N;
-                    const float sc = e4m3_scale(p.qs[rr * p.ngroups + v * N / kGroup]);
-                    uint32_t q[2] = {0, 0};
-                    if constexpr (N == 8) {
-                        const uint2 u = *reinterpret_cast<const uint2*>(src);
-                        q[0] = u.x, q[1] = u.y;
-                    } else {
-                        q[0] = *reinterpret_cast<const uint32_t*>(src);
-                    }
-#pragma unroll
-                    for (int e = 0; e < N / 2; ++e) {
-                        const __nv_fp8x2_storage_t h = static_cast<__nv_fp8x2_storage_t>(q[e / 2] >> (16 * (e & 1)));
-                        const float2 f = __half22float2(static_cast<__half2>(__nv_cvt_fp8x2_to_halfraw2(h, __NV_E4M3)));
-                        x[k][e] = make_float2(f.x * sc, f.y * sc);
-                    }
+                    const uint8_t* src = p.q + row * p.ngroups * kGroup + v * N;
+                    in.sc[k] = p.qs[row * p.ngroups + v * N / kGroup];
+                    if constexpr (N == 8) in.q[k] = *reinterpret_cast<const uint2*>(src);
+                    else in.q[k].x = *reinterpret_cast<const uint32_t*>(src);
                 } else {
-                    Pc::load(static_cast<const T*>(p.x) + rr * p.xs + v * N, x[k]);
+                    in.x[k] = Pc::load(static_cast<const T*>(p.x) + row * p.xs + v * N, p.C - v * N);
                 }
             }
         }
-        const float r = live ? p.rstd[rr] : 0.0f;
-        float gn = 0.0f, none = 0.0f;
+    };
+    const int64_t stride = int64_t(gridDim.x) * rpb;
+    fetch(int64_t(blockIdx.x) * rpb + sub);
+    for (int64_t base = int64_t(blockIdx.x) * rpb; base < p.rows; base += stride) {
+        const int64_t row = base + sub;
+        const RowIn<NP, CK> cur = in;
+        if (base + stride < p.rows) fetch(row + stride);  // in flight while this row is worked on
+        auto n_of = [&](int k, int e) {  // n = x rstd of a pair
+            if constexpr (CK) {
+                const uint32_t w = e / 2 == 0 ? cur.q[k].x : cur.q[k].y;
+                const __nv_fp8x2_storage_t h = static_cast<__nv_fp8x2_storage_t>(w >> (16 * (e & 1)));
+                const float2 f = __half22float2(static_cast<__half2>(__nv_cvt_fp8x2_to_halfraw2(h, __NV_E4M3)));
+                return fmul2(fmul2(f, splat2(e4m3_scale(cur.sc[k]))), splat2(cur.r));
+            } else {
+                return fmul2(pair_of<T>(cur.x[k], e), splat2(cur.r));
+            }
+        };
+        float gn = 0.0f;
 #pragma unroll
         for (int k = 0; k < NP; ++k) {
             const int v = l0 + k * step;
-            float2 w[N / 2];
+            if (v < nvec) {
 #pragma unroll
-            for (int e = 0; e < N / 2; ++e) w[e] = splat2(0.0f);
-            if (v < nvec) Pc::load_w(p.w + v * N, w);
-#pragma unroll
-            for (int e = 0; e < N / 2; ++e) {
-                x[k][e] = fmul2(x[k][e], splat2(r));  // n
-                dw[k][e] = ffma2(g[k][e], x[k][e], dw[k][e]);
-                g[k][e] = fmul2(g[k][e], w[e]);
-                gn = fmaf(g[k][e].x, x[k][e].x, fmaf(g[k][e].y, x[k][e].y, gn));
+                for (int e = 0; e < N / 2; ++e) {
+                    const float2 n = n_of(k, e), go = pair_of<T>(cur.g[k], e);
+                    const float2 gw = fmul2(go, Pc::weight(p.w + v * N, e, p.C - v * N));
+                    dw[k][e] = ffma2(go, n, dw[k][e]);
+                    gn = fmaf(gw.x, n.x, fmaf(gw.y, n.y, gn));
+                }
             }
         }
-        row_sums(gn, none, p.wpr, s_red);
-        const float m = -gn * p.inv_c;
-        T* out = static_cast<T*>(p.out) + rr * p.C;
+        gn = row_sum(gn, p.wpr, s_red);
+        const float2 m = splat2(-gn * p.inv_c), r2 = splat2(cur.r);
+        T* out = static_cast<T*>(p.out) + row * p.os;
 #pragma unroll
         for (int k = 0; k < NP; ++k) {
             const int v = l0 + k * step;
-            if (live && v < nvec) {
-                float2 o[N / 2];
+            if (row < p.rows && v < nvec) {
+                uint4 o;
 #pragma unroll
-                for (int e = 0; e < N / 2; ++e) o[e] = fmul2(ffma2(x[k][e], splat2(m), g[k][e]), splat2(r));
-                Pc::store(out + v * N, o);
+                for (int e = 0; e < N / 2; ++e) {
+                    const float2 gw = fmul2(pair_of<T>(cur.g[k], e), Pc::weight(p.w + v * N, e, p.C - v * N));
+                    set_pair<T>(o, e, fmul2(ffma2(n_of(k, e), m, gw), r2));
+                }
+                Pc::store(out + v * N, p.C - v * N, o);
             }
         }
     }
@@ -293,29 +324,32 @@ NormPlan norm_plan(int64_t nvec) {
 }
 // Blocks of the backward: enough to fill the device, few enough that the
 // partial rows they leave are a small part of the traffic.
-constexpr int kBwdBlocks = 148 * 3;
+#ifndef K_NBLK
+#define K_NBLK 2
+#endif
+constexpr int kBwdBlocks = 148 * K_NBLK;
 int64_t bwd_blocks(int64_t rows, const NormPlan& pl) {
     return std::max<int64_t>(1, std::min<int64_t>(kBwdBlocks, (rows + pl.rpb - 1) / pl.rpb));
 }
 
-template <typename T, bool CK>
+template <typename T, bool CK, bool VEC>
 int launch_norm(bool bwd, const NormPlan& pl, const NormTrainParams& p, cudaStream_t s) {
     const int threads = 32 * pl.wpr * pl.rpb;
     const int64_t blocks = bwd ? bwd_blocks(p.rows, pl) : (p.rows + pl.rpb - 1) / pl.rpb;
     if (blocks > INT32_MAX) return fail(NEED_ERR_UNSUPPORTED, "rms norm: too many rows");
     const unsigned grid = static_cast<unsigned>(blocks);
-    const size_t sm = bwd ? size_t(p.C) * 4 : 0;
+    const size_t sm = bwd ? size_t(p.C + 7) / 8 * 8 * 4 : 0;
     auto go = [&](auto np) {
         constexpr int NP = decltype(np)::value;
         if (bwd) {
             if (sm > 48 * 1024) {
                 static std::atomic<uint64_t> done{0};
-                const cudaError_t e = ensure_smem(norm_train_bwd<T, CK, NP>, 64 * 1024, done);
+                const cudaError_t e = ensure_smem(norm_train_bwd<T, CK, NP, VEC>, 64 * 1024, done);
                 if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(norm_train_bwd)");
             }
-            norm_train_bwd<T, CK, NP><<<grid, threads, sm, s>>>(p);
+            norm_train_bwd<T, CK, NP, VEC><<<grid, threads, sm, s>>>(p);
         } else {
-            norm_train_fwd<T, CK, NP><<<grid, threads, 0, s>>>(p);
+            norm_train_fwd<T, CK, NP, VEC><<<grid, threads, 0, s>>>(p);
         }
         const cudaError_t e = cudaGetLastError();
         return e == cudaSuccess ? int(NEED_OK) : cuda_fail(e, "rms norm training launch");
@@ -330,36 +364,41 @@ int norm_train(const need_norm_train_args* a, bool bwd, cudaStream_t s) {
     if (!dtype_ok(a->dtype)) return fail(NEED_ERR_UNSUPPORTED, "rms norm: dtype %d", a->dtype);
     if (a->rows < 1 || a->C < 1) return fail(NEED_ERR_INVALID, "rms norm: sizes must be >= 1");
     const int64_t vec = 16 / dtype_bytes(a->dtype);
-    if (a->C % vec != 0 || a->C / vec > int64_t(kMaxWarps) * 32 * kPieces)
-        return fail(NEED_ERR_UNSUPPORTED, "rms norm: C=%lld must be a multiple of %lld and at most %lld",
-                    (long long)a->C, (long long)vec, (long long)(vec * kMaxWarps * 32 * kPieces));
-    if (a->C_mean < 1 || a->C_mean > a->C) return fail(NEED_ERR_INVALID, "rms norm: C_mean=%lld", (long long)a->C_mean);
+    if (a->C > vec * kMaxWarps * 32 * kPieces)
+        return fail(NEED_ERR_UNSUPPORTED, "rms norm: C=%lld, at most %lld", (long long)a->C,
+                    (long long)(vec * kMaxWarps * 32 * kPieces));
     if (!(a->eps >= 0.0)) return fail(NEED_ERR_INVALID, "rms norm: eps must be >= 0");
     if (a->checkpoint != 0 && a->checkpoint != 1) return fail(NEED_ERR_INVALID, "checkpoint %d", a->checkpoint);
     if (a->checkpoint != 0 && (a->ckpt_values == nullptr || a->ckpt_scales == nullptr ||
                                reinterpret_cast<uintptr_t>(a->ckpt_values) % 8 != 0))
         return fail(NEED_ERR_INVALID, "rms norm: the 8-bit checkpoint is null or not 8-byte aligned");
-    if (a->weight == nullptr || !aligned16(a->weight) || a->rstd == nullptr)
-        return fail(NEED_ERR_INVALID, "rms norm: weight (16-byte aligned) and rstd must be non-null");
-    const bool need_x = !bwd || a->checkpoint == 0;
-    if (need_x && (a->x == nullptr || !aligned16(a->x) || (a->rows > 1 && a->x_stride % vec != 0)))
-        return fail(NEED_ERR_UNSUPPORTED, "rms norm: x needs 16-byte aligned rows");
-    if (bwd && (a->gout == nullptr || !aligned16(a->gout) || (a->rows > 1 && a->gout_stride % vec != 0)))
-        return fail(NEED_ERR_UNSUPPORTED, "rms norm: gout needs 16-byte aligned rows");
+    if (a->weight == nullptr || a->rstd == nullptr)
+        return fail(NEED_ERR_INVALID, "rms norm: weight and rstd must be non-null");
+    if ((!bwd || a->checkpoint == 0) && a->x == nullptr) return fail(NEED_ERR_INVALID, "rms norm: x is null");
+    if (bwd && (a->gout == nullptr || a->grad_weight == nullptr))
+        return fail(NEED_ERR_INVALID, "rms norm: gout and grad_weight must be non-null");
     void* out = bwd ? a->grad_x : a->out;
-    if (out == nullptr || !aligned16(out)) return fail(NEED_ERR_INVALID, "rms norm: the output is null or not 16-byte aligned");
-    if (bwd && a->grad_weight == nullptr) return fail(NEED_ERR_INVALID, "rms norm: grad_weight is null");
-    const NormPlan pl = norm_plan(a->C / vec);
+    if (out == nullptr) return fail(NEED_ERR_INVALID, "rms norm: the output is null");
+    if (a->rows > 1 && a->out_stride < a->C) return fail(NEED_ERR_INVALID, "rms norm: the output's rows overlap");
+    const NormPlan pl = norm_plan((a->C + vec - 1) / vec);
     if (bwd && (a->workspace == nullptr || a->workspace_bytes < need_rms_norm_train_workspace_size(a->rows, a->C)))
         return fail(NEED_ERR_WORKSPACE, "rms norm: workspace missing or too small");
     NormTrainParams p{};
-    p.x = a->x, p.xs = a->x_stride, p.gout = a->gout, p.gs = a->gout_stride, p.w = a->weight, p.out = out;
+    p.x = a->x, p.xs = a->x_stride, p.gout = a->gout, p.gs = a->gout_stride, p.w = a->weight;
+    p.out = out, p.os = a->out_stride;
+    auto al = [&](const void* q, int64_t stride) { return aligned16(q) && (a->rows == 1 || stride % vec == 0); };
+    const bool whole = a->C % vec == 0 && al(p.out, p.os) && al(p.w, 0) && (bwd ? al(p.gout, p.gs) : true) &&
+                       (bwd && a->checkpoint != 0 ? true : al(p.x, p.xs));
     p.rstd = a->rstd, p.q = a->ckpt_values, p.qs = a->ckpt_scales, p.part = static_cast<float*>(a->workspace);
     p.rows = a->rows, p.C = int32_t(a->C), p.ngroups = int32_t((a->C + kGroup - 1) / kGroup), p.wpr = pl.wpr;
-    p.inv_c = 1.0f / static_cast<float>(a->C_mean), p.eps = static_cast<float>(a->eps);
+    p.inv_c = 1.0f / static_cast<float>(a->C), p.eps = static_cast<float>(a->eps);
     auto run = [&](auto tag) {
         using T = decltype(tag);
-        return a->checkpoint != 0 ? launch_norm<T, true>(bwd, pl, p, s) : launch_norm<T, false>(bwd, pl, p, s);
+        auto go = [&](auto ck) {
+            constexpr bool CK = decltype(ck)::value;
+            return whole ? launch_norm<T, CK, true>(bwd, pl, p, s) : launch_norm<T, CK, false>(bwd, pl, p, s);
+        };
+        return a->checkpoint != 0 ? go(std::true_type{}) : go(std::false_type{});
     };
     int rc;
     if (a->dtype == NEED_F32) rc = run(float{});

@@ -27,7 +27,6 @@ from __future__ import annotations
 from typing import Optional
 
 import torch
-import torch.nn.functional as F
 
 from . import abi
 
@@ -176,18 +175,12 @@ def ssd_conv_silu_train(u: torch.Tensor, weight: torch.Tensor, bias: Optional[to
     if bias is not None and tuple(bias.shape) != (C,):
         raise ValueError(f"bias must be [C] = [{C}]; got {tuple(bias.shape)}")
     seg = _mask(seg_start, B, T)
-    w = weight.reshape(C, K).float()
+    w = weight.float()
     b = None if bias is None else bias.float()
     if u.numel() == 0:
-        out = u * w.sum(dim=1) if b is None else u * w.sum(dim=1) + b
-        return out.to(u.dtype)
-    pad = -C % (4 if u.dtype == torch.float32 else 8)
-    if pad:
-        u = F.pad(u, (0, pad))
-        w = F.pad(w, (0, 0, 0, pad))
-        b = None if b is None else F.pad(b, (0, pad))
-    out = _ext().conv_train(u, w, b, seg)
-    return out[..., :C] if pad else out
+        taps = w.reshape(C, K).sum(dim=1)
+        return (u * taps if b is None else u * taps + b).to(u.dtype)
+    return _ext().conv_train(u, w, b, seg)
 
 
 # --------------------------------------------------------------------------
@@ -207,14 +200,9 @@ def rms_norm_train(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, *,
         raise ValueError(f"weight must have as many elements as x's last dim; got {tuple(weight.shape)} for {tuple(x.shape)}")
     if not float(eps) >= 0.0:
         raise ValueError(f"eps must be >= 0; got {eps}")
-    w = weight.reshape(-1).float()
+    w = weight.float()
     if x.numel() == 0:
-        return (x * w).to(x.dtype)
-    pad = -C % (4 if x.dtype == torch.float32 else 8)
-    if (C + pad) * x.element_size() > _MAX_NORM_BYTES:
+        return (x * w.reshape(-1)).to(x.dtype)
+    if C * x.element_size() > _MAX_NORM_BYTES:
         raise NotImplementedError(f"rms_norm_train takes rows of at most {_MAX_NORM_BYTES} bytes; got C={C} of {x.dtype}")
-    rows = x.reshape(-1, C)
-    if pad:
-        rows, w = F.pad(rows, (0, pad)), F.pad(w, (0, pad))
-    y = _ext().norm_train(rows, w, float(eps), ckpt, C)
-    return (y[:, :C] if pad else y).reshape(x.shape)
+    return _ext().norm_train(x, w, float(eps), ckpt)
