@@ -36,7 +36,7 @@
 // TMA from the slots they were computed in.
 //
 // Across tiles the carry travels as in scan_kernel.cuh (single pass, decoupled
-// look-back over the kTrainDepth tiles before and the inclusive carry of the
+// look-back over the few tiles before and the inclusive carry of the
 // one before those, composed in that fixed order, so results are
 // bit-reproducible), but with its own records: 32-bit words holding the
 // complement of a float's bits, 0 while unwritten.  The call clears them on
@@ -64,22 +64,14 @@ using namespace need;
 
 namespace {
 
-constexpr int kCB = 64;                // channels per tile
+constexpr int kGroup = 64;             // channels of a token that share an 8-bit scale
 constexpr int kSpan = 64;              // tokens between kept states
 constexpr int kNW = 8;                 // row warps
 constexpr int kNT = (kNW + 1) * 32;    // threads: the row warps and the look-back warp
-#ifndef K_FWD_MINB
-#define K_FWD_MINB 4
-#endif
-#ifndef K_BWD_MINB
-#define K_BWD_MINB 3
-#endif
-#ifndef K_DEEP
-#define K_DEEP 7
-#endif
-constexpr int kDeep = K_DEEP;              // most tile maps composed before an inclusive carry
+constexpr int kTileElems = 4096;       // tokens x channels per tile
+constexpr int kNear = 3, kDeep = 5;    // tile maps composed before an inclusive carry
 constexpr int kHdrBytes = WS_HDR_WORDS * 4;
-constexpr int kTileRecBytes = kCB * 12;  // per tile: (A, B) and the inclusive carry of each channel
+constexpr int kRecBytes = 12;           // per tile and channel: (A, B) and the inclusive carry
 
 struct TrainParams {
     CUtensorMap tm[6];   // the streamed inputs, and gout (backward, last)
@@ -88,7 +80,7 @@ struct TrainParams {
     const void* src[6];
     int64_t ssb[6], sst[6];
     int32_t nb, T, C, ncb, nchains, nchunks;  // tiles along T
-    int32_t nspans, depth;                    // kept states along T; look-back depth
+    int32_t nspans, depth, ngroups;           // kept states along T; look-back depth; 8-bit scales per token
     const float* dskip;
     float dt_min, dt_scale;
     const float* h0;       // forward: initial state; backward: unused (the states hold it)
@@ -96,16 +88,16 @@ struct TrainParams {
     const uint8_t* seg;
     int64_t sgb, sgt;
     float* states;         // [nb, nspans, C] the state entering each span
-    uint8_t* q;            // 8-bit values [nin][nb][T][ncb * 64]
-    uint8_t* qs;           // their scales [nin][nb][T][ncb]
+    uint8_t* q;            // 8-bit values [nin][nb][T][ngroups * 64]
+    uint8_t* qs;           // their scales [nin][nb][T][ngroups]
     const float* g_final;  // backward: gradient of the final state or null
     float* grad_h0;        // backward, optional
     float* dpart;          // backward SSD: [nb * nchunks, C] partial sums of the gradient of D,
     uint32_t* dcount;      // [ncb] tiles of each channel block that have written theirs,
     float* grad_d;         // and [C] their sum
     uint32_t* hdr;
-    ulonglong2* agg;           // [ntiles][32] (A, B) of the lane's two channels
-    unsigned long long* incl;  // [ntiles][32] the carry past the tile, two channels
+    unsigned long long* agg;  // [ntiles][CB] (A, B)
+    uint32_t* incl;           // [ntiles][CB] the carry past the tile
     uint32_t polls;
 };
 
@@ -116,6 +108,12 @@ __device__ __forceinline__ float2 apply(float2 A, float2 c, float2 B, bool seg) 
     float2 r = ffma2(A, c, B);
     if (seg) r = make_float2(A.x == 0.0f ? B.x : r.x, A.y == 0.0f ? B.y : r.y);
     return r;
+}
+__device__ __forceinline__ float apply(float A, float c, float B, bool seg) {
+    return seg && A == 0.0f ? B : fmaf(A, c, B);
+}
+__device__ __forceinline__ float mulz(float a, float b, bool seg) {
+    return seg && (a == 0.0f || b == 0.0f) ? 0.0f : a * b;
 }
 __device__ __forceinline__ float2 mulz(float2 a, float2 b, bool seg) {
     float2 r = fmul2(a, b);
@@ -148,36 +146,95 @@ __device__ __forceinline__ unsigned long long ld_relaxed_u64(const unsigned long
     asm volatile("ld.relaxed.gpu.global.u64 %0, [%1];" : "=l"(v) : "l"(p) : "memory");
     return v;
 }
+__device__ __forceinline__ void st_relaxed_u32(uint32_t* p, uint32_t a) {
+    asm volatile("st.relaxed.gpu.global.u32 [%0], %1;" ::"l"(p), "r"(a) : "memory");
+}
+__device__ __forceinline__ uint32_t ld_relaxed_u32(const uint32_t* p) {
+    uint32_t v;
+    asm volatile("ld.relaxed.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+    return v;
+}
+// A lane's NC channels of a record.
+template <int NC>
+struct Agg {
+    unsigned long long w[NC];
+    __device__ __forceinline__ void load(const unsigned long long* p) {
+        if constexpr (NC == 2) {
+            const ulonglong2 v = ld_relaxed_v2u64(reinterpret_cast<const ulonglong2*>(p));
+            w[0] = v.x, w[1] = v.y;
+        } else {
+            w[0] = ld_relaxed_u64(p);
+        }
+    }
+    __device__ __forceinline__ void store(unsigned long long* p) const {
+        if constexpr (NC == 2) st_relaxed_v2u64(reinterpret_cast<ulonglong2*>(p), w[0], w[1]);
+        else st_relaxed_u64(p, w[0]);
+    }
+    __device__ __forceinline__ bool set() const {
+        bool ok = true;
+#pragma unroll
+        for (int k = 0; k < NC; ++k) ok &= rec_set(w[k]);
+        return ok;
+    }
+};
+template <int NC>
+struct Incl {
+    uint32_t w[NC];
+    __device__ __forceinline__ void load(const uint32_t* p) {
+        if constexpr (NC == 2) {
+            const unsigned long long v = ld_relaxed_u64(reinterpret_cast<const unsigned long long*>(p));
+            w[0] = static_cast<uint32_t>(v), w[1] = static_cast<uint32_t>(v >> 32);
+        } else {
+            w[0] = ld_relaxed_u32(p);
+        }
+    }
+    __device__ __forceinline__ void store(uint32_t* p) const {
+        if constexpr (NC == 2)
+            st_relaxed_u64(reinterpret_cast<unsigned long long*>(p), (static_cast<unsigned long long>(w[1]) << 32) | w[0]);
+        else st_relaxed_u32(p, w[0]);
+    }
+    __device__ __forceinline__ bool set() const {
+        bool ok = true;
+#pragma unroll
+        for (int k = 0; k < NC; ++k) ok &= w[k] != 0u;
+        return ok;
+    }
+};
+template <int NC>
+struct Ch {  // a lane's channels in the look-back warp
+    float v[NC];
+};
 
 // ------------------------------------------------------------------ inputs
 struct F4 {  // four channels
     float2 p[2];
 };
 // Channels 4 v .. 4 v + 3 of row r of a slot.
-template <typename T>
+template <typename T, int CB>
 __device__ __forceinline__ F4 row4(const unsigned char* slot, int r, int v) {
     F4 f;
     if constexpr (Ops<T>::BYTES == 4) {
-        const float4 x = reinterpret_cast<const float4*>(slot)[r * (kCB / 4) + v];
+        const float4 x = reinterpret_cast<const float4*>(slot)[r * (CB / 4) + v];
         f.p[0] = make_float2(x.x, x.y);
         f.p[1] = make_float2(x.z, x.w);
     } else {
-        const uint2 x = reinterpret_cast<const uint2*>(slot)[r * (kCB / 4) + v];
+        const uint2 x = reinterpret_cast<const uint2*>(slot)[r * (CB / 4) + v];
         f.p[0] = widen(*reinterpret_cast<const typename Ops<T>::P*>(&x.x));
         f.p[1] = widen(*reinterpret_cast<const typename Ops<T>::P*>(&x.y));
     }
     return f;
 }
-template <typename T>
+template <typename T, int CB>
 __device__ __forceinline__ void put4(unsigned char* slot, int r, int v, const F4& f) {
     const typename Ops<T>::P h[2] = {Ops<T>::pack(f.p[0].x, f.p[0].y), Ops<T>::pack(f.p[1].x, f.p[1].y)};
     if constexpr (Ops<T>::BYTES == 4)
-        reinterpret_cast<float4*>(slot)[r * (kCB / 4) + v] = *reinterpret_cast<const float4*>(h);
-    else reinterpret_cast<uint2*>(slot)[r * (kCB / 4) + v] = *reinterpret_cast<const uint2*>(h);
+        reinterpret_cast<float4*>(slot)[r * (CB / 4) + v] = *reinterpret_cast<const float4*>(h);
+    else reinterpret_cast<uint2*>(slot)[r * (CB / 4) + v] = *reinterpret_cast<const uint2*>(h);
 }
 // The same of an 8-bit slot, times its row's scale.
+template <int CB>
 __device__ __forceinline__ F4 row4_8(const unsigned char* slot, int r, int v, float scale) {
-    const uint32_t q = reinterpret_cast<const uint32_t*>(slot)[r * (kCB / 4) + v];
+    const uint32_t q = reinterpret_cast<const uint32_t*>(slot)[r * (CB / 4) + v];
     F4 f;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -195,10 +252,10 @@ __device__ __forceinline__ F4 row4_8(const unsigned char* slot, int r, int v, fl
 // themselves: there the logit stays and the sigmoid is computed again.
 template <typename T>
 constexpr bool kKeep = !std::is_same<T, __half>::value;
-template <typename T>
+template <typename T, int CB>
 __device__ __forceinline__ void keep4(unsigned char* slot, int r, int v, const F4& s) {
     if constexpr (Ops<T>::BYTES == 4) {
-        put4<float>(slot, r, v, s);
+        put4<float, CB>(slot, r, v, s);
     } else if constexpr (kKeep<T>) {
         F4 y;
 #pragma unroll
@@ -206,22 +263,22 @@ __device__ __forceinline__ void keep4(unsigned char* slot, int r, int v, const F
             const float2 n = fadd2(splat2(1.0f), make_float2(-s.p[i].x, -s.p[i].y));
             y.p[i] = make_float2(s.p[i].x >= 0.5f ? -n.x : s.p[i].x, s.p[i].y >= 0.5f ? -n.y : s.p[i].y);
         }
-        put4<__half>(slot, r, v, y);
+        put4<__half, CB>(slot, r, v, y);
     }
 }
 __device__ __forceinline__ float one_if_negative(float y) {  // by the sign bit: -0 too
     return __int_as_float((__float_as_int(y) >> 31) & 0x3f800000);
 }
 // s and s (1 - s) from a kept slot.
-template <typename T>
+template <typename T, int CB>
 __device__ __forceinline__ void kept4(const unsigned char* slot, int r, int v, F4& s, F4& slope) {
     static_assert(kKeep<T>, "kept as fp32 or f16");
     if constexpr (Ops<T>::BYTES == 4) {
-        s = row4<float>(slot, r, v);
+        s = row4<float, CB>(slot, r, v);
 #pragma unroll
         for (int i = 0; i < 2; ++i) slope.p[i] = fmul2(s.p[i], fadd2(splat2(1.0f), make_float2(-s.p[i].x, -s.p[i].y)));
     } else {
-        const F4 y = row4<__half>(slot, r, v);
+        const F4 y = row4<__half, CB>(slot, r, v);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             s.p[i] = fadd2(y.p[i], make_float2(one_if_negative(y.p[i].x), one_if_negative(y.p[i].y)));
@@ -237,102 +294,139 @@ __device__ __forceinline__ F4 sig4(const F4& x) {
     return s;
 }
 
-// Tokens per tile.
-__host__ __device__ constexpr int tile_tokens(int bytes, bool ck, bool bwd) {
-    return 64;
-}
-
 // DT: how the SSD form gets a = e^-r (r <= dt_max): 0 any range, 1 dt_max <= 1/4.
-template <int FORM, typename T, bool CK, int DT, bool BWD>
+template <int FORM, typename T, bool CK, int DT, int CB_, bool BWD>
 struct TrainCfg {
     static constexpr int NIN = FORM == FORM_GATED ? 3 : 5;
     static constexpr int IN_BYTES = (BWD && CK) ? 1 : Ops<T>::BYTES;  // per streamed input element
-    static constexpr int L = tile_tokens(Ops<T>::BYTES, CK, BWD), R = L / kNW, RT = R / 2;  // rows per warp, thread
-    static constexpr int IN_SLOT = L * kCB * IN_BYTES;
-    static constexpr int SLOT = L * kCB * Ops<T>::BYTES;
+    static constexpr int CB = CB_, NC = CB / 32;                     // channels; of a look-back lane
+    static constexpr int L = kTileElems / CB, R = L / kNW;           // tokens; rows per warp
+    static_assert(CB == 32 || CB == 64, "32 or 64 channels per tile");
+    static_assert(BWD || !CK || CB == kGroup, "the 8-bit forward sees whole groups");
+    static constexpr int LPR = CB / 4, SS = 32 / LPR, RT = R / SS;   // lanes per row, row groups, rows per thread
+    static constexpr int IN_SLOT = L * CB * IN_BYTES;
+    static constexpr int SLOT = L * CB * Ops<T>::BYTES;
     static constexpr int OFF_GOUT = NIN * IN_SLOT;
     // where kept sigmoids and results go: the input slots, or (8-bit inputs) slots of their own
     static constexpr bool STAGED = BWD && CK;
     static constexpr int OFF_STAGE = STAGED ? OFF_GOUT + SLOT : 0;
-    static constexpr int OFF_MAP = OFF_GOUT + (BWD ? SLOT : 0) + (STAGED ? NIN * SLOT : 0);  // [NW][32] (A, B)
-    static constexpr int OFF_FWD = OFF_MAP + kNW * 32 * 16;                // BWD: [NW][32] forward B
-    static constexpr int OFF_IN = OFF_FWD + (BWD ? kNW * 32 * 8 : 0);      // [NW][32] carry entering each warp
-    static constexpr int OFF_HIN = OFF_IN + kNW * 32 * 8;                  // BWD: [NW][32] state entering each warp
-    static constexpr int OFF_SCALE = OFF_HIN + (BWD ? kNW * 32 * 8 : 0);   // BWD CK: [NW][NIN][R] fp32 scales
+    static constexpr int OFF_MAP = OFF_GOUT + (BWD ? SLOT : 0) + (STAGED ? NIN * SLOT : 0);  // [NW][CB] (A, B)
+    static constexpr int OFF_FWD = OFF_MAP + kNW * CB * 8;                 // BWD: [NW][CB] forward B
+    static constexpr int OFF_IN = OFF_FWD + (BWD ? kNW * CB * 4 : 0);      // [NW][CB] carry entering each warp
+    static constexpr int OFF_HIN = OFF_IN + kNW * CB * 4;                  // BWD: [NW][CB] state entering each warp
+    static constexpr int OFF_SCALE = OFF_HIN + (BWD ? kNW * CB * 4 : 0);    // BWD CK: [NW][NIN][R] fp32 scales
     static constexpr int OFF_BAR = OFF_SCALE + (BWD && CK ? kNW * NIN * R * 4 : 0);
     static constexpr int SMEM = OFF_BAR + (kNW + 1) * 8 + 8;
+    // CTAs per SM that registers are planned for (16 bit: 56 to 96 registers).  Most of
+    // a tile's time is latency -- its loads 2 us, the carry 1 us -- so residents count for
+    // more than a few spilled registers: SSD 8x2048x832 forward 42 us at 4, 44 at 3;
+    // backward 87 at 3, 100 at 2.
+    static constexpr int MINB = Ops<T>::BYTES == 4 ? 2 : BWD ? (CK ? 2 : 3) : (CK ? 3 : 4);
 };
 
 // ------------------------------------------------------------------ look-back
 // The look-back warp's work for one tile: composes the tile's map from the
 // warps' maps, publishes it, takes the carry that enters the tile, publishes
 // the one that leaves it, and leaves in s_in the carry entering each warp's
-// rows.  `order(w)` gives the w-th warp met by the carry; `carry` holds the
-// initial value when `first`, else it is read.  Returns the carry past the tile.
-template <bool REV, class Wait>
-__device__ __forceinline__ float2 look_back(const TrainParams& p, int64_t tile, int pos, bool last, int lane,
-                                            float2& carry, const float4* s_map, float2* s_in, Wait maps_ready) {
+// rows.  `carry` holds the initial value where pos == 0, else it is read.  REV:
+// the carry meets the warps from last to first.  Returns the carry past the tile.
+template <bool REV, int NC, class Wait>
+__device__ __forceinline__ Ch<NC> look_back(const TrainParams& p, int64_t tile, int pos, bool last, int lane,
+                                            Ch<NC>& carry, const float2* s_map, float* s_in, Wait maps_ready) {
+    constexpr int CB = 32 * NC;
     const int nagg = min(pos - 1, p.depth);
     const bool seg = p.seg != nullptr;
     bool have = pos == 0, mapped = false;
-    float2 A, B;
-    const int64_t step = int64_t(p.nchains) * 32;
-    for (uint32_t it = 0;; ++it) {
-        bool progressed = false;
-        if (!have) {
-            const ulonglong2* src = p.agg + (tile - p.nchains) * 32 + lane;
-            const unsigned long long c = ld_relaxed_u64(p.incl + (tile - int64_t(nagg + 1) * p.nchains) * 32 + lane);
-            bool valid = rec_set(c);
-            float2 accA = splat2(1.0f), accB = splat2(0.0f);
-            for (int j = 0; j < nagg; ++j, src -= step) {
-                const ulonglong2 m = ld_relaxed_v2u64(src);
-                valid &= rec_set(m.x) & rec_set(m.y);  // (A0, B0), (A1, B1)
-                accB = apply(accA, make_float2(rec_hi(m.x), rec_hi(m.y)), accB, seg);
-                accA = mulz(accA, make_float2(rec_lo(m.x), rec_lo(m.y)), seg);
+    const int64_t step = int64_t(p.nchains) * CB;
+    const unsigned long long* young = p.agg + (tile - p.nchains) * CB + lane * NC;
+    const uint32_t* old = p.incl + (tile - int64_t(nagg + 1) * p.nchains) * CB + lane * NC;
+    Ch<NC> A, B;
+    // one look at the records: all of them read at once, composed if all are there
+    auto look = [&](auto depth) {
+        constexpr int D = decltype(depth)::value;
+        Agg<NC> m[D];
+        Incl<NC> c;
+#pragma unroll
+        for (int j = 0; j < D; ++j)
+            if (j < nagg) m[j].load(young - j * step);
+        c.load(old);
+        bool valid = c.set();
+#pragma unroll
+        for (int j = 0; j < D; ++j)
+            if (j < nagg) valid &= m[j].set();
+        if (!__all_sync(0xffffffffu, valid)) return false;
+#pragma unroll
+        for (int k = 0; k < NC; ++k) {
+            float accA = 1.0f, accB = 0.0f;
+#pragma unroll
+            for (int j = 0; j < D; ++j) {
+                if (j < nagg) {
+                    accB = apply(accA, rec_hi(m[j].w[k]), accB, seg);
+                    accA = mulz(accA, rec_lo(m[j].w[k]), seg);
+                }
             }
-            if (__all_sync(0xffffffffu, valid)) {
-                carry = apply(accA, make_float2(rec_lo(c), rec_hi(c)), accB, seg);
-                have = progressed = true;
-            }
+            carry.v[k] = apply(accA, __uint_as_float(~c.w[k]), accB, seg);
         }
+        return true;
+    };
+    auto map_of = [&](int w, int k) { return s_map[w * CB + lane * NC + k]; };
+    for (uint32_t it = 0;; ++it) {
+        if (!have) have = p.depth > kNear ? look(std::integral_constant<int, kDeep>{}) : look(std::integral_constant<int, kNear>{});
         // with the carry in, nothing else is polled: suspend on the barrier
         if (!mapped && maps_ready(have)) {
-            A = splat2(1.0f);
-            B = splat2(0.0f);
 #pragma unroll
-            for (int k = 0; k < kNW; ++k) {  // in the order the carry meets the warps
-                const float4 m = s_map[(REV ? kNW - 1 - k : k) * 32 + lane];
-                B = apply(make_float2(m.x, m.y), B, make_float2(m.z, m.w), seg);
-                A = mulz(make_float2(m.x, m.y), A, seg);
+            for (int k = 0; k < NC; ++k) {
+                A.v[k] = 1.0f;
+                B.v[k] = 0.0f;
+#pragma unroll
+                for (int w = 0; w < kNW; ++w) {  // in the order the carry meets the warps
+                    const float2 m = map_of(REV ? kNW - 1 - w : w, k);
+                    B.v[k] = apply(m.x, B.v[k], m.y, seg);
+                    A.v[k] = mulz(m.x, A.v[k], seg);
+                }
             }
-            if (!last && pos > 0)  // the first tile's map is never composed: its carry is known
-                st_relaxed_v2u64(p.agg + tile * 32 + lane, rec_pair(A.x, B.x), rec_pair(A.y, B.y));
-            mapped = progressed = true;
+            if (!last && pos > 0) {  // the first tile's map is never composed: its carry is known
+                Agg<NC> r;
+#pragma unroll
+                for (int k = 0; k < NC; ++k) r.w[k] = rec_pair(A.v[k], B.v[k]);
+                r.store(p.agg + tile * CB + lane * NC);
+            }
+            mapped = true;
         }
         if (mapped && have) break;
         if (!have && it >= p.polls) {  // go on without a predecessor's carry
             if (lane == 0) atomicOr(&p.hdr[WS_ERROR], ERR_LOOKBACK);
-            carry = splat2(__int_as_float(0x7fc00000));
+#pragma unroll
+            for (int k = 0; k < NC; ++k) carry.v[k] = __int_as_float(0x7fc00000);
             have = true;
         } else if (have && it - min(it, p.polls) >= kTmaPolls) {  // the row warps' own waits are shorter
             if (lane == 0) atomicOr(&p.hdr[WS_ERROR], ERR_TMA);
-            A = splat2(0.0f);
-            B = splat2(__int_as_float(0x7fc00000));
+#pragma unroll
+            for (int k = 0; k < NC; ++k) {
+                A.v[k] = 0.0f;
+                B.v[k] = __int_as_float(0x7fc00000);
+            }
             break;
         }
-        if (!progressed && !have && it >= 2) __nanosleep(64);
     }
-    const float2 past = apply(A, carry, B, seg);
-    if (!last) {
-        st_relaxed_u64(p.incl + tile * 32 + lane, rec_pair(past.x, past.y));
-    }
-    float2 c = carry;
+    Ch<NC> past;
+    Incl<NC> r;
 #pragma unroll
-    for (int k = 0; k < kNW; ++k) {
-        const int w = REV ? kNW - 1 - k : k;
-        s_in[w * 32 + lane] = c;
-        const float4 m = s_map[w * 32 + lane];
-        c = apply(make_float2(m.x, m.y), c, make_float2(m.z, m.w), seg);
+    for (int k = 0; k < NC; ++k) {
+        past.v[k] = apply(A.v[k], carry.v[k], B.v[k], seg);
+        r.w[k] = rec_enc(past.v[k]);
+    }
+    if (!last) r.store(p.incl + tile * CB + lane * NC);
+    Ch<NC> c = carry;
+#pragma unroll
+    for (int n = 0; n < kNW; ++n) {
+        const int w = REV ? kNW - 1 - n : n;
+#pragma unroll
+        for (int k = 0; k < NC; ++k) {
+            s_in[w * CB + lane * NC + k] = c.v[k];
+            const float2 m = map_of(w, k);
+            c.v[k] = apply(m.x, c.v[k], m.y, seg);
+        }
     }
     return past;
 }
@@ -340,9 +434,6 @@ __device__ __forceinline__ float2 look_back(const TrainParams& p, int64_t tile, 
 // This lane's two channels of a [.., C] fp32 row (0 past C).
 __device__ __forceinline__ float2 ld_pair(const float* row, int c, int C) {
     return make_float2(c < C ? row[c] : 0.0f, c + 1 < C ? row[c + 1] : 0.0f);
-}
-__device__ __forceinline__ float2 ld_pair_cg(const float* row, int c, int C) {  // another block's writes: from L2
-    return make_float2(c < C ? __ldcg(row + c) : 0.0f, c + 1 < C ? __ldcg(row + c + 1) : 0.0f);
 }
 __device__ __forceinline__ float2 shfl2(float2 x, int m) {
     return make_float2(__shfl_xor_sync(0xffffffffu, x.x, m), __shfl_xor_sync(0xffffffffu, x.y, m));
@@ -352,11 +443,25 @@ __device__ __forceinline__ void st_pair(float* row, int c, int C, float2 v) {
     if (c + 1 < C) row[c + 1] = v.y;
 }
 
+template <int NC>
+__device__ __forceinline__ Ch<NC> ld_ch(const float* row, int c, int C) {
+    Ch<NC> r;
+#pragma unroll
+    for (int k = 0; k < NC; ++k) r.v[k] = c + k < C ? row[c + k] : 0.0f;
+    return r;
+}
+template <int NC>
+__device__ __forceinline__ void st_ch(float* row, int c, int C, const Ch<NC>& x) {
+#pragma unroll
+    for (int k = 0; k < NC; ++k)
+        if (c + k < C) row[c + k] = x.v[k];
+}
+
 struct Tile {
     int pos, chunk, cblk, b, t0, c0, nvalid;
     int64_t tile;
 };
-template <int L>
+template <int L, int CB>
 __device__ __forceinline__ Tile tile_of(const TrainParams& p, bool rev) {
     Tile t;
     // chains along x, then positions along them (y, then z): blocks start in that
@@ -368,7 +473,7 @@ __device__ __forceinline__ Tile tile_of(const TrainParams& p, bool rev) {
     t.b = chain / p.ncb;
     t.cblk = chain - t.b * p.ncb;
     t.t0 = t.chunk * L;
-    t.c0 = t.cblk * kCB;
+    t.c0 = t.cblk * CB;
     t.nvalid = min(L, p.T - t.t0);
     return t;
 }
@@ -383,22 +488,22 @@ __device__ __forceinline__ uint32_t reset_bits(const TrainParams& p, const Tile&
 }
 
 // A warp's rows of stream k with plain loads, as TMA would leave them (zeros past C and T).
-template <typename T, int R>
+template <typename T, int R, int CB>
 __device__ __forceinline__ void plain_rows(const TrainParams& p, const Tile& tl, int k, unsigned char* slot, int wr0,
                                            int rows, int lane) {
-    const T* src = static_cast<const T*>(p.src[k]) + tl.b * p.ssb[k] + int64_t(tl.t0 + wr0) * p.sst[k];
-    const int c = tl.c0 + 2 * lane;
-    for (int r = 0; r < R; ++r) {
-        const float x = r < rows && c < p.C ? to_f(src[r * p.sst[k] + c]) : 0.0f;
-        const float y = r < rows && c + 1 < p.C ? to_f(src[r * p.sst[k] + c + 1]) : 0.0f;
-        reinterpret_cast<typename Ops<T>::P*>(slot)[r * (kCB / 2) + lane] = Ops<T>::pack(x, y);
+    const T* src = static_cast<const T*>(p.src[k]) + tl.b * p.ssb[k] + int64_t(tl.t0 + wr0) * p.sst[k] + tl.c0;
+    for (int i = lane; i < R * CB / 2; i += 32) {
+        const int r = i / (CB / 2), e = 2 * (i - r * (CB / 2));
+        const float x = r < rows && tl.c0 + e < p.C ? to_f(src[r * p.sst[k] + e]) : 0.0f;
+        const float y = r < rows && tl.c0 + e + 1 < p.C ? to_f(src[r * p.sst[k] + e + 1]) : 0.0f;
+        reinterpret_cast<typename Ops<T>::P*>(slot)[i] = Ops<T>::pack(x, y);
     }
     __syncwarp();
 }
 
 // Starts the loads of a warp's rows: n streams, of `bytes` per element (gout,
 // stream n - 1 of the backward, of sizeof(T)), into slot(k).
-template <typename T, int N, int NIN, int IN_BYTES, int R, class Slot>
+template <typename T, int N, int NIN, int IN_BYTES, int R, int CB, class Slot>
 __device__ __forceinline__ void load_rows(const TrainParams& p, const Tile& tl, int wr0, int rows, int lane,
                                           uint64_t* bar, bool stacked, Slot slot) {
     if (rows > 0) {
@@ -406,7 +511,7 @@ __device__ __forceinline__ void load_rows(const TrainParams& p, const Tile& tl, 
             uint32_t tx = 0;
 #pragma unroll
             for (int k = 0; k < N; ++k)
-                if (!((p.plain >> k) & 1u)) tx += R * kCB * (k < NIN ? IN_BYTES : Ops<T>::BYTES);
+                if (!((p.plain >> k) & 1u)) tx += R * CB * (k < NIN ? IN_BYTES : Ops<T>::BYTES);
             mbar_arrive_expect_tx(bar, tx);
 #pragma unroll
             for (int k = 0; k < N; ++k)
@@ -415,7 +520,7 @@ __device__ __forceinline__ void load_rows(const TrainParams& p, const Tile& tl, 
         }
         if (p.plain != 0)
             for (int k = 0; k < N; ++k)
-                if ((p.plain >> k) & 1u) plain_rows<T, R>(p, tl, k, slot(k), wr0, rows, lane);
+                if ((p.plain >> k) & 1u) plain_rows<T, R, CB>(p, tl, k, slot(k), wr0, rows, lane);
     }
 }
 
@@ -440,9 +545,9 @@ __device__ __forceinline__ void decay4(const TrainParams& p, const F4& x, F4& a,
 template <typename T, int NIN, int R>
 __device__ __forceinline__ void write_e4m3(const TrainParams& p, const Tile& tl, const unsigned char* base, int slot_bytes,
                                            int wr0, int rows, int lane) {
-    constexpr int N = 16 / Ops<T>::BYTES, LPR = kCB / N, RP = 32 / LPR;  // elements, lanes per row, rows at once
+    constexpr int N = 16 / Ops<T>::BYTES, LPR = kGroup / N, RP = 32 / LPR;  // elements, lanes per row, rows at once
     const int v = lane % LPR;
-    const int64_t pitch = int64_t(p.ncb) * kCB;
+    const int64_t pitch = int64_t(p.ngroups) * kGroup;
 #pragma unroll
     for (int k = 0; k < NIN; ++k) {
         const unsigned char* slot = base + k * slot_bytes;
@@ -483,24 +588,96 @@ __device__ __forceinline__ void write_e4m3(const TrainParams& p, const Tile& tl,
                 uint8_t* dst = p.q + (first + r) * pitch + tl.c0 + v * N;
                 if constexpr (N == 8) *reinterpret_cast<uint2*>(dst) = make_uint2(q[0], q[1]);
                 else *reinterpret_cast<uint32_t*>(dst) = q[0];
-                if (v == 0) p.qs[(first + r) * p.ncb + tl.cblk] = static_cast<uint8_t>(sc);
+                if (v == 0) p.qs[(first + r) * p.ngroups + tl.cblk] = static_cast<uint8_t>(sc);
             }
         }
     }
 }
 
+// ------------------------------------------------------------------ in-warp scan
+template <class Shfl>
+__device__ __forceinline__ F4 shfl4(const F4& x, Shfl f) {
+    F4 r;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) r.p[i] = make_float2(f(x.p[i].x), f(x.p[i].y));
+    return r;
+}
+// The SS row groups of a warp hold consecutive rows.  In: each thread's map of its
+// rows.  Out: (A, B) of its and the groups' before it, (EA, EB) of those before
+// it alone.  The last group's (A, B) is the warp's.
+template <int LPR, int SS>
+__device__ __forceinline__ void warp_prefix(F4& A, F4& B, F4& EA, F4& EB, int q, bool seg) {
+    F4 oA, oB;
+#pragma unroll
+    for (int d = 1; d < SS; d *= 2) {
+        oA = shfl4(A, [&](float x) { return __shfl_up_sync(0xffffffffu, x, d * LPR); });
+        oB = shfl4(B, [&](float x) { return __shfl_up_sync(0xffffffffu, x, d * LPR); });
+        if (q >= d) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                B.p[i] = apply(A.p[i], oB.p[i], B.p[i], seg);
+                A.p[i] = mulz(A.p[i], oA.p[i], seg);
+            }
+        }
+    }
+    if constexpr (SS == 2) {
+        EA = oA, EB = oB;
+    } else {
+        EA = shfl4(A, [&](float x) { return __shfl_up_sync(0xffffffffu, x, LPR); });
+        EB = shfl4(B, [&](float x) { return __shfl_up_sync(0xffffffffu, x, LPR); });
+    }
+    if (q == 0) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) EA.p[i] = splat2(1.0f), EB.p[i] = splat2(0.0f);
+    }
+}
+// The same from the last group to the first: the carry enters the last.
+template <int LPR, int SS>
+__device__ __forceinline__ void warp_suffix(F4& A, F4& M, F4& EA, F4& EM, int q, bool seg) {
+    F4 oA, oM;
+#pragma unroll
+    for (int d = 1; d < SS; d *= 2) {
+        oA = shfl4(A, [&](float x) { return __shfl_down_sync(0xffffffffu, x, d * LPR); });
+        oM = shfl4(M, [&](float x) { return __shfl_down_sync(0xffffffffu, x, d * LPR); });
+        if (q + d < SS) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                M.p[i] = apply(A.p[i], oM.p[i], M.p[i], seg);
+                A.p[i] = mulz(A.p[i], oA.p[i], seg);
+            }
+        }
+    }
+    if constexpr (SS == 2) {
+        EA = oA, EM = oM;
+    } else {
+        EA = shfl4(A, [&](float x) { return __shfl_down_sync(0xffffffffu, x, LPR); });
+        EM = shfl4(M, [&](float x) { return __shfl_down_sync(0xffffffffu, x, LPR); });
+    }
+    if (q == SS - 1) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) EA.p[i] = splat2(1.0f), EM.p[i] = splat2(0.0f);
+    }
+}
+__device__ __forceinline__ void put_maps(float2* dst, const F4& A, const F4& B) {
+    float4* d = reinterpret_cast<float4*>(dst);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) d[i] = make_float4(A.p[i].x, B.p[i].x, A.p[i].y, B.p[i].y);
+}
+__device__ __forceinline__ float4 as_float4(const F4& x) { return make_float4(x.p[0].x, x.p[0].y, x.p[1].x, x.p[1].y); }
+
 // ------------------------------------------------------------------ forward
-template <int FORM, typename T, bool CK, int DT>
-__global__ void __launch_bounds__(kNT, K_FWD_MINB) train_fwd_kernel(const __grid_constant__ TrainParams p) {
-    using K = TrainCfg<FORM, T, CK, DT, false>;
+template <int FORM, typename T, bool CK, int DT, int CBW>
+__global__ void __launch_bounds__(kNT, (TrainCfg<FORM, T, CK, DT, CBW, false>::MINB))
+    train_fwd_kernel(const __grid_constant__ TrainParams p) {
+    using K = TrainCfg<FORM, T, CK, DT, CBW, false>;
     extern __shared__ __align__(128) unsigned char base[];
-    float4* s_map = reinterpret_cast<float4*>(base + K::OFF_MAP);
-    float2* s_in = reinterpret_cast<float2*>(base + K::OFF_IN);
+    float2* s_map = reinterpret_cast<float2*>(base + K::OFF_MAP);
+    float* s_in = reinterpret_cast<float*>(base + K::OFF_IN);
     uint64_t* s_bar = reinterpret_cast<uint64_t*>(base + K::OFF_BAR);
     uint64_t* s_maps = s_bar + kNW;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const bool seg = p.seg != nullptr;
-    const Tile tl = tile_of<K::L>(p, false);
+    const Tile tl = tile_of<K::L, K::CB>(p, false);
     if (tl.pos >= p.nchunks) return;
     if (threadIdx.x == 0) {
         for (int w = 0; w < kNW; ++w) mbar_init(&s_bar[w], 1);
@@ -510,30 +687,32 @@ __global__ void __launch_bounds__(kNT, K_FWD_MINB) train_fwd_kernel(const __grid
     __syncthreads();
 
     if (warp == kNW) {
-        const int c = tl.c0 + 2 * lane;
+        const int c = tl.c0 + K::NC * lane;
         const bool last = tl.chunk + 1 == p.nchunks;
-        float2 carry = splat2(0.0f);
-        if (tl.pos == 0 && p.h0 != nullptr) carry = ld_pair(p.h0 + int64_t(tl.b) * p.C, c, p.C);
-        const float2 past = look_back<false>(p, tl.tile, tl.pos, last, lane, carry, s_map, s_in, [&](bool block) {
-            return __all_sync(0xffffffffu, block ? mbar_try_wait(s_maps, 0) : mbar_test_wait(s_maps, 0));
-        });
+        Ch<K::NC> carry{};
+        if (tl.pos == 0 && p.h0 != nullptr) carry = ld_ch<K::NC>(p.h0 + int64_t(tl.b) * p.C, c, p.C);
+        const Ch<K::NC> past =
+            look_back<false, K::NC>(p, tl.tile, tl.pos, last, lane, carry, s_map, s_in, [&](bool block) {
+                return __all_sync(0xffffffffu, block ? mbar_try_wait(s_maps, 0) : mbar_test_wait(s_maps, 0));
+            });
         __syncwarp();
         named_arrive(1, kNT);
         float* st = p.states + (int64_t(tl.b) * p.nspans + tl.t0 / kSpan) * p.C;
-        st_pair(st, c, p.C, carry);
-        if (K::L > kSpan && tl.nvalid > kSpan) st_pair(st + p.C, c, p.C, s_in[kSpan / K::R * 32 + lane]);
-        if (last && p.h_final != nullptr) st_pair(p.h_final + int64_t(tl.b) * p.C, c, p.C, past);
+        st_ch(st, c, p.C, carry);
+        if (K::L > kSpan && tl.nvalid > kSpan)
+            st_ch(st + p.C, c, p.C, *reinterpret_cast<const Ch<K::NC>*>(s_in + kSpan / K::R * K::CB + K::NC * lane));
+        if (last && p.h_final != nullptr) st_ch(p.h_final + int64_t(tl.b) * p.C, c, p.C, past);
         return;
     }
 
-    constexpr int RT = K::RT;
+    constexpr int RT = K::RT, LPR = K::LPR, SS = K::SS, CB = K::CB;
     const int wr0 = warp * K::R;
     const int rows = max(0, min(K::R, tl.nvalid - wr0));
-    unsigned char* slots = base + wr0 * kCB * K::IN_BYTES;  // this warp's rows of stream 0
+    unsigned char* slots = base + wr0 * K::CB * K::IN_BYTES;  // this warp's rows of stream 0
     auto slot = [&](int k) { return slots + k * K::IN_SLOT; };
-    load_rows<T, K::NIN, K::NIN, K::IN_BYTES, K::R>(p, tl, wr0, rows, lane, &s_bar[warp], false, slot);
+    load_rows<T, K::NIN, K::NIN, K::IN_BYTES, K::R, K::CB>(p, tl, wr0, rows, lane, &s_bar[warp], false, slot);
     const uint32_t wresets = reset_bits<K::R>(p, tl, wr0, lane);
-    const int q = lane >> 4, v = lane & 15;          // row group (half the warp's rows) and four channels
+    const int q = lane / LPR, v = lane % LPR;  // row group and four channels
     const int c = tl.c0 + 4 * v;
     const uint32_t resets = (wresets >> (RT * q)) & ((1u << RT) - 1u);
     F4 D;
@@ -557,8 +736,8 @@ __global__ void __launch_bounds__(kNT, K_FWD_MINB) train_fwd_kernel(const __grid
         for (int j = 0; j < RT; ++j) {
             const int r = q * RT + j;
             F4 a, na, s;
-            decay4<FORM, T, DT>(p, row4<T>(slot(0), r, v), a, na, s);
-            const F4 g = sig4<T>(row4<T>(slot(1), r, v)), x = row4<T>(slot(2), r, v);
+            decay4<FORM, T, DT>(p, row4<T, CB>(slot(0), r, v), a, na, s);
+            const F4 g = sig4<T>(row4<T, CB>(slot(1), r, v)), x = row4<T, CB>(slot(2), r, v);
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 const float2 b = fmul2(na.p[i], fmul2(g.p[i], x.p[i]));
@@ -578,19 +757,9 @@ __global__ void __launch_bounds__(kNT, K_FWD_MINB) train_fwd_kernel(const __grid
     const bool whole = rows == K::R && wresets == 0u;
     if (whole) phase1(std::true_type{});
     else if (rows > 0) phase1(std::false_type{});
-    // the two groups of a warp: EA, EB the map of the rows before this thread's,
-    // and the warp's map from the second group
-    F4 EA, EB;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const float2 oA = shfl2(A.p[i], 16), oB = shfl2(B.p[i], 16);
-        EA.p[i] = q == 0 ? splat2(1.0f) : oA;
-        EB.p[i] = q == 0 ? splat2(0.0f) : oB;
-        if (q == 1) {
-            const float2 tB = apply(A.p[i], oB, B.p[i], seg), tA = mulz(A.p[i], oA, seg);
-            s_map[warp * 32 + 2 * v + i] = make_float4(tA.x, tA.y, tB.x, tB.y);
-        }
-    }
+    F4 EA, EB;  // the map of the warp's rows before this thread's
+    warp_prefix<LPR, SS>(A, B, EA, EB, q, seg);
+    if (q == SS - 1) put_maps(s_map + warp * CB + 4 * v, A, B);
     mbar_arrive(s_maps);
     if constexpr (CK)  // while the carry comes in
         if (rows > 0) write_e4m3<T, K::NIN, K::R>(p, tl, slots, K::IN_SLOT, wr0, rows, lane);
@@ -598,7 +767,7 @@ __global__ void __launch_bounds__(kNT, K_FWD_MINB) train_fwd_kernel(const __grid
     if (rows == 0) return;
 
     // phase 2: the states from the entering one, and the outputs
-    const float4 in4 = reinterpret_cast<const float4*>(s_in)[warp * 16 + v];
+    const float4 in4 = reinterpret_cast<const float4*>(s_in)[warp * LPR + v];
     F4 h0;
     h0.p[0] = apply(EA.p[0], make_float2(in4.x, in4.y), EB.p[0], seg);
     h0.p[1] = apply(EA.p[1], make_float2(in4.z, in4.w), EB.p[1], seg);
@@ -609,9 +778,9 @@ __global__ void __launch_bounds__(kNT, K_FWD_MINB) train_fwd_kernel(const __grid
             const int r = q * RT + j;
             F4 o, sc, so, u;
             if constexpr (FORM == FORM_SSD) {
-                sc = sig4<T>(row4<T>(slot(3), r, v));
-                so = sig4<T>(row4<T>(slot(4), r, v));
-                u = row4<T>(slot(2), r, v);
+                sc = sig4<T>(row4<T, CB>(slot(3), r, v));
+                so = sig4<T>(row4<T, CB>(slot(4), r, v));
+                u = row4<T, CB>(slot(2), r, v);
             }
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
@@ -621,7 +790,7 @@ __global__ void __launch_bounds__(kNT, K_FWD_MINB) train_fwd_kernel(const __grid
                 if constexpr (FORM == FORM_SSD)
                     o.p[i] = fmul2(ffma2(sc.p[i], o.p[i], fmul2(D.p[i], u.p[i])), so.p[i]);
             }
-            put4<T>(slot(OUT), r, v, o);
+            put4<T, CB>(slot(OUT), r, v, o);
         }
     };
     if (whole) phase2(std::true_type{});
@@ -636,22 +805,23 @@ __global__ void __launch_bounds__(kNT, K_FWD_MINB) train_fwd_kernel(const __grid
 }
 
 // ------------------------------------------------------------------ backward
-template <int FORM, typename T, bool CK, int DT>
-__global__ void __launch_bounds__(kNT, K_BWD_MINB) train_bwd_kernel(const __grid_constant__ TrainParams p) {
-    using K = TrainCfg<FORM, T, CK, DT, true>;
+template <int FORM, typename T, bool CK, int DT, int CBW>
+__global__ void __launch_bounds__(kNT, (TrainCfg<FORM, T, CK, DT, CBW, true>::MINB))
+    train_bwd_kernel(const __grid_constant__ TrainParams p) {
+    using K = TrainCfg<FORM, T, CK, DT, CBW, true>;
     using O = Ops<T>;
     extern __shared__ __align__(128) unsigned char base[];
-    float4* s_map = reinterpret_cast<float4*>(base + K::OFF_MAP);
-    float2* s_fwd = reinterpret_cast<float2*>(base + K::OFF_FWD);
-    float2* s_in = reinterpret_cast<float2*>(base + K::OFF_IN);
-    float2* s_hin = reinterpret_cast<float2*>(base + K::OFF_HIN);
+    float2* s_map = reinterpret_cast<float2*>(base + K::OFF_MAP);
+    float* s_fwd = reinterpret_cast<float*>(base + K::OFF_FWD);
+    float* s_in = reinterpret_cast<float*>(base + K::OFF_IN);
+    float* s_hin = reinterpret_cast<float*>(base + K::OFF_HIN);
     float* s_scale = reinterpret_cast<float*>(base + K::OFF_SCALE);
     uint64_t* s_bar = reinterpret_cast<uint64_t*>(base + K::OFF_BAR);
     uint64_t* s_maps = s_bar + kNW;
     uint32_t* s_last = reinterpret_cast<uint32_t*>(s_maps + 1);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const bool seg = p.seg != nullptr;
-    const Tile tl = tile_of<K::L>(p, true);
+    const Tile tl = tile_of<K::L, K::CB>(p, true);
     if (tl.pos >= p.nchunks) return;
     if (threadIdx.x == 0) {
         for (int w = 0; w < kNW; ++w) mbar_init(&s_bar[w], 1);
@@ -661,60 +831,63 @@ __global__ void __launch_bounds__(kNT, K_BWD_MINB) train_bwd_kernel(const __grid
     __syncthreads();
 
     if (warp == kNW) {
-        const int c = tl.c0 + 2 * lane;
+        const int c = tl.c0 + K::NC * lane;
         const bool last = tl.chunk == 0;
         const float* st = p.states + (int64_t(tl.b) * p.nspans + tl.t0 / kSpan) * p.C;
-        float2 h = ld_pair(st, c, p.C), hmid = splat2(0.0f);
-        if (K::L > kSpan && tl.nvalid > kSpan) hmid = ld_pair(st + p.C, c, p.C);
-        float2 carry = splat2(0.0f);
-        if (tl.pos == 0 && p.g_final != nullptr) carry = ld_pair(p.g_final + int64_t(tl.b) * p.C, c, p.C);
+        Ch<K::NC> h = ld_ch<K::NC>(st, c, p.C), hmid{}, carry{};
+        if (K::L > kSpan && tl.nvalid > kSpan) hmid = ld_ch<K::NC>(st + p.C, c, p.C);
+        if (tl.pos == 0 && p.g_final != nullptr) carry = ld_ch<K::NC>(p.g_final + int64_t(tl.b) * p.C, c, p.C);
         bool handed = false;
-        const float2 past = look_back<true>(p, tl.tile, tl.pos, last, lane, carry, s_map, s_in, [&](bool block) {
-            const bool ready =
-                __all_sync(0xffffffffu, block ? mbar_try_wait(s_maps, 0) : mbar_test_wait(s_maps, 0));
-            if (ready) {  // the states entering the warps first: they wait for no other tile
-                handed = true;
+        const Ch<K::NC> past =
+            look_back<true, K::NC>(p, tl.tile, tl.pos, last, lane, carry, s_map, s_in, [&](bool block) {
+                const bool ready =
+                    __all_sync(0xffffffffu, block ? mbar_try_wait(s_maps, 0) : mbar_test_wait(s_maps, 0));
+                if (ready) {  // the states entering the warps first: they wait for no other tile
+                    handed = true;
 #pragma unroll
-                for (int w = 0; w < kNW; ++w) {
-                    if (K::L > kSpan && w == kSpan / K::R) h = hmid;
-                    s_hin[w * 32 + lane] = h;
-                    const float4 m = s_map[w * 32 + lane];
-                    h = apply(make_float2(m.x, m.y), h, s_fwd[w * 32 + lane], seg);
+                    for (int w = 0; w < kNW; ++w) {
+                        if (K::L > kSpan && w == kSpan / K::R) h = hmid;
+#pragma unroll
+                        for (int k = 0; k < K::NC; ++k) {
+                            const int e = w * K::CB + K::NC * lane + k;
+                            s_hin[e] = h.v[k];
+                            h.v[k] = apply(s_map[e].x, h.v[k], s_fwd[e], seg);
+                        }
+                    }
+                    __syncwarp();
+                    named_arrive(1, kNT);
                 }
-                __syncwarp();
-                named_arrive(1, kNT);
-            }
-            return ready;
-        });
+                return ready;
+            });
         if (!handed) named_arrive(1, kNT);  // gave up: the row warps are let go
         __syncwarp();
         named_arrive(2, kNT);
-        if (last && p.grad_h0 != nullptr) st_pair(p.grad_h0 + int64_t(tl.b) * p.C, c, p.C, past);
+        if (last && p.grad_h0 != nullptr) st_ch(p.grad_h0 + int64_t(tl.b) * p.C, c, p.C, past);
         return;
     }
 
-    constexpr int RT = K::RT;
+    constexpr int RT = K::RT, LPR = K::LPR, SS = K::SS, CB = K::CB;
     const int wr0 = warp * K::R;
     const int rows = max(0, min(K::R, tl.nvalid - wr0));
     auto slot = [&](int k) {
-        return k < K::NIN ? base + k * K::IN_SLOT + wr0 * kCB * K::IN_BYTES : base + K::OFF_GOUT + wr0 * kCB * O::BYTES;
+        return k < K::NIN ? base + k * K::IN_SLOT + wr0 * K::CB * K::IN_BYTES : base + K::OFF_GOUT + wr0 * K::CB * O::BYTES;
     };
     auto stage = [&](int k) {  // kept sigmoids, then gradients
-        return K::STAGED ? base + K::OFF_STAGE + k * K::SLOT + wr0 * kCB * O::BYTES : slot(k);
+        return K::STAGED ? base + K::OFF_STAGE + k * K::SLOT + wr0 * K::CB * O::BYTES : slot(k);
     };
-    load_rows<T, K::NIN + 1, K::NIN, K::IN_BYTES, K::R>(p, tl, wr0, rows, lane, &s_bar[warp], CK, slot);
+    load_rows<T, K::NIN + 1, K::NIN, K::IN_BYTES, K::R, K::CB>(p, tl, wr0, rows, lane, &s_bar[warp], CK, slot);
     const uint32_t wresets = reset_bits<K::R>(p, tl, wr0, lane);
     if constexpr (CK) {
         for (int i = lane; i < K::NIN * K::R; i += 32) {
             const int k = i / K::R, j = i - k * K::R;
             float f = 0.0f;
             if (j < rows)
-                f = e4m3_scale(p.qs[((int64_t(k) * p.nb + tl.b) * p.T + tl.t0 + wr0 + j) * p.ncb + tl.cblk]);
+                f = e4m3_scale(p.qs[((int64_t(k) * p.nb + tl.b) * p.T + tl.t0 + wr0 + j) * p.ngroups + tl.c0 / kGroup]);
             s_scale[warp * K::NIN * K::R + i] = f;
         }
         __syncwarp();
     }
-    const int q = lane >> 4, v = lane & 15;
+    const int q = lane / LPR, v = lane % LPR;
     const int c = tl.c0 + 4 * v;
     const uint32_t resets = (wresets >> (RT * q)) & ((1u << RT) - 1u);
     F4 D;
@@ -727,14 +900,14 @@ __global__ void __launch_bounds__(kNT, K_BWD_MINB) train_bwd_kernel(const __grid
         mbar_wait_bounded(&s_bar[warp], 0, kTmaPolls);
     }
     auto input = [&](int k, int r) {
-        if constexpr (CK) return row4_8(slot(k), r, v, s_scale[(warp * K::NIN + k) * K::R + r]);
-        else return row4<T>(slot(k), r, v);
+        if constexpr (CK) return row4_8<CB>(slot(k), r, v, s_scale[(warp * K::NIN + k) * K::R + r]);
+        else return row4<T, CB>(slot(k), r, v);
     };
-    auto gout = [&](int r) { return row4<T>(slot(K::NIN), r, v); };
+    auto gout = [&](int r) { return row4<T, CB>(slot(K::NIN), r, v); };
     // sigmoid of logit stream k again (or as kept), and its slope
     auto gate = [&](int k, int r, F4& s, F4& slope) {
         if constexpr (kKeep<T>) {
-            kept4<T>(stage(k), r, v, s, slope);
+            kept4<T, CB>(stage(k), r, v, s, slope);
         } else {
             const F4 x = input(k, r);
 #pragma unroll
@@ -763,12 +936,12 @@ __global__ void __launch_bounds__(kNT, K_BWD_MINB) train_bwd_kernel(const __grid
             decay4<FORM, T, DT>(p, input(0, r), a, na[j], sd);
             const F4 g = sig4<T>(input(1, r)), x = input(2, r);
             F4 e = gout(r);
-            keep4<T>(stage(1), r, v, g);
+            keep4<T, CB>(stage(1), r, v, g);
             if constexpr (FORM == FORM_SSD) {
                 const F4 sc = sig4<T>(input(3, r)), so = sig4<T>(input(4, r));
-                keep4<T>(stage(0), r, v, sd);
-                keep4<T>(stage(3), r, v, sc);
-                keep4<T>(stage(4), r, v, so);
+                keep4<T, CB>(stage(0), r, v, sd);
+                keep4<T, CB>(stage(3), r, v, sc);
+                keep4<T, CB>(stage(4), r, v, so);
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     const float2 gs = fmul2(e.p[i], so.p[i]);
@@ -799,33 +972,25 @@ __global__ void __launch_bounds__(kNT, K_BWD_MINB) train_bwd_kernel(const __grid
     const bool whole = rows == K::R && wresets == 0u;
     if (whole) phase1(std::true_type{});
     else if (rows > 0) phase1(std::false_type{});
-    // the other row group's maps: the state enters the second group through the
-    // first's (fA, fB), mu enters the first through the second's (fA, fM)
-    F4 fA, fC;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const float2 oA = shfl2(A.p[i], 16), oB = shfl2(B.p[i], 16), oM = shfl2(M.p[i], 16);
-        fA.p[i] = oA;
-        fC.p[i] = q == 1 ? oB : oM;
-        if (q == 1) {
-            const float2 tA = mulz(A.p[i], oA, seg), tB = apply(A.p[i], oB, B.p[i], seg);
-            const float2 tM = apply(oA, M.p[i], oM, seg);
-            s_map[warp * 32 + 2 * v + i] = make_float4(tA.x, tA.y, tM.x, tM.y);
-            s_fwd[warp * 32 + 2 * v + i] = tB;
-        }
-    }
+    // the maps of the warp's rows before this thread's (pA, pB: the state enters
+    // through them) and after them (fA, fM: mu does)
+    F4 pA, pB, fA, fM, SA = A;
+    warp_suffix<LPR, SS>(SA, M, fA, fM, q, seg);
+    warp_prefix<LPR, SS>(A, B, pA, pB, q, seg);
+    if (q == 0) put_maps(s_map + warp * CB + 4 * v, SA, M);
+    if (q == SS - 1) reinterpret_cast<float4*>(s_fwd)[warp * LPR + v] = as_float4(B);
     mbar_arrive(s_maps);
     named_sync(1, kNT);
 
     // the states of the thread's rows, from the one entering them
     F4 hin;
     {
-        const float4 in4 = reinterpret_cast<const float4*>(s_hin)[warp * 16 + v];
+        const float4 in4 = reinterpret_cast<const float4*>(s_hin)[warp * LPR + v];
         hin.p[0] = make_float2(in4.x, in4.y);
         hin.p[1] = make_float2(in4.z, in4.w);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            if (q == 1) hin.p[i] = apply(fA.p[i], hin.p[i], fC.p[i], seg);
+            hin.p[i] = apply(pA.p[i], hin.p[i], pB.p[i], seg);
             float2 hp = hin.p[i];
             if (rows > 0) {
 #pragma unroll
@@ -842,12 +1007,12 @@ __global__ void __launch_bounds__(kNT, K_BWD_MINB) train_bwd_kernel(const __grid
     // phase 2: the rows from last to first
     F4 mu;
     {
-        const float4 in4 = reinterpret_cast<const float4*>(s_in)[warp * 16 + v];
+        const float4 in4 = reinterpret_cast<const float4*>(s_in)[warp * LPR + v];
         mu.p[0] = make_float2(in4.x, in4.y);
         mu.p[1] = make_float2(in4.z, in4.w);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            if (q == 0) mu.p[i] = apply(fA.p[i], mu.p[i], fC.p[i], seg);
+            mu.p[i] = apply(fA.p[i], mu.p[i], fM.p[i], seg);
         }
     }
     auto phase2 = [&](auto whole) {
@@ -870,8 +1035,8 @@ __global__ void __launch_bounds__(kNT, K_BWD_MINB) train_bwd_kernel(const __grid
                     d[3].p[i] = fmul2(fmul2(gs.p[i], h[j].p[i]), lc.p[i]);
                     d[4].p[i] = fmul2(fmul2(go, ffma2(sc.p[i], h[j].p[i], fmul2(D.p[i], val.p[i]))), lo.p[i]);
                 }
-                put4<T>(stage(3), r, v, d[3]);
-                put4<T>(stage(4), r, v, d[4]);
+                put4<T, CB>(stage(3), r, v, d[3]);
+                put4<T, CB>(stage(4), r, v, d[4]);
             }
             F4 sd, ld;
             if constexpr (FORM == FORM_SSD) gate(0, r, sd, ld);
@@ -893,9 +1058,9 @@ __global__ void __launch_bounds__(kNT, K_BWD_MINB) train_bwd_kernel(const __grid
                     d[2].p[i] = ffma2(dw, sg.p[i], fmul2(D.p[i], gs.p[i]));
                 }
             }
-            put4<T>(stage(0), r, v, d[0]);
-            put4<T>(stage(1), r, v, d[1]);
-            put4<T>(stage(2), r, v, d[2]);
+            put4<T, CB>(stage(0), r, v, d[0]);
+            put4<T, CB>(stage(1), r, v, d[1]);
+            put4<T, CB>(stage(2), r, v, d[2]);
         }
     };
     if (whole) phase2(std::true_type{});
@@ -912,17 +1077,24 @@ __global__ void __launch_bounds__(kNT, K_BWD_MINB) train_bwd_kernel(const __grid
         // of the channel block to come here, the sum over the block's tiles --
         // each in a fixed order, whichever tile is last.
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            dD.p[i] = fadd2(dD.p[i], shfl2(dD.p[i], 16));
-            if (q == 0) s_fwd[warp * 32 + 2 * v + i] = dD.p[i];  // the look-back warp is done with it
-        }
-        named_sync(3, kNW * 32);
-        const int ntile = p.nb * p.nchunks;
-        if (warp == 0) {
-            float2 sum = splat2(0.0f);
+        for (int d = LPR; d < 32; d *= 2)
 #pragma unroll
-            for (int w = 0; w < kNW; ++w) sum = fadd2(sum, s_fwd[w * 32 + lane]);
-            st_pair(p.dpart + (int64_t(tl.b) * p.nchunks + tl.chunk) * p.C, tl.c0 + 2 * lane, p.C, sum);
+            for (int i = 0; i < 2; ++i) dD.p[i] = fadd2(dD.p[i], shfl2(dD.p[i], d));
+        if (q == 0) reinterpret_cast<float4*>(s_fwd)[warp * LPR + v] = as_float4(dD);  // the look-back warp is done with it
+        named_sync(3, kNW * 32);
+        const int ntile = p.nb * p.nchunks, e = K::NC * lane, ch = tl.c0 + e;
+        auto sum_warps = [&](const float* s) {
+            Ch<K::NC> r;
+#pragma unroll
+            for (int k = 0; k < K::NC; ++k) {
+                r.v[k] = 0.0f;
+#pragma unroll
+                for (int w = 0; w < kNW; ++w) r.v[k] += s[w * CB + e + k];
+            }
+            return r;
+        };
+        if (warp == 0) {
+            st_ch(p.dpart + (int64_t(tl.b) * p.nchunks + tl.chunk) * p.C, ch, p.C, sum_warps(s_fwd));
             __threadfence();
             __syncwarp();
             if (lane == 0) *s_last = atomicAdd(&p.dcount[tl.cblk], 1u) == static_cast<uint32_t>(ntile) - 1u;
@@ -930,18 +1102,17 @@ __global__ void __launch_bounds__(kNT, K_BWD_MINB) train_bwd_kernel(const __grid
         named_sync(3, kNW * 32);
         if (*s_last != 0u) {
             __threadfence();
-            const int ch = tl.c0 + 2 * lane;
-            float2 sum = splat2(0.0f);
-#pragma unroll 8
-            for (int i = warp; i < ntile; i += kNW) sum = fadd2(sum, ld_pair_cg(p.dpart + int64_t(i) * p.C, ch, p.C));
-            s_hin[warp * 32 + lane] = sum;
-            named_sync(3, kNW * 32);
-            if (warp == 0) {
-                sum = splat2(0.0f);
 #pragma unroll
-                for (int w = 0; w < kNW; ++w) sum = fadd2(sum, s_hin[w * 32 + lane]);
-                st_pair(p.grad_d, ch, p.C, sum);
+            for (int k = 0; k < K::NC; ++k) {
+                float sum = 0.0f;
+                if (ch + k < p.C) {
+#pragma unroll 8
+                    for (int i = warp; i < ntile; i += kNW) sum += __ldcg(p.dpart + int64_t(i) * p.C + ch + k);
+                }
+                s_hin[warp * CB + e + k] = sum;
             }
+            named_sync(3, kNW * 32);
+            if (warp == 0) st_ch(p.grad_d, ch, p.C, sum_warps(s_hin));
         }
     }
     if (lane == 0 && rows > 0) tma_store_drain();
@@ -961,24 +1132,32 @@ int launch(Kern kern, int smem, std::atomic<uint64_t>& done, const TrainParams& 
     return e == cudaSuccess ? NEED_OK : cuda_fail(e, "training scan launch");
 }
 
-template <int FORM, typename T, bool CK, int DT, bool BWD>
+template <int FORM, typename T, bool CK, int DT, int CB, bool BWD>
 int run_cfg(const TrainParams& P, cudaStream_t s) {
     static std::atomic<uint64_t> done{0};
-    constexpr int smem = TrainCfg<FORM, T, CK, DT, BWD>::SMEM;
-    if constexpr (BWD) return launch(train_bwd_kernel<FORM, T, CK, DT>, smem, done, P, s);
-    else return launch(train_fwd_kernel<FORM, T, CK, DT>, smem, done, P, s);
+    constexpr int smem = TrainCfg<FORM, T, CK, DT, CB, BWD>::SMEM;
+    if constexpr (BWD) return launch(train_bwd_kernel<FORM, T, CK, DT, CB>, smem, done, P, s);
+    else return launch(train_fwd_kernel<FORM, T, CK, DT, CB>, smem, done, P, s);
 }
 
 template <bool BWD>
-int run(const need_scan_train_args* a, const TrainParams& P, cudaStream_t s) {
+int run(const need_scan_train_args* a, const TrainParams& P, bool narrow, cudaStream_t s) {
     auto form = [&](auto tag) {
         using T = decltype(tag);
         auto go = [&](auto ck) {
             constexpr bool CK = decltype(ck)::value;
-            if (a->form == NEED_FORM_GATED) return run_cfg<FORM_GATED, T, CK, 0, BWD>(P, s);
+            auto width = [&](auto form, auto dt) {
+                constexpr int F = decltype(form)::value, DT = decltype(dt)::value;
+                if constexpr (!CK)
+                    if (narrow) return run_cfg<F, T, CK, DT, 32, BWD>(P, s);
+                return run_cfg<F, T, CK, DT, 64, BWD>(P, s);
+            };
+            constexpr std::integral_constant<int, 0> any{};
+            if (a->form == NEED_FORM_GATED) return width(std::integral_constant<int, FORM_GATED>{}, any);
+            constexpr std::integral_constant<int, FORM_SSD> ssd{};
             // steps of at most 1/4 (the block's are at most 0.2): e^-r by its series, see exp_neg_small
-            if (a->dt_max <= 0.25) return run_cfg<FORM_SSD, T, CK, 1, BWD>(P, s);
-            return run_cfg<FORM_SSD, T, CK, 0, BWD>(P, s);
+            if (a->dt_max <= 0.25) return width(ssd, std::integral_constant<int, 1>{});
+            return width(ssd, any);
         };
         return a->checkpoint != 0 ? go(std::true_type{}) : go(std::false_type{});
     };
@@ -988,12 +1167,18 @@ int run(const need_scan_train_args* a, const TrainParams& P, cudaStream_t s) {
 }
 
 struct Geom {
-    int64_t L, ncb, nchains, nchunks, ntiles;
+    int64_t L, CB, ncb, nchains, nchunks, ntiles;
 };
-Geom geom(int dtype, bool ck, bool bwd, int64_t nb, int64_t T, int64_t C) {
+// Channels per tile.  64 where the call has enough chains to fill the device;
+// 32 (tiles twice as long) where it has not: then fewer tiles of one chain are in
+// flight and wait for each other's carries (bf16, us, 64 / 32 channels: SSD
+// 1x16384x832 175 / 142, 8x2048x832 135 / 130, gated 16x4096x1024 341 / 355).
+// The 8-bit forms keep the 64 that share a scale.
+Geom geom(bool ck, int64_t nb, int64_t T, int64_t C) {
     Geom g;
-    g.L = tile_tokens(dtype_bytes(dtype), ck, bwd);
-    g.ncb = (C + kCB - 1) / kCB;
+    g.CB = !ck && nb * ((C + 63) / 64) < 192 ? 32 : 64;
+    g.L = kTileElems / g.CB;
+    g.ncb = (C + g.CB - 1) / g.CB;
     g.nchains = nb * g.ncb;
     g.nchunks = (T + g.L - 1) / g.L;
     g.ntiles = g.nchains * g.nchunks;
@@ -1001,7 +1186,7 @@ Geom geom(int dtype, bool ck, bool bwd, int64_t nb, int64_t T, int64_t C) {
 }
 // The workspace: header, look-back records and (SSD backward) the counters,
 // which the call clears, then the partial sums of the gradient of D.
-size_t rec_bytes(const Geom& g) { return g.nchunks > 1 ? size_t(g.ntiles) * kTileRecBytes : 0; }
+size_t rec_bytes(const Geom& g) { return g.nchunks > 1 ? size_t(g.ntiles) * size_t(g.CB) * kRecBytes : 0; }
 size_t clear_bytes(const Geom& g, bool dpart) {
     return kHdrBytes + rec_bytes(g) + (dpart ? (size_t(g.ncb) * 4 + 15) / 16 * 16 : 0);
 }
@@ -1017,11 +1202,11 @@ bool tma_rows(const void* ptr, int64_t sb, int64_t st, int es, int64_t nb, int64
 
 // Such a tensor (element strides) as a 3-D tensor map with boxes of one warp's rows.
 int encode(CUtensorMap* tm, const void* ptr, int64_t sb, int64_t st, int es, CUtensorMapDataType ty, int64_t nb,
-           int64_t T, int64_t C, int64_t L, const char* what) {
+           int64_t T, int64_t C, const Geom& g, const char* what) {
     const cuuint64_t row = (C * es + 15) / 16 * 16;  // a size-1 dim's stride is not used
     const cuuint64_t gs[2] = {T > 1 ? cuuint64_t(st * es) : row, nb > 1 ? cuuint64_t(sb * es) : row};
     const cuuint64_t dims[3] = {cuuint64_t(C), cuuint64_t(T), cuuint64_t(nb)};
-    const cuuint32_t box[3] = {kCB, cuuint32_t(L / kNW), 1}, estr[3] = {1, 1, 1};
+    const cuuint32_t box[3] = {cuuint32_t(g.CB), cuuint32_t(g.L / kNW), 1}, estr[3] = {1, 1, 1};
     auto fn = encode_fn();
     if (fn == nullptr) return fail(NEED_ERR_CUDA, "cuTensorMapEncodeTiled entry point unavailable");
     const CUresult r = fn(tm, ty, 3, const_cast<void*>(ptr), dims, gs, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
@@ -1049,7 +1234,7 @@ int prepare(const need_scan_train_args* a, bool bwd, TrainParams* P, Geom* g) {
     const int es = dtype_bytes(a->dtype);
     if (a->nb > INT32_MAX / 8 || a->nb * ((a->T + kSpan - 1) / kSpan) > INT32_MAX / 2 || a->T > INT32_MAX / 2 || a->C > INT32_MAX / 2)
         return fail(NEED_ERR_UNSUPPORTED, "sizes exceed the 32-bit index range");
-    *g = geom(a->dtype, a->checkpoint != 0, bwd, a->nb, a->T, a->C);
+    *g = geom(a->checkpoint != 0, a->nb, a->T, a->C);
     if (g->nchains > INT32_MAX || g->ntiles > INT32_MAX)
         return fail(NEED_ERR_UNSUPPORTED, "too many tiles (%lld)", (long long)g->ntiles);
     const int nin = a->form == NEED_FORM_GATED ? 3 : 5;
@@ -1091,17 +1276,17 @@ int prepare(const need_scan_train_args* a, bool bwd, TrainParams* P, Geom* g) {
     const auto ty = map_type(a->dtype);
     auto stream = [&](int k, const need_view& v, const char* name) {
         if (tma_rows(v.ptr, v.stride_b, v.stride_t, es, a->nb, a->T))
-            return encode(&P->tm[k], v.ptr, v.stride_b, v.stride_t, es, ty, a->nb, a->T, a->C, g->L, name);
+            return encode(&P->tm[k], v.ptr, v.stride_b, v.stride_t, es, ty, a->nb, a->T, a->C, *g, name);
         P->plain |= 1u << k;
         P->src[k] = v.ptr, P->ssb[k] = v.stride_b, P->sst[k] = v.stride_t;
         return int(NEED_OK);
     };
     for (int k = 0; k < nin; ++k) {
-        const int64_t pitch = g->ncb * kCB;
+        const int64_t pitch = (a->C + kGroup - 1) / kGroup * kGroup;
         // the 8-bit values of every stream as one [nin * nb, T, ncb * 64] tensor: the
         // kernel adds its stream's first sequence to b
         const int rc = stored ? encode(&P->tm[k], a->ckpt_values, a->T * pitch, pitch, 1, CU_TENSOR_MAP_DATA_TYPE_UINT8,
-                                       nin * a->nb, a->T, pitch, g->L, "ckpt_values")
+                                       nin * a->nb, a->T, pitch, *g, "ckpt_values")
                               : stream(k, a->in[k], names[k]);
         if (rc) return rc;
     }
@@ -1109,8 +1294,8 @@ int prepare(const need_scan_train_args* a, bool bwd, TrainParams* P, Geom* g) {
         if (int rc = stream(nin, a->gout, names[5])) return rc;
     for (int k = 0; k < (bwd ? nin : 1); ++k)
         if (int rc = bwd ? encode(&P->tmo[k], a->grad[k], a->grad_stride_b, a->grad_stride_t, es, ty, a->nb, a->T, a->C,
-                                  g->L, "grad")
-                         : encode(&P->tmo[0], a->out, a->out_stride_b, a->out_stride_t, es, ty, a->nb, a->T, a->C, g->L, "out"))
+                                  *g, "grad")
+                         : encode(&P->tmo[0], a->out, a->out_stride_b, a->out_stride_t, es, ty, a->nb, a->T, a->C, *g, "out"))
             return rc;
     P->nb = int32_t(a->nb);
     P->T = int32_t(a->T);
@@ -1118,9 +1303,10 @@ int prepare(const need_scan_train_args* a, bool bwd, TrainParams* P, Geom* g) {
     P->ncb = int32_t(g->ncb);
     P->nchains = int32_t(g->nchains);
     P->nchunks = int32_t(g->nchunks);
+    P->ngroups = int32_t((a->C + kGroup - 1) / kGroup);
     P->nspans = int32_t((a->T + kSpan - 1) / kSpan);
     // few chains have many of their tiles in flight at once: look further back
-    P->depth = g->nchains < 148 ? kDeep : 3;
+    P->depth = g->nchains < 64 ? kDeep : kNear;
     P->dskip = a->d_skip;
     P->dt_min = static_cast<float>(a->dt_min);
     P->dt_scale = static_cast<float>(a->dt_max - a->dt_min);
@@ -1136,8 +1322,8 @@ int prepare(const need_scan_train_args* a, bool bwd, TrainParams* P, Geom* g) {
     P->grad_h0 = a->grad_h0;
     unsigned char* ws = static_cast<unsigned char*>(a->workspace);
     P->hdr = reinterpret_cast<uint32_t*>(ws);
-    P->agg = reinterpret_cast<ulonglong2*>(ws + kHdrBytes);
-    P->incl = reinterpret_cast<unsigned long long*>(ws + kHdrBytes + size_t(g->ntiles) * kCB * 8);
+    P->agg = reinterpret_cast<unsigned long long*>(ws + kHdrBytes);
+    P->incl = reinterpret_cast<uint32_t*>(ws + kHdrBytes + size_t(g->ntiles) * size_t(g->CB) * 8);
     P->dcount = reinterpret_cast<uint32_t*>(ws + kHdrBytes + rec_bytes(*g));
     P->dpart = reinterpret_cast<float*>(ws + clear_bytes(*g, dpart));
     P->grad_d = a->grad_d;
@@ -1156,12 +1342,12 @@ extern "C" {
 
 int64_t need_scan_train_chunk_len(void) { return kSpan; }
 
-int64_t need_scan_train_group(void) { return kCB; }
+int64_t need_scan_train_group(void) { return kGroup; }
 
-size_t need_scan_train_workspace_size(int32_t form, int32_t dtype, int32_t checkpoint, int32_t backward, int64_t nb,
-                                      int64_t T, int64_t C) {
-    if (nb < 1 || T < 1 || C < 1 || !dtype_ok(dtype)) return kHdrBytes;
-    return ws_size(geom(dtype, checkpoint != 0, backward != 0, nb, T, C), nb, C, backward != 0 && form == NEED_FORM_SSD);
+size_t need_scan_train_workspace_size(int32_t form, int32_t checkpoint, int32_t backward, int64_t nb, int64_t T,
+                                      int64_t C) {
+    if (nb < 1 || T < 1 || C < 1) return kHdrBytes;
+    return ws_size(geom(checkpoint != 0, nb, T, C), nb, C, backward != 0 && form == NEED_FORM_SSD);
 }
 
 int need_scan_train_forward(const need_scan_train_args* args, need_stream_t stream) {
@@ -1169,7 +1355,7 @@ int need_scan_train_forward(const need_scan_train_args* args, need_stream_t stre
     Geom g;
     if (int rc = prepare(args, false, &P, &g)) return rc;
     if (int rc = clear_records(args, g, false, stream)) return rc;
-    if (int rc = run<false>(args, P, stream)) return rc;
+    if (int rc = run<false>(args, P, g.CB == 32, stream)) return rc;
     return ok();
 }
 
@@ -1178,7 +1364,7 @@ int need_scan_train_backward(const need_scan_train_args* args, need_stream_t str
     Geom g;
     if (int rc = prepare(args, true, &P, &g)) return rc;
     if (int rc = clear_records(args, g, args->form == NEED_FORM_SSD, stream)) return rc;
-    if (int rc = run<true>(args, P, stream)) return rc;
+    if (int rc = run<true>(args, P, g.CB == 32, stream)) return rc;
     return ok();
 }
 
