@@ -6,8 +6,8 @@
 //   dw[K-1-d] = sum over b, t of dv_t u_{t-d};  dbias = sum of dv
 //
 // All in fp32, rounded once on the way out.  Bound by HBM (4 B per 16-bit
-// element forward, 6 B backward): a thread walks kTok tokens of 4 channels in
-// groups of kGroupRows rows, the next group's loads in flight while it works on
+// element forward, 6 B backward): a thread walks kTok tokens of 4 channels
+// (backward 2) in groups of kGroupRows rows, the next group's loads in flight while it works on
 // one; the last K-1 inputs, and backward the K-1 unfinished du, stay in
 // registers, and v is computed again rather than kept.  The backward reads the
 // K-1 rows behind its tokens a second time (L2) for the dv they need.  A thread's
@@ -15,6 +15,10 @@
 // memory, and column_sums adds the blocks' rows in a fixed order.  Rows that are
 // not aligned to 4 elements, and the channels of a last odd group, are read and
 // written one by one.
+#include <string.h>
+
+#include <type_traits>
+
 #include "host_common.h"
 #include "need_scan.h"
 #include "scan_kernel.cuh"
@@ -25,15 +29,14 @@ using namespace need;
 namespace {
 
 constexpr int kMaxTaps = 4;
-#ifndef K_CTOK
-#define K_CTOK 32
-#endif
-#ifndef K_CMINB
-#define K_CMINB 1
-#endif
-constexpr int kTok = K_CTOK;    // tokens per thread
+constexpr int kTok = 32;        // tokens per thread
 constexpr int kGroupRows = 4;   // rows loaded together
 constexpr int kRanges = 4;      // token ranges per block (threadIdx.y)
+// Channel pairs per thread.  The backward keeps du, the sums and a second stream
+// besides: two pairs took 182 registers, 2 blocks per SM and 44 us (29 us with one) at
+// 8x2048x832 bf16, K = 3.
+template <bool BWD>
+constexpr int kPairs = BWD ? 1 : 2;
 
 struct ConvTrainParams {
     const void* u;
@@ -47,75 +50,76 @@ struct ConvTrainParams {
     void* out;    // y, or du
     int64_t osb, ost;
     float* part;  // [nb * ntb, C * (K + 1)]
-    int32_t nb, T, C, ncg, ntb;      // channel groups (of 128) and token blocks
-    int32_t uvec, gvec, ovec;        // rows aligned to 4 elements
+    int32_t nb, T, C, ncg, ntb;      // channel groups (of 32 threads) and token blocks
+    int32_t uvec, gvec, ovec;        // rows aligned to a thread's channels
 };
 
-// Four channels as loaded: packed, so that a row in flight costs few registers.
-template <typename T>
-struct Raw4 {
-    typename Ops<T>::P h[2];
+// 2 NP channels as loaded: packed, so that a row in flight costs few registers.
+template <typename T, int NP>
+struct Raw {
+    typename Ops<T>::P h[NP];
 };
-// n: how many of the four lie inside C.
-template <typename T>
-__device__ __forceinline__ Raw4<T> load4(const T* p, bool vec, int n) {
-    Raw4<T> r;
-    if (vec && n >= 4) {
-        if constexpr (Ops<T>::BYTES == 4) {
-            const float4 v = *reinterpret_cast<const float4*>(p);
-            r.h[0] = make_float2(v.x, v.y);
-            r.h[1] = make_float2(v.z, v.w);
-        } else {
-            const uint2 v = *reinterpret_cast<const uint2*>(p);
-            r.h[0] = *reinterpret_cast<const typename Ops<T>::P*>(&v.x);
-            r.h[1] = *reinterpret_cast<const typename Ops<T>::P*>(&v.y);
-        }
+// n: how many of the channels lie inside C.
+template <typename T, int NP>
+__device__ __forceinline__ Raw<T, NP> load_row(const T* p, bool vec, int n) {
+    using V = typename std::conditional<sizeof(Raw<T, NP>) == 16, uint4,
+                                        typename std::conditional<sizeof(Raw<T, NP>) == 8, uint2, uint32_t>::type>::type;
+    Raw<T, NP> r;
+    if (vec && n >= 2 * NP) {
+        const V v = *reinterpret_cast<const V*>(p);
+        memcpy(&r, &v, sizeof(v));
     } else {
-        float f[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) f[e] = e < n ? to_f(p[e]) : 0.0f;
-        r.h[0] = Ops<T>::pack(f[0], f[1]);
-        r.h[1] = Ops<T>::pack(f[2], f[3]);
+        for (int e = 0; e < NP; ++e)
+            r.h[e] = Ops<T>::pack(2 * e < n ? to_f(p[2 * e]) : 0.0f, 2 * e + 1 < n ? to_f(p[2 * e + 1]) : 0.0f);
     }
     return r;
 }
-template <typename T>
-__device__ __forceinline__ void store4(T* p, bool vec, int n, const float2 (&f)[2]) {
-    const typename Ops<T>::P h[2] = {Ops<T>::pack(f[0].x, f[0].y), Ops<T>::pack(f[1].x, f[1].y)};
-    if (vec && n >= 4) {
-        if constexpr (Ops<T>::BYTES == 4) *reinterpret_cast<float4*>(p) = *reinterpret_cast<const float4*>(h);
-        else *reinterpret_cast<uint2*>(p) = *reinterpret_cast<const uint2*>(h);
+template <typename T, int NP>
+__device__ __forceinline__ void store_row(T* p, bool vec, int n, const float2 (&f)[NP]) {
+    using V = typename std::conditional<sizeof(Raw<T, NP>) == 16, uint4,
+                                        typename std::conditional<sizeof(Raw<T, NP>) == 8, uint2, uint32_t>::type>::type;
+    Raw<T, NP> r;
+#pragma unroll
+    for (int e = 0; e < NP; ++e) r.h[e] = Ops<T>::pack(f[e].x, f[e].y);
+    if (vec && n >= 2 * NP) {
+        V v;
+        memcpy(&v, &r, sizeof(v));
+        *reinterpret_cast<V*>(p) = v;
     } else {
-        const T* e = reinterpret_cast<const T*>(h);
-        for (int i = 0; i < 4 && i < n; ++i) p[i] = e[i];
+        const T* e = reinterpret_cast<const T*>(&r);
+        for (int i = 0; i < 2 * NP && i < n; ++i) p[i] = e[i];
     }
 }
 
 template <typename T, int K, bool BWD, bool SEG>
-__global__ void __launch_bounds__(32 * kRanges, K_CMINB) conv_train_kernel(const ConvTrainParams p) {
+__global__ void __launch_bounds__(32 * kRanges) conv_train_kernel(const ConvTrainParams p) {
     constexpr int G = kGroupRows, W = K - 1;  // W: tokens a tap reaches back
+    constexpr int NP = kPairs<BWD>, NC = 2 * NP;
     const int cg = blockIdx.x % p.ncg;
     const int rest = blockIdx.x / p.ncg;
     const int tb = rest % p.ntb, b = rest / p.ntb;
-    const int c0 = cg * 128 + threadIdx.x * 4, n = p.C - c0;
+    const int c0 = (cg * 32 + threadIdx.x) * NC, n = p.C - c0;
     const int64_t tfirst = (int64_t(tb) * kRanges + threadIdx.y) * kTok;
     const bool live = n > 0 && tfirst < p.T;
     const int t0 = live ? static_cast<int>(tfirst) : 0;
     const int t1 = live ? min(t0 + kTok, p.T) : 0;  // this thread's tokens
 
-    float2 sum[K + 1][2];  // BWD: dw by distance back, then dbias
+    float2 sum[K + 1][NP];  // BWD: dw by distance back, then dbias
 #pragma unroll
-    for (int d = 0; d <= K; ++d) sum[d][0] = sum[d][1] = splat2(0.0f);
+    for (int d = 0; d <= K; ++d)
+#pragma unroll
+        for (int e = 0; e < NP; ++e) sum[d][e] = splat2(0.0f);
 
     if (live) {
         const T* u = static_cast<const T*>(p.u) + b * p.usb + c0;
         const T* go = BWD ? static_cast<const T*>(p.gout) + b * p.gsb + c0 : nullptr;
         T* out = static_cast<T*>(p.out) + b * p.osb + c0;
         const uint8_t* seg = SEG ? p.seg + b * p.sgb : nullptr;
-        float2 w[K][2], bs[2];  // w[d]: the tap that multiplies the input d tokens back
+        float2 w[K][NP], bs[NP];  // w[d]: the tap that multiplies the input d tokens back
         auto param = [&](const float* q, int64_t stride, int e) { return e < n ? q[int64_t(c0 + e) * stride] : 0.0f; };
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < NP; ++i) {
             bs[i] = p.bias != nullptr ? make_float2(param(p.bias, 1, 2 * i), param(p.bias, 1, 2 * i + 1)) : splat2(0.0f);
 #pragma unroll
             for (int d = 0; d < K; ++d)
@@ -124,57 +128,67 @@ __global__ void __launch_bounds__(32 * kRanges, K_CMINB) conv_train_kernel(const
         // x[W + i]: the input of the group's row i; x[0 .. W-1]: the W rows before.
         // du likewise: rows W back are finished by the group.  starts, bit W + i: row i
         // starts a segment.
-        float2 x[W + G][2], du[W + G][2];
+        float2 x[W + G][NP], du[W + G][NP];
         uint32_t starts = 0;
 #pragma unroll
         for (int d = 0; d < W; ++d) {
-            x[d][0] = x[d][1] = du[d][0] = du[d][1] = splat2(0.0f);
+#pragma unroll
+            for (int e = 0; e < NP; ++e) x[d][e] = du[d][e] = splat2(0.0f);
             const int t = t0 - W + d;
             if (t >= 0) {
-                const Raw4<T> r = load4<T>(u + int64_t(t) * p.ust, p.uvec != 0, n);
-                x[d][0] = widen(r.h[0]);
-                x[d][1] = widen(r.h[1]);
+                const Raw<T, NP> r = load_row<T, NP>(u + int64_t(t) * p.ust, p.uvec != 0, n);
+#pragma unroll
+                for (int e = 0; e < NP; ++e) x[d][e] = widen(r.h[e]);
                 if (SEG && seg[int64_t(t) * p.sgt] != 0) starts |= 1u << d;
             }
         }
-        Raw4<T> nu[G], ng[G];  // the next group, in flight
+        Raw<T, NP> nu[G], ng[G];  // the next group, in flight
         uint32_t nst = 0;
-        auto fetch = [&](int tg) {
+        const int tend = BWD ? t1 + W : t1, tin = min(tend, p.T);
+        const bool vec = p.uvec != 0 && p.ovec != 0 && (!BWD || p.gvec != 0) && n >= NC;
+        const T* fu = u + int64_t(t0) * p.ust;  // the next group's first row
+        const T* fg = BWD ? go + int64_t(t0) * p.gst : nullptr;
+        // ALL: every row of the group is one of [t0, tin) and aligned
+        auto fetch = [&](int tg, auto all) {
             nst = 0;
 #pragma unroll
             for (int i = 0; i < G; ++i) {
-                const int t = tg + i;
-                const bool in = t < p.T && t < (BWD ? t1 + W : t1);
-                nu[i].h[0] = nu[i].h[1] = Ops<T>::zero();
-                if (BWD) ng[i].h[0] = ng[i].h[1] = Ops<T>::zero();
-                if (in) {
-                    nu[i] = load4<T>(u + int64_t(t) * p.ust, p.uvec != 0, n);
-                    if constexpr (BWD) ng[i] = load4<T>(go + int64_t(t) * p.gst, p.gvec != 0, n);
-                    if (SEG && seg[int64_t(t) * p.sgt] != 0) nst |= 1u << (W + i);
+                constexpr bool ALL = decltype(all)::value;
+                if (ALL || tg + i < tin) {
+                    nu[i] = load_row<T, NP>(fu + i * p.ust, ALL || p.uvec != 0, ALL ? NC : n);
+                    if constexpr (BWD) ng[i] = load_row<T, NP>(fg + i * p.gst, ALL || p.gvec != 0, ALL ? NC : n);
+                    if (SEG && seg[int64_t(tg + i) * p.sgt] != 0) nst |= 1u << (W + i);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < NP; ++e) nu[i].h[e] = ng[i].h[e] = Ops<T>::zero();
                 }
             }
+            fu += G * p.ust;
+            if (BWD) fg += G * p.gst;
         };
-        fetch(t0);
-        const int tend = BWD ? t1 + W : t1;
-        for (int tg = t0; tg < tend; tg += G) {
-            Raw4<T> g[G];
+        auto next = [&](int tg) {
+            if (vec && tg + G <= tin) fetch(tg, std::true_type{});
+            else fetch(tg, std::false_type{});
+        };
+        T* orow = out + int64_t(t0 - (BWD ? W : 0)) * p.ost;  // the row the group finishes first
+        auto group = [&](int tg, auto all) {
+            constexpr bool ALL = decltype(all)::value;  // all rows are this thread's, and so are those it finishes
+            Raw<T, NP> g[G];
 #pragma unroll
             for (int i = 0; i < G; ++i) {
-                x[W + i][0] = widen(nu[i].h[0]);
-                x[W + i][1] = widen(nu[i].h[1]);
+#pragma unroll
+                for (int e = 0; e < NP; ++e) x[W + i][e] = widen(nu[i].h[e]), du[W + i][e] = splat2(0.0f);
                 if (BWD) g[i] = ng[i];
-                du[W + i][0] = du[W + i][1] = splat2(0.0f);
             }
             starts |= nst;
-            if (tg + G < tend) fetch(tg + G);
+            if (tg + G < tend) next(tg + G);
 #pragma unroll
             for (int i = 0; i < G; ++i) {
-                const int t = tg + i;
-                // the input d back is in reach when none of the rows after it, up to t, starts a segment
+                // the input d back is in reach when none of the rows after it, up to this one, starts a segment
                 auto reach = [&](int d) { return !SEG || ((starts >> (W + i - d + 1)) & ((1u << d) - 1u)) == 0u; };
-                float2 y[2];
+                float2 y[NP];
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
+                for (int e = 0; e < NP; ++e) {
                     float2 v = bs[e];
 #pragma unroll
                     for (int d = W; d >= 0; --d)
@@ -188,7 +202,7 @@ __global__ void __launch_bounds__(32 * kRanges, K_CMINB) conv_train_kernel(const
 #pragma unroll
                         for (int d = 0; d < K; ++d)
                             if (reach(d)) du[W + i - d][e] = ffma2(w[d][e], dv, du[W + i - d][e]);
-                        if (t < t1) {
+                        if (ALL || tg + i < t1) {
                             sum[K][e] = fadd2(sum[K][e], dv);
 #pragma unroll
                             for (int d = 0; d < K; ++d)
@@ -197,42 +211,48 @@ __global__ void __launch_bounds__(32 * kRanges, K_CMINB) conv_train_kernel(const
                     }
                 }
                 if constexpr (!BWD)
-                    if (t < t1) store4<T>(out + int64_t(t) * p.ost, p.ovec != 0, n, y);
+                    if (ALL || tg + i < t1)
+                        store_row<T, NP>(orow + i * p.ost, ALL || p.ovec != 0, ALL ? NC : n, y);
             }
             if constexpr (BWD) {
 #pragma unroll
-                for (int i = 0; i < G; ++i) {  // these rows have met every dv they feed
-                    const int t = tg - W + i;
-                    if (t >= t0 && t < t1) store4<T>(out + int64_t(t) * p.ost, p.ovec != 0, n, du[i]);
-                }
+                for (int i = 0; i < G; ++i)  // these rows have met every dv they feed
+                    if (ALL || (tg - W + i >= t0 && tg - W + i < t1))
+                        store_row<T, NP>(orow + i * p.ost, ALL || p.ovec != 0, ALL ? NC : n, du[i]);
             }
+            orow += G * p.ost;
 #pragma unroll
             for (int d = 0; d < W; ++d)
 #pragma unroll
-                for (int e = 0; e < 2; ++e) x[d][e] = x[G + d][e], du[d][e] = du[G + d][e];
+                for (int e = 0; e < NP; ++e) x[d][e] = x[G + d][e], du[d][e] = du[G + d][e];
             starts >>= G;
+        };
+        next(t0);
+        for (int tg = t0; tg < tend; tg += G) {
+            if (vec && tg + G <= t1 && (!BWD || tg - W >= t0)) group(tg, std::true_type{});
+            else group(tg, std::false_type{});
         }
         if constexpr (BWD && W > 0) {  // rows the last group left behind
 #pragma unroll
             for (int d = 0; d < W; ++d) {
                 const int t = t0 + (tend - t0 + G - 1) / G * G - W + d;
-                if (t >= t0 && t < t1) store4<T>(out + int64_t(t) * p.ost, p.ovec != 0, n, du[d]);
+                if (t >= t0 && t < t1) store_row<T, NP>(out + int64_t(t) * p.ost, p.ovec != 0, n, du[d]);
             }
         }
     }
     if constexpr (BWD) {
-        __shared__ float2 s_sum[kRanges][(K + 1) * 2][32];
+        __shared__ float2 s_sum[kRanges][(K + 1) * NP][32];
 #pragma unroll
         for (int d = 0; d <= K; ++d)
 #pragma unroll
-            for (int e = 0; e < 2; ++e) s_sum[threadIdx.y][2 * d + e][threadIdx.x] = sum[d][e];
+            for (int e = 0; e < NP; ++e) s_sum[threadIdx.y][NP * d + e][threadIdx.x] = sum[d][e];
         __syncthreads();
         float* part = p.part + (int64_t(b) * p.ntb + tb) * int64_t(p.C) * (K + 1);
-        for (int k = threadIdx.y; k < (K + 1) * 2; k += kRanges) {
+        for (int k = threadIdx.y; k < (K + 1) * NP; k += kRanges) {
             float2 t = splat2(0.0f);
 #pragma unroll
             for (int r = 0; r < kRanges; ++r) t = fadd2(t, s_sum[r][k][threadIdx.x]);
-            const int d = k / 2, ch = c0 + 2 * (k & 1), j = d < K ? W - d : K;
+            const int d = k / NP, ch = c0 + 2 * (k % NP), j = d < K ? W - d : K;
             if (ch < p.C) part[int64_t(ch) * (K + 1) + j] = t.x;
             if (ch + 1 < p.C) part[int64_t(ch + 1) * (K + 1) + j] = t.y;
         }
@@ -262,15 +282,16 @@ int conv_train(const need_conv_train_args* a, cudaStream_t s) {
         return fail(NEED_ERR_UNSUPPORTED, "conv: sizes too large");
     if (a->u == nullptr) return fail(NEED_ERR_INVALID, "conv: u is null");
     if (a->weight == nullptr) return fail(NEED_ERR_INVALID, "conv: weight is null");
-    const uintptr_t al = 4 * dtype_bytes(a->dtype);
+    constexpr int NC = 2 * kPairs<BWD>;
+    const uintptr_t al = NC * dtype_bytes(a->dtype);
     auto vec = [&](const void* q, int64_t sb, int64_t st) {
-        return reinterpret_cast<uintptr_t>(q) % al == 0 && (a->T == 1 || st % 4 == 0) && (a->nb == 1 || sb % 4 == 0);
+        return reinterpret_cast<uintptr_t>(q) % al == 0 && (a->T == 1 || st % NC == 0) && (a->nb == 1 || sb % NC == 0);
     };
     ConvTrainParams p{};
     p.u = a->u, p.usb = a->u_stride_b, p.ust = a->u_stride_t, p.w = a->weight, p.bias = a->bias;
     p.seg = a->seg_start, p.sgb = a->seg_stride_b, p.sgt = a->seg_stride_t;
     p.nb = int32_t(a->nb), p.T = int32_t(a->T), p.C = int32_t(a->C);
-    p.ncg = int32_t((a->C + 127) / 128), p.ntb = int32_t(token_blocks(a->T));
+    p.ncg = int32_t((a->C + 64 * kPairs<BWD> - 1) / (64 * kPairs<BWD>)), p.ntb = int32_t(token_blocks(a->T));
     const int64_t blocks = int64_t(p.ncg) * p.ntb * a->nb;
     if (int64_t(p.ncg) * p.ntb > INT32_MAX || blocks > INT32_MAX) return fail(NEED_ERR_UNSUPPORTED, "conv: sizes too large");
     p.out = BWD ? a->grad_u : a->out;
