@@ -68,7 +68,13 @@ constexpr int kGroup = 64;             // channels of a token that share an 8-bi
 constexpr int kSpan = 64;              // tokens between kept states
 constexpr int kNW = 8;                 // row warps
 constexpr int kNT = (kNW + 1) * 32;    // threads: the row warps and the look-back warp
-constexpr int kTileElems = 4096;       // tokens x channels per tile
+// Tokens x channels per tile.  The wide GATED forward, with little to keep per
+// element, takes tiles twice as long (16x4096x1024 bf16: 112 us against 129 us);
+// the others lose more residents than they save (SSD 8x2048x832 backward 102
+// against 83 us).
+__host__ __device__ constexpr int tile_elems(int form, bool ck, int cb, bool bwd) {
+    return form == FORM_GATED && !ck && cb == 64 && !bwd ? 8192 : 4096;
+}
 constexpr int kNear = 3, kDeep = 5;    // tile maps composed before an inclusive carry
 constexpr int kHdrBytes = WS_HDR_WORDS * 4;
 constexpr int kRecBytes = 12;           // per tile and channel: (A, B) and the inclusive carry
@@ -300,7 +306,7 @@ struct TrainCfg {
     static constexpr int NIN = FORM == FORM_GATED ? 3 : 5;
     static constexpr int IN_BYTES = (BWD && CK) ? 1 : Ops<T>::BYTES;  // per streamed input element
     static constexpr int CB = CB_, NC = CB / 32;                     // channels; of a look-back lane
-    static constexpr int L = kTileElems / CB, R = L / kNW;           // tokens; rows per warp
+    static constexpr int L = tile_elems(FORM, CK, CB, BWD) / CB, R = L / kNW;           // tokens; rows per warp
     static_assert(CB == 32 || CB == 64, "32 or 64 channels per tile");
     static_assert(BWD || !CK || CB == kGroup, "the 8-bit forward sees whole groups");
     static constexpr int LPR = CB / 4, SS = 32 / LPR, RT = R / SS;   // lanes per row, row groups, rows per thread
@@ -319,9 +325,9 @@ struct TrainCfg {
     static constexpr int SMEM = OFF_BAR + (kNW + 1) * 8 + 8;
     // CTAs per SM that registers are planned for (16 bit: 56 to 96 registers).  Most of
     // a tile's time is latency -- its loads 2 us, the carry 1 us -- so residents count for
-    // more than a few spilled registers: SSD 8x2048x832 forward 42 us at 4, 44 at 3;
-    // backward 87 at 3, 100 at 2.
-    static constexpr int MINB = Ops<T>::BYTES == 4 ? 2 : BWD ? (CK ? 2 : 3) : (CK ? 3 : 4);
+    // more than a few spilled registers: SSD 8x2048x832 forward 39 us at 4, 44 at 3;
+    // backward 83 at 3, 100 at 2.
+    static constexpr int MINB = Ops<T>::BYTES == 4 ? 2 : BWD ? (CK ? 2 : 3) : (CK || L * CB > 4096 ? 3 : 4);
 };
 
 // ------------------------------------------------------------------ look-back
@@ -492,11 +498,19 @@ template <typename T, int R, int CB>
 __device__ __forceinline__ void plain_rows(const TrainParams& p, const Tile& tl, int k, unsigned char* slot, int wr0,
                                            int rows, int lane) {
     const T* src = static_cast<const T*>(p.src[k]) + tl.b * p.ssb[k] + int64_t(tl.t0 + wr0) * p.sst[k] + tl.c0;
-    for (int i = lane; i < R * CB / 2; i += 32) {
-        const int r = i / (CB / 2), e = 2 * (i - r * (CB / 2));
-        const float x = r < rows && tl.c0 + e < p.C ? to_f(src[r * p.sst[k] + e]) : 0.0f;
-        const float y = r < rows && tl.c0 + e + 1 < p.C ? to_f(src[r * p.sst[k] + e + 1]) : 0.0f;
-        reinterpret_cast<typename Ops<T>::P*>(slot)[i] = Ops<T>::pack(x, y);
+    constexpr int G = 8;  // pairs on their way at once
+    static_assert(R * CB / 2 % (32 * G) == 0, "whole batches");
+    for (int i0 = lane; i0 < R * CB / 2; i0 += 32 * G) {
+        float x[G], y[G];
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            const int i = i0 + 32 * g, r = i / (CB / 2), e = 2 * (i - r * (CB / 2));
+            x[g] = r < rows && tl.c0 + e < p.C ? to_f(src[r * p.sst[k] + e]) : 0.0f;
+            y[g] = r < rows && tl.c0 + e + 1 < p.C ? to_f(src[r * p.sst[k] + e + 1]) : 0.0f;
+        }
+#pragma unroll
+        for (int g = 0; g < G; ++g)
+            reinterpret_cast<typename Ops<T>::P*>(slot)[i0 + 32 * g] = Ops<T>::pack(x[g], y[g]);
     }
     __syncwarp();
 }
@@ -547,13 +561,17 @@ __device__ __forceinline__ void write_e4m3(const TrainParams& p, const Tile& tl,
                                            int wr0, int rows, int lane) {
     constexpr int N = 16 / Ops<T>::BYTES, LPR = kGroup / N, RP = 32 / LPR;  // elements, lanes per row, rows at once
     const int v = lane % LPR;
-    const int64_t pitch = int64_t(p.ngroups) * kGroup;
+    // this lane's first row of stream 0, and the way to the next rows and streams
+    const int64_t first = int64_t(tl.b) * p.T + tl.t0 + wr0 + lane / LPR, stream = int64_t(p.nb) * p.T;
+    const int pitch = p.ngroups * kGroup;
+    uint8_t* dst0 = p.q + first * pitch + tl.c0 + v * N;
+    uint8_t* sc0 = p.qs + first * p.ngroups + tl.cblk;
 #pragma unroll
-    for (int k = 0; k < NIN; ++k) {
+    for (int k = 0; k < NIN; ++k, dst0 += stream * pitch, sc0 += stream * p.ngroups) {
         const unsigned char* slot = base + k * slot_bytes;
-        const int64_t first = (int64_t(k) * p.nb + tl.b) * p.T + tl.t0 + wr0;
+        uint8_t *dst = dst0, *scp = sc0;
 #pragma unroll
-        for (int r0 = 0; r0 < R; r0 += RP) {
+        for (int r0 = 0; r0 < R; r0 += RP, dst += RP * pitch, scp += RP * p.ngroups) {
             const int r = r0 + lane / LPR;
             const uint4 raw = reinterpret_cast<const uint4*>(slot)[r * LPR + v];
             const typename Ops<T>::P* h = reinterpret_cast<const typename Ops<T>::P*>(&raw);
@@ -585,10 +603,9 @@ __device__ __forceinline__ void write_e4m3(const TrainParams& p, const Tile& tl,
             for (int e = 0; e < N / 4; ++e)
                 q[e] = e4m3_round(fmul2(f[2 * e], splat2(inv))) | uint32_t(e4m3_round(fmul2(f[2 * e + 1], splat2(inv)))) << 16;
             if (r < rows) {
-                uint8_t* dst = p.q + (first + r) * pitch + tl.c0 + v * N;
                 if constexpr (N == 8) *reinterpret_cast<uint2*>(dst) = make_uint2(q[0], q[1]);
                 else *reinterpret_cast<uint32_t*>(dst) = q[0];
-                if (v == 0) p.qs[(first + r) * p.ngroups + tl.cblk] = static_cast<uint8_t>(sc);
+                if (v == 0) *scp = static_cast<uint8_t>(sc);
             }
         }
     }
@@ -665,6 +682,22 @@ __device__ __forceinline__ void put_maps(float2* dst, const F4& A, const F4& B) 
 }
 __device__ __forceinline__ float4 as_float4(const F4& x) { return make_float4(x.p[0].x, x.p[0].y, x.p[1].x, x.p[1].y); }
 
+// The product of a up to a row, kept from phase 1 to phase 2: f16 where the
+// output is bf16 (2^-12 of the entering state's part of it; the states and the
+// final state come from the fp32 maps), which frees registers.
+template <typename T>
+struct Prod {
+    F4 f;
+    __device__ __forceinline__ void set(int i, float2 x) { f.p[i] = x; }
+    __device__ __forceinline__ float2 get(int i) const { return f.p[i]; }
+};
+template <>
+struct Prod<__nv_bfloat16> {
+    __half2 f[2];
+    __device__ __forceinline__ void set(int i, float2 x) { f[i] = __float22half2_rn(x); }
+    __device__ __forceinline__ float2 get(int i) const { return __half22float2(f[i]); }
+};
+
 // ------------------------------------------------------------------ forward
 template <int FORM, typename T, bool CK, int DT, int CBW>
 __global__ void __launch_bounds__(kNT, (TrainCfg<FORM, T, CK, DT, CBW, false>::MINB))
@@ -699,8 +732,11 @@ __global__ void __launch_bounds__(kNT, (TrainCfg<FORM, T, CK, DT, CBW, false>::M
         named_arrive(1, kNT);
         float* st = p.states + (int64_t(tl.b) * p.nspans + tl.t0 / kSpan) * p.C;
         st_ch(st, c, p.C, carry);
-        if (K::L > kSpan && tl.nvalid > kSpan)
-            st_ch(st + p.C, c, p.C, *reinterpret_cast<const Ch<K::NC>*>(s_in + kSpan / K::R * K::CB + K::NC * lane));
+#pragma unroll
+        for (int m = 1; m < K::L / kSpan; ++m)  // the spans that start inside the tile
+            if (tl.nvalid > m * kSpan)
+                st_ch(st + int64_t(m) * p.C, c, p.C,
+                      *reinterpret_cast<const Ch<K::NC>*>(s_in + m * kSpan / K::R * K::CB + K::NC * lane));
         if (last && p.h_final != nullptr) st_ch(p.h_final + int64_t(tl.b) * p.C, c, p.C, past);
         return;
     }
@@ -728,7 +764,8 @@ __global__ void __launch_bounds__(kNT, (TrainCfg<FORM, T, CK, DT, CBW, false>::M
     // phase 1: each row's state from a zero entering state (H) and the product
     // of a up to it (P); the last are the thread's map.  Rows past T pass the
     // state on; a reset drops it.
-    F4 P[RT], H[RT], A, B;
+    Prod<T> P[RT];
+    F4 H[RT], A, B;
 #pragma unroll
     for (int i = 0; i < 2; ++i) A.p[i] = splat2(1.0f), B.p[i] = splat2(0.0f);
     auto phase1 = [&](auto whole) {
@@ -749,7 +786,7 @@ __global__ void __launch_bounds__(kNT, (TrainCfg<FORM, T, CK, DT, CBW, false>::M
                     B.p[i] = cut ? b : ffma2(a.p[i], B.p[i], b);
                     A.p[i] = (resets & ((2u << j) - 1u)) != 0u ? splat2(0.0f) : fmul2(a.p[i], A.p[i]);
                 }
-                P[j].p[i] = A.p[i];
+                P[j].set(i, A.p[i]);
                 H[j].p[i] = B.p[i];
             }
         }
@@ -784,7 +821,7 @@ __global__ void __launch_bounds__(kNT, (TrainCfg<FORM, T, CK, DT, CBW, false>::M
             }
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                o.p[i] = ffma2(P[j].p[i], h0.p[i], H[j].p[i]);
+                o.p[i] = ffma2(P[j].get(i), h0.p[i], H[j].p[i]);
                 if constexpr (!decltype(whole)::value)
                     if ((resets & ((2u << j) - 1u)) != 0u) o.p[i] = H[j].p[i];
                 if constexpr (FORM == FORM_SSD)
@@ -834,8 +871,10 @@ __global__ void __launch_bounds__(kNT, (TrainCfg<FORM, T, CK, DT, CBW, true>::MI
         const int c = tl.c0 + K::NC * lane;
         const bool last = tl.chunk == 0;
         const float* st = p.states + (int64_t(tl.b) * p.nspans + tl.t0 / kSpan) * p.C;
-        Ch<K::NC> h = ld_ch<K::NC>(st, c, p.C), hmid{}, carry{};
-        if (K::L > kSpan && tl.nvalid > kSpan) hmid = ld_ch<K::NC>(st + p.C, c, p.C);
+        Ch<K::NC> kept[K::L / kSpan], carry{};
+#pragma unroll
+        for (int m = 0; m < K::L / kSpan; ++m)
+            kept[m] = tl.nvalid > m * kSpan ? ld_ch<K::NC>(st + int64_t(m) * p.C, c, p.C) : Ch<K::NC>{};
         if (tl.pos == 0 && p.g_final != nullptr) carry = ld_ch<K::NC>(p.g_final + int64_t(tl.b) * p.C, c, p.C);
         bool handed = false;
         const Ch<K::NC> past =
@@ -844,9 +883,10 @@ __global__ void __launch_bounds__(kNT, (TrainCfg<FORM, T, CK, DT, CBW, true>::MI
                     __all_sync(0xffffffffu, block ? mbar_try_wait(s_maps, 0) : mbar_test_wait(s_maps, 0));
                 if (ready) {  // the states entering the warps first: they wait for no other tile
                     handed = true;
+                    Ch<K::NC> h = kept[0];
 #pragma unroll
                     for (int w = 0; w < kNW; ++w) {
-                        if (K::L > kSpan && w == kSpan / K::R) h = hmid;
+                        if (w * K::R % kSpan == 0) h = kept[w * K::R / kSpan];
 #pragma unroll
                         for (int k = 0; k < K::NC; ++k) {
                             const int e = w * K::CB + K::NC * lane + k;
@@ -1172,12 +1212,12 @@ struct Geom {
 // Channels per tile.  64 where the call has enough chains to fill the device;
 // 32 (tiles twice as long) where it has not: then fewer tiles of one chain are in
 // flight and wait for each other's carries (bf16, us, 64 / 32 channels: SSD
-// 1x16384x832 175 / 142, 8x2048x832 135 / 130, gated 16x4096x1024 341 / 355).
+// 1x16384x832 175 / 139, 8x2048x832 135 / 125, gated 16x4096x1024 341 / 355).
 // The 8-bit forms keep the 64 that share a scale.
-Geom geom(bool ck, int64_t nb, int64_t T, int64_t C) {
+Geom geom(int form, bool ck, bool bwd, int64_t nb, int64_t T, int64_t C) {
     Geom g;
     g.CB = !ck && nb * ((C + 63) / 64) < 192 ? 32 : 64;
-    g.L = kTileElems / g.CB;
+    g.L = tile_elems(form == NEED_FORM_GATED ? FORM_GATED : FORM_SSD, ck, int(g.CB), bwd) / g.CB;
     g.ncb = (C + g.CB - 1) / g.CB;
     g.nchains = nb * g.ncb;
     g.nchunks = (T + g.L - 1) / g.L;
@@ -1234,7 +1274,7 @@ int prepare(const need_scan_train_args* a, bool bwd, TrainParams* P, Geom* g) {
     const int es = dtype_bytes(a->dtype);
     if (a->nb > INT32_MAX / 8 || a->nb * ((a->T + kSpan - 1) / kSpan) > INT32_MAX / 2 || a->T > INT32_MAX / 2 || a->C > INT32_MAX / 2)
         return fail(NEED_ERR_UNSUPPORTED, "sizes exceed the 32-bit index range");
-    *g = geom(a->checkpoint != 0, a->nb, a->T, a->C);
+    *g = geom(a->form, a->checkpoint != 0, bwd, a->nb, a->T, a->C);
     if (g->nchains > INT32_MAX || g->ntiles > INT32_MAX)
         return fail(NEED_ERR_UNSUPPORTED, "too many tiles (%lld)", (long long)g->ntiles);
     const int nin = a->form == NEED_FORM_GATED ? 3 : 5;
@@ -1347,7 +1387,7 @@ int64_t need_scan_train_group(void) { return kGroup; }
 size_t need_scan_train_workspace_size(int32_t form, int32_t checkpoint, int32_t backward, int64_t nb, int64_t T,
                                       int64_t C) {
     if (nb < 1 || T < 1 || C < 1) return kHdrBytes;
-    return ws_size(geom(checkpoint != 0, nb, T, C), nb, C, backward != 0 && form == NEED_FORM_SSD);
+    return ws_size(geom(form, checkpoint != 0, backward != 0, nb, T, C), nb, C, backward != 0 && form == NEED_FORM_SSD);
 }
 
 int need_scan_train_forward(const need_scan_train_args* args, need_stream_t stream) {
