@@ -65,7 +65,7 @@ def _ext_command() -> list:
             "-DTORCH_EXTENSION_NAME=_train", "-DTORCH_API_INCLUDE_EXTENSION_H", f"-I{INCLUDE}",
             *[x for d in inc for x in ("-isystem", d)], os.path.join(CSRC, EXT_SOURCE), "-o", EXT + ".tmp",
             "-L" + os.path.join(torch_dir, "lib"), "-L" + LIBDIR, "-l:libneed_scan.so", "-lc10", "-lc10_cuda", "-ltorch",
-            "-ltorch_cpu", "-ltorch_python", "-Wl,-rpath,$ORIGIN"]
+            "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python", "-Wl,-rpath,$ORIGIN"]
 
 
 def build(force: bool = False, verbose: bool = False) -> str:

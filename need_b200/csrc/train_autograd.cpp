@@ -3,13 +3,14 @@
 //
 // A training pass of a small call is bound by the host, not the GPU: as Python
 // autograd functions over ctypes these operators took 160 to 390 us a pass
-// where their kernels took 20 to 60.  The nodes, their argument structs and
-// their allocations are therefore here; need_b200/train.py checks the arguments
-// and documents the operators.
+// where their kernels took 20 to 60.  The nodes, the checks of their arguments,
+// the argument structs and the allocations are therefore here (70 to 130 us, of
+// which torch's engine is 30 to 40); need_b200/train.py documents the operators.
 //
 // Nothing is kept between calls: outputs, saved tensors and scratch come from
 // torch's allocator on the current stream, so a call can be captured into a
 // graph and run on any stream.
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -17,6 +18,8 @@
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/extension.h>
 
+#include <cstdio>
+#include <stdexcept>
 #include <string>
 
 #include "need_scan.h"
@@ -29,17 +32,63 @@ namespace {
 
 constexpr int64_t kSpan = 64, kGroup = 64;  // need_scan_train_chunk_len(), need_scan_train_group()
 
+// Error texts.  Not by iostreams (TORCH_CHECK's arguments included): in this
+// process a stream's number formatting, compiled outside torch's own libraries,
+// can end in a segmentation fault.
+std::string str(const char* s) { return s; }
+std::string str(int64_t v) { return std::to_string(v); }
+std::string str(double v) {
+    char buf[32];
+    std::snprintf(buf, sizeof(buf), "%g", v);
+    return buf;
+}
+std::string str(at::IntArrayRef v) {
+    std::string r = "[";
+    for (size_t i = 0; i < v.size(); ++i) r += (i ? ", " : "") + std::to_string(v[i]);
+    return r + "]";
+}
+template <class... Args>
+std::string text(const Args&... args) {
+    return (str(args) + ...);
+}
+template <class... Args>
+void check_value(bool ok, const Args&... args) {
+    if (!ok) throw py::value_error(text(args...));
+}
 void check(const char* fn, int rc) {
-    TORCH_CHECK(rc == NEED_OK, fn, " failed (status ", rc, "): ", need_last_error());
+    if (rc != NEED_OK)
+        throw std::runtime_error(text(fn, " failed (status ", int64_t(rc), "): ", need_last_error()));
 }
 
-int32_t dtype_of(const Tensor& t) {
-    switch (t.scalar_type()) {
-        case at::kFloat: return NEED_F32;
-        case at::kBFloat16: return NEED_BF16;
-        case at::kHalf: return NEED_F16;
-        default: TORCH_CHECK_TYPE(false, "fp32, bf16 or f16 expected; got ", t.scalar_type());
-    }
+int32_t dtype_of(at::ScalarType t) {
+    return t == at::kFloat ? NEED_F32 : t == at::kBFloat16 ? NEED_BF16 : NEED_F16;
+}
+int32_t dtype_of(const Tensor& t) { return dtype_of(t.scalar_type()); }
+
+using OptTensor = std::optional<Tensor>;
+Tensor or_none(const OptTensor& t) { return t.has_value() ? *t : Tensor(); }
+OptTensor opt(const Tensor& t) { return t.defined() ? OptTensor(t) : std::nullopt; }
+
+// CUDA tensors of one device, x of a dtype the kernels take.
+void check_tensors(const char* name, const Tensor& x, std::initializer_list<const Tensor*> others) {
+    if (!x.is_cuda()) throw std::runtime_error("need_b200 kernels take CUDA tensors only (no CPU fallback)");
+    for (const Tensor* t : others)
+        if (t->defined() && t->device() != x.device())
+            throw std::runtime_error("all tensors must be on the same CUDA device (no CPU fallback)");
+    const auto ty = x.scalar_type();
+    if (ty != at::kFloat && ty != at::kBFloat16 && ty != at::kHalf)
+        throw py::type_error(text(name, " takes fp32, bf16 or f16 data; got ", c10::toString(ty)));
+}
+// The reset mask as the kernels read it.
+Tensor mask_of(const Tensor& seg, int64_t B, int64_t T) {
+    if (!seg.defined()) return seg;
+    check_value(seg.dim() == 2 && seg.size(0) == B && seg.size(1) == T, "seg_start must be [B, T] = [", B, ", ", T,
+                "]; got ", seg.sizes());
+    return seg.scalar_type() == at::kByte ? seg : seg.ne(0).to(at::kByte);
+}
+
+Tensor empty(const Tensor& like, at::IntArrayRef shape, at::ScalarType type) {
+    return at::detail::empty_cuda(shape, type, like.device(), std::nullopt);
 }
 
 // `t` with channel stride 1; a copy if its channels are apart.
@@ -48,24 +97,18 @@ Tensor channels(const Tensor& t) {
 }
 // A new [B, T, C] tensor whose rows start 16-byte aligned: contiguous, or with
 // rows apart by C rounded up.
-Tensor rows_like(const at::TensorOptions& opts, int64_t B, int64_t T, int64_t C) {
-    const int64_t n = 16 / static_cast<int64_t>(opts.dtype().itemsize()), pitch = (C + n - 1) / n * n;
-    return pitch == C ? at::empty({B, T, C}, opts) : at::empty_strided({B, T, C}, {T * pitch, pitch, 1}, opts);
+Tensor rows_like(const Tensor& like, at::ScalarType type, int64_t B, int64_t T, int64_t C) {
+    const int64_t n = 16 / static_cast<int64_t>(c10::elementSize(type)), pitch = (C + n - 1) / n * n;
+    if (pitch == C) return empty(like, {B, T, C}, type);
+    return at::detail::empty_strided_cuda({B, T, C}, {T * pitch, pitch, 1}, type, like.device());
 }
-
-Tensor scratch(const Tensor& like, size_t bytes) {
-    return at::empty({static_cast<int64_t>(bytes)}, like.options().dtype(at::kByte));
-}
-Tensor floats(const Tensor& like, at::IntArrayRef shape) { return at::empty(shape, like.options().dtype(at::kFloat)); }
+Tensor scratch(const Tensor& like, size_t bytes) { return empty(like, {static_cast<int64_t>(bytes)}, at::kByte); }
+Tensor floats(const Tensor& like, at::IntArrayRef shape) { return empty(like, shape, at::kFloat); }
 template <typename T = void>
 T* ptr(const Tensor& t) {
     return t.defined() ? static_cast<T*>(t.data_ptr()) : nullptr;
 }
 need_view view(const Tensor& t) { return need_view{t.const_data_ptr(), t.stride(0), 0, t.stride(1)}; }
-
-using OptTensor = std::optional<Tensor>;
-Tensor or_none(const OptTensor& t) { return t.has_value() ? *t : Tensor(); }
-OptTensor opt(const Tensor& t) { return t.defined() ? OptTensor(t) : std::nullopt; }
 
 // The current stream of t's device, which is made current for the guard's life.
 struct On {
@@ -118,7 +161,7 @@ ScanOut scan_forward(const ScanShape& s, const variable_list& x, const Tensor& s
     On on(x[0]);
     ScanOut r;
     const int64_t nin = static_cast<int64_t>(x.size());
-    r.out = rows_like(x[0].options(), s.B, s.T, s.C);
+    r.out = rows_like(x[0], x[0].scalar_type(), s.B, s.T, s.C);
     r.final = floats(x[0], {s.B, s.C});
     r.states = floats(x[0], {s.B, (s.T + kSpan - 1) / kSpan, s.C});
     need_scan_train_args a = scan_args(s, dtype_of(x[0]), seg, d_skip, r.states);
@@ -167,9 +210,9 @@ struct ScanTrain : torch::autograd::Function<ScanTrain> {
         variable_list saved = ctx->get_saved_variables();
         const Tensor &states = saved[0], &seg = saved[1], &d_skip = saved[2];
         On on(states);
-        const auto opts = states.options().dtype(static_cast<at::ScalarType>(d["dtype"].toInt()));
+        const auto type = static_cast<at::ScalarType>(d["dtype"].toInt());
         const int nin = s.form == NEED_FORM_GATED ? 3 : 5;
-        const Tensor gout = go[0].defined() ? channels(go[0]) : at::zeros({s.B, s.T, s.C}, opts);
+        const Tensor gout = go[0].defined() ? channels(go[0]) : at::zeros({s.B, s.T, s.C}, states.options().dtype(type));
         const Tensor gfin = go[1].defined() ? go[1].contiguous() : Tensor();
         need_scan_train_args a = scan_args(s, dtype_of(gout), seg, d_skip, states);
         if (s.ckpt) a.ckpt_values = ptr<uint8_t>(saved[3]), a.ckpt_scales = ptr<uint8_t>(saved[4]);
@@ -178,7 +221,7 @@ struct ScanTrain : torch::autograd::Function<ScanTrain> {
         a.gout = view(gout), a.g_final = ptr<float>(gfin);
         variable_list g(12);  // as forward's arguments
         for (int k = 0; k < nin; ++k) {
-            g[7 + k] = rows_like(opts, s.B, s.T, s.C);
+            g[7 + k] = rows_like(states, type, s.B, s.T, s.C);
             a.grad[k] = g[7 + k].data_ptr();
         }
         a.grad_stride_b = g[7].stride(0), a.grad_stride_t = g[7].stride(1);
@@ -191,22 +234,58 @@ struct ScanTrain : torch::autograd::Function<ScanTrain> {
     }
 };
 
-std::tuple<Tensor, Tensor> scan_train(int64_t form, bool ckpt, double dt_min, double dt_max, const OptTensor& seg_,
-                                      const OptTensor& h0_, const OptTensor& d_skip_, const Tensor& x0, const Tensor& x1,
-                                      const Tensor& x2, const OptTensor& x3_, const OptTensor& x4_) {
-    const Tensor seg = or_none(seg_), x3 = or_none(x3_), x4 = or_none(x4_);
-    Tensor h0 = or_none(h0_), d_skip = or_none(d_skip_);
-    if (h0.defined()) h0 = h0.contiguous();
-    if (d_skip.defined()) d_skip = d_skip.contiguous();
-    if (!wants_grad({&h0, &d_skip, &x0, &x1, &x2, &x3, &x4})) {  // nothing to keep
+// (out, final state); x in the C ABI's in[] order, of one shape and device.
+variable_list scan_train(int64_t form, variable_list x, const Tensor& seg_, Tensor h0, Tensor d_skip,
+                         double dt_min, double dt_max, bool ckpt) {
+    const Tensor& x2 = x[2];  // x or u
+    const int64_t B = x2.size(0), T = x2.size(1), C = x2.size(2);
+    if (h0.defined()) {
+        check_value(h0.dim() == 2 && h0.size(0) == B && h0.size(1) == C, "h0 must be [B, C] = [", B, ", ", C, "]; got ",
+                    h0.sizes());
+        h0 = h0.to(at::kFloat).contiguous();
+    }
+    if (d_skip.defined()) d_skip = d_skip.to(at::kFloat).contiguous();
+    const Tensor seg = mask_of(seg_, B, T);
+    if (x2.numel() == 0) {  // nothing to scan: the state passes through
+        Tensor out = x[0];
+        for (size_t k = 1; k < x.size(); ++k) out = out * x[k];
+        if (d_skip.defined()) out = (out * d_skip).to(x2.scalar_type());
+        return {out, h0.defined() ? h0 : at::zeros({B, C}, x2.options().dtype(at::kFloat))};
+    }
+    const Tensor none;
+    const Tensor &x3 = x.size() > 3 ? x[3] : none, &x4 = x.size() > 4 ? x[4] : none;
+    if (!wants_grad({&h0, &d_skip, &x[0], &x[1], &x2, &x3, &x4})) {  // nothing to keep
         at::NoGradGuard no_grad;
-        variable_list x{channels(x0), channels(x1), channels(x2)};
-        if (x3.defined()) x.insert(x.end(), {channels(x3), channels(x4)});
-        ScanOut r = scan_forward({form, x0.size(0), x0.size(1), x0.size(2), dt_min, dt_max, false}, x, seg, h0, d_skip);
+        for (Tensor& t : x) t = channels(t);
+        ScanOut r = scan_forward({form, B, T, C, dt_min, dt_max, false}, x, seg, h0, d_skip);
         return {r.out, r.final};
     }
-    variable_list r = ScanTrain::apply(form, ckpt, dt_min, dt_max, seg_, opt(h0), opt(d_skip), x0, x1, x2, x3_, x4_);
-    return {r[0], r[1]};
+    return ScanTrain::apply(form, ckpt, dt_min, dt_max, opt(seg), opt(h0), opt(d_skip), x[0], x[1], x2, opt(x3), opt(x4));
+}
+
+variable_list gated_scan_train(const Tensor& x, const Tensor& z, const Tensor& g, const OptTensor& seg_,
+                               const OptTensor& h0_, bool ckpt) {
+    const Tensor seg = or_none(seg_), h0 = or_none(h0_);
+    check_tensors("gated_scan_train", x, {&z, &g, &seg, &h0});
+    check_value(x.dim() == 3 && z.sizes() == x.sizes() && g.sizes() == x.sizes(),
+                "x, decay_logit and gate_logit must have the same [B, T, C] shape");
+    const auto ty = x.scalar_type();
+    return scan_train(NEED_FORM_GATED, {z.to(ty), g.to(ty), x}, seg, h0, Tensor(), 0.0, 0.0, ckpt);
+}
+
+variable_list ssd_scan_train(const Tensor& u, const Tensor& bg, const Tensor& cg, const Tensor& dt, const Tensor& og,
+                             const Tensor& d_skip, double dt_min, double dt_max, const OptTensor& seg_,
+                             const OptTensor& h0_, bool ckpt) {
+    const Tensor seg = or_none(seg_), h0 = or_none(h0_);
+    check_tensors("ssd_scan_train", u, {&bg, &cg, &dt, &og, &d_skip, &seg, &h0});
+    bool same = u.dim() == 3;
+    for (const Tensor* t : {&bg, &cg, &dt, &og}) same = same && t->sizes() == u.sizes();
+    check_value(same, "u, b_gate, c_gate, dt_raw and out_gate must have the same [B, T, D] shape");
+    check_value(d_skip.numel() == u.size(2), "d_skip must have D=", u.size(2), " elements; got ", d_skip.sizes());
+    check_value(dt_min >= 0.0 && dt_max >= dt_min, "0 <= dt_min <= dt_max expected; got ", dt_min, ", ", dt_max);
+    const auto ty = u.scalar_type();
+    return scan_train(NEED_FORM_SSD, {dt.to(ty), bg.to(ty), u, cg.to(ty), og.to(ty)}, seg, h0,
+                      d_skip.dim() == 1 ? d_skip : d_skip.reshape(-1), dt_min, dt_max, ckpt);
 }
 
 // ------------------------------------------------------------------ the conv
@@ -227,7 +306,7 @@ struct ConvTrain : torch::autograd::Function<ConvTrain> {
         const Tensor u = channels(u_), w = w_.contiguous(), seg = or_none(seg_);
         const Tensor b = b_.has_value() ? b_->contiguous() : Tensor();
         On on(u);
-        Tensor out = rows_like(u.options(), u.size(0), u.size(1), u.size(2));
+        Tensor out = rows_like(u, u.scalar_type(), u.size(0), u.size(1), u.size(2));
         need_conv_train_args a = conv_args(u, w, b, seg);
         a.out = out.data_ptr(), a.out_stride_b = out.stride(0), a.out_stride_t = out.stride(1);
         check("need_conv_silu_train_forward", need_conv_silu_train_forward(&a, on.stream));
@@ -241,7 +320,7 @@ struct ConvTrain : torch::autograd::Function<ConvTrain> {
         const Tensor gout = channels(go[0]);
         need_conv_train_args a = conv_args(u, w, b, seg);
         a.gout = gout.const_data_ptr(), a.gout_stride_b = gout.stride(0), a.gout_stride_t = gout.stride(1);
-        Tensor gu = rows_like(u.options(), a.nb, a.T, a.C), gwb = floats(u, {a.C, a.K + 1});
+        Tensor gu = rows_like(u, u.scalar_type(), a.nb, a.T, a.C), gwb = floats(u, {a.C, a.K + 1});
         const Tensor ws = scratch(u, need_conv_silu_train_workspace_size(a.K, a.nb, a.T, a.C));
         a.grad_u = gu.data_ptr(), a.out_stride_b = gu.stride(0), a.out_stride_t = gu.stride(1);
         a.grad_wb = ptr<float>(gwb);
@@ -252,8 +331,24 @@ struct ConvTrain : torch::autograd::Function<ConvTrain> {
     }
 };
 
-Tensor conv_train(const Tensor& u, const Tensor& w, const OptTensor& b, const OptTensor& seg) {
-    return ConvTrain::apply(u, w, b, seg);
+Tensor conv_train(const Tensor& u, const Tensor& weight, const OptTensor& bias, const OptTensor& seg_) {
+    Tensor b = or_none(bias), seg = or_none(seg_);
+    check_tensors("ssd_conv_silu_train", u, {&weight, &b, &seg});
+    check_value(u.dim() == 3, "u must be [B, T, C]; got ", u.sizes());
+    const int64_t B = u.size(0), T = u.size(1), C = u.size(2);
+    check_value((weight.dim() == 2 || (weight.dim() == 3 && weight.size(1) == 1)) && weight.size(0) == C,
+                "weight must be [C, 1, K] or [C, K] with C=", C, "; got ", weight.sizes());
+    check_value(weight.size(-1) >= 1 && weight.size(-1) <= 4, "1 to 4 taps expected; got ", weight.size(-1));
+    check_value(!b.defined() || (b.dim() == 1 && b.size(0) == C), "bias must be [C] = [", C, "]; got ",
+                b.defined() ? b.sizes() : u.sizes());
+    seg = mask_of(seg, B, T);
+    const Tensor w = weight.to(at::kFloat);
+    if (b.defined()) b = b.to(at::kFloat);
+    if (u.numel() == 0) {
+        Tensor out = u * w.flatten(1).sum(1);
+        return (b.defined() ? out + b : out).to(u.scalar_type());
+    }
+    return ConvTrain::apply(u, w, opt(b), opt(seg));
 }
 
 // ------------------------------------------------------------------ the norm
@@ -285,7 +380,7 @@ struct NormTrain : torch::autograd::Function<NormTrain> {
         const Tensor x = even_rows(x_), w = w_.contiguous();
         const int64_t C = x.size(-1), n = x.numel() / C;
         On on(x);
-        Tensor out = at::empty(x.sizes(), x.options()), rstd = floats(x, {n}), q, qs;
+        Tensor out = empty(x, x.sizes(), x.scalar_type()), rstd = floats(x, {n}), q, qs;
         need_norm_train_args a = norm_args(dtype_of(x), n, C, w, rstd, eps, ckpt);
         a.x = x.const_data_ptr(), a.x_stride = row_stride(x), a.out = out.data_ptr(), a.out_stride = C;
         if (ckpt) {
@@ -309,7 +404,7 @@ struct NormTrain : torch::autograd::Function<NormTrain> {
         if (ckpt) a.ckpt_values = ptr<uint8_t>(s[2]), a.ckpt_scales = ptr<uint8_t>(s[3]);
         else a.x = s[2].const_data_ptr(), a.x_stride = row_stride(s[2]);
         a.gout = gout.const_data_ptr(), a.gout_stride = row_stride(gout);
-        Tensor gx = at::empty(gout.sizes(), gout.options()), gw = floats(gout, s[0].sizes());
+        Tensor gx = empty(gout, gout.sizes(), gout.scalar_type()), gw = floats(gout, s[0].sizes());
         const Tensor ws = scratch(gout, need_rms_norm_train_workspace_size(n, C));
         a.grad_x = gx.data_ptr(), a.out_stride = C, a.grad_weight = ptr<float>(gw);
         a.workspace = ws.data_ptr(), a.workspace_bytes = ws.numel();
@@ -318,7 +413,13 @@ struct NormTrain : torch::autograd::Function<NormTrain> {
     }
 };
 
-Tensor norm_train(const Tensor& x, const Tensor& w, double eps, bool ckpt) {
+Tensor norm_train(const Tensor& x, const Tensor& weight, double eps, bool ckpt) {
+    check_tensors("rms_norm_train", x, {&weight});
+    check_value(x.dim() >= 1 && weight.numel() == x.size(-1),
+                "weight must have as many elements as x's last dim; got ", weight.sizes(), " for ", x.sizes());
+    check_value(eps >= 0.0, "eps must be >= 0; got ", eps);
+    const Tensor w = weight.to(at::kFloat);
+    if (x.numel() == 0) return (x * w.flatten()).to(x.scalar_type());
     return NormTrain::apply(x, w, eps, ckpt && wants_grad({&x, &w}));
 }
 
@@ -326,7 +427,8 @@ Tensor norm_train(const Tensor& x, const Tensor& w, double eps, bool ckpt) {
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     const auto nogil = py::call_guard<py::gil_scoped_release>();
-    m.def("scan_train", &scan_train, nogil);
+    m.def("gated_scan_train", &gated_scan_train, nogil);
+    m.def("ssd_scan_train", &ssd_scan_train, nogil);
     m.def("conv_train", &conv_train, nogil);
     m.def("norm_train", &norm_train, nogil);
 }

@@ -30,7 +30,6 @@ import torch
 
 from . import abi
 
-_DTYPES = (torch.bfloat16, torch.float16, torch.float32)
 _MAX_NORM_BYTES = 32768  # need_rms_norm_train_forward's longest row
 _EXT = None
 
@@ -49,57 +48,15 @@ def _ext():
     return _EXT
 
 
-def _check(name: str, x: torch.Tensor, *others: Optional[torch.Tensor]) -> None:
-    dev = x.device
-    for t in (x, *others):
-        if t is not None and t.device != dev or not x.is_cuda:
-            if any(o is not None and not o.is_cuda for o in (x, *others)):
-                raise RuntimeError("need_b200 kernels take CUDA tensors only (no CPU fallback)")
-            raise RuntimeError("all tensors must be on the same CUDA device")
-    if x.dtype not in _DTYPES:
-        raise TypeError(f"{name} takes fp32, bf16 or f16 data; got {x.dtype}")
-
-
 def _checkpoint(checkpoint) -> bool:
     if checkpoint is not None and checkpoint is not torch.float8_e4m3fn:
         raise ValueError(f"checkpoint must be None or torch.float8_e4m3fn; got {checkpoint}")
     return checkpoint is not None
 
 
-def _mask(seg_start: Optional[torch.Tensor], B: int, T: int) -> Optional[torch.Tensor]:
-    if seg_start is None:
-        return None
-    if seg_start.shape != (B, T):
-        raise ValueError(f"seg_start must be [B, T] = [{B}, {T}]; got {tuple(seg_start.shape)}")
-    return seg_start if seg_start.dtype == torch.uint8 else (seg_start != 0).to(torch.uint8)
-
-
 # --------------------------------------------------------------------------
 # the recurrences
 # --------------------------------------------------------------------------
-
-def _scan_train(form, streams, seg_start, h0, checkpoint, return_final_state, d_skip=None, dt_min=0.0, dt_max=0.0):
-    x = streams[0]
-    ckpt = _checkpoint(checkpoint)
-    B, T, C = x.shape
-    if h0 is not None:
-        if h0.shape != (B, C):
-            raise ValueError(f"h0 must be [B, C] = [{B}, {C}]; got {tuple(h0.shape)}")
-        h0 = h0.float()
-    seg = _mask(seg_start, B, T)
-    if x.numel() == 0:  # nothing to scan: the state passes through
-        out = x
-        for s in streams[1:]:
-            out = out * s
-        if d_skip is not None:
-            out = (out * d_skip).to(x.dtype)
-        final = h0 if h0 is not None else torch.zeros((B, C), device=x.device)
-        return (out, final) if return_final_state else out
-    if form == abi.FORM_GATED:
-        streams = (*streams, None, None)
-    out, final = _ext().scan_train(form, ckpt, dt_min, dt_max, seg, h0, d_skip, *streams)
-    return (out, final) if return_final_state else out
-
 
 def gated_scan_train(x: torch.Tensor, decay_logit: torch.Tensor, gate_logit: torch.Tensor, *,
                      seg_start: Optional[torch.Tensor] = None, h0: Optional[torch.Tensor] = None,
@@ -114,11 +71,8 @@ def gated_scan_train(x: torch.Tensor, decay_logit: torch.Tensor, gate_logit: tor
     token does not reach it, nor do later gradients reach back across it, even
     where either is an infinity or NaN.  ``checkpoint``: see the module.
     """
-    _check("gated_scan_train", x, decay_logit, gate_logit, seg_start, h0)
-    if x.dim() != 3 or not (x.shape == decay_logit.shape == gate_logit.shape):
-        raise ValueError("x, decay_logit and gate_logit must have the same [B, T, C] shape")
-    return _scan_train(abi.FORM_GATED, [decay_logit.to(x.dtype), gate_logit.to(x.dtype), x], seg_start, h0, checkpoint,
-                       return_final_state)
+    out, final = _ext().gated_scan_train(x, decay_logit, gate_logit, seg_start, h0, _checkpoint(checkpoint))
+    return (out, final) if return_final_state else out
 
 
 def ssd_scan_train(u: torch.Tensor, b_gate: torch.Tensor, c_gate: torch.Tensor, dt_raw: torch.Tensor,
@@ -138,17 +92,9 @@ def ssd_scan_train(u: torch.Tensor, b_gate: torch.Tensor, c_gate: torch.Tensor, 
     the module.  The streams may be chunks of one in-projection: no copy is made of
     views with channel stride 1.
     """
-    streams = (u, b_gate, c_gate, dt_raw, out_gate)
-    _check("ssd_scan_train", *streams, d_skip, seg_start, h0)
-    if u.dim() != 3 or any(s.shape != u.shape for s in streams):
-        raise ValueError("u, b_gate, c_gate, dt_raw and out_gate must have the same [B, T, D] shape")
-    if d_skip.numel() != u.shape[-1]:
-        raise ValueError(f"d_skip must have D={u.shape[-1]} elements; got {tuple(d_skip.shape)}")
-    if not 0.0 <= float(dt_min) <= float(dt_max):
-        raise ValueError(f"0 <= dt_min <= dt_max expected; got {dt_min}, {dt_max}")
-    order = [s.to(u.dtype) for s in (dt_raw, b_gate, u, c_gate, out_gate)]
-    return _scan_train(abi.FORM_SSD, order, seg_start, h0, checkpoint, return_final_state,
-                       (d_skip if d_skip.dim() == 1 else d_skip.reshape(-1)).float(), float(dt_min), float(dt_max))
+    out, final = _ext().ssd_scan_train(u, b_gate, c_gate, dt_raw, out_gate, d_skip, dt_min, dt_max, seg_start, h0,
+                                       _checkpoint(checkpoint))
+    return (out, final) if return_final_state else out
 
 
 # --------------------------------------------------------------------------
@@ -163,24 +109,7 @@ def ssd_conv_silu_train(u: torch.Tensor, weight: torch.Tensor, bias: Optional[to
     K] (or [C, K]), K <= 4, ``bias`` [C] or None, both used in fp32.  Differentiable
     in all three.  ``seg_start`` [B, T]: inputs before a token's segment start do
     not feed it."""
-    _check("ssd_conv_silu_train", u, weight, bias, seg_start)
-    if u.dim() != 3:
-        raise ValueError(f"u must be [B, T, C]; got {tuple(u.shape)}")
-    B, T, C = u.shape
-    if weight.dim() not in (2, 3) or weight.shape[0] != C or (weight.dim() == 3 and weight.shape[1] != 1):
-        raise ValueError(f"weight must be [C, 1, K] or [C, K] with C={C}; got {tuple(weight.shape)}")
-    K = weight.shape[-1]
-    if not 1 <= K <= 4:
-        raise ValueError(f"1 to 4 taps expected; got {K}")
-    if bias is not None and tuple(bias.shape) != (C,):
-        raise ValueError(f"bias must be [C] = [{C}]; got {tuple(bias.shape)}")
-    seg = _mask(seg_start, B, T)
-    w = weight.float()
-    b = None if bias is None else bias.float()
-    if u.numel() == 0:
-        taps = w.reshape(C, K).sum(dim=1)
-        return (u * taps if b is None else u * taps + b).to(u.dtype)
-    return _ext().conv_train(u, w, b, seg)
+    return _ext().conv_train(u, weight, bias, seg_start)
 
 
 # --------------------------------------------------------------------------
@@ -193,16 +122,7 @@ def rms_norm_train(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, *,
     weight`` over the last dim, in fp32, rounded once to ``x.dtype``; ``weight`` [C] is
     used in fp32.  Differentiable in both.  Rows of up to 32 KB.  ``checkpoint``: x is
     kept in 8 bits for the backward, 1 / sqrt(...) in fp32; see the module."""
-    _check("rms_norm_train", x, weight)
-    ckpt = _checkpoint(checkpoint)
-    C = x.shape[-1] if x.dim() else 0
-    if x.dim() < 1 or weight.numel() != C:
-        raise ValueError(f"weight must have as many elements as x's last dim; got {tuple(weight.shape)} for {tuple(x.shape)}")
-    if not float(eps) >= 0.0:
-        raise ValueError(f"eps must be >= 0; got {eps}")
-    w = weight.float()
-    if x.numel() == 0:
-        return (x * w.reshape(-1)).to(x.dtype)
-    if C * x.element_size() > _MAX_NORM_BYTES:
-        raise NotImplementedError(f"rms_norm_train takes rows of at most {_MAX_NORM_BYTES} bytes; got C={C} of {x.dtype}")
-    return _ext().norm_train(x, w, float(eps), ckpt)
+    if x.dim() and x.shape[-1] * x.element_size() > _MAX_NORM_BYTES:
+        raise NotImplementedError(f"rms_norm_train takes rows of at most {_MAX_NORM_BYTES} bytes; got {tuple(x.shape)} "
+                                  f"of {x.dtype}")
+    return _ext().norm_train(x, weight, eps, _checkpoint(checkpoint))
