@@ -495,9 +495,9 @@ NEED_API int64_t need_scan_train_chunk_len(void);
 /* Channels of one token that share a scale in an 8-bit checkpoint. */
 NEED_API int64_t need_scan_train_group(void);
 
-/* Workspace bytes of a training scan of this form and shape. */
-NEED_API size_t need_scan_train_workspace_size(int32_t form, int32_t checkpoint, int32_t backward, int64_t nb,
-                                               int64_t T, int64_t C);
+/* Workspace bytes of a training scan of this form, dtype and shape. */
+NEED_API size_t need_scan_train_workspace_size(int32_t form, int32_t dtype, int32_t checkpoint, int32_t backward,
+                                               int64_t nb, int64_t T, int64_t C);
 
 /* The GATED or SSD scan for training (need_core.py:1630-1642 computes it with
  * torch ops under grad).  Gates, states and epilogue are fp32, rounded once to

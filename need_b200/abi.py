@@ -175,7 +175,7 @@ SIGNATURES = {
     "need_ssd_conv_silu": (c_int32, [POINTER(NeedConvArgs), c_void_p]),
     "need_scan_train_chunk_len": (c_int64, []),
     "need_scan_train_group": (c_int64, []),
-    "need_scan_train_workspace_size": (c_size_t, [c_int32, c_int32, c_int32, c_int64, c_int64, c_int64]),
+    "need_scan_train_workspace_size": (c_size_t, [c_int32, c_int32, c_int32, c_int32, c_int64, c_int64, c_int64]),
     "need_scan_train_forward": (c_int32, [POINTER(NeedScanTrainArgs), c_void_p]),
     "need_scan_train_backward": (c_int32, [POINTER(NeedScanTrainArgs), c_void_p]),
     "need_conv_silu_train_workspace_size": (c_size_t, [c_int32, c_int64, c_int64, c_int64]),

@@ -175,7 +175,7 @@ ScanOut scan_forward(const ScanShape& s, const variable_list& x, const Tensor& s
     a.h0 = ptr<float>(h0);
     a.out = r.out.data_ptr(), a.out_stride_b = r.out.stride(0), a.out_stride_t = r.out.stride(1);
     a.h_final = ptr<float>(r.final);
-    const Tensor ws = scratch(x[0], need_scan_train_workspace_size(a.form, a.checkpoint, 0, s.B, s.T, s.C));
+    const Tensor ws = scratch(x[0], need_scan_train_workspace_size(a.form, a.dtype, a.checkpoint, 0, s.B, s.T, s.C));
     a.workspace = ws.data_ptr(), a.workspace_bytes = ws.numel();
     check("need_scan_train_forward", need_scan_train_forward(&a, on.stream));
     return r;
@@ -227,7 +227,7 @@ struct ScanTrain : torch::autograd::Function<ScanTrain> {
         a.grad_stride_b = g[7].stride(0), a.grad_stride_t = g[7].stride(1);
         if (d["h0"].toBool()) g[5] = floats(states, {s.B, s.C}), a.grad_h0 = ptr<float>(g[5]);
         if (d_skip.defined()) g[6] = floats(states, {s.C}), a.grad_d = ptr<float>(g[6]);
-        const Tensor ws = scratch(states, need_scan_train_workspace_size(a.form, a.checkpoint, 1, s.B, s.T, s.C));
+        const Tensor ws = scratch(states, need_scan_train_workspace_size(a.form, a.dtype, a.checkpoint, 1, s.B, s.T, s.C));
         a.workspace = ws.data_ptr(), a.workspace_bytes = ws.numel();
         check("need_scan_train_backward", need_scan_train_backward(&a, on.stream));
         return once(std::move(g));

@@ -25,25 +25,40 @@
 // segment reaches neither the next segment's states nor the gradients of the
 // one before.
 //
-// Tiles are 64 tokens x 64 channels, one CTA each: 8 row warps of 8 rows and a
-// look-back warp.  A lane owns 4 channels (two packed fp32 pairs) of 4 rows, half
-// a warp a row.  The forward writes the fp32 state entering each tile ([nb,
-// chunks, C], 1/32 of one 16-bit stream); the backward runs its tile's states
-// again from there, so it reads neither h nor any gate from memory, and both
-// directions stream their algorithmic bytes once: 8 and 14 B per element
-// (GATED, 16 bit), 12 and 22 B (SSD).  Tiles come by TMA (streams whose rows
-// are not 16-byte aligned by plain loads into the same slots), results leave by
-// TMA from the slots they were computed in.
+// A tile is 64 channels x 64 or 128 tokens, or 32 channels x 128 tokens (see
+// tile_elems and geom), one CTA each: 8 row warps and a look-back warp.  A lane
+// owns 4 channels (two packed fp32 pairs) of 4 or 8 consecutive rows, 8 or 16
+// lanes a row.  Every row is mapped once to its part of the recurrence (phase 1),
+// the maps are combined in the warp by shuffles, over the warps and the tiles
+// before by the look-back warp, and the rows are finished from the carry that
+// enters them (phase 2).  The forward keeps the fp32 state entering every 64th
+// token ([nb, spans, C], 1/32 of one 16-bit stream); the backward runs its
+// states again from there, so it reads neither h nor any gate from memory, and
+// both directions stream their algorithmic bytes once: 8 and 14 B per element
+// (GATED, 16 bit), 12 and 22 B (SSD).  Tiles come by TMA (streams whose rows are
+// not 16-byte aligned by plain loads into the same slots), results leave by TMA
+// from the slots they were computed in.
+//
+// What bounds it (B200, bf16; the copy's rate is 6.55 TB/s):
+//   SSD 8x2048x832     forward 40 us, 4.1 TB/s; backward 84-90 us, 3.3-3.6 TB/s
+//   GATED 16x4096x1024 forward 112-115 us, 4.7-4.8 TB/s; backward 189 us, 5.0 TB/s
+// Neither DRAM nor any pipe is full: a tile's life is 2 us of loads, 1 to 1.6 us
+// of phase 1, 0.8 to 1.5 us until its carry is handed out (an L2 round trip to
+// the tile before) and 0.3 to 1 us of phase 2, and registers and shared memory
+// hold 3 or 4 such tiles on an SM.  A persistent form that loads the next tile
+// during this one measured slower (gated forward 134-139 us at 3 to 4 CTAs, SSD
+// forward 63 us at 2): the second stage takes residents away.
 //
 // Across tiles the carry travels as in scan_kernel.cuh (single pass, decoupled
-// look-back over the few tiles before and the inclusive carry of the
-// one before those, composed in that fixed order, so results are
-// bit-reproducible), but with its own records: 32-bit words holding the
-// complement of a float's bits, 0 while unwritten.  The call clears them on
-// its stream before the launch, so a workspace carries nothing from one call
-// to the next: captured graphs may share one, or be replayed in any order.
-// Every wait is bounded; a tile that gives up sets the workspace's error word
-// and passes NaN on.
+// look-back over a few tiles before and the inclusive carry of the one before
+// those, composed in a fixed order, so results are bit-reproducible), but with
+// its own records: 32-bit words holding the complement of a float's bits, 0 while
+// unwritten.  The call clears them on its stream before the launch, so a
+// workspace carries nothing from one call to the next, and graphs that captured
+// calls can be replayed in any order.  Blocks start in the order of the tiles
+// (chains along x, positions along y and z), so the tiles a block waits for are
+// resident or finished.  Every wait is bounded; a tile that gives up sets the
+// workspace's error word and passes NaN on.
 //
 // Checkpoints in 8 bits: the forward also writes its inputs as e4m3 with one
 // power of two per token and 64 channels, and the backward reads those (5 + 2
@@ -68,12 +83,12 @@ constexpr int kGroup = 64;             // channels of a token that share an 8-bi
 constexpr int kSpan = 64;              // tokens between kept states
 constexpr int kNW = 8;                 // row warps
 constexpr int kNT = (kNW + 1) * 32;    // threads: the row warps and the look-back warp
-// Tokens x channels per tile.  The wide GATED forward, with little to keep per
-// element, takes tiles twice as long (16x4096x1024 bf16: 112 us against 129 us);
-// the others lose more residents than they save (SSD 8x2048x832 backward 102
-// against 83 us).
-__host__ __device__ constexpr int tile_elems(int form, bool ck, int cb, bool bwd) {
-    return form == FORM_GATED && !ck && cb == 64 && !bwd ? 8192 : 4096;
+// Tokens x channels per tile.  The wide GATED scans, with little to keep per
+// element, take tiles twice as long (16x4096x1024 bf16: forward 112 us against
+// 129 us, the bf16 backward, which keeps less, 189 against 206 us); the others
+// lose more residents than they save (SSD 8x2048x832 backward 102 against 83 us).
+__host__ __device__ constexpr int tile_elems(int form, bool bf16, bool ck, int cb, bool bwd) {
+    return form == FORM_GATED && !ck && cb == 64 && (bf16 || !bwd) ? 8192 : 4096;
 }
 constexpr int kNear = 3, kDeep = 5;    // tile maps composed before an inclusive carry
 constexpr int kHdrBytes = WS_HDR_WORDS * 4;
@@ -306,7 +321,8 @@ struct TrainCfg {
     static constexpr int NIN = FORM == FORM_GATED ? 3 : 5;
     static constexpr int IN_BYTES = (BWD && CK) ? 1 : Ops<T>::BYTES;  // per streamed input element
     static constexpr int CB = CB_, NC = CB / 32;                     // channels; of a look-back lane
-    static constexpr int L = tile_elems(FORM, CK, CB, BWD) / CB, R = L / kNW;           // tokens; rows per warp
+    static constexpr int L = tile_elems(FORM, std::is_same<T, __nv_bfloat16>::value, CK, CB, BWD) / CB;
+    static constexpr int R = L / kNW;                                // tokens; rows per warp
     static_assert(CB == 32 || CB == 64, "32 or 64 channels per tile");
     static_assert(BWD || !CK || CB == kGroup, "the 8-bit forward sees whole groups");
     static constexpr int LPR = CB / 4, SS = 32 / LPR, RT = R / SS;   // lanes per row, row groups, rows per thread
@@ -847,6 +863,10 @@ __global__ void __launch_bounds__(kNT, (TrainCfg<FORM, T, CK, DT, CBW, true>::MI
     train_bwd_kernel(const __grid_constant__ TrainParams p) {
     using K = TrainCfg<FORM, T, CK, DT, CBW, true>;
     using O = Ops<T>;
+    // bf16 GATED: 1 - a is computed again in phase 2, and the states come from each
+    // row's local state and f16 product (as in the forward), so that neither a nor
+    // 1 - a is kept.  The SSD form gains nothing from it (90 us either way).
+    constexpr bool LEAN = FORM == FORM_GATED && std::is_same<T, __nv_bfloat16>::value;
     extern __shared__ __align__(128) unsigned char base[];
     float2* s_map = reinterpret_cast<float2*>(base + K::OFF_MAP);
     float* s_fwd = reinterpret_cast<float*>(base + K::OFF_FWD);
@@ -964,7 +984,8 @@ __global__ void __launch_bounds__(kNT, (TrainCfg<FORM, T, CK, DT, CBW, true>::MI
     // to the row) e.  1 - a stays in registers (and a = 1 - (1 - a): of the two
     // the small one is the one whose relative error matters), b too, where the
     // states then take its place.
-    F4 na[RT], h[RT], A, B, M, dD;
+    F4 na[LEAN ? 1 : RT], h[RT], A, B, M, dD;
+    Prod<T> P[LEAN ? RT : 1];
 #pragma unroll
     for (int i = 0; i < 2; ++i) A.p[i] = splat2(1.0f), B.p[i] = M.p[i] = dD.p[i] = splat2(0.0f);
     auto one_minus = [](float2 x) { return fadd2(splat2(1.0f), make_float2(-x.x, -x.y)); };
@@ -973,7 +994,8 @@ __global__ void __launch_bounds__(kNT, (TrainCfg<FORM, T, CK, DT, CBW, true>::MI
         for (int j = 0; j < RT; ++j) {
             const int r = q * RT + j;
             F4 a, sd;
-            decay4<FORM, T, DT>(p, input(0, r), a, na[j], sd);
+            F4& nj = na[LEAN ? 0 : j];
+            decay4<FORM, T, DT>(p, input(0, r), a, nj, sd);
             const F4 g = sig4<T>(input(1, r)), x = input(2, r);
             F4 e = gout(r);
             keep4<T, CB>(stage(1), r, v, g);
@@ -991,7 +1013,7 @@ __global__ void __launch_bounds__(kNT, (TrainCfg<FORM, T, CK, DT, CBW, true>::MI
             }
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                const float2 b = fmul2(na[j].p[i], fmul2(g.p[i], x.p[i]));
+                const float2 b = fmul2(nj.p[i], fmul2(g.p[i], x.p[i]));
                 h[j].p[i] = b;
                 if constexpr (decltype(whole)::value) {
                     B.p[i] = j == 0 ? b : ffma2(a.p[i], B.p[i], b);
@@ -1005,6 +1027,10 @@ __global__ void __launch_bounds__(kNT, (TrainCfg<FORM, T, CK, DT, CBW, true>::MI
                         A.p[i] = fmul2(a.p[i], A.p[i]);
                         M.p[i] = ffma2(A.p[i], e.p[i], M.p[i]);
                     }
+                }
+                if constexpr (LEAN) {
+                    h[j].p[i] = B.p[i];
+                    P[j].set(i, A.p[i]);
                 }
             }
         }
@@ -1031,13 +1057,17 @@ __global__ void __launch_bounds__(kNT, (TrainCfg<FORM, T, CK, DT, CBW, true>::MI
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             hin.p[i] = apply(pA.p[i], hin.p[i], pB.p[i], seg);
-            float2 hp = hin.p[i];
+                    [[maybe_unused]] float2 hp = hin.p[i];
             if (rows > 0) {
 #pragma unroll
                 for (int j = 0; j < RT; ++j) {
-                    const bool cut = ((resets >> j) & 1u) != 0u;
-                    h[j].p[i] = cut ? h[j].p[i] : ffma2(one_minus(na[j].p[i]), hp, h[j].p[i]);
-                    hp = h[j].p[i];
+                    if constexpr (LEAN) {
+                        if ((resets & ((2u << j) - 1u)) == 0u) h[j].p[i] = ffma2(P[j].get(i), hin.p[i], h[j].p[i]);
+                    } else {
+                        const bool cut = ((resets >> j) & 1u) != 0u;
+                        h[j].p[i] = cut ? h[j].p[i] : ffma2(one_minus(na[j].p[i]), hp, h[j].p[i]);
+                        hp = h[j].p[i];
+                    }
                 }
             }
         }
@@ -1078,11 +1108,12 @@ __global__ void __launch_bounds__(kNT, (TrainCfg<FORM, T, CK, DT, CBW, true>::MI
                 put4<T, CB>(stage(3), r, v, d[3]);
                 put4<T, CB>(stage(4), r, v, d[4]);
             }
-            F4 sd, ld;
+            F4 sd, ld, aj, nj;
             if constexpr (FORM == FORM_SSD) gate(0, r, sd, ld);
+            if constexpr (LEAN) decay4<FORM, T, DT>(p, input(0, r), aj, nj, sd);
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                const float2 a = one_minus(na[j].p[i]), n = na[j].p[i];
+                const float2 n = LEAN ? nj.p[i] : na[LEAN ? 0 : j].p[i], a = LEAN ? aj.p[i] : one_minus(n);
                 const float2 prev = reset ? splat2(0.0f) : (j > 0 ? h[j > 0 ? j - 1 : 0].p[i] : hin.p[i]);
                 const float2 lam = fadd2(e.p[i], mu.p[i]);
                 mu.p[i] = reset ? splat2(0.0f) : fmul2(a, lam);
@@ -1214,10 +1245,10 @@ struct Geom {
 // flight and wait for each other's carries (bf16, us, 64 / 32 channels: SSD
 // 1x16384x832 175 / 139, 8x2048x832 135 / 125, gated 16x4096x1024 341 / 355).
 // The 8-bit forms keep the 64 that share a scale.
-Geom geom(int form, bool ck, bool bwd, int64_t nb, int64_t T, int64_t C) {
+Geom geom(int form, int dtype, bool ck, bool bwd, int64_t nb, int64_t T, int64_t C) {
     Geom g;
     g.CB = !ck && nb * ((C + 63) / 64) < 192 ? 32 : 64;
-    g.L = tile_elems(form == NEED_FORM_GATED ? FORM_GATED : FORM_SSD, ck, int(g.CB), bwd) / g.CB;
+    g.L = tile_elems(form == NEED_FORM_GATED ? FORM_GATED : FORM_SSD, dtype == NEED_BF16, ck, int(g.CB), bwd) / g.CB;
     g.ncb = (C + g.CB - 1) / g.CB;
     g.nchains = nb * g.ncb;
     g.nchunks = (T + g.L - 1) / g.L;
@@ -1274,7 +1305,7 @@ int prepare(const need_scan_train_args* a, bool bwd, TrainParams* P, Geom* g) {
     const int es = dtype_bytes(a->dtype);
     if (a->nb > INT32_MAX / 8 || a->nb * ((a->T + kSpan - 1) / kSpan) > INT32_MAX / 2 || a->T > INT32_MAX / 2 || a->C > INT32_MAX / 2)
         return fail(NEED_ERR_UNSUPPORTED, "sizes exceed the 32-bit index range");
-    *g = geom(a->form, a->checkpoint != 0, bwd, a->nb, a->T, a->C);
+    *g = geom(a->form, a->dtype, a->checkpoint != 0, bwd, a->nb, a->T, a->C);
     if (g->nchains > INT32_MAX || g->ntiles > INT32_MAX)
         return fail(NEED_ERR_UNSUPPORTED, "too many tiles (%lld)", (long long)g->ntiles);
     const int nin = a->form == NEED_FORM_GATED ? 3 : 5;
@@ -1384,10 +1415,10 @@ int64_t need_scan_train_chunk_len(void) { return kSpan; }
 
 int64_t need_scan_train_group(void) { return kGroup; }
 
-size_t need_scan_train_workspace_size(int32_t form, int32_t checkpoint, int32_t backward, int64_t nb, int64_t T,
-                                      int64_t C) {
+size_t need_scan_train_workspace_size(int32_t form, int32_t dtype, int32_t checkpoint, int32_t backward, int64_t nb,
+                                      int64_t T, int64_t C) {
     if (nb < 1 || T < 1 || C < 1) return kHdrBytes;
-    return ws_size(geom(form, checkpoint != 0, backward != 0, nb, T, C), nb, C, backward != 0 && form == NEED_FORM_SSD);
+    return ws_size(geom(form, dtype, checkpoint != 0, backward != 0, nb, T, C), nb, C, backward != 0 && form == NEED_FORM_SSD);
 }
 
 int need_scan_train_forward(const need_scan_train_args* args, need_stream_t stream) {

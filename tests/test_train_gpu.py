@@ -307,6 +307,25 @@ def test_long_against_the_scan_kernels(cuda, B, T, C):
         assert float((a - b).abs().max()) <= 64 * 2.0 ** -22 * 4 * float(a.abs().max())
 
 
+def test_more_tiles_than_a_grid_dimension(cuda):
+    """A sequence of more than 65535 tiles, against its two halves joined by the state."""
+    T, C = 65536 * 128 + 300, 8
+    gen = torch.Generator(device=cuda).manual_seed(2)
+    x, z, g, go = (torch.randn(1, T, C, device=cuda, generator=gen).to(BF) for _ in range(4))
+    ls = [t.requires_grad_() for t in (x, z, g)]
+    h, f = nk.gated_scan_train(*ls, return_final_state=True)
+    whole = torch.autograd.grad(h, ls, go)
+    cut = 128 * 40000  # at a tile: both runs then round alike
+    h1, s1 = nk.gated_scan_train(*[t[:, :cut] for t in ls], return_final_state=True)
+    h2, f2 = nk.gated_scan_train(*[t[:, cut:] for t in ls], h0=s1, return_final_state=True)
+    halves = torch.autograd.grad([h1, h2], ls, [go[:, :cut], go[:, cut:]])
+    # the carries into a tile compose other tiles' maps in the halves: a few fp32
+    # roundings, which turn at most the rare value next to a tie
+    for a, b in zip([h, f, *whole], [torch.cat([h1, h2], 1), f2, *halves]):
+        assert float((a.float() - b.float()).abs().max()) <= 2.0 ** -7 * float(b.float().abs().max())
+        assert float((a != b).float().mean()) <= 0.01
+
+
 def test_look_back_gives_up_and_says_so(cuda):
     """A wait that runs out (4 polls, far less than a tile needs to load): the launch
     ends, the error word says so, the outputs past the break are NaN and not wrong
