@@ -244,7 +244,7 @@ typedef struct {
     need_view in[5];        /* as need_scan_args.in (stride_h unused), but any alignment and strides will do;
                                backward: unused with checkpoint */
     const float* d_skip;    /* SSD: [C] fp32 */
-    double dt_min, dt_max;  /* SSD: 0 <= dt_min <= dt_max */
+    double dt_min, dt_max;  /* SSD: 0 <= dt_min <= dt_max <= 1e30 */
     const float* h0;        /* forward: optional [nb, C] fp32 initial state */
     const uint8_t* seg_start; /* optional reset mask [nb, T] */
     int64_t seg_stride_b, seg_stride_t;

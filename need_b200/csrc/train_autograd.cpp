@@ -282,7 +282,8 @@ variable_list ssd_scan_train(const Tensor& u, const Tensor& bg, const Tensor& cg
     for (const Tensor* t : {&bg, &cg, &dt, &og}) same = same && t->sizes() == u.sizes();
     check_value(same, "u, b_gate, c_gate, dt_raw and out_gate must have the same [B, T, D] shape");
     check_value(d_skip.numel() == u.size(2), "d_skip must have D=", u.size(2), " elements; got ", d_skip.sizes());
-    check_value(dt_min >= 0.0 && dt_max >= dt_min, "0 <= dt_min <= dt_max expected; got ", dt_min, ", ", dt_max);
+    check_value(dt_min >= 0.0 && dt_max >= dt_min && dt_max <= 1e30, "0 <= dt_min <= dt_max (finite) expected; got ", dt_min, ", ",
+                dt_max);
     const auto ty = u.scalar_type();
     return scan_train(NEED_FORM_SSD, {dt.to(ty), bg.to(ty), u, cg.to(ty), og.to(ty)}, seg, h0,
                       d_skip.dim() == 1 ? d_skip : d_skip.reshape(-1), dt_min, dt_max, ckpt);

@@ -1312,8 +1312,8 @@ int prepare(const need_scan_train_args* a, bool bwd, TrainParams* P, Geom* g) {
     if (a->states == nullptr) return fail(NEED_ERR_INVALID, "states is null");
     if (a->form == NEED_FORM_SSD) {
         if (a->d_skip == nullptr) return fail(NEED_ERR_INVALID, "d_skip is null");
-        if (!(a->dt_min >= 0.0) || !(a->dt_max >= a->dt_min))
-            return fail(NEED_ERR_INVALID, "0 <= dt_min <= dt_max (got %g, %g)", a->dt_min, a->dt_max);
+        if (!(a->dt_min >= 0.0) || !(a->dt_max >= a->dt_min) || a->dt_max > 1e30)
+            return fail(NEED_ERR_INVALID, "0 <= dt_min <= dt_max <= 1e30 (got %g, %g)", a->dt_min, a->dt_max);
     }
     if (a->checkpoint != 0 && (a->ckpt_values == nullptr || a->ckpt_scales == nullptr))
         return fail(NEED_ERR_INVALID, "the 8-bit checkpoint needs ckpt_values and ckpt_scales");

@@ -83,7 +83,7 @@ def scan_args(form=abi.FORM_SSD, **kw):
     ({"nb": 1 << 27, "T": 1 << 29}, abi.ERR_UNSUPPORTED),
     ({"states": None}, abi.ERR_INVALID), ({"d_skip": None}, abi.ERR_INVALID),
     ({"dt_min": -0.1}, abi.ERR_INVALID), ({"dt_max": 0.0}, abi.ERR_INVALID),
-    ({"dt_max": float("nan")}, abi.ERR_INVALID),
+    ({"dt_max": float("nan")}, abi.ERR_INVALID), ({"dt_max": float("inf")}, abi.ERR_INVALID),
     ({"checkpoint": 1}, abi.ERR_INVALID), ({"workspace": None}, abi.ERR_WORKSPACE),
     ({"workspace": P + 8}, abi.ERR_WORKSPACE), ({"workspace_bytes": 127}, abi.ERR_WORKSPACE),
 ])

@@ -522,7 +522,7 @@ def test_refusals(cuda):
         nk.gated_scan_train(x, x, x, h0=torch.zeros(2, 16))
     with pytest.raises(ValueError):
         nk.ssd_scan_train(x, x, x, x, x, D[:15], LO, HI)
-    for lo, hi in ((-0.1, 0.2), (0.2, 0.1), (0.0, float("nan"))):
+    for lo, hi in ((-0.1, 0.2), (0.2, 0.1), (0.0, float("nan")), (0.0, float("inf"))):
         with pytest.raises(ValueError):
             nk.ssd_scan_train(x, x, x, x, x, D, lo, hi)
     with pytest.raises(ValueError):
