@@ -113,9 +113,7 @@ struct TrainParams {
     uint8_t* qs;           // their scales [nin][nb][T][ngroups]
     const float* g_final;  // backward: gradient of the final state or null
     float* grad_h0;        // backward, optional
-    float* dpart;          // backward SSD: [nb * nchunks, C] partial sums of the gradient of D,
-    uint32_t* dcount;      // [ncb] tiles of each channel block that have written theirs,
-    float* grad_d;         // and [C] their sum
+    float* dpart;          // backward SSD: [nb * nchunks, C] partial sums of the gradient of D
     uint32_t* hdr;
     unsigned long long* agg;  // [ntiles][CB] (A, B)
     uint32_t* incl;           // [ntiles][CB] the carry past the tile
@@ -336,9 +334,10 @@ struct TrainCfg {
     static constexpr int OFF_FWD = OFF_MAP + kNW * CB * 8;                 // BWD: [NW][CB] forward B
     static constexpr int OFF_IN = OFF_FWD + (BWD ? kNW * CB * 4 : 0);      // [NW][CB] carry entering each warp
     static constexpr int OFF_HIN = OFF_IN + kNW * CB * 4;                  // BWD: [NW][CB] state entering each warp
-    static constexpr int OFF_SCALE = OFF_HIN + (BWD ? kNW * CB * 4 : 0);    // BWD CK: [NW][NIN][R] fp32 scales
+    static constexpr int OFF_DD = OFF_HIN + (BWD ? kNW * CB * 4 : 0);      // BWD SSD: [NW][CB] sums for D's gradient
+    static constexpr int OFF_SCALE = OFF_DD + (BWD && FORM == FORM_SSD ? kNW * CB * 4 : 0);  // BWD CK: [NW][NIN][R]
     static constexpr int OFF_BAR = OFF_SCALE + (BWD && CK ? kNW * NIN * R * 4 : 0);
-    static constexpr int SMEM = OFF_BAR + (kNW + 1) * 8 + 8;
+    static constexpr int SMEM = OFF_BAR + (kNW + 1) * 8;
     // CTAs per SM that registers are planned for (16 bit: 56 to 96 registers).  Most of
     // a tile's time is latency -- its loads 2 us, the carry 1 us -- so residents count for
     // more than a few spilled registers: SSD 8x2048x832 forward 39 us at 4, 44 at 3;
@@ -872,10 +871,10 @@ __global__ void __launch_bounds__(kNT, (TrainCfg<FORM, T, CK, DT, CBW, true>::MI
     float* s_fwd = reinterpret_cast<float*>(base + K::OFF_FWD);
     float* s_in = reinterpret_cast<float*>(base + K::OFF_IN);
     float* s_hin = reinterpret_cast<float*>(base + K::OFF_HIN);
+    float* s_dd = reinterpret_cast<float*>(base + K::OFF_DD);
     float* s_scale = reinterpret_cast<float*>(base + K::OFF_SCALE);
     uint64_t* s_bar = reinterpret_cast<uint64_t*>(base + K::OFF_BAR);
     uint64_t* s_maps = s_bar + kNW;
-    uint32_t* s_last = reinterpret_cast<uint32_t*>(s_maps + 1);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const bool seg = p.seg != nullptr;
     const Tile tl = tile_of<K::L, K::CB>(p, true);
@@ -1038,6 +1037,13 @@ __global__ void __launch_bounds__(kNT, (TrainCfg<FORM, T, CK, DT, CBW, true>::MI
     const bool whole = rows == K::R && wresets == 0u;
     if (whole) phase1(std::true_type{});
     else if (rows > 0) phase1(std::false_type{});
+    if constexpr (FORM == FORM_SSD) {
+#pragma unroll
+        for (int d = LPR; d < 32; d *= 2)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) dD.p[i] = fadd2(dD.p[i], shfl2(dD.p[i], d));
+        if (q == 0) reinterpret_cast<float4*>(s_dd)[warp * LPR + v] = as_float4(dD);
+    }
     // the maps of the warp's rows before this thread's (pA, pB: the state enters
     // through them) and after them (fA, fM: mu does)
     F4 pA, pB, fA, fM, SA = A;
@@ -1144,46 +1150,16 @@ __global__ void __launch_bounds__(kNT, (TrainCfg<FORM, T, CK, DT, CBW, true>::MI
         tma_store_commit();
     }
     if constexpr (FORM == FORM_SSD) {
-        // The gradient of D: the tile's sum over its rows, then, by the last tile
-        // of the channel block to come here, the sum over the block's tiles --
-        // each in a fixed order, whichever tile is last.
+        // the tile's sum for the gradient of D, over its warps in a fixed order (their
+        // parts are there since the barriers above)
+        if (warp == kNW - 1) {
+            const int e = K::NC * lane;
+            Ch<K::NC> sum{};
 #pragma unroll
-        for (int d = LPR; d < 32; d *= 2)
+            for (int k = 0; k < K::NC; ++k)
 #pragma unroll
-            for (int i = 0; i < 2; ++i) dD.p[i] = fadd2(dD.p[i], shfl2(dD.p[i], d));
-        if (q == 0) reinterpret_cast<float4*>(s_fwd)[warp * LPR + v] = as_float4(dD);  // the look-back warp is done with it
-        named_sync(3, kNW * 32);
-        const int ntile = p.nb * p.nchunks, e = K::NC * lane, ch = tl.c0 + e;
-        auto sum_warps = [&](const float* s) {
-            Ch<K::NC> r;
-#pragma unroll
-            for (int k = 0; k < K::NC; ++k) {
-                r.v[k] = 0.0f;
-#pragma unroll
-                for (int w = 0; w < kNW; ++w) r.v[k] += s[w * CB + e + k];
-            }
-            return r;
-        };
-        if (warp == 0) {
-            st_ch(p.dpart + (int64_t(tl.b) * p.nchunks + tl.chunk) * p.C, ch, p.C, sum_warps(s_fwd));
-            __threadfence();
-            __syncwarp();
-            if (lane == 0) *s_last = atomicAdd(&p.dcount[tl.cblk], 1u) == static_cast<uint32_t>(ntile) - 1u;
-        }
-        named_sync(3, kNW * 32);
-        if (*s_last != 0u) {
-            __threadfence();
-#pragma unroll
-            for (int k = 0; k < K::NC; ++k) {
-                float sum = 0.0f;
-                if (ch + k < p.C) {
-#pragma unroll 8
-                    for (int i = warp; i < ntile; i += kNW) sum += __ldcg(p.dpart + int64_t(i) * p.C + ch + k);
-                }
-                s_hin[warp * CB + e + k] = sum;
-            }
-            named_sync(3, kNW * 32);
-            if (warp == 0) st_ch(p.grad_d, ch, p.C, sum_warps(s_hin));
+                for (int w = 0; w < kNW; ++w) sum.v[k] += s_dd[w * CB + e + k];
+            st_ch(p.dpart + (int64_t(tl.b) * p.nchunks + tl.chunk) * p.C, tl.c0 + e, p.C, sum);
         }
     }
     if (lane == 0 && rows > 0) tma_store_drain();
@@ -1255,14 +1231,13 @@ Geom geom(int form, int dtype, bool ck, bool bwd, int64_t nb, int64_t T, int64_t
     g.ntiles = g.nchains * g.nchunks;
     return g;
 }
-// The workspace: header, look-back records and (SSD backward) the counters,
-// which the call clears, then the partial sums of the gradient of D.
-size_t rec_bytes(const Geom& g) { return g.nchunks > 1 ? size_t(g.ntiles) * size_t(g.CB) * kRecBytes : 0; }
-size_t clear_bytes(const Geom& g, bool dpart) {
-    return kHdrBytes + rec_bytes(g) + (dpart ? (size_t(g.ncb) * 4 + 15) / 16 * 16 : 0);
+// The workspace: header and look-back records, which the call clears, then (SSD
+// backward) the partial sums of the gradient of D.
+size_t clear_bytes(const Geom& g) {
+    return kHdrBytes + (g.nchunks > 1 ? size_t(g.ntiles) * size_t(g.CB) * kRecBytes : 0);
 }
 size_t ws_size(const Geom& g, int64_t nb, int64_t C, bool dpart) {
-    return clear_bytes(g, dpart) + (dpart ? size_t(nb) * size_t(g.nchunks) * size_t(C) * 4 : 0);
+    return clear_bytes(g) + (dpart ? size_t(nb) * size_t(g.nchunks) * size_t(C) * 4 : 0);
 }
 
 // Whether a [nb, T, C] tensor's rows can be read or written by TMA.
@@ -1366,7 +1341,8 @@ int prepare(const need_scan_train_args* a, bool bwd, TrainParams* P, Geom* g) {
     for (int k = 0; k < (bwd ? nin : 1); ++k)
         if (int rc = bwd ? encode(&P->tmo[k], a->grad[k], a->grad_stride_b, a->grad_stride_t, es, ty, a->nb, a->T, a->C,
                                   *g, "grad")
-                         : encode(&P->tmo[0], a->out, a->out_stride_b, a->out_stride_t, es, ty, a->nb, a->T, a->C, *g, "out"))
+                         : encode(&P->tmo[0], a->out, a->out_stride_b, a->out_stride_t, es, ty, a->nb, a->T, a->C, *g,
+                                  "out"))
             return rc;
     P->nb = int32_t(a->nb);
     P->T = int32_t(a->T);
@@ -1395,15 +1371,13 @@ int prepare(const need_scan_train_args* a, bool bwd, TrainParams* P, Geom* g) {
     P->hdr = reinterpret_cast<uint32_t*>(ws);
     P->agg = reinterpret_cast<unsigned long long*>(ws + kHdrBytes);
     P->incl = reinterpret_cast<uint32_t*>(ws + kHdrBytes + size_t(g->ntiles) * size_t(g->CB) * 8);
-    P->dcount = reinterpret_cast<uint32_t*>(ws + kHdrBytes + rec_bytes(*g));
-    P->dpart = reinterpret_cast<float*>(ws + clear_bytes(*g, dpart));
-    P->grad_d = a->grad_d;
+    P->dpart = reinterpret_cast<float*>(ws + clear_bytes(*g));
     P->polls = lookback_polls();
     return NEED_OK;
 }
 
-int clear_records(const need_scan_train_args* a, const Geom& g, bool dpart, cudaStream_t s) {
-    const cudaError_t e = cudaMemsetAsync(a->workspace, 0, clear_bytes(g, dpart), s);
+int clear_records(const need_scan_train_args* a, const Geom& g, cudaStream_t s) {
+    const cudaError_t e = cudaMemsetAsync(a->workspace, 0, clear_bytes(g), s);
     return e == cudaSuccess ? NEED_OK : cuda_fail(e, "cudaMemsetAsync(training scan records)");
 }
 
@@ -1425,7 +1399,7 @@ int need_scan_train_forward(const need_scan_train_args* args, need_stream_t stre
     TrainParams P;
     Geom g;
     if (int rc = prepare(args, false, &P, &g)) return rc;
-    if (int rc = clear_records(args, g, false, stream)) return rc;
+    if (int rc = clear_records(args, g, stream)) return rc;
     if (int rc = run<false>(args, P, g.CB == 32, stream)) return rc;
     return ok();
 }
@@ -1434,8 +1408,10 @@ int need_scan_train_backward(const need_scan_train_args* args, need_stream_t str
     TrainParams P;
     Geom g;
     if (int rc = prepare(args, true, &P, &g)) return rc;
-    if (int rc = clear_records(args, g, args->form == NEED_FORM_SSD, stream)) return rc;
+    if (int rc = clear_records(args, g, stream)) return rc;
     if (int rc = run<true>(args, P, g.CB == 32, stream)) return rc;
+    if (args->form == NEED_FORM_SSD)
+        if (int rc = column_sums(P.dpart, args->nb * g.nchunks, args->C, args->grad_d, stream)) return rc;
     return ok();
 }
 
