@@ -1218,12 +1218,14 @@ struct Geom {
 };
 // Channels per tile.  64 where the call has enough chains to fill the device;
 // 32 (tiles twice as long) where it has not: then fewer tiles of one chain are in
-// flight and wait for each other's carries (bf16, us, 64 / 32 channels: SSD
-// 1x16384x832 175 / 139, 8x2048x832 135 / 125, gated 16x4096x1024 341 / 355).
+// flight and wait for each other's carries, against more shuffles in a warp, of
+// which the backward has three times the forward's (bf16 device us, 64 / 32
+// channels: SSD 1x16384x832, 13 chains of 64, 175 / 138 the pass; 8x2048x832, 104,
+// 43 / 40 forward, 79 / 84 backward; gated 16x4096x1024, 256, 341 / 355 the pass).
 // The 8-bit forms keep the 64 that share a scale.
 Geom geom(int form, int dtype, bool ck, bool bwd, int64_t nb, int64_t T, int64_t C) {
     Geom g;
-    g.CB = !ck && nb * ((C + 63) / 64) < 192 ? 32 : 64;
+    g.CB = !ck && nb * ((C + 63) / 64) < (bwd ? 64 : 192) ? 32 : 64;
     g.L = tile_elems(form == NEED_FORM_GATED ? FORM_GATED : FORM_SSD, dtype == NEED_BF16, ck, int(g.CB), bwd) / g.CB;
     g.ncb = (C + g.CB - 1) / g.CB;
     g.nchains = nb * g.ncb;

@@ -51,6 +51,8 @@ def test_sizes(lib):
     assert ws(gated, bf, 0, 1, 96, 129, 65) == 128 + 96 * 2 * 2 * 64 * 12         # many: 64 x 128
     assert ws(gated, f32, 0, 1, 96, 65, 65) == 128 + 96 * 2 * 2 * 64 * 12         # 64 x 64
     assert ws(ssd, bf, 1, 1, 2, 65, 65) == 128 + 2 * 2 * 2 * 64 * 12 + 2 * 2 * 65 * 4
+    assert ws(ssd, bf, 0, 1, 40, 65, 65) == 128 + 40 * 2 * 2 * 64 * 12 + 40 * 2 * 65 * 4  # 80 chains: wide backward,
+    assert ws(ssd, bf, 0, 0, 40, 129, 65) == 128 + 40 * 3 * 2 * 32 * 12                  # narrow forward
     assert ws(ssd, bf, 0, 1, 0, 65, 65) == 128
     assert lib.need_conv_silu_train_workspace_size(3, 2, 129, 8) == 2 * 2 * 8 * 4 * 4
     assert lib.need_rms_norm_train_workspace_size(3, 8) == 3 * 8 * 4

@@ -51,7 +51,7 @@ def compare(outs, grads, wouts, wgrads, dtype, reach):
 SHAPES = [  # B, T, C, reset every
     (1, 1, 8, 0), (2, 1, 72, 1), (1, 3, 64, 0), (2, 8, 64, 3), (3, 63, 40, 0), (2, 64, 64, 9), (2, 65, 136, 0),
     (1, 129, 200, 20), (2, 200, 13, 0), (1, 330, 100, 50), (1, 700, 64, 0),
-    (200, 70, 24, 15), (97, 131, 70, 0),  # chains enough for the wide tiles
+    (200, 70, 24, 15), (97, 131, 70, 0), (70, 90, 40, 0),  # chains enough for the wide tiles
 ]
 
 
