@@ -5,10 +5,11 @@
 //   r = 1 / sqrt(sum(x^2) / C + eps), n = x r
 //   y = n w;  g = w dy:  dx = r (g - n sum(g n) / C),  dw = sum over rows of dy n
 //
-// Bound by HBM: 4 B per 16-bit element forward, 6 B backward (5 and 5 with x
-// kept in 8 bits).  A row is read once into the registers of 1 to 16 warps --
-// the fewest that leave a lane at most 4 16-byte pieces -- and the two sums of
-// the backward are reduced together.  The backward's blocks stride over the
+// 4 B move per 16-bit element forward, 6 B backward, 5 and 5 with x kept in 8
+// bits (8x2048x832 bf16: 14 us, 4.0 TB/s; 23 us, 3.6 TB/s, where 126 registers
+// leave 16 warps an SM, each with its next row's loads in flight).  A row is read
+// once into the registers of 1 to 16 warps -- the fewest that leave a lane at most
+// 4 16-byte pieces -- and the two sums of the backward are reduced together.  The backward's blocks stride over the
 // rows, so that a lane's channels stay the same and their share of dw stays in
 // its registers, the next row's loads in flight while one is worked on; each
 // block ends with one row of partial sums, and column_sums adds those rows in a

@@ -40,7 +40,7 @@
 // from the slots they were computed in.
 //
 // What bounds it (B200, bf16; the copy's rate is 6.55 TB/s):
-//   SSD 8x2048x832     forward 40 us, 4.1 TB/s; backward 84-90 us, 3.3-3.6 TB/s
+//   SSD 8x2048x832     forward 40 us, 4.1 TB/s; backward 79-83 us, 3.6-3.8 TB/s
 //   GATED 16x4096x1024 forward 112-115 us, 4.7-4.8 TB/s; backward 189 us, 5.0 TB/s
 // Neither DRAM nor any pipe is full: a tile's life is 2 us of loads, 1 to 1.6 us
 // of phase 1, 0.8 to 1.5 us until its carry is handed out (an L2 round trip to

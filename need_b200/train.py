@@ -19,6 +19,8 @@ state.  A group that holds an infinity or NaN gives NaN gradients.
 
 All take CUDA tensors of one device in fp32, bf16 or f16, run on the current
 stream, allocate their scratch per call, and can be captured into CUDA graphs.
+Rows of their results are 16-byte aligned: where C elements are not a whole number
+of 16 bytes, the rows lie further apart than C and the result is not contiguous.
 Gradients of gradients raise.  The autograd nodes are compiled
 (csrc/train_autograd.cpp, ``_lib/_train.so``); there is no other path.
 """
