@@ -5,18 +5,22 @@
 //   dv = dy s(v) (1 + v s(-v));  du_t = sum_d w[K-1-d] dv_{t+d}  (t+d in t's segment)
 //   dw[K-1-d] = sum over b, t of dv_t u_{t-d};  dbias = sum of dv
 //
-// All in fp32, rounded once on the way out.  4 B move per 16-bit element forward,
-// 6 B backward (8x2048x832 bf16: 14 us, 3.9 TB/s; 29 us, 2.8 TB/s, where 96 registers
-// leave 20 warps an SM to cover the loads and the taps' products).  A thread
-// walks kTok tokens of 4 channels (backward 2) in groups of kGroupRows rows, the
-// next group's loads in flight while it works on one; the last K-1 inputs, and
-// backward the K-1 unfinished du, stay in registers, and v is computed again
-// rather than kept.  The backward reads the
-// K-1 rows behind its tokens a second time (L2) for the dv they need.  A thread's
-// sums for dw and dbias are added over the block's token ranges in shared
-// memory, and column_sums adds the blocks' rows in a fixed order.  Rows that are
-// not aligned to 4 elements, and the channels of a last odd group, are read and
-// written one by one.
+// All in fp32, rounded once on the way out.  A thread walks its tokens of 4
+// channels (backward 2) in groups of kGroupRows rows.  The next groups are on their
+// way into shared memory meanwhile, copied asynchronously to places that only this
+// thread reads, so that rows in flight cost no registers.  The last K-1 inputs, and
+// backward the K-1 unfinished du, stay in registers, and v is computed again rather
+// than kept.  The backward reads the K-1 rows behind its tokens a second time (L2)
+// for the dv they need.  A thread's sums for dw and dbias are added over the block's
+// token ranges in shared memory, and column_sums adds the blocks' rows in a fixed
+// order.  Rows that are not aligned to a thread's channels, and the channels of a
+// last odd group, are read and written one by one.
+//
+// What bounds it (B200, bf16, K = 3): 4 B move per element forward, 6 B backward;
+// 8x2048x832 12 us (4.5 TB/s) and 25 us (3.3 TB/s), 16x4096x1024 146 us the pass (4.6
+// TB/s).  The backward issues 63 instructions per row of a warp, 54 % of its issue
+// slots.  With the next group in registers in place of shared memory, one group ahead
+// and 32 tokens, the passes took 45 and 180 us.
 #include <string.h>
 
 #include <type_traits>
@@ -31,9 +35,10 @@ using namespace need;
 namespace {
 
 constexpr int kMaxTaps = 4;
-constexpr int kTok = 32;        // tokens per thread
 constexpr int kGroupRows = 4;   // rows loaded together
 constexpr int kRanges = 4;      // token ranges per block (threadIdx.y)
+constexpr int kStages = 3;      // groups in shared memory: one worked on, two on their way
+constexpr int kBlocks = 5;      // per SM (96 registers); 6 spill and measured the same
 // Channel pairs per thread.  The backward keeps du, the sums and a second stream
 // besides: two pairs took 182 registers, 2 blocks per SM and 44 us (29 us with one) at
 // 8x2048x832 bf16, K = 3.
@@ -52,6 +57,7 @@ struct ConvTrainParams {
     void* out;    // y, or du
     int64_t osb, ost;
     float* part;  // [nb * ntb, C * (K + 1)]
+    int32_t tok;   // tokens per thread
     int32_t nb, T, C, ncg, ntb;      // channel groups (of 32 threads) and token blocks
     int32_t uvec, gvec, ovec;        // rows aligned to a thread's channels
 };
@@ -77,6 +83,22 @@ __device__ __forceinline__ Raw<T, NP> load_row(const T* p, bool vec, int n) {
     }
     return r;
 }
+// The row into this thread's place in shared memory, asynchronously where it is
+// aligned; `ok` false: zeros.
+template <typename T, int NP>
+__device__ __forceinline__ void copy_row(Raw<T, NP>* dst, const T* src, bool vec, int n, bool ok) {
+    if (ok && vec && n >= 2 * NP) {
+        const uint32_t d = static_cast<uint32_t>(__cvta_generic_to_shared(dst));
+        asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(d), "l"(src), "n"(sizeof(Raw<T, NP>)) : "memory");
+    } else if (ok) {
+        *dst = load_row<T, NP>(src, vec, n);
+    } else {
+        Raw<T, NP> z;
+#pragma unroll
+        for (int e = 0; e < NP; ++e) z.h[e] = Ops<T>::zero();
+        *dst = z;
+    }
+}
 template <typename T, int NP>
 __device__ __forceinline__ void store_row(T* p, bool vec, int n, const float2 (&f)[NP]) {
     using V = typename std::conditional<sizeof(Raw<T, NP>) == 16, uint4,
@@ -95,17 +117,23 @@ __device__ __forceinline__ void store_row(T* p, bool vec, int n, const float2 (&
 }
 
 template <typename T, int K, bool BWD, bool SEG>
-__global__ void __launch_bounds__(32 * kRanges) conv_train_kernel(const ConvTrainParams p) {
+__global__ void __launch_bounds__(32 * kRanges, kBlocks) conv_train_kernel(const ConvTrainParams p) {
     constexpr int G = kGroupRows, W = K - 1;  // W: tokens a tap reaches back
     constexpr int NP = kPairs<BWD>, NC = 2 * NP;
     const int cg = blockIdx.x % p.ncg;
     const int rest = blockIdx.x / p.ncg;
     const int tb = rest % p.ntb, b = rest / p.ntb;
     const int c0 = (cg * 32 + threadIdx.x) * NC, n = p.C - c0;
-    const int64_t tfirst = (int64_t(tb) * kRanges + threadIdx.y) * kTok;
+    const int64_t tfirst = (int64_t(tb) * kRanges + threadIdx.y) * p.tok;
     const bool live = n > 0 && tfirst < p.T;
     const int t0 = live ? static_cast<int>(tfirst) : 0;
-    const int t1 = live ? min(t0 + kTok, p.T) : 0;  // this thread's tokens
+    const int t1 = live ? min(t0 + p.tok, p.T) : 0;  // this thread's tokens
+
+    // a ring of kStages groups, each thread's own places: [stage][row][thread]
+    using Place = Raw<T, NP>;
+    __shared__ __align__(16) Place s_u[kStages * G][32 * kRanges];
+    __shared__ __align__(16) Place s_g[BWD ? kStages * G : 1][32 * kRanges];
+    const int tid = threadIdx.y * 32 + threadIdx.x;
 
     float2 sum[K + 1][NP];  // BWD: dw by distance back, then dbias
 #pragma unroll
@@ -118,6 +146,33 @@ __global__ void __launch_bounds__(32 * kRanges) conv_train_kernel(const ConvTrai
         const T* go = BWD ? static_cast<const T*>(p.gout) + b * p.gsb + c0 : nullptr;
         T* out = static_cast<T*>(p.out) + b * p.osb + c0;
         const uint8_t* seg = SEG ? p.seg + b * p.sgb : nullptr;
+        const int tend = BWD ? t1 + W : t1, tin = min(tend, p.T);
+        const bool vec = p.uvec != 0 && p.ovec != 0 && (!BWD || p.gvec != 0) && n >= NC;
+        const T* fu = u + int64_t(t0) * p.ust;  // the first row of the group fetched next
+        const T* fg = BWD ? go + int64_t(t0) * p.gst : nullptr;
+        int ft = t0, fs = 0;  // its token and its stage's first place
+        auto fetch = [&] {
+            if (vec && ft + G <= tin) {
+#pragma unroll
+                for (int i = 0; i < G; ++i) {
+                    copy_row<T, NP>(&s_u[fs + i][tid], fu + i * p.ust, true, NC, true);
+                    if constexpr (BWD) copy_row<T, NP>(&s_g[fs + i][tid], fg + i * p.gst, true, NC, true);
+                }
+            } else if (ft < tend) {
+#pragma unroll
+                for (int i = 0; i < G; ++i) {
+                    copy_row<T, NP>(&s_u[fs + i][tid], fu + i * p.ust, p.uvec != 0, n, ft + i < tin);
+                    if constexpr (BWD) copy_row<T, NP>(&s_g[fs + i][tid], fg + i * p.gst, p.gvec != 0, n, ft + i < tin);
+                }
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+            fu += G * p.ust;
+            if (BWD) fg += G * p.gst;
+            ft += G;
+            fs = fs == (kStages - 1) * G ? 0 : fs + G;
+        };
+#pragma unroll
+        for (int k = 0; k < kStages - 1; ++k) fetch();
         float2 w[K][NP], bs[NP];  // w[d]: the tap that multiplies the input d tokens back
         auto param = [&](const float* q, int64_t stride, int e) { return e < n ? q[int64_t(c0 + e) * stride] : 0.0f; };
 #pragma unroll
@@ -144,46 +199,32 @@ __global__ void __launch_bounds__(32 * kRanges) conv_train_kernel(const ConvTrai
                 if (SEG && seg[int64_t(t) * p.sgt] != 0) starts |= 1u << d;
             }
         }
-        Raw<T, NP> nu[G], ng[G];  // the next group, in flight
-        uint32_t nst = 0;
-        const int tend = BWD ? t1 + W : t1, tin = min(tend, p.T);
-        const bool vec = p.uvec != 0 && p.ovec != 0 && (!BWD || p.gvec != 0) && n >= NC;
-        const T* fu = u + int64_t(t0) * p.ust;  // the next group's first row
-        const T* fg = BWD ? go + int64_t(t0) * p.gst : nullptr;
-        // ALL: every row of the group is one of [t0, tin) and aligned
-        auto fetch = [&](int tg, auto all) {
+        uint32_t nst = 0;  // the next group's segment starts
+        auto marks = [&](int tg) {
             nst = 0;
+            if constexpr (SEG) {
 #pragma unroll
-            for (int i = 0; i < G; ++i) {
-                constexpr bool ALL = decltype(all)::value;
-                if (ALL || tg + i < tin) {
-                    nu[i] = load_row<T, NP>(fu + i * p.ust, ALL || p.uvec != 0, ALL ? NC : n);
-                    if constexpr (BWD) ng[i] = load_row<T, NP>(fg + i * p.gst, ALL || p.gvec != 0, ALL ? NC : n);
-                    if (SEG && seg[int64_t(tg + i) * p.sgt] != 0) nst |= 1u << (W + i);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < NP; ++e) nu[i].h[e] = ng[i].h[e] = Ops<T>::zero();
-                }
+                for (int i = 0; i < G; ++i)
+                    if (tg + i < tin && seg[int64_t(tg + i) * p.sgt] != 0) nst |= 1u << (W + i);
             }
-            fu += G * p.ust;
-            if (BWD) fg += G * p.gst;
         };
-        auto next = [&](int tg) {
-            if (vec && tg + G <= tin) fetch(tg, std::true_type{});
-            else fetch(tg, std::false_type{});
-        };
+        int rs = 0;  // the first place of the group worked on
         T* orow = out + int64_t(t0 - (BWD ? W : 0)) * p.ost;  // the row the group finishes first
         auto group = [&](int tg, auto all) {
             constexpr bool ALL = decltype(all)::value;  // all rows are this thread's, and so are those it finishes
-            Raw<T, NP> g[G];
+            asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
+            Place g[G];
 #pragma unroll
             for (int i = 0; i < G; ++i) {
+                const Place r = s_u[rs + i][tid];
 #pragma unroll
-                for (int e = 0; e < NP; ++e) x[W + i][e] = widen(nu[i].h[e]), du[W + i][e] = splat2(0.0f);
-                if (BWD) g[i] = ng[i];
+                for (int e = 0; e < NP; ++e) x[W + i][e] = widen(r.h[e]), du[W + i][e] = splat2(0.0f);
+                if (BWD) g[i] = s_g[rs + i][tid];
             }
+            rs = rs == (kStages - 1) * G ? 0 : rs + G;
             starts |= nst;
-            if (tg + G < tend) next(tg + G);
+            marks(tg + G);
+            fetch();  // into the places of the group before this one
 #pragma unroll
             for (int i = 0; i < G; ++i) {
                 // the input d back is in reach when none of the rows after it, up to this one, starts a segment
@@ -229,7 +270,8 @@ __global__ void __launch_bounds__(32 * kRanges) conv_train_kernel(const ConvTrai
                 for (int e = 0; e < NP; ++e) x[d][e] = x[G + d][e], du[d][e] = du[G + d][e];
             starts >>= G;
         };
-        next(t0);
+
+        marks(t0);
         for (int tg = t0; tg < tend; tg += G) {
             if (vec && tg + G <= t1 && (!BWD || tg - W >= t0)) group(tg, std::true_type{});
             else group(tg, std::false_type{});
@@ -261,7 +303,21 @@ __global__ void __launch_bounds__(32 * kRanges) conv_train_kernel(const ConvTrai
     }
 }
 
-int64_t token_blocks(int64_t T) { return (T + kTok * kRanges - 1) / (kTok * kRanges); }
+// Tokens per thread: 64 where that leaves enough threads, down to 16 where a
+// thread's walk is what the call waits for (B200 device us of a bf16 pass, K = 3, at
+// 16 / 32 / 64 / 128 tokens both ways: 16x4096x1024 202 / 161 / 146 / 147, 8x2048x832
+// 46.9 / 41.7 / 40.8 / -, 4x1024x832 18.5 / 17.2 / 20.0 / 27.7, 1x1024x2048 13.5 / 14.1 /
+// 17.8 / 27.3).
+int tokens(bool bwd, int64_t nb, int64_t T, int64_t C) {
+    const int64_t nc = 2 * (bwd ? kPairs<true> : kPairs<false>);
+    int t = 64;
+    while (t > 16 && nb * ((T + t - 1) / t) * ((C + nc - 1) / nc) < 1480 * t) t /= 2;
+    return t;
+}
+int64_t token_blocks(bool bwd, int64_t nb, int64_t T, int64_t C) {
+    const int64_t t = int64_t(tokens(bwd, nb, T, C)) * kRanges;
+    return (T + t - 1) / t;
+}
 
 template <typename T, bool BWD, bool SEG>
 void launch_taps(int K, unsigned grid, const ConvTrainParams& p, cudaStream_t s) {
@@ -293,7 +349,8 @@ int conv_train(const need_conv_train_args* a, cudaStream_t s) {
     p.u = a->u, p.usb = a->u_stride_b, p.ust = a->u_stride_t, p.w = a->weight, p.bias = a->bias;
     p.seg = a->seg_start, p.sgb = a->seg_stride_b, p.sgt = a->seg_stride_t;
     p.nb = int32_t(a->nb), p.T = int32_t(a->T), p.C = int32_t(a->C);
-    p.ncg = int32_t((a->C + 64 * kPairs<BWD> - 1) / (64 * kPairs<BWD>)), p.ntb = int32_t(token_blocks(a->T));
+    p.ncg = int32_t((a->C + 64 * kPairs<BWD> - 1) / (64 * kPairs<BWD>)), p.ntb = int32_t(token_blocks(BWD, a->nb, a->T, a->C));
+    p.tok = tokens(BWD, a->nb, a->T, a->C);
     const int64_t blocks = int64_t(p.ncg) * p.ntb * a->nb;
     if (int64_t(p.ncg) * p.ntb > INT32_MAX || blocks > INT32_MAX) return fail(NEED_ERR_UNSUPPORTED, "conv: sizes too large");
     p.out = BWD ? a->grad_u : a->out;
@@ -332,7 +389,7 @@ extern "C" {
 
 size_t need_conv_silu_train_workspace_size(int32_t K, int64_t nb, int64_t T, int64_t C) {
     if (K < 1 || nb < 1 || T < 1 || C < 1) return 16;
-    return size_t(nb) * size_t(token_blocks(T)) * size_t(C) * size_t(K + 1) * 4;
+    return size_t(nb) * size_t(token_blocks(true, nb, T, C)) * size_t(C) * size_t(K + 1) * 4;
 }
 int need_conv_silu_train_forward(const need_conv_train_args* args, need_stream_t stream) {
     return conv_train<false>(args, stream);

@@ -417,6 +417,19 @@ def test_conv(cuda, B, T, C, K, every, bias, dtype):
     compare([y], torch.autograd.grad(y, ls, go.to(cuda)), *want, dtype, 128 if T > 4 else 4)
 
 
+@pytest.mark.parametrize("B,T,C,K,every,dtype", [(3, 333, 10530, 3, 0, BF), (3, 333, 10529, 4, 40, HF), (9, 150, 14040, 3, 60, BF),
+                                                 (9, 150, 14041, 2, 0, HF), (3, 333, 2880, 3, 50, FP), (3, 333, 2881, 4, 0, BF)])
+def test_conv_wide(cuda, B, T, C, K, every, dtype):
+    """Widths at which a thread walks 32 and 64 tokens, backward or both ways."""
+    gen = torch.Generator().manual_seed(C)
+    leaves = [rnd(gen, B, T, C, dtype=dtype), rnd(gen, C, K), rnd(gen, C)]
+    seg, go = marks(gen, B, T, every), rnd(gen, B, T, C, dtype=dtype)
+    want = grads64(lambda u, w, b: ref.conv_silu(u, w, b, seg), leaves, [go])
+    ls = on(cuda, leaves)
+    y = nk.ssd_conv_silu_train(ls[0], ls[1][:, None], ls[2], seg_start=None if seg is None else seg.to(cuda))
+    compare([y], torch.autograd.grad(y, ls, go.to(cuda)), *want, dtype, 128)
+
+
 def test_conv_chunk_and_repeat(cuda):
     gen = torch.Generator().manual_seed(8)
     proj = rnd(gen, 2, 400, 5 * 72, dtype=BF)
