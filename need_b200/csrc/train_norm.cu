@@ -6,14 +6,14 @@
 //   y = n w;  g = w dy:  dx = r (g - n sum(g n) / C),  dw = sum over rows of dy n
 //
 // 4 B move per 16-bit element forward, 6 B backward, 5 and 5 with x kept in 8
-// bits (8x2048x832 bf16: 14 us, 4.0 TB/s; 23 us, 3.6 TB/s, where 126 registers
-// leave 16 warps an SM, each with its next row's loads in flight).  A row is read
-// once into the registers of 1 to 16 warps -- the fewest that leave a lane at most
-// 4 16-byte pieces -- and the two sums of the backward are reduced together.  The backward's blocks stride over the
-// rows, so that a lane's channels stay the same and their share of dw stays in
-// its registers, the next row's loads in flight while one is worked on; each
-// block ends with one row of partial sums, and column_sums adds those rows in a
-// fixed order.
+// bits (8x2048x832 bf16: 11 us, 5.0 TB/s; 18 us, 4.5 TB/s, where 126 registers
+// leave 16 warps an SM, each with its next row's loads in flight; 65536x1024: 112 us
+// the pass, 6.0 TB/s).  A row is read once into the registers of 1 to 16 warps --
+// the fewest that leave a lane at most 4 16-byte pieces -- and the two sums of the
+// backward are reduced together.  The backward's blocks stride over the rows, so that
+// a lane's channels stay the same and their share of dw stays in its registers, the
+// next row's loads in flight while one is worked on; each block ends with one row of
+// partial sums, and column_sums adds those rows in a fixed order.
 #include <cuda_fp8.h>
 
 #include <algorithm>
@@ -91,9 +91,18 @@ struct Piece {
             for (int e = 0; e < N && e < n; ++e) p[e] = q[e];
         }
     }
-    static __device__ __forceinline__ float2 weight(const float* w, int e, int n) {  // of elements 2 e, 2 e + 1
-        if constexpr (VEC) return __ldg(reinterpret_cast<const float2*>(w) + e);
-        else return make_float2(2 * e < n ? w[2 * e] : 0.0f, 2 * e + 1 < n ? w[2 * e + 1] : 0.0f);
+    static __device__ __forceinline__ void weights(const float* w, int n, float2 (&f)[N / 2]) {
+        if constexpr (VEC) {
+#pragma unroll
+            for (int e = 0; e < N / 4; ++e) {
+                const float4 q = __ldg(reinterpret_cast<const float4*>(w) + e);
+                f[2 * e] = make_float2(q.x, q.y), f[2 * e + 1] = make_float2(q.z, q.w);
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < N / 2; ++e)
+                f[e] = make_float2(2 * e < n ? w[2 * e] : 0.0f, 2 * e + 1 < n ? w[2 * e + 1] : 0.0f);
+        }
     }
 };
 template <typename T>
@@ -165,9 +174,11 @@ __global__ void __launch_bounds__(512) norm_train_fwd(const NormTrainParams p) {
         }
         if (in) {
             uint4 o;
+            float2 w[N / 2];
+            Pc::weights(p.w + v * N, p.C - v * N, w);
 #pragma unroll
             for (int e = 0; e < N / 2; ++e)
-                set_pair<T>(o, e, fmul2(fmul2(pair_of<T>(u[k], e), splat2(r)), Pc::weight(p.w + v * N, e, p.C - v * N)));
+                set_pair<T>(o, e, fmul2(fmul2(pair_of<T>(u[k], e), splat2(r)), w[e]));
             Pc::store(out + v * N, p.C - v * N, o);
         }
     }
@@ -189,6 +200,9 @@ __global__ void __launch_bounds__(512) norm_train_bwd(const NormTrainParams p) {
     constexpr int N = Pc::N;
     __shared__ float s_red[kMaxWarps];
     extern __shared__ __align__(16) float s_dw[];  // [C rounded up to a piece]
+    // the weights, [N / 4][nvec], so that a warp reads neighbouring 16 bytes (from
+    // memory a piece's lie 4 N bytes apart: a pass of 4096x16384 bf16 160 us, 137 so)
+    float4* s_w = reinterpret_cast<float4*>(s_dw + (p.C + N - 1) / N * N);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rpb = (blockDim.x >> 5) / p.wpr, sub = warp / p.wpr;
     const int l0 = (warp % p.wpr) * 32 + lane, step = 32 * p.wpr, nvec = (p.C + N - 1) / N;
@@ -223,6 +237,20 @@ __global__ void __launch_bounds__(512) norm_train_bwd(const NormTrainParams p) {
     };
     const int64_t stride = int64_t(gridDim.x) * rpb;
     fetch(int64_t(blockIdx.x) * rpb + sub);
+    for (int v = threadIdx.x; v < nvec; v += blockDim.x) {
+        float2 w[N / 2];
+        Pc::weights(p.w + v * N, p.C - v * N, w);
+#pragma unroll
+        for (int e = 0; e < N / 4; ++e) s_w[e * nvec + v] = make_float4(w[2 * e].x, w[2 * e].y, w[2 * e + 1].x, w[2 * e + 1].y);
+    }
+    auto weights = [&](int v, float2 (&w)[N / 2]) {
+#pragma unroll
+        for (int e = 0; e < N / 4; ++e) {
+            const float4 q = s_w[e * nvec + v];
+            w[2 * e] = make_float2(q.x, q.y), w[2 * e + 1] = make_float2(q.z, q.w);
+        }
+    };
+    __syncthreads();
     for (int64_t base = int64_t(blockIdx.x) * rpb; base < p.rows; base += stride) {
         const int64_t row = base + sub;
         const RowIn<NP, CK> cur = in;
@@ -242,10 +270,12 @@ __global__ void __launch_bounds__(512) norm_train_bwd(const NormTrainParams p) {
         for (int k = 0; k < NP; ++k) {
             const int v = l0 + k * step;
             if (v < nvec) {
+                float2 w[N / 2];
+                weights(v, w);
 #pragma unroll
                 for (int e = 0; e < N / 2; ++e) {
                     const float2 n = n_of(k, e), go = pair_of<T>(cur.g[k], e);
-                    const float2 gw = fmul2(go, Pc::weight(p.w + v * N, e, p.C - v * N));
+                    const float2 gw = fmul2(go, w[e]);
                     dw[k][e] = ffma2(go, n, dw[k][e]);
                     gn = fmaf(gw.x, n.x, fmaf(gw.y, n.y, gn));
                 }
@@ -259,27 +289,30 @@ __global__ void __launch_bounds__(512) norm_train_bwd(const NormTrainParams p) {
             const int v = l0 + k * step;
             if (row < p.rows && v < nvec) {
                 uint4 o;
+                float2 w[N / 2];
+                weights(v, w);
 #pragma unroll
                 for (int e = 0; e < N / 2; ++e) {
-                    const float2 gw = fmul2(pair_of<T>(cur.g[k], e), Pc::weight(p.w + v * N, e, p.C - v * N));
+                    const float2 gw = fmul2(pair_of<T>(cur.g[k], e), w[e]);
                     set_pair<T>(o, e, fmul2(ffma2(n_of(k, e), m, gw), r2));
                 }
                 Pc::store(out + v * N, p.C - v * N, o);
             }
         }
     }
-    // the block's rows, one after another in a fixed order
-    for (int s = 0; s < rpb; ++s) {
-        if (sub == s) {
+    // the block's rows, one after another in a fixed order; a row's pieces follow each
+    // other by a step, so that up to NP rows add at once
+    for (int s = 0; s < rpb + NP - 1; ++s) {
 #pragma unroll
-            for (int k = 0; k < NP; ++k) {
-                const int v = l0 + k * step;
-                if (v < nvec) {
+        for (int k = 0; k < NP; ++k) {
+            const int v = l0 + k * step;
+            if (sub + k == s && v < nvec) {
+                float4* d = reinterpret_cast<float4*>(s_dw + v * N);
 #pragma unroll
-                    for (int e = 0; e < N / 2; ++e) {
-                        float2* d = reinterpret_cast<float2*>(s_dw + v * N) + e;
-                        *d = s == 0 ? dw[k][e] : fadd2(*d, dw[k][e]);
-                    }
+                for (int e = 0; e < N / 4; ++e) {
+                    const float2 a = dw[k][2 * e], b = dw[k][2 * e + 1];
+                    const float4 o = sub == 0 ? make_float4(0.0f, 0.0f, 0.0f, 0.0f) : d[e];
+                    d[e] = make_float4(o.x + a.x, o.y + a.y, o.z + b.x, o.w + b.y);
                 }
             }
         }
@@ -290,19 +323,25 @@ __global__ void __launch_bounds__(512) norm_train_bwd(const NormTrainParams p) {
 }
 
 // ------------------------------------------------------------------ column sums
-constexpr int kSumY = 16;
+constexpr int kSumY = 16;     // threads that share a column
+constexpr int kSumRows = 4;   // rows each has on their way
 __global__ void __launch_bounds__(32 * kSumY) column_sums_kernel(const float* part, int64_t rows, int64_t C, float* out) {
     __shared__ float s[kSumY][32];
     const int64_t c = int64_t(blockIdx.x) * 32 + threadIdx.x;
-    float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (c < C) {
-        int64_t r = threadIdx.y;
-        for (; r + 3 * kSumY < rows; r += 4 * kSumY)
+    float acc[kSumRows] = {};
+    if (c < C)
+        for (int64_t r = threadIdx.y; r < rows; r += kSumRows * kSumY) {
+            float x[kSumRows];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) acc[k] += part[(r + k * kSumY) * C + c];
-        for (int k = 0; r < rows; r += kSumY, ++k) acc[k] += part[r * C + c];
-    }
-    s[threadIdx.y][threadIdx.x] = (acc[0] + acc[1]) + (acc[2] + acc[3]);
+            for (int k = 0; k < kSumRows; ++k) x[k] = r + k * kSumY < rows ? part[(r + k * kSumY) * C + c] : 0.0f;
+#pragma unroll
+            for (int k = 0; k < kSumRows; ++k) acc[k] += x[k];
+        }
+#pragma unroll
+    for (int k = kSumRows / 2; k >= 1; k /= 2)
+#pragma unroll
+        for (int e = 0; e < k; ++e) acc[e] += acc[e + k];
+    s[threadIdx.y][threadIdx.x] = acc[0];
     __syncthreads();
     if (threadIdx.y == 0 && c < C) {
         float t = 0.0f;
@@ -324,8 +363,7 @@ NormPlan norm_plan(int64_t nvec) {
     return pl;
 }
 // Blocks of the backward: as many as are resident at once, so that every block
-// walks the same number of rows (8x2048x832 bf16: 23 us; 31 us with 3 per SM, 27 us
-// with 4), and few enough that the partial rows they leave are a small part of the
+// walks the same number of rows (8x2048x832 bf16: 18 us; 23 us with 3 per SM), and few enough that the partial rows they leave are a small part of the
 // traffic.
 constexpr int kBwdBlocks = 148 * 2;
 int64_t bwd_blocks(int64_t rows, const NormPlan& pl) {
@@ -338,13 +376,13 @@ int launch_norm(bool bwd, const NormPlan& pl, const NormTrainParams& p, cudaStre
     const int64_t blocks = bwd ? bwd_blocks(p.rows, pl) : (p.rows + pl.rpb - 1) / pl.rpb;
     if (blocks > INT32_MAX) return fail(NEED_ERR_UNSUPPORTED, "rms norm: too many rows");
     const unsigned grid = static_cast<unsigned>(blocks);
-    const size_t sm = bwd ? size_t(p.C + 7) / 8 * 8 * 4 : 0;
+    const size_t sm = bwd ? 2 * (size_t(p.C + 7) / 8 * 8 * 4) : 0;
     auto go = [&](auto np) {
         constexpr int NP = decltype(np)::value;
         if (bwd) {
             if (sm > 48 * 1024) {
                 static std::atomic<uint64_t> done{0};
-                const cudaError_t e = ensure_smem(norm_train_bwd<T, CK, NP, VEC>, 64 * 1024, done);
+                const cudaError_t e = ensure_smem(norm_train_bwd<T, CK, NP, VEC>, 128 * 1024, done);
                 if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(norm_train_bwd)");
             }
             norm_train_bwd<T, CK, NP, VEC><<<grid, threads, sm, s>>>(p);
