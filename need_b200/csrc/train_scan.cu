@@ -85,10 +85,13 @@ constexpr int kNW = 8;                 // row warps
 constexpr int kNT = (kNW + 1) * 32;    // threads: the row warps and the look-back warp
 // Tokens x channels per tile.  The wide GATED scans, with little to keep per
 // element, take tiles twice as long (16x4096x1024 bf16: forward 112 us against
-// 129 us, the bf16 backward, which keeps less, 189 against 206 us); the others
-// lose more residents than they save (SSD 8x2048x832 backward 102 against 83 us).
+// 129 us, the bf16 backward, which keeps less, 189 against 206 us; with 8-bit copies
+// forward 176 against 184 us, and 46 against 68 us at 1x16384x832, whose chains are few);
+// the others lose more residents than they save (SSD 8x2048x832 backward 102 against 83
+// us; with 8-bit copies forward 76 against 65 us, GATED backward 260 against 215 us at
+// 16x4096x1024).
 __host__ __device__ constexpr int tile_elems(int form, bool bf16, bool ck, int cb, bool bwd) {
-    return form == FORM_GATED && !ck && cb == 64 && (bf16 || !bwd) ? 8192 : 4096;
+    return form == FORM_GATED && cb == 64 && (!bwd || (bf16 && !ck)) ? 8192 : 4096;
 }
 constexpr int kNear = 3, kDeep = 5;    // tile maps composed before an inclusive carry
 constexpr int kHdrBytes = WS_HDR_WORDS * 4;
@@ -341,8 +344,9 @@ struct TrainCfg {
     // CTAs per SM that registers are planned for (16 bit: 56 to 96 registers).  Most of
     // a tile's time is latency -- its loads 2 us, the carry 1 us -- so residents count for
     // more than a few spilled registers: SSD 8x2048x832 forward 39 us at 4, 44 at 3;
-    // backward 83 at 3, 100 at 2.
-    static constexpr int MINB = Ops<T>::BYTES == 4 ? 2 : BWD ? (CK ? 2 : 3) : (CK || L * CB > 4096 ? 3 : 4);
+    // backward 83 at 3, 100 at 2; with 8-bit copies the SSD backward 94 at 2, 102 at 3,
+    // the GATED one of 16x4096x1024 268 at 2, 215 at 3.
+    static constexpr int MINB = Ops<T>::BYTES == 4 ? 2 : BWD ? (CK && FORM == FORM_SSD ? 2 : 3) : (CK || L * CB > 4096 ? 3 : 4);
 };
 
 // ------------------------------------------------------------------ look-back
