@@ -102,6 +102,7 @@ struct TrainParams {
     CUtensorMap tmo[5];  // the streamed outputs: out, or grad[]
     uint32_t plain;      // bit k: stream k is read with plain loads, from
     const void* src[6];
+    uint8_t unit[6];     // elements per such load: the largest of 4, 2, 1 that its rows allow
     int64_t ssb[6], sst[6];
     int32_t nb, T, C, ncb, nchains, nchunks;  // tiles along T
     int32_t nspans, depth, ngroups;           // kept states along T; look-back depth; 8-bit scales per token
@@ -512,26 +513,51 @@ __device__ __forceinline__ uint32_t reset_bits(const TrainParams& p, const Tile&
     return __ballot_sync(0xffffffffu, r);
 }
 
-// A warp's rows of stream k with plain loads, as TMA would leave them (zeros past C and T).
+// A warp's rows of stream k with ordinary loads, as TMA would leave them (zeros past C
+// and T), U elements each.  4 and 8 bytes are copied asynchronously, so that all streams
+// are on their way together; the caller waits (SSD 8 x 2048 bf16, forward / backward us:
+// C = 828, 8 bytes, 57 / 93; 830, 4 bytes, 66 / 107; 831, one element a load, 86 / 145;
+// 832 by TMA 40 / 75).
+template <typename T, int R, int CB, int U>
+__device__ __forceinline__ void plain_units(const TrainParams& p, const Tile& tl, const T* src, int64_t st,
+                                            unsigned char* slot, int rows, int lane) {
+    constexpr int UR = CB / U, BYTES = U * sizeof(T);  // units in a row, bytes in a unit
+    static_assert(R * UR % 32 == 0, "whole warps");
+    if constexpr (BYTES >= 4) {
+#pragma unroll 4
+        for (int i = lane; i < R * UR; i += 32) {
+            const int r = i / UR, e = U * (i - r * UR);
+            const bool in = r < rows && tl.c0 + e < p.C;
+            asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(smem_addr(slot + i * BYTES)),
+                         "l"(in ? src + r * st + e : src), "n"(BYTES), "r"(in ? BYTES : 0)
+                         : "memory");
+        }
+    } else {
+        constexpr int G = 8;  // loads on their way at once
+        static_assert(R * UR % (32 * G) == 0, "whole batches");
+        for (int i0 = lane; i0 < R * UR; i0 += 32 * G) {
+            T x[G];
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+                const int i = i0 + 32 * g, r = i / UR, e = i - r * UR;
+                memset(&x[g], 0, sizeof(T));
+                if (r < rows && tl.c0 + e < p.C) x[g] = src[r * st + e];
+            }
+#pragma unroll
+            for (int g = 0; g < G; ++g) reinterpret_cast<T*>(slot)[i0 + 32 * g] = x[g];
+        }
+    }
+}
 template <typename T, int R, int CB>
 __device__ __forceinline__ void plain_rows(const TrainParams& p, const Tile& tl, int k, unsigned char* slot, int wr0,
                                            int rows, int lane) {
-    const T* src = static_cast<const T*>(p.src[k]) + tl.b * p.ssb[k] + int64_t(tl.t0 + wr0) * p.sst[k] + tl.c0;
-    constexpr int G = 8;  // pairs on their way at once
-    static_assert(R * CB / 2 % (32 * G) == 0, "whole batches");
-    for (int i0 = lane; i0 < R * CB / 2; i0 += 32 * G) {
-        float x[G], y[G];
-#pragma unroll
-        for (int g = 0; g < G; ++g) {
-            const int i = i0 + 32 * g, r = i / (CB / 2), e = 2 * (i - r * (CB / 2));
-            x[g] = r < rows && tl.c0 + e < p.C ? to_f(src[r * p.sst[k] + e]) : 0.0f;
-            y[g] = r < rows && tl.c0 + e + 1 < p.C ? to_f(src[r * p.sst[k] + e + 1]) : 0.0f;
-        }
-#pragma unroll
-        for (int g = 0; g < G; ++g)
-            reinterpret_cast<typename Ops<T>::P*>(slot)[i0 + 32 * g] = Ops<T>::pack(x[g], y[g]);
+    const int64_t st = p.sst[k];
+    const T* src = static_cast<const T*>(p.src[k]) + tl.b * p.ssb[k] + int64_t(tl.t0 + wr0) * st + tl.c0;
+    if constexpr (sizeof(T) == 2) {
+        if (p.unit[k] == 4) plain_units<T, R, CB, 4>(p, tl, src, st, slot, rows, lane);
     }
-    __syncwarp();
+    if (p.unit[k] == 2) plain_units<T, R, CB, 2>(p, tl, src, st, slot, rows, lane);
+    if (p.unit[k] == 1) plain_units<T, R, CB, 1>(p, tl, src, st, slot, rows, lane);
 }
 
 // Starts the loads of a warp's rows: n streams, of `bytes` per element (gout,
@@ -551,9 +577,12 @@ __device__ __forceinline__ void load_rows(const TrainParams& p, const Tile& tl, 
                 if (!((p.plain >> k) & 1u))
                     tma_load_3d(slot(k), &p.tm[k], tl.c0, tl.t0 + wr0, stacked && k < NIN ? k * p.nb + tl.b : tl.b, bar);
         }
-        if (p.plain != 0)
+        if (p.plain != 0) {
             for (int k = 0; k < N; ++k)
                 if ((p.plain >> k) & 1u) plain_rows<T, R, CB>(p, tl, k, slot(k), wr0, rows, lane);
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            __syncwarp();
+        }
     }
 }
 
@@ -1331,6 +1360,11 @@ int prepare(const need_scan_train_args* a, bool bwd, TrainParams* P, Geom* g) {
             return encode(&P->tm[k], v.ptr, v.stride_b, v.stride_t, es, ty, a->nb, a->T, a->C, *g, name);
         P->plain |= 1u << k;
         P->src[k] = v.ptr, P->ssb[k] = v.stride_b, P->sst[k] = v.stride_t;
+        auto units = [&](int64_t u) {
+            return a->C % u == 0 && reinterpret_cast<uintptr_t>(v.ptr) % (u * es) == 0 && (a->T == 1 || v.stride_t % u == 0) &&
+                   (a->nb == 1 || v.stride_b % u == 0);
+        };
+        P->unit[k] = es == 2 && units(4) ? 4 : units(2) ? 2 : 1;
         return int(NEED_OK);
     };
     for (int k = 0; k < nin; ++k) {

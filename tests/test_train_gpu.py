@@ -171,6 +171,34 @@ def test_layouts(cuda):
     assert float((got[0].cpu().double() - want[1][0]).abs().max()) <= (B + 1) * 2 ** -8 * float(want[1][0].abs().max()) * 2
 
 
+@pytest.mark.parametrize("dtype", [FP, BF], ids=["f32", "bf16"])
+@pytest.mark.parametrize("B,T,C", [(2, 150, 100), (3, 70, 98), (2, 131, 97), (1, 1, 100)])
+def test_alignments(cuda, B, T, C, dtype):
+    """Every stream at its own alignment: 16, 8, 4 bytes and one element; the results are those of aligned copies."""
+    leaves, seg, gos = ssd_case(B, T, C, 40, dtype, seed=9)
+    ls = on(cuda, leaves)
+
+    def view(t, off, width):  # a copy that lies off elements into rows of `width`
+        buf = torch.full((B * T * width + 16,), float("nan"), dtype=dtype, device=cuda)
+        v = buf[off:].as_strided((B, T, C), (T * width, width, 1))
+        v.copy_(t)
+        return v
+
+    def run(place, go):
+        with torch.no_grad():
+            xs = [place(k, x) for k, x in enumerate(ls[:5])]
+        xs = [x.requires_grad_() for x in xs]
+        out = nk.ssd_scan_train(*xs, ls[5], LO, HI, seg_start=seg.to(cuda), h0=ls[6])
+        return [out, *torch.autograd.grad(out, [*xs, ls[5], ls[6]], go)]
+
+    go = gos[0].to(cuda)
+    want = run(lambda k, x: x.clone(), go)
+    spots = [(0, 128), (4, 108), (2, 102), (1, 101), (3, 128)]
+    for turn in range(5):
+        got = run(lambda k, x: view(x, *spots[(k + turn) % 5]), view(go, *spots[turn]))
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 def test_mixed_dtypes(cuda):
     """Gates in another dtype take x's; gradients come back in their own."""
     leaves, _, gos = gated_case(2, 40, 64, 0, BF, seed=2)
