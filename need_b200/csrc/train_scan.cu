@@ -36,18 +36,21 @@
 // states again from there, so it reads neither h nor any gate from memory, and
 // both directions stream their algorithmic bytes once: 8 and 14 B per element
 // (GATED, 16 bit), 12 and 22 B (SSD).  Tiles come by TMA (streams whose rows are
-// not 16-byte aligned by plain loads into the same slots), results leave by TMA
+// not 16-byte aligned by smaller copies into the same slots), results leave by TMA
 // from the slots they were computed in.
 //
 // What bounds it (B200, bf16; the copy's rate is 6.55 TB/s):
-//   SSD 8x2048x832     forward 40 us, 4.1 TB/s; backward 79-83 us, 3.6-3.8 TB/s
-//   GATED 16x4096x1024 forward 112-115 us, 4.7-4.8 TB/s; backward 189 us, 5.0 TB/s
+//   SSD 8x2048x832     forward 40 us, 4.1 TB/s; backward 73-76 us, 4.0-4.1 TB/s
+//   GATED 16x4096x1024 forward 112-115 us, 4.7-4.8 TB/s; backward 189-192 us, 4.9-5.0 TB/s
+//   8-bit copies: SSD 8x2048x832 65 and 89 us, GATED 16x4096x1024 176 and 215 us
 // Neither DRAM nor any pipe is full: a tile's life is 2 us of loads, 1 to 1.6 us
 // of phase 1, 0.8 to 1.5 us until its carry is handed out (an L2 round trip to
 // the tile before) and 0.3 to 1 us of phase 2, and registers and shared memory
 // hold 3 or 4 such tiles on an SM.  A persistent form that loads the next tile
 // during this one measured slower (gated forward 134-139 us at 3 to 4 CTAs, SSD
-// forward 63 us at 2): the second stage takes residents away.
+// forward 63 us at 2): the second stage takes residents away.  Asking L2 for the tile
+// that starts 148 tiles later gave the gated forward 3 % and the others nothing, 444 later
+// cost the backward 3 %: the loads' latency is not what is left.
 //
 // Across tiles the carry travels as in scan_kernel.cuh (single pass, decoupled
 // look-back over a few tiles before and the inclusive carry of the one before
@@ -87,7 +90,7 @@ constexpr int kNT = (kNW + 1) * 32;    // threads: the row warps and the look-ba
 // element, take tiles twice as long (16x4096x1024 bf16: forward 112 us against
 // 129 us, the bf16 backward, which keeps less, 189 against 206 us; with 8-bit copies
 // forward 176 against 184 us, and 46 against 68 us at 1x16384x832, whose chains are few);
-// the others lose more residents than they save (SSD 8x2048x832 backward 102 against 83
+// the others lose more residents than they save (SSD 8x2048x832 backward 88 against 76
 // us; with 8-bit copies forward 76 against 65 us, GATED backward 260 against 215 us at
 // 16x4096x1024).
 __host__ __device__ constexpr int tile_elems(int form, bool bf16, bool ck, int cb, bool bwd) {
@@ -344,8 +347,8 @@ struct TrainCfg {
     static constexpr int SMEM = OFF_BAR + (kNW + 1) * 8;
     // CTAs per SM that registers are planned for (16 bit: 56 to 96 registers).  Most of
     // a tile's time is latency -- its loads 2 us, the carry 1 us -- so residents count for
-    // more than a few spilled registers: SSD 8x2048x832 forward 39 us at 4, 44 at 3;
-    // backward 83 at 3, 100 at 2; with 8-bit copies the SSD backward 94 at 2, 102 at 3,
+    // more than a few spilled registers: SSD 8x2048x832 forward 40 us at 4, 44 at 3;
+    // backward 76 at 3, 87 at 2; with 8-bit copies the SSD backward 94 at 2, 102 at 3,
     // the GATED one of 16x4096x1024 268 at 2, 215 at 3.
     static constexpr int MINB = Ops<T>::BYTES == 4 ? 2 : BWD ? (CK && FORM == FORM_SSD ? 2 : 3) : (CK || L * CB > 4096 ? 3 : 4);
 };
@@ -897,7 +900,7 @@ __global__ void __launch_bounds__(kNT, (TrainCfg<FORM, T, CK, DT, CBW, true>::MI
     using O = Ops<T>;
     // bf16 GATED: 1 - a is computed again in phase 2, and the states come from each
     // row's local state and f16 product (as in the forward), so that neither a nor
-    // 1 - a is kept.  The SSD form gains nothing from it (90 us either way).
+    // 1 - a is kept.  The SSD form loses by it (75.5 against 72.8 us).
     constexpr bool LEAN = FORM == FORM_GATED && std::is_same<T, __nv_bfloat16>::value;
     extern __shared__ __align__(128) unsigned char base[];
     float2* s_map = reinterpret_cast<float2*>(base + K::OFF_MAP);
@@ -1253,8 +1256,8 @@ struct Geom {
 // 32 (tiles twice as long) where it has not: then fewer tiles of one chain are in
 // flight and wait for each other's carries, against more shuffles in a warp, of
 // which the backward has three times the forward's (bf16 device us, 64 / 32
-// channels: SSD 1x16384x832, 13 chains of 64, 175 / 138 the pass; 8x2048x832, 104,
-// 43 / 40 forward, 79 / 84 backward; gated 16x4096x1024, 256, 341 / 355 the pass).
+// channels: SSD 1x16384x832, 13 chains of 64, 156 / 134 the pass; 8x2048x832, 104,
+// 43 / 40 forward, 76 / 79 backward; gated 16x4096x1024, 256, 302 / 355 the pass).
 // The 8-bit forms keep the 64 that share a scale.
 Geom geom(int form, int dtype, bool ck, bool bwd, int64_t nb, int64_t T, int64_t C) {
     Geom g;
