@@ -54,7 +54,10 @@ def test_sizes(lib):
     assert ws(ssd, bf, 0, 1, 40, 65, 65) == 128 + 40 * 2 * 2 * 64 * 12 + 40 * 2 * 65 * 4  # 80 chains: wide backward,
     assert ws(ssd, bf, 0, 0, 40, 129, 65) == 128 + 40 * 3 * 2 * 32 * 12                  # narrow forward
     assert ws(ssd, bf, 0, 1, 0, 65, 65) == 128
-    assert lib.need_conv_silu_train_workspace_size(3, 2, 129, 8) == 2 * 2 * 8 * 4 * 4
+    conv = lib.need_conv_silu_train_workspace_size
+    assert conv(3, 2, 129, 8) == 2 * 3 * 8 * 4 * 4            # 16 tokens a thread, 4 threads a block
+    assert conv(3, 3, 333, 2880) == 3 * 3 * 2880 * 4 * 4      # 32
+    assert conv(3, 3, 333, 10530) == 3 * 2 * 10530 * 4 * 4    # 64
     assert lib.need_rms_norm_train_workspace_size(3, 8) == 3 * 8 * 4
 
 
