@@ -380,7 +380,7 @@ int launch_norm(bool bwd, const NormPlan& pl, const NormTrainParams& p, cudaStre
     auto go = [&](auto np) {
         constexpr int NP = decltype(np)::value;
         if (bwd) {
-            if (sm > 48 * 1024) {
+            if (sm + sizeof(float) * kMaxWarps > 48 * 1024) {  // with the kernel's static shared memory
                 static std::atomic<uint64_t> done{0};
                 const cudaError_t e = ensure_smem(norm_train_bwd<T, CK, NP, VEC>, 128 * 1024, done);
                 if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(norm_train_bwd)");

@@ -486,6 +486,18 @@ def test_norm(cuda, rows, C, dtype, ckpt):
     compare([y], torch.autograd.grad(y, ls, go.to(cuda)), *want, dtype, 64) if C > 1 else ref.close(y, want[0][0], dtype, 64)
 
 
+@pytest.mark.parametrize("ckpt", [None, F8], ids=["full", "8bit"])
+@pytest.mark.parametrize("C", [6136, 6144, 6152])
+def test_norm_at_the_default_shared_memory(cuda, C, ckpt):
+    """Rows whose backward takes just under, all of and just over the shared memory a launch has unasked."""
+    gen = torch.Generator().manual_seed(C)
+    leaves, go = [rnd(gen, 5, C, dtype=BF), 1 + 0.1 * rnd(gen, C)], rnd(gen, 5, C, dtype=BF)
+    want = grads64(lambda x, w: ref.rms_norm(x, w, 1e-6, ckpt is not None), leaves, [go])
+    ls = on(cuda, leaves)
+    y = nk.rms_norm_train(*ls, 1e-6, checkpoint=ckpt)
+    compare([y], torch.autograd.grad(y, ls, go.to(cuda)), *want, BF, 64)
+
+
 def test_norm_longest_row_and_layouts(cuda):
     gen = torch.Generator().manual_seed(4)
     for C, dtype in ((16384, BF), (8192, FP)):
