@@ -458,6 +458,30 @@ def test_conv_wide(cuda, B, T, C, K, every, dtype):
     compare([y], torch.autograd.grad(y, ls, go.to(cuda)), *want, dtype, 128)
 
 
+@pytest.mark.parametrize("dtype", [FP, BF], ids=["f32", "bf16"])
+@pytest.mark.parametrize("B,T,C,K", [(2, 150, 100, 3), (3, 70, 98, 4), (2, 131, 97, 2), (1, 1, 101, 3)])
+def test_conv_alignments(cuda, B, T, C, K, dtype):
+    """Rows aligned to 16 bytes down to one element: the results are those of aligned copies."""
+    gen = torch.Generator().manual_seed(C)
+    u, go, w, b = rnd(gen, B, T, C, dtype=dtype), rnd(gen, B, T, C, dtype=dtype), rnd(gen, C, K), rnd(gen, C)
+    seg = marks(gen, B, T, 30).to(cuda)
+
+    def view(t, off, width):
+        buf = torch.full((B * T * width + 16,), float("nan"), dtype=dtype, device=cuda)
+        return buf[off:].as_strided((B, T, C), (T * width, width, 1)).copy_(t)
+
+    def run(spot, gspot):
+        ls = [view(u, *spot).requires_grad_(), *on(cuda, [w, b])]
+        y = nk.ssd_conv_silu_train(*ls, seg_start=seg)
+        return [y, *torch.autograd.grad(y, ls, view(go, *gspot))]
+
+    want = run((0, 128), (0, 128))
+    spots = [(4, 108), (2, 102), (1, 101), (3, 128)]
+    for k, spot in enumerate(spots):
+        for gspot in (spots[(k + 1) % 4], (0, 128)):
+            assert all(torch.equal(x, y) for x, y in zip(run(spot, gspot), want))
+
+
 def test_conv_chunk_and_repeat(cuda):
     gen = torch.Generator().manual_seed(8)
     proj = rnd(gen, 2, 400, 5 * 72, dtype=BF)
