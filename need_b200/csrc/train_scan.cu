@@ -41,8 +41,8 @@
 //
 // What bounds it (B200, bf16; the copy's rate is 6.55 TB/s):
 //   SSD 8x2048x832     forward 40 us, 4.1 TB/s; backward 73-76 us, 4.0-4.1 TB/s
-//   GATED 16x4096x1024 forward 112-115 us, 4.7-4.8 TB/s; backward 189-192 us, 4.9-5.0 TB/s
-//   8-bit copies: SSD 8x2048x832 65 and 89 us, GATED 16x4096x1024 176 and 215 us
+//   GATED 16x4096x1024 forward 107-108 us, 5.0 TB/s; backward 189-192 us, 4.9-5.0 TB/s
+//   8-bit copies: SSD 8x2048x832 64 and 89 us, GATED 16x4096x1024 161 and 215 us
 // Neither DRAM nor any pipe is full: a tile's life is 2 us of loads, 1 to 1.6 us
 // of phase 1, 0.8 to 1.5 us until its carry is handed out (an L2 round trip to
 // the tile before) and 0.3 to 1 us of phase 2, and registers and shared memory
@@ -87,11 +87,11 @@ constexpr int kSpan = 64;              // tokens between kept states
 constexpr int kNW = 8;                 // row warps
 constexpr int kNT = (kNW + 1) * 32;    // threads: the row warps and the look-back warp
 // Tokens x channels per tile.  The wide GATED scans, with little to keep per
-// element, take tiles twice as long (16x4096x1024 bf16: forward 112 us against
-// 129 us, the bf16 backward, which keeps less, 189 against 206 us; with 8-bit copies
-// forward 176 against 184 us, and 46 against 68 us at 1x16384x832, whose chains are few);
+// element, take tiles twice as long (16x4096x1024 bf16: forward 107 us against
+// 130 us, the bf16 backward, which keeps less, 189 against 206 us; with 8-bit copies
+// forward 161 against 201 us, and 47 against 68 us at 1x16384x832, whose chains are few);
 // the others lose more residents than they save (SSD 8x2048x832 backward 88 against 76
-// us; with 8-bit copies forward 76 against 65 us, GATED backward 260 against 215 us at
+// us; with 8-bit copies forward 76 against 64 us, GATED backward 260 against 215 us at
 // 16x4096x1024).
 __host__ __device__ constexpr int tile_elems(int form, bool bf16, bool ck, int cb, bool bwd) {
     return form == FORM_GATED && cb == 64 && (!bwd || (bf16 && !ck)) ? 8192 : 4096;
@@ -733,7 +733,38 @@ __device__ __forceinline__ void put_maps(float2* dst, const F4& A, const F4& B) 
 }
 __device__ __forceinline__ float4 as_float4(const F4& x) { return make_float4(x.p[0].x, x.p[0].y, x.p[1].x, x.p[1].y); }
 
-// The product of a up to a row, kept from phase 1 to phase 2: f16 where the
+// The forward's product of a up to a row, kept from phase 1 to phase 2 in fp32 (held in
+// f16 it loses its last bits, and all of them below 6e-8).  In place of the logits of
+// streams 0 and 1, which phase 2 does not read: their two 16-bit slots hold the upper
+// and the lower halves, so that it costs no registers.
+template <typename T, int CB>
+__device__ __forceinline__ void put_prod(unsigned char* slot0, unsigned char* slot1, int r, int v, const F4& x) {
+    if constexpr (Ops<T>::BYTES == 4) {
+        put4<float, CB>(slot0, r, v, x);
+    } else {
+        const uint32_t w[4] = {__float_as_uint(x.p[0].x), __float_as_uint(x.p[0].y), __float_as_uint(x.p[1].x),
+                               __float_as_uint(x.p[1].y)};
+        reinterpret_cast<uint2*>(slot0)[r * (CB / 4) + v] =
+            make_uint2(__byte_perm(w[0], w[1], 0x7632), __byte_perm(w[2], w[3], 0x7632));
+        reinterpret_cast<uint2*>(slot1)[r * (CB / 4) + v] =
+            make_uint2(__byte_perm(w[0], w[1], 0x5410), __byte_perm(w[2], w[3], 0x5410));
+    }
+}
+template <typename T, int CB>
+__device__ __forceinline__ F4 get_prod(const unsigned char* slot0, const unsigned char* slot1, int r, int v) {
+    if constexpr (Ops<T>::BYTES == 4) {
+        return row4<float, CB>(slot0, r, v);
+    } else {
+        const uint2 hi = reinterpret_cast<const uint2*>(slot0)[r * (CB / 4) + v];
+        const uint2 lo = reinterpret_cast<const uint2*>(slot1)[r * (CB / 4) + v];
+        F4 x;
+        x.p[0] = make_float2(__uint_as_float(__byte_perm(lo.x, hi.x, 0x5410)), __uint_as_float(__byte_perm(lo.x, hi.x, 0x7632)));
+        x.p[1] = make_float2(__uint_as_float(__byte_perm(lo.y, hi.y, 0x5410)), __uint_as_float(__byte_perm(lo.y, hi.y, 0x7632)));
+        return x;
+    }
+}
+
+// The backward's product of a up to a row, kept from phase 1 to phase 2: f16 where the
 // output is bf16 (2^-12 of the entering state's part of it; the states and the
 // final state come from the fp32 maps), which frees registers.
 template <typename T>
@@ -812,10 +843,17 @@ __global__ void __launch_bounds__(kNT, (TrainCfg<FORM, T, CK, DT, CBW, false>::M
         mbar_wait_bounded(&s_bar[warp], 0, kTmaPolls);
     }
 
+    // The copies before phase 1, which writes into the slots they are made from: they
+    // delay the tile's map, but kept in registers the products spill (GATED 16x4096x1024
+    // bf16 223 us against 161, on short tiles 194; SSD 8x2048x832 68 against 64).
+    if constexpr (CK) {
+        if (rows > 0) write_e4m3<T, K::NIN, K::R>(p, tl, slots, K::IN_SLOT, wr0, rows, lane);
+        __syncwarp();
+    }
+
     // phase 1: each row's state from a zero entering state (H) and the product
-    // of a up to it (P); the last are the thread's map.  Rows past T pass the
+    // of a up to it (put_prod); the last are the thread's map.  Rows past T pass the
     // state on; a reset drops it.
-    Prod<T> P[RT];
     F4 H[RT], A, B;
 #pragma unroll
     for (int i = 0; i < 2; ++i) A.p[i] = splat2(1.0f), B.p[i] = splat2(0.0f);
@@ -837,9 +875,9 @@ __global__ void __launch_bounds__(kNT, (TrainCfg<FORM, T, CK, DT, CBW, false>::M
                     B.p[i] = cut ? b : ffma2(a.p[i], B.p[i], b);
                     A.p[i] = (resets & ((2u << j) - 1u)) != 0u ? splat2(0.0f) : fmul2(a.p[i], A.p[i]);
                 }
-                P[j].set(i, A.p[i]);
                 H[j].p[i] = B.p[i];
             }
+            put_prod<T, CB>(slot(0), slot(1), r, v, A);
         }
     };
     const bool whole = rows == K::R && wresets == 0u;
@@ -849,8 +887,6 @@ __global__ void __launch_bounds__(kNT, (TrainCfg<FORM, T, CK, DT, CBW, false>::M
     warp_prefix<LPR, SS>(A, B, EA, EB, q, seg);
     if (q == SS - 1) put_maps(s_map + warp * CB + 4 * v, A, B);
     mbar_arrive(s_maps);
-    if constexpr (CK)  // while the carry comes in
-        if (rows > 0) write_e4m3<T, K::NIN, K::R>(p, tl, slots, K::IN_SLOT, wr0, rows, lane);
     named_sync(1, kNT);
     if (rows == 0) return;
 
@@ -864,6 +900,7 @@ __global__ void __launch_bounds__(kNT, (TrainCfg<FORM, T, CK, DT, CBW, false>::M
 #pragma unroll
         for (int j = 0; j < RT; ++j) {
             const int r = q * RT + j;
+            const F4 P = get_prod<T, CB>(slot(0), slot(1), r, v);
             F4 o, sc, so, u;
             if constexpr (FORM == FORM_SSD) {
                 sc = sig4<T>(row4<T, CB>(slot(3), r, v));
@@ -872,7 +909,7 @@ __global__ void __launch_bounds__(kNT, (TrainCfg<FORM, T, CK, DT, CBW, false>::M
             }
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                o.p[i] = ffma2(P[j].get(i), h0.p[i], H[j].p[i]);
+                o.p[i] = ffma2(P.p[i], h0.p[i], H[j].p[i]);
                 if constexpr (!decltype(whole)::value)
                     if ((resets & ((2u << j) - 1u)) != 0u) o.p[i] = H[j].p[i];
                 if constexpr (FORM == FORM_SSD)
