@@ -270,47 +270,24 @@ __device__ __forceinline__ F4 row4_8(const unsigned char* slot, int r, int v, fl
     return f;
 }
 
-// What a sigmoid computed in phase 1 leaves in its stream's slot for phase 2,
-// in place of the logit: fp32 s itself; bf16 the nearer of s and s - 1 to 0 as
-// f16 (2^-12 relative against the 2^-9 the gradient is rounded to, of whichever
-// of s and 1 - s is small; below 6e-5 a fixed 3e-8), which saves the second
-// round of exponentials and reciprocals.  f16 gradients are rounded to 2^-12
-// themselves: there the logit stays and the sigmoid is computed again.
+// What a sigmoid computed in phase 1 leaves in its stream's slot for phase 2, in place
+// of the logit: fp32 streams s itself.  A 16-bit slot cannot hold s to the precision the
+// gradients are rounded to (f16 ends at 3e-8, bf16 has 8 bits): there the logit stays and
+// the sigmoid is computed again (bf16 backward: SSD 8x2048x832 77 us, GATED 16x4096x1024
+// 185; 75 and 182 with s kept as f16, wrong below 1e-5).
 template <typename T>
-constexpr bool kKeep = !std::is_same<T, __half>::value;
+constexpr bool kKeep = Ops<T>::BYTES == 4;
 template <typename T, int CB>
 __device__ __forceinline__ void keep4(unsigned char* slot, int r, int v, const F4& s) {
-    if constexpr (Ops<T>::BYTES == 4) {
-        put4<float, CB>(slot, r, v, s);
-    } else if constexpr (kKeep<T>) {
-        F4 y;
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {  // s = 1 is kept as -0
-            const float2 n = fadd2(splat2(1.0f), make_float2(-s.p[i].x, -s.p[i].y));
-            y.p[i] = make_float2(s.p[i].x >= 0.5f ? -n.x : s.p[i].x, s.p[i].y >= 0.5f ? -n.y : s.p[i].y);
-        }
-        put4<__half, CB>(slot, r, v, y);
-    }
-}
-__device__ __forceinline__ float one_if_negative(float y) {  // by the sign bit: -0 too
-    return __int_as_float((__float_as_int(y) >> 31) & 0x3f800000);
+    if constexpr (kKeep<T>) put4<float, CB>(slot, r, v, s);
 }
 // s and s (1 - s) from a kept slot.
 template <typename T, int CB>
 __device__ __forceinline__ void kept4(const unsigned char* slot, int r, int v, F4& s, F4& slope) {
-    static_assert(kKeep<T>, "kept as fp32 or f16");
-    if constexpr (Ops<T>::BYTES == 4) {
-        s = row4<float, CB>(slot, r, v);
+    static_assert(kKeep<T>, "kept as fp32");
+    s = row4<float, CB>(slot, r, v);
 #pragma unroll
-        for (int i = 0; i < 2; ++i) slope.p[i] = fmul2(s.p[i], fadd2(splat2(1.0f), make_float2(-s.p[i].x, -s.p[i].y)));
-    } else {
-        const F4 y = row4<__half, CB>(slot, r, v);
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            s.p[i] = fadd2(y.p[i], make_float2(one_if_negative(y.p[i].x), one_if_negative(y.p[i].y)));
-            slope.p[i] = make_float2(fmaf(-y.p[i].x, y.p[i].x, fabsf(y.p[i].x)), fmaf(-y.p[i].y, y.p[i].y, fabsf(y.p[i].y)));
-        }
-    }
+    for (int i = 0; i < 2; ++i) slope.p[i] = fmul2(s.p[i], fadd2(splat2(1.0f), make_float2(-s.p[i].x, -s.p[i].y)));
 }
 template <typename T>
 __device__ __forceinline__ F4 sig4(const F4& x) {

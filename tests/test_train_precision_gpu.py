@@ -168,3 +168,56 @@ def test_decayed_states(cuda, dtype, B, ckpt):
     gated, ssd, T = decaying(dtype, B)
     run_gated(cuda, gated, dtype, ckpt, (T + 16) * gate_error(dtype, 4), parts=("h", "final"))
     run_ssd(cuda, ssd, 2.5, 3.5, dtype, ckpt, (T + 16) * gate_error(dtype, 4, 3.5), parts=("y", "final"))
+
+
+# ------------------------------------------------------------------ saturated gates
+
+def marks(gen, B, T):
+    m = (torch.rand(B, T, generator=gen) < 0.3).to(torch.uint8)
+    m[:, -1] = 1
+    return m
+
+
+# B, T, C, resets: whole rows of warps and none; tiles of 32 and of 64 channels
+SHAPES = pytest.mark.parametrize("B,T,C,resets", [(1, 70, 40, False), (2, 21, 72, True), (200, 64, 24, False)])
+
+
+@CKPTS
+@pytest.mark.parametrize("dtype", [BF, HF], ids=["bf16", "f16"])
+@SHAPES
+@pytest.mark.parametrize("lo,hi", [(0.001, 0.2)])
+def test_saturated_gates_ssd(cuda, B, T, C, resets, lo, hi, dtype, ckpt):
+    """Logits to +-20: every gradient to its own last bits, where s, 1 - s or both
+    their products are as small as 1e-17."""
+    gen = torch.Generator().manual_seed(4)
+    logits = [40 * torch.rand(B, T, C, generator=gen) - 20 for _ in range(4)]
+    case = [positive(gen, B, T, C), *logits, positive(gen, C), positive(gen, B, C), positive(gen, B, T, C), positive(gen, B, C)]
+    case = [t.to(dtype) if t.dim() == 3 else t for t in case]
+    run_ssd(cuda, case, lo, hi, dtype, ckpt, (T + 16) * gate_error(dtype, 20, hi), marks(gen, B, T) if resets else None)
+
+
+# ------------------------------------------------------------------ ordinary inputs
+
+def turned(got, want):
+    """How many bf16 results are not `want` rounded."""
+    return float((got.detach().cpu() != want.detach().to(BF)).float().mean())
+
+
+@CKPTS
+def test_ssd_is_rounded_once(cuda, ckpt):
+    """bf16 results on ordinary inputs are the 64-bit ones rounded, but for values next
+    to a tie: an error e in fp32 turns e / (eps / 2) of them, and e is some 2^-17 of the
+    value (tens of tokens at 2^-21 each, and differences).  A factor rounded to 11 bits
+    between the passes would turn 2^-12 / 2^-8 = 1 in 16 of them."""
+    gen = torch.Generator().manual_seed(5)
+    B, T, C = 4, 200, 64
+    r = lambda *s: torch.randn(*s, generator=gen)  # noqa: E731
+    xs, D, h0, go, gf = [r(B, T, C).to(BF) for _ in range(5)], 1 + 0.1 * r(C), r(B, C), r(B, T, C).to(BF), r(B, C)
+    ls = [t.double().requires_grad_() for t in (*xs, D, h0)]
+    w = ref.ssd(*ls, 0.001, 0.2, None, ckpt is not None)
+    want = [w[0], *torch.autograd.grad(w, ls, [go.double(), gf.double()])[:5]]
+    ls = [t.to(cuda).requires_grad_() for t in (*xs, D, h0)]
+    o = nk.ssd_scan_train(*ls[:6], 0.001, 0.2, h0=ls[6], return_final_state=True, checkpoint=ckpt)
+    got = [o[0], *torch.autograd.grad(o, ls, [go.to(cuda), gf.to(cuda)])[:5]]
+    off = [turned(a, b) for a, b in zip(got, want)]
+    assert max(off) <= 0.02, off
