@@ -41,7 +41,7 @@
 //
 // What bounds it (B200, bf16; the copy's rate is 6.55 TB/s):
 //   SSD 8x2048x832     forward 40 us, 4.1 TB/s; backward 73-76 us, 4.0-4.1 TB/s
-//   GATED 16x4096x1024 forward 107-108 us, 5.0 TB/s; backward 189-192 us, 4.9-5.0 TB/s
+//   GATED 16x4096x1024 forward 107-108 us, 5.0 TB/s; backward 191 us, 4.9 TB/s
 //   8-bit copies: SSD 8x2048x832 64 and 89 us, GATED 16x4096x1024 161 and 215 us
 // Neither DRAM nor any pipe is full: a tile's life is 2 us of loads, 1 to 1.6 us
 // of phase 1, 0.8 to 1.5 us until its carry is handed out (an L2 round trip to
@@ -88,7 +88,7 @@ constexpr int kNW = 8;                 // row warps
 constexpr int kNT = (kNW + 1) * 32;    // threads: the row warps and the look-back warp
 // Tokens x channels per tile.  The wide GATED scans, with little to keep per
 // element, take tiles twice as long (16x4096x1024 bf16: forward 107 us against
-// 130 us, the bf16 backward, which keeps less, 189 against 206 us; with 8-bit copies
+// 130 us, the bf16 backward, which keeps less, 191 against 209 us; with 8-bit copies
 // forward 161 against 201 us, and 47 against 68 us at 1x16384x832, whose chains are few);
 // the others lose more residents than they save (SSD 8x2048x832 backward 88 against 76
 // us; with 8-bit copies forward 76 against 64 us, GATED backward 260 against 215 us at
@@ -741,22 +741,6 @@ __device__ __forceinline__ F4 get_prod(const unsigned char* slot0, const unsigne
     }
 }
 
-// The backward's product of a up to a row, kept from phase 1 to phase 2: f16 where the
-// output is bf16 (2^-12 of the entering state's part of it; the states and the
-// final state come from the fp32 maps), which frees registers.
-template <typename T>
-struct Prod {
-    F4 f;
-    __device__ __forceinline__ void set(int i, float2 x) { f.p[i] = x; }
-    __device__ __forceinline__ float2 get(int i) const { return f.p[i]; }
-};
-template <>
-struct Prod<__nv_bfloat16> {
-    __half2 f[2];
-    __device__ __forceinline__ void set(int i, float2 x) { f[i] = __float22half2_rn(x); }
-    __device__ __forceinline__ float2 get(int i) const { return __half22float2(f[i]); }
-};
-
 // ------------------------------------------------------------------ forward
 template <int FORM, typename T, bool CK, int DT, int CBW>
 __global__ void __launch_bounds__(kNT, (TrainCfg<FORM, T, CK, DT, CBW, false>::MINB))
@@ -912,10 +896,10 @@ __global__ void __launch_bounds__(kNT, (TrainCfg<FORM, T, CK, DT, CBW, true>::MI
     train_bwd_kernel(const __grid_constant__ TrainParams p) {
     using K = TrainCfg<FORM, T, CK, DT, CBW, true>;
     using O = Ops<T>;
-    // bf16 GATED: 1 - a is computed again in phase 2, and the states come from each
-    // row's local state and f16 product (as in the forward), so that neither a nor
-    // 1 - a is kept.  The SSD form loses by it (75.5 against 72.8 us).
-    constexpr bool LEAN = FORM == FORM_GATED && std::is_same<T, __nv_bfloat16>::value;
+    // The long tiles of bf16 GATED: a is computed again for the states and in phase 2, and
+    // neither it nor 1 - a is kept (16x4096x1024 190 us; 209 kept, on short tiles 209).  The
+    // SSD form loses by it (75.5 against 72.8 us), and so do the 8-bit copies (226, 210).
+    constexpr bool LEAN = FORM == FORM_GATED && std::is_same<T, __nv_bfloat16>::value && !CK;
     extern __shared__ __align__(128) unsigned char base[];
     float2* s_map = reinterpret_cast<float2*>(base + K::OFF_MAP);
     float* s_fwd = reinterpret_cast<float*>(base + K::OFF_FWD);
@@ -1034,7 +1018,6 @@ __global__ void __launch_bounds__(kNT, (TrainCfg<FORM, T, CK, DT, CBW, true>::MI
     // the small one is the one whose relative error matters), b too, where the
     // states then take its place.
     F4 na[LEAN ? 1 : RT], h[RT], A, B, M, dD;
-    Prod<T> P[LEAN ? RT : 1];
 #pragma unroll
     for (int i = 0; i < 2; ++i) A.p[i] = splat2(1.0f), B.p[i] = M.p[i] = dD.p[i] = splat2(0.0f);
     auto one_minus = [](float2 x) { return fadd2(splat2(1.0f), make_float2(-x.x, -x.y)); };
@@ -1077,10 +1060,6 @@ __global__ void __launch_bounds__(kNT, (TrainCfg<FORM, T, CK, DT, CBW, true>::MI
                         M.p[i] = ffma2(A.p[i], e.p[i], M.p[i]);
                     }
                 }
-                if constexpr (LEAN) {
-                    h[j].p[i] = B.p[i];
-                    P[j].set(i, A.p[i]);
-                }
             }
         }
     };
@@ -1113,17 +1092,14 @@ __global__ void __launch_bounds__(kNT, (TrainCfg<FORM, T, CK, DT, CBW, true>::MI
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             hin.p[i] = apply(pA.p[i], hin.p[i], pB.p[i], seg);
-                    [[maybe_unused]] float2 hp = hin.p[i];
+            float2 hp = hin.p[i];
             if (rows > 0) {
 #pragma unroll
                 for (int j = 0; j < RT; ++j) {
-                    if constexpr (LEAN) {
-                        if ((resets & ((2u << j) - 1u)) == 0u) h[j].p[i] = ffma2(P[j].get(i), hin.p[i], h[j].p[i]);
-                    } else {
-                        const bool cut = ((resets >> j) & 1u) != 0u;
-                        h[j].p[i] = cut ? h[j].p[i] : ffma2(one_minus(na[j].p[i]), hp, h[j].p[i]);
-                        hp = h[j].p[i];
-                    }
+                    float2 a;
+                    if constexpr (LEAN) a = sig_only<T>(input(0, q * RT + j).p[i]);
+                    else a = one_minus(na[j].p[i]);
+                    hp = h[j].p[i] = ((resets >> j) & 1u) != 0u ? h[j].p[i] : ffma2(a, hp, h[j].p[i]);
                 }
             }
         }

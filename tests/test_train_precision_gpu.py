@@ -170,6 +170,35 @@ def test_decayed_states(cuda, dtype, B, ckpt):
     run_ssd(cuda, ssd, 2.5, 3.5, dtype, ckpt, (T + 16) * gate_error(dtype, 4, 3.5), parts=("y", "final"))
 
 
+@DTYPES
+@pytest.mark.parametrize("B", [2, 200])
+def test_decayed_states_in_the_backward(cuda, dtype, B):
+    """Gradients that hold such states."""
+    gated, ssd, T = decaying(dtype, B)
+    run_gated(cuda, gated, dtype, None, (T + 16) * gate_error(dtype, 4))
+    run_ssd(cuda, ssd, 2.5, 3.5, dtype, None, (T + 16) * gate_error(dtype, 4, 3.5))
+
+
+# ------------------------------------------------------------------ streams that hardly vary
+
+@DTYPES
+@pytest.mark.parametrize("B", [2, 200])
+def test_constant_stream(cuda, dtype, B):
+    """A stream at its own limit: h_t = w for good, so the decay's gradient, lam a (1 -
+    a) (h_{t-1} - w_t), is 0 but for the rounding of states to fp32 -- not of anything
+    held in 16 bits between the passes."""
+    gen = torch.Generator().manual_seed(2)
+    T, C = 16, 40
+    x = (100 * positive(gen, B, 1, C)).to(dtype).expand(B, T, C).contiguous()
+    g = torch.randn(B, 1, C, generator=gen).to(dtype).expand(B, T, C).contiguous()
+    z = (1 + 3 * torch.rand(B, T, C, generator=gen)).to(dtype)
+    h0 = (torch.sigmoid(g[:, 0].double()) * x[:, 0].double()).float()
+    go, gf = positive(gen, B, T, C).to(dtype), positive(gen, B, C)
+    run_gated(cuda, (x, z, g, h0, go, gf), dtype, None, (T + 16) * gate_error(dtype, 4))
+    xs = [x, g] + [torch.randn(B, T, C, generator=gen).to(dtype) for _ in range(3)]
+    run_ssd(cuda, (*xs, positive(gen, C), h0, go, gf), 0.001, 0.2, dtype, None, (T + 16) * gate_error(dtype, 4, 0.2))
+
+
 # ------------------------------------------------------------------ saturated gates
 
 def marks(gen, B, T):
@@ -219,5 +248,22 @@ def test_ssd_is_rounded_once(cuda, ckpt):
     ls = [t.to(cuda).requires_grad_() for t in (*xs, D, h0)]
     o = nk.ssd_scan_train(*ls[:6], 0.001, 0.2, h0=ls[6], return_final_state=True, checkpoint=ckpt)
     got = [o[0], *torch.autograd.grad(o, ls, [go.to(cuda), gf.to(cuda)])[:5]]
+    off = [turned(a, b) for a, b in zip(got, want)]
+    assert max(off) <= 0.02, off
+
+
+@CKPTS
+def test_gated_is_rounded_once(cuda, ckpt):
+    """As test_ssd_is_rounded_once."""
+    gen = torch.Generator().manual_seed(6)
+    B, T, C = 4, 200, 64
+    r = lambda *s: torch.randn(*s, generator=gen)  # noqa: E731
+    case, go, gf = [r(B, T, C).to(BF), (r(B, T, C) + 4).to(BF), r(B, T, C).to(BF), r(B, C)], r(B, T, C).to(BF), r(B, C)
+    ls = [t.double().requires_grad_() for t in case]
+    w = ref.gated(*ls, None, ckpt is not None)
+    want = [w[0], *torch.autograd.grad(w, ls, [go.double(), gf.double()])[:3]]
+    ls = [t.to(cuda).requires_grad_() for t in case]
+    o = nk.gated_scan_train(*ls[:3], h0=ls[3], return_final_state=True, checkpoint=ckpt)
+    got = [o[0], *torch.autograd.grad(o, ls, [go.to(cuda), gf.to(cuda)])[:3]]
     off = [turned(a, b) for a, b in zip(got, want)]
     assert max(off) <= 0.02, off
