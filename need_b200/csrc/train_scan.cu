@@ -270,24 +270,44 @@ __device__ __forceinline__ F4 row4_8(const unsigned char* slot, int r, int v, fl
     return f;
 }
 
+// A pair s, n = 1 - s in one number y: s where it is the smaller, else -n (s = 1: -0).
+__device__ __forceinline__ float2 smaller(float2 s, float2 n) {
+    return make_float2(s.x < 0.5f ? s.x : -n.x, s.y < 0.5f ? s.y : -n.y);
+}
+__device__ __forceinline__ float2 one_if_negative(float2 y) {  // by the sign bit: -0 too
+    return make_float2(__int_as_float((__float_as_int(y.x) >> 31) & 0x3f800000),
+                       __int_as_float((__float_as_int(y.y) >> 31) & 0x3f800000));
+}
+__device__ __forceinline__ float2 s_of(float2 y) { return fadd2(one_if_negative(y), y); }
+
 // What a sigmoid computed in phase 1 leaves in its stream's slot for phase 2, in place
-// of the logit: fp32 streams s itself.  A 16-bit slot cannot hold s to the precision the
+// of the logit: fp32 streams the smaller of s and 1 - s, each as the exponential gives
+// it, 1 - s with its sign turned; the other one follows by a subtraction that loses
+// nothing (from s alone, 1 - s at a logit of 16 was off by 6 %).  A 16-bit slot cannot hold s to the precision the
 // gradients are rounded to (f16 ends at 3e-8, bf16 has 8 bits): there the logit stays and
 // the sigmoid is computed again (bf16 backward: SSD 8x2048x832 77 us, GATED 16x4096x1024
 // 185; 75 and 182 with s kept as f16, wrong below 1e-5).
 template <typename T>
 constexpr bool kKeep = Ops<T>::BYTES == 4;
 template <typename T, int CB>
-__device__ __forceinline__ void keep4(unsigned char* slot, int r, int v, const F4& s) {
-    if constexpr (kKeep<T>) put4<float, CB>(slot, r, v, s);
+__device__ __forceinline__ void keep4(unsigned char* slot, int r, int v, const F4& s, const F4& n) {
+    if constexpr (kKeep<T>) {
+        F4 y;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) y.p[i] = smaller(s.p[i], n.p[i]);
+        put4<float, CB>(slot, r, v, y);
+    }
 }
 // s and s (1 - s) from a kept slot.
 template <typename T, int CB>
 __device__ __forceinline__ void kept4(const unsigned char* slot, int r, int v, F4& s, F4& slope) {
     static_assert(kKeep<T>, "kept as fp32");
-    s = row4<float, CB>(slot, r, v);
+    const F4 y = row4<float, CB>(slot, r, v);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) slope.p[i] = fmul2(s.p[i], fadd2(splat2(1.0f), make_float2(-s.p[i].x, -s.p[i].y)));
+    for (int i = 0; i < 2; ++i) {
+        s.p[i] = s_of(y.p[i]);
+        slope.p[i] = make_float2(fmaf(-y.p[i].x, y.p[i].x, fabsf(y.p[i].x)), fmaf(-y.p[i].y, y.p[i].y, fabsf(y.p[i].y)));
+    }
 }
 template <typename T>
 __device__ __forceinline__ F4 sig4(const F4& x) {
@@ -295,6 +315,19 @@ __device__ __forceinline__ F4 sig4(const F4& x) {
     s.p[0] = sig_only<T>(x.p[0]);
     s.p[1] = sig_only<T>(x.p[1]);
     return s;
+}
+// The same of a logit whose sigmoid phase 2 uses again.
+template <typename T, int CB>
+__device__ __forceinline__ F4 sig4_keep(unsigned char* slot, int r, int v, const F4& x) {
+    if constexpr (kKeep<T>) {
+        F4 s, n;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) sig_pair<T>(x.p[i], s.p[i], n.p[i]);
+        keep4<T, CB>(slot, r, v, s, n);
+        return s;
+    } else {
+        return sig4<T>(x);
+    }
 }
 
 // DT: how the SSD form gets a = e^-r (r <= dt_max): 0 any range, 1 dt_max <= 1/4.
@@ -566,15 +599,16 @@ __device__ __forceinline__ void load_rows(const TrainParams& p, const Tile& tl, 
     }
 }
 
-// a and 1 - a of the decay stream's four channels.
-template <int FORM, typename T, int DT>
-__device__ __forceinline__ void decay4(const TrainParams& p, const F4& x, F4& a, F4& na, F4& s) {
+// a and 1 - a of the decay stream's four channels, and of the SSD form's step s and (PAIR) 1 - s.
+template <int FORM, typename T, int DT, bool PAIR>
+__device__ __forceinline__ void decay4(const TrainParams& p, const F4& x, F4& a, F4& na, F4& s, F4& ns) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         if constexpr (FORM == FORM_GATED) {
             sig_pair<T>(x.p[i], a.p[i], na.p[i]);
         } else {
-            s.p[i] = sig_only<T>(x.p[i]);
+            if constexpr (PAIR) sig_pair<T>(x.p[i], s.p[i], ns.p[i]);
+            else s.p[i] = sig_only<T>(x.p[i]);
             const float2 r = ffma2(s.p[i], splat2(p.dt_scale), splat2(p.dt_min));
             if constexpr (DT == 1) exp_neg_small(r, a.p[i], na.p[i]);
             else exp_neg<T>(r, a.p[i], na.p[i]);
@@ -822,8 +856,8 @@ __global__ void __launch_bounds__(kNT, (TrainCfg<FORM, T, CK, DT, CBW, false>::M
 #pragma unroll
         for (int j = 0; j < RT; ++j) {
             const int r = q * RT + j;
-            F4 a, na, s;
-            decay4<FORM, T, DT>(p, row4<T, CB>(slot(0), r, v), a, na, s);
+            F4 a, na, s, ns;
+            decay4<FORM, T, DT, false>(p, row4<T, CB>(slot(0), r, v), a, na, s, ns);
             const F4 g = sig4<T>(row4<T, CB>(slot(1), r, v)), x = row4<T, CB>(slot(2), r, v);
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
@@ -1025,17 +1059,15 @@ __global__ void __launch_bounds__(kNT, (TrainCfg<FORM, T, CK, DT, CBW, true>::MI
 #pragma unroll
         for (int j = 0; j < RT; ++j) {
             const int r = q * RT + j;
-            F4 a, sd;
+            F4 a, sd, nd;
             F4& nj = na[LEAN ? 0 : j];
-            decay4<FORM, T, DT>(p, input(0, r), a, nj, sd);
-            const F4 g = sig4<T>(input(1, r)), x = input(2, r);
+            decay4<FORM, T, DT, kKeep<T>>(p, input(0, r), a, nj, sd, nd);
+            const F4 g = sig4_keep<T, CB>(stage(1), r, v, input(1, r)), x = input(2, r);
             F4 e = gout(r);
-            keep4<T, CB>(stage(1), r, v, g);
             if constexpr (FORM == FORM_SSD) {
-                const F4 sc = sig4<T>(input(3, r)), so = sig4<T>(input(4, r));
-                keep4<T, CB>(stage(0), r, v, sd);
-                keep4<T, CB>(stage(3), r, v, sc);
-                keep4<T, CB>(stage(4), r, v, so);
+                const F4 sc = sig4_keep<T, CB>(stage(3), r, v, input(3, r));
+                const F4 so = sig4_keep<T, CB>(stage(4), r, v, input(4, r));
+                keep4<T, CB>(stage(0), r, v, sd, nd);
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     const float2 gs = fmul2(e.p[i], so.p[i]);
@@ -1140,9 +1172,9 @@ __global__ void __launch_bounds__(kNT, (TrainCfg<FORM, T, CK, DT, CBW, true>::MI
                 put4<T, CB>(stage(3), r, v, d[3]);
                 put4<T, CB>(stage(4), r, v, d[4]);
             }
-            F4 sd, ld, aj, nj;
+            F4 sd, ld, nd, aj, nj;
             if constexpr (FORM == FORM_SSD) gate(0, r, sd, ld);
-            if constexpr (LEAN) decay4<FORM, T, DT>(p, input(0, r), aj, nj, sd);
+            if constexpr (LEAN) decay4<FORM, T, DT, false>(p, input(0, r), aj, nj, sd, nd);
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 const float2 n = LEAN ? nj.p[i] : na[LEAN ? 0 : j].p[i], a = LEAN ? aj.p[i] : one_minus(n);

@@ -212,7 +212,7 @@ SHAPES = pytest.mark.parametrize("B,T,C,resets", [(1, 70, 40, False), (2, 21, 72
 
 
 @CKPTS
-@pytest.mark.parametrize("dtype", [BF, HF], ids=["bf16", "f16"])
+@DTYPES
 @SHAPES
 @pytest.mark.parametrize("lo,hi", [(0.001, 0.2)])
 def test_saturated_gates_ssd(cuda, B, T, C, resets, lo, hi, dtype, ckpt):
