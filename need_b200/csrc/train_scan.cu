@@ -40,9 +40,9 @@
 // from the slots they were computed in.
 //
 // What bounds it (B200, bf16; the copy's rate is 6.55 TB/s):
-//   SSD 8x2048x832     forward 40 us, 4.1 TB/s; backward 73-76 us, 4.0-4.1 TB/s
+//   SSD 8x2048x832     forward 40 us, 4.1 TB/s; backward 77-78 us, 3.9 TB/s
 //   GATED 16x4096x1024 forward 107-108 us, 5.0 TB/s; backward 191 us, 4.9 TB/s
-//   8-bit copies: SSD 8x2048x832 64 and 89 us, GATED 16x4096x1024 161 and 215 us
+//   8-bit copies: SSD 8x2048x832 64 and 92 us, GATED 16x4096x1024 161 and 223 us
 // Neither DRAM nor any pipe is full: a tile's life is 2 us of loads, 1 to 1.6 us
 // of phase 1, 0.8 to 1.5 us until its carry is handed out (an L2 round trip to
 // the tile before) and 0.3 to 1 us of phase 2, and registers and shared memory
@@ -88,13 +88,13 @@ constexpr int kNW = 8;                 // row warps
 constexpr int kNT = (kNW + 1) * 32;    // threads: the row warps and the look-back warp
 // Tokens x channels per tile.  The wide GATED scans, with little to keep per
 // element, take tiles twice as long (16x4096x1024 bf16: forward 107 us against
-// 130 us, the bf16 backward, which keeps less, 191 against 209 us; with 8-bit copies
+// 130 us, the 16-bit backward, which keeps less, 191 against 209 us (f16 190, 213); with 8-bit copies
 // forward 161 against 201 us, and 47 against 68 us at 1x16384x832, whose chains are few);
 // the others lose more residents than they save (SSD 8x2048x832 backward 88 against 76
-// us; with 8-bit copies forward 76 against 64 us, GATED backward 260 against 215 us at
+// us; with 8-bit copies forward 76 against 64 us, GATED backward 260 against 223 us at
 // 16x4096x1024).
-__host__ __device__ constexpr int tile_elems(int form, bool bf16, bool ck, int cb, bool bwd) {
-    return form == FORM_GATED && cb == 64 && (!bwd || (bf16 && !ck)) ? 8192 : 4096;
+__host__ __device__ constexpr int tile_elems(int form, bool half, bool ck, int cb, bool bwd) {
+    return form == FORM_GATED && cb == 64 && (!bwd || (half && !ck)) ? 8192 : 4096;
 }
 constexpr int kNear = 3, kDeep = 5;    // tile maps composed before an inclusive carry
 constexpr int kHdrBytes = WS_HDR_WORDS * 4;
@@ -279,6 +279,10 @@ __device__ __forceinline__ float2 one_if_negative(float2 y) {  // by the sign bi
                        __int_as_float((__float_as_int(y.y) >> 31) & 0x3f800000));
 }
 __device__ __forceinline__ float2 s_of(float2 y) { return fadd2(one_if_negative(y), y); }
+__device__ __forceinline__ float2 n_of_s(float2 y) {
+    const float2 o = one_if_negative(y);
+    return make_float2((1.0f - o.x) - y.x, (1.0f - o.y) - y.y);
+}
 
 // What a sigmoid computed in phase 1 leaves in its stream's slot for phase 2, in place
 // of the logit: fp32 streams the smaller of s and 1 - s, each as the exponential gives
@@ -336,7 +340,7 @@ struct TrainCfg {
     static constexpr int NIN = FORM == FORM_GATED ? 3 : 5;
     static constexpr int IN_BYTES = (BWD && CK) ? 1 : Ops<T>::BYTES;  // per streamed input element
     static constexpr int CB = CB_, NC = CB / 32;                     // channels; of a look-back lane
-    static constexpr int L = tile_elems(FORM, std::is_same<T, __nv_bfloat16>::value, CK, CB, BWD) / CB;
+    static constexpr int L = tile_elems(FORM, Ops<T>::BYTES == 2, CK, CB, BWD) / CB;
     static constexpr int R = L / kNW;                                // tokens; rows per warp
     static_assert(CB == 32 || CB == 64, "32 or 64 channels per tile");
     static_assert(BWD || !CK || CB == kGroup, "the 8-bit forward sees whole groups");
@@ -930,10 +934,10 @@ __global__ void __launch_bounds__(kNT, (TrainCfg<FORM, T, CK, DT, CBW, true>::MI
     train_bwd_kernel(const __grid_constant__ TrainParams p) {
     using K = TrainCfg<FORM, T, CK, DT, CBW, true>;
     using O = Ops<T>;
-    // The long tiles of bf16 GATED: a is computed again for the states and in phase 2, and
+    // The long tiles of 16-bit GATED: a is computed again for the states and in phase 2, and
     // neither it nor 1 - a is kept (16x4096x1024 190 us; 209 kept, on short tiles 209).  The
-    // SSD form loses by it (75.5 against 72.8 us), and so do the 8-bit copies (226, 210).
-    constexpr bool LEAN = FORM == FORM_GATED && std::is_same<T, __nv_bfloat16>::value && !CK;
+    // SSD form loses by it (75.5 against 72.8 us), and so do the 8-bit copies (226, 223).
+    constexpr bool LEAN = FORM == FORM_GATED && Ops<T>::BYTES == 2 && !CK;
     extern __shared__ __align__(128) unsigned char base[];
     float2* s_map = reinterpret_cast<float2*>(base + K::OFF_MAP);
     float* s_fwd = reinterpret_cast<float*>(base + K::OFF_FWD);
@@ -1048,20 +1052,22 @@ __global__ void __launch_bounds__(kNT, (TrainCfg<FORM, T, CK, DT, CBW, true>::MI
 
     // phase 1: the thread's maps.  Forward: h_out = A h_in + B.  Backward, over
     // the same a: mu_first = A mu_in + M, M = sum over rows of (product of a up
-    // to the row) e.  1 - a stays in registers (and a = 1 - (1 - a): of the two
-    // the small one is the one whose relative error matters), b too, where the
-    // states then take its place.
-    F4 na[LEAN ? 1 : RT], h[RT], A, B, M, dD;
+    // to the row) e.  The smaller of a and 1 - a stays in registers (the other one
+    // follows without a loss), b too, where the states then take its place.
+    F4 ka[LEAN ? 1 : RT], h[RT], A, B, M, dD;
 #pragma unroll
     for (int i = 0; i < 2; ++i) A.p[i] = splat2(1.0f), B.p[i] = M.p[i] = dD.p[i] = splat2(0.0f);
     auto one_minus = [](float2 x) { return fadd2(splat2(1.0f), make_float2(-x.x, -x.y)); };
+    constexpr bool NEAR1 = FORM == FORM_SSD && DT == 1;  // a >= e^-1/4: it follows from 1 - a
+    auto keep_a = [&](float2 a, float2 n) { return NEAR1 ? n : smaller(a, n); };
+    auto a_of = [&](float2 y) { return NEAR1 ? one_minus(y) : s_of(y); };
+    auto n_of = [&](float2 y) { return NEAR1 ? y : n_of_s(y); };
     auto phase1 = [&](auto whole) {
 #pragma unroll
         for (int j = 0; j < RT; ++j) {
             const int r = q * RT + j;
-            F4 a, sd, nd;
-            F4& nj = na[LEAN ? 0 : j];
-            decay4<FORM, T, DT, kKeep<T>>(p, input(0, r), a, nj, sd, nd);
+            F4 a, na, sd, nd;
+            decay4<FORM, T, DT, kKeep<T>>(p, input(0, r), a, na, sd, nd);
             const F4 g = sig4_keep<T, CB>(stage(1), r, v, input(1, r)), x = input(2, r);
             F4 e = gout(r);
             if constexpr (FORM == FORM_SSD) {
@@ -1077,7 +1083,8 @@ __global__ void __launch_bounds__(kNT, (TrainCfg<FORM, T, CK, DT, CBW, true>::MI
             }
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                const float2 b = fmul2(nj.p[i], fmul2(g.p[i], x.p[i]));
+                const float2 b = fmul2(na.p[i], fmul2(g.p[i], x.p[i]));
+                if constexpr (!LEAN) ka[j].p[i] = keep_a(a.p[i], na.p[i]);
                 h[j].p[i] = b;
                 if constexpr (decltype(whole)::value) {
                     B.p[i] = j == 0 ? b : ffma2(a.p[i], B.p[i], b);
@@ -1130,7 +1137,7 @@ __global__ void __launch_bounds__(kNT, (TrainCfg<FORM, T, CK, DT, CBW, true>::MI
                 for (int j = 0; j < RT; ++j) {
                     float2 a;
                     if constexpr (LEAN) a = sig_only<T>(input(0, q * RT + j).p[i]);
-                    else a = one_minus(na[j].p[i]);
+                    else a = a_of(ka[j].p[i]);
                     hp = h[j].p[i] = ((resets >> j) & 1u) != 0u ? h[j].p[i] : ffma2(a, hp, h[j].p[i]);
                 }
             }
@@ -1177,7 +1184,8 @@ __global__ void __launch_bounds__(kNT, (TrainCfg<FORM, T, CK, DT, CBW, true>::MI
             if constexpr (LEAN) decay4<FORM, T, DT, false>(p, input(0, r), aj, nj, sd, nd);
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                const float2 n = LEAN ? nj.p[i] : na[LEAN ? 0 : j].p[i], a = LEAN ? aj.p[i] : one_minus(n);
+                const F4& k = ka[LEAN ? 0 : j];
+                const float2 a = LEAN ? aj.p[i] : a_of(k.p[i]), n = LEAN ? nj.p[i] : n_of(k.p[i]);
                 const float2 prev = reset ? splat2(0.0f) : (j > 0 ? h[j > 0 ? j - 1 : 0].p[i] : hin.p[i]);
                 const float2 lam = fadd2(e.p[i], mu.p[i]);
                 mu.p[i] = reset ? splat2(0.0f) : fmul2(a, lam);
@@ -1284,7 +1292,7 @@ struct Geom {
 Geom geom(int form, int dtype, bool ck, bool bwd, int64_t nb, int64_t T, int64_t C) {
     Geom g;
     g.CB = !ck && nb * ((C + 63) / 64) < (bwd ? 64 : 192) ? 32 : 64;
-    g.L = tile_elems(form == NEED_FORM_GATED ? FORM_GATED : FORM_SSD, dtype == NEED_BF16, ck, int(g.CB), bwd) / g.CB;
+    g.L = tile_elems(form == NEED_FORM_GATED ? FORM_GATED : FORM_SSD, dtype != NEED_F32, ck, int(g.CB), bwd) / g.CB;
     g.ncb = (C + g.CB - 1) / g.CB;
     g.nchains = nb * g.ncb;
     g.nchunks = (T + g.L - 1) / g.L;

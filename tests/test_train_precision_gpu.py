@@ -214,10 +214,22 @@ SHAPES = pytest.mark.parametrize("B,T,C,resets", [(1, 70, 40, False), (2, 21, 72
 @CKPTS
 @DTYPES
 @SHAPES
-@pytest.mark.parametrize("lo,hi", [(0.001, 0.2)])
-def test_saturated_gates_ssd(cuda, B, T, C, resets, lo, hi, dtype, ckpt):
+def test_saturated_gates_gated(cuda, B, T, C, resets, dtype, ckpt):
     """Logits to +-20: every gradient to its own last bits, where s, 1 - s or both
     their products are as small as 1e-17."""
+    gen = torch.Generator().manual_seed(3)
+    z, g = (40 * torch.rand(B, T, C, generator=gen) - 20 for _ in range(2))
+    case = [positive(gen, B, T, C), z, g, positive(gen, B, C), positive(gen, B, T, C), positive(gen, B, C)]
+    case = [t.to(dtype) if t.dim() == 3 else t for t in case]
+    run_gated(cuda, case, dtype, ckpt, (T + 16) * gate_error(dtype, 20), marks(gen, B, T) if resets else None)
+
+
+@CKPTS
+@DTYPES
+@SHAPES
+@pytest.mark.parametrize("lo,hi", [(0.001, 0.2), (0.0, 12.0)])
+def test_saturated_gates_ssd(cuda, B, T, C, resets, lo, hi, dtype, ckpt):
+    """The same; with steps to 12, where e^-r is small too."""
     gen = torch.Generator().manual_seed(4)
     logits = [40 * torch.rand(B, T, C, generator=gen) - 20 for _ in range(4)]
     case = [positive(gen, B, T, C), *logits, positive(gen, C), positive(gen, B, C), positive(gen, B, T, C), positive(gen, B, C)]
