@@ -128,22 +128,25 @@ struct TrainParams {
 };
 
 // ------------------------------------------------------------------ maps
-// Affine maps c -> A c + B.  With segments in the call (`seg`), A == 0 means
-// "drops c", whatever c holds.
+// Affine maps c -> A c + B.  With segments in the call (`seg`), A == -0 means "drops
+// c", whatever c holds.  A product of a's is never negative: one that has underflowed is
+// +0, and an infinity or NaN that it multiplies stays in its segment.
+__device__ __forceinline__ float2 drop2() { return splat2(-0.0f); }
+__device__ __forceinline__ bool drops(float A) { return __float_as_uint(A) == 0x80000000u; }
 __device__ __forceinline__ float2 apply(float2 A, float2 c, float2 B, bool seg) {
     float2 r = ffma2(A, c, B);
-    if (seg) r = make_float2(A.x == 0.0f ? B.x : r.x, A.y == 0.0f ? B.y : r.y);
+    if (seg) r = make_float2(drops(A.x) ? B.x : r.x, drops(A.y) ? B.y : r.y);
     return r;
 }
 __device__ __forceinline__ float apply(float A, float c, float B, bool seg) {
-    return seg && A == 0.0f ? B : fmaf(A, c, B);
+    return seg && drops(A) ? B : fmaf(A, c, B);
 }
 __device__ __forceinline__ float mulz(float a, float b, bool seg) {
-    return seg && (a == 0.0f || b == 0.0f) ? 0.0f : a * b;
+    return seg && (drops(a) || drops(b)) ? -0.0f : a * b;
 }
 __device__ __forceinline__ float2 mulz(float2 a, float2 b, bool seg) {
     float2 r = fmul2(a, b);
-    if (seg) r = make_float2(a.x == 0.0f || b.x == 0.0f ? 0.0f : r.x, a.y == 0.0f || b.y == 0.0f ? 0.0f : r.y);
+    if (seg) r = make_float2(drops(a.x) || drops(b.x) ? -0.0f : r.x, drops(a.y) || drops(b.y) ? -0.0f : r.y);
     return r;
 }
 
@@ -872,7 +875,7 @@ __global__ void __launch_bounds__(kNT, (TrainCfg<FORM, T, CK, DT, CBW, false>::M
                 } else if (r < rows) {
                     const bool cut = ((resets >> j) & 1u) != 0u;
                     B.p[i] = cut ? b : ffma2(a.p[i], B.p[i], b);
-                    A.p[i] = (resets & ((2u << j) - 1u)) != 0u ? splat2(0.0f) : fmul2(a.p[i], A.p[i]);
+                    A.p[i] = (resets & ((2u << j) - 1u)) != 0u ? drop2() : fmul2(a.p[i], A.p[i]);
                 }
                 H[j].p[i] = B.p[i];
             }
@@ -1093,7 +1096,7 @@ __global__ void __launch_bounds__(kNT, (TrainCfg<FORM, T, CK, DT, CBW, true>::MI
                 } else if (r < rows) {
                     B.p[i] = ((resets >> j) & 1u) != 0u ? b : ffma2(a.p[i], B.p[i], b);
                     if ((resets & ((2u << j) - 1u)) != 0u) {
-                        A.p[i] = splat2(0.0f);
+                        A.p[i] = drop2();
                     } else {
                         A.p[i] = fmul2(a.p[i], A.p[i]);
                         M.p[i] = ffma2(A.p[i], e.p[i], M.p[i]);
