@@ -22,17 +22,18 @@ __device__ __forceinline__ void sig_pair(float2 x, float2& s, float2& n) {
         s = make_float2(x.x < 0.0f ? m0 : r0, x.y < 0.0f ? m1 : r1);
         n = make_float2(x.x < 0.0f ? r0 : m0, x.y < 0.0f ? r1 : m1);
     } else {
-        // the exponent is capped at 2^126, so that t s stays a number; a NaN passes through
+        // e^-x may overflow: s is then 0 -- not the least number, which times a value near
+        // the type's largest is no zero -- and t s is not a number.  Below x = 0 the
+        // difference is exact enough
         const float2 k = fmul2(x, splat2(-1.4426950408889634f));
-        float e0, e1, t0, t1;
-        asm("min.NaN.f32 %0, %1, 0f42FC0000;" : "=f"(e0) : "f"(k.x));
-        asm("min.NaN.f32 %0, %1, 0f42FC0000;" : "=f"(e1) : "f"(k.y));
-        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(t0) : "f"(e0));
-        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(t1) : "f"(e1));
+        float t0, t1;
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(t0) : "f"(k.x));
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(t1) : "f"(k.y));
         const float2 d = fadd2(make_float2(t0, t1), splat2(1.0f));
         asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s.x) : "f"(d.x));
         asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s.y) : "f"(d.y));
-        n = fmul2(make_float2(t0, t1), s);
+        const float2 m = fmul2(make_float2(t0, t1), s), c = fadd2(splat2(1.0f), make_float2(-s.x, -s.y));
+        n = make_float2(k.x > 0.0f ? c.x : m.x, k.y > 0.0f ? c.y : m.y);
     }
 }
 

@@ -42,3 +42,45 @@ def test_a_bad_value_lasts_to_the_end_of_its_segment(cuda, dtype, B, segments):
         assert torch.equal(h[0, :, 5].isnan().cpu(), (rows >= 20) & (rows < last))
         assert int(h.isnan().sum()) == last - 20 and bool(f[0, 5].isnan()) != segments
         assert torch.equal(dx[0, :, 6].isnan().cpu(), (rows >= first) & (rows <= 560))
+
+
+# ------------------------------------------------------------------ the type's lowest value
+
+@DTYPES
+@pytest.mark.parametrize("K", [1, 3])
+def test_conv_of_the_lowest_value(cuda, dtype, K):
+    """silu and its slope are 0 far below 0, however far: nothing is left of the type's
+    lowest value, which padding may hold (and whose s = 2^-126 would leave 4).  Bound: half
+    a step and 2^-18 (a gate's few ulp and six products) of the largest result."""
+    B, T, C = 2, 37, 24
+    gen = torch.Generator().manual_seed(5)
+    u, go = (torch.randn(B, T, C, generator=gen).to(dtype) for _ in range(2))
+    w = 0.1 + 0.2 * torch.rand(C, K, generator=gen)
+    u[0, 10] = torch.finfo(dtype).min
+    u[1, 20] = -90.0
+    l64 = [t.double().requires_grad_() for t in (u, w)]
+    y64 = ref.conv_silu(*l64, None)
+    want = [y64, torch.autograd.grad(y64, l64, go.double())[0]]
+    ls = [t.to(cuda).requires_grad_() for t in (u, w)]
+    y = nk.ssd_conv_silu_train(*ls)
+    got = [y, torch.autograd.grad(y, ls, go.to(cuda))[0]]
+    for a, b in zip(got, want):
+        off = (a.detach().cpu().double() - b.detach()).abs()
+        assert float(off.max()) <= (torch.finfo(dtype).eps / 2 + 2.0 ** -18) * float(b.detach().abs().max())
+
+
+@DTYPES
+@pytest.mark.parametrize("B", [1, 200])
+def test_a_closed_decay_gate_drops_the_lowest_value(cuda, dtype, B):
+    """decay_logit far below 0 (-1000, -inf): nothing of the state before is left, though
+    it is near the type's largest."""
+    T, C = 70, 40
+    z = torch.full((B, T, C), 3.0, dtype=dtype)
+    x, g = torch.zeros(B, T, C, dtype=dtype), torch.full((B, T, C), 30.0, dtype=dtype)
+    x[:, 4] = torch.finfo(dtype).min
+    z[:, 5], z[:, 4] = -1000.0, -1000.0
+    z[:, 5, 7] = -float("inf")
+    with torch.no_grad():
+        h, f = nk.gated_scan_train(x.to(cuda), z.to(cuda), g.to(cuda), return_final_state=True)
+    assert bool((h[:, 4] <= 0.99 * torch.finfo(dtype).min).all())
+    assert not bool(h[:, 5:].any()) and not bool(f.any())
