@@ -254,7 +254,9 @@ __global__ void __launch_bounds__(32 * kRanges, kBlocks) conv_train_kernel(const
                     if constexpr (!BWD) {
                         y[e] = fmul2(v, s);
                     } else {
-                        const float2 dv = fmul2(fmul2(widen(g[i].h[e]), s), ffma2(v, m, splat2(1.0f)));
+                        float2 dv = fmul2(fmul2(widen(g[i].h[e]), s), ffma2(v, m, splat2(1.0f)));
+                        // behind the sequence gout is 0, but v may be past fp32 where none of its rows is
+                        if (!ALL && tg + i >= tin) dv = splat2(0.0f);
 #pragma unroll
                         for (int d = 0; d < K; ++d)
                             if (reach(d)) du[W + i - d][e] = ffma2(w[d][e], dv, du[W + i - d][e]);

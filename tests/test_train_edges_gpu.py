@@ -84,3 +84,18 @@ def test_a_closed_decay_gate_drops_the_lowest_value(cuda, dtype, B):
         h, f = nk.gated_scan_train(x.to(cuda), z.to(cuda), g.to(cuda), return_final_state=True)
     assert bool((h[:, 4] <= 0.99 * torch.finfo(dtype).min).all())
     assert not bool(h[:, 5:].any()) and not bool(f.any())
+
+
+@pytest.mark.parametrize("dtype", [FP, BF], ids=["f32", "bf16"])
+@pytest.mark.parametrize("T", [1, 2, 5, 64, 67])
+def test_conv_rows_behind_the_sequence(cuda, dtype, T):
+    """The last input overflows only in rows that the sequence does not have: its own
+    gradient is w[K-1] dv, dv = 1 (silu's slope far above 0), and no NaN."""
+    u = torch.zeros(2, T, 8, dtype=dtype, device=cuda)
+    u[:, T - 1] = 2.0 ** 126
+    w = torch.tensor([[8.0, 8.0, 0.5]], device=cuda).repeat(8, 1).requires_grad_()
+    u.requires_grad_()
+    y = nk.ssd_conv_silu_train(u, w)
+    du, dw = torch.autograd.grad(y, [u, w], torch.ones_like(y))
+    assert bool((y[:, T - 1] == 2.0 ** 125).all()) and bool((du[:, T - 1] == 0.5).all())
+    assert bool(du.isfinite().all()) and bool(dw.isfinite().all())
