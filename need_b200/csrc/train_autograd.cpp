@@ -124,6 +124,14 @@ bool wants_grad(std::initializer_list<const Tensor*> ts) {
     return false;
 }
 
+// Whether one of them carries a forward-mode tangent.  A node refuses it; a plain launch
+// would drop it.
+bool has_tangent(std::initializer_list<const Tensor*> ts) {
+    for (const Tensor* t : ts)
+        if (t->defined() && t->_fw_grad(0).defined()) return true;
+    return false;
+}
+
 // Under create_graph: gradients of these gradients raise instead of being left out.
 variable_list once(variable_list g) {
     if (!at::GradMode::is_enabled()) return g;
@@ -254,7 +262,8 @@ variable_list scan_train(int64_t form, variable_list x, const Tensor& seg_, Tens
     }
     const Tensor none;
     const Tensor &x3 = x.size() > 3 ? x[3] : none, &x4 = x.size() > 4 ? x[4] : none;
-    if (!wants_grad({&h0, &d_skip, &x[0], &x[1], &x2, &x3, &x4})) {  // nothing to keep
+    const std::initializer_list<const Tensor*> all{&h0, &d_skip, &x[0], &x[1], &x2, &x3, &x4};
+    if (!wants_grad(all) && !has_tangent(all)) {  // nothing to keep
         at::NoGradGuard no_grad;
         for (Tensor& t : x) t = channels(t);
         ScanOut r = scan_forward({form, B, T, C, dt_min, dt_max, false}, x, seg, h0, d_skip);

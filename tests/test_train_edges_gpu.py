@@ -99,3 +99,33 @@ def test_conv_rows_behind_the_sequence(cuda, dtype, T):
     du, dw = torch.autograd.grad(y, [u, w], torch.ones_like(y))
     assert bool((y[:, T - 1] == 2.0 ** 125).all()) and bool((du[:, T - 1] == 0.5).all())
     assert bool(du.isfinite().all()) and bool(dw.isfinite().all())
+
+
+# ------------------------------------------------------------------ other kinds of differentiation
+
+@pytest.mark.parametrize("op", ["gated", "ssd", "conv", "norm"])
+def test_forward_mode_and_transforms_raise(cuda, op):
+    """A tangent is refused, not dropped, also where nothing asks for a gradient; so are
+    torch.func's transforms."""
+    import torch.autograd.forward_ad as fa
+    x, D = torch.randn(2, 6, 16, device=cuda), torch.ones(16, device=cuda)
+    w = torch.ones(16, 1, 3, device=cuda)
+    f = {"gated": lambda t: nk.gated_scan_train(x, t, x), "ssd": lambda t: nk.ssd_scan_train(x, x, t, x, x, D, 0.001, 0.2),
+         "conv": lambda t: nk.ssd_conv_silu_train(t, w), "norm": lambda t: nk.rms_norm_train(t, D)}[op]
+    with fa.dual_level():
+        dual = fa.make_dual(x, torch.ones_like(x))
+        with pytest.raises(RuntimeError):
+            f(dual)
+        with torch.no_grad(), pytest.raises(RuntimeError):
+            f(dual)
+    if op == "gated":
+        h0 = torch.zeros(2, 16, device=cuda)
+        with fa.dual_level(), pytest.raises(RuntimeError):
+            nk.gated_scan_train(x, x, x, h0=fa.make_dual(h0, torch.ones_like(h0)))
+    for transform in (lambda: torch.func.jvp(f, (x,), (x,)), lambda: torch.vmap(f)(torch.stack([x, x])),
+                      lambda: torch.func.grad(lambda t: f(t).sum())(x)):
+        with pytest.raises(RuntimeError):
+            transform()
+    assert not f(x).requires_grad
+    with torch.inference_mode():
+        assert torch.equal(f(x), f(x.clone()))
