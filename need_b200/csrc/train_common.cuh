@@ -37,6 +37,22 @@ __device__ __forceinline__ void sig_pair(float2 x, float2& s, float2& n) {
     }
 }
 
+// s and its slope s (1 - s) = t s^2 of a 16-bit pair.  Where e^-x overflows s is 0, and so
+// is the slope: t is capped for it.  A NaN stays in s.
+template <typename T>
+__device__ __forceinline__ void sig_slope(float2 x, float2& s, float2& slope) {
+    static_assert(Ops<T>::BYTES == 2, "fp32 streams keep their sigmoids");
+    const float2 k = fmul2(x, splat2(-1.4426950408889634f));
+    float t0, t1;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(t0) : "f"(k.x));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(t1) : "f"(k.y));
+    const float2 d = fadd2(make_float2(t0, t1), splat2(1.0f));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s.x) : "f"(d.x));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s.y) : "f"(d.y));
+    constexpr float top = 0x1p126f;
+    slope = fmul2(fmul2(make_float2(fminf(t0, top), fminf(t1, top)), s), s);
+}
+
 // s alone (e^-x may overflow: s is then 0)
 template <typename T>
 __device__ __forceinline__ float2 sig_only(float2 x) {

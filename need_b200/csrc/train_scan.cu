@@ -1045,11 +1045,7 @@ __global__ void __launch_bounds__(kNT, (TrainCfg<FORM, T, CK, DT, CBW, true>::MI
         } else {
             const F4 x = input(k, r);
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                float2 n;
-                sig_pair<T>(x.p[i], s.p[i], n);
-                slope.p[i] = fmul2(s.p[i], n);
-            }
+            for (int i = 0; i < 2; ++i) sig_slope<T>(x.p[i], s.p[i], slope.p[i]);
         }
     };
 

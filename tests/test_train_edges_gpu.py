@@ -129,3 +129,22 @@ def test_forward_mode_and_transforms_raise(cuda, op):
     assert not f(x).requires_grad
     with torch.inference_mode():
         assert torch.equal(f(x), f(x.clone()))
+
+
+@DTYPES
+@pytest.mark.parametrize("far", [-86.0, -87.5, -88.5, -1000.0, -float("inf")])
+def test_a_closed_gate_drops_the_lowest_value(cuda, dtype, far):
+    """An input gate as far below 0: the type's lowest input leaves nothing, in the output
+    or in any gradient that the true one (e^far of it) does not."""
+    B, T, C = 2, 40, 24
+    x = torch.full((B, T, C), torch.finfo(dtype).min, dtype=dtype, device=cuda).requires_grad_()
+    g = torch.full((B, T, C), far, dtype=dtype, device=cuda).requires_grad_()
+    z = torch.zeros(B, T, C, dtype=dtype, device=cuda).requires_grad_()
+    o, D = torch.zeros_like(z, requires_grad=True), torch.zeros(C, device=cuda)
+    # half of e^far of the input enters, twice that is in the state
+    size = float(torch.exp(torch.tensor(far, dtype=torch.float64).to(dtype).double())) * torch.finfo(dtype).max
+    for call in (lambda: nk.gated_scan_train(x, z, g), lambda: nk.ssd_scan_train(x, g, o, z, o, D, 0.7, 0.7)):
+        y = call()
+        assert float(y.detach().abs().max()) <= 1.01 * size
+        for d in torch.autograd.grad(y, [x, z, g], torch.ones_like(y)):
+            assert bool(d.isfinite().all()) and float(d.abs().max()) <= 2.02 * size + 2.0 ** -20
