@@ -517,6 +517,19 @@ NEED_API int need_scan_train_forward(const need_scan_train_args* args, need_stre
  * depend on the order in which blocks run. */
 NEED_API int need_scan_train_backward(const need_scan_train_args* args, need_stream_t stream);
 
+/* Reads (and clears) the current device's error word of the training scans: bit 0 = a
+ * look-back wait gave up, bit 1 = a tile load wait gave up, in any call on the device
+ * since the word was last read (a call's outputs are NaN where they depend on such a
+ * wait).  The call's own workspace holds its bits too (need_workspace_error).  Covers
+ * calls that `stream` has finished or waited for; synchronises `stream`. */
+NEED_API int need_scan_train_error(uint32_t* error_out, need_stream_t stream);
+
+/* Test hook, no counterpart in the reference: with on != 0 every load wait of the
+ * training scans launched afterwards in this process gives up at once (sets bit 1 of the
+ * error word, lets the copies land and passes NaN on); 0 restores the default (2^22
+ * polls).  Nothing is read or written out of bounds and every wait ends. */
+NEED_API void need_test_scan_train_load_give_up(int32_t on);
+
 /* Workspace bytes of need_conv_silu_train_backward. */
 NEED_API size_t need_conv_silu_train_workspace_size(int32_t K, int64_t nb, int64_t T, int64_t C);
 

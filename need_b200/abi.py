@@ -178,6 +178,8 @@ SIGNATURES = {
     "need_scan_train_workspace_size": (c_size_t, [c_int32, c_int32, c_int32, c_int32, c_int64, c_int64, c_int64]),
     "need_scan_train_forward": (c_int32, [POINTER(NeedScanTrainArgs), c_void_p]),
     "need_scan_train_backward": (c_int32, [POINTER(NeedScanTrainArgs), c_void_p]),
+    "need_scan_train_error": (c_int32, [POINTER(c_uint32), c_void_p]),
+    "need_test_scan_train_load_give_up": (None, [c_int32]),
     "need_conv_silu_train_workspace_size": (c_size_t, [c_int32, c_int64, c_int64, c_int64]),
     "need_conv_silu_train_forward": (c_int32, [POINTER(NeedConvTrainArgs), c_void_p]),
     "need_conv_silu_train_backward": (c_int32, [POINTER(NeedConvTrainArgs), c_void_p]),

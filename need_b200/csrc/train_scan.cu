@@ -60,8 +60,8 @@
 // workspace carries nothing from one call to the next, and graphs that captured
 // calls can be replayed in any order.  Blocks start in the order of the tiles
 // (chains along x, positions along y and z), so the tiles a block waits for are
-// resident or finished.  Every wait is bounded; a tile that gives up sets the
-// workspace's error word and passes NaN on.
+// resident or finished.  Every wait is bounded; one that gives up sets a bit of the
+// device's error word (need_scan_train_error) and passes NaN on.
 //
 // Checkpoints in 8 bits: the forward also writes its inputs as e4m3 with one
 // power of two per token and 64 channels, and the backward reads those (5 + 2
@@ -124,8 +124,17 @@ struct TrainParams {
     uint32_t* hdr;
     unsigned long long* agg;  // [ntiles][CB] (A, B)
     uint32_t* incl;           // [ntiles][CB] the carry past the tile
-    uint32_t polls;
+    uint32_t polls, load_polls;  // before a wait for another tile's records, or for this warp's loads, gives up
 };
+
+// What the waits that gave up have set since need_scan_train_error last read it: a call's
+// workspace is gone when it returns, so its own word cannot tell.
+__device__ uint32_t g_train_error;
+__device__ __forceinline__ void give_up(const TrainParams& p, uint32_t bit) {
+    atomicOr(&p.hdr[WS_ERROR], bit);
+    atomicOr(&g_train_error, bit);
+}
+__device__ __forceinline__ float nan32() { return __int_as_float(0x7fc00000); }
 
 // ------------------------------------------------------------------ maps
 // Affine maps c -> A c + B.  With segments in the call (`seg`), A == -0 means "drops
@@ -441,17 +450,14 @@ __device__ __forceinline__ Ch<NC> look_back(const TrainParams& p, int64_t tile, 
         }
         if (mapped && have) break;
         if (!have && it >= p.polls) {  // go on without a predecessor's carry
-            if (lane == 0) atomicOr(&p.hdr[WS_ERROR], ERR_LOOKBACK);
+            if (lane == 0) give_up(p, ERR_LOOKBACK);
 #pragma unroll
-            for (int k = 0; k < NC; ++k) carry.v[k] = __int_as_float(0x7fc00000);
+            for (int k = 0; k < NC; ++k) carry.v[k] = nan32();
             have = true;
-        } else if (have && it - min(it, p.polls) >= kTmaPolls) {  // the row warps' own waits are shorter
-            if (lane == 0) atomicOr(&p.hdr[WS_ERROR], ERR_TMA);
+        } else if (have && it - min(it, p.polls) >= kTmaPolls) {  // without this tile's maps: NaN for all its warps
+            if (lane == 0) give_up(p, ERR_TMA);
 #pragma unroll
-            for (int k = 0; k < NC; ++k) {
-                A.v[k] = 0.0f;
-                B.v[k] = __int_as_float(0x7fc00000);
-            }
+            for (int k = 0; k < NC; ++k) A.v[k] = B.v[k] = nan32();
             break;
         }
     }
@@ -469,7 +475,7 @@ __device__ __forceinline__ Ch<NC> look_back(const TrainParams& p, int64_t tile, 
         const int w = REV ? kNW - 1 - n : n;
 #pragma unroll
         for (int k = 0; k < NC; ++k) {
-            s_in[w * CB + lane * NC + k] = c.v[k];
+            s_in[w * CB + lane * NC + k] = mapped ? c.v[k] : nan32();
             const float2 m = map_of(w, k);
             c.v[k] = apply(m.x, c.v[k], m.y, seg);
         }
@@ -603,6 +609,22 @@ __device__ __forceinline__ void load_rows(const TrainParams& p, const Tile& tl, 
             asm volatile("cp.async.wait_all;" ::: "memory");
             __syncwarp();
         }
+    }
+}
+
+// Waits for them.  Rows whose wait runs out become NaN in every stream (all bits set, in
+// e4m3 too), and with them whatever depends on them -- once the copies have landed, which
+// a second wait gives them time for.
+template <typename T, int N, int NIN, int IN_BYTES, int R, int CB, class Slot>
+__device__ __forceinline__ void await_rows(const TrainParams& p, int rows, int lane, uint64_t* bar, Slot slot) {
+    const bool late = rows > 0 && !mbar_wait_bounded(bar, 0, p.load_polls);
+    if (__any_sync(0xffffffffu, late)) {
+        if (lane == 0) give_up(p, ERR_TMA);
+        mbar_wait_bounded(bar, 0, kTmaPolls);
+        for (int k = 0; k < N; ++k)
+            for (int i = lane; i < R * CB * (k < NIN ? IN_BYTES : int(sizeof(T))) / 4; i += 32)
+                reinterpret_cast<uint32_t*>(slot(k))[i] = ~0u;
+        __syncwarp();
     }
 }
 
@@ -840,10 +862,7 @@ __global__ void __launch_bounds__(kNT, (TrainCfg<FORM, T, CK, DT, CBW, false>::M
         D.p[0] = ld_pair(p.dskip, c, p.C);
         D.p[1] = ld_pair(p.dskip, c + 2, p.C);
     }
-    if (rows > 0 && !mbar_wait_bounded(&s_bar[warp], 0, kTmaPolls)) {
-        atomicOr(&p.hdr[WS_ERROR], ERR_TMA);
-        mbar_wait_bounded(&s_bar[warp], 0, kTmaPolls);
-    }
+    await_rows<T, K::NIN, K::NIN, K::IN_BYTES, K::R, K::CB>(p, rows, lane, &s_bar[warp], slot);
 
     // The copies before phase 1, which writes into the slots they are made from: they
     // delay the tile's map, but kept in registers the products spill (GATED 16x4096x1024
@@ -993,7 +1012,14 @@ __global__ void __launch_bounds__(kNT, (TrainCfg<FORM, T, CK, DT, CBW, true>::MI
                 }
                 return ready;
             });
-        if (!handed) named_arrive(1, kNT);  // gave up: the row warps are let go
+        if (!handed) {  // gave up: the row warps are let go, with NaN
+#pragma unroll
+            for (int w = 0; w < kNW; ++w)
+#pragma unroll
+                for (int k = 0; k < K::NC; ++k) s_hin[w * K::CB + K::NC * lane + k] = nan32();
+            __syncwarp();
+            named_arrive(1, kNT);
+        }
         __syncwarp();
         named_arrive(2, kNT);
         if (last && p.grad_h0 != nullptr) st_ch(p.grad_h0 + int64_t(tl.b) * p.C, c, p.C, past);
@@ -1029,10 +1055,7 @@ __global__ void __launch_bounds__(kNT, (TrainCfg<FORM, T, CK, DT, CBW, true>::MI
         D.p[0] = ld_pair(p.dskip, c, p.C);
         D.p[1] = ld_pair(p.dskip, c + 2, p.C);
     }
-    if (rows > 0 && !mbar_wait_bounded(&s_bar[warp], 0, kTmaPolls)) {
-        atomicOr(&p.hdr[WS_ERROR], ERR_TMA);
-        mbar_wait_bounded(&s_bar[warp], 0, kTmaPolls);
-    }
+    await_rows<T, K::NIN + 1, K::NIN, K::IN_BYTES, K::R, K::CB>(p, rows, lane, &s_bar[warp], slot);
     auto input = [&](int k, int r) {
         if constexpr (CK) return row4_8<CB>(slot(k), r, v, s_scale[(warp * K::NIN + k) * K::R + r]);
         else return row4<T, CB>(slot(k), r, v);
@@ -1232,6 +1255,7 @@ __global__ void __launch_bounds__(kNT, (TrainCfg<FORM, T, CK, DT, CBW, true>::MI
 
 // ------------------------------------------------------------------ launch
 constexpr unsigned kMaxGridY = 65535;
+std::atomic<bool> g_load_give_up{false};  // need_test_scan_train_load_give_up
 
 template <class Kern>
 int launch(Kern kern, int smem, std::atomic<uint64_t>& done, const TrainParams& P, cudaStream_t s) {
@@ -1445,6 +1469,7 @@ int prepare(const need_scan_train_args* a, bool bwd, TrainParams* P, Geom* g) {
     P->incl = reinterpret_cast<uint32_t*>(ws + kHdrBytes + size_t(g->ntiles) * size_t(g->CB) * 8);
     P->dpart = reinterpret_cast<float*>(ws + clear_bytes(*g));
     P->polls = lookback_polls();
+    P->load_polls = g_load_give_up.load(std::memory_order_relaxed) ? 0 : kTmaPolls;
     return NEED_OK;
 }
 
@@ -1466,6 +1491,19 @@ size_t need_scan_train_workspace_size(int32_t form, int32_t dtype, int32_t check
     if (nb < 1 || T < 1 || C < 1) return kHdrBytes;
     return ws_size(geom(form, dtype, checkpoint != 0, backward != 0, nb, T, C), nb, C, backward != 0 && form == NEED_FORM_SSD);
 }
+
+int need_scan_train_error(uint32_t* error_out, need_stream_t stream) {
+    if (error_out == nullptr) return fail(NEED_ERR_INVALID, "null argument");
+    void* word = nullptr;
+    cudaError_t e = cudaGetSymbolAddress(&word, g_train_error);
+    if (e == cudaSuccess) e = cudaMemcpyAsync(error_out, word, 4, cudaMemcpyDeviceToHost, stream);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(stream);
+    if (e == cudaSuccess && *error_out != 0) e = cudaMemsetAsync(word, 0, 4, stream);
+    if (e != cudaSuccess) return cuda_fail(e, "need_scan_train_error");
+    return ok();
+}
+
+void need_test_scan_train_load_give_up(int32_t on) { g_load_give_up.store(on != 0, std::memory_order_relaxed); }
 
 int need_scan_train_forward(const need_scan_train_args* args, need_stream_t stream) {
     TrainParams P;

@@ -100,9 +100,13 @@ def workspace(dev: torch.device, nbytes: int, kind: str = "scan", stream: Option
 
 
 def workspace_error(dev: Optional[torch.device] = None) -> int:
-    """Reads and clears the device error word of this stream's workspace (synchronises)."""
+    """Reads and clears the device error words of this stream's workspaces and, over all
+    its calls, of the device's training scans (synchronises)."""
     dev = dev or torch.device("cuda", torch.cuda.current_device())
-    err = 0
+    word = ctypes.c_uint32(0)
+    with torch.cuda.device(dev):
+        abi.check("need_scan_train_error", _lib().need_scan_train_error(ctypes.byref(word), _stream(dev)))
+    err = int(word.value)
     for kind in ("scan", "assoc"):
         ws = _workspaces.get((dev.index, torch.cuda.current_stream(dev).cuda_stream, kind))
         if ws is not None:

@@ -4,6 +4,7 @@ import pytest
 import torch
 
 import train_reference as ref
+from need_b200 import abi
 from need_b200 import need_kernels as nk
 
 pytestmark = pytest.mark.gpu
@@ -148,3 +149,74 @@ def test_a_closed_gate_drops_the_lowest_value(cuda, dtype, far):
         assert float(y.detach().abs().max()) <= 1.01 * size
         for d in torch.autograd.grad(y, [x, z, g], torch.ones_like(y)):
             assert bool(d.isfinite().all()) and float(d.abs().max()) <= 2.02 * size + 2.0 ** -20
+
+
+# ------------------------------------------------------------------ waits that run out
+
+ERR_LOOKBACK, ERR_LOAD = 1, 2
+
+
+@pytest.mark.parametrize("ckpt", [None, F8], ids=["full", "8bit"])
+def test_look_back_that_gives_up_is_reported(cuda, ckpt):
+    """4 polls, far less than a tile needs to load: forward or backward, the launch ends,
+    the error word says so, what depends on the break is NaN, and the next call is right."""
+    lib = abi.load()
+    gen = torch.Generator(device=cuda).manual_seed(1)
+    ls = [torch.randn(2, 2048, 512, device=cuda, generator=gen).to(BF).requires_grad_() for _ in range(3)]
+    go = torch.randn(2, 2048, 512, device=cuda, generator=gen).to(BF)
+    run = lambda: nk.gated_scan_train(*ls, checkpoint=ckpt)  # noqa: E731
+    nk.workspace_error()
+    h = run()
+    good = [h, *torch.autograd.grad(h, ls, go, retain_graph=True)]
+    assert nk.workspace_error() == 0
+    for call in (lambda: [run()], lambda: torch.autograd.grad(h, ls, go, retain_graph=True)):
+        lib.need_test_set_lookback_polls(4)
+        try:
+            bad = call()
+            torch.cuda.synchronize()
+        finally:
+            lib.need_test_set_lookback_polls(0)
+        for a, b in zip(bad, good[:1] if len(bad) == 1 else good[1:]):
+            assert bool(((a == b) | a.isnan()).all()) and bool(a.isnan().any())
+        assert nk.workspace_error() == ERR_LOOKBACK and nk.workspace_error() == 0
+    assert all(torch.equal(a, b) for a, b in zip([run(), *torch.autograd.grad(h, ls, go)], good))
+
+
+@pytest.mark.parametrize("ckpt", [None, F8], ids=["full", "8bit"])
+@DTYPES
+@pytest.mark.parametrize("B", [2, 200])
+def test_load_that_gives_up_is_reported(cuda, dtype, B, ckpt):
+    """Every load wait gives up: all results are NaN, none a number made of whatever the
+    rows held, and the error word says so, for a call on any stream."""
+    lib = abi.load()
+    T, C = 100, 40
+    gen = torch.Generator(device=cuda).manual_seed(2)
+    xs = [torch.randn(B, T, C, device=cuda, generator=gen).to(dtype).requires_grad_() for _ in range(5)]
+    D, h0 = torch.ones(C, device=cuda, requires_grad=True), torch.zeros(B, C, device=cuda, requires_grad=True)
+    go = torch.randn(B, T, C, device=cuda, generator=gen).to(dtype)
+    for leaves, run in (([*xs[:3], h0], lambda *a: nk.gated_scan_train(*a[:3], h0=a[3], return_final_state=True, checkpoint=ckpt)),
+                        ([*xs, D, h0], lambda *a: nk.ssd_scan_train(*a[:6], 0.001, 0.2, h0=a[6], return_final_state=True,
+                                                                    checkpoint=ckpt))):
+        nk.workspace_error()
+        good = run(*leaves)
+        want = torch.autograd.grad(good[0], leaves, go, retain_graph=True)
+        assert nk.workspace_error() == 0
+        s = torch.cuda.Stream(cuda)
+        s.wait_stream(torch.cuda.current_stream(cuda))
+        lib.need_test_scan_train_load_give_up(1)
+        try:
+            with torch.cuda.stream(s):
+                bad = run(*(t.detach() for t in leaves))
+                kept = run(*leaves)  # with what the backward keeps
+            grads = torch.autograd.grad(good[0], leaves, go, retain_graph=True)
+            torch.cuda.synchronize()
+        finally:
+            lib.need_test_scan_train_load_give_up(0)
+        assert all(bool(t.isnan().all()) for t in (*bad, *kept, *grads))
+        assert nk.workspace_error() == ERR_LOAD and nk.workspace_error() == 0
+        after = torch.autograd.grad(kept[0], leaves[:-1], go)
+        if ckpt:  # the copies it made are NaN,
+            assert all(bool(t.isnan().all()) for t in after)
+        assert any(bool(t.isnan().any()) for t in after)  # and the state it kept at token 64 is
+        again = torch.autograd.grad(good[0], leaves, go)
+        assert all(torch.equal(a, b) for a, b in zip(again, want))
