@@ -258,7 +258,7 @@ variable_list scan_train(int64_t form, variable_list x, const Tensor& seg_, Tens
         Tensor out = x[0];
         for (size_t k = 1; k < x.size(); ++k) out = out * x[k];
         if (d_skip.defined()) out = (out * d_skip).to(x2.scalar_type());
-        return {out, h0.defined() ? h0 : at::zeros({B, C}, x2.options().dtype(at::kFloat))};
+        return {out, h0.defined() ? h0.clone() : at::zeros({B, C}, x2.options().dtype(at::kFloat))};
     }
     const Tensor none;
     const Tensor &x3 = x.size() > 3 ? x[3] : none, &x4 = x.size() > 4 ? x[4] : none;

@@ -220,3 +220,19 @@ def test_load_that_gives_up_is_reported(cuda, dtype, B, ckpt):
         assert any(bool(t.isnan().any()) for t in after)  # and the state it kept at token 64 is
         again = torch.autograd.grad(good[0], leaves, go)
         assert all(torch.equal(a, b) for a, b in zip(again, want))
+
+
+# ------------------------------------------------------------------ empty calls
+
+@pytest.mark.parametrize("B,T,C", [(2, 0, 8), (0, 4, 8), (2, 4, 0)])
+def test_an_empty_call_returns_a_state_of_its_own(cuda, B, T, C):
+    """The final state of an empty call is a new tensor, as that of any other: updated in
+    place it leaves the caller's h0 alone."""
+    x, D = torch.zeros(B, T, C, device=cuda), torch.ones(C, device=cuda)
+    h0 = torch.ones(B, C, device=cuda)
+    for call in (lambda: nk.gated_scan_train(x, x, x, h0=h0, return_final_state=True),
+                 lambda: nk.ssd_scan_train(x, x, x, x, x, D, 0.001, 0.2, h0=h0, return_final_state=True)):
+        out, final = call()
+        assert out.shape == x.shape and torch.equal(final, h0)
+        final.add_(1)
+        assert bool((h0 == 1).all())
