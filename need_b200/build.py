@@ -55,7 +55,12 @@ def _ext_stale() -> bool:
 
 
 def _ext_command() -> list:
-    """The host compile of the autograd module (no torch import: its headers are found by path)."""
+    """The host compile of the autograd module (no torch import: its headers are found by path).
+
+    The C++ library is named as the shared one that torch runs on: a compiler that finds only
+    the archive (a $CXX of its own tree) would link a second copy into the module, whose
+    locale is not the one torch's exports have set up, and a stream that formats a number
+    there ends the process."""
     import importlib.util
     import sysconfig
     torch_dir = os.path.dirname(importlib.util.find_spec("torch").origin)
@@ -65,7 +70,7 @@ def _ext_command() -> list:
             "-DTORCH_EXTENSION_NAME=_train", "-DTORCH_API_INCLUDE_EXTENSION_H", f"-I{INCLUDE}",
             *[x for d in inc for x in ("-isystem", d)], os.path.join(CSRC, EXT_SOURCE), "-o", EXT + ".tmp",
             "-L" + os.path.join(torch_dir, "lib"), "-L" + LIBDIR, "-l:libneed_scan.so", "-lc10", "-lc10_cuda", "-ltorch",
-            "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python", "-Wl,-rpath,$ORIGIN"]
+            "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python", "-nostdlib++", "-l:libstdc++.so.6", "-lm", "-Wl,-rpath,$ORIGIN"]
 
 
 def build(force: bool = False, verbose: bool = False) -> str:

@@ -18,7 +18,6 @@
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/extension.h>
 
-#include <cstdio>
 #include <stdexcept>
 #include <string>
 
@@ -32,32 +31,13 @@ namespace {
 
 constexpr int64_t kSpan = 64, kGroup = 64;  // need_scan_train_chunk_len(), need_scan_train_group()
 
-// Error texts.  Not by iostreams (TORCH_CHECK's arguments included): in this
-// process a stream's number formatting, compiled outside torch's own libraries,
-// can end in a segmentation fault.
-std::string str(const char* s) { return s; }
-std::string str(int64_t v) { return std::to_string(v); }
-std::string str(double v) {
-    char buf[32];
-    std::snprintf(buf, sizeof(buf), "%g", v);
-    return buf;
-}
-std::string str(at::IntArrayRef v) {
-    std::string r = "[";
-    for (size_t i = 0; i < v.size(); ++i) r += (i ? ", " : "") + std::to_string(v[i]);
-    return r + "]";
-}
-template <class... Args>
-std::string text(const Args&... args) {
-    return (str(args) + ...);
-}
 template <class... Args>
 void check_value(bool ok, const Args&... args) {
-    if (!ok) throw py::value_error(text(args...));
+    if (!ok) throw py::value_error(c10::str(args...));
 }
 void check(const char* fn, int rc) {
     if (rc != NEED_OK)
-        throw std::runtime_error(text(fn, " failed (status ", int64_t(rc), "): ", need_last_error()));
+        throw std::runtime_error(c10::str(fn, " failed (status ", rc, "): ", need_last_error()));
 }
 
 int32_t dtype_of(at::ScalarType t) {
@@ -71,13 +51,14 @@ OptTensor opt(const Tensor& t) { return t.defined() ? OptTensor(t) : std::nullop
 
 // CUDA tensors of one device, x of a dtype the kernels take.
 void check_tensors(const char* name, const Tensor& x, std::initializer_list<const Tensor*> others) {
-    if (!x.is_cuda()) throw std::runtime_error("need_b200 kernels take CUDA tensors only (no CPU fallback)");
+    if (!x.is_cuda())
+        throw std::runtime_error(c10::str(name, " takes CUDA tensors only (no CPU fallback); got ", x.sizes(), " on ", x.device()));
     for (const Tensor* t : others)
         if (t->defined() && t->device() != x.device())
             throw std::runtime_error("all tensors must be on the same CUDA device (no CPU fallback)");
     const auto ty = x.scalar_type();
     if (ty != at::kFloat && ty != at::kBFloat16 && ty != at::kHalf)
-        throw py::type_error(text(name, " takes fp32, bf16 or f16 data; got ", c10::toString(ty)));
+        throw py::type_error(c10::str(name, " takes fp32, bf16 or f16 data; got ", c10::toString(ty)));
 }
 // The reset mask as the kernels read it.
 Tensor mask_of(const Tensor& seg, int64_t B, int64_t T) {
