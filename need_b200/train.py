@@ -12,8 +12,11 @@ every gate op as its torch path does.
 
 ``checkpoint=torch.float8_e4m3fn`` keeps the activations the backward needs in 8
 bits (one power-of-two scale per token and 64 channels) instead of the inputs
-themselves: half the memory of 16-bit inputs, provided nothing else holds them.
-The forward's results are unchanged.  The gradient is the formula's at the
+themselves: half the memory of 16-bit inputs, provided nothing else holds them -- a
+chunk of a projection that another operator saves holds all of it, so give
+``ssd_conv_silu_train`` a ``u`` of its own there (see it).  Outputs are those without
+it, but for the order of a few fp32 sums (such a call may take other tiles).  The
+gradient is the formula's at the
 stored values; the recurrences start every 64-token chunk from the true fp32
 state.  A group that holds an infinity or NaN gives NaN gradients.
 
@@ -110,7 +113,12 @@ def ssd_conv_silu_train(u: torch.Tensor, weight: torch.Tensor, bias: Optional[to
     in fp32, rounded once to ``u.dtype``.  ``weight`` is the Conv1d weight [C, 1,
     K] (or [C, K]), K <= 4, ``bias`` [C] or None, both used in fp32.  Differentiable
     in all three.  ``seg_start`` [B, T]: inputs before a token's segment start do
-    not feed it."""
+    not feed it.
+
+    The backward keeps ``u`` as it is given, in the memory it lies in.  Where ``u`` is
+    a chunk of a projection whose other chunks are kept in 8 bits only, pass
+    ``u.contiguous()``: the projection can then be freed (2 bytes an element instead
+    of 10)."""
     return _ext().conv_train(u, weight, bias, seg_start)
 
 
