@@ -365,9 +365,10 @@ NormPlan norm_plan(int64_t nvec) {
     pl.rpb = std::max(1, 8 / pl.wpr);
     return pl;
 }
-// Blocks of the backward: as many as are resident at once, so that every block
-// walks the same number of rows (8x2048x832 bf16: 18 us; 23 us with 3 per SM), and few enough that the partial rows they leave are a small part of the
-// traffic.
+// Blocks of the backward: as many as are resident at once where rows take up to 8 warps,
+// so that blocks walk the same number of rows or one more (8x2048x832 bf16: 18 us; 23 us with 3
+// per SM), and few enough that the partial rows they leave are a small part of the
+// traffic.  Rows of 16 warps (past 16 KB) leave one block on an SM: two waves.
 constexpr int kBwdBlocks = 148 * 2;
 int64_t bwd_blocks(int64_t rows, const NormPlan& pl) {
     return std::max<int64_t>(1, std::min<int64_t>(kBwdBlocks, (rows + pl.rpb - 1) / pl.rpb));

@@ -374,9 +374,12 @@ struct TrainCfg {
     // CTAs per SM that registers are planned for (16 bit: 56 to 96 registers).  Most of
     // a tile's time is latency -- its loads 2 us, the carry 1 us -- so residents count for
     // more than a few spilled registers: SSD 8x2048x832 forward 40 us at 4, 44 at 3;
-    // backward 76 at 3, 87 at 2; with 8-bit copies the SSD backward 94 at 2, 102 at 3,
-    // the GATED one of 16x4096x1024 268 at 2, 215 at 3.
-    static constexpr int MINB = Ops<T>::BYTES == 4 ? 2 : BWD ? (CK && FORM == FORM_SSD ? 2 : 3) : (CK || L * CB > 4096 ? 3 : 4);
+    // backward 76 at 3, 87 at 2; the GATED one of 16x4096x1024 with 8-bit copies 268 at 2,
+    // 215 at 3 (before its gates were computed again: 221 now).  The SSD backward with 8-bit
+    // copies: shared memory holds two tiles, of fp32 one (registers for three 102 us, for two
+    // 94; fp32 for two 244, for one 238).
+    static constexpr bool SSD8 = BWD && CK && FORM == FORM_SSD;
+    static constexpr int MINB = Ops<T>::BYTES == 4 ? (SSD8 ? 1 : 2) : BWD ? (SSD8 ? 2 : 3) : (CK || L * CB > 4096 ? 3 : 4);
 };
 
 // ------------------------------------------------------------------ look-back
@@ -1306,12 +1309,21 @@ struct Geom {
     int64_t L, CB, ncb, nchains, nchunks, ntiles;
 };
 // Channels per tile.  64 where the call has enough chains to fill the device;
-// 32 (tiles twice as long) where it has not: then fewer tiles of one chain are in
-// flight and wait for each other's carries, against more shuffles in a warp, of
-// which the backward has three times the forward's (bf16 device us, 64 / 32
-// channels: SSD 1x16384x832, 13 chains of 64, 156 / 134 the pass; 8x2048x832, 104,
-// 43 / 40 forward, 76 / 79 backward; gated 16x4096x1024, 256, 302 / 355 the pass).
-// The 8-bit forms keep the 64 that share a scale.
+// 32 (tiles twice as long, where those of 64 are not long already) where it has not: then
+// fewer tiles of one chain are in flight and wait for each other's carries, against more
+// shuffles in a warp, of which the backward has three times the forward's.  The 8-bit
+// forms keep the 64 that share a scale.  The bounds are those of the SSD form in 16 bits;
+// device us at 832 channels, 64 / 32 wide, forward and backward:
+//   chains of 64      13 (1x16384)              104 (8x2048)              208 (16x1024)
+//   SSD bf16     62.7 / 45.2, 86.1 / 82.9   41.8 / 39.1, 74.2 / 77.2   39.3 / 39.0, 73.1 / 77.1
+//   SSD f16      63.2 / 45.1, 86.2 / 82.5   41.8 / 38.8, 74.7 / 77.4   39.6 / 38.9, 73.8 / 77.7
+//   SSD fp32     110 / 103, 162 / 160       98.6 / 98.4, 154 / 153     99.0 / 98.3, 152 / 152
+//   GATED bf16   35.1 / 35.5, 50.2 / 55.7   27.6 / 29.7, 45.2 / 49.9   26.8 / 29.3, 45.2 / 49.7
+//   GATED f16    34.7 / 35.4, 49.9 / 55.6   27.3 / 29.9, 45.3 / 50.0   26.6 / 29.6, 45.0 / 49.9
+//   GATED fp32   63.2 / 57.7, 100 / 98.0    56.6 / 51.0, 91.2 / 92.4   56.4 / 51.6, 90.1 / 91.4
+// So the GATED form in 16 bits, whose 64-wide tiles are the long ones, pays up to a tenth
+// for the one rule at 13 to 191 chains (below 8 it gains by it: 4x8192x64 backward 20.3 /
+// 16.5), and its fp32 forward a tenth above 191.
 Geom geom(int form, int dtype, bool ck, bool bwd, int64_t nb, int64_t T, int64_t C) {
     Geom g;
     g.CB = !ck && nb * ((C + 63) / 64) < (bwd ? 64 : 192) ? 32 : 64;
