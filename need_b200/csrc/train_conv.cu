@@ -19,9 +19,9 @@
 //
 // What bounds it (B200, bf16, K = 3): 4 B move per element forward, 6 B backward;
 // 8x2048x832 12 us (4.5 TB/s) and 25 us (3.3 TB/s), 16x4096x1024 146 us the pass (4.6
-// TB/s).  The backward issues 63 instructions per row of a warp, 54 % of its issue
-// slots.  With the next group in registers in place of shared memory, one group ahead
-// and 32 tokens, the passes took 45 and 180 us.
+// TB/s).  Nothing is full backward (58 % of the issue slots, 25 % of the warps active): a
+// thread's walk over its rows, in one wave and a fifth.  With the next group in registers
+// in place of shared memory, one group ahead and 32 tokens, the passes took 45 and 180 us.
 #include <string.h>
 
 #include <type_traits>

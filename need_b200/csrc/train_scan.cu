@@ -40,9 +40,9 @@
 // from the slots they were computed in.
 //
 // What bounds it (B200, bf16; the copy's rate is 6.55 TB/s):
-//   SSD 8x2048x832     forward 40 us, 4.1 TB/s; backward 77-78 us, 3.9 TB/s
-//   GATED 16x4096x1024 forward 107-108 us, 5.0 TB/s; backward 191 us, 4.9 TB/s
-//   8-bit copies: SSD 8x2048x832 64 and 92 us, GATED 16x4096x1024 161 and 223 us
+//   SSD 8x2048x832     forward 40 us, 4.1 TB/s; backward 75-77 us, 3.9-4.0 TB/s
+//   GATED 16x4096x1024 forward 109 us, 4.9 TB/s; backward 195 us, 4.8 TB/s (resets: 112, 204)
+//   8-bit copies: SSD 8x2048x832 64 and 92 us, GATED 16x4096x1024 164 and 221 us
 // Neither DRAM nor any pipe is full: a tile's life is 2 us of loads, 1 to 1.6 us
 // of phase 1, 0.8 to 1.5 us until its carry is handed out (an L2 round trip to
 // the tile before) and 0.3 to 1 us of phase 2, and registers and shared memory
@@ -88,7 +88,7 @@ constexpr int kNW = 8;                 // row warps
 constexpr int kNT = (kNW + 1) * 32;    // threads: the row warps and the look-back warp
 // Tokens x channels per tile.  The wide GATED scans, with little to keep per
 // element, take tiles twice as long (16x4096x1024 bf16: forward 107 us against
-// 130 us, the 16-bit backward, which keeps less, 191 against 209 us (f16 190, 213); with 8-bit copies
+// 130 us, the 16-bit backward, which keeps less, 191 against 209 us (f16 189, 213); with 8-bit copies
 // forward 161 against 201 us, and 47 against 68 us at 1x16384x832, whose chains are few);
 // the others lose more residents than they save (SSD 8x2048x832 backward 88 against 76
 // us; with 8-bit copies forward 76 against 64 us, GATED backward 260 against 223 us at
@@ -302,7 +302,7 @@ __device__ __forceinline__ float2 n_of_s(float2 y) {
 // nothing (from s alone, 1 - s at a logit of 16 was off by 6 %).  A 16-bit slot cannot hold s to the precision the
 // gradients are rounded to (f16 ends at 3e-8, bf16 has 8 bits): there the logit stays and
 // the sigmoid is computed again (bf16 backward: SSD 8x2048x832 77 us, GATED 16x4096x1024
-// 185; 75 and 182 with s kept as f16, wrong below 1e-5).
+// 185; 75 and 182 with s kept as f16, which was wrong below 1e-5).
 template <typename T>
 constexpr bool kKeep = Ops<T>::BYTES == 4;
 template <typename T, int CB>
@@ -545,8 +545,8 @@ __device__ __forceinline__ uint32_t reset_bits(const TrainParams& p, const Tile&
 // A warp's rows of stream k with ordinary loads, as TMA would leave them (zeros past C
 // and T), U elements each.  4 and 8 bytes are copied asynchronously, so that all streams
 // are on their way together; the caller waits (SSD 8 x 2048 bf16, forward / backward us:
-// C = 828, 8 bytes, 57 / 93; 830, 4 bytes, 66 / 107; 831, one element a load, 86 / 145;
-// 832 by TMA 40 / 75).
+// C = 828, 8 bytes, 57 / 96; 830, 4 bytes, 67 / 107; 831, one element a load, 87 / 142;
+// 832 by TMA 40 / 76).
 template <typename T, int R, int CB, int U>
 __device__ __forceinline__ void plain_units(const TrainParams& p, const Tile& tl, const T* src, int64_t st,
                                             unsigned char* slot, int rows, int lane) {
@@ -960,7 +960,8 @@ __global__ void __launch_bounds__(kNT, (TrainCfg<FORM, T, CK, DT, CBW, true>::MI
     using K = TrainCfg<FORM, T, CK, DT, CBW, true>;
     using O = Ops<T>;
     // The long tiles of 16-bit GATED: a is computed again for the states and in phase 2, and
-    // neither it nor 1 - a is kept (16x4096x1024 190 us; 209 kept, on short tiles 209).  The
+    // neither it nor 1 - a is kept (16x4096x1024 191 us; kept in registers 209 on short tiles
+    // and on long ones, in the logits' slots and registers 220 against 195).  The
     // SSD form loses by it (75.5 against 72.8 us), and so do the 8-bit copies (226, 223).
     constexpr bool LEAN = FORM == FORM_GATED && Ops<T>::BYTES == 2 && !CK;
     extern __shared__ __align__(128) unsigned char base[];

@@ -16,16 +16,16 @@ themselves: half the memory of 16-bit inputs, provided nothing else holds them -
 chunk of a projection that another operator saves holds all of it, so give
 ``ssd_conv_silu_train`` a ``u`` of its own there (see it).  Outputs are those without
 it, but for the order of a few fp32 sums (such a call may take other tiles).  The
-gradient is the formula's at the
-stored values; the recurrences start every 64-token chunk from the true fp32
-state.  A group that holds an infinity or NaN gives NaN gradients.
+gradient is the formula's at the stored values; the recurrences start every 64-token
+chunk from the true fp32 state.  A group that holds an infinity or NaN gives NaN
+gradients.
 
 All take CUDA tensors of one device in fp32, bf16 or f16, run on the current
 stream, allocate their scratch per call, and can be captured into CUDA graphs.
 Rows of their results are 16-byte aligned: where C elements are not a whole number
 of 16 bytes, the rows lie further apart than C and the result is not contiguous.
-Gradients of gradients raise.  The autograd nodes are compiled
-(csrc/train_autograd.cpp, ``_lib/_train.so``); there is no other path.
+Gradients of gradients and forward-mode tangents raise.  The autograd nodes are
+compiled (csrc/train_autograd.cpp, ``_lib/_train.so``); there is no other path.
 """
 from __future__ import annotations
 
