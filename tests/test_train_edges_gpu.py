@@ -1,5 +1,7 @@
 """The training operators at the edges of their documentation, on the GPU: values that
 are not finite or the type's lowest, calls that they refuse, waits that run out."""
+import threading
+
 import pytest
 import torch
 
@@ -236,3 +238,54 @@ def test_an_empty_call_returns_a_state_of_its_own(cuda, B, T, C):
         assert out.shape == x.shape and torch.equal(final, h0)
         final.add_(1)
         assert bool((h0 == 1).all())
+
+
+# ------------------------------------------------------------------ calls at once
+
+def test_calls_at_once(cuda):
+    """Threads on streams of their own, and captured passes replayed on two streams at
+    once: every result is that of the call alone."""
+    gen = torch.Generator(device=cuda).manual_seed(7)
+    jobs = []
+    for B, T, C, dtype, ckpt in ((2, 700, 200, BF, None), (3, 333, 136, FP, F8), (40, 150, 64, HF, None), (1, 2000, 328, BF, F8)):
+        xs = [torch.randn(B, T, C, device=cuda, generator=gen).to(dtype).requires_grad_() for _ in range(5)]
+        D, go = torch.ones(C, device=cuda, requires_grad=True), torch.randn(B, T, C, device=cuda, generator=gen).to(dtype)
+
+        def job(xs=xs, D=D, go=go, ckpt=ckpt):
+            ls = [t.detach().requires_grad_() for t in (*xs, D)]  # leaves of its own: their streams are the caller's
+            y = nk.ssd_scan_train(*ls, 0.001, 0.2, checkpoint=ckpt)
+            h = nk.gated_scan_train(*ls[:3], checkpoint=ckpt)
+            return [y, h, *torch.autograd.grad([y, h], ls, [go, go])]
+
+        jobs.append((job, [t.detach() for t in job()]))
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(job, want):
+        with torch.cuda.stream(torch.cuda.Stream(cuda)):
+            for _ in range(10):
+                got = job()
+                if not all(torch.equal(a, b) for a, b in zip(got, want)):
+                    wrong.append(job)
+
+    threads = [threading.Thread(target=work, args=j) for j in jobs]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+    graphs = []
+    for job, want in jobs[:2]:
+        s = torch.cuda.Stream(cuda)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=s):
+            got = job()
+        graphs.append((graph, s, got, want))
+    for _ in range(5):
+        for graph, s, _, _ in graphs:
+            with torch.cuda.stream(s):
+                graph.replay()
+    torch.cuda.synchronize()
+    for _, _, got, want in graphs:
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    assert nk.workspace_error() == 0
