@@ -88,11 +88,11 @@ constexpr int kNW = 8;                 // row warps
 constexpr int kNT = (kNW + 1) * 32;    // threads: the row warps and the look-back warp
 // Tokens x channels per tile.  The wide GATED scans, with little to keep per
 // element, take tiles twice as long (16x4096x1024 bf16: forward 107 us against
-// 130 us, the 16-bit backward, which keeps less, 191 against 209 us (f16 189, 213); with 8-bit copies
-// forward 161 against 201 us, and 47 against 68 us at 1x16384x832, whose chains are few);
-// the others lose more residents than they save (SSD 8x2048x832 backward 88 against 76
-// us; with 8-bit copies forward 76 against 64 us, GATED backward 260 against 223 us at
-// 16x4096x1024).
+// 130 us, the 16-bit backward, which keeps less, 191 against 209 us (f16 189, 213);
+// with 8-bit copies forward 161 against 201 us, and 47 against 68 us at 1x16384x832,
+// whose chains are few); the others lose more residents than they save (SSD 8x2048x832
+// backward 88 against 76 us; with 8-bit copies forward 76 against 64 us, GATED backward
+// 303 against 223 us at 16x4096x1024).
 __host__ __device__ constexpr int tile_elems(int form, bool half, bool ck, int cb, bool bwd) {
     return form == FORM_GATED && cb == 64 && (!bwd || (half && !ck)) ? 8192 : 4096;
 }
