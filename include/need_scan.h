@@ -312,6 +312,70 @@ typedef struct {
     size_t workspace_bytes;
 } need_norm_train_args;
 
+/* A tensor of heads: [nb, T, heads, features], features next to each other. */
+typedef struct {
+    const void* ptr;
+    int64_t stride_b, stride_t, stride_h;  /* elements */
+    int64_t heads;         /* divides H: heads h * heads / H .. share one */
+} need_heads;
+
+#define NEED_LINEAR_ATTENTION_MAX_DK 128
+
+typedef struct {
+    int32_t dtype;         /* NEED_F32, NEED_BF16 or NEED_F16: q, k, v and out */
+    float scale;
+    int64_t nb, T, H, dk, dv;
+    need_heads q, k, v;    /* dk features of q and k, dv of v */
+    const float* log_decay; int64_t ld_stride_b, ld_stride_t, ld_stride_h; /* [nb, T, H]; strides may be 0 */
+    const uint8_t* seg_start; int64_t seg_stride_b, seg_stride_t;          /* optional [nb, T] */
+    const float* state;    /* optional [nb, H, dk, dv] contiguous: before the first token */
+    float* final_state;    /* optional, likewise: after the last */
+    void* out; int64_t out_stride_b, out_stride_t, out_stride_h;           /* [nb, T, H, dv] */
+    void* workspace; size_t workspace_bytes;
+} need_linear_attention_args;
+
+typedef struct {
+    int32_t dtype;         /* q, k, v and out */
+    float scale;
+    int64_t n, H, dk, dv;  /* n tokens, one of each sequence */
+    need_heads q, k, v;    /* stride_b from token to token; stride_t unused */
+    const float* log_decay; int64_t ld_stride_n, ld_stride_h;
+    float* state; int64_t state_stride; int64_t slots;  /* [slots][H, dk, dv contiguous], updated in place */
+    const int32_t* slot;   /* optional [n]: the state of each token (default i) */
+    void* out; int64_t out_stride_n, out_stride_h;
+} need_linear_attention_step_args;
+
+typedef struct {
+    int32_t dtype;         /* x, y, stream, and out without out8 */
+    int32_t out8;          /* 1: out in 8 bits with scales */
+    int64_t rows, C, group;  /* group: channels of a scale, 32, 64, 128 or C (out8 only) */
+    const void* x; int64_t x_stride;   /* [rows, C], element strides between rows */
+    const void* y; int64_t y_stride;
+    const float* weight;   /* [C] */
+    double eps, scale;
+    void* stream; int64_t stream_stride;
+    void* out; int64_t out_stride;     /* elements (out8: bytes) */
+    float* scales;         /* out8: [rows, ceil(C / group)] contiguous */
+} need_residual_norm_args;
+
+#define NEED_TOKEN_LOG_PROBS_MAX_TOP 32
+
+typedef struct {
+    int32_t dtype, top;    /* of logits and grad; alternatives per row */
+    int64_t rows, V;
+    const void* logits; int64_t stride;   /* [rows, V], element stride between rows */
+    const int64_t* tokens; /* [rows] */
+    double temperature;
+    float* log_prob;       /* [rows] */
+    float* entropy;        /* [rows] */
+    float* stats;          /* [rows, 2]: the largest logit, log(sum exp) less it (kept for the backward) */
+    float* top_log_probs; int64_t* top_tokens;  /* [rows, top] */
+    const float* g_log_prob; const float* g_entropy;  /* backward: [rows], either may be null */
+    void* grad; int64_t grad_stride;      /* backward: [rows, V] */
+    void* workspace; size_t workspace_bytes;
+} need_token_log_probs_args;
+
+
 /* Version of this header the library was built from. */
 NEED_API int need_abi_version(void);
 
@@ -553,6 +617,55 @@ NEED_API int need_rms_norm_train_forward(const need_norm_train_args* args, need_
  * grad_x = rstd (g - n sum(g n) / C), grad_weight = sum over rows of gout n.
  * With checkpoint, x is the stored 8-bit values and rstd the true row's. */
 NEED_API int need_rms_norm_train_backward(const need_norm_train_args* args, need_stream_t stream);
+
+/* ------------------------------------------------------------------------ */
+/* Language-model operators beside the scan                                  */
+/* ------------------------------------------------------------------------ */
+
+/* Workspace bytes of need_linear_attention: the states between the parts that a
+ * prompt is cut into where there are few sequences and heads. */
+NEED_API size_t need_linear_attention_workspace_size(int64_t nb, int64_t T, int64_t H, int64_t dk, int64_t dv);
+
+/* Linear attention with a decay for each head (the matrix-state form of the
+ * retention scan: need_core.py:1590-1592 keeps k v by element where this keeps
+ * k^T v), over whole prompts:
+ *     S_t = exp(log_decay_t) S_{t-1} + k_t^T v_t,   out_t = scale q_t S_t,
+ * sums and states in fp32, out rounded once.  At a marked token, or one whose log
+ * decay is -infinity, the state before it is dropped, whatever it holds.  At most
+ * NEED_LINEAR_ATTENTION_MAX_DK features a head. */
+NEED_API int need_linear_attention(const need_linear_attention_args* args, need_stream_t stream);
+
+/* The same for one token of each of n sequences, whose states in a pool are
+ * updated in place.  A negative slot: no sequence (out 0, nothing updated).  A
+ * slot outside the pool, or one that an earlier token of the call has: out NaN,
+ * nothing updated for it. */
+NEED_API int need_linear_attention_step(const need_linear_attention_step_args* args, need_stream_t stream);
+
+/* The residual's addition and the norm of what it gives, one pass (need_kernels
+ * residual_scale_add and rms_norm, need_kernels.py:294-299, :266-276, whose 16-bit
+ * torch forms round in between): per row in fp32,
+ *     stream = x + scale y  (rounded to dtype),
+ *     n = stream / sqrt(sum(stream^2) / C + eps) weight,
+ * out = n rounded to dtype, or with out8 e4m3(n / 2^e), scales = 2^e for each
+ * `group` channels, e the least exponent >= -126 that fits every |n| under 448 2^e
+ * (a group with an infinity or NaN: scale NaN).  Rows of up to 32 KB. */
+NEED_API int need_residual_rms_norm(const need_residual_norm_args* args, need_stream_t stream);
+
+/* Workspace bytes of need_token_log_probs: the parts of rows that are cut up where
+ * there are few. */
+NEED_API size_t need_token_log_probs_workspace_size(int32_t dtype, int64_t rows, int64_t V, int32_t top);
+
+/* Of each row x = logits / temperature, p = softmax(x): log p(token), the entropy
+ * -sum p log p, and the `top` largest log p with their tokens, in order, the lower
+ * token first where they are equal.  fp32.  Logits of -infinity have p = 0; where fewer
+ * than `top` others are left the rest are -infinity, token -1.  A row of nothing else
+ * has log p = -infinity, entropy 0.  A row with a NaN or +infinity gives NaN (NaN orders
+ * above +infinity).  A negative token: none given, log p 0.  One >= V: NaN. */
+NEED_API int need_token_log_probs(const need_token_log_probs_args* args, need_stream_t stream);
+
+/* Its gradient: grad = (g (token's one-hot - p) - gh p (log p + entropy)) / temperature
+ * from g_log_prob, g_entropy, and the forward's stats and entropy. */
+NEED_API int need_token_log_probs_backward(const need_token_log_probs_args* args, need_stream_t stream);
 
 /* ------------------------------------------------------------------------ */
 /* Ragged decode / speculative verify                                        */

@@ -8,7 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import (POINTER, Structure, c_char_p, c_double, c_int32, c_int64, c_size_t, c_uint32,
+from ctypes import (POINTER, Structure, c_char_p, c_double, c_float, c_int32, c_int64, c_size_t, c_uint32,
                     c_void_p, c_uint64)
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -148,6 +148,55 @@ class NeedNormTrainArgs(Structure):
     ]
 
 
+class NeedHeads(Structure):
+    _fields_ = [("ptr", c_void_p), ("stride_b", c_int64), ("stride_t", c_int64), ("stride_h", c_int64), ("heads", c_int64)]
+
+
+class NeedLinearAttentionArgs(Structure):
+    _fields_ = [
+        ("dtype", c_int32), ("scale", c_float),
+        ("nb", c_int64), ("T", c_int64), ("H", c_int64), ("dk", c_int64), ("dv", c_int64),
+        ("q", NeedHeads), ("k", NeedHeads), ("v", NeedHeads),
+        ("log_decay", c_void_p), ("ld_stride_b", c_int64), ("ld_stride_t", c_int64), ("ld_stride_h", c_int64),
+        ("seg_start", c_void_p), ("seg_stride_b", c_int64), ("seg_stride_t", c_int64),
+        ("state", c_void_p), ("final_state", c_void_p),
+        ("out", c_void_p), ("out_stride_b", c_int64), ("out_stride_t", c_int64), ("out_stride_h", c_int64),
+        ("workspace", c_void_p), ("workspace_bytes", c_size_t),
+    ]
+
+
+class NeedLinearAttentionStepArgs(Structure):
+    _fields_ = [
+        ("dtype", c_int32), ("scale", c_float),
+        ("n", c_int64), ("H", c_int64), ("dk", c_int64), ("dv", c_int64),
+        ("q", NeedHeads), ("k", NeedHeads), ("v", NeedHeads),
+        ("log_decay", c_void_p), ("ld_stride_n", c_int64), ("ld_stride_h", c_int64),
+        ("state", c_void_p), ("state_stride", c_int64), ("slots", c_int64), ("slot", c_void_p),
+        ("out", c_void_p), ("out_stride_n", c_int64), ("out_stride_h", c_int64),
+    ]
+
+
+class NeedResidualNormArgs(Structure):
+    _fields_ = [
+        ("dtype", c_int32), ("out8", c_int32), ("rows", c_int64), ("C", c_int64), ("group", c_int64),
+        ("x", c_void_p), ("x_stride", c_int64), ("y", c_void_p), ("y_stride", c_int64),
+        ("weight", c_void_p), ("eps", c_double), ("scale", c_double),
+        ("stream", c_void_p), ("stream_stride", c_int64), ("out", c_void_p), ("out_stride", c_int64),
+        ("scales", c_void_p),
+    ]
+
+
+class NeedTokenLogProbsArgs(Structure):
+    _fields_ = [
+        ("dtype", c_int32), ("top", c_int32), ("rows", c_int64), ("V", c_int64),
+        ("logits", c_void_p), ("stride", c_int64), ("tokens", c_void_p), ("temperature", c_double),
+        ("log_prob", c_void_p), ("entropy", c_void_p), ("stats", c_void_p),
+        ("top_log_probs", c_void_p), ("top_tokens", c_void_p),
+        ("g_log_prob", c_void_p), ("g_entropy", c_void_p), ("grad", c_void_p), ("grad_stride", c_int64),
+        ("workspace", c_void_p), ("workspace_bytes", c_size_t),
+    ]
+
+
 # every symbol the header declares, with (restype, argtypes)
 SIGNATURES = {
     "need_abi_version": (c_int32, []),
@@ -186,6 +235,13 @@ SIGNATURES = {
     "need_rms_norm_train_workspace_size": (c_size_t, [c_int64, c_int64]),
     "need_rms_norm_train_forward": (c_int32, [POINTER(NeedNormTrainArgs), c_void_p]),
     "need_rms_norm_train_backward": (c_int32, [POINTER(NeedNormTrainArgs), c_void_p]),
+    "need_linear_attention_workspace_size": (c_size_t, [c_int64, c_int64, c_int64, c_int64, c_int64]),
+    "need_linear_attention": (c_int32, [POINTER(NeedLinearAttentionArgs), c_void_p]),
+    "need_linear_attention_step": (c_int32, [POINTER(NeedLinearAttentionStepArgs), c_void_p]),
+    "need_residual_rms_norm": (c_int32, [POINTER(NeedResidualNormArgs), c_void_p]),
+    "need_token_log_probs_workspace_size": (c_size_t, [c_int32, c_int64, c_int64, c_int32]),
+    "need_token_log_probs": (c_int32, [POINTER(NeedTokenLogProbsArgs), c_void_p]),
+    "need_token_log_probs_backward": (c_int32, [POINTER(NeedTokenLogProbsArgs), c_void_p]),
     "need_commit_states": (c_int32, [c_int32, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p,
                                      c_void_p, c_void_p]),
     "need_sp_local_scan": (c_int32, [POINTER(NeedScanArgs), c_int32, c_void_p]),

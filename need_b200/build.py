@@ -1,6 +1,6 @@
 """Builds need_b200/_lib/libneed_scan.so from need_b200/csrc with nvcc for sm_100a,
-and need_b200/_lib/_train.so, the autograd nodes of need_b200.train over it, with
-the host compiler against torch's headers.
+and over it, with the host compiler against torch's headers, need_b200/_lib/_train.so
+(the autograd nodes of need_b200.train) and _lm.so (the operators of need_b200.lm).
 
     python -m need_b200.build            # build if sources changed
     python -m need_b200.build --force
@@ -26,8 +26,11 @@ LIBDIR = os.path.join(HERE, "_lib")
 LIB = os.path.join(LIBDIR, "libneed_scan.so")
 EXT = os.path.join(LIBDIR, "_train.so")
 EXT_SOURCE = "train_autograd.cpp"
+EXTS = {EXT: EXT_SOURCE, os.path.join(LIBDIR, "_lm.so"): "lm_autograd.cpp"}
+EXT_HEADERS = ["torch_common.h"]
 SOURCES = ["need_scan.cu", "decode.cu", "sp.cu", "noalloc.cu", "segments.cu", "prologue.cu", "epilogue.cu", "assoc.cu",
-           "train_scan.cu", "train_conv.cu", "train_norm.cu"]
+           "train_scan.cu", "train_conv.cu", "train_norm.cu", "linear_attention.cu", "linear_attention_step.cu",
+           "residual_norm.cu", "token_log_probs.cu"]
 HEADERS = ["ptx.cuh", "scan_kernel.cuh", "host_common.h", "umma.cuh", "train_common.cuh"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
@@ -50,12 +53,12 @@ def _stale() -> bool:
     return _older(LIB, [os.path.join(CSRC, f) for f in SOURCES + HEADERS] + [os.path.join(INCLUDE, "need_scan.h")])
 
 
-def _ext_stale() -> bool:
-    return _older(EXT, [os.path.join(CSRC, EXT_SOURCE), os.path.join(INCLUDE, "need_scan.h")])
+def _ext_stale(ext: str = EXT) -> bool:
+    return _older(ext, [os.path.join(CSRC, f) for f in [EXTS[ext]] + EXT_HEADERS] + [os.path.join(INCLUDE, "need_scan.h")])
 
 
-def _ext_command() -> list:
-    """The host compile of the autograd module (no torch import: its headers are found by path).
+def _ext_command(ext: str = EXT) -> list:
+    """The host compile of a module over torch (no torch import: its headers are found by path).
 
     The C++ library is named as the shared one that torch runs on: a compiler that finds only
     the archive (a $CXX of its own tree) would link a second copy into the module, whose
@@ -67,25 +70,33 @@ def _ext_command() -> list:
     inc = [os.path.join(torch_dir, "include"), os.path.join(torch_dir, "include", "torch", "csrc", "api", "include"),
            sysconfig.get_path("include"), os.path.join(os.path.dirname(os.path.dirname(nvcc())), "include")]
     return [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-shared",
-            "-DTORCH_EXTENSION_NAME=_train", "-DTORCH_API_INCLUDE_EXTENSION_H", f"-I{INCLUDE}",
-            *[x for d in inc for x in ("-isystem", d)], os.path.join(CSRC, EXT_SOURCE), "-o", EXT + ".tmp",
+            f"-DTORCH_EXTENSION_NAME={os.path.basename(ext)[:-3]}", "-DTORCH_API_INCLUDE_EXTENSION_H", f"-I{INCLUDE}",
+            *[x for d in inc for x in ("-isystem", d)], os.path.join(CSRC, EXTS[ext]), "-o", ext + ".tmp",
             "-L" + os.path.join(torch_dir, "lib"), "-L" + LIBDIR, "-l:libneed_scan.so", "-lc10", "-lc10_cuda", "-ltorch",
             "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python", "-nostdlib++", "-l:libstdc++.so.6", "-lm", "-Wl,-rpath,$ORIGIN"]
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
-    """Compiles the shared library and the autograd module if needed; returns the library's path."""
+    """Compiles the shared library and the modules over torch if needed; returns the library's path."""
     os.makedirs(LIBDIR, exist_ok=True)
     if force or _stale():
         _build_lib(verbose)
-    if force or _ext_stale():
-        cmd = _ext_command()
-        if verbose:
-            print(" ".join(cmd), file=sys.stderr)
-        p = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT)
+    procs = []
+    for ext, src in EXTS.items():
+        if force or _ext_stale(ext):
+            cmd = _ext_command(ext)
+            if verbose:
+                print(" ".join(cmd), file=sys.stderr)
+            procs.append((ext, src, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT)))
+    failed = []
+    for ext, src, p in procs:
+        out, _ = p.communicate()
         if p.returncode != 0:
-            raise RuntimeError(f"--- {EXT_SOURCE}\n{p.stdout.decode(errors='replace')}")
-        os.replace(EXT + ".tmp", EXT)
+            failed.append(f"--- {src}\n{out.decode(errors='replace')}")
+        else:
+            os.replace(ext + ".tmp", ext)
+    if failed:
+        raise RuntimeError("\n".join(failed))
     return LIB
 
 

@@ -1,0 +1,723 @@
+// linear_attention.cu -- linear attention with a decay for each head
+// (need_linear_attention): over whole prompts, in chunks on the tensor cores.
+//
+//   S_t = a_t S_{t-1} + k_t^T v_t,   o_t = scale q_t S_t,   a = exp(log_decay)
+//
+// With G the running sum of the log decays inside a chunk of 64 tokens and S the
+// state that enters it,
+//
+//   o_t = scale (e^{G_t} q_t S + sum_{s <= t} e^{G_t - G_s} (q_t . k_s) v_s)
+//   S'  = e^{G_end} S + sum_s e^{G_end - G_s} k_s^T v_s
+//
+// A marked token (or a log decay of -infinity) starts a segment: the terms that
+// would cross it are left out by selection, whatever they hold.
+//
+// One CTA walks the chunks of one (sequence, head, 64 columns of v).  Its warps own 16
+// columns each, of the outputs and of the state, which stays in their registers in
+// fp32 as the accumulators of (v e^{G_end - G_s})^T k: transposed, so that the same
+// registers are the B operand of q S.  The scores are computed a row block per warp
+// and shared through shared memory.
+//
+// Precision.  The tensor cores take bf16.  An operand that is not exactly bf16 is
+// given as a sum of bf16 values (planes), each the rounding of what the ones before it
+// leave: 16-bit results need 2 planes of the scores and of the state (2^-17 of a
+// value; one plane would add an error as large as the result's own rounding), fp32
+// ones and the state itself 3 (2^-25).  f16 inputs are 2 planes exactly, fp32 ones 3;
+// products of planes below the last place are left out.  Sums are fp32.  The decays'
+// running sums are fp64, kept as two floats: a difference of two of them is exact to
+// fp32 however far the chunk has decayed.
+//
+// A chunk whose k or v holds an infinity or NaN (or fp32 values that a bf16 rounding
+// would carry over the largest), or whose log decays hold a NaN or a value over 1, is
+// run token by token in fp32 instead: under a score of 0 it would reach the tokens
+// before it, and other segments.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <algorithm>
+#include <type_traits>
+
+#include "host_common.h"
+#include "need_scan.h"
+#include "ptx.cuh"
+
+using namespace need;
+
+namespace {
+
+constexpr int C = 64;       // tokens of a chunk
+constexpr int kWarps = 4;   // of 16 columns of v each
+constexpr int DV = 16 * kWarps;
+constexpr int kThreads = 32 * kWarps;
+
+struct Stream {
+    const void* p;
+    int64_t sb, st, sh;  // element strides of sequence, token, head
+    int32_t share;       // heads that share one of this tensor's
+};
+
+struct AttnParams {
+    Stream q, k, v;
+    const float* ld;
+    int64_t lb, lt, lh;
+    const uint8_t* seg;
+    int64_t gb, gt;
+    const float* s0;
+    float* sT;
+    void* out;
+    int64_t ob, ot, oh;
+    int64_t T;
+    int32_t H, dk, dv, slices, nseg;
+    int32_t seg_chunks;   // chunks of a segment of the sequence
+    float scale;
+    float* part;          // [chain, nseg - 1, dk, dv]: segments' own states, then those that enter the next
+    float* part_d;        // [chain, nseg - 1]: their decays, below 0 where a reset lies in between
+};
+
+// ------------------------------------------------------------------ pieces
+__device__ __forceinline__ float to_float(float x) { return x; }
+__device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
+__device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+// x and y as the sums of N bf16 values each.
+template <int N>
+__device__ __forceinline__ void split(float x, float y, uint32_t (&pl)[N]) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+        pl[n] = pack_bf16(x, y);
+        if (n + 1 < N) x -= __uint_as_float(pl[n] << 16), y -= __uint_as_float(pl[n] & 0xffff0000u);
+    }
+}
+
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool live) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void cp_wait_all() { asm volatile("cp.async.wait_group 0;" ::: "memory"); }
+
+// Byte offset of 16-byte piece `piece` of row `row` in a plane of COLS bf16 columns: pieces
+// change places within 8 rows, so that ldmatrix meets every bank once.
+template <int COLS>
+__device__ __forceinline__ uint32_t at(int row, int piece) {
+    return static_cast<uint32_t>(row * COLS * 2 + ((piece ^ (row & 7)) << 4));
+}
+
+// Planes of a type's inputs, of computed operands, and the sum of plane numbers below
+// which a product counts (of the scores; of the products with the scores and the state).
+template <typename T>
+struct Split {
+    static constexpr int IN = 1, SCORE = 2, QK = 1, OUT = 2;
+};
+template <>
+struct Split<__half> {
+    static constexpr int IN = 2, SCORE = 2, QK = 2, OUT = 2;
+};
+template <>
+struct Split<float> {
+    static constexpr int IN = 3, SCORE = 3, QK = 3, OUT = 3;
+};
+constexpr int kStatePlanes = 3;  // of v e^{...}: what the state sums
+
+// A chunk's decays.
+struct alignas(16) Decays {
+    float hi[C], lo[C];  // log2 of the product from the chunk's first token on, as a sum
+    float w[C];          // from a token to the chunk's end; 0 where a segment starts in between
+    float eg[C];         // from the entering state to a token; 0 likewise
+    int seg[C];          // segments started up to the token
+    float d;             // over the chunk; -1 where a segment starts in it
+};
+
+template <typename T, int DK, bool VEC>
+struct Layout {
+    using S = Split<T>;
+    static constexpr int STAGES = S::IN == 1 && VEC ? 2 : 1;
+    static constexpr int Q = 0, K = S::IN * C * DK * 2, V = 2 * K, STAGE = V + S::IN * C * DV * 2;
+    static constexpr int P = STAGES * STAGE, G = P + S::SCORE * C * C * 2, BYTES = G + 2 * static_cast<int>(sizeof(Decays));
+};
+
+// ------------------------------------------------------------------ loads
+// 8 values of a row from column `col` on; 0 outside the tensor.
+template <typename T, bool VEC>
+__device__ __forceinline__ void load8(const T* row, int col, int cols, bool live, float (&f)[8]) {
+    if constexpr (VEC) {
+        constexpr int N = 16 / sizeof(T);
+#pragma unroll
+        for (int h = 0; h < 8 / N; ++h) {
+            uint4 u = make_uint4(0, 0, 0, 0);
+            if (live && col + h * N < cols) u = *reinterpret_cast<const uint4*>(row + col + h * N);
+            const T* x = reinterpret_cast<const T*>(&u);
+#pragma unroll
+            for (int e = 0; e < N; ++e) f[h * N + e] = to_float(x[e]);
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] = live && col + e < cols ? to_float(row[col + e]) : 0.0f;
+    }
+}
+
+// Rows [t0, t0 + C) of one tensor into its planes; true where a value is not finite
+// (or too near the largest to be rounded).
+template <typename T, int COLS, bool VEC>
+__device__ __forceinline__ bool load_planes(char* dst, const T* base, int64_t st, int64_t t0, int64_t T_, int col0,
+                                            int cols) {
+    constexpr int IN = Split<T>::IN, PIECES = COLS / 8;
+    float chk = 0.0f;
+    for (int n = threadIdx.x; n < C * PIECES; n += kThreads) {
+        const int row = n / PIECES, piece = n % PIECES;
+        float f[8];
+        load8<T, VEC>(base + (t0 + row) * st, col0 + piece * 8, cols, t0 + row < T_, f);
+        uint32_t pl[4][IN];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            split<IN>(f[2 * e], f[2 * e + 1], pl[e]);
+            // of a value that rounds to an infinity the first plane is one
+            chk = fmaf(__uint_as_float(pl[e][0] << 16), 0.0f, chk);
+            chk = fmaf(__uint_as_float(pl[e][0] & 0xffff0000u), 0.0f, chk);
+        }
+#pragma unroll
+        for (int p = 0; p < IN; ++p)
+            *reinterpret_cast<uint4*>(dst + p * C * COLS * 2 + at<COLS>(row, piece)) =
+                make_uint4(pl[0][p], pl[1][p], pl[2][p], pl[3][p]);
+    }
+    return !(chk == 0.0f);
+}
+
+// The same of bf16 rows by asynchronous copies, 16 bytes each.
+template <int COLS>
+__device__ __forceinline__ void copy_rows(uint32_t dst, const __nv_bfloat16* base, int64_t st, int64_t t0, int64_t T_,
+                                          int col0, int cols) {
+    constexpr int PIECES = COLS / 8;
+#pragma unroll
+    for (int n0 = 0; n0 < C * PIECES; n0 += kThreads) {
+        const int n = n0 + threadIdx.x, row = n / PIECES, piece = n % PIECES, col = col0 + piece * 8;
+        const bool live = t0 + row < T_ && col < cols;
+        cp_async16(dst + at<COLS>(row, piece), live ? base + (t0 + row) * st + col : base, live);
+    }
+}
+// Whether a piece that this thread has copied holds an infinity or NaN.
+template <int COLS>
+__device__ __forceinline__ bool check_rows(const char* src) {
+    constexpr int PIECES = COLS / 8;
+    const __nv_bfloat162 zero = __floats2bfloat162_rn(0.0f, 0.0f);
+    __nv_bfloat162 chk = zero;
+#pragma unroll
+    for (int n0 = 0; n0 < C * PIECES; n0 += kThreads) {
+        const int n = n0 + threadIdx.x;
+        const uint4 u = *reinterpret_cast<const uint4*>(src + at<COLS>(n / PIECES, n % PIECES));
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) chk = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&w[e]), zero, chk);
+    }
+    const float2 f = __bfloat1622float2(chk);
+    return !(f.x == 0.0f && f.y == 0.0f);
+}
+
+// ------------------------------------------------------------------ decays
+// A lane's two tokens of a chunk.
+struct TokenPair {
+    float ld[2];
+    bool reset[2];
+};
+__device__ __forceinline__ TokenPair load_decays(const AttnParams& p, const float* ld, const uint8_t* seg, int64_t t0) {
+    TokenPair r;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+        const int64_t t = t0 + 2 * (threadIdx.x & 31) + e;
+        const bool live = t < p.T;
+        const float x = live ? ld[t * p.lt] : 0.0f;
+        r.reset[e] = (live && seg != nullptr && seg[t * p.gt] != 0) || x == -INFINITY;
+        // a token's state falls below every fp32 value long before e^-10000; a NaN stays one
+        r.ld[e] = r.reset[e] ? 0.0f : x < -10000.0f ? -10000.0f : x;
+    }
+    return r;
+}
+// One warp: the chunk's running sums from its 64 log decays.  True where one of them is no
+// number or so far above 0 that a product of 64 leaves fp32's range.
+__device__ __forceinline__ bool make_decays(const TokenPair& tp, Decays& g) {
+    const int lane = threadIdx.x & 31;
+    const double x0 = static_cast<double>(tp.ld[0]) * 1.4426950408889634074, x1 = static_cast<double>(tp.ld[1]) * 1.4426950408889634074;
+    double incl = x0 + x1;
+#pragma unroll
+    for (int m = 1; m < 32; m <<= 1) {
+        const double o = __shfl_up_sync(0xffffffffu, incl, m);
+        if (lane >= m) incl += o;
+    }
+    double before = __shfl_up_sync(0xffffffffu, incl, 1);
+    if (lane == 0) before = 0.0;
+    const uint32_t m0 = __ballot_sync(0xffffffffu, tp.reset[0]), m1 = __ballot_sync(0xffffffffu, tp.reset[1]);
+    const uint32_t lt = (1u << lane) - 1u;
+    const double G[2] = {before + x0, incl};
+    int s[2];
+    s[0] = __popc(m0 & lt) + __popc(m1 & lt) + (tp.reset[0] ? 1 : 0);
+    s[1] = s[0] + (tp.reset[1] ? 1 : 0);
+    const double end = __shfl_sync(0xffffffffu, incl, 31);
+    const int send = __popc(m0) + __popc(m1);
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+        const int i = 2 * lane + e;
+        const float hi = static_cast<float>(G[e]);
+        g.hi[i] = hi, g.lo[i] = static_cast<float>(G[e] - hi);
+        g.seg[i] = s[e];
+        g.w[i] = s[e] == send ? ex2(static_cast<float>(end - G[e])) : 0.0f;
+        g.eg[i] = s[e] == 0 ? ex2(hi) : 0.0f;
+    }
+    if (lane == 0) g.d = send == 0 ? ex2(static_cast<float>(end)) : -1.0f;
+    return __any_sync(0xffffffffu, !(tp.ld[0] <= 1.0f && tp.ld[1] <= 1.0f));
+}
+__device__ __forceinline__ float times_state(float d, float s) { return d == -1.0f ? 0.0f : d * s; }
+
+// ------------------------------------------------------------------ the kernel
+// STATE: only the state of a segment of the sequence, from zero, and its decay.
+template <typename T, int DK, bool VEC, bool STATE>
+__global__ void __launch_bounds__(kThreads) attention_kernel(const AttnParams p) {
+    using S = Split<T>;
+    using L = Layout<T, DK, VEC>;
+    constexpr int NI = DK / 8;  // 8-feature tiles of the state
+    extern __shared__ __align__(128) char smem[];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c2 = (lane & 3) * 2;
+    int64_t id = blockIdx.x;
+    const int nseg = STATE ? p.nseg - 1 : p.nseg;
+    const int seg = static_cast<int>(id % nseg);
+    id /= nseg;
+    const int slice = static_cast<int>(id % p.slices);
+    const int64_t chain = id / p.slices;
+    const int64_t b = chain / p.H;
+    const int h = static_cast<int>(chain % p.H), col0 = slice * DV, jw = col0 + 16 * warp;
+    const T* q = static_cast<const T*>(p.q.p) + b * p.q.sb + (h / p.q.share) * p.q.sh;
+    const T* k = static_cast<const T*>(p.k.p) + b * p.k.sb + (h / p.k.share) * p.k.sh;
+    const T* v = static_cast<const T*>(p.v.p) + b * p.v.sb + (h / p.v.share) * p.v.sh;
+    const float* ld = p.ld + b * p.lb + h * p.lh;
+    const uint8_t* marks = p.seg == nullptr ? nullptr : p.seg + b * p.gb;
+    T* out = static_cast<T*>(p.out) + b * p.ob + h * p.oh;
+    const int64_t chunks = (p.T + C - 1) / C, c0 = int64_t(seg) * p.seg_chunks;
+    const int64_t c1 = c0 + p.seg_chunks < chunks ? c0 + p.seg_chunks : chunks;
+    Decays* const gates = reinterpret_cast<Decays*>(smem + L::G);
+    const uint32_t sm = smem_addr(smem);
+
+    // the state, transposed: rows j = jw + g and + 8, columns i = 8 n + c2 and + 1
+    float s[NI][4];
+    {
+        const float* from = STATE ? nullptr : seg > 0 ? p.part + (chain * (p.nseg - 1) + seg - 1) * p.dk * int64_t(p.dv)
+                                  : p.s0 != nullptr   ? p.s0 + chain * p.dk * int64_t(p.dv) : nullptr;
+#pragma unroll
+        for (int n = 0; n < NI; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int i = 8 * n + c2 + (e & 1), j = jw + g + (e >> 1) * 8;
+                s[n][e] = from != nullptr && i < p.dk && j < p.dv ? from[int64_t(i) * p.dv + j] : 0.0f;
+            }
+    }
+    float total = 1.0f;  // STATE: the segment's decay
+
+    auto issue = [&](int64_t c) {  // the asynchronous copies of a chunk
+        if constexpr (L::STAGES == 2) {
+            const uint32_t to = sm + (c & 1) * L::STAGE;
+            if (!STATE) copy_rows<DK>(to + L::Q, q, p.q.st, c * C, p.T, 0, p.dk);
+            copy_rows<DK>(to + L::K, k, p.k.st, c * C, p.T, 0, p.dk);
+            copy_rows<DV>(to + L::V, v, p.v.st, c * C, p.T, col0, p.dv);
+            cp_commit();
+        }
+    };
+    issue(c0);
+    bool wild = false;  // warp 0: of the next chunk's decays
+    if (warp == 0) wild = make_decays(load_decays(p, ld, marks, c0 * C), gates[c0 & 1]);
+
+    for (int64_t c = c0; c < c1; ++c) {
+        const int64_t t0 = c * C;
+        const int stage = L::STAGES == 2 ? static_cast<int>(c & 1) : 0;
+        char* const buf = smem + stage * L::STAGE;
+        const uint32_t sbuf = sm + stage * L::STAGE;
+        bool bad;
+        if constexpr (L::STAGES == 2) {
+            cp_wait_all();
+            bad = check_rows<DK>(buf + L::K) | check_rows<DV>(buf + L::V);
+        } else {
+            __syncthreads();  // the chunk before this one has been read
+            if (!STATE) load_planes<T, DK, VEC>(buf + L::Q, q, p.q.st, t0, p.T, 0, p.dk);
+            bad = load_planes<T, DK, VEC>(buf + L::K, k, p.k.st, t0, p.T, 0, p.dk);
+            bad |= load_planes<T, DV, VEC>(buf + L::V, v, p.v.st, t0, p.T, col0, p.dv);
+        }
+        bad = __syncthreads_or(bad | wild);  // the chunk and its decays are there
+        const Decays& gt = gates[c & 1];
+        TokenPair next{};
+        if (c + 1 < c1) {
+            issue(c + 1);
+            if (warp == 0) next = load_decays(p, ld, marks, t0 + C);
+        }
+        if (STATE) total = total == -1.0f || gt.d == -1.0f ? -1.0f : total * gt.d;
+
+        if (bad) {  // token by token, in fp32, from the inputs themselves
+            const int n = static_cast<int>(p.T - t0 < C ? p.T - t0 : C);
+            for (int r = 0; r < n; ++r) {
+                const int64_t t = t0 + r;
+                const float x = ld[t * p.lt];
+                const bool reset = (marks != nullptr && marks[t * p.gt] != 0) || x == -INFINITY;
+                const float a = expf(x);
+                const int j = jw + g;
+                const float v0 = j < p.dv ? to_float(v[t * p.v.st + j]) : 0.0f;
+                const float v1 = j + 8 < p.dv ? to_float(v[t * p.v.st + j + 8]) : 0.0f;
+                float o0 = 0.0f, o1 = 0.0f;
+#pragma unroll
+                for (int m = 0; m < NI; ++m)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const int i = 8 * m + c2 + e;
+                        if (i < p.dk) {
+                            const float kk = to_float(k[t * p.k.st + i]);
+                            s[m][e] = reset ? kk * v0 : fmaf(a, s[m][e], kk * v0);
+                            s[m][2 + e] = reset ? kk * v1 : fmaf(a, s[m][2 + e], kk * v1);
+                            if (!STATE) {
+                                const float qq = to_float(q[t * p.q.st + i]);
+                                o0 = fmaf(qq, s[m][e], o0), o1 = fmaf(qq, s[m][2 + e], o1);
+                            }
+                        }
+                    }
+                if (!STATE) {
+#pragma unroll
+                    for (int m = 1; m < 4; m <<= 1) {
+                        o0 += __shfl_xor_sync(0xffffffffu, o0, m);
+                        o1 += __shfl_xor_sync(0xffffffffu, o1, m);
+                    }
+                    if (c2 == 0 && j < p.dv) out[t * p.ot + j] = static_cast<T>(p.scale * o0);
+                    if (c2 == 2 && j + 8 < p.dv) out[t * p.ot + j + 8] = static_cast<T>(p.scale * o1);
+                }
+            }
+            if (warp == 0 && c + 1 < c1) wild = make_decays(next, gates[(c + 1) & 1]);
+            continue;
+        }
+
+        // rows and pieces of this lane's ldmatrix addresses: 16 rows x 16 columns a load
+        const int lr = lane & 15, lp = lane >> 4;               // [m][k] tiles, and [k][n] ones transposed
+        const int br = (lane & 7) + ((lane >> 4) << 3), bp = (lane >> 3) & 1;  // [n][k] tiles
+        float o[4][2][4] = {};
+        if constexpr (!STATE) {
+            // scores of row block `warp`, a block of 16 tokens before or at it each
+            uint32_t qa[S::IN][DK / 16][4];
+#pragma unroll
+            for (int a = 0; a < S::IN; ++a)
+#pragma unroll
+                for (int ks = 0; ks < DK / 16; ++ks)
+                    ldsm4(qa[a][ks], sbuf + L::Q + a * C * DK * 2 + at<DK>(16 * warp + lr, 2 * ks + lp));
+            const int r0 = 16 * warp + g;
+            const float h0 = gt.hi[r0], l0 = gt.lo[r0], h1 = gt.hi[r0 + 8], l1 = gt.lo[r0 + 8];
+            const int s0 = gt.seg[r0], s1 = gt.seg[r0 + 8];
+            for (int nb = 0; nb <= warp; ++nb) {
+                float acc[2][4] = {};
+#pragma unroll
+                for (int ks = 0; ks < DK / 16; ++ks)
+#pragma unroll
+                    for (int b2 = 0; b2 < S::QK; ++b2) {
+                        uint32_t kb[4];
+                        ldsm4(kb, sbuf + L::K + b2 * C * DK * 2 + at<DK>(16 * nb + br, 2 * ks + bp));
+#pragma unroll
+                        for (int a = 0; a + b2 < S::QK; ++a) {
+                            mma(acc[0], qa[a][ks], kb[0], kb[1]);
+                            mma(acc[1], qa[a][ks], kb[2], kb[3]);
+                        }
+                    }
+#pragma unroll
+                for (int n = 0; n < 2; ++n) {
+                    const int col = 16 * nb + 8 * n + c2;
+                    float f[4];
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const float hs = gt.hi[col + e], ls = gt.lo[col + e];
+                        const int ss = gt.seg[col + e];
+                        f[e] = ss == s0 && col + e <= r0 ? ex2((h0 - hs) + (l0 - ls)) * acc[n][e] : 0.0f;
+                        f[2 + e] = ss == s1 && col + e <= r0 + 8 ? ex2((h1 - hs) + (l1 - ls)) * acc[n][2 + e] : 0.0f;
+                    }
+                    uint32_t p0[S::SCORE], p1[S::SCORE];
+                    split<S::SCORE>(f[0], f[1], p0);
+                    split<S::SCORE>(f[2], f[3], p1);
+#pragma unroll
+                    for (int a = 0; a < S::SCORE; ++a) {
+                        char* const to = smem + L::P + a * C * C * 2 + c2 * 2;
+                        *reinterpret_cast<uint32_t*>(to + at<C>(r0, 2 * nb + n)) = p0[a];
+                        *reinterpret_cast<uint32_t*>(to + at<C>(r0 + 8, 2 * nb + n)) = p1[a];
+                    }
+                }
+            }
+            // what the entering state gives: all 64 rows, this warp's 16 columns
+#pragma unroll
+            for (int ks = 0; ks < DK / 16; ++ks) {
+                uint32_t sb0[2][S::SCORE], sb1[2][S::SCORE];  // [column tile][plane], features 0-7 and 8-15 of the step
+#pragma unroll
+                for (int n = 0; n < 2; ++n) {
+                    split<S::SCORE>(s[2 * ks][2 * n], s[2 * ks][2 * n + 1], sb0[n]);
+                    split<S::SCORE>(s[2 * ks + 1][2 * n], s[2 * ks + 1][2 * n + 1], sb1[n]);
+                }
+#pragma unroll
+                for (int m = 0; m < 4; ++m)
+#pragma unroll
+                    for (int a = 0; a < S::IN; ++a) {
+                        uint32_t qf[4];
+                        ldsm4(qf, sbuf + L::Q + a * C * DK * 2 + at<DK>(16 * m + lr, 2 * ks + lp));
+#pragma unroll
+                        for (int b2 = 0; b2 < S::SCORE && a + b2 < S::OUT; ++b2)
+#pragma unroll
+                            for (int n = 0; n < 2; ++n) mma(o[m][n], qf, sb0[n][b2], sb1[n][b2]);
+                    }
+            }
+#pragma unroll
+            for (int m = 0; m < 4; ++m)
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    const int row = 16 * m + g + 8 * r;
+                    const float eg = gt.eg[row];
+                    const bool reach = gt.seg[row] == 0;
+#pragma unroll
+                    for (int n = 0; n < 2; ++n)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) o[m][n][2 * r + e] = reach ? eg * o[m][n][2 * r + e] : 0.0f;
+                }
+        }
+        if (warp == 0 && c + 1 < c1) wild = make_decays(next, gates[(c + 1) & 1]);
+        if constexpr (!STATE) __syncthreads();  // the scores are there
+
+        // the scores times v, and the state
+#pragma unroll
+        for (int n = 0; n < NI; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[n][e] = times_state(gt.d, s[n][e]);
+#pragma unroll
+        for (int kb = 0; kb < 4; ++kb) {  // blocks of 16 tokens
+            uint32_t vf[S::IN][4];  // (tokens 0-7, columns 0-7), (0-7, 8-15), (8-15, 0-7), (8-15, 8-15)
+            const int vr = 16 * kb + (lane & 7) + ((lane >> 4) << 3), vp = (lane >> 3) & 1;
+#pragma unroll
+            for (int a = 0; a < S::IN; ++a) ldsm4_t(vf[a], sbuf + L::V + a * C * DV * 2 + at<DV>(vr, 2 * warp + vp));
+            if constexpr (!STATE) {
+#pragma unroll
+                for (int m = kb; m < 4; ++m)
+#pragma unroll
+                    for (int a = 0; a < S::SCORE; ++a) {
+                        uint32_t pf[4];
+                        ldsm4(pf, sm + L::P + a * C * C * 2 + at<C>(16 * m + lr, 2 * kb + lp));
+#pragma unroll
+                        for (int b2 = 0; b2 < S::IN && a + b2 < S::OUT; ++b2) {
+                            mma(o[m][0], pf, vf[b2][0], vf[b2][2]);
+                            mma(o[m][1], pf, vf[b2][1], vf[b2][3]);
+                        }
+                    }
+            }
+            uint32_t vw[kStatePlanes][4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const float2 w = *reinterpret_cast<const float2*>(&gt.w[16 * kb + (r >> 1) * 8 + c2]);
+                float x = 0.0f, y = 0.0f;
+#pragma unroll
+                for (int a = S::IN - 1; a >= 0; --a)  // the planes' sum is the input itself
+                    x += __uint_as_float(vf[a][r] << 16), y += __uint_as_float(vf[a][r] & 0xffff0000u);
+                uint32_t pl[kStatePlanes];
+                split<kStatePlanes>(w.x * x, w.y * y, pl);
+#pragma unroll
+                for (int a = 0; a < kStatePlanes; ++a) vw[a][r] = pl[a];
+            }
+#pragma unroll
+            for (int n = 0; n < NI / 2; ++n)  // 16 features each
+#pragma unroll
+                for (int b2 = 0; b2 < S::IN; ++b2) {
+                    uint32_t kf[4];
+                    ldsm4_t(kf, sbuf + L::K + b2 * C * DK * 2 + at<DK>(16 * kb + lr, 2 * n + lp));
+#pragma unroll
+                    for (int a = 0; a < kStatePlanes && a + b2 < kStatePlanes; ++a) {
+                        mma(s[2 * n], vw[a], kf[0], kf[1]);
+                        mma(s[2 * n + 1], vw[a], kf[2], kf[3]);
+                    }
+                }
+        }
+        if constexpr (!STATE) {
+#pragma unroll
+            for (int m = 0; m < 4; ++m)
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    const int64_t t = t0 + 16 * m + g + 8 * r;
+                    if (t < p.T)
+#pragma unroll
+                        for (int n = 0; n < 2; ++n) {
+                            const int j = jw + 8 * n + c2;
+                            const float x = p.scale * o[m][n][2 * r], y = p.scale * o[m][n][2 * r + 1];
+                            T* const to = out + t * p.ot + j;
+                            if (VEC) {  // whole pairs, aligned
+                                if (j < p.dv) {
+                                    if constexpr (sizeof(T) == 4) *reinterpret_cast<float2*>(to) = make_float2(x, y);
+                                    else if constexpr (std::is_same<T, __half>::value) *reinterpret_cast<__half2*>(to) = __floats2half2_rn(x, y);
+                                    else *reinterpret_cast<uint32_t*>(to) = pack_bf16(x, y);
+                                }
+                            } else {
+                                if (j < p.dv) to[0] = static_cast<T>(x);
+                                if (j + 1 < p.dv) to[1] = static_cast<T>(y);
+                            }
+                        }
+                }
+        }
+    }
+
+    float* const to = STATE ? p.part + (chain * (p.nseg - 1) + seg) * p.dk * int64_t(p.dv)
+                            : seg == p.nseg - 1 && p.sT != nullptr ? p.sT + chain * p.dk * int64_t(p.dv) : nullptr;
+    if (to != nullptr) {
+#pragma unroll
+        for (int n = 0; n < NI; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int i = 8 * n + c2 + (e & 1), j = jw + g + (e >> 1) * 8;
+                if (i < p.dk && j < p.dv) to[int64_t(i) * p.dv + j] = s[n][e];
+            }
+    }
+    if (STATE && slice == 0 && threadIdx.x == 0) p.part_d[chain * (p.nseg - 1) + seg] = total;
+}
+
+// The state that enters each segment after the first, in the place of the own state of
+// the one before it.
+__global__ void __launch_bounds__(256) enter_kernel(const AttnParams p) {
+    const int64_t n = p.dk * int64_t(p.dv), chain = blockIdx.x;
+    const int64_t i = blockIdx.y * int64_t(256) + threadIdx.x;
+    if (i >= n) return;
+    float* s = p.part + chain * (p.nseg - 1) * n + i;
+    const float* d = p.part_d + chain * (p.nseg - 1);
+    float x = p.s0 != nullptr ? p.s0[chain * n + i] : 0.0f;
+    constexpr int B = 8;  // loads in flight
+    for (int k0 = 0; k0 < p.nseg - 1; k0 += B) {
+        float own[B];
+#pragma unroll
+        for (int e = 0; e < B; ++e) own[e] = k0 + e < p.nseg - 1 ? s[(k0 + e) * n] : 0.0f;
+#pragma unroll
+        for (int e = 0; e < B; ++e)
+            if (k0 + e < p.nseg - 1) {
+                x = times_state(d[k0 + e], x) + own[e];
+                s[(k0 + e) * n] = x;
+            }
+    }
+}
+
+// ------------------------------------------------------------------ host
+struct Plan {
+    int64_t chains, chunks;
+    int32_t slices, nseg, seg_chunks;
+};
+// Chains below one for each place of the GPU (3 CTAs a multiprocessor) are cut into segments
+// of at least 4 chunks.
+Plan plan(int64_t nb, int64_t T, int64_t H, int64_t dv) {
+    Plan pl{};
+    pl.chains = nb * H, pl.chunks = (T + C - 1) / C, pl.slices = int32_t((dv + DV - 1) / DV);
+    const int64_t ctas = pl.chains * pl.slices;
+    int64_t nseg = ctas >= 222 ? 1 : (444 + ctas - 1) / std::max<int64_t>(ctas, 1);
+    nseg = std::max<int64_t>(1, std::min(nseg, pl.chunks / 4));
+    pl.seg_chunks = int32_t((pl.chunks + nseg - 1) / nseg);
+    pl.nseg = int32_t((pl.chunks + pl.seg_chunks - 1) / pl.seg_chunks);
+    return pl;
+}
+
+template <typename T, int DK, bool VEC, bool STATE>
+int launch(const AttnParams& p, int64_t blocks, cudaStream_t s) {
+    static std::atomic<uint64_t> done{0};
+    auto kern = attention_kernel<T, DK, VEC, STATE>;
+    constexpr int bytes = Layout<T, DK, VEC>::BYTES;
+    cudaError_t e = ensure_smem(kern, bytes, done);
+    if (e != cudaSuccess) return cuda_fail(e, "linear attention shared memory");
+    kern<<<static_cast<unsigned>(blocks), kThreads, bytes, s>>>(p);
+    e = cudaGetLastError();
+    return e == cudaSuccess ? NEED_OK : cuda_fail(e, "linear attention launch");
+}
+
+template <typename T, int DK, bool VEC>
+int run(const AttnParams& p, const Plan& pl, cudaStream_t s) {
+    const int64_t per = pl.chains * pl.slices;
+    if (pl.nseg > 1) {
+        int rc = launch<T, DK, VEC, true>(p, per * (pl.nseg - 1), s);
+        if (rc != NEED_OK) return rc;
+        const dim3 grid(static_cast<unsigned>(pl.chains), static_cast<unsigned>((int64_t(p.dk) * p.dv + 255) / 256));
+        enter_kernel<<<grid, 256, 0, s>>>(p);
+        const cudaError_t e = cudaGetLastError();
+        if (e != cudaSuccess) return cuda_fail(e, "linear attention launch");
+    }
+    return launch<T, DK, VEC, false>(p, per * pl.nseg, s);
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t need_linear_attention_workspace_size(int64_t nb, int64_t T, int64_t H, int64_t dk, int64_t dv) {
+    if (nb < 1 || T < 1 || H < 1 || dk < 1 || dv < 1) return 16;
+    const Plan pl = plan(nb, T, H, dv);
+    return 16 + size_t(pl.chains) * size_t(pl.nseg - 1) * (size_t(dk) * size_t(dv) + 1) * 4;
+}
+
+int need_linear_attention(const need_linear_attention_args* a, need_stream_t stream) {
+    if (a == nullptr) return fail(NEED_ERR_INVALID, "linear attention: args is null");
+    if (!dtype_ok(a->dtype)) return fail(NEED_ERR_UNSUPPORTED, "linear attention: dtype %d", a->dtype);
+    if (a->nb < 1 || a->T < 1 || a->H < 1 || a->dk < 1 || a->dv < 1)
+        return fail(NEED_ERR_INVALID, "linear attention: sizes must be positive");
+    if (a->dk > NEED_LINEAR_ATTENTION_MAX_DK || a->dv > (1 << 20) || a->H > (1 << 24) || a->T > (int64_t(1) << 36))
+        return fail(NEED_ERR_UNSUPPORTED, "linear attention: at most %d features a head (got %lld), sizes out of range",
+                    NEED_LINEAR_ATTENTION_MAX_DK, static_cast<long long>(a->dk));
+    const need_heads* in[3] = {&a->q, &a->k, &a->v};
+    for (const need_heads* x : in) {
+        if (x->ptr == nullptr) return fail(NEED_ERR_INVALID, "linear attention: an input is null");
+        if (x->heads < 1 || a->H % x->heads != 0)
+            return fail(NEED_ERR_INVALID, "linear attention: heads must divide H = %lld", static_cast<long long>(a->H));
+    }
+    if (a->log_decay == nullptr || a->out == nullptr) return fail(NEED_ERR_INVALID, "linear attention: log_decay and out are required");
+    if (a->T > 1 && a->out_stride_t < a->dv) return fail(NEED_ERR_INVALID, "linear attention: the output's rows overlap");
+    const Plan pl = plan(a->nb, a->T, a->H, a->dv);
+    if (pl.chains > (int64_t(1) << 30) / pl.slices / pl.nseg)
+        return fail(NEED_ERR_UNSUPPORTED, "linear attention: too many sequences and heads");
+    if (pl.nseg > 1 && (a->workspace == nullptr || (reinterpret_cast<uintptr_t>(a->workspace) & 3u) != 0 ||
+                        a->workspace_bytes < need_linear_attention_workspace_size(a->nb, a->T, a->H, a->dk, a->dv)))
+        return fail(NEED_ERR_WORKSPACE, "linear attention: workspace missing, misaligned or too small");
+    const int es = dtype_bytes(a->dtype), per = 16 / es;
+    AttnParams p{};
+    Stream* to[3] = {&p.q, &p.k, &p.v};
+    // whole 16-byte pieces: of the rows of all inputs, and pairs of the output
+    bool vec = a->dk % per == 0 && a->dv % per == 0;
+    for (int n = 0; n < 3; ++n) {
+        const need_heads& x = *in[n];
+        *to[n] = Stream{x.ptr, x.stride_b, x.stride_t, x.stride_h, int32_t(a->H / x.heads)};
+        vec = vec && aligned16(x.ptr) && (x.stride_t % per == 0 || a->T == 1) && (x.stride_b % per == 0 || a->nb == 1) &&
+              (x.stride_h % per == 0 || x.heads == 1);
+    }
+    vec = vec && aligned16(a->out) && a->out_stride_t % 2 == 0 && a->out_stride_b % 2 == 0 && a->out_stride_h % 2 == 0;
+    p.ld = a->log_decay, p.lb = a->ld_stride_b, p.lt = a->ld_stride_t, p.lh = a->ld_stride_h;
+    p.seg = a->seg_start, p.gb = a->seg_stride_b, p.gt = a->seg_stride_t;
+    p.s0 = a->state, p.sT = a->final_state;
+    p.out = a->out, p.ob = a->out_stride_b, p.ot = a->out_stride_t, p.oh = a->out_stride_h;
+    p.T = a->T, p.H = int32_t(a->H), p.dk = int32_t(a->dk), p.dv = int32_t(a->dv);
+    p.slices = pl.slices, p.nseg = pl.nseg, p.seg_chunks = pl.seg_chunks, p.scale = a->scale;
+    if (pl.nseg > 1) {
+        p.part = static_cast<float*>(a->workspace);
+        p.part_d = p.part + pl.chains * (pl.nseg - 1) * a->dk * a->dv;
+    }
+    auto go = [&](auto tag) {
+        using T = decltype(tag);
+        if (a->dk <= 64) return vec ? run<T, 64, true>(p, pl, stream) : run<T, 64, false>(p, pl, stream);
+        return vec ? run<T, 128, true>(p, pl, stream) : run<T, 128, false>(p, pl, stream);
+    };
+    const int rc = a->dtype == NEED_F32 ? go(float{}) : a->dtype == NEED_BF16 ? go(__nv_bfloat16{}) : go(__half{});
+    return rc != NEED_OK ? rc : ok();
+}
+
+}  // extern "C"

@@ -1,0 +1,248 @@
+// residual_norm.cu -- the residual's addition and the RMSNorm of what it gives, with an
+// output in the row's type or in 8 bits with scales (need_residual_rms_norm):
+//
+//   r = x + scale y (rounded, the stream that goes on),  n = r / sqrt(sum(r^2) / C + eps) w
+//   out = n, or e4m3(n / 2^e) with one 2^e for each `group` channels
+//
+// x and y are read once, the stream and the output written once: 8 B per 16-bit element,
+// 7 with 8 bits, so HBM bounds it.  A row lies in the registers of 1 to 16 warps (the
+// fewest that leave a lane at most 4 16-byte pieces), from the addition to the output; its
+// sum and the groups' largest values are taken by shuffles, a group's pieces lying in
+// neighbouring lanes.
+#include <algorithm>
+#include <type_traits>
+
+#include "host_common.h"
+#include "need_scan.h"
+#include "scan_kernel.cuh"
+#include "train_common.cuh"
+
+using namespace need;
+
+namespace {
+
+constexpr int kPieces = 4;      // 16-byte pieces per lane
+constexpr int kMaxWarps = 16;   // warps per row
+constexpr int kRowBytes = kMaxWarps * 32 * kPieces * 16;
+
+struct ResidualParams {
+    const void* x;
+    int64_t xs;
+    const void* y;
+    int64_t ys;
+    const float* w;
+    void* stream;
+    int64_t ss;
+    void* out;
+    int64_t os;
+    float* scales;
+    int64_t rows;
+    int32_t C, wpr, group, ngroups;  // group: of an 8-bit output; C for one scale a row
+    float inv_c, eps, scale;
+};
+
+// A 16-byte piece of a row.  VEC: rows are 16-byte aligned and whole pieces; else element
+// by element, n of the piece's N inside the row.
+template <typename T, bool VEC>
+__device__ __forceinline__ uint4 load_piece(const T* p, int n) {
+    if constexpr (VEC) {
+        return __ldcs(reinterpret_cast<const uint4*>(p));
+    } else {
+        constexpr int N = 16 / sizeof(T);
+        union { uint4 u; T e[N]; } r;
+        r.u = make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int e = 0; e < N; ++e)
+            if (e < n) r.e[e] = p[e];
+        return r.u;
+    }
+}
+template <typename T, bool VEC>
+__device__ __forceinline__ void store_piece(T* p, int n, const uint4& u) {
+    if constexpr (VEC) {
+        *reinterpret_cast<uint4*>(p) = u;
+    } else {
+        constexpr int N = 16 / sizeof(T);
+        const T* q = reinterpret_cast<const T*>(&u);
+#pragma unroll
+        for (int e = 0; e < N; ++e)
+            if (e < n) p[e] = q[e];
+    }
+}
+
+// blockDim = 32 * wpr * (rows per block); lane l of a row's warp w holds pieces
+// (w * 32 + l) + k * 32 * wpr.  OUT8: the output in 8 bits.
+template <typename T, int NP, bool VEC, bool OUT8>
+__global__ void __launch_bounds__(512) residual_norm_kernel(const ResidualParams p) {
+    using P = typename Ops<T>::P;
+    constexpr int N = 16 / Ops<T>::BYTES;
+    __shared__ float s_red[kMaxWarps];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, w0 = warp / p.wpr * p.wpr;
+    const int rpb = (blockDim.x >> 5) / p.wpr;
+    const int64_t row = int64_t(blockIdx.x) * rpb + warp / p.wpr;
+    const bool live = row < p.rows;
+    const int l0 = (warp % p.wpr) * 32 + lane, step = 32 * p.wpr, nvec = (p.C + N - 1) / N;
+    const T* x = static_cast<const T*>(p.x) + (live ? row : 0) * p.xs;
+    const T* y = static_cast<const T*>(p.y) + (live ? row : 0) * p.ys;
+    uint4 u[NP], v[NP];
+#pragma unroll
+    for (int k = 0; k < NP; ++k) {
+        const int i = l0 + k * step;
+        u[k] = v[k] = make_uint4(0, 0, 0, 0);
+        if (live && i < nvec) u[k] = load_piece<T, VEC>(x + i * N, p.C - i * N), v[k] = load_piece<T, VEC>(y + i * N, p.C - i * N);
+    }
+    float ss = 0.0f;
+#pragma unroll
+    for (int k = 0; k < NP; ++k) {
+        P* a = reinterpret_cast<P*>(&u[k]);
+        const P* b = reinterpret_cast<const P*>(&v[k]);
+#pragma unroll
+        for (int e = 0; e < N / 2; ++e) {
+            const float2 r = ffma2(widen(b[e]), splat2(p.scale), widen(a[e]));
+            a[e] = Ops<T>::pack(r.x, r.y);
+            const float2 f = widen(a[e]);  // the stream as it goes on
+            ss = fmaf(f.x, f.x, ss), ss = fmaf(f.y, f.y, ss);
+        }
+        const int i = l0 + k * step;
+        if (live && i < nvec) store_piece<T, VEC>(static_cast<T*>(p.stream) + row * p.ss + i * N, p.C - i * N, u[k]);
+    }
+#pragma unroll
+    for (int m = 16; m >= 1; m >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, m);
+    if (p.wpr > 1) {
+        if (lane == 0) s_red[warp] = ss;
+        __syncthreads();
+        ss = 0.0f;
+        for (int w = 0; w < p.wpr; ++w) ss += s_red[w0 + w];
+    }
+    const float inv = rsqrtf(fmaf(ss, p.inv_c, p.eps));
+
+    if constexpr (!OUT8) {
+#pragma unroll
+        for (int k = 0; k < NP; ++k) {
+            const int i = l0 + k * step;
+            if (!live || i >= nvec) continue;
+            P* a = reinterpret_cast<P*>(&u[k]);
+#pragma unroll
+            for (int e = 0; e < N / 2; ++e) {
+                const int c = i * N + 2 * e;
+                const float2 f = widen(a[e]);
+                const float wx = VEC || c < p.C ? __ldg(p.w + c) : 0.0f, wy = VEC || c + 1 < p.C ? __ldg(p.w + c + 1) : 0.0f;
+                a[e] = Ops<T>::pack(f.x * inv * wx, f.y * inv * wy);
+            }
+            store_piece<T, VEC>(static_cast<T*>(p.out) + row * p.os + i * N, p.C - i * N, u[k]);
+        }
+    } else {
+        // n in fp32, and the largest magnitudes as bit patterns (a NaN above an infinity)
+        float2 n[NP][N / 2];
+        uint32_t top[NP], all = 0;
+#pragma unroll
+        for (int k = 0; k < NP; ++k) {
+            const int i = l0 + k * step;
+            const P* a = reinterpret_cast<const P*>(&u[k]);
+            top[k] = 0;
+#pragma unroll
+            for (int e = 0; e < N / 2; ++e) {
+                const int c = i * N + 2 * e;
+                const float2 f = widen(a[e]);
+                const bool in0 = live && (VEC ? i < nvec : c < p.C), in1 = live && (VEC ? i < nvec : c + 1 < p.C);
+                n[k][e].x = in0 ? f.x * inv * __ldg(p.w + c) : 0.0f;
+                n[k][e].y = in1 ? f.y * inv * __ldg(p.w + c + 1) : 0.0f;
+                top[k] = max(top[k], max(__float_as_uint(n[k][e].x) & 0x7fffffffu, __float_as_uint(n[k][e].y) & 0x7fffffffu));
+            }
+            all = max(all, top[k]);
+        }
+        if (p.group == p.C) {  // one scale a row
+            all = __reduce_max_sync(0xffffffffu, all);
+            if (p.wpr > 1) {
+                __syncthreads();  // the sums have been read
+                if (lane == 0) s_red[warp] = __uint_as_float(all);
+                __syncthreads();
+                for (int w = 0; w < p.wpr; ++w) all = max(all, __float_as_uint(s_red[w0 + w]));
+            }
+        }
+        const int lanes = p.group / N;  // that share a scale
+#pragma unroll
+        for (int k = 0; k < NP; ++k) {
+            const int i = l0 + k * step;
+            uint32_t t = all;
+            if (p.group != p.C) {
+                t = top[k];
+                for (int m = 1; m < lanes; m <<= 1) t = max(t, __shfl_xor_sync(0xffffffffu, t, m));
+            }
+            const uint32_t byte = e4m3_scale_byte(t);
+            if (!live || i >= nvec) continue;
+            const bool first = p.group != p.C ? (i & (lanes - 1)) == 0 : i == 0;
+            if (first) p.scales[row * p.ngroups + (p.group != p.C ? i / lanes : 0)] = e4m3_scale(byte);
+            union { uint16_t h[N / 2]; uint2 w2; uint32_t w1; } q;
+#pragma unroll
+            for (int e = 0; e < N / 2; ++e) q.h[e] = e4m3_pair(n[k][e], byte);
+            uint8_t* to = static_cast<uint8_t*>(p.out) + row * p.os + i * N;
+            if constexpr (VEC) {
+                if constexpr (N == 8) *reinterpret_cast<uint2*>(to) = q.w2;
+                else *reinterpret_cast<uint32_t*>(to) = q.w1;
+            } else {
+#pragma unroll
+                for (int e = 0; e < N; ++e)
+                    if (i * N + e < p.C) to[e] = static_cast<uint8_t>(q.h[e / 2] >> (8 * (e & 1)));
+            }
+        }
+    }
+}
+
+template <typename T, int NP, bool VEC>
+int launch(const ResidualParams& p, bool out8, cudaStream_t s) {
+    const int warps = std::max(p.wpr, 4), rpb = warps / p.wpr;
+    const int64_t blocks = (p.rows + rpb - 1) / rpb;
+    if (out8) residual_norm_kernel<T, NP, VEC, true><<<static_cast<unsigned>(blocks), 32 * warps, 0, s>>>(p);
+    else residual_norm_kernel<T, NP, VEC, false><<<static_cast<unsigned>(blocks), 32 * warps, 0, s>>>(p);
+    const cudaError_t e = cudaGetLastError();
+    return e == cudaSuccess ? NEED_OK : cuda_fail(e, "residual norm launch");
+}
+
+}  // namespace
+
+extern "C" int need_residual_rms_norm(const need_residual_norm_args* a, need_stream_t stream) {
+    if (a == nullptr) return fail(NEED_ERR_INVALID, "residual norm: args is null");
+    if (!dtype_ok(a->dtype)) return fail(NEED_ERR_UNSUPPORTED, "residual norm: dtype %d", a->dtype);
+    if (a->rows < 1 || a->C < 1) return fail(NEED_ERR_INVALID, "residual norm: sizes must be positive");
+    const int es = dtype_bytes(a->dtype), n = 16 / es;
+    if (a->C * es > kRowBytes || a->rows > (int64_t(1) << 31) - 1)
+        return fail(NEED_ERR_UNSUPPORTED, "residual norm: rows of at most %d bytes, 2^31 - 1 of them", kRowBytes);
+    if (!(a->eps >= 0.0)) return fail(NEED_ERR_INVALID, "residual norm: eps must be >= 0");
+    if (a->x == nullptr || a->y == nullptr || a->weight == nullptr || a->stream == nullptr || a->out == nullptr)
+        return fail(NEED_ERR_INVALID, "residual norm: x, y, weight, stream and out are required");
+    if (a->out8 != 0 && (a->out8 != 1 || a->scales == nullptr || (a->group != 32 && a->group != 64 && a->group != 128 && a->group != a->C)))
+        return fail(NEED_ERR_INVALID, "residual norm: an 8-bit output needs scales, one for 32, 64, 128 or all channels");
+    if (a->rows > 1 && (a->stream_stride < a->C || a->out_stride < a->C))
+        return fail(NEED_ERR_INVALID, "residual norm: the outputs' rows overlap");
+    ResidualParams p{};
+    p.x = a->x, p.xs = a->x_stride, p.y = a->y, p.ys = a->y_stride, p.w = a->weight;
+    p.stream = a->stream, p.ss = a->stream_stride, p.out = a->out, p.os = a->out_stride, p.scales = a->scales;
+    p.rows = a->rows, p.C = int32_t(a->C), p.group = a->out8 ? int32_t(a->group) : 0;
+    p.ngroups = a->out8 ? int32_t((a->C + a->group - 1) / a->group) : 0;
+    p.inv_c = 1.0f / static_cast<float>(a->C), p.eps = static_cast<float>(a->eps), p.scale = static_cast<float>(a->scale);
+    const int nvec = int32_t((a->C + n - 1) / n);
+    p.wpr = 1;
+    while (p.wpr * 32 * kPieces < nvec) p.wpr *= 2;
+    const int np = (nvec + 32 * p.wpr - 1) / (32 * p.wpr);
+    auto al = [&](const void* q, int64_t stride, int bytes) {
+        return reinterpret_cast<uintptr_t>(q) % bytes == 0 && (a->rows == 1 || stride * (q == a->out && a->out8 ? 1 : es) % bytes == 0);
+    };
+    const bool vec = a->C % n == 0 && al(p.x, p.xs, 16) && al(p.y, p.ys, 16) && al(p.stream, p.ss, 16) &&
+                     al(p.out, p.os, a->out8 ? n : 16);
+    auto run = [&](auto tag) {
+        using T = decltype(tag);
+        auto go = [&](auto v) {
+            constexpr bool V = decltype(v)::value;
+            switch (np) {
+                case 1: return launch<T, 1, V>(p, a->out8 != 0, stream);
+                case 2: return launch<T, 2, V>(p, a->out8 != 0, stream);
+                case 3: return launch<T, 3, V>(p, a->out8 != 0, stream);
+                default: return launch<T, 4, V>(p, a->out8 != 0, stream);
+            }
+        };
+        return vec ? go(std::true_type{}) : go(std::false_type{});
+    };
+    const int rc = a->dtype == NEED_F32 ? run(float{}) : a->dtype == NEED_BF16 ? run(__nv_bfloat16{}) : run(__half{});
+    return rc != NEED_OK ? rc : ok();
+}

@@ -1,0 +1,529 @@
+// token_log_probs.cu -- log probabilities of given tokens, the entropy and the largest
+// alternatives of rows of logits (need_token_log_probs), and the gradient
+// (need_token_log_probs_backward).  With x = logits / temperature, m its largest,
+//
+//   S = sum e^{x - m},  log p_j = x_j - m - log S,  H = log S - sum e^{x - m} (x - m) / S
+//   dx_j = g (1[j = token] - p_j) - gh p_j (log p_j + H)
+//
+// The sums run in one pass with a running maximum, which a warp shares; what they leave
+// out are the maxima themselves, which are counted: with r the rest, log S = log(count) +
+// log1p(r / count), so that probabilities near 1 and small entropies keep their relative
+// precision (both terms of H are positive).
+//
+// The largest: among the maxima of a row's threads the k-th is a bound that k logits reach,
+// so a second pass (from L2) has only few to gather, and their order is counted out.  Keys
+// order by value, then by the lower token.
+//
+// Short rows take a warp each, longer ones 8; where there are few, rows are cut into parts
+// that a second launch joins, in order.  Rows of any alignment: the elements before the
+// first and after the last whole 16 bytes are taken one by one.  Per logit: 2 or 4 B, one
+// ex2 (16 a cycle and SM, which comes near HBM's rate for 16 bits) and some 6 other
+// instructions.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <float.h>
+
+#include <algorithm>
+
+#include "host_common.h"
+#include "need_scan.h"
+
+using namespace need;
+
+namespace {
+
+constexpr int kThreads = 256, kWarps = kThreads / 32;
+constexpr int UN = 4;              // 16-byte pieces of a lane in flight
+constexpr int kList = 1024;        // keys that a block gathers (a warp of its own: an eighth)
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.69314718055994531f;
+constexpr float kLow = -200.0f;    // 2^kLow is 0, and its product with kLow too
+using u64 = unsigned long long;
+
+struct LogpParams {
+    const void* logits;
+    int64_t stride;
+    const int64_t* tokens;
+    float* log_prob;
+    float* entropy;
+    float* stats;
+    float* top_lp;
+    int64_t* top_id;
+    int64_t rows, V, len;  // len: logits of a part
+    int32_t top, parts;
+    float inv_t;
+    float4* part;          // [rows, parts]: m, count, r, u
+    u64* part_top;         // [rows, parts, top]
+    const float* g;
+    const float* gh;
+    void* grad;
+    int64_t grad_stride;
+};
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float to_float(float x) { return x; }
+__device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
+__device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
+__device__ __forceinline__ float nan32() { return __int_as_float(0x7fc00000); }
+
+template <typename T>
+struct Vec {
+    static constexpr int N = 16 / sizeof(T);
+    static __device__ __forceinline__ void widen(const uint4& u, float* f) {
+        const T* e = reinterpret_cast<const T*>(&u);
+#pragma unroll
+        for (int i = 0; i < N; ++i) f[i] = to_float(e[i]);
+    }
+};
+
+// A run of a row's logits: `head` elements, `nvec` whole 16-byte pieces, `tail` elements.
+template <typename T>
+struct Run {
+    static constexpr int N = Vec<T>::N;
+    const T* x;
+    int64_t nvec;
+    int head, tail;
+    __device__ __forceinline__ Run(const T* x_, int64_t len) : x(x_) {
+        const int off = static_cast<int>((reinterpret_cast<uintptr_t>(x_) & 15u) / sizeof(T));
+        const int64_t h = off == 0 ? 0 : N - off;
+        head = static_cast<int>(h < len ? h : len);
+        nvec = (len - head) / N;
+        tail = static_cast<int>(len - head - nvec * N);
+    }
+    __device__ __forceinline__ const uint4* body() const { return reinterpret_cast<const uint4*>(x + head); }
+    __device__ __forceinline__ int edges() const { return head + tail; }
+    __device__ __forceinline__ int64_t edge(int n) const { return n < head ? n : nvec * N + n; }  // its index
+};
+
+// ------------------------------------------------------------------ sums
+struct Sums {
+    float m, cnt, r, u;  // the largest, how many equal it, the others' sum of 2^z, and of z 2^z
+};
+// b joined to a
+__device__ __forceinline__ void join(Sums& a, const Sums& b, float c) {
+    const float m = fmaxf(a.m, b.m);
+    const float da = a.m == m ? 0.0f : fmaxf((a.m - m) * c, kLow), db = b.m == m ? 0.0f : fmaxf((b.m - m) * c, kLow);
+    const float fa = a.m == m ? 1.0f : ex2(da), fb = b.m == m ? 1.0f : ex2(db);
+    // of a side below the maximum the largest are among the rest
+    const float ra = a.m == m ? a.r : fa * (a.r + a.cnt), rb = b.m == m ? b.r : fb * (b.r + b.cnt);
+    a.u = fa * (a.u + da * (a.r + a.cnt)) + fb * (b.u + db * (b.r + b.cnt));
+    a.cnt = (a.m == m ? a.cnt : 0.0f) + (b.m == m ? b.cnt : 0.0f);
+    a.r = ra + rb;
+    a.m = m;
+}
+__device__ __forceinline__ int order(float x) {  // signed, no NaN
+    const int b = __float_as_int(x);
+    return b ^ ((b >> 31) & 0x7fffffff);
+}
+__device__ __forceinline__ float unorder(int k) { return __int_as_float(k ^ ((k >> 31) & 0x7fffffff)); }
+
+// K logits of each lane into the warp's sums (s.m is the warp's, the rest the lane's); tm:
+// the lane's largest.
+template <int K>
+__device__ __forceinline__ void add(const float (&x)[K], Sums& s, float& tm, float c) {
+    float lm = x[0];
+#pragma unroll
+    for (int i = 1; i < K; ++i) lm = fmaxf(lm, x[i]);
+    lm = fmaxf(lm, -INFINITY);  // a NaN is no maximum
+    tm = fmaxf(tm, lm);
+    const float wm = unorder(__reduce_max_sync(0xffffffffu, order(lm)));
+    if (wm > s.m) {
+        const float d = fmaxf((s.m - wm) * c, kLow), f = ex2(d);
+        s.u = f * (s.u + d * (s.r + s.cnt));
+        s.r = f * (s.r + s.cnt);
+        s.cnt = 0.0f, s.m = wm;
+    }
+    const float m = s.m == -INFINITY ? 0.0f : s.m;
+    if (wm == s.m && wm > -INFINITY) {  // the largest are in this batch
+#pragma unroll
+        for (int i = 0; i < K; ++i) {
+            const bool hit = x[i] == m;
+            const float z = (x[i] - m) * c, e = hit ? 0.0f : ex2(z);
+            s.cnt += hit ? 1.0f : 0.0f;
+            s.r += e;
+            s.u = fmaf(e, fmaxf(z, kLow), s.u);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < K; ++i) {
+            const float z = (x[i] - m) * c, e = ex2(z);
+            s.r += e;
+            s.u = fmaf(e, fmaxf(z, kLow), s.u);
+        }
+    }
+}
+
+// ------------------------------------------------------------------ keys
+__device__ __forceinline__ u64 key_of(float x, int64_t i) {
+    const uint32_t v = x != x ? 0xffffffffu : static_cast<uint32_t>(order(x)) ^ 0x80000000u;
+    return (static_cast<u64>(v) << 32) | (0xffffffffu - static_cast<uint32_t>(i));
+}
+__device__ __forceinline__ float value_of(u64 k) {
+    const uint32_t v = static_cast<uint32_t>(k >> 32);
+    return v == 0xffffffffu ? nan32() : unorder(static_cast<int>(v ^ 0x80000000u));
+}
+__device__ __forceinline__ int64_t token_of(u64 k) { return 0xffffffffu - static_cast<uint32_t>(k); }
+
+// The `top` largest of n keys in order, 0 behind them; threads t, t + step, ...
+__device__ __forceinline__ void rank_keys(const u64* keys, int n, int top, u64* out, int t, int step) {
+    for (int i = t; i < n; i += step) {
+        const u64 k = keys[i];
+        int r = 0;
+        if (k == 0) continue;
+        for (int j = 0; j < n; ++j) r += keys[j] > k ? 1 : 0;
+        if (r < top) out[r] = k;
+    }
+}
+
+// ------------------------------------------------------------------ the row's results
+struct Result {
+    float m, l, inv_t;  // the largest logit, log S
+    __device__ __forceinline__ float log_p(float x) const { return m == -INFINITY ? l - INFINITY : fmaf(x - m, inv_t, -l); }
+};
+// One thread writes the row's log p, entropy and stats.
+template <typename T>
+__device__ __forceinline__ Result finish(const LogpParams& p, int64_t row, const Sums& s, bool write) {
+    Result res{s.m, 0.0f, p.inv_t};
+    float h = 0.0f;
+    if (s.m == INFINITY || s.r != s.r) {
+        res.l = h = nan32();
+    } else if (s.m > -INFINITY) {
+        res.l = s.cnt == 1.0f ? log1pf(s.r) : logf(s.cnt) + log1pf(s.r / s.cnt);
+        h = res.l - kLn2 * (s.u / (s.cnt + s.r));
+    }
+    if (write) {
+        const int64_t tok = p.tokens[row];
+        float lp = 0.0f;
+        if (tok >= p.V) lp = nan32();
+        else if (tok >= 0) lp = res.log_p(to_float(static_cast<const T*>(p.logits)[row * p.stride + tok]));
+        p.log_prob[row] = lp, p.entropy[row] = h;
+        if (p.stats != nullptr) p.stats[2 * row] = s.m, p.stats[2 * row + 1] = res.l;
+    }
+    return res;
+}
+__device__ __forceinline__ void write_top(const LogpParams& p, int64_t row, const Result& res, const u64* keys, int t, int step) {
+    for (int i = t; i < p.top; i += step) {
+        const u64 k = keys[i];
+        p.top_lp[row * p.top + i] = k == 0 ? (res.l != res.l ? res.l : -INFINITY) : res.log_p(value_of(k));
+        p.top_id[row * p.top + i] = k == 0 ? -1 : token_of(k);
+    }
+}
+
+// ------------------------------------------------------------------ kernels
+// WPR warps a row: 1, or all of the block's, which then take part blockIdx.y of the row.
+template <typename T, int WPR>
+__global__ void __launch_bounds__(kThreads) logp_kernel(const LogpParams p) {
+    constexpr int N = Vec<T>::N, TEAM = 32 * WPR, CAP = kList * WPR / kWarps;
+    __shared__ Sums s_sums[kWarps];
+    __shared__ int s_max[kThreads];
+    __shared__ u64 s_keys[kList], s_top[kWarps * NEED_TOKEN_LOG_PROBS_MAX_TOP];
+    __shared__ int s_n[kWarps];
+    __shared__ float s_thr[kWarps];
+    auto sync = [] {
+        if (WPR == 1) __syncwarp();
+        else __syncthreads();
+    };
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int team = warp / WPR, tt = threadIdx.x % TEAM;
+    const int64_t row = int64_t(blockIdx.x) * (kWarps / WPR) + team;
+    if (row >= p.rows) return;  // a whole team
+    const int64_t first = int64_t(blockIdx.y) * p.len;
+    const Run<T> run(static_cast<const T*>(p.logits) + row * p.stride + first, p.len < p.V - first ? p.len : p.V - first);
+    const float c = p.inv_t * kLog2e;
+
+    Sums s{-INFINITY, 0.0f, 0.0f, 0.0f};
+    float tm = -INFINITY;
+    // the pieces, UN a lane at a time; every lane of a warp takes part in every batch
+    for (int64_t v0 = 0; v0 < run.nvec; v0 += TEAM * UN) {
+        float x[UN * N];
+        uint4 u[UN];
+#pragma unroll
+        for (int k = 0; k < UN; ++k) {
+            const int64_t v = v0 + k * TEAM + tt;
+            if (v < run.nvec) u[k] = __ldg(run.body() + v);
+        }
+#pragma unroll
+        for (int k = 0; k < UN; ++k) {
+            if (v0 + k * TEAM + tt < run.nvec) {
+                Vec<T>::widen(u[k], x + k * N);
+            } else {
+#pragma unroll
+                for (int e = 0; e < N; ++e) x[k * N + e] = -INFINITY;
+            }
+        }
+        add(x, s, tm, c);
+    }
+    if (warp % WPR == 0 && run.edges() > 0) {
+        const float x[1] = {lane < run.edges() ? to_float(run.x[run.edge(lane)]) : -INFINITY};
+        add(x, s, tm, c);
+    }
+#pragma unroll
+    for (int m = 16; m >= 1; m >>= 1) {
+        s.cnt += __shfl_xor_sync(0xffffffffu, s.cnt, m);
+        s.r += __shfl_xor_sync(0xffffffffu, s.r, m);
+        s.u += __shfl_xor_sync(0xffffffffu, s.u, m);
+    }
+    if (WPR > 1) {
+        if (lane == 0) s_sums[warp] = s;
+        __syncthreads();
+        s = s_sums[0];
+        for (int w = 1; w < WPR; ++w) join(s, s_sums[w], c);
+    }
+
+    u64* const keys = s_keys + team * CAP;
+    u64* const top = s_top + team * NEED_TOKEN_LOG_PROBS_MAX_TOP;
+    if (p.top > 0) {
+        // the top-th largest of the threads' maxima
+        s_max[threadIdx.x] = order(tm);
+        if (tt == 0) s_n[team] = 0;
+        for (int i = tt; i < p.top; i += TEAM) top[i] = 0;
+        sync();
+        const int mine = order(tm), base = team * TEAM;
+        int rank = 0;
+        for (int j = 0; j < TEAM; ++j) rank += s_max[base + j] > mine || (s_max[base + j] == mine && j < tt) ? 1 : 0;
+        if (rank == p.top - 1) s_thr[team] = tm == -INFINITY ? -FLT_MAX : tm;
+        sync();
+        const float thr = s_thr[team];
+        auto gather = [&](float x, int64_t i) {
+            if (!(x < thr)) {
+                const int n = atomicAdd(&s_n[team], 1);
+                if (n < CAP) keys[n] = key_of(x, first + i);
+            }
+        };
+        auto each = [&](auto&& f) {
+            for (int64_t v = tt; v < run.nvec; v += TEAM) {
+                float x[N];
+                Vec<T>::widen(__ldg(run.body() + v), x);
+#pragma unroll
+                for (int e = 0; e < N; ++e) f(x[e], run.head + v * N + e);
+            }
+            if (tt < run.edges()) f(to_float(run.x[run.edge(tt)]), run.edge(tt));
+        };
+        each(gather);
+        sync();
+        const int n = s_n[team];
+        if (n <= CAP) {
+            rank_keys(keys, n, p.top, top, tt, TEAM);
+        } else {  // too many reach the bound: one after another, a pass each
+            u64 below = ~0ull;
+            for (int k = 0; k < p.top; ++k) {
+                u64 best = 0;
+                each([&](float x, int64_t i) {
+                    const u64 key = x == -INFINITY ? 0 : key_of(x, first + i);
+                    if (key < below && key > best) best = key;
+                });
+#pragma unroll
+                for (int m = 16; m >= 1; m >>= 1) {
+                    const u64 o = __shfl_xor_sync(0xffffffffu, best, m);
+                    best = o > best ? o : best;
+                }
+                if (WPR > 1) {
+                    __syncthreads();  // the keys of the last round have been read
+                    if (lane == 0) s_keys[warp] = best;
+                    __syncthreads();
+                    for (int w = 0; w < WPR; ++w) best = s_keys[w] > best ? s_keys[w] : best;
+                }
+                if (tt == 0) top[k] = best;
+                if (best == 0) break;
+                below = best;
+            }
+        }
+        sync();
+    }
+    if (p.parts > 1) {
+        const int64_t at = row * p.parts + blockIdx.y;
+        if (tt == 0) p.part[at] = make_float4(s.m, s.cnt, s.r, s.u);
+        for (int i = tt; i < p.top; i += TEAM) p.part_top[at * p.top + i] = top[i];
+        return;
+    }
+    const Result res = finish<T>(p, row, s, tt == 0);
+    if (p.top > 0) write_top(p, row, res, top, tt, TEAM);
+}
+
+// A block joins a row's parts.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) join_kernel(const LogpParams p) {
+    __shared__ u64 s_top[NEED_TOKEN_LOG_PROBS_MAX_TOP];
+    const int64_t row = blockIdx.x;
+    const float4* part = p.part + row * p.parts;
+    Sums s{part[0].x, part[0].y, part[0].z, part[0].w};
+    for (int i = 1; i < p.parts; ++i) {
+        const float4 f = part[i];
+        join(s, Sums{f.x, f.y, f.z, f.w}, p.inv_t * kLog2e);
+    }
+    if (p.top > 0) {
+        if (threadIdx.x < p.top) s_top[threadIdx.x] = 0;
+        __syncthreads();
+        rank_keys(p.part_top + row * p.parts * p.top, p.parts * p.top, p.top, s_top, threadIdx.x, kThreads);
+        __syncthreads();
+    }
+    const Result res = finish<T>(p, row, s, threadIdx.x == 0);
+    if (p.top > 0) write_top(p, row, res, s_top, threadIdx.x, kThreads);
+}
+
+// A warp takes 32 * UN pieces of a row.  SAME: the gradient's rows lie as the logits' do
+// within 16 bytes.
+template <typename T, bool SAME>
+__global__ void __launch_bounds__(kThreads) logp_backward_kernel(const LogpParams p) {
+    constexpr int N = Vec<T>::N;
+    const int lane = threadIdx.x & 31;
+    const int64_t id = int64_t(blockIdx.x) * kWarps + (threadIdx.x >> 5), row = id / p.parts, part = id % p.parts;
+    if (row >= p.rows) return;
+    const Run<T> run(static_cast<const T*>(p.logits) + row * p.stride, p.V);
+    T* const out = static_cast<T*>(p.grad) + row * p.grad_stride;
+    uint4 u[UN];
+    const int64_t v0 = part * 32 * UN + lane;
+#pragma unroll
+    for (int k = 0; k < UN; ++k)
+        if (v0 + k * 32 < run.nvec) u[k] = __ldcs(run.body() + v0 + k * 32);
+    const float m = p.stats[2 * row], l = p.stats[2 * row + 1], h = p.entropy[row];
+    const float g = p.g != nullptr ? p.g[row] : 0.0f, gh = p.gh != nullptr ? p.gh[row] : 0.0f;
+    const int64_t tok = p.tokens[row];
+    const bool given = tok >= 0;
+    const float gt = tok >= p.V ? nan32() : given ? g : 0.0f;  // of the token's log p
+    const float c = p.inv_t * kLog2e, l2 = l * kLog2e, ms = m == -INFINITY ? 0.0f : m;
+    const float a = p.inv_t * -(gt + gh * h), b = p.inv_t * -gh * kLn2;  // dx = p (a + b log2 p)
+    auto grad = [&](float x) {
+        const float z = fmaf(x - ms, c, -l2);
+        return ex2(z) * fmaf(b, fmaxf(z, kLow), a);
+    };
+    auto at_token = [&](float x) {  // 1 - p from log p: p may be near 1
+        const float lp = fmaf(x - ms, p.inv_t, -l);
+        const float q = expf(lp);
+        return p.inv_t * (gt * -expm1f(lp) - gh * q * (fmaxf(lp, kLow) + h));
+    };
+    auto one = [&](float x, int64_t i) {
+        if (m == -INFINITY && l == l) return gt == gt ? 0.0f : gt;  // a row of nothing
+        return i == tok ? at_token(x) : grad(x);
+    };
+#pragma unroll
+    for (int k = 0; k < UN; ++k) {
+        const int64_t v = v0 + k * 32, i0 = run.head + v * N;
+        if (v >= run.nvec) break;
+        float x[N];
+        Vec<T>::widen(u[k], x);
+        const bool plain = !(m == -INFINITY) && (tok < i0 || tok >= i0 + N);
+#pragma unroll
+        for (int e = 0; e < N; ++e) x[e] = plain ? grad(x[e]) : one(x[e], i0 + e);
+        union { uint4 u; T e[N]; } r;
+#pragma unroll
+        for (int e = 0; e < N; ++e) r.e[e] = static_cast<T>(x[e]);
+        if constexpr (SAME) {
+            __stcs(reinterpret_cast<uint4*>(out + i0), r.u);
+        } else {
+#pragma unroll
+            for (int e = 0; e < N; ++e) out[i0 + e] = r.e[e];
+        }
+    }
+    if (part == 0 && lane < run.edges()) {
+        const int64_t i = run.edge(lane);
+        out[i] = static_cast<T>(one(to_float(run.x[i]), i));
+    }
+}
+
+// ------------------------------------------------------------------ host
+struct Shape {
+    bool wide;      // 8 warps a row
+    int32_t parts;
+    int64_t len;
+};
+Shape shape_of(int32_t dtype, int64_t rows, int64_t V) {
+    const int n = 16 / dtype_bytes(dtype);
+    Shape s{V > 2048, 1, V};
+    if (s.wide && rows < 148) {  // two blocks a multiprocessor, whole batches each
+        const int64_t batch = int64_t(kThreads) * UN * n;
+        int64_t parts = std::min((296 + rows - 1) / rows, (V + batch - 1) / batch);
+        s.len = (V + parts - 1) / parts;
+        s.len = (s.len + n - 1) / n * n;  // parts lie alike within 16 bytes
+        s.parts = int32_t((V + s.len - 1) / s.len);
+    }
+    return s;
+}
+
+int check_args(const need_token_log_probs_args* a) {
+    if (a == nullptr) return fail(NEED_ERR_INVALID, "token log probs: args is null");
+    if (!dtype_ok(a->dtype)) return fail(NEED_ERR_UNSUPPORTED, "token log probs: dtype %d", a->dtype);
+    if (a->rows < 1 || a->V < 1) return fail(NEED_ERR_INVALID, "token log probs: sizes must be positive");
+    if (a->rows > (int64_t(1) << 31) - 1 || a->V > (int64_t(1) << 31) - 1)
+        return fail(NEED_ERR_UNSUPPORTED, "token log probs: at most 2^31 - 1 rows and logits a row");
+    if (a->logits == nullptr || a->tokens == nullptr || a->entropy == nullptr)
+        return fail(NEED_ERR_INVALID, "token log probs: logits, tokens and entropy are required");
+    if (!(a->temperature >= 1e-30 && a->temperature <= 1e30)) return fail(NEED_ERR_INVALID, "token log probs: temperature must lie in [1e-30, 1e30]");
+    return NEED_OK;
+}
+LogpParams params(const need_token_log_probs_args* a) {
+    LogpParams p{};
+    p.logits = a->logits, p.stride = a->stride, p.tokens = a->tokens, p.log_prob = a->log_prob, p.entropy = a->entropy;
+    p.stats = a->stats, p.rows = a->rows, p.V = a->V, p.inv_t = static_cast<float>(1.0 / a->temperature);
+    return p;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t need_token_log_probs_workspace_size(int32_t dtype, int64_t rows, int64_t V, int32_t top) {
+    if (!dtype_ok(dtype) || rows < 1 || V < 1 || top < 0) return 16;
+    const Shape s = shape_of(dtype, rows, V);
+    return s.parts == 1 ? 16 : size_t(rows) * s.parts * (sizeof(float4) + sizeof(u64) * top);
+}
+
+int need_token_log_probs(const need_token_log_probs_args* a, need_stream_t stream) {
+    int rc = check_args(a);
+    if (rc != NEED_OK) return rc;
+    if (a->log_prob == nullptr) return fail(NEED_ERR_INVALID, "token log probs: log_prob is required");
+    if (a->top < 0 || a->top > a->V || (a->top > 0 && (a->top_log_probs == nullptr || a->top_tokens == nullptr)))
+        return fail(NEED_ERR_INVALID, "token log probs: 0 to V alternatives, and their outputs");
+    if (a->top > NEED_TOKEN_LOG_PROBS_MAX_TOP)
+        return fail(NEED_ERR_UNSUPPORTED, "token log probs: at most %d alternatives", NEED_TOKEN_LOG_PROBS_MAX_TOP);
+    const Shape s = shape_of(a->dtype, a->rows, a->V);
+    if (s.parts > 1 && (a->workspace == nullptr || !aligned16(a->workspace) ||
+                        a->workspace_bytes < need_token_log_probs_workspace_size(a->dtype, a->rows, a->V, a->top)))
+        return fail(NEED_ERR_WORKSPACE, "token log probs: workspace missing, misaligned or too small");
+    LogpParams p = params(a);
+    p.top = a->top, p.top_lp = a->top_log_probs, p.top_id = a->top_tokens, p.parts = s.parts, p.len = s.len;
+    if (s.parts > 1) {
+        p.part = static_cast<float4*>(a->workspace);
+        p.part_top = reinterpret_cast<u64*>(p.part + a->rows * s.parts);
+    }
+    auto run = [&](auto tag) {
+        using T = decltype(tag);
+        if (s.wide) logp_kernel<T, kWarps><<<dim3(static_cast<unsigned>(a->rows), s.parts), kThreads, 0, stream>>>(p);
+        else logp_kernel<T, 1><<<static_cast<unsigned>((a->rows + kWarps - 1) / kWarps), kThreads, 0, stream>>>(p);
+        if (s.parts > 1) join_kernel<T><<<static_cast<unsigned>(a->rows), kThreads, 0, stream>>>(p);
+    };
+    if (a->dtype == NEED_F32) run(float{});
+    else if (a->dtype == NEED_BF16) run(__nv_bfloat16{});
+    else run(__half{});
+    const cudaError_t e = cudaGetLastError();
+    return e == cudaSuccess ? ok() : cuda_fail(e, "token log probs launch");
+}
+
+int need_token_log_probs_backward(const need_token_log_probs_args* a, need_stream_t stream) {
+    int rc = check_args(a);
+    if (rc != NEED_OK) return rc;
+    if (a->stats == nullptr || a->grad == nullptr) return fail(NEED_ERR_INVALID, "token log probs: stats and grad are required");
+    if (a->rows > 1 && a->grad_stride < a->V) return fail(NEED_ERR_INVALID, "token log probs: the gradient's rows overlap");
+    LogpParams p = params(a);
+    const int es = dtype_bytes(a->dtype), n = 16 / es;
+    const int64_t parts = std::max<int64_t>(1, (a->V / n + 32 * UN - 1) / (32 * UN)), blocks = (a->rows * parts + kWarps - 1) / kWarps;
+    if (blocks > (int64_t(1) << 31) - 1) return fail(NEED_ERR_UNSUPPORTED, "token log probs: too many logits");
+    p.parts = static_cast<int32_t>(parts), p.g = a->g_log_prob, p.gh = a->g_entropy, p.grad = a->grad, p.grad_stride = a->grad_stride;
+    const bool same = (reinterpret_cast<uintptr_t>(a->logits) - reinterpret_cast<uintptr_t>(a->grad)) % 16 == 0 &&
+                      (a->rows == 1 || (a->stride - a->grad_stride) * es % 16 == 0);
+    auto run = [&](auto tag) {
+        using T = decltype(tag);
+        if (same) logp_backward_kernel<T, true><<<static_cast<unsigned>(blocks), kThreads, 0, stream>>>(p);
+        else logp_backward_kernel<T, false><<<static_cast<unsigned>(blocks), kThreads, 0, stream>>>(p);
+    };
+    if (a->dtype == NEED_F32) run(float{});
+    else if (a->dtype == NEED_BF16) run(__nv_bfloat16{});
+    else run(__half{});
+    const cudaError_t e = cudaGetLastError();
+    return e == cudaSuccess ? ok() : cuda_fail(e, "token log probs launch");
+}
+
+}  // extern "C"

@@ -29,7 +29,12 @@ out_norm fused), ``linear_associative_memory`` (HierarchicalMemory's
 matrix-state memory, need_core.py:1960-2001), the pieces of the
 sequence-parallel scan used by ``need_b200.sp``, and the block's operators for
 training, with gradients (``need_b200.train``): ``gated_scan_train``,
-``ssd_scan_train``, ``ssd_conv_silu_train`` and ``rms_norm_train``.
+``ssd_scan_train``, ``ssd_conv_silu_train`` and ``rms_norm_train``; and around the
+block (``need_b200.lm``) ``linear_attention`` and ``linear_attention_step`` (matrix
+states with a decay for each head, over prompts and for single tokens),
+``residual_rms_norm`` (the residual's addition, the norm, optionally in 8 bits) and
+``token_log_probs`` (log probabilities of given tokens, with entropy,
+alternatives and gradient).
 """
 from __future__ import annotations
 
@@ -42,6 +47,7 @@ import torch
 import torch.nn.functional as F
 
 from . import abi
+from .lm import TokenLogProbs, linear_attention, linear_attention_step, residual_rms_norm, token_log_probs  # noqa: F401
 from .train import gated_scan_train, rms_norm_train, ssd_conv_silu_train, ssd_scan_train  # noqa: F401
 
 HAS_TRITON = False  # the reference's flag: this module uses no Triton
