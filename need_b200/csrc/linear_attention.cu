@@ -90,13 +90,20 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
     asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
     return r;
 }
-// x and y as the sums of N bf16 values each.
+__device__ __forceinline__ float2 unpack_bf16(uint32_t u) {
+    return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+}
+__device__ __forceinline__ float2 splat(float x) { return make_float2(x, x); }
+// The two of x as the sums of N bf16 values each.
 template <int N>
-__device__ __forceinline__ void split(float x, float y, uint32_t (&pl)[N]) {
+__device__ __forceinline__ void split(float2 x, uint32_t (&pl)[N]) {
 #pragma unroll
     for (int n = 0; n < N; ++n) {
-        pl[n] = pack_bf16(x, y);
-        if (n + 1 < N) x -= __uint_as_float(pl[n] << 16), y -= __uint_as_float(pl[n] & 0xffff0000u);
+        pl[n] = pack_bf16(x.x, x.y);
+        if (n + 1 < N) {
+            const float2 f = unpack_bf16(pl[n]);
+            x = __fadd2_rn(x, make_float2(-f.x, -f.y));
+        }
     }
 }
 
@@ -109,7 +116,7 @@ __device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t addr) {
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
 __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
@@ -119,11 +126,11 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool l
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 __device__ __forceinline__ void cp_wait_all() { asm volatile("cp.async.wait_group 0;" ::: "memory"); }
 
-// Byte offset of 16-byte piece `piece` of row `row` in a plane of COLS bf16 columns: pieces
-// change places within 8 rows, so that ldmatrix meets every bank once.
-template <int COLS>
+// Byte offset of 16-byte piece `piece` of row `row` in a plane of bf16 rows, 64 columns
+// (128 bytes) at a time: pieces change places within 8 rows, so that ldmatrix meets every
+// bank once.
 __device__ __forceinline__ uint32_t at(int row, int piece) {
-    return static_cast<uint32_t>(row * COLS * 2 + ((piece ^ (row & 7)) << 4));
+    return static_cast<uint32_t>((piece >> 3) * C * 128 + row * 128 + (((piece & 7) ^ (row & 7)) << 4));
 }
 
 // Planes of a type's inputs, of computed operands, and the sum of plane numbers below
@@ -142,11 +149,28 @@ struct Split<float> {
 };
 constexpr int kStatePlanes = 3;  // of v e^{...}: what the state sums
 
+// f(a, b) for the planes a < NA and b < NB whose numbers sum to less than LIM, the smallest
+// products first.
+template <int LIM, int NA, int NB, typename F>
+__device__ __forceinline__ void products(F&& f) {
+#pragma unroll
+    for (int sum = LIM - 1; sum >= 0; --sum)
+#pragma unroll
+        for (int a = 0; a < NA; ++a)
+            if (a <= sum && sum - a < NB) f(a, sum - a);
+}
+__device__ __forceinline__ void add4(float (&x)[4], const float (&y)[4]) {
+    const float2 a = __fadd2_rn(make_float2(x[0], x[1]), make_float2(y[0], y[1]));
+    const float2 b = __fadd2_rn(make_float2(x[2], x[3]), make_float2(y[2], y[3]));
+    x[0] = a.x, x[1] = a.y, x[2] = b.x, x[3] = b.y;
+}
+
 // A chunk's decays.
 struct alignas(16) Decays {
     float hi[C], lo[C];  // log2 of the product from the chunk's first token on, as a sum
     float w[C];          // from a token to the chunk's end; 0 where a segment starts in between
-    float eg[C];         // from the entering state to a token; 0 likewise
+    float eg[C];         // scale times that from the entering state to a token; 0 likewise
+    float end[C];        // from a token to the end of its block of 16
     int seg[C];          // segments started up to the token
     float d;             // over the chunk; -1 where a segment starts in it
 };
@@ -193,31 +217,51 @@ __device__ __forceinline__ bool load_planes(char* dst, const T* base, int64_t st
         uint32_t pl[4][IN];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            split<IN>(f[2 * e], f[2 * e + 1], pl[e]);
+            split<IN>(make_float2(f[2 * e], f[2 * e + 1]), pl[e]);
             // of a value that rounds to an infinity the first plane is one
             chk = fmaf(__uint_as_float(pl[e][0] << 16), 0.0f, chk);
             chk = fmaf(__uint_as_float(pl[e][0] & 0xffff0000u), 0.0f, chk);
         }
 #pragma unroll
         for (int p = 0; p < IN; ++p)
-            *reinterpret_cast<uint4*>(dst + p * C * COLS * 2 + at<COLS>(row, piece)) =
+            *reinterpret_cast<uint4*>(dst + p * C * COLS * 2 + at(row, piece)) =
                 make_uint4(pl[0][p], pl[1][p], pl[2][p], pl[3][p]);
     }
     return !(chk == 0.0f);
 }
 
-// The same of bf16 rows by asynchronous copies, 16 bytes each.
+// The same of bf16 rows by asynchronous copies of 16 bytes.  A thread copies one piece of
+// every 16th row (of 64 columns), or of every 8th (of 128).
 template <int COLS>
-__device__ __forceinline__ void copy_rows(uint32_t dst, const __nv_bfloat16* base, int64_t st, int64_t t0, int64_t T_,
-                                          int col0, int cols) {
-    constexpr int PIECES = COLS / 8;
-#pragma unroll
-    for (int n0 = 0; n0 < C * PIECES; n0 += kThreads) {
-        const int n = n0 + threadIdx.x, row = n / PIECES, piece = n % PIECES, col = col0 + piece * 8;
-        const bool live = t0 + row < T_ && col < cols;
-        cp_async16(dst + at<COLS>(row, piece), live ? base + (t0 + row) * st + col : base, live);
+struct Copier {
+    static constexpr int PIECES = COLS / 8, STEP = kThreads / PIECES, N = C / STEP;  // rows apart, copies
+    const __nv_bfloat16* from;
+    int64_t st;
+    uint32_t to;  // within the plane
+    int row;
+    bool in;
+    __device__ __forceinline__ Copier(const __nv_bfloat16* base, int64_t st_, int64_t t0, int col0, int cols) : st(st_) {
+        row = threadIdx.x / PIECES;
+        const int piece = threadIdx.x % PIECES, col = col0 + piece * 8;
+        in = col < cols;
+        to = at(row, piece);
+        from = base + (in ? (t0 + row) * st + col : 0);
     }
-}
+    // rows of a chunk of `rows` of them, into the plane at dst; then on to the next chunk
+    __device__ __forceinline__ void copy(uint32_t dst, const __nv_bfloat16* base, int64_t rows) {
+        if (rows >= C) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) cp_async16(dst + to + i * STEP * 128, from + i * STEP * st, in);
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const bool live = in && row + i * STEP < rows;
+                cp_async16(dst + to + i * STEP * 128, live ? from + i * STEP * st : base, live);
+            }
+        }
+        if (in) from += C * st;
+    }
+};
 // Whether a piece that this thread has copied holds an infinity or NaN.
 template <int COLS>
 __device__ __forceinline__ bool check_rows(const char* src) {
@@ -227,7 +271,7 @@ __device__ __forceinline__ bool check_rows(const char* src) {
 #pragma unroll
     for (int n0 = 0; n0 < C * PIECES; n0 += kThreads) {
         const int n = n0 + threadIdx.x;
-        const uint4 u = *reinterpret_cast<const uint4*>(src + at<COLS>(n / PIECES, n % PIECES));
+        const uint4 u = *reinterpret_cast<const uint4*>(src + at(n / PIECES, n % PIECES));
         const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
         for (int e = 0; e < 4; ++e) chk = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&w[e]), zero, chk);
@@ -257,7 +301,7 @@ __device__ __forceinline__ TokenPair load_decays(const AttnParams& p, const floa
 }
 // One warp: the chunk's running sums from its 64 log decays.  True where one of them is no
 // number or so far above 0 that a product of 64 leaves fp32's range.
-__device__ __forceinline__ bool make_decays(const TokenPair& tp, Decays& g) {
+__device__ __forceinline__ bool make_decays(const TokenPair& tp, float scale, Decays& g) {
     const int lane = threadIdx.x & 31;
     const double x0 = static_cast<double>(tp.ld[0]) * 1.4426950408889634074, x1 = static_cast<double>(tp.ld[1]) * 1.4426950408889634074;
     double incl = x0 + x1;
@@ -274,7 +318,7 @@ __device__ __forceinline__ bool make_decays(const TokenPair& tp, Decays& g) {
     int s[2];
     s[0] = __popc(m0 & lt) + __popc(m1 & lt) + (tp.reset[0] ? 1 : 0);
     s[1] = s[0] + (tp.reset[1] ? 1 : 0);
-    const double end = __shfl_sync(0xffffffffu, incl, 31);
+    const double end = __shfl_sync(0xffffffffu, incl, 31), block_end = __shfl_sync(0xffffffffu, incl, lane | 7);
     const int send = __popc(m0) + __popc(m1);
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
@@ -283,7 +327,8 @@ __device__ __forceinline__ bool make_decays(const TokenPair& tp, Decays& g) {
         g.hi[i] = hi, g.lo[i] = static_cast<float>(G[e] - hi);
         g.seg[i] = s[e];
         g.w[i] = s[e] == send ? ex2(static_cast<float>(end - G[e])) : 0.0f;
-        g.eg[i] = s[e] == 0 ? ex2(hi) : 0.0f;
+        g.eg[i] = s[e] == 0 ? scale * ex2(hi) : 0.0f;
+        g.end[i] = ex2(static_cast<float>(block_end - G[e]));
     }
     if (lane == 0) g.d = send == 0 ? ex2(static_cast<float>(end)) : -1.0f;
     return __any_sync(0xffffffffu, !(tp.ld[0] <= 1.0f && tp.ld[1] <= 1.0f));
@@ -293,10 +338,12 @@ __device__ __forceinline__ float times_state(float d, float s) { return d == -1.
 // ------------------------------------------------------------------ the kernel
 // STATE: only the state of a segment of the sequence, from zero, and its decay.
 template <typename T, int DK, bool VEC, bool STATE>
-__global__ void __launch_bounds__(kThreads) attention_kernel(const AttnParams p) {
+__global__ void __launch_bounds__(kThreads, DK == 64 && Split<T>::IN < 3 ? 3 : 2) attention_kernel(const AttnParams p) {
     using S = Split<T>;
     using L = Layout<T, DK, VEC>;
     constexpr int NI = DK / 8;  // 8-feature tiles of the state
+    constexpr int MQ = S::IN == 1 ? 4 : 2;  // row blocks whose products with the state run side by side
+    constexpr bool FRESH = S::IN == 3;      // fp32: partial sums apart, as for the state
     extern __shared__ __align__(128) char smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c2 = (lane & 3) * 2;
     int64_t id = blockIdx.x;
@@ -333,18 +380,22 @@ __global__ void __launch_bounds__(kThreads) attention_kernel(const AttnParams p)
     }
     float total = 1.0f;  // STATE: the segment's decay
 
-    auto issue = [&](int64_t c) {  // the asynchronous copies of a chunk
+    using B16 = __nv_bfloat16;
+    const B16 *qc = reinterpret_cast<const B16*>(q), *kc = reinterpret_cast<const B16*>(k), *vc = reinterpret_cast<const B16*>(v);
+    Copier<DK> copy_q(qc, p.q.st, c0 * C, 0, p.dk), copy_k(kc, p.k.st, c0 * C, 0, p.dk);
+    Copier<DV> copy_v(vc, p.v.st, c0 * C, col0, p.dv);
+    auto issue = [&](int64_t c) {  // the asynchronous copies of a chunk, in turn
         if constexpr (L::STAGES == 2) {
             const uint32_t to = sm + (c & 1) * L::STAGE;
-            if (!STATE) copy_rows<DK>(to + L::Q, q, p.q.st, c * C, p.T, 0, p.dk);
-            copy_rows<DK>(to + L::K, k, p.k.st, c * C, p.T, 0, p.dk);
-            copy_rows<DV>(to + L::V, v, p.v.st, c * C, p.T, col0, p.dv);
+            if (!STATE) copy_q.copy(to + L::Q, qc, p.T - c * C);
+            copy_k.copy(to + L::K, kc, p.T - c * C);
+            copy_v.copy(to + L::V, vc, p.T - c * C);
             cp_commit();
         }
     };
     issue(c0);
     bool wild = false;  // warp 0: of the next chunk's decays
-    if (warp == 0) wild = make_decays(load_decays(p, ld, marks, c0 * C), gates[c0 & 1]);
+    if (warp == 0) wild = make_decays(load_decays(p, ld, marks, c0 * C), p.scale, gates[c0 & 1]);
 
     for (int64_t c = c0; c < c1; ++c) {
         const int64_t t0 = c * C;
@@ -406,58 +457,69 @@ __global__ void __launch_bounds__(kThreads) attention_kernel(const AttnParams p)
                     if (c2 == 2 && j + 8 < p.dv) out[t * p.ot + j + 8] = static_cast<T>(p.scale * o1);
                 }
             }
-            if (warp == 0 && c + 1 < c1) wild = make_decays(next, gates[(c + 1) & 1]);
+            if (warp == 0 && c + 1 < c1) wild = make_decays(next, p.scale, gates[(c + 1) & 1]);
             continue;
         }
 
         // rows and pieces of this lane's ldmatrix addresses: 16 rows x 16 columns a load
-        const int lr = lane & 15, lp = lane >> 4;               // [m][k] tiles, and [k][n] ones transposed
-        const int br = (lane & 7) + ((lane >> 4) << 3), bp = (lane >> 3) & 1;  // [n][k] tiles
+        const int lr = lane & 15, lp = lane >> 4;                              // [m][k] tiles, and [k][n] ones transposed
+        const int br = (lane & 7) + ((lane >> 4) << 3), bp = (lane >> 3) & 1;  // [n][k] tiles, and [k][m] ones transposed
+        const bool resets = gt.d == -1.0f;
         float o[4][2][4] = {};
         if constexpr (!STATE) {
-            // scores of row block `warp`, a block of 16 tokens before or at it each
-            uint32_t qa[S::IN][DK / 16][4];
+            // the scores on and below the diagonal, in blocks of 16 x 16: each warp the one on
+            // the diagonal and one or two others
+            for (int i = 0; i < (warp == 1 || warp == 2 ? 3 : 2); ++i) {
+                const int rb = i == 0 || warp == 2 || (warp == 1 && i == 1) ? warp : 3;
+                const int cb = i == 0 ? warp : warp == 3 ? 2 : warp == 0 ? 0 : i == 1 ? 0 : 1;
+                float acc[2][2][4] = {};  // [steps taken in turn][8 tokens]
 #pragma unroll
-            for (int a = 0; a < S::IN; ++a)
+                for (int ks = 0; ks < DK / 16; ++ks) {
+                    uint32_t qa[S::IN][4], kb[S::IN][4];
 #pragma unroll
-                for (int ks = 0; ks < DK / 16; ++ks)
-                    ldsm4(qa[a][ks], sbuf + L::Q + a * C * DK * 2 + at<DK>(16 * warp + lr, 2 * ks + lp));
-            const int r0 = 16 * warp + g;
-            const float h0 = gt.hi[r0], l0 = gt.lo[r0], h1 = gt.hi[r0 + 8], l1 = gt.lo[r0 + 8];
-            const int s0 = gt.seg[r0], s1 = gt.seg[r0 + 8];
-            for (int nb = 0; nb <= warp; ++nb) {
-                float acc[2][4] = {};
-#pragma unroll
-                for (int ks = 0; ks < DK / 16; ++ks)
-#pragma unroll
-                    for (int b2 = 0; b2 < S::QK; ++b2) {
-                        uint32_t kb[4];
-                        ldsm4(kb, sbuf + L::K + b2 * C * DK * 2 + at<DK>(16 * nb + br, 2 * ks + bp));
-#pragma unroll
-                        for (int a = 0; a + b2 < S::QK; ++a) {
-                            mma(acc[0], qa[a][ks], kb[0], kb[1]);
-                            mma(acc[1], qa[a][ks], kb[2], kb[3]);
-                        }
+                    for (int a = 0; a < S::IN; ++a) {
+                        ldsm4(qa[a], sbuf + L::Q + a * C * DK * 2 + at(16 * rb + lr, 2 * ks + lp));
+                        ldsm4(kb[a], sbuf + L::K + a * C * DK * 2 + at(16 * cb + br, 2 * ks + bp));
                     }
+                    products<S::QK, S::IN, S::IN>([&](int a, int b2) {
+                        mma(acc[ks & 1][0], qa[a], kb[b2][0], kb[b2][1]);
+                        mma(acc[ks & 1][1], qa[a], kb[b2][2], kb[b2][3]);
+                    });
+                }
+                const int r0 = 16 * rb + g;
+                const float h0 = gt.hi[r0], l0 = gt.lo[r0], h1 = gt.hi[r0 + 8], l1 = gt.lo[r0 + 8];
+                const bool pairwise = rb == cb || resets;
+                float f0 = 0.0f, f1 = 0.0f;  // of a block below the diagonal: from its columns' end on
+                if (!pairwise) {
+                    const float he = gt.hi[16 * cb + 15], le = gt.lo[16 * cb + 15];
+                    f0 = p.scale * ex2((h0 - he) + (l0 - le)), f1 = p.scale * ex2((h1 - he) + (l1 - le));
+                }
 #pragma unroll
                 for (int n = 0; n < 2; ++n) {
-                    const int col = 16 * nb + 8 * n + c2;
-                    float f[4];
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const float hs = gt.hi[col + e], ls = gt.lo[col + e];
-                        const int ss = gt.seg[col + e];
-                        f[e] = ss == s0 && col + e <= r0 ? ex2((h0 - hs) + (l0 - ls)) * acc[n][e] : 0.0f;
-                        f[2 + e] = ss == s1 && col + e <= r0 + 8 ? ex2((h1 - hs) + (l1 - ls)) * acc[n][2 + e] : 0.0f;
+                    const int col = 16 * cb + 8 * n + c2;
+                    float2 x0 = make_float2(acc[0][n][0] + acc[1][n][0], acc[0][n][1] + acc[1][n][1]);
+                    float2 x1 = make_float2(acc[0][n][2] + acc[1][n][2], acc[0][n][3] + acc[1][n][3]);
+                    if (!pairwise) {
+                        const float2 end = *reinterpret_cast<const float2*>(&gt.end[col]);
+                        x0 = __fmul2_rn(x0, __fmul2_rn(end, splat(f0)));
+                        x1 = __fmul2_rn(x1, __fmul2_rn(end, splat(f1)));
+                    } else {
+                        const int s0 = gt.seg[r0], s1 = gt.seg[r0 + 8];
+                        const float2 hs = *reinterpret_cast<const float2*>(&gt.hi[col]), ls = *reinterpret_cast<const float2*>(&gt.lo[col]);
+                        const int2 ss = *reinterpret_cast<const int2*>(&gt.seg[col]);
+                        x0.x = ss.x == s0 && col <= r0 ? x0.x * (p.scale * ex2((h0 - hs.x) + (l0 - ls.x))) : 0.0f;
+                        x0.y = ss.y == s0 && col + 1 <= r0 ? x0.y * (p.scale * ex2((h0 - hs.y) + (l0 - ls.y))) : 0.0f;
+                        x1.x = ss.x == s1 && col <= r0 + 8 ? x1.x * (p.scale * ex2((h1 - hs.x) + (l1 - ls.x))) : 0.0f;
+                        x1.y = ss.y == s1 && col + 1 <= r0 + 8 ? x1.y * (p.scale * ex2((h1 - hs.y) + (l1 - ls.y))) : 0.0f;
                     }
                     uint32_t p0[S::SCORE], p1[S::SCORE];
-                    split<S::SCORE>(f[0], f[1], p0);
-                    split<S::SCORE>(f[2], f[3], p1);
+                    split<S::SCORE>(x0, p0);
+                    split<S::SCORE>(x1, p1);
 #pragma unroll
                     for (int a = 0; a < S::SCORE; ++a) {
                         char* const to = smem + L::P + a * C * C * 2 + c2 * 2;
-                        *reinterpret_cast<uint32_t*>(to + at<C>(r0, 2 * nb + n)) = p0[a];
-                        *reinterpret_cast<uint32_t*>(to + at<C>(r0 + 8, 2 * nb + n)) = p1[a];
+                        *reinterpret_cast<uint32_t*>(to + at(r0, 2 * cb + n)) = p0[a];
+                        *reinterpret_cast<uint32_t*>(to + at(r0 + 8, 2 * cb + n)) = p1[a];
                     }
                 }
             }
@@ -467,20 +529,30 @@ __global__ void __launch_bounds__(kThreads) attention_kernel(const AttnParams p)
                 uint32_t sb0[2][S::SCORE], sb1[2][S::SCORE];  // [column tile][plane], features 0-7 and 8-15 of the step
 #pragma unroll
                 for (int n = 0; n < 2; ++n) {
-                    split<S::SCORE>(s[2 * ks][2 * n], s[2 * ks][2 * n + 1], sb0[n]);
-                    split<S::SCORE>(s[2 * ks + 1][2 * n], s[2 * ks + 1][2 * n + 1], sb1[n]);
+                    split<S::SCORE>(make_float2(s[2 * ks][2 * n], s[2 * ks][2 * n + 1]), sb0[n]);
+                    split<S::SCORE>(make_float2(s[2 * ks + 1][2 * n], s[2 * ks + 1][2 * n + 1]), sb1[n]);
                 }
 #pragma unroll
-                for (int m = 0; m < 4; ++m)
+                for (int m0 = 0; m0 < 4; m0 += MQ) {
+                    uint32_t qf[MQ][S::IN][4];
 #pragma unroll
-                    for (int a = 0; a < S::IN; ++a) {
-                        uint32_t qf[4];
-                        ldsm4(qf, sbuf + L::Q + a * C * DK * 2 + at<DK>(16 * m + lr, 2 * ks + lp));
+                    for (int m = 0; m < MQ; ++m)
 #pragma unroll
-                        for (int b2 = 0; b2 < S::SCORE && a + b2 < S::OUT; ++b2)
+                        for (int a = 0; a < S::IN; ++a)
+                            ldsm4(qf[m][a], sbuf + L::Q + a * C * DK * 2 + at(16 * (m0 + m) + lr, 2 * ks + lp));
+                    float t[MQ][2][4] = {};
+                    products<S::OUT, S::IN, S::SCORE>([&](int a, int b2) {
 #pragma unroll
-                            for (int n = 0; n < 2; ++n) mma(o[m][n], qf, sb0[n][b2], sb1[n][b2]);
-                    }
+                        for (int m = 0; m < MQ; ++m)
+#pragma unroll
+                            for (int n = 0; n < 2; ++n) mma(FRESH ? t[m][n] : o[m0 + m][n], qf[m][a], sb0[n][b2], sb1[n][b2]);
+                    });
+                    if (FRESH)
+#pragma unroll
+                        for (int m = 0; m < MQ; ++m)
+#pragma unroll
+                            for (int n = 0; n < 2; ++n) add4(o[m0 + m][n], t[m][n]);
+                }
             }
 #pragma unroll
             for (int m = 0; m < 4; ++m)
@@ -488,79 +560,96 @@ __global__ void __launch_bounds__(kThreads) attention_kernel(const AttnParams p)
                 for (int r = 0; r < 2; ++r) {
                     const int row = 16 * m + g + 8 * r;
                     const float eg = gt.eg[row];
-                    const bool reach = gt.seg[row] == 0;
+                    const bool reach = !resets || gt.seg[row] == 0;
 #pragma unroll
                     for (int n = 0; n < 2; ++n)
 #pragma unroll
                         for (int e = 0; e < 2; ++e) o[m][n][2 * r + e] = reach ? eg * o[m][n][2 * r + e] : 0.0f;
                 }
         }
-        if (warp == 0 && c + 1 < c1) wild = make_decays(next, gates[(c + 1) & 1]);
+        if (warp == 0 && c + 1 < c1) wild = make_decays(next, p.scale, gates[(c + 1) & 1]);
         if constexpr (!STATE) __syncthreads();  // the scores are there
 
         // the scores times v, and the state
+        if (resets) {
 #pragma unroll
-        for (int n = 0; n < NI; ++n)
+            for (int n = 0; n < NI; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
+        } else {
+            const float2 d = splat(gt.d);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s[n][e] = times_state(gt.d, s[n][e]);
+            for (int n = 0; n < NI; ++n) {
+                const float2 x = __fmul2_rn(make_float2(s[n][0], s[n][1]), d), y = __fmul2_rn(make_float2(s[n][2], s[n][3]), d);
+                s[n][0] = x.x, s[n][1] = x.y, s[n][2] = y.x, s[n][3] = y.y;
+            }
+        }
 #pragma unroll
         for (int kb = 0; kb < 4; ++kb) {  // blocks of 16 tokens
             uint32_t vf[S::IN][4];  // (tokens 0-7, columns 0-7), (0-7, 8-15), (8-15, 0-7), (8-15, 8-15)
-            const int vr = 16 * kb + (lane & 7) + ((lane >> 4) << 3), vp = (lane >> 3) & 1;
 #pragma unroll
-            for (int a = 0; a < S::IN; ++a) ldsm4_t(vf[a], sbuf + L::V + a * C * DV * 2 + at<DV>(vr, 2 * warp + vp));
+            for (int a = 0; a < S::IN; ++a) ldsm4_t(vf[a], sbuf + L::V + a * C * DV * 2 + at(16 * kb + br, 2 * warp + bp));
             if constexpr (!STATE) {
+                float t[4][2][4] = {};
+                products<S::OUT, S::SCORE, S::IN>([&](int a, int b2) {
 #pragma unroll
-                for (int m = kb; m < 4; ++m)
-#pragma unroll
-                    for (int a = 0; a < S::SCORE; ++a) {
+                    for (int m = kb; m < 4; ++m) {
                         uint32_t pf[4];
-                        ldsm4(pf, sm + L::P + a * C * C * 2 + at<C>(16 * m + lr, 2 * kb + lp));
-#pragma unroll
-                        for (int b2 = 0; b2 < S::IN && a + b2 < S::OUT; ++b2) {
-                            mma(o[m][0], pf, vf[b2][0], vf[b2][2]);
-                            mma(o[m][1], pf, vf[b2][1], vf[b2][3]);
-                        }
+                        ldsm4(pf, sm + L::P + a * C * C * 2 + at(16 * m + lr, 2 * kb + lp));
+                        mma(FRESH ? t[m][0] : o[m][0], pf, vf[b2][0], vf[b2][2]);
+                        mma(FRESH ? t[m][1] : o[m][1], pf, vf[b2][1], vf[b2][3]);
                     }
+                });
+                if (FRESH)
+#pragma unroll
+                    for (int m = kb; m < 4; ++m) add4(o[m][0], t[m][0]), add4(o[m][1], t[m][1]);
             }
             uint32_t vw[kStatePlanes][4];
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const float2 w = *reinterpret_cast<const float2*>(&gt.w[16 * kb + (r >> 1) * 8 + c2]);
-                float x = 0.0f, y = 0.0f;
+                float2 x = unpack_bf16(vf[S::IN - 1][r]);
 #pragma unroll
-                for (int a = S::IN - 1; a >= 0; --a)  // the planes' sum is the input itself
-                    x += __uint_as_float(vf[a][r] << 16), y += __uint_as_float(vf[a][r] & 0xffff0000u);
+                for (int a = S::IN - 2; a >= 0; --a) x = __fadd2_rn(x, unpack_bf16(vf[a][r]));  // the input itself
                 uint32_t pl[kStatePlanes];
-                split<kStatePlanes>(w.x * x, w.y * y, pl);
+                split<kStatePlanes>(__fmul2_rn(w, x), pl);
 #pragma unroll
                 for (int a = 0; a < kStatePlanes; ++a) vw[a][r] = pl[a];
             }
+            // 16 tokens' part of the state is summed apart and added by rounding: the tensor
+            // cores' own additions cut, and a long sum of one sign would drift
 #pragma unroll
-            for (int n = 0; n < NI / 2; ++n)  // 16 features each
+            for (int n0 = 0; n0 < NI; n0 += 4) {  // 32 features each
+                uint32_t kf[2][S::IN][4];
 #pragma unroll
-                for (int b2 = 0; b2 < S::IN; ++b2) {
-                    uint32_t kf[4];
-                    ldsm4_t(kf, sbuf + L::K + b2 * C * DK * 2 + at<DK>(16 * kb + lr, 2 * n + lp));
+                for (int n = 0; n < 2; ++n)
 #pragma unroll
-                    for (int a = 0; a < kStatePlanes && a + b2 < kStatePlanes; ++a) {
-                        mma(s[2 * n], vw[a], kf[0], kf[1]);
-                        mma(s[2 * n + 1], vw[a], kf[2], kf[3]);
+                    for (int b2 = 0; b2 < S::IN; ++b2)
+                        ldsm4_t(kf[n][b2], sbuf + L::K + b2 * C * DK * 2 + at(16 * kb + lr, n0 + 2 * n + lp));
+                float t[4][4] = {};
+                products<kStatePlanes, kStatePlanes, S::IN>([&](int a, int b2) {
+#pragma unroll
+                    for (int n = 0; n < 2; ++n) {
+                        mma(t[2 * n], vw[a], kf[n][b2][0], kf[n][b2][1]);
+                        mma(t[2 * n + 1], vw[a], kf[n][b2][2], kf[n][b2][3]);
                     }
-                }
+                });
+#pragma unroll
+                for (int n = 0; n < 4; ++n) add4(s[n0 + n], t[n]);
+            }
         }
         if constexpr (!STATE) {
+            const int64_t rows = p.T - t0;
+            T* const row0 = out + t0 * p.ot + jw + c2;
 #pragma unroll
             for (int m = 0; m < 4; ++m)
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
-                    const int64_t t = t0 + 16 * m + g + 8 * r;
-                    if (t < p.T)
+                    const int row = 16 * m + g + 8 * r;
+                    if (row < rows)
 #pragma unroll
                         for (int n = 0; n < 2; ++n) {
                             const int j = jw + 8 * n + c2;
-                            const float x = p.scale * o[m][n][2 * r], y = p.scale * o[m][n][2 * r + 1];
-                            T* const to = out + t * p.ot + j;
+                            const float x = o[m][n][2 * r], y = o[m][n][2 * r + 1];
+                            T* const to = row0 + row * p.ot + 8 * n;
                             if (VEC) {  // whole pairs, aligned
                                 if (j < p.dv) {
                                     if constexpr (sizeof(T) == 4) *reinterpret_cast<float2*>(to) = make_float2(x, y);
@@ -618,13 +707,13 @@ struct Plan {
     int64_t chains, chunks;
     int32_t slices, nseg, seg_chunks;
 };
-// Chains below one for each place of the GPU (3 CTAs a multiprocessor) are cut into segments
-// of at least 4 chunks.
-Plan plan(int64_t nb, int64_t T, int64_t H, int64_t dv) {
+// Where there are few chains they are cut into segments of at least 4 chunks, as many as the
+// GPU holds at once (2 or 3 CTAs a multiprocessor).
+Plan plan(int64_t nb, int64_t T, int64_t H, int64_t dk, int64_t dv) {
     Plan pl{};
     pl.chains = nb * H, pl.chunks = (T + C - 1) / C, pl.slices = int32_t((dv + DV - 1) / DV);
-    const int64_t ctas = pl.chains * pl.slices;
-    int64_t nseg = ctas >= 222 ? 1 : (444 + ctas - 1) / std::max<int64_t>(ctas, 1);
+    const int64_t ctas = pl.chains * pl.slices, places = dk <= 64 ? 444 : 296;
+    int64_t nseg = ctas >= 222 ? 1 : places / std::max<int64_t>(ctas, 1);
     nseg = std::max<int64_t>(1, std::min(nseg, pl.chunks / 4));
     pl.seg_chunks = int32_t((pl.chunks + nseg - 1) / nseg);
     pl.nseg = int32_t((pl.chunks + pl.seg_chunks - 1) / pl.seg_chunks);
@@ -663,7 +752,7 @@ extern "C" {
 
 size_t need_linear_attention_workspace_size(int64_t nb, int64_t T, int64_t H, int64_t dk, int64_t dv) {
     if (nb < 1 || T < 1 || H < 1 || dk < 1 || dv < 1) return 16;
-    const Plan pl = plan(nb, T, H, dv);
+    const Plan pl = plan(nb, T, H, dk, dv);
     return 16 + size_t(pl.chains) * size_t(pl.nseg - 1) * (size_t(dk) * size_t(dv) + 1) * 4;
 }
 
@@ -683,7 +772,7 @@ int need_linear_attention(const need_linear_attention_args* a, need_stream_t str
     }
     if (a->log_decay == nullptr || a->out == nullptr) return fail(NEED_ERR_INVALID, "linear attention: log_decay and out are required");
     if (a->T > 1 && a->out_stride_t < a->dv) return fail(NEED_ERR_INVALID, "linear attention: the output's rows overlap");
-    const Plan pl = plan(a->nb, a->T, a->H, a->dv);
+    const Plan pl = plan(a->nb, a->T, a->H, a->dk, a->dv);
     if (pl.chains > (int64_t(1) << 30) / pl.slices / pl.nseg)
         return fail(NEED_ERR_UNSUPPORTED, "linear attention: too many sequences and heads");
     if (pl.nseg > 1 && (a->workspace == nullptr || (reinterpret_cast<uintptr_t>(a->workspace) & 3u) != 0 ||
