@@ -623,8 +623,9 @@ NEED_API int need_rms_norm_train_backward(const need_norm_train_args* args, need
 /* ------------------------------------------------------------------------ */
 
 /* Workspace bytes of need_linear_attention: the states between the parts that a
- * prompt is cut into where there are few sequences and heads. */
-NEED_API size_t need_linear_attention_workspace_size(int64_t nb, int64_t T, int64_t H, int64_t dk, int64_t dv);
+ * prompt is cut into where there are few sequences and heads, and a word for each
+ * block that has to be run again (see linear_attention_umma.cu). */
+NEED_API size_t need_linear_attention_workspace_size(int32_t dtype, int64_t nb, int64_t T, int64_t H, int64_t dk, int64_t dv);
 
 /* Linear attention with a decay for each head (the matrix-state form of the
  * retention scan: need_core.py:1590-1592 keeps k v by element where this keeps
@@ -634,6 +635,12 @@ NEED_API size_t need_linear_attention_workspace_size(int64_t nb, int64_t T, int6
  * decay is -infinity, the state before it is dropped, whatever it holds.  At most
  * NEED_LINEAR_ATTENTION_MAX_DK features a head. */
 NEED_API int need_linear_attention(const need_linear_attention_args* args, need_stream_t stream);
+
+/* Test hook, no counterpart in the reference: the waits inside need_linear_attention's
+ * tensor-core kernel launched afterwards in this process give up after `polls` polls
+ * (0 restores the default, 2^18).  A block that gave up is run again by another kernel,
+ * so results stay right. */
+NEED_API void need_test_linear_attention_polls(uint32_t polls);
 
 /* The same for one token of each of n sequences, whose states in a pool are
  * updated in place.  A negative slot: no sequence (out 0, nothing updated).  A

@@ -235,8 +235,9 @@ SIGNATURES = {
     "need_rms_norm_train_workspace_size": (c_size_t, [c_int64, c_int64]),
     "need_rms_norm_train_forward": (c_int32, [POINTER(NeedNormTrainArgs), c_void_p]),
     "need_rms_norm_train_backward": (c_int32, [POINTER(NeedNormTrainArgs), c_void_p]),
-    "need_linear_attention_workspace_size": (c_size_t, [c_int64, c_int64, c_int64, c_int64, c_int64]),
+    "need_linear_attention_workspace_size": (c_size_t, [c_int32, c_int64, c_int64, c_int64, c_int64, c_int64]),
     "need_linear_attention": (c_int32, [POINTER(NeedLinearAttentionArgs), c_void_p]),
+    "need_test_linear_attention_polls": (None, [c_uint32]),
     "need_linear_attention_step": (c_int32, [POINTER(NeedLinearAttentionStepArgs), c_void_p]),
     "need_residual_rms_norm": (c_int32, [POINTER(NeedResidualNormArgs), c_void_p]),
     "need_token_log_probs_workspace_size": (c_size_t, [c_int32, c_int64, c_int64, c_int32]),

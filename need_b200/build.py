@@ -29,9 +29,10 @@ EXT_SOURCE = "train_autograd.cpp"
 EXTS = {EXT: EXT_SOURCE, os.path.join(LIBDIR, "_lm.so"): "lm_autograd.cpp"}
 EXT_HEADERS = ["torch_common.h"]
 SOURCES = ["need_scan.cu", "decode.cu", "sp.cu", "noalloc.cu", "segments.cu", "prologue.cu", "epilogue.cu", "assoc.cu",
-           "train_scan.cu", "train_conv.cu", "train_norm.cu", "linear_attention.cu", "linear_attention_step.cu",
+           "train_scan.cu", "train_conv.cu", "train_norm.cu", "linear_attention.cu", "linear_attention_umma.cu",
+           "linear_attention_step.cu",
            "residual_norm.cu", "token_log_probs.cu"]
-HEADERS = ["ptx.cuh", "scan_kernel.cuh", "host_common.h", "umma.cuh", "train_common.cuh"]
+HEADERS = ["ptx.cuh", "scan_kernel.cuh", "host_common.h", "umma.cuh", "train_common.cuh", "linear_attention.cuh"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 

@@ -38,10 +38,12 @@
 #include <type_traits>
 
 #include "host_common.h"
+#include "linear_attention.cuh"
 #include "need_scan.h"
 #include "ptx.cuh"
 
 using namespace need;
+using namespace need::attention;
 
 namespace {
 
@@ -50,62 +52,10 @@ constexpr int kWarps = 4;   // of 16 columns of v each
 constexpr int DV = 16 * kWarps;
 constexpr int kThreads = 32 * kWarps;
 
-struct Stream {
-    const void* p;
-    int64_t sb, st, sh;  // element strides of sequence, token, head
-    int32_t share;       // heads that share one of this tensor's
-};
-
-struct AttnParams {
-    Stream q, k, v;
-    const float* ld;
-    int64_t lb, lt, lh;
-    const uint8_t* seg;
-    int64_t gb, gt;
-    const float* s0;
-    float* sT;
-    void* out;
-    int64_t ob, ot, oh;
-    int64_t T;
-    int32_t H, dk, dv, slices, nseg;
-    int32_t seg_chunks;   // chunks of a segment of the sequence
-    float scale;
-    float* part;          // [chain, nseg - 1, dk, dv]: segments' own states, then those that enter the next
-    float* part_d;        // [chain, nseg - 1]: their decays, below 0 where a reset lies in between
-};
-
 // ------------------------------------------------------------------ pieces
 __device__ __forceinline__ float to_float(float x) { return x; }
 __device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
 __device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
-
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
-__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
-    uint32_t r;
-    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-    return r;
-}
-__device__ __forceinline__ float2 unpack_bf16(uint32_t u) {
-    return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
-}
-__device__ __forceinline__ float2 splat(float x) { return make_float2(x, x); }
-// The two of x as the sums of N bf16 values each.
-template <int N>
-__device__ __forceinline__ void split(float2 x, uint32_t (&pl)[N]) {
-#pragma unroll
-    for (int n = 0; n < N; ++n) {
-        pl[n] = pack_bf16(x.x, x.y);
-        if (n + 1 < N) {
-            const float2 f = unpack_bf16(pl[n]);
-            x = __fadd2_rn(x, make_float2(-f.x, -f.y));
-        }
-    }
-}
 
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
@@ -333,8 +283,6 @@ __device__ __forceinline__ bool make_decays(const TokenPair& tp, float scale, De
     if (lane == 0) g.d = send == 0 ? ex2(static_cast<float>(end)) : -1.0f;
     return __any_sync(0xffffffffu, !(tp.ld[0] <= 1.0f && tp.ld[1] <= 1.0f));
 }
-__device__ __forceinline__ float times_state(float d, float s) { return d == -1.0f ? 0.0f : d * s; }
-
 // ------------------------------------------------------------------ the kernel
 // STATE: only the state of a segment of the sequence, from zero, and its decay.
 template <typename T, int DK, bool VEC, bool STATE>
@@ -345,6 +293,7 @@ __global__ void __launch_bounds__(kThreads, DK == 64 && Split<T>::IN < 3 ? 3 : 2
     constexpr int MQ = S::IN == 1 ? 4 : 2;  // row blocks whose products with the state run side by side
     constexpr bool FRESH = S::IN == 3;      // fp32: partial sums apart, as for the state
     extern __shared__ __align__(128) char smem[];
+    if (p.redo != nullptr && p.redo[blockIdx.x] == 0) return;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c2 = (lane & 3) * 2;
     int64_t id = blockIdx.x;
     const int nseg = STATE ? p.nseg - 1 : p.nseg;
@@ -704,20 +653,26 @@ __global__ void __launch_bounds__(256) enter_kernel(const AttnParams p) {
 
 // ------------------------------------------------------------------ host
 struct Plan {
-    int64_t chains, chunks;
+    bool umma;  // sm_100a's tensor cores take it, in chunks of 128
+    int64_t chains, chunks, blocks;
     int32_t slices, nseg, seg_chunks;
 };
-// Where there are few chains they are cut into segments of at least 4 chunks, as many as the
-// GPU holds at once (2 or 3 CTAs a multiprocessor).
-Plan plan(int64_t nb, int64_t T, int64_t H, int64_t dk, int64_t dv) {
+// Where there are few chains they are cut into segments, as many as the GPU holds at once: one
+// CTA a multiprocessor (umma), 2 or 3 of attention_kernel.
+Plan plan(bool umma, int64_t nb, int64_t T, int64_t H, int64_t dk, int64_t dv) {
     Plan pl{};
+    pl.umma = umma;
     pl.chains = nb * H, pl.chunks = (T + C - 1) / C, pl.slices = int32_t((dv + DV - 1) / DV);
-    const int64_t ctas = pl.chains * pl.slices, places = dk <= 64 ? 444 : 296;
-    int64_t nseg = ctas >= 222 ? 1 : places / std::max<int64_t>(ctas, 1);
-    nseg = std::max<int64_t>(1, std::min(nseg, pl.chunks / 4));
+    const int64_t ctas = std::max<int64_t>(1, pl.chains * pl.slices), places = umma ? 148 : dk <= 64 ? 444 : 296;
+    int64_t nseg = std::max<int64_t>(1, std::min(places / ctas, pl.chunks / 4));
     pl.seg_chunks = int32_t((pl.chunks + nseg - 1) / nseg);
+    if (umma) pl.seg_chunks += pl.seg_chunks & 1;
     pl.nseg = int32_t((pl.chunks + pl.seg_chunks - 1) / pl.seg_chunks);
+    pl.blocks = pl.chains * pl.slices * pl.nseg;
     return pl;
+}
+size_t workspace_of(const Plan& pl, int64_t dk, int64_t dv) {
+    return 16 + size_t(pl.chains) * size_t(pl.nseg - 1) * (size_t(dk) * size_t(dv) + 1) * 4 + (pl.umma ? size_t(pl.blocks) * 4 : 0);
 }
 
 template <typename T, int DK, bool VEC, bool STATE>
@@ -733,27 +688,35 @@ int launch(const AttnParams& p, int64_t blocks, cudaStream_t s) {
 }
 
 template <typename T, int DK, bool VEC>
-int run(const AttnParams& p, const Plan& pl, cudaStream_t s) {
+int run(AttnParams p, const Plan& pl, int64_t nb, uint32_t* redo, cudaStream_t s) {
     const int64_t per = pl.chains * pl.slices;
+    auto all = [&](auto state) {
+        constexpr bool STATE = decltype(state)::value;
+        if (pl.umma) {
+            if (int rc = umma_run(p, nb, STATE, redo, s)) return rc;
+        }
+        return launch<T, DK, VEC, STATE>(p, per * (STATE ? pl.nseg - 1 : pl.nseg), s);  // or what umma has left
+    };
+    p.redo = pl.umma ? redo : nullptr;
     if (pl.nseg > 1) {
-        int rc = launch<T, DK, VEC, true>(p, per * (pl.nseg - 1), s);
-        if (rc != NEED_OK) return rc;
+        if (int rc = all(std::true_type{})) return rc;
         const dim3 grid(static_cast<unsigned>(pl.chains), static_cast<unsigned>((int64_t(p.dk) * p.dv + 255) / 256));
         enter_kernel<<<grid, 256, 0, s>>>(p);
         const cudaError_t e = cudaGetLastError();
         if (e != cudaSuccess) return cuda_fail(e, "linear attention launch");
     }
-    return launch<T, DK, VEC, false>(p, per * pl.nseg, s);
+    return all(std::false_type{});
 }
 
 }  // namespace
 
 extern "C" {
 
-size_t need_linear_attention_workspace_size(int64_t nb, int64_t T, int64_t H, int64_t dk, int64_t dv) {
-    if (nb < 1 || T < 1 || H < 1 || dk < 1 || dv < 1) return 16;
-    const Plan pl = plan(nb, T, H, dk, dv);
-    return 16 + size_t(pl.chains) * size_t(pl.nseg - 1) * (size_t(dk) * size_t(dv) + 1) * 4;
+size_t need_linear_attention_workspace_size(int32_t dtype, int64_t nb, int64_t T, int64_t H, int64_t dk, int64_t dv) {
+    if (!dtype_ok(dtype) || nb < 1 || T < 1 || H < 1 || dk < 1 || dv < 1) return 16;
+    size_t n = workspace_of(plan(false, nb, T, H, dk, dv), dk, dv);
+    if (dtype == NEED_BF16) n = std::max(n, workspace_of(plan(true, nb, T, H, dk, dv), dk, dv));
+    return n;
 }
 
 int need_linear_attention(const need_linear_attention_args* a, need_stream_t stream) {
@@ -772,12 +735,8 @@ int need_linear_attention(const need_linear_attention_args* a, need_stream_t str
     }
     if (a->log_decay == nullptr || a->out == nullptr) return fail(NEED_ERR_INVALID, "linear attention: log_decay and out are required");
     if (a->T > 1 && a->out_stride_t < a->dv) return fail(NEED_ERR_INVALID, "linear attention: the output's rows overlap");
-    const Plan pl = plan(a->nb, a->T, a->H, a->dk, a->dv);
-    if (pl.chains > (int64_t(1) << 30) / pl.slices / pl.nseg)
+    if (a->nb > (int64_t(1) << 30) / a->H / ((a->dv + DV - 1) / DV))
         return fail(NEED_ERR_UNSUPPORTED, "linear attention: too many sequences and heads");
-    if (pl.nseg > 1 && (a->workspace == nullptr || (reinterpret_cast<uintptr_t>(a->workspace) & 3u) != 0 ||
-                        a->workspace_bytes < need_linear_attention_workspace_size(a->nb, a->T, a->H, a->dk, a->dv)))
-        return fail(NEED_ERR_WORKSPACE, "linear attention: workspace missing, misaligned or too small");
     const int es = dtype_bytes(a->dtype), per = 16 / es;
     AttnParams p{};
     Stream* to[3] = {&p.q, &p.k, &p.v};
@@ -795,15 +754,19 @@ int need_linear_attention(const need_linear_attention_args* a, need_stream_t str
     p.s0 = a->state, p.sT = a->final_state;
     p.out = a->out, p.ob = a->out_stride_b, p.ot = a->out_stride_t, p.oh = a->out_stride_h;
     p.T = a->T, p.H = int32_t(a->H), p.dk = int32_t(a->dk), p.dv = int32_t(a->dv);
-    p.slices = pl.slices, p.nseg = pl.nseg, p.seg_chunks = pl.seg_chunks, p.scale = a->scale;
-    if (pl.nseg > 1) {
-        p.part = static_cast<float*>(a->workspace);
-        p.part_d = p.part + pl.chains * (pl.nseg - 1) * a->dk * a->dv;
-    }
+    p.scale = a->scale;
+    const Plan pl = plan(vec && a->dtype == NEED_BF16 && a->T > C && umma_takes(p, a->nb), a->nb, a->T, a->H, a->dk, a->dv);
+    if ((pl.nseg > 1 || pl.umma) && (a->workspace == nullptr || (reinterpret_cast<uintptr_t>(a->workspace) & 3u) != 0 ||
+                                     a->workspace_bytes < workspace_of(pl, a->dk, a->dv)))
+        return fail(NEED_ERR_WORKSPACE, "linear attention: workspace missing, misaligned or too small");
+    p.slices = pl.slices, p.nseg = pl.nseg, p.seg_chunks = pl.seg_chunks;
+    p.part = static_cast<float*>(a->workspace);
+    p.part_d = p.part + pl.chains * (pl.nseg - 1) * a->dk * a->dv;
+    uint32_t* redo = reinterpret_cast<uint32_t*>(p.part_d + pl.chains * (pl.nseg - 1));
     auto go = [&](auto tag) {
         using T = decltype(tag);
-        if (a->dk <= 64) return vec ? run<T, 64, true>(p, pl, stream) : run<T, 64, false>(p, pl, stream);
-        return vec ? run<T, 128, true>(p, pl, stream) : run<T, 128, false>(p, pl, stream);
+        if (a->dk <= 64) return vec ? run<T, 64, true>(p, pl, a->nb, redo, stream) : run<T, 64, false>(p, pl, a->nb, redo, stream);
+        return vec ? run<T, 128, true>(p, pl, a->nb, redo, stream) : run<T, 128, false>(p, pl, a->nb, redo, stream);
     };
     const int rc = a->dtype == NEED_F32 ? go(float{}) : a->dtype == NEED_BF16 ? go(__nv_bfloat16{}) : go(__half{});
     return rc != NEED_OK ? rc : ok();

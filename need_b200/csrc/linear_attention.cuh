@@ -1,0 +1,74 @@
+// linear_attention.cuh -- what the two kernels of linear attention share
+// (linear_attention.cu, linear_attention_umma.cu): their parameters, and values as sums
+// of bf16 ones.
+#pragma once
+
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace need {
+namespace attention {
+
+struct Stream {
+    const void* p;
+    int64_t sb, st, sh;  // element strides of sequence, token, head
+    int32_t share;       // heads that share one of this tensor's
+};
+
+struct AttnParams {
+    Stream q, k, v;
+    const float* ld;
+    int64_t lb, lt, lh;
+    const uint8_t* seg;
+    int64_t gb, gt;
+    const float* s0;
+    float* sT;
+    void* out;
+    int64_t ob, ot, oh;
+    int64_t T;
+    int32_t H, dk, dv, slices, nseg;
+    int32_t seg_chunks;   // chunks of a segment of the sequence
+    float scale;
+    float* part;          // [chain, nseg - 1, dk, dv]: segments' own states, then those that enter the next
+    float* part_d;        // [chain, nseg - 1]: their decays, below 0 where a reset lies in between
+    const uint32_t* redo; // of each block, null for all: whether it has to run
+};
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+__device__ __forceinline__ float2 unpack_bf16(uint32_t u) {
+    return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+}
+__device__ __forceinline__ float2 splat(float x) { return make_float2(x, x); }
+// The two of x as the sums of N bf16 values each.
+template <int N>
+__device__ __forceinline__ void split(float2 x, uint32_t (&pl)[N]) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+        pl[n] = pack_bf16(x.x, x.y);
+        if (n + 1 < N) {
+            const float2 f = unpack_bf16(pl[n]);
+            x = __fadd2_rn(x, make_float2(-f.x, -f.y));
+        }
+    }
+}
+
+__device__ __forceinline__ float times_state(float d, float s) { return d == -1.0f ? 0.0f : d * s; }
+
+// The kernel on the tensor cores of sm_100a (linear_attention_umma.cu): chunks of 128
+// tokens, bf16, up to 128 features.  `redo` [blocks] tells which of attention_kernel's
+// blocks it leaves to that.  state: only the segments' states.
+bool umma_takes(const AttnParams& p, int64_t nb);
+int umma_run(const AttnParams& p, int64_t nb, bool state, uint32_t* redo, cudaStream_t stream);
+
+}  // namespace attention
+}  // namespace need

@@ -75,7 +75,7 @@ std::pair<Tensor, OptTensor> linear_attention(const Tensor& q_, const Tensor& k_
     if (seg.defined()) a.seg_start = ptr<uint8_t>(seg), a.seg_stride_b = seg.stride(0), a.seg_stride_t = seg.stride(1);
     a.state = ptr<float>(state), a.final_state = ptr<float>(final);
     a.out = out.data_ptr(), a.out_stride_b = out.stride(0), a.out_stride_t = out.stride(1), a.out_stride_h = out.stride(2);
-    const size_t bytes = need_linear_attention_workspace_size(B, T, H, dk, dv);
+    const size_t bytes = need_linear_attention_workspace_size(a.dtype, B, T, H, dk, dv);
     Tensor ws;
     if (bytes > 16) ws = scratch(q, bytes), a.workspace = ws.data_ptr(), a.workspace_bytes = bytes;
     check("need_linear_attention", need_linear_attention(&a, on.stream));

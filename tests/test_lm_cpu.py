@@ -64,7 +64,7 @@ def attention_args(**kw):
     ({"nb": 1 << 40}, abi.ERR_UNSUPPORTED), ({"q.ptr": None}, abi.ERR_INVALID), ({"v.ptr": None}, abi.ERR_INVALID),
     ({"k.heads": 3}, abi.ERR_INVALID), ({"k.heads": 0}, abi.ERR_INVALID), ({"v.heads": 8}, abi.ERR_INVALID),
     ({"log_decay": None}, abi.ERR_INVALID), ({"out": None}, abi.ERR_INVALID), ({"out_stride_t": 63}, abi.ERR_INVALID),
-    ({"T": 4096, "workspace": None}, abi.ERR_WORKSPACE), ({"T": 4096, "workspace_bytes": 1000}, abi.ERR_WORKSPACE),
+    ({"workspace": None}, abi.ERR_WORKSPACE), ({"T": 4096, "workspace": None}, abi.ERR_WORKSPACE), ({"T": 4096, "workspace_bytes": 1000}, abi.ERR_WORKSPACE),
 ])
 def test_attention_refuses(lib, change, code):
     assert lib.need_linear_attention(ctypes.byref(attention_args(**change)), None) == code
@@ -166,9 +166,10 @@ def test_null_args(lib):
 
 def test_workspaces(lib):
     size = lib.need_linear_attention_workspace_size
-    assert size(16, 4096, 16, 64, 64) == 16          # chains enough: nothing between parts
-    assert size(1, 64, 1, 64, 64) == 16              # one chunk
-    assert size(1, 16384, 4, 32, 48) > 16 and size(0, 1, 1, 1, 1) == 16
+    assert size(abi.F32, 16, 4096, 32, 64, 64) == 16  # chains enough: nothing between parts
+    assert size(abi.F32, 1, 64, 1, 64, 64) == 16      # one chunk
+    assert size(abi.F32, 1, 16384, 4, 32, 48) > 16 and size(abi.F32, 0, 1, 1, 1, 1) == 16 and size(9, 1, 16384, 4, 32, 48) == 16
+    assert size(abi.BF16, 16, 4096, 16, 64, 64) == 16 + 4 * 256  # a word a block
     size = lib.need_token_log_probs_workspace_size
     assert size(abi.BF16, 1000, 50000, 20) == 16 and size(abi.BF16, 4, 784, 20) == 16
     assert size(abi.F32, 4, 131072, 5) > 16 and size(9, 4, 131072, 5) == 16

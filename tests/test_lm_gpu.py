@@ -38,7 +38,7 @@ def close(got, want, mag, sums, half=0.0):
     assert not bad.any(), f"{int(bad.sum())} of {bad.numel()} off, worst {float((err / lim).nan_to_num(math.inf).max()):.3g} of the bound"
 
 
-def check_attention(q, k, v, ld, scale=1.0, seg=None, state=None):
+def check_attention(q, k, v, ld, scale=1.0, seg=None, state=None, twice=True):
     out, fin = nk.linear_attention(q, k, v, ld, scale=scale, seg_start=seg, state=state, return_final_state=True)
     want, s, mag, m = ref.attention(q, k, v, ld, float(torch.tensor(scale, dtype=F32)), seg, state)
     assert out.dtype == q.dtype and out.shape == want.shape and fin.shape == s.shape
@@ -46,7 +46,7 @@ def check_attention(q, k, v, ld, scale=1.0, seg=None, state=None):
     close(out, want, mag + small / SUMS[q.dtype], SUMS[q.dtype], ref.HALF_STEP[q.dtype])
     close(fin, s, m, STATE)
     alone = nk.linear_attention(q, k, v, ld, scale=scale, seg_start=seg, state=state)
-    assert torch.equal(alone, out)
+    assert torch.equal(alone, out) or not twice
     return out, fin
 
 
@@ -143,7 +143,8 @@ def test_attention_views(cuda, dtype):
         buf = torch.zeros(B, T, H * d + 1, dtype=dtype, device=cuda)
         buf[..., 1:] = t.flatten(2)
         odd.append(buf[..., 1:].unflatten(-1, (H, d)))
-    assert torch.equal(nk.linear_attention(*odd, ld), want)
+    if dtype != BF:  # unaligned bf16 rows go through the kernel of shorter chunks: other sums, within the same bound
+        assert torch.equal(nk.linear_attention(*odd, ld), want)
     check_attention(*odd, ld)
 
 
@@ -204,6 +205,22 @@ def test_attention_long_sums_of_one_sign(cuda):
     want = torch.einsum("bthi,bthj->bhij", k.double(), v.double())
     err = float(((fin.double() - want).abs() / want).max())
     assert err < 2.0 ** -20  # 64 additions, 2^-24 at most and of either sign: 8 of them
+
+
+def test_attention_waits_given_up(cuda):
+    """Blocks of the tensor-core kernel that give a wait up are run again: nothing is lost
+    (which do so depends on their timing, and two kernels' sums differ within the bounds)."""
+    from need_b200 import abi
+    cases = [make(cuda, 2, 500, 3, 64, 64, BF, state=True, resets=90), make(cuda, 1, 3000, 1, 128, 72, BF, decay="head", state=True)]
+    torch.cuda.synchronize()
+    for polls in (1, 3, 0):
+        abi.load().need_test_linear_attention_polls(polls)
+        try:
+            for c in cases:
+                check_attention(*c[:4], 0.125, *c[4:], twice=False)
+            torch.cuda.synchronize()
+        finally:
+            abi.load().need_test_linear_attention_polls(0)
 
 
 def test_attention_empty(cuda):
