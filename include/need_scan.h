@@ -638,7 +638,7 @@ NEED_API int need_linear_attention(const need_linear_attention_args* args, need_
 
 /* Test hook, no counterpart in the reference: the waits inside need_linear_attention's
  * tensor-core kernel launched afterwards in this process give up after `polls` polls
- * (0 restores the default, 2^18).  A block that gave up is run again by another kernel,
+ * (0 restores the default, 2^16).  A block that gave up is run again by another kernel,
  * so results stay right. */
 NEED_API void need_test_linear_attention_polls(uint32_t polls);
 

@@ -57,7 +57,7 @@ __device__ __forceinline__ void split(float2 x, uint32_t (&pl)[N]) {
         pl[n] = pack_bf16(x.x, x.y);
         if (n + 1 < N) {
             const float2 f = unpack_bf16(pl[n]);
-            x = __fadd2_rn(x, make_float2(-f.x, -f.y));
+            x = __ffma2_rn(f, splat(-1.0f), x);
         }
     }
 }

@@ -6,8 +6,8 @@
 // One CTA walks the chunks of one (sequence, head, 64 columns of v).  Per chunk, with
 // fp32 accumulators in tensor memory:
 //
-//   P    = Q K^T                 128 x 128          (two buffers)
-//   O2   = Q S                   128 x 64           S: 2 planes, shared memory
+//   P    = Q K^T                 128 x 128
+//   O2   = Q S                   128 x 64           S: 2 planes, shared memory; two buffers
 //   O1   = P' V                  128 x 64           P' = P with its decays, 2 planes, in P's place
 //   dS^T = (V w)^T K             64 x features      V w: 3 planes, shared memory
 //   out  = O1 + e^G O2,  S' = e^{G_end} S + dS
@@ -16,13 +16,15 @@
 // warps of its own, which meet at mbarriers only, so that a chunk's scores, outputs and
 // state run beside its neighbours':
 //
-//   warps 0-3    P'    a row per thread; below the diagonal's blocks a decay is a row's factor
-//                      times a column's, so that only the blocks on it take an exponential
-//                      per score
-//   warps 4-7    V w, the state and its planes, the check for infinities
-//   warps 8-11   outputs
-//   warp 12      one lane: TMA loads (no multicast) and all MMAs
-//   warp 13      the decays of the chunks ahead
+//   warps 0-7    P' and the outputs: two for each 32 rows, a row per thread; a decay is a row's
+//                factor times a column's, but where one of them would leave fp32's range
+//   warps 8-15   V w, the check for infinities, the state and its planes
+//   warp 16      the decays of the chunks ahead
+//   warps 17-19  the MMAs, each with the loads (TMA, no multicast) whose place they free: P and
+//                O2; dS; O1.  One elected lane issues.
+//
+// All roles' code runs on every part of the multiprocessor, so that it is kept short: straight
+// code of the same work took twice the time, waiting for instructions.
 //
 // Every wait is bounded.  A block that gave one up, or met a value that is not finite (or
 // a log decay that makes a chunk's products leave fp32's range), says so in `redo`:
@@ -31,6 +33,7 @@
 #include <cuda_bf16.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "host_common.h"
 #include "linear_attention.cuh"
@@ -45,11 +48,10 @@ namespace {
 
 constexpr int CT = 128;      // tokens of a chunk
 constexpr int DVS = 64;      // columns of v of a CTA
-constexpr int kThreads = 448;
+constexpr int kThreads = 640;
 constexpr int GR = 4;        // chunks whose decays are held
-constexpr uint32_t kPolls = 1u << 18;  // of a wait before it is given up
-constexpr uint32_t kTmem = 512, T_P = 0, T_O1 = 256, T_O2 = 320, T_DS = 384;  // tensor memory columns
-constexpr int kVPlanes = 3;
+constexpr uint32_t kPolls = 1u << 16;  // of a wait before it is given up
+constexpr uint32_t kTmem = 512, T_O1 = 0, T_O2 = 64, T_DS = 192;  // tensor memory columns
 
 struct alignas(16) Gates {
     float hi[CT], lo[CT], w[CT], eg[CT], end[CT];  // as Decays; end: of its block of 32
@@ -58,11 +60,16 @@ struct alignas(16) Gates {
     int wild;
 };
 
+// VP: planes of V w.  3 where the state itself is a result; where only outputs of bf16 come
+// of it, 2 as of the other operands (16x4096 16x64: see below).
 template <int DK>
 struct Map {  // shared memory, from a 1024-byte aligned base
     static constexpr int NQ = DK == 64 ? 2 : 1, NK = DK == 64 ? 3 : 2, NV = NK;  // chunks loaded ahead
+    static constexpr int NP = DK == 64 ? 2 : 1;                                  // buffers of P
+    static constexpr uint32_t T_P = T_DS + DK;
+    static_assert(T_P + NP * 128 <= kTmem, "tensor memory");
     static constexpr int QB = CT * DK * 2, VB = CT * DVS * 2, SB = DVS * DK * 2;
-    static constexpr int Q = 0, K = Q + NQ * QB, V = K + NK * QB, W = V + NV * VB, S = W + kVPlanes * VB, G = S + 2 * SB;
+    static constexpr int Q = 0, K = Q + NQ * QB, V = K + NK * QB, W = V + NV * VB, S = W + 3 * VB, G = S + 2 * SB;
     static constexpr int BAR = G + GR * static_cast<int>(sizeof(Gates)), BYTES = BAR + 512 + 1024;
 };
 
@@ -73,11 +80,38 @@ struct UmmaParams {
     uint32_t polls;
 };
 
-__device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* tm, int c0, int c1, int c2, int c3, uint64_t* bar) {
+__device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* tm, int c0, int c1, int c2, int c3, uint32_t bar) {
     asm volatile(
         "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
-        " [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst), "l"(tm), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(smem_addr(bar))
+        " [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst), "l"(tm), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(bar)
         : "memory");
+}
+__device__ __forceinline__ void st_shared(uint32_t to, uint32_t v) { asm volatile("st.shared.b32 [%0], %1;" ::"r"(to), "r"(v) : "memory"); }
+__device__ __forceinline__ bool try_wait(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+// Bounded; after one wait was given up (the word at `dead`) nobody waits any more.
+__device__ __noinline__ void wait_on(uint32_t bar, uint32_t parity, uint32_t dead, uint32_t polls) {
+    for (uint32_t i = 1; !try_wait(bar, parity); ++i) {
+        if (i % 64 != 0 && i < polls) continue;
+        uint32_t d;
+        asm volatile("ld.volatile.shared.u32 %0, [%1];" : "=r"(d) : "r"(dead) : "memory");
+        if (d != 0) return;
+        if (i >= polls) asm volatile("st.volatile.shared.u32 [%0], %1;" ::"r"(dead), "r"(1u) : "memory");
+    }
+}
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p != 0;
 }
 // D[tmem] (+)= A[tmem] B[smem]
 __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool accumulate) {
@@ -88,20 +122,38 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint3
         "r"(accumulate ? 1u : 0u)
         : "memory");
 }
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&v)[32]) {
+// 16 words into this thread's lane
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16]) {
     asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-        "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
-        "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
         "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]),
-        "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]),
-        "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]),
-        "r"(v[31])
+        "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
         : "memory");
 }
-// 64 columns of 16 lanes: the four values of 8 columns lie as in a 16 x 8 accumulator of
-// mma.sync (rows lane / 4 and + 8, columns 2 (lane % 4) and + 1).
-__device__ __forceinline__ void tmem_ld16x64(uint32_t taddr, float (&v)[32]) {
+// 16 fp32 columns of this thread's lane
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, float (&v)[16]) {
+    uint32_t r[16];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+          "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr));
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+}
+// 32 or 64 columns of 16 lanes: the four values of 8 columns lie as in a 16 x 8 accumulator
+// of mma.sync (rows lane / 4 and + 8, columns 2 (lane % 4) and + 1).
+__device__ __forceinline__ void tmem_ld_half(uint32_t taddr, float (&v)[16]) {
+    uint32_t r[16];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+          "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr));
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void tmem_ld_half(uint32_t taddr, float (&v)[32]) {
     uint32_t r[32];
     asm volatile(
         "tcgen05.ld.sync.aligned.16x256b.x8.b32 "
@@ -117,95 +169,101 @@ __device__ __forceinline__ void tmem_ld16x64(uint32_t taddr, float (&v)[32]) {
 }
 
 // ------------------------------------------------------------------ decays
-struct Tokens {  // a lane's 4 tokens of a chunk
-    float ld[4];
-    bool reset[4];
+// A sum as two floats: a + b with what rounding left of it.
+struct Sum2 {
+    float hi, lo;
 };
-__device__ __forceinline__ Tokens load_tokens(const AttnParams& p, const float* ld, const uint8_t* seg, int64_t t0) {
-    Tokens r;
+__device__ __forceinline__ Sum2 add(const Sum2& a, const Sum2& b) {
+    const float s = a.hi + b.hi, t = s - a.hi;
+    return {s, ((a.hi - (s - t)) + (b.hi - t)) + (a.lo + b.lo)};
+}
+__device__ __forceinline__ float minus(const Sum2& a, const Sum2& b) { return (a.hi - b.hi) + (a.lo - b.lo); }
+
+// One warp; x, the lane's 4 log decays (tokens 4 lane + e), -infinity where a segment starts.
+// The running sums hold some 44 bits: sums of fp64 took three times the time.
+__device__ __forceinline__ void make_gates(const float (&x)[4], float scale, Gates& g) {
+    const int lane = threadIdx.x & 31;
+    Sum2 G[4], sum{0.0f, 0.0f};
+    int s = 0, send = 0;
+    bool wild = false, reset[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-        const int64_t t = t0 + 4 * (threadIdx.x & 31) + e;
-        const bool live = t < p.T;
-        const float x = live ? ld[t * p.lt] : 0.0f;
-        r.reset[e] = (live && seg != nullptr && seg[t * p.gt] != 0) || x == -INFINITY;
-        r.ld[e] = r.reset[e] ? 0.0f : x < -10000.0f ? -10000.0f : x;  // a NaN stays one
+        reset[e] = x[e] == -INFINITY;
+        wild |= !(x[e] <= 0.5f);  // 128 of them stay below 2^93
+        // a token's state falls below every fp32 value long before e^-10000; a NaN stays one
+        const float v = reset[e] ? 0.0f : x[e] < -10000.0f ? -10000.0f : x[e];
+        constexpr float l2e = 1.4426950408889634f, l2e_lo = 1.9259629911266175e-8f;  // log2(e) as two floats
+        const float y = v * l2e;
+        sum = add(sum, {y, fmaf(v, l2e, -y) + v * l2e_lo});
+        G[e] = sum;
+        const uint32_t m = __ballot_sync(0xffffffffu, reset[e]);
+        s += __popc(m & ((1u << lane) - 1u)), send += __popc(m);
     }
-    return r;
-}
-__device__ __forceinline__ void make_gates(const Tokens& tp, float scale, Gates& g) {
-    const int lane = threadIdx.x & 31;
-    double G[4], sum = 0.0;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) G[e] = sum += static_cast<double>(tp.ld[e]) * 1.4426950408889634074;
-    double incl = sum;
+    Sum2 incl = sum;
 #pragma unroll
     for (int m = 1; m < 32; m <<= 1) {
-        const double o = __shfl_up_sync(0xffffffffu, incl, m);
-        if (lane >= m) incl += o;
+        const Sum2 o{__shfl_up_sync(0xffffffffu, incl.hi, m), __shfl_up_sync(0xffffffffu, incl.lo, m)};
+        if (lane >= m) incl = add(o, incl);
     }
-    double before = __shfl_up_sync(0xffffffffu, incl, 1);
-    if (lane == 0) before = 0.0;
-    const uint32_t lt = (1u << lane) - 1u;
-    int s = 0, send = 0;
+    auto of = [&](int l) { return Sum2{__shfl_sync(0xffffffffu, incl.hi, l), __shfl_sync(0xffffffffu, incl.lo, l)}; };
+    Sum2 before = of((lane + 31) & 31);
+    if (lane == 0) before = {0.0f, 0.0f};
+    const Sum2 end = of(31), block_end = of(lane | 7);
+    float4 hi, lo, w, eg, be;
+    int4 seg;
+    float *ph = &hi.x, *pl = &lo.x, *pw = &w.x, *pe = &eg.x, *pb = &be.x;
+    int* ps = &seg.x;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-        const uint32_t m = __ballot_sync(0xffffffffu, tp.reset[e]);
-        s += __popc(m & lt), send += __popc(m);
+        const Sum2 t = add(before, G[e]);
+        s += reset[e] ? 1 : 0;
+        ph[e] = t.hi, pl[e] = t.lo, ps[e] = s;
+        pw[e] = s == send ? ex2(minus(end, t)) : 0.0f;
+        pe[e] = s == 0 ? scale * ex2(t.hi + t.lo) : 0.0f;
+        pb[e] = ex2(minus(block_end, t));
     }
-    const double end = __shfl_sync(0xffffffffu, incl, 31), block_end = __shfl_sync(0xffffffffu, incl, lane | 7);
-    bool wild = false;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        const int i = 4 * lane + e;
-        const double x = before + G[e];
-        const float hi = static_cast<float>(x);
-        s += tp.reset[e] ? 1 : 0;
-        g.hi[i] = hi, g.lo[i] = static_cast<float>(x - hi);
-        g.seg[i] = s;
-        g.w[i] = s == send ? ex2(static_cast<float>(end - x)) : 0.0f;
-        g.eg[i] = s == 0 ? scale * ex2(hi) : 0.0f;
-        g.end[i] = ex2(static_cast<float>(block_end - x));
-        wild |= !(tp.ld[e] <= 0.5f);  // 128 of them stay below 2^93
-    }
+    reinterpret_cast<float4*>(g.hi)[lane] = hi, reinterpret_cast<float4*>(g.lo)[lane] = lo, reinterpret_cast<float4*>(g.w)[lane] = w;
+    reinterpret_cast<float4*>(g.eg)[lane] = eg, reinterpret_cast<float4*>(g.end)[lane] = be, reinterpret_cast<int4*>(g.seg)[lane] = seg;
     wild = __any_sync(0xffffffffu, wild);
-    if (lane == 0) g.d = send == 0 ? ex2(static_cast<float>(end)) : -1.0f, g.wild = wild ? 1 : 0;
+    if (lane == 0) g.d = send == 0 ? ex2(end.hi + end.lo) : -1.0f, g.wild = wild ? 1 : 0;
 }
 
-// Whether one of 8 bf16 values is an infinity or NaN.
-__device__ __forceinline__ void check8(const uint4& u, __nv_bfloat162& chk) {
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-        chk = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&w[e]), __floats2bfloat162_rn(0.0f, 0.0f), chk);
+// One lane of a warp: a chunk's 128 rows of one tensor, 64 columns at a time.
+__device__ __noinline__ void load_rows(uint32_t full, const CUtensorMap* tm, uint32_t to, int bytes, int col, int head, int t, int b) {
+    if (elect_one()) {
+        asm volatile("mbarrier.arrive.expect_tx.release.cta.shared::cta.b64 _, [%0], %1;" ::"r"(full), "r"(bytes) : "memory");
+#pragma unroll 1
+        for (int j = 0; j < bytes; j += CT * 128) tma_load(to + j, tm, col + j / 256, head, t, b, full);
+    }
+    __syncwarp();
 }
 
 // ------------------------------------------------------------------ the kernel
-template <int DK, bool STATE>
+template <int DK, bool STATE, int VP>
 __global__ void __launch_bounds__(kThreads, 1) umma_attention_kernel(const __grid_constant__ UmmaParams up) {
     using M = Map<DK>;
-    constexpr int NQ = M::NQ, NK = M::NK, NV = M::NV, NI = DK / 8;
+    constexpr int NQ = M::NQ, NK = M::NK, NV = M::NV, NP = M::NP;
     const AttnParams& p = up.a;
     extern __shared__ unsigned char smem_raw[];
     unsigned char* const base = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const uint32_t sb = smem_addr(base);
     uint64_t* bar = reinterpret_cast<uint64_t*>(base + M::BAR);
+    // Those with two by turns are told apart so that none is asked of a phase that another has
+    // followed: a waiter may be a chunk behind.
     uint64_t *full_q = bar, *full_k = full_q + NQ, *full_v = full_k + NK, *gates_full = full_v + NV, *gates_free = gates_full + GR,
-             *s_ready = gates_free + GR, *vw_ready = s_ready + 1, *qk_done = vw_ready + 1 /* 2 */, *ds_done = qk_done + 2,
-             *p_ready = ds_done + 1 /* 2 */, *o_done = p_ready + 2, *o1_free = o_done + 1, *o2_free = o1_free + 1, *drain = o2_free + 1;
-    uint32_t* const tbase = reinterpret_cast<uint32_t*>(drain + 1);
+             *k_free = gates_free + GR, *v_free = k_free + NK, *s_ready = v_free + NV, *vw_ready = s_ready + 1,
+             *qk_done = vw_ready + 1 /* 2 */, *qs_done = qk_done + 2 /* 2 */, *ds_done = qs_done + 2, *ds_free = ds_done + 1,
+             *p_ready = ds_free + 1 /* 2 */, *o_done = p_ready + 2 /* 2 */, *o_free = o_done + 2 /* 2 */, *drain = o_free + 2 /* 3 */;
+    uint32_t* const tbase = reinterpret_cast<uint32_t*>(drain + 3);
     volatile uint32_t* const dead = tbase + 1;
     uint32_t* const bad_word = tbase + 2;
     Gates* const gates = reinterpret_cast<Gates*>(base + M::G);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    int64_t id = blockIdx.x;
-    const int nseg = STATE ? p.nseg - 1 : p.nseg;
-    const int seg = static_cast<int>(id % nseg);
-    id /= nseg;
-    const int slice = static_cast<int>(id % p.slices);
-    const int64_t chain = id / p.slices;
-    const int b = static_cast<int>(chain / p.H), h = static_cast<int>(chain % p.H), col0 = slice * DVS;
+    const uint32_t nseg = STATE ? p.nseg - 1 : p.nseg, rest = blockIdx.x / nseg;
+    const int seg = static_cast<int>(blockIdx.x % nseg), slice = static_cast<int>(rest % p.slices);
+    const int64_t chain = rest / p.slices;
+    const int b = static_cast<int>(static_cast<uint32_t>(chain) / p.H), h = static_cast<int>(static_cast<uint32_t>(chain) % p.H), col0 = slice * DVS;
     const int64_t first = int64_t(seg) * p.seg_chunks * 64;
     const int64_t last = first + int64_t(p.seg_chunks) * 64 < p.T ? first + int64_t(p.seg_chunks) * 64 : p.T;
     const int n = static_cast<int>((last - first + CT - 1) / CT);
@@ -213,15 +271,17 @@ __global__ void __launch_bounds__(kThreads, 1) umma_attention_kernel(const __gri
     const uint8_t* marks = p.seg == nullptr ? nullptr : p.seg + b * p.gb;
 
     if (threadIdx.x == 0) {
-        for (uint64_t* x = full_q; x < gates_full; ++x) mbar_init(x, 1);
-        for (int i = 0; i < GR; ++i) mbar_init(gates_full + i, 1), mbar_init(gates_free + i, STATE ? 4 : 12);
-        mbar_init(s_ready, 4), mbar_init(vw_ready, 4), mbar_init(qk_done, 1), mbar_init(qk_done + 1, 1), mbar_init(ds_done, 1);
-        mbar_init(p_ready, 4), mbar_init(p_ready + 1, 4), mbar_init(o_done, 1), mbar_init(o1_free, 4), mbar_init(o2_free, 4);
-        mbar_init(drain, 1);
+        auto init = [](uint64_t* x, int n, int count) {  // arrivals: of warps, or of MMAs and loads
+#pragma unroll 1
+            for (int i = 0; i < n; ++i) mbar_init(x + i, count);
+        };
+        init(full_q, NQ + NK + NV + GR, 1), init(gates_free, GR, STATE ? 8 : 16), init(k_free, NK, STATE ? 1 : 2);
+        init(v_free, NV, STATE ? 8 : 9), init(s_ready, 2, 8), init(qk_done, 5, 1), init(ds_free, 1, 8), init(p_ready, 2, 8);
+        init(o_done, 2, 1), init(o_free, 2, 8), init(drain, 3, 1);
         *dead = 0, *bad_word = 0;
         fence_barrier_init();
     }
-    if (warp == 12) {
+    if (warp == 16) {
         umma::tmem_alloc(tbase, kTmem);
         umma::tmem_relinquish();
     }
@@ -231,355 +291,377 @@ __global__ void __launch_bounds__(kThreads, 1) umma_attention_kernel(const __gri
     const uint32_t tmem = *tbase;
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;  // this warp's part of tensor memory
 
-    // bounded; after one was given up nobody waits any more
-    auto wait = [&](uint64_t* x, uint32_t phase) {
-        for (uint32_t i = 0; i < up.polls; ++i) {
-            if (mbar_try_wait(x, phase & 1u)) return;
-            if (*dead) return;
-        }
-        *dead = 1;
+    auto wait = [&](const uint64_t* x, uint32_t phase) {
+        const uint32_t at = smem_addr(x);
+        if (!try_wait(at, phase & 1u)) wait_on(at, phase & 1u, smem_addr(tbase + 1), up.polls);
     };
     auto arrive = [&](uint64_t* x) {  // one of a warp's lanes, for all
         __syncwarp();
         if (lane == 0) mbar_arrive(x);
     };
 
-    if (warp < 4) {
-        // ---------------------------------------------------------------- P'
+    if (warp < 8) {
+        // ---------------------------------------------------------------- P', outputs
         if constexpr (!STATE) {
-            const int r = 32 * warp + lane;
-            for (int c = 0; c < n; ++c) {
+            const int quad = warp & 3, half = warp >> 2, r = 32 * quad + lane;
+            __nv_bfloat16* const out = static_cast<__nv_bfloat16*>(p.out) + b * p.ob + h * p.oh + col0 + 32 * half;
+            const int cols = p.dv - col0 - 32 * half;
+            float eg_last = 0.0f;  // of the chunk whose outputs come next
+            auto outputs = [&](int c) {  // 32 columns of chunk c
+                wait(o_done + (c & 1), c >> 1);
+                wait(qs_done + (c & 1), c >> 1);
+                umma::fence_after_sync();
+                float x[32], y[32];
+                umma::tmem_ld32(tmem + T_O1 + 32 * half + lanes, x);
+                umma::tmem_ld32(tmem + T_O2 + 64 * (c & 1) + 32 * half + lanes, y);
+                umma::tmem_wait_ld();
+                umma::fence_before_sync();
+                arrive(o_free + (c & 1));
+                const int64_t t = first + int64_t(c) * CT + r;
+                __nv_bfloat16* const to = out + t * p.ot;
+#pragma unroll
+                for (int e = 0; e < 32; e += 8) {
+                    uint32_t w[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        float2 z = make_float2(x[e + 2 * i], x[e + 2 * i + 1]);
+                        if (eg_last >= 0.0f) z = __ffma2_rn(splat(eg_last), make_float2(y[e + 2 * i], y[e + 2 * i + 1]), z);
+                        w[i] = pack_bf16(z.x, z.y);
+                    }
+                    if (t < p.T && e < cols) *reinterpret_cast<uint4*>(to + e) = make_uint4(w[0], w[1], w[2], w[3]);
+                }
+            };
+#pragma unroll 1
+            for (int c = 0; c <= n; ++c) {  // P' of chunk c, the outputs of the one before it
+                float eg = 0.0f;  // of the chunk; below 0: the entering state does not reach the row
+                if (c < n) {
                 const Gates& g = gates[c % GR];
                 wait(gates_full + c % GR, c / GR);
                 const float hr = g.hi[r], lr = g.lo[r];
-                const int sr = g.seg[r];
+                eg = g.seg[r] == 0 ? g.eg[r] : -1.0f;
                 const bool resets = g.d == -1.0f;
+                const bool steep = resets || !(g.hi[32 * quad] - g.hi[32 * quad + 31] < 80.0f);  // the factors leave the range
                 wait(qk_done + (c & 1), c >> 1);
                 umma::fence_after_sync();
-                const uint32_t tp = tmem + T_P + 128 * (c & 1) + lanes;
-#pragma unroll 1
-                for (int cb = 0; cb < 4; ++cb) {
-                    uint32_t pl[32];  // the first planes of 32 scores, then the second
-                    if (cb > warp) {
+                const uint32_t tp = tmem + M::T_P + 128 * (c % NP) + lanes;
+                // 16 columns at a time, every other one, two of them in flight; after the diagonal's they are 0
+                auto scores = [&](int cb, float (&x)[16]) {
+                    uint32_t pl[16];  // the first planes of 16 scores, then the second
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) pl[e] = 0u;
-                    } else {
-                        float x[32];
-                        umma::tmem_ld32(tp + 32 * cb, x);
-                        const bool pairwise = cb == warp || resets;
-                        float f = 0.0f;
-                        if (!pairwise) f = p.scale * ex2((hr - g.hi[32 * cb + 31]) + (lr - g.lo[32 * cb + 31]));
-                        umma::tmem_wait_ld();
-                        if (!pairwise) {
+                    for (int e = 0; e < 16; ++e) pl[e] = 0u;
+                    if (cb < 2 * quad + 2) {
+                        const int i32 = 16 * cb | 31;
+                        const float f = p.scale * ex2((hr - g.hi[i32]) + (lr - g.lo[i32]));  // from the end of the columns' 32 on
+                        if (cb >= 2 * quad ? !steep : !resets) {
+                            const float2 ff = splat(f);
 #pragma unroll
-                            for (int e = 0; e < 32; e += 4) {
-                                const float4 end = *reinterpret_cast<const float4*>(&g.end[32 * cb + e]);
-                                const float2 a = __fmul2_rn(make_float2(x[e], x[e + 1]), __fmul2_rn(make_float2(end.x, end.y), splat(f)));
-                                const float2 d = __fmul2_rn(make_float2(x[e + 2], x[e + 3]), __fmul2_rn(make_float2(end.z, end.w), splat(f)));
-                                x[e] = a.x, x[e + 1] = a.y, x[e + 2] = d.x, x[e + 3] = d.y;
+                            for (int e = 0; e < 16; e += 4) {
+                                const float4 end = *reinterpret_cast<const float4*>(&g.end[16 * cb + e]);
+                                const float2 u = __fmul2_rn(make_float2(x[e], x[e + 1]), __fmul2_rn(make_float2(end.x, end.y), ff));
+                                const float2 d = __fmul2_rn(make_float2(x[e + 2], x[e + 3]), __fmul2_rn(make_float2(end.z, end.w), ff));
+                                x[e] = u.x, x[e + 1] = u.y, x[e + 2] = d.x, x[e + 3] = d.y;
                             }
+                            if (cb >= 2 * quad)
+#pragma unroll
+                                for (int e = 0; e < 16; ++e) x[e] = 16 * cb + e <= r ? x[e] : 0.0f;
                         } else {
+                            const int sr = g.seg[r];
 #pragma unroll
-                            for (int e = 0; e < 32; e += 4) {
-                                const float4 hs = *reinterpret_cast<const float4*>(&g.hi[32 * cb + e]);
-                                const float4 ls = *reinterpret_cast<const float4*>(&g.lo[32 * cb + e]);
-                                const int4 ss = *reinterpret_cast<const int4*>(&g.seg[32 * cb + e]);
-                                const float hv[4] = {hs.x, hs.y, hs.z, hs.w}, lv[4] = {ls.x, ls.y, ls.z, ls.w};
-                                const int sv[4] = {ss.x, ss.y, ss.z, ss.w};
-#pragma unroll
-                                for (int i = 0; i < 4; ++i)
-                                    x[e + i] = sv[i] == sr && 32 * cb + e + i <= r ? x[e + i] * (p.scale * ex2((hr - hv[i]) + (lr - lv[i]))) : 0.0f;
+                            for (int e = 0; e < 16; ++e) {
+                                const int i = 16 * cb + e;
+                                x[e] = g.seg[i] == sr && i <= r ? x[e] * (p.scale * ex2((hr - g.hi[i]) + (lr - g.lo[i]))) : 0.0f;
                             }
                         }
 #pragma unroll
-                        for (int e = 0; e < 16; ++e) {
+                        for (int e = 0; e < 8; ++e) {
                             uint32_t two[2];
                             split<2>(make_float2(x[2 * e], x[2 * e + 1]), two);
-                            pl[e] = two[0], pl[16 + e] = two[1];
+                            pl[e] = two[0], pl[8 + e] = two[1];
                         }
                     }
-                    tmem_st32(tp + 32 * cb, pl);
+                    tmem_st16(tp + 16 * cb, pl);
+                };
+#pragma unroll 1
+                for (int cb = half; cb < 8; cb += 4) {
+                    float x[16], y[16];
+                    tmem_ld16(tp + 16 * cb, x);
+                    tmem_ld16(tp + 16 * cb + 32, y);
+                    umma::tmem_wait_ld();
+                    scores(cb, x);
+                    scores(cb + 2, y);
                 }
                 umma::tmem_wait_st();
                 umma::fence_before_sync();
                 arrive(p_ready + (c & 1));
                 arrive(gates_free + c % GR);
+                }
+                if (c > 0) outputs(c - 1);
+                eg_last = eg;
             }
         }
-    } else if (warp < 8) {
-        // ---------------------------------------------------------------- V w and the state
-        const int bw = warp - 4, bt = threadIdx.x - 128, gr = lane >> 2, c2 = (lane & 3) * 2, j0 = col0 + 16 * bw + gr;
-        float s[NI][4];  // transposed: rows j0 and + 8, columns 8 n + c2 and + 1
+    } else if (warp < 16) {
+        // ---------------------------------------------------------------- V w, the state
+        // 16 columns of v and half of the features a warp
+        constexpr int NH = DK / 16;  // 8-feature tiles of a warp
+        const int bt = threadIdx.x - 256, quad = warp & 3, gr = lane >> 2, c2 = (lane & 3) * 2, j0 = col0 + 16 * quad + gr;
+        const int m0 = (warp >= 12 ? NH : 0);  // its first tile
+        float s[NH][4];  // transposed: rows j0 and + 8, columns 8 (m0 + m) + c2 and + 1
         {
             const float* from = STATE ? nullptr : seg > 0 ? p.part + (chain * (p.nseg - 1) + seg - 1) * p.dk * int64_t(p.dv)
                                       : p.s0 != nullptr   ? p.s0 + chain * p.dk * int64_t(p.dv) : nullptr;
 #pragma unroll
-            for (int m = 0; m < NI; ++m)
+            for (int m = 0; m < NH; ++m)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const int i = 8 * m + c2 + (e & 1), j = j0 + (e >> 1) * 8;
+                    const int i = 8 * (m0 + m) + c2 + (e & 1), j = j0 + (e >> 1) * 8;
                     s[m][e] = from != nullptr && i < p.dk && j < p.dv ? from[int64_t(i) * p.dv + j] : 0.0f;
                 }
         }
-        auto publish = [&] {  // the state's planes, as the K-major B of Q S
-#pragma unroll
-            for (int m = 0; m < NI; ++m)
-#pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    uint32_t two[2];
-                    split<2>(make_float2(s[m][2 * r], s[m][2 * r + 1]), two);
-#pragma unroll
-                    for (int a = 0; a < 2; ++a)
-                        *reinterpret_cast<uint32_t*>(base + M::S + a * M::SB + (m >> 3) * (DVS * 128) +
-                                                     umma::sw128(16 * bw + gr + 8 * r, m & 7) + c2 * 2) = two[a];
-                }
-            fence_proxy_async_shared();
-            arrive(s_ready);
-        };
-        if (!STATE) publish();
         float total = 1.0f;
         bool bad = false;
         for (int c = 0; c < n; ++c) {
             const Gates& g = gates[c % GR];
-            wait(gates_full + c % GR, c / GR);
             wait(full_v + c % NV, c / NV);
-            wait(full_k + c % NK, c / NK);
-            const unsigned char *vt = base + M::V + (c % NV) * M::VB, *kt = base + M::K + (c % NK) * M::QB;
-            __nv_bfloat162 chk = __floats2bfloat162_rn(0.0f, 0.0f);
+            wait(gates_full + c % GR, c / GR);
+            const unsigned char *vt = base + M::V + (c % NV) * M::VB + umma::sw128(bt / 8, bt % 8);  // rows 32 apart: 4096 bytes
+            unsigned char* const wt = base + M::W + umma::sw128(bt / 8, bt % 8);
+            const float d = g.d;
+            bad |= g.wild != 0;
+            total = total == -1.0f || d == -1.0f ? -1.0f : total * d;
+            uint4 u[4];
+            float w[4];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int row = bt / 8 + 16 * i;
-                const uint32_t off = umma::sw128(row, bt % 8);
-                const uint4 u = *reinterpret_cast<const uint4*>(vt + off);
-                check8(u, chk);
-                const float2 w = splat(g.w[row]);
-                const uint32_t x[4] = {u.x, u.y, u.z, u.w};
-                uint32_t pl[4][kVPlanes];
+            for (int i = 0; i < 4; ++i) u[i] = *reinterpret_cast<const uint4*>(vt + 4096 * i), w[i] = g.w[bt / 8 + 32 * i];
+            // (the planes of the last chunk have been read: its dS is there)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) split<kVPlanes>(__fmul2_rn(w, unpack_bf16(x[e])), pl[e]);
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t x[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
+                uint32_t pl[4][VP];
 #pragma unroll
-                for (int a = 0; a < kVPlanes; ++a)
-                    *reinterpret_cast<uint4*>(base + M::W + a * M::VB + off) = make_uint4(pl[0][a], pl[1][a], pl[2][a], pl[3][a]);
+                for (int e = 0; e < 4; ++e) split<VP>(__fmul2_rn(splat(w[i]), unpack_bf16(x[e])), pl[e]);
+#pragma unroll
+                for (int a = 0; a < VP; ++a)
+                    *reinterpret_cast<uint4*>(wt + a * M::VB + 4096 * i) = make_uint4(pl[0][a], pl[1][a], pl[2][a], pl[3][a]);
             }
             fence_proxy_async_shared();
-            umma::fence_before_sync();  // the last chunk's dS has been read
             arrive(vw_ready);
+            arrive(gates_free + c % GR);
+            arrive(v_free + c % NV);
+            if constexpr (!STATE) {  // the planes of the state that enters, as the K-major B of Q S
+                if (c > 0) wait(qs_done + ((c - 1) & 1), (c - 1) >> 1);  // the last ones have been read
+                const uint32_t row = sb + M::S + umma::sw128(16 * quad + gr, 0) + c2 * 2;  // and the one 8 below, 1024 bytes on
 #pragma unroll
-            for (int i = 0; i < DK / 8; ++i)
-                check8(*reinterpret_cast<const uint4*>(kt + (i / 8) * (CT * 128) + umma::sw128(bt / 8 + 16 * (i % 8), bt % 8)), chk);
-            const float2 f = __bfloat1622float2(chk);
-            bad |= !(f.x == 0.0f && f.y == 0.0f) || g.wild != 0;
-            const float d = g.d;
-            total = total == -1.0f || d == -1.0f ? -1.0f : total * d;
+                for (int m = 0; m < NH; ++m) {
+                    // the row's 16-byte piece k lies at k ^ gr, piece 0 at gr
+                    const uint32_t to = (row ^ (((m0 + m) & 7) << 4)) + ((m0 + m) >> 3) * (DVS * 128);
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) {
+                        uint32_t two[2];
+                        split<2>(make_float2(s[m][2 * r], s[m][2 * r + 1]), two);
+                        st_shared(to + r * 1024, two[0]), st_shared(to + r * 1024 + M::SB, two[1]);
+                    }
+                }
+                fence_proxy_async_shared();
+                arrive(s_ready);
+            }
             wait(ds_done, c);
             umma::fence_after_sync();
+            float x[NH * 4];
+            tmem_ld_half(tmem + T_DS + 8 * m0 + lanes, x);
+            umma::tmem_wait_ld();
+            umma::fence_before_sync();
+            arrive(ds_free);
+            // an infinity or NaN of k or v leaves one here, under a weight of 0 too (V w is a NaN
+            // then): a sum of 0 x is 0 otherwise
+            float2 chk = splat(0.0f);
+            const float2 dd = splat(d == -1.0f ? 0.0f : d);
 #pragma unroll
-            for (int m0 = 0; m0 < NI; m0 += 8) {
-                float x[32];
-                tmem_ld16x64(tmem + T_DS + 8 * m0 + lanes, x);
-                umma::tmem_wait_ld();
+            for (int m = 0; m < NH; ++m)
 #pragma unroll
-                for (int m = 0; m < 8; ++m)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        float& y = s[m0 + m][e];
-                        y = d == -1.0f ? x[4 * m + e] : fmaf(d, y, x[4 * m + e]);
-                    }
-            }
-            if (!STATE && c + 1 < n) publish();
-            arrive(gates_free + c % GR);
+                for (int e = 0; e < 4; e += 2) {
+                    const float2 z = make_float2(x[4 * m + e], x[4 * m + e + 1]);
+                    float2 y = make_float2(s[m][e], s[m][e + 1]);
+                    if (d == -1.0f) y = splat(0.0f);  // whatever it holds
+                    chk = __ffma2_rn(z, splat(0.0f), chk);
+                    y = __ffma2_rn(dd, y, z);
+                    s[m][e] = y.x, s[m][e + 1] = y.y;
+                }
+            bad |= !(chk.x == 0.0f && chk.y == 0.0f);
         }
         if (bad) *bad_word = 1;
         float* const to = STATE ? p.part + (chain * (p.nseg - 1) + seg) * p.dk * int64_t(p.dv)
                                 : seg == p.nseg - 1 && p.sT != nullptr ? p.sT + chain * p.dk * int64_t(p.dv) : nullptr;
         if (to != nullptr)
 #pragma unroll
-            for (int m = 0; m < NI; ++m)
+            for (int m = 0; m < NH; ++m)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const int i = 8 * m + c2 + (e & 1), j = j0 + (e >> 1) * 8;
+                    const int i = 8 * (m0 + m) + c2 + (e & 1), j = j0 + (e >> 1) * 8;
                     if (i < p.dk && j < p.dv) to[int64_t(i) * p.dv + j] = s[m][e];
                 }
         if (STATE && slice == 0 && bt == 0) p.part_d[chain * (p.nseg - 1) + seg] = total;
-    } else if (warp < 12) {
-        // ---------------------------------------------------------------- outputs
-        if constexpr (!STATE) {
-            const int r = 32 * (warp - 8) + lane;
-            __nv_bfloat16* const out = static_cast<__nv_bfloat16*>(p.out) + b * p.ob + h * p.oh + col0;
-            for (int c = 0; c < n; ++c) {
-                const Gates& g = gates[c % GR];
-                wait(gates_full + c % GR, c / GR);
-                const float eg = g.eg[r];
-                const bool reach = g.seg[r] == 0;
-                arrive(gates_free + c % GR);
-                wait(qk_done + (c & 1), c >> 1);
-                umma::fence_after_sync();
-                float x[2][32];
-                umma::tmem_ld32(tmem + T_O2 + lanes, x[0]);
-                umma::tmem_ld32(tmem + T_O2 + 32 + lanes, x[1]);
-                umma::tmem_wait_ld();
-                umma::fence_before_sync();
-                arrive(o2_free);
-#pragma unroll
-                for (int i = 0; i < 2; ++i)
-#pragma unroll
-                    for (int e = 0; e < 32; ++e) x[i][e] = reach ? eg * x[i][e] : 0.0f;
-                wait(o_done, c);
-                umma::fence_after_sync();
-                const int64_t t = first + int64_t(c) * CT + r;
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    float y[32];
-                    umma::tmem_ld32(tmem + T_O1 + 32 * i + lanes, y);
-                    umma::tmem_wait_ld();
-                    if (i == 1) {
-                        umma::fence_before_sync();
-                        arrive(o1_free);
-                    }
-                    if (t < p.T) {
-                        __nv_bfloat16* const to = out + t * p.ot + 32 * i;
-#pragma unroll
-                        for (int e = 0; e < 32; e += 8) {
-                            uint32_t w[4];
-#pragma unroll
-                            for (int k = 0; k < 4; ++k) w[k] = pack_bf16(x[i][e + 2 * k] + y[e + 2 * k], x[i][e + 2 * k + 1] + y[e + 2 * k + 1]);
-                            if (col0 + 32 * i + e < p.dv) *reinterpret_cast<uint4*>(to + e) = make_uint4(w[0], w[1], w[2], w[3]);
-                        }
-                    }
-                }
-            }
-        }
-    } else if (warp == 12) {
-        // ---------------------------------------------------------------- loads and MMAs
-        if (lane == 0) {
-            const int hq = h / p.q.share, hk = h / p.k.share, hv = h / p.v.share;
-            int nq = 0, nk = 0, nv = 0;  // loads issued
-            auto load_q = [&] {
-                if (STATE || nq >= n) return;
-                const int st = nq % NQ, t = static_cast<int>(first) + nq * CT;
-                mbar_arrive_expect_tx(full_q + st, M::QB);
-#pragma unroll
-                for (int i = 0; i < DK / 64; ++i) tma_load(sb + M::Q + st * M::QB + i * CT * 128, &up.q, 64 * i, hq, t, b, full_q + st);
-                ++nq;
-            };
-            auto load_k = [&] {
-                if (nk >= n) return;
-                const int st = nk % NK, t = static_cast<int>(first) + nk * CT;
-                mbar_arrive_expect_tx(full_k + st, M::QB);
-#pragma unroll
-                for (int i = 0; i < DK / 64; ++i) tma_load(sb + M::K + st * M::QB + i * CT * 128, &up.k, 64 * i, hk, t, b, full_k + st);
-                ++nk;
-            };
-            auto load_v = [&] {
-                if (nv >= n) return;
-                const int st = nv % NV, t = static_cast<int>(first) + nv * CT;
-                mbar_arrive_expect_tx(full_v + st, M::VB);
-                tma_load(sb + M::V + st * M::VB, &up.v, col0, hv, t, b, full_v + st);
-                ++nv;
-            };
-            for (int i = 0; i < (NK > NQ ? NK : NQ); ++i) {
-                if (i < NK) load_k();
-                if (i < NQ) load_q();
-                if (i < NV) load_v();
-            }
-            constexpr uint32_t ID_QK = umma::idesc_bf16(128, 128, umma::K_MAJOR, umma::K_MAJOR);
-            constexpr uint32_t ID_QS = umma::idesc_bf16(128, DVS, umma::K_MAJOR, umma::K_MAJOR);
-            constexpr uint32_t ID_PV = umma::idesc_bf16(128, DVS, umma::K_MAJOR, umma::MN_MAJOR);
-            constexpr uint32_t ID_VK = umma::idesc_bf16(DVS, DK, umma::MN_MAJOR, umma::MN_MAJOR);
-            auto issue_vk = [&](int c) {
-                umma::fence_after_sync();
-                const uint32_t k0 = sb + M::K + (c % NK) * M::QB;
-#pragma unroll
-                for (int a = kVPlanes - 1; a >= 0; --a)  // the smallest products first
-#pragma unroll
-                    for (int k = 0; k < CT / 16; ++k)
-                        umma::mma_bf16(tmem + T_DS, umma::smem_desc(sb + M::W + a * M::VB + 2048 * k, CT * 128, 1024),
-                                       umma::smem_desc(k0 + 2048 * k, CT * 128, 1024), ID_VK, a < kVPlanes - 1 || k > 0);
-                umma::mma_commit(ds_done);
-            };
-            if constexpr (STATE) {
-                for (int c = 0; c < n; ++c) {
-                    wait(full_k + c % NK, c / NK);
-                    wait(vw_ready, c);
-                    if (c > 0) load_k(), load_v();  // chunk c - 1 has been read: its dS has been added
-                    issue_vk(c);
-                }
-            } else {
-                for (int c = 0; c <= n; ++c) {
-                    if (c < n) {
-                        wait(s_ready, c);
-                        if (c > 0) load_k();  // chunk c - 1's MMAs with K are done: its dS has been added
-                        wait(full_q + c % NQ, c / NQ);
-                        wait(full_k + c % NK, c / NK);
-                        if (c > 0) wait(o2_free, c - 1);
-                        if (c > 1) wait(o_done, c - 2);  // P's buffer has been read
-                        umma::fence_after_sync();
-                        const uint32_t q0 = sb + M::Q + (c % NQ) * M::QB, k0 = sb + M::K + (c % NK) * M::QB;
-#pragma unroll
-                        for (int k = 0; k < DK / 16; ++k) {
-                            const uint32_t off = (k >> 2) * (CT * 128) + 32 * (k & 3);
-                            umma::mma_bf16(tmem + T_P + 128 * (c & 1), umma::smem_desc(q0 + off, 16, 1024),
-                                           umma::smem_desc(k0 + off, 16, 1024), ID_QK, k > 0);
-                        }
-#pragma unroll
-                        for (int a = 1; a >= 0; --a)
-#pragma unroll
-                            for (int k = 0; k < DK / 16; ++k)
-                                umma::mma_bf16(tmem + T_O2, umma::smem_desc(q0 + (k >> 2) * (CT * 128) + 32 * (k & 3), 16, 1024),
-                                               umma::smem_desc(sb + M::S + a * M::SB + (k >> 2) * (DVS * 128) + 32 * (k & 3), 16, 1024),
-                                               ID_QS, a < 1 || k > 0);
-                        umma::mma_commit(qk_done + (c & 1));
-                    }
-                    // whichever can go: dS of this chunk, O1 of the one before it, loads
-                    bool vk = c < n, pv = c > 0, lq = c < n, lv = false;
-                    for (uint32_t i = 0; vk || pv || lq || lv; ++i) {
-                        if (vk && mbar_test_wait(vw_ready, c & 1)) issue_vk(c), vk = false;
-                        if (lq && mbar_test_wait(qk_done + (c & 1), (c >> 1) & 1)) load_q(), lq = false;
-                        if (pv && mbar_test_wait(p_ready + ((c - 1) & 1), ((c - 1) >> 1) & 1) &&
-                            (c == 1 || mbar_test_wait(o1_free, (c - 2) & 1))) {
-                            umma::fence_after_sync();
-                            const uint32_t tp = tmem + T_P + 128 * ((c - 1) & 1), v0 = sb + M::V + ((c - 1) % NV) * M::VB;
-#pragma unroll
-                            for (int a = 1; a >= 0; --a)
-#pragma unroll
-                                for (int k = 0; k < CT / 16; ++k)
-                                    mma_ts(tmem + T_O1, tp + 32 * (k >> 1) + 16 * a + 8 * (k & 1), umma::smem_desc(v0 + 2048 * k, CT * 128, 1024),
-                                           ID_PV, a < 1 || k > 0);
-                            umma::mma_commit(o_done);
-                            pv = false, lv = true;
-                        }
-                        if (lv && mbar_test_wait(o_done, (c - 1) & 1)) load_v(), lv = false;
-                        if (*dead) break;
-                        if (i >= up.polls * 16) *dead = 1;
-                    }
-                }
-            }
-            // every MMA and load issued ends before the block does
-            umma::mma_commit(drain);
-            for (uint32_t i = 0; i < kPolls && !mbar_try_wait(drain, 0); ++i) {
-            }
-            auto landed = [&](uint64_t* full, int issued, int ring) {
-                for (int l = issued > ring ? issued - ring : 0; l < issued; ++l)
-                    for (uint32_t i = 0; i < kPolls && !mbar_try_wait(full + l % ring, (l / ring) & 1); ++i) {
-                    }
-            };
-            landed(full_q, nq, NQ), landed(full_k, nk, NK), landed(full_v, nv, NV);
-        }
-        __syncwarp();
-    } else {
+    } else if (warp == 16) {
         // ---------------------------------------------------------------- decays
-        Tokens next = load_tokens(p, ld, marks, first);
+        const float* at = ld + (first + 4 * lane) * p.lt;
+        const uint8_t* mark = marks == nullptr ? nullptr : marks + (first + 4 * lane) * p.gt;
+        float next[4];
+        auto fetch = [&](int c) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const bool live = first + c * CT + 4 * lane + i < p.T;
+                next[i] = live ? at[i * p.lt] : 0.0f;
+                if (live && marks != nullptr && mark[i * p.gt] != 0) next[i] = -INFINITY;
+            }
+            at += CT * p.lt;
+            if (marks != nullptr) mark += CT * p.gt;
+        };
+        fetch(0);
+#pragma unroll 1
         for (int c = 0; c < n; ++c) {
-            const Tokens now = next;
-            if (c + 1 < n) next = load_tokens(p, ld, marks, first + int64_t(c + 1) * CT);
+            float now[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) now[i] = next[i];
+            if (c + 1 < n) fetch(c + 1);
             if (c >= GR) wait(gates_free + c % GR, c / GR - 1);
             make_gates(now, p.scale, gates[c % GR]);
             arrive(gates_full + c % GR);
         }
+    } else {
+        // ---------------------------------------------------------------- MMAs and loads
+        const uint64_t desc_k = umma::smem_desc(sb, 16, 1024), desc_mn = umma::smem_desc(sb, CT * 128, 1024);  // + bytes / 16
+        auto load = [&](uint64_t* full, const CUtensorMap* tm, uint32_t to, int bytes, int col, int head, int c) {
+            if (c < n) load_rows(smem_addr(full), tm, to, bytes, col, head, static_cast<int>(first) + c * CT, b);
+        };
+        auto load_q = [&](int c) { load(full_q + c % NQ, &up.q, sb + M::Q + c % NQ * M::QB, M::QB, 0, h / p.q.share, c); };
+        auto load_k = [&](int c) { load(full_k + c % NK, &up.k, sb + M::K + c % NK * M::QB, M::QB, 0, h / p.k.share, c); };
+        auto load_v = [&](int c) { load(full_v + c % NV, &up.v, sb + M::V + c % NV * M::VB, M::VB, col0, h / p.v.share, c); };
+        if (warp == 17) {  // P = Q K^T of the chunk ahead, O2 = Q S
+            if constexpr (!STATE) {
+                constexpr uint32_t ID_QK = umma::idesc_bf16(128, 128, umma::K_MAJOR, umma::K_MAJOR);
+                constexpr uint32_t ID_QS = umma::idesc_bf16(128, DVS, umma::K_MAJOR, umma::K_MAJOR);
+    #pragma unroll 1
+            for (int c = 0; c < NQ; ++c) load_q(c);
+                for (int c = 0; c <= n; ++c) {  // P of chunk c, O2 of the one before it
+                    auto scores = [&] {
+                        wait(full_q + c % NQ, c / NQ);
+                        wait(full_k + c % NK, c / NK);
+                        if (c >= NP) wait(o_done + ((c - NP) & 1), (c - NP) >> 1);  // the scores in P's place have been read
+                        umma::fence_after_sync();
+                        if (elect_one()) {
+                            const uint64_t q0 = desc_k + ((M::Q + (c % NQ) * M::QB) >> 4), k0 = desc_k + ((M::K + (c % NK) * M::QB) >> 4);
+#pragma unroll 4
+                            for (int k = 0; k < DK / 16; ++k) {
+                                const uint32_t off = ((k >> 2) * (CT * 128) + 32 * (k & 3)) >> 4;
+                                umma::mma_bf16(tmem + M::T_P + 128 * (c % NP), q0 + off, k0 + off, ID_QK, k > 0);
+                            }
+                            umma::mma_commit(qk_done + (c & 1));
+                            umma::mma_commit(k_free + c % NK);
+                        }
+                        __syncwarp();
+                    };
+                    if (NQ > 1 && c < n) scores();
+                    if (c > 0) {
+                        const int l = c - 1;
+                        wait(s_ready, l);
+                        if (l > 1) wait(o_free + (l & 1), (l - 2) >> 1);  // the outputs two chunks back are read
+                        umma::fence_after_sync();
+                        if (elect_one()) {
+                            const uint64_t q0 = desc_k + ((M::Q + (l % NQ) * M::QB) >> 4), s0 = desc_k + (M::S >> 4);
+#pragma unroll 1
+                            for (int a = 1; a >= 0; --a)
+#pragma unroll 4
+                                for (int k = 0; k < DK / 16; ++k)
+                                    umma::mma_bf16(tmem + T_O2 + 64 * (l & 1), q0 + (((k >> 2) * (CT * 128) + 32 * (k & 3)) >> 4),
+                                                   s0 + ((a * M::SB + (k >> 2) * (DVS * 128) + 32 * (k & 3)) >> 4), ID_QS, a < 1 || k > 0);
+                            umma::mma_commit(qs_done + (l & 1));
+                        }
+                        __syncwarp();
+                        if (l + NQ < n) {
+                            wait(qs_done + (l & 1), l >> 1);  // and the scores before it
+                            load_q(l + NQ);
+                        }
+                    }
+                    if (NQ == 1 && c < n) scores();
+                }
+            }
+        } else if (warp == 18) {  // dS = (V w)^T K
+            constexpr uint32_t ID_VK = umma::idesc_bf16(DVS, DK, umma::MN_MAJOR, umma::MN_MAJOR);
+#pragma unroll 1
+            for (int c = 0; c < NK; ++c) {
+                load_k(c);
+                if (STATE) load_v(c);
+            }
+            for (int c = 0; c < n; ++c) {
+                if (c > 0) {
+                    wait(k_free + (c - 1) % NK, (c - 1) / NK);
+                    load_k(c - 1 + NK);
+                    if (STATE) {
+                        wait(v_free + (c - 1) % NV, (c - 1) / NV);
+                        load_v(c - 1 + NV);
+                    }
+                }
+                wait(full_k + c % NK, c / NK);
+                wait(vw_ready, c);
+                if (c > 0) wait(ds_free, c - 1);  // the last one has been read
+                umma::fence_after_sync();
+                if (elect_one()) {
+                    const uint64_t k0 = desc_mn + ((M::K + (c % NK) * M::QB) >> 4), w0 = desc_mn + (M::W >> 4);
+#pragma unroll 1
+                    for (int a = VP - 1; a >= 0; --a)  // the smallest products first
+#pragma unroll
+                        for (int k = 0; k < CT / 16; ++k)
+                            umma::mma_bf16(tmem + T_DS, w0 + ((a * M::VB + 2048 * k) >> 4), k0 + (2048 * k >> 4), ID_VK, a < VP - 1 || k > 0);
+                    umma::mma_commit(ds_done);
+                    umma::mma_commit(k_free + c % NK);
+                }
+                __syncwarp();
+            }
+        } else if constexpr (!STATE) {  // O1 = P' V
+            constexpr uint32_t ID_PV = umma::idesc_bf16(128, DVS, umma::K_MAJOR, umma::MN_MAJOR);
+#pragma unroll 1
+            for (int c = 0; c < NV; ++c) load_v(c);
+            for (int c = 0; c < n; ++c) {
+                if (c > 0) {
+                    wait(v_free + (c - 1) % NV, (c - 1) / NV);
+                    load_v(c - 1 + NV);
+                }
+                wait(full_v + c % NV, c / NV);
+                wait(p_ready + (c & 1), c >> 1);
+                if (c > 0) wait(o_free + ((c - 1) & 1), (c - 1) >> 1);  // the last outputs have been read
+                umma::fence_after_sync();
+                if (elect_one()) {
+                    const uint32_t tp = tmem + M::T_P + 128 * (c % NP);
+                    const uint64_t v0 = desc_mn + ((M::V + (c % NV) * M::VB) >> 4);
+#pragma unroll 1
+                    for (int a = 1; a >= 0; --a)
+#pragma unroll
+                        for (int k = 0; k < CT / 16; ++k)
+                            mma_ts(tmem + T_O1, tp + 16 * k + 8 * a, v0 + (2048 * k >> 4), ID_PV, a < 1 || k > 0);
+                    umma::mma_commit(o_done + (c & 1));
+                    umma::mma_commit(v_free + c % NV);
+                }
+                __syncwarp();
+            }
+        }
+        // every MMA and load issued ends before the block does
+        if (elect_one()) {
+            umma::mma_commit(drain + (warp - 17));
+            for (uint32_t i = 0; i < kPolls && !mbar_try_wait(drain + (warp - 17), 0); ++i) {
+            }
+            auto landed = [&](uint64_t* full, int ring) {
+                for (int c = n > ring ? n - ring : 0; c < n; ++c)
+                    for (uint32_t i = 0; i < kPolls && !mbar_try_wait(full + c % ring, (c / ring) & 1); ++i) {
+                    }
+            };
+            if (warp == 17 && !STATE) landed(full_q, NQ);
+            if (warp == 18) landed(full_k, NK);
+            if (warp == (STATE ? 18 : 19)) landed(full_v, NV);
+        }
+        __syncwarp();
     }
     umma::fence_before_sync();
     __syncthreads();
-    if (warp == 12) {
+    if (warp == 16) {
         umma::fence_after_sync();
         umma::tmem_dealloc(tmem, kTmem);
     }
@@ -602,10 +684,10 @@ int encode(CUtensorMap* tm, const Stream& x, int64_t nb, int64_t T, int64_t head
 
 std::atomic<uint32_t> umma_polls{kPolls};
 
-template <int DK, bool STATE>
+template <int DK, bool STATE, int VP>
 int launch(const UmmaParams& up, int64_t blocks, cudaStream_t s) {
     static std::atomic<uint64_t> done{0};
-    auto kern = umma_attention_kernel<DK, STATE>;
+    auto kern = umma_attention_kernel<DK, STATE, VP>;
     cudaError_t e = ensure_smem(kern, Map<DK>::BYTES, done);
     if (e != cudaSuccess) return cuda_fail(e, "linear attention shared memory");
     kern<<<static_cast<unsigned>(blocks), kThreads, Map<DK>::BYTES, s>>>(up);
@@ -635,8 +717,12 @@ int umma_run(const AttnParams& p, int64_t nb, bool state, uint32_t* redo, cudaSt
     if (int rc = encode(&up.k, p.k, nb, p.T, p.H / p.k.share, p.dk)) return rc;
     if (int rc = encode(&up.v, p.v, nb, p.T, p.H / p.v.share, p.dv)) return rc;
     const int64_t blocks = nb * p.H * p.slices * (state ? p.nseg - 1 : p.nseg);
-    if (p.dk <= 64) return state ? launch<64, true>(up, blocks, stream) : launch<64, false>(up, blocks, stream);
-    return state ? launch<128, true>(up, blocks, stream) : launch<128, false>(up, blocks, stream);
+    auto go = [&](auto dk) {
+        constexpr int DK = decltype(dk)::value;
+        if (state) return p.sT != nullptr ? launch<DK, true, 3>(up, blocks, stream) : launch<DK, true, 2>(up, blocks, stream);
+        return p.sT != nullptr ? launch<DK, false, 3>(up, blocks, stream) : launch<DK, false, 2>(up, blocks, stream);
+    };
+    return p.dk <= 64 ? go(std::integral_constant<int, 64>{}) : go(std::integral_constant<int, 128>{});
 }
 
 }  // namespace attention

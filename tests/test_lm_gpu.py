@@ -46,7 +46,12 @@ def check_attention(q, k, v, ld, scale=1.0, seg=None, state=None, twice=True):
     close(out, want, mag + small / SUMS[q.dtype], SUMS[q.dtype], ref.HALF_STEP[q.dtype])
     close(fin, s, m, STATE)
     alone = nk.linear_attention(q, k, v, ld, scale=scale, seg_start=seg, state=state)
-    assert torch.equal(alone, out) or not twice
+    if q.dtype == BF:  # without a state to return its sums may hold 2^-17 of their terms (as the scores do), within the bound
+        close(alone, want, mag, SUMS[BF], ref.HALF_STEP[BF])
+        alone, out2 = (nk.linear_attention(q, k, v, ld, scale=scale, seg_start=seg, state=state) for _ in range(2))
+        assert torch.equal(alone, out2) or not twice
+    else:
+        assert torch.equal(alone, out)
     return out, fin
 
 
