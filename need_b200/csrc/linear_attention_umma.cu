@@ -16,8 +16,9 @@
 // warps of its own, which meet at mbarriers only, so that a chunk's scores, outputs and
 // state run beside its neighbours':
 //
-//   warps 0-7    P' and the outputs: two for each 32 rows, a row per thread; a decay is a row's
-//                factor times a column's, but where one of them would leave fp32's range
+//   warps 0-7    P' and the outputs: two for each 32 rows, a row per thread.  A decay is a row's
+//                factor, which can wait for the outputs, times a column's -- but in a chunk that a
+//                segment starts in, or that decays by more than 2^-64
 //   warps 8-15   V w, the check for infinities, the state and its planes
 //   warp 16      the decays of the chunks ahead
 //   warps 17-19  the MMAs, each with the loads (TMA, no multicast) whose place they free: P and
@@ -54,10 +55,12 @@ constexpr uint32_t kPolls = 1u << 16;  // of a wait before it is given up
 constexpr uint32_t kTmem = 512, T_O1 = 0, T_O2 = 64, T_DS = 192;  // tensor memory columns
 
 struct alignas(16) Gates {
-    float hi[CT], lo[CT], w[CT], eg[CT], end[CT];  // as Decays; end: of its block of 32
+    float hi[CT], lo[CT], w[CT], eg[CT];  // as Decays
+    float row[CT];  // what a row of O1 is multiplied with: where a decay is a row's factor times a column's
+                    // (w), scale times that from the chunk's end back to the token; else 1
     int seg[CT];
     float d;
-    int wild;
+    int wild, factors;
 };
 
 // VP: planes of V w.  3 where the state itself is a result; where only outputs of bf16 come
@@ -65,7 +68,9 @@ struct alignas(16) Gates {
 template <int DK>
 struct Map {  // shared memory, from a 1024-byte aligned base
     static constexpr int NQ = DK == 64 ? 2 : 1, NK = DK == 64 ? 3 : 2, NV = NK;  // chunks loaded ahead
-    static constexpr int NP = DK == 64 ? 2 : 1;                                  // buffers of P
+    // buffers of P (tensor memory holds a second one at 64 features; at 128 in the place of O2's
+    // second, which took longer: 1x16384 32x128 406 us against 343)
+    static constexpr int NP = DK == 64 ? 2 : 1;
     static constexpr uint32_t T_P = T_DS + DK;
     static_assert(T_P + NP * 128 <= kTmem, "tensor memory");
     static constexpr int QB = CT * DK * 2, VB = CT * DVS * 2, SB = DVS * DK * 2;
@@ -78,6 +83,7 @@ struct UmmaParams {
     AttnParams a;
     uint32_t* redo;
     uint32_t polls;
+    int32_t wide;  // the outputs' rows lie apart by whole 32 bytes
 };
 
 __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* tm, int c0, int c1, int c2, int c3, uint32_t bar) {
@@ -208,7 +214,9 @@ __device__ __forceinline__ void make_gates(const float (&x)[4], float scale, Gat
     auto of = [&](int l) { return Sum2{__shfl_sync(0xffffffffu, incl.hi, l), __shfl_sync(0xffffffffu, incl.lo, l)}; };
     Sum2 before = of((lane + 31) & 31);
     if (lane == 0) before = {0.0f, 0.0f};
-    const Sum2 end = of(31), block_end = of(lane | 7);
+    const Sum2 end = of(31);
+    // a row's factor is up to 2^64 then
+    const bool factors = send == 0 && end.hi > -64.0f;
     float4 hi, lo, w, eg, be;
     int4 seg;
     float *ph = &hi.x, *pl = &lo.x, *pw = &w.x, *pe = &eg.x, *pb = &be.x;
@@ -220,12 +228,12 @@ __device__ __forceinline__ void make_gates(const float (&x)[4], float scale, Gat
         ph[e] = t.hi, pl[e] = t.lo, ps[e] = s;
         pw[e] = s == send ? ex2(minus(end, t)) : 0.0f;
         pe[e] = s == 0 ? scale * ex2(t.hi + t.lo) : 0.0f;
-        pb[e] = ex2(minus(block_end, t));
+        pb[e] = factors ? scale * ex2(minus(t, end)) : 1.0f;
     }
     reinterpret_cast<float4*>(g.hi)[lane] = hi, reinterpret_cast<float4*>(g.lo)[lane] = lo, reinterpret_cast<float4*>(g.w)[lane] = w;
-    reinterpret_cast<float4*>(g.eg)[lane] = eg, reinterpret_cast<float4*>(g.end)[lane] = be, reinterpret_cast<int4*>(g.seg)[lane] = seg;
+    reinterpret_cast<float4*>(g.eg)[lane] = eg, reinterpret_cast<float4*>(g.row)[lane] = be, reinterpret_cast<int4*>(g.seg)[lane] = seg;
     wild = __any_sync(0xffffffffu, wild);
-    if (lane == 0) g.d = send == 0 ? ex2(end.hi + end.lo) : -1.0f, g.wild = wild ? 1 : 0;
+    if (lane == 0) g.d = send == 0 ? ex2(end.hi + end.lo) : -1.0f, g.wild = wild ? 1 : 0, g.factors = factors ? 1 : 0;
 }
 
 // One lane of a warp: a chunk's 128 rows of one tensor, 64 columns at a time.
@@ -306,7 +314,7 @@ __global__ void __launch_bounds__(kThreads, 1) umma_attention_kernel(const __gri
             const int quad = warp & 3, half = warp >> 2, r = 32 * quad + lane;
             __nv_bfloat16* const out = static_cast<__nv_bfloat16*>(p.out) + b * p.ob + h * p.oh + col0 + 32 * half;
             const int cols = p.dv - col0 - 32 * half;
-            float eg_last = 0.0f;  // of the chunk whose outputs come next
+            float eg_last = 0.0f, row_last = 0.0f;  // of the chunk whose outputs come next
             auto outputs = [&](int c) {  // 32 columns of chunk c
                 wait(o_done + (c & 1), c >> 1);
                 wait(qs_done + (c & 1), c >> 1);
@@ -320,51 +328,53 @@ __global__ void __launch_bounds__(kThreads, 1) umma_attention_kernel(const __gri
                 const int64_t t = first + int64_t(c) * CT + r;
                 __nv_bfloat16* const to = out + t * p.ot;
 #pragma unroll
-                for (int e = 0; e < 32; e += 8) {
-                    uint32_t w[4];
+                for (int e = 0; e < 32; e += 16) {
+                    uint32_t w[8];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        float2 z = make_float2(x[e + 2 * i], x[e + 2 * i + 1]);
+                    for (int i = 0; i < 8; ++i) {
+                        float2 z = __fmul2_rn(splat(row_last), make_float2(x[e + 2 * i], x[e + 2 * i + 1]));
                         if (eg_last >= 0.0f) z = __ffma2_rn(splat(eg_last), make_float2(y[e + 2 * i], y[e + 2 * i + 1]), z);
                         w[i] = pack_bf16(z.x, z.y);
                     }
-                    if (t < p.T && e < cols) *reinterpret_cast<uint4*>(to + e) = make_uint4(w[0], w[1], w[2], w[3]);
+                    if (t >= p.T) continue;
+                    if (up.wide && e + 16 <= cols) {
+                        asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(to + e), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]),
+                                     "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                                     : "memory");
+                    } else {
+                        if (e < cols) *reinterpret_cast<uint4*>(to + e) = make_uint4(w[0], w[1], w[2], w[3]);
+                        if (e + 8 < cols) *reinterpret_cast<uint4*>(to + e + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+                    }
                 }
             };
 #pragma unroll 1
             for (int c = 0; c <= n; ++c) {  // P' of chunk c, the outputs of the one before it
-                float eg = 0.0f;  // of the chunk; below 0: the entering state does not reach the row
+                float eg = 0.0f, row = 0.0f;  // of the chunk; eg below 0: the entering state does not reach the row
                 if (c < n) {
                 const Gates& g = gates[c % GR];
                 wait(gates_full + c % GR, c / GR);
-                const float hr = g.hi[r], lr = g.lo[r];
-                eg = g.seg[r] == 0 ? g.eg[r] : -1.0f;
-                const bool resets = g.d == -1.0f;
-                const bool steep = resets || !(g.hi[32 * quad] - g.hi[32 * quad + 31] < 80.0f);  // the factors leave the range
+                eg = g.seg[r] == 0 ? g.eg[r] : -1.0f, row = g.row[r];
+                const bool factors = g.factors != 0;
                 wait(qk_done + (c & 1), c >> 1);
                 umma::fence_after_sync();
                 const uint32_t tp = tmem + M::T_P + 128 * (c % NP) + lanes;
                 // 16 columns at a time, every other one, two of them in flight; after the diagonal's they are 0
                 auto scores = [&](int cb, float (&x)[16]) {
                     uint32_t pl[16];  // the first planes of 16 scores, then the second
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) pl[e] = 0u;
                     if (cb < 2 * quad + 2) {
-                        const int i32 = 16 * cb | 31;
-                        const float f = p.scale * ex2((hr - g.hi[i32]) + (lr - g.lo[i32]));  // from the end of the columns' 32 on
-                        if (cb >= 2 * quad ? !steep : !resets) {
-                            const float2 ff = splat(f);
+                        if (factors) {
 #pragma unroll
                             for (int e = 0; e < 16; e += 4) {
-                                const float4 end = *reinterpret_cast<const float4*>(&g.end[16 * cb + e]);
-                                const float2 u = __fmul2_rn(make_float2(x[e], x[e + 1]), __fmul2_rn(make_float2(end.x, end.y), ff));
-                                const float2 d = __fmul2_rn(make_float2(x[e + 2], x[e + 3]), __fmul2_rn(make_float2(end.z, end.w), ff));
+                                const float4 w = *reinterpret_cast<const float4*>(&g.w[16 * cb + e]);
+                                const float2 u = __fmul2_rn(make_float2(x[e], x[e + 1]), make_float2(w.x, w.y));
+                                const float2 d = __fmul2_rn(make_float2(x[e + 2], x[e + 3]), make_float2(w.z, w.w));
                                 x[e] = u.x, x[e + 1] = u.y, x[e + 2] = d.x, x[e + 3] = d.y;
                             }
                             if (cb >= 2 * quad)
 #pragma unroll
                                 for (int e = 0; e < 16; ++e) x[e] = 16 * cb + e <= r ? x[e] : 0.0f;
                         } else {
+                            const float hr = g.hi[r], lr = g.lo[r];
                             const int sr = g.seg[r];
 #pragma unroll
                             for (int e = 0; e < 16; ++e) {
@@ -378,6 +388,9 @@ __global__ void __launch_bounds__(kThreads, 1) umma_attention_kernel(const __gri
                             split<2>(make_float2(x[2 * e], x[2 * e + 1]), two);
                             pl[e] = two[0], pl[8 + e] = two[1];
                         }
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) pl[e] = 0u;
                     }
                     tmem_st16(tp + 16 * cb, pl);
                 };
@@ -396,7 +409,7 @@ __global__ void __launch_bounds__(kThreads, 1) umma_attention_kernel(const __gri
                 arrive(gates_free + c % GR);
                 }
                 if (c > 0) outputs(c - 1);
-                eg_last = eg;
+                eg_last = eg, row_last = row;
             }
         }
     } else if (warp < 16) {
@@ -713,6 +726,7 @@ int umma_run(const AttnParams& p, int64_t nb, bool state, uint32_t* redo, cudaSt
     if (int rc = ensure_context()) return rc;
     UmmaParams up{};
     up.a = p, up.redo = redo, up.polls = umma_polls.load(std::memory_order_relaxed);
+    up.wide = reinterpret_cast<uintptr_t>(p.out) % 32 == 0 && p.ob % 16 == 0 && p.ot % 16 == 0 && p.oh % 16 == 0;
     if (int rc = encode(&up.q, p.q, nb, p.T, p.H / p.q.share, p.dk)) return rc;
     if (int rc = encode(&up.k, p.k, nb, p.T, p.H / p.k.share, p.dk)) return rc;
     if (int rc = encode(&up.v, p.v, nb, p.T, p.H / p.v.share, p.dv)) return rc;
