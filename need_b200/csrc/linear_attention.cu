@@ -657,16 +657,29 @@ struct Plan {
     int64_t chains, chunks, blocks;
     int32_t slices, nseg, seg_chunks;
 };
-// Where there are few chains they are cut into segments, as many as the GPU holds at once: one
-// CTA a multiprocessor (umma), 2 or 3 of attention_kernel.
-Plan plan(bool umma, int64_t nb, int64_t T, int64_t H, int64_t dk, int64_t dv) {
+// CTAs of attention_kernel that a multiprocessor holds (registers for 3, 227 KB).
+template <typename T>
+constexpr int held(bool small) {
+    const int bytes = (small ? Layout<T, 64, true>::BYTES : Layout<T, 128, true>::BYTES) + 1024;
+    return std::min(3, 227 * 1024 / bytes);
+}
+// Where there are few chains they are cut into segments, as many as the GPU holds at once (of
+// umma's CTAs one a multiprocessor): all but the last are run for the state that they leave
+// (four fifths of a chunk's time), a launch joins those, then all are run for the outputs.  That is worth it where it saves more chunks in a row than the two more
+// launches cost (a chunk of attention_kernel's, five of umma's 128 tokens).  Uncut and cut:
+// 4 bf16 chains of 64 features 14.3 and 18.2 us at 512 tokens, 22.3 and 18.8 at 1024; 4
+// fp32 ones 20.5 and 20.6 at 128 tokens, 30 and 21 at 192; 52 bf16 ones in two segments 71
+// and 74 at 4096.
+Plan plan(bool umma, int32_t dtype, int64_t nb, int64_t T, int64_t H, int64_t dk, int64_t dv) {
     Plan pl{};
     pl.umma = umma;
     pl.chains = nb * H, pl.chunks = (T + C - 1) / C, pl.slices = int32_t((dv + DV - 1) / DV);
-    const int64_t ctas = std::max<int64_t>(1, pl.chains * pl.slices), places = umma ? 148 : dk <= 64 ? 444 : 296;
-    int64_t nseg = std::max<int64_t>(1, std::min(places / ctas, pl.chunks / 4));
-    pl.seg_chunks = int32_t((pl.chunks + nseg - 1) / nseg);
-    if (umma) pl.seg_chunks += pl.seg_chunks & 1;
+    const bool small = dk <= 64;
+    const int64_t ctas = std::max<int64_t>(1, pl.chains * pl.slices), unit = umma ? 2 : 1, chunks = (pl.chunks + unit - 1) / unit;
+    const int64_t places = 148 * (umma ? 1 : dtype == NEED_F32 ? held<float>(small) : dtype == NEED_BF16 ? held<__nv_bfloat16>(small) : held<__half>(small));
+    const int64_t nseg = std::max<int64_t>(1, std::min(places / ctas, chunks)), seg = (chunks + nseg - 1) / nseg;
+    const bool cut = 18 * seg + (umma ? 50 : 10) <= 10 * chunks;
+    pl.seg_chunks = int32_t(cut ? seg * unit : chunks * unit);
     pl.nseg = int32_t((pl.chunks + pl.seg_chunks - 1) / pl.seg_chunks);
     pl.blocks = pl.chains * pl.slices * pl.nseg;
     return pl;
@@ -714,8 +727,8 @@ extern "C" {
 
 size_t need_linear_attention_workspace_size(int32_t dtype, int64_t nb, int64_t T, int64_t H, int64_t dk, int64_t dv) {
     if (!dtype_ok(dtype) || nb < 1 || T < 1 || H < 1 || dk < 1 || dv < 1) return 16;
-    size_t n = workspace_of(plan(false, nb, T, H, dk, dv), dk, dv);
-    if (dtype == NEED_BF16) n = std::max(n, workspace_of(plan(true, nb, T, H, dk, dv), dk, dv));
+    size_t n = workspace_of(plan(false, dtype, nb, T, H, dk, dv), dk, dv);
+    if (dtype == NEED_BF16) n = std::max(n, workspace_of(plan(true, dtype, nb, T, H, dk, dv), dk, dv));
     return n;
 }
 
@@ -755,7 +768,8 @@ int need_linear_attention(const need_linear_attention_args* a, need_stream_t str
     p.out = a->out, p.ob = a->out_stride_b, p.ot = a->out_stride_t, p.oh = a->out_stride_h;
     p.T = a->T, p.H = int32_t(a->H), p.dk = int32_t(a->dk), p.dv = int32_t(a->dv);
     p.scale = a->scale;
-    const Plan pl = plan(vec && a->dtype == NEED_BF16 && a->T > C && umma_takes(p, a->nb), a->nb, a->T, a->H, a->dk, a->dv);
+    const Plan pl = plan(vec && a->dtype == NEED_BF16 && a->T > C && umma_takes(p, a->nb), a->dtype, a->nb, a->T, a->H,
+                         a->dk, a->dv);
     if ((pl.nseg > 1 || pl.umma) && (a->workspace == nullptr || (reinterpret_cast<uintptr_t>(a->workspace) & 3u) != 0 ||
                                      a->workspace_bytes < workspace_of(pl, a->dk, a->dv)))
         return fail(NEED_ERR_WORKSPACE, "linear attention: workspace missing, misaligned or too small");
