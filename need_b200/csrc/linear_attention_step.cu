@@ -4,14 +4,15 @@
 //   S = a S + k^T v,   out = scale q S,   a = exp(log_decay)
 //
 // in fp32, the states in place in a pool.  The state is read and written once, 8 B per
-// element: that is all the traffic that counts, so the kernel is bound by HBM.  One CTA
-// per (sequence, head, up to 128 columns): a thread owns 4 columns (16 bytes) of every
-// R-th row, its rows' loads in flight together, and the row groups' parts of q S are added
-// in a fixed order.
+// element: that is all the traffic that counts, so the kernel is bound by HBM.  A team of
+// threads takes a (sequence, head, up to 128 columns): a thread owns 4 columns (16 bytes) of
+// every R-th row, its rows' loads in flight together, and the row groups' parts of q S are
+// added in a fixed order.  A CTA is 1 to 4 teams, heads of one sequence.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "host_common.h"
 #include "need_scan.h"
@@ -20,7 +21,8 @@ using namespace need;
 
 namespace {
 
-constexpr int kThreads = 128, kCols = 128;  // columns of a CTA
+constexpr int kThreads = 128, kMaxThreads = 512, kCols = 128;  // columns of a team
+constexpr int kRows = 8;                                          // of a thread in flight
 
 struct StepParams {
     need_heads q, k, v;
@@ -31,7 +33,7 @@ struct StepParams {
     const int32_t* slot;
     void* out;
     int64_t on, oh;
-    int32_t H, dk, dv, groups;  // groups: of columns in a CTA, a power of two
+    int32_t H, dk, dv, groups;  // groups: of a team's columns, a power of two
     float scale;
 };
 
@@ -45,36 +47,29 @@ __device__ __forceinline__ const T* row_of(const need_heads& x, int64_t n, int h
 }
 
 // VEC: rows of the state in whole, aligned groups of 4 columns; else a thread owns one.
-template <typename T, bool VEC>
-__global__ void __launch_bounds__(kThreads) step_kernel(const StepParams p) {
-    constexpr int W = VEC ? 4 : 1, B = 8;  // columns of a thread, rows in flight
-    extern __shared__ float sh[];          // k, q, then the row groups' sums
-    const int64_t n = blockIdx.x / p.H;
-    const int h = static_cast<int>(blockIdx.x % p.H), tid = threadIdx.x;
-    const int rows = kThreads / p.groups, r0 = tid / p.groups, j = blockIdx.y * (p.groups * W) + (tid % p.groups) * W;
-    const bool mine = j < p.dv;
+// TEAMS of a CTA.
+template <typename T, bool VEC, int TEAMS>
+__global__ void __launch_bounds__(TEAMS == 1 ? kMaxThreads : kThreads) step_kernel(const StepParams p) {
+    constexpr int W = VEC ? 4 : 1, B = kRows;  // columns of a thread
+    extern __shared__ float smem[];        // of each team k, q, then the row groups' sums
+    const int threads = TEAMS == 1 ? blockDim.x : kThreads / TEAMS;
+    const int tid = TEAMS == 1 ? threadIdx.x : threadIdx.x % (kThreads / TEAMS), team = TEAMS == 1 ? 0 : threadIdx.x / (kThreads / TEAMS);
+    const int per = (p.H + TEAMS - 1) / TEAMS;  // CTAs of a sequence
+    const int64_t n = blockIdx.x / per;
+    const int h0 = static_cast<int>(blockIdx.x % per) * TEAMS + team, h = TEAMS == 1 || h0 < p.H ? h0 : p.H - 1;
+    float* const sh = smem + team * (2 * p.dk + threads * W);
+    const int rows = threads / p.groups, r0 = tid / p.groups, j = blockIdx.y * (p.groups * W) + (tid % p.groups) * W;
+    const bool mine = (TEAMS == 1 || h0 < p.H) && j < p.dv;
     const int64_t where = p.slot != nullptr ? p.slot[n] : n;
     T* const out = static_cast<T*>(p.out) + n * p.on + h * p.oh;
     bool taken = where >= p.slots;
     if (p.slot != nullptr && where >= 0)
-        for (int64_t m = tid; m < n; m += kThreads) taken |= p.slot[m] == where;
+        for (int64_t m = threadIdx.x; m < n; m += blockDim.x) taken |= p.slot[m] == where;
     const T *k = row_of<T>(p.k, n, h, p.H), *q = row_of<T>(p.q, n, h, p.H), *v = row_of<T>(p.v, n, h, p.H);
-    for (int i = tid; i < p.dk; i += kThreads) sh[i] = to_float(k[i]), sh[p.dk + i] = to_float(q[i]);
-    if (__syncthreads_or(taken) || where < 0) {
-        if (r0 == 0)
-            for (int e = 0; e < W; ++e)
-                if (mine) out[j + e] = static_cast<T>(where < 0 ? 0.0f : __int_as_float(0x7fc00000));
-        return;
-    }
     const float x = p.ld[n * p.ln + h * p.lh];
-    const bool reset = x == -INFINITY;
-    const float a = expf(x);
     float* const s = p.state + where * p.ss + h * (int64_t(p.dk) * p.dv) + j;
-    float vj[W], o[W];
-#pragma unroll
-    for (int e = 0; e < W; ++e) vj[e] = mine ? to_float(v[j + e]) : 0.0f, o[e] = 0.0f;
-    for (int i0 = r0; i0 < p.dk; i0 += rows * B) {
-        float u[B][W];
+    float vj[W], o[W], u[B][W];
+    auto load = [&](int i0) {
 #pragma unroll
         for (int b = 0; b < B; ++b) {
             const int i = i0 + b * rows;
@@ -87,6 +82,21 @@ __global__ void __launch_bounds__(kThreads) step_kernel(const StepParams p) {
                 }
             }
         }
+    };
+    if (where >= 0 && where < p.slots) load(r0);  // not kept where the slot turns out to be taken
+#pragma unroll
+    for (int e = 0; e < W; ++e) vj[e] = mine ? to_float(v[j + e]) : 0.0f, o[e] = 0.0f;
+    for (int i = tid; i < p.dk; i += threads) sh[i] = to_float(k[i]), sh[p.dk + i] = to_float(q[i]);
+    if (__syncthreads_or(taken) || where < 0) {
+        if (r0 == 0)
+            for (int e = 0; e < W; ++e)
+                if (mine) out[j + e] = static_cast<T>(where < 0 ? 0.0f : __int_as_float(0x7fc00000));
+        return;
+    }
+    const bool reset = x == -INFINITY;
+    const float a = expf(x);
+    for (int i0 = r0; i0 < p.dk; i0 += rows * B) {
+        if (i0 != r0) load(i0);
 #pragma unroll
         for (int b = 0; b < B; ++b) {
             const int i = i0 + b * rows;
@@ -107,9 +117,9 @@ __global__ void __launch_bounds__(kThreads) step_kernel(const StepParams p) {
     for (int e = 0; e < W; ++e) red[(r0 * p.groups + tid % p.groups) * W + e] = o[e];
     __syncthreads();
     const int cols = p.groups * W;
-    for (int c = tid; c < cols; c += kThreads) {
+    for (int c = tid; c < cols; c += threads) {
         const int jc = blockIdx.y * cols + c;
-        if (jc >= p.dv) break;
+        if (jc >= p.dv || (TEAMS > 1 && h0 >= p.H)) break;
         float sum = 0.0f;
         for (int r = 0; r < rows; ++r) sum += red[r * cols + c];
         out[jc] = static_cast<T>(p.scale * sum);
@@ -146,14 +156,28 @@ extern "C" int need_linear_attention_step(const need_linear_attention_step_args*
     const int64_t need = (std::min<int64_t>(a->dv, kCols) + w - 1) / w;
     p.groups = 1;
     while (p.groups < need) p.groups *= 2;
+    // Where the threads of all states fit the GPU at once, a state's rows are in flight at
+    // once (3 of 8 heads of 128 x 96 in fp16 take 512 threads each 4.7 us, 128 each 6.7;
+    // but 16 of 32 of 128 x 128 15.9 and 9.8).  Small states share a CTA.
+    const int64_t states = a->n * a->H, rows = (a->dk + kRows - 1) / kRows;  // threads that a column group can use
+    int threads = kThreads;
+    while (threads < kMaxThreads && threads < p.groups * rows && states * threads * 2 <= 148 * kMaxThreads) threads *= 2;
+    int teams = 1;
+    while (teams < 4 && teams < a->H && threads == kThreads && threads / teams / 2 >= std::max<int64_t>(32, p.groups * rows)) teams *= 2;
     const int64_t cols = int64_t(p.groups) * w, tiles = (a->dv + cols - 1) / cols;
     if (tiles > 65535) return fail(NEED_ERR_UNSUPPORTED, "linear attention step: dv out of range");
-    const dim3 grid(static_cast<unsigned>(a->n * a->H), static_cast<unsigned>(tiles));
-    const size_t bytes = (2 * a->dk + kThreads * w) * sizeof(float);
+    const dim3 grid(static_cast<unsigned>(a->n * ((a->H + teams - 1) / teams)), static_cast<unsigned>(tiles));
+    const size_t bytes = (teams * 2 * a->dk + threads * w) * sizeof(float);
     auto go = [&](auto tag) {
         using T = decltype(tag);
-        if (vec) step_kernel<T, true><<<grid, kThreads, bytes, stream>>>(p);
-        else step_kernel<T, false><<<grid, kThreads, bytes, stream>>>(p);
+        auto launch = [&](auto v) {
+            constexpr bool V = decltype(v)::value;
+            if (teams == 1) step_kernel<T, V, 1><<<grid, threads, bytes, stream>>>(p);
+            else if (teams == 2) step_kernel<T, V, 2><<<grid, threads, bytes, stream>>>(p);
+            else step_kernel<T, V, 4><<<grid, threads, bytes, stream>>>(p);
+        };
+        if (vec) launch(std::true_type{});
+        else launch(std::false_type{});
     };
     if (a->dtype == NEED_F32) go(float{});
     else if (a->dtype == NEED_BF16) go(__nv_bfloat16{});

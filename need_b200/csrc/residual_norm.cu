@@ -70,6 +70,21 @@ __device__ __forceinline__ void store_piece(T* p, int n, const uint4& u) {
     }
 }
 
+// The weights of a piece's N channels, of which the first n are there.
+template <bool VEC, int N>
+__device__ __forceinline__ void load_weights(const float* w, int n, float (&f)[N]) {
+    if constexpr (VEC) {
+#pragma unroll
+        for (int e = 0; e < N; e += 4) {
+            const float4 u = __ldg(reinterpret_cast<const float4*>(w + e));
+            f[e] = u.x, f[e + 1] = u.y, f[e + 2] = u.z, f[e + 3] = u.w;
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < N; ++e) f[e] = e < n ? __ldg(w + e) : 0.0f;
+    }
+}
+
 // blockDim = 32 * wpr * (rows per block); lane l of a row's warp w holds pieces
 // (w * 32 + l) + k * 32 * wpr.  OUT8: the output in 8 bits.
 template <typename T, int NP, bool VEC, bool OUT8>
@@ -122,12 +137,12 @@ __global__ void __launch_bounds__(512) residual_norm_kernel(const ResidualParams
             const int i = l0 + k * step;
             if (!live || i >= nvec) continue;
             P* a = reinterpret_cast<P*>(&u[k]);
+            float w[N];
+            load_weights<VEC>(p.w + i * N, p.C - i * N, w);
 #pragma unroll
             for (int e = 0; e < N / 2; ++e) {
-                const int c = i * N + 2 * e;
                 const float2 f = widen(a[e]);
-                const float wx = VEC || c < p.C ? __ldg(p.w + c) : 0.0f, wy = VEC || c + 1 < p.C ? __ldg(p.w + c + 1) : 0.0f;
-                a[e] = Ops<T>::pack(f.x * inv * wx, f.y * inv * wy);
+                a[e] = Ops<T>::pack(f.x * inv * w[2 * e], f.y * inv * w[2 * e + 1]);
             }
             store_piece<T, VEC>(static_cast<T*>(p.out) + row * p.os + i * N, p.C - i * N, u[k]);
         }
@@ -139,14 +154,16 @@ __global__ void __launch_bounds__(512) residual_norm_kernel(const ResidualParams
         for (int k = 0; k < NP; ++k) {
             const int i = l0 + k * step;
             const P* a = reinterpret_cast<const P*>(&u[k]);
+            const bool mine = live && i < nvec;
+            float w[N] = {};
+            if (mine) load_weights<VEC>(p.w + i * N, p.C - i * N, w);
             top[k] = 0;
 #pragma unroll
             for (int e = 0; e < N / 2; ++e) {
-                const int c = i * N + 2 * e;
                 const float2 f = widen(a[e]);
-                const bool in0 = live && (VEC ? i < nvec : c < p.C), in1 = live && (VEC ? i < nvec : c + 1 < p.C);
-                n[k][e].x = in0 ? f.x * inv * __ldg(p.w + c) : 0.0f;
-                n[k][e].y = in1 ? f.y * inv * __ldg(p.w + c + 1) : 0.0f;
+                const bool in0 = mine && (VEC || i * N + 2 * e < p.C), in1 = mine && (VEC || i * N + 2 * e + 1 < p.C);
+                n[k][e].x = in0 ? f.x * inv * w[2 * e] : 0.0f;
+                n[k][e].y = in1 ? f.y * inv * w[2 * e + 1] : 0.0f;
                 top[k] = max(top[k], max(__float_as_uint(n[k][e].x) & 0x7fffffffu, __float_as_uint(n[k][e].y) & 0x7fffffffu));
             }
             all = max(all, top[k]);
@@ -228,7 +245,7 @@ extern "C" int need_residual_rms_norm(const need_residual_norm_args* a, need_str
     auto al = [&](const void* q, int64_t stride, int bytes) {
         return reinterpret_cast<uintptr_t>(q) % bytes == 0 && (a->rows == 1 || stride * (q == a->out && a->out8 ? 1 : es) % bytes == 0);
     };
-    const bool vec = a->C % n == 0 && al(p.x, p.xs, 16) && al(p.y, p.ys, 16) && al(p.stream, p.ss, 16) &&
+    const bool vec = a->C % n == 0 && aligned16(a->weight) && al(p.x, p.xs, 16) && al(p.y, p.ys, 16) && al(p.stream, p.ss, 16) &&
                      al(p.out, p.os, a->out8 ? n : 16);
     auto run = [&](auto tag) {
         using T = decltype(tag);

@@ -118,6 +118,14 @@ def test_attention_few_chains(cuda, B, T, H, dk, dv, dtype, resets):
     check_attention(q, k, v, ld, dk ** -0.5, seg, s0)
 
 
+@pytest.mark.parametrize("dtype", [BF, HF, F32])
+@pytest.mark.parametrize("T", [129, 192, 193, 320, 900, 1024])
+def test_attention_short_parts(cuda, T, dtype):
+    """Down to a chunk each, the last one short."""
+    q, k, v, ld, seg, s0 = make(cuda, 1, T, 2, 64, 64, dtype, state=True, resets=150)
+    check_attention(q, k, v, ld, 0.125, seg, s0)
+
+
 def test_attention_parts_and_batches_agree(cuda):
     """One sequence alone (cut into parts) and among many (not cut): the same but for fp32 sums."""
     q, k, v, ld, _, _ = make(cuda, 1, 2048, 2, 64, 64, F32, decay="head")
@@ -279,6 +287,27 @@ def test_step(cuda, N, H, dk, dv, heads, dtype):
     again = before[slot.long()].clone()
     out2 = nk.linear_attention_step(q[:, 0], k[:, 0], v[:, 0], ld[:, 0], again, scale=0.3)
     assert torch.equal(out2, out) and torch.equal(again, pool[slot.long()])
+
+
+@pytest.mark.parametrize("N,H,dk,dv", [(3, 5, 16, 16), (2, 3, 32, 64), (4, 7, 9, 5), (600, 2, 128, 128)])
+def test_step_shared_blocks(cuda, N, H, dk, dv):
+    """Small states, some heads of a sequence side by side; slots of none, twice and past the pool among them."""
+    q, k, v, ld, _, _ = make(cuda, N, 1, H, dk, dv, BF)
+    pool = torch.randn(N, H, dk, dv, device=cuda)
+    before = pool.clone()
+    slot = torch.arange(N, device=cuda, dtype=torch.int32)
+    slot[1] = -1
+    if N > 2:
+        slot[2] = 0
+    if N > 3:
+        slot[3] = N
+    out = nk.linear_attention_step(q[:, 0], k[:, 0], v[:, 0], ld[:, 0], pool, slot=slot)
+    want, s, mag, m = ref.attention(q, k, v, ld, 1.0, None, before)
+    good = [0] + list(range(4, N))
+    close(out[good, None], want[good], mag[good], 2.0 ** -18, ref.HALF_STEP[BF])
+    close(pool[good], s[good], m[good], 2.0 ** -21)
+    assert torch.equal(pool[1:4], before[1:4])
+    assert (out[1] == 0).all() and torch.isnan(out[2:4]).all()
 
 
 def test_step_slots(cuda):
@@ -461,6 +490,13 @@ def test_logp(cuda, N, V, top, dtype):
     x, t = logits_of(cuda, N, V, dtype, N + V)
     check_logp(x, t, top=top)
     check_logp(x, t.int(), temperature=0.6)
+
+
+@pytest.mark.parametrize("N,V,top,dtype", [(700, 20001, 9, BF), (600, 70001, 20, F32), (310, 9000, 32, HF), (4096, 300, 17, BF), (1, 1 << 21, 32, BF)])
+def test_logp_many(cuda, N, V, top, dtype):
+    """Rows uncut and cut, many pieces of a thread, blocks for short rows."""
+    x, t = logits_of(cuda, N, V, dtype, N + V)
+    check_logp(x, t, top=top)
 
 
 @pytest.mark.parametrize("V", [100, 784, 5001, 70000])
