@@ -134,51 +134,52 @@ struct Layout {
 };
 
 // ------------------------------------------------------------------ loads
-// 8 values of a row from column `col` on; 0 outside the tensor.
-template <typename T, bool VEC>
-__device__ __forceinline__ void load8(const T* row, int col, int cols, bool live, float (&f)[8]) {
-    if constexpr (VEC) {
-        constexpr int N = 16 / sizeof(T);
-#pragma unroll
-        for (int h = 0; h < 8 / N; ++h) {
-            uint4 u = make_uint4(0, 0, 0, 0);
-            if (live && col + h * N < cols) u = *reinterpret_cast<const uint4*>(row + col + h * N);
-            const T* x = reinterpret_cast<const T*>(&u);
-#pragma unroll
-            for (int e = 0; e < N; ++e) f[h * N + e] = to_float(x[e]);
-        }
-    } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) f[e] = live && col + e < cols ? to_float(row[col + e]) : 0.0f;
-    }
-}
-
-// Rows [t0, t0 + C) of one tensor into its planes; true where a value is not finite
-// (or too near the largest to be rounded).
+// Rows [t0, t0 + C) of one tensor into its planes, 8 values of a thread at a time.  All of
+// a thread's loads are issued before the first is split: one after another they cost a
+// fp16 chunk 4 us.
 template <typename T, int COLS, bool VEC>
-__device__ __forceinline__ bool load_planes(char* dst, const T* base, int64_t st, int64_t t0, int64_t T_, int col0,
-                                            int cols) {
-    constexpr int IN = Split<T>::IN, PIECES = COLS / 8;
-    float chk = 0.0f;
-    for (int n = threadIdx.x; n < C * PIECES; n += kThreads) {
-        const int row = n / PIECES, piece = n % PIECES;
-        float f[8];
-        load8<T, VEC>(base + (t0 + row) * st, col0 + piece * 8, cols, t0 + row < T_, f);
-        uint32_t pl[4][IN];
+struct Loader {
+    static constexpr int IN = Split<T>::IN, PIECES = COLS / 8, N = C * PIECES / kThreads;
+    static constexpr int W = VEC ? 8 * static_cast<int>(sizeof(T)) / 16 : 8;
+    using Raw = typename std::conditional<VEC, uint4, T>::type;
+    Raw raw[N][W];
+
+    __device__ __forceinline__ void load(const T* base, int64_t st, int64_t t0, int64_t T_, int col0, int cols) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            split<IN>(make_float2(f[2 * e], f[2 * e + 1]), pl[e]);
-            // of a value that rounds to an infinity the first plane is one
-            chk = fmaf(__uint_as_float(pl[e][0] << 16), 0.0f, chk);
-            chk = fmaf(__uint_as_float(pl[e][0] & 0xffff0000u), 0.0f, chk);
+        for (int i = 0; i < N; ++i) {
+            const int n = i * kThreads + threadIdx.x, row = n / PIECES, col = col0 + (n % PIECES) * 8;
+            const T* from = base + (t0 + row) * st + col;
+#pragma unroll
+            for (int w = 0; w < W; ++w) {
+                const bool live = t0 + row < T_ && col + w * (8 / W) < cols;
+                if constexpr (VEC) raw[i][w] = live ? __ldg(reinterpret_cast<const uint4*>(from) + w) : make_uint4(0, 0, 0, 0);
+                else raw[i][w] = live ? from[w] : T(0.0f);
+            }
         }
-#pragma unroll
-        for (int p = 0; p < IN; ++p)
-            *reinterpret_cast<uint4*>(dst + p * C * COLS * 2 + at(row, piece)) =
-                make_uint4(pl[0][p], pl[1][p], pl[2][p], pl[3][p]);
     }
-    return !(chk == 0.0f);
-}
+    // true where a value is not finite (or too near the largest to be rounded)
+    __device__ __forceinline__ bool store(char* dst) const {
+        float chk = 0.0f;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int n = i * kThreads + threadIdx.x, row = n / PIECES, piece = n % PIECES;
+            const T* x = reinterpret_cast<const T*>(&raw[i][0]);
+            uint32_t pl[4][IN];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                split<IN>(make_float2(to_float(x[2 * e]), to_float(x[2 * e + 1])), pl[e]);
+                // of a value that rounds to an infinity the first plane is one
+                chk = fmaf(__uint_as_float(pl[e][0] << 16), 0.0f, chk);
+                chk = fmaf(__uint_as_float(pl[e][0] & 0xffff0000u), 0.0f, chk);
+            }
+#pragma unroll
+            for (int p = 0; p < IN; ++p)
+                *reinterpret_cast<uint4*>(dst + p * C * COLS * 2 + at(row, piece)) =
+                    make_uint4(pl[0][p], pl[1][p], pl[2][p], pl[3][p]);
+        }
+        return !(chk == 0.0f);
+    }
+};
 
 // The same of bf16 rows by asynchronous copies of 16 bytes.  A thread copies one piece of
 // every 16th row (of 64 columns), or of every 8th (of 128).
@@ -356,10 +357,17 @@ __global__ void __launch_bounds__(kThreads, DK == 64 && Split<T>::IN < 3 ? 3 : 2
             cp_wait_all();
             bad = check_rows<DK>(buf + L::K) | check_rows<DV>(buf + L::V);
         } else {
+            // K and V together, then Q: that many registers
+            Loader<T, DK, VEC> lk;
+            Loader<T, DV, VEC> lv;
+            lk.load(k, p.k.st, t0, p.T, 0, p.dk), lv.load(v, p.v.st, t0, p.T, col0, p.dv);
             __syncthreads();  // the chunk before this one has been read
-            if (!STATE) load_planes<T, DK, VEC>(buf + L::Q, q, p.q.st, t0, p.T, 0, p.dk);
-            bad = load_planes<T, DK, VEC>(buf + L::K, k, p.k.st, t0, p.T, 0, p.dk);
-            bad |= load_planes<T, DV, VEC>(buf + L::V, v, p.v.st, t0, p.T, col0, p.dv);
+            bad = lk.store(buf + L::K) | lv.store(buf + L::V);
+            if (!STATE) {
+                Loader<T, DK, VEC> lq;
+                lq.load(q, p.q.st, t0, p.T, 0, p.dk);
+                lq.store(buf + L::Q);
+            }
         }
         bad = __syncthreads_or(bad | wild);  // the chunk and its decays are there
         const Decays& gt = gates[c & 1];
