@@ -357,17 +357,15 @@ __global__ void __launch_bounds__(kThreads, DK == 64 && Split<T>::IN < 3 ? 3 : 2
             cp_wait_all();
             bad = check_rows<DK>(buf + L::K) | check_rows<DV>(buf + L::V);
         } else {
-            // K and V together, then Q: that many registers
-            Loader<T, DK, VEC> lk;
+            constexpr bool ALL = DK == 64 || S::IN < 3;  // else the registers hold K and V only
+            Loader<T, DK, VEC> lk, lq;
             Loader<T, DV, VEC> lv;
             lk.load(k, p.k.st, t0, p.T, 0, p.dk), lv.load(v, p.v.st, t0, p.T, col0, p.dv);
+            if (!STATE && ALL) lq.load(q, p.q.st, t0, p.T, 0, p.dk);
             __syncthreads();  // the chunk before this one has been read
             bad = lk.store(buf + L::K) | lv.store(buf + L::V);
-            if (!STATE) {
-                Loader<T, DK, VEC> lq;
-                lq.load(q, p.q.st, t0, p.T, 0, p.dk);
-                lq.store(buf + L::Q);
-            }
+            if (!STATE && !ALL) lq.load(q, p.q.st, t0, p.T, 0, p.dk);
+            if (!STATE) lq.store(buf + L::Q);
         }
         bad = __syncthreads_or(bad | wild);  // the chunk and its decays are there
         const Decays& gt = gates[c & 1];
@@ -673,11 +671,12 @@ constexpr int held(bool small) {
 }
 // Where there are few chains they are cut into segments, as many as the GPU holds at once (of
 // umma's CTAs one a multiprocessor): all but the last are run for the state that they leave
-// (four fifths of a chunk's time), a launch joins those, then all are run for the outputs.  That is worth it where it saves more chunks in a row than the two more
-// launches cost (a chunk of attention_kernel's, five of umma's 128 tokens).  Uncut and cut:
-// 4 bf16 chains of 64 features 14.3 and 18.2 us at 512 tokens, 22.3 and 18.8 at 1024; 4
-// fp32 ones 20.5 and 20.6 at 128 tokens, 30 and 21 at 192; 52 bf16 ones in two segments 71
-// and 74 at 4096.
+// (four fifths of a chunk's time), a launch joins those, then all are run for the outputs.
+// That is worth it where it saves more chunks in a row than the two more launches cost (1.5
+// of attention_kernel's, five of umma's 128 tokens).  Uncut and cut: 4 bf16 chains of 64
+// features 14.3 and 18.2 us at 512 tokens, 22.3 and 18.8 at 1024; 52 in two segments 71 and
+// 74 at 4096; 64 fp16 ones 13.8 and 17.7 at 128 tokens, 24 and 21.6 at 256, 385 and 171 at
+// 4096; 104 fp32 ones of 64 features 521 and 475 at 4096.
 Plan plan(bool umma, int32_t dtype, int64_t nb, int64_t T, int64_t H, int64_t dk, int64_t dv) {
     Plan pl{};
     pl.umma = umma;
@@ -686,7 +685,7 @@ Plan plan(bool umma, int32_t dtype, int64_t nb, int64_t T, int64_t H, int64_t dk
     const int64_t ctas = std::max<int64_t>(1, pl.chains * pl.slices), unit = umma ? 2 : 1, chunks = (pl.chunks + unit - 1) / unit;
     const int64_t places = 148 * (umma ? 1 : dtype == NEED_F32 ? held<float>(small) : dtype == NEED_BF16 ? held<__nv_bfloat16>(small) : held<__half>(small));
     const int64_t nseg = std::max<int64_t>(1, std::min(places / ctas, chunks)), seg = (chunks + nseg - 1) / nseg;
-    const bool cut = 18 * seg + (umma ? 50 : 10) <= 10 * chunks;
+    const bool cut = 18 * seg + (umma ? 50 : 15) <= 10 * chunks;
     pl.seg_chunks = int32_t(cut ? seg * unit : chunks * unit);
     pl.nseg = int32_t((pl.chunks + pl.seg_chunks - 1) / pl.seg_chunks);
     pl.blocks = pl.chains * pl.slices * pl.nseg;
