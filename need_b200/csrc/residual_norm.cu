@@ -70,6 +70,12 @@ __device__ __forceinline__ void store_piece(T* p, int n, const uint4& u) {
     }
 }
 
+// The larger of a (at least 0) and |b|; NaN if one of them is.
+__device__ __forceinline__ float max_abs(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(fabsf(b)));
+    return r;
+}
 // The weights of a piece's N channels, of which the first n are there.
 template <bool VEC, int N>
 __device__ __forceinline__ void load_weights(const float* w, int n, float (&f)[N]) {
@@ -106,7 +112,19 @@ __global__ void __launch_bounds__(512) residual_norm_kernel(const ResidualParams
         u[k] = v[k] = make_uint4(0, 0, 0, 0);
         if (live && i < nvec) u[k] = load_piece<T, VEC>(x + i * N, p.C - i * N), v[k] = load_piece<T, VEC>(y + i * N, p.C - i * N);
     }
-    float ss = 0.0f;
+    // the weights meanwhile, where a lane has at most 16: 64 rows of 832 fp32 channels 2.8 us,
+    // 3.6 with them after the sum; at 32 of them they push rows out of the registers (16384
+    // rows of 832 bf16 channels 18.7 us, 16.9 after the sum)
+    constexpr bool EARLY = NP * N <= 16;
+    float w[NP][N] = {};
+    auto weights = [&](int k) {
+        const int i = l0 + k * step;
+        if (live && i < nvec) load_weights<VEC>(p.w + i * N, p.C - i * N, w[k]);
+    };
+#pragma unroll
+    for (int k = 0; k < NP; ++k)
+        if (EARLY) weights(k);
+    float2 ss2 = make_float2(0.0f, 0.0f);
 #pragma unroll
     for (int k = 0; k < NP; ++k) {
         P* a = reinterpret_cast<P*>(&u[k]);
@@ -116,11 +134,12 @@ __global__ void __launch_bounds__(512) residual_norm_kernel(const ResidualParams
             const float2 r = ffma2(widen(b[e]), splat2(p.scale), widen(a[e]));
             a[e] = Ops<T>::pack(r.x, r.y);
             const float2 f = widen(a[e]);  // the stream as it goes on
-            ss = fmaf(f.x, f.x, ss), ss = fmaf(f.y, f.y, ss);
+            ss2 = ffma2(f, f, ss2);
         }
         const int i = l0 + k * step;
         if (live && i < nvec) store_piece<T, VEC>(static_cast<T*>(p.stream) + row * p.ss + i * N, p.C - i * N, u[k]);
     }
+    float ss = ss2.x + ss2.y;
 #pragma unroll
     for (int m = 16; m >= 1; m >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, m);
     if (p.wpr > 1) {
@@ -137,37 +156,32 @@ __global__ void __launch_bounds__(512) residual_norm_kernel(const ResidualParams
             const int i = l0 + k * step;
             if (!live || i >= nvec) continue;
             P* a = reinterpret_cast<P*>(&u[k]);
-            float w[N];
-            load_weights<VEC>(p.w + i * N, p.C - i * N, w);
+            if (!EARLY) weights(k);
 #pragma unroll
             for (int e = 0; e < N / 2; ++e) {
-                const float2 f = widen(a[e]);
-                a[e] = Ops<T>::pack(f.x * inv * w[2 * e], f.y * inv * w[2 * e + 1]);
+                const float2 f = fmul2(fmul2(widen(a[e]), splat2(inv)), make_float2(w[k][2 * e], w[k][2 * e + 1]));
+                a[e] = Ops<T>::pack(f.x, f.y);
             }
             store_piece<T, VEC>(static_cast<T*>(p.out) + row * p.os + i * N, p.C - i * N, u[k]);
         }
     } else {
-        // n in fp32, and the largest magnitudes as bit patterns (a NaN above an infinity)
+        // n in fp32, and the largest magnitudes (a NaN above an infinity).  Places outside the
+        // row are 0 here, and under a weight of 0: in a row without NaN they stay 0
         float2 n[NP][N / 2];
-        uint32_t top[NP], all = 0;
+        float top[NP], most = 0.0f;
 #pragma unroll
         for (int k = 0; k < NP; ++k) {
-            const int i = l0 + k * step;
             const P* a = reinterpret_cast<const P*>(&u[k]);
-            const bool mine = live && i < nvec;
-            float w[N] = {};
-            if (mine) load_weights<VEC>(p.w + i * N, p.C - i * N, w);
-            top[k] = 0;
+            if (!EARLY) weights(k);
+            top[k] = 0.0f;
 #pragma unroll
             for (int e = 0; e < N / 2; ++e) {
-                const float2 f = widen(a[e]);
-                const bool in0 = mine && (VEC || i * N + 2 * e < p.C), in1 = mine && (VEC || i * N + 2 * e + 1 < p.C);
-                n[k][e].x = in0 ? f.x * inv * w[2 * e] : 0.0f;
-                n[k][e].y = in1 ? f.y * inv * w[2 * e + 1] : 0.0f;
-                top[k] = max(top[k], max(__float_as_uint(n[k][e].x) & 0x7fffffffu, __float_as_uint(n[k][e].y) & 0x7fffffffu));
+                n[k][e] = fmul2(fmul2(widen(a[e]), splat2(inv)), make_float2(w[k][2 * e], w[k][2 * e + 1]));
+                top[k] = max_abs(max_abs(top[k], n[k][e].x), n[k][e].y);
             }
-            all = max(all, top[k]);
+            most = max_abs(most, top[k]);
         }
+        uint32_t all = __float_as_uint(most);
         if (p.group == p.C) {  // one scale a row
             all = __reduce_max_sync(0xffffffffu, all);
             if (p.wpr > 1) {
@@ -183,7 +197,7 @@ __global__ void __launch_bounds__(512) residual_norm_kernel(const ResidualParams
             const int i = l0 + k * step;
             uint32_t t = all;
             if (p.group != p.C) {
-                t = top[k];
+                t = __float_as_uint(top[k]);
                 for (int m = 1; m < lanes; m <<= 1) t = max(t, __shfl_xor_sync(0xffffffffu, t, m));
             }
             const uint32_t byte = e4m3_scale_byte(t);
@@ -240,7 +254,10 @@ extern "C" int need_residual_rms_norm(const need_residual_norm_args* a, need_str
     p.inv_c = 1.0f / static_cast<float>(a->C), p.eps = static_cast<float>(a->eps), p.scale = static_cast<float>(a->scale);
     const int nvec = int32_t((a->C + n - 1) / n);
     p.wpr = 1;
-    while (p.wpr * 32 * kPieces < nvec) p.wpr *= 2;
+    // up to 2 MB of rows (which the GPU holds at once) a piece a lane, as far as the warps go:
+    // 64 rows of 832 bf16 channels take 3.6 us at 4 pieces and 2.4 at one, 16384 17.0 and 20.1
+    const int pieces = int64_t(a->rows) * a->C * es <= (2 << 20) ? 1 : kPieces;
+    while (p.wpr * 32 * pieces < nvec && p.wpr < kMaxWarps) p.wpr *= 2;
     const int np = (nvec + 32 * p.wpr - 1) / (32 * p.wpr);
     auto al = [&](const void* q, int64_t stride, int bytes) {
         return reinterpret_cast<uintptr_t>(q) % bytes == 0 && (a->rows == 1 || stride * (q == a->out && a->out8 ? 1 : es) % bytes == 0);

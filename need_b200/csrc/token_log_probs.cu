@@ -527,53 +527,49 @@ __global__ void __launch_bounds__(kJoin) join_kernel(const LogpParams p) {
 }
 
 // A warp takes 32 * UN pieces of a row.  SAME: the gradient's rows lie as the logits' do
-// within 16 bytes.
+// within 16 bytes.  The token's own place is written again, by 1 - p from log p, since p may
+// be near 1.
 template <typename T, bool SAME>
 __global__ void __launch_bounds__(kThreads) logp_backward_kernel(const LogpParams p) {
     constexpr int N = Vec<T>::N;
     const int lane = threadIdx.x & 31;
-    const int64_t id = int64_t(blockIdx.x) * kWarps + (threadIdx.x >> 5), row = id / p.parts, part = id % p.parts;
+    const int64_t id = int64_t(blockIdx.x) * kWarps + (threadIdx.x >> 5), row = id / p.parts;
+    const int part = static_cast<int>(id % p.parts);
     if (row >= p.rows) return;
     const Run<T> run(static_cast<const T*>(p.logits) + row * p.stride, p.V);
     T* const out = static_cast<T*>(p.grad) + row * p.grad_stride;
     uint4 u[UN];
-    const int v0 = static_cast<int>(part) * 32 * UN + lane;
+    const int v0 = part * 32 * UN + lane;
 #pragma unroll
     for (int k = 0; k < UN; ++k)
         if (v0 + k * 32 < run.nvec) u[k] = __ldcs(run.body() + v0 + k * 32);
     const float m = p.stats[2 * row], l = p.stats[2 * row + 1], h = p.entropy[row];
     const float g = p.g != nullptr ? p.g[row] : 0.0f, gh = p.gh != nullptr ? p.gh[row] : 0.0f;
     const int64_t tok = p.tokens[row];
-    const bool given = tok >= 0;
-    const float gt = tok >= p.V ? nan32() : given ? g : 0.0f;  // of the token's log p
-    const float c = p.inv_t * kLog2e, l2 = l * kLog2e, ms = m == -INFINITY ? 0.0f : m;
+    const float gt = tok >= p.V ? nan32() : tok >= 0 ? g : 0.0f;  // of the token's log p
+    const bool none = m == -INFINITY && l == l;                   // a row of nothing
+    const float c = p.inv_t * kLog2e, ms = none ? 0.0f : m;
     const float a = p.inv_t * -(gt + gh * h), b = p.inv_t * -gh * kLn2;  // dx = p (a + b log2 p)
-    auto grad = [&](float x) {
-        const float z = fmaf(x - ms, c, -l2);
-        return ex2(z) * fmaf(b, fmaxf(z, kLow), a);
+    const float2 mm = make_float2(-ms, -ms), cc = make_float2(c, c), ll = make_float2(-l * kLog2e, -l * kLog2e);
+    const float2 aa = make_float2(a, a), bb = make_float2(b, b);
+    auto grad = [&](float x, float y) {
+        const float2 z = __ffma2_rn(__fadd2_rn(make_float2(x, y), mm), cc, ll);
+        return __fmul2_rn(make_float2(ex2(z.x), ex2(z.y)), __ffma2_rn(bb, make_float2(fmaxf(z.x, kLow), fmaxf(z.y, kLow)), aa));
     };
-    auto at_token = [&](float x) {  // 1 - p from log p: p may be near 1
-        const float lp = fmaf(x - ms, p.inv_t, -l);
-        const float q = expf(lp);
-        return p.inv_t * (gt * -expm1f(lp) - gh * q * (fmaxf(lp, kLow) + h));
-    };
-    auto one = [&](float x, int64_t i) {
-        if (m == -INFINITY && l == l) return gt == gt ? 0.0f : gt;  // a row of nothing
-        return i == tok ? at_token(x) : grad(x);
-    };
+    const float zero = gt == gt ? 0.0f : gt;  // a row of nothing's gradient
 #pragma unroll
     for (int k = 0; k < UN; ++k) {
         const int v = v0 + k * 32;
-        const int64_t i0 = run.head + int64_t(v) * N;
         if (v >= run.nvec) break;
+        const int64_t i0 = run.head + int64_t(v) * N;
         float x[N];
         Vec<T>::widen(u[k], x);
-        const bool plain = !(m == -INFINITY) && (tok < i0 || tok >= i0 + N);
-#pragma unroll
-        for (int e = 0; e < N; ++e) x[e] = plain ? grad(x[e]) : one(x[e], i0 + e);
         union { uint4 u; T e[N]; } r;
 #pragma unroll
-        for (int e = 0; e < N; ++e) r.e[e] = static_cast<T>(x[e]);
+        for (int e = 0; e < N; e += 2) {
+            const float2 d = none ? make_float2(zero, zero) : grad(x[e], x[e + 1]);
+            r.e[e] = static_cast<T>(d.x), r.e[e + 1] = static_cast<T>(d.y);
+        }
         if constexpr (SAME) {
             __stcs(reinterpret_cast<uint4*>(out + i0), r.u);
         } else {
@@ -583,7 +579,18 @@ __global__ void __launch_bounds__(kThreads) logp_backward_kernel(const LogpParam
     }
     if (part == 0 && lane < run.edges()) {
         const int i = run.edge(lane);
-        out[i] = static_cast<T>(one(to_float(run.x[i]), i));
+        out[i] = static_cast<T>(none ? zero : grad(to_float(run.x[i]), 0.0f).x);
+    }
+    if (none || tok < 0 || tok >= p.V) return;
+    // after the stores above, by the thread that made the one at its place
+    const int64_t in = tok - run.head;
+    const bool body = in >= 0 && in < int64_t(run.nvec) * N;
+    const int v = static_cast<int>(in / N);
+    const bool mine = body ? v / (32 * UN) == part && (v & 31) == lane : part == 0 && lane == (in < 0 ? tok : tok - int64_t(run.nvec) * N);
+    if (mine) {
+        const float lp = fmaf(to_float(run.x[tok]) - ms, p.inv_t, -l);
+        const float q = expf(lp);
+        out[tok] = static_cast<T>(p.inv_t * (gt * -expm1f(lp) - gh * q * (fmaxf(lp, kLow) + h)));
     }
 }
 
