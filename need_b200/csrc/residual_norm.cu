@@ -5,10 +5,12 @@
 //   out = n, or e4m3(n / 2^e) with one 2^e for each `group` channels
 //
 // x and y are read once, the stream and the output written once: 8 B per 16-bit element,
-// 7 with 8 bits, so HBM bounds it.  A row lies in the registers of 1 to 16 warps (the
-// fewest that leave a lane at most 4 16-byte pieces), from the addition to the output; its
-// sum and the groups' largest values are taken by shuffles, a group's pieces lying in
-// neighbouring lanes.
+// 7 with 8 bits, so HBM bounds it.  A row lies in the registers of 1 to 16 warps, from the
+// addition to the output; its sum and the groups' largest values are taken by shuffles, a
+// group's pieces lying in neighbouring lanes.  16384 rows of 832 bf16 channels: 17.0 us, 6.4
+// TB/s; with 8 bits 20.3 us, 4.8 TB/s, by its instructions; 64 rows: 2.4 us, a launch and two round trips.  Rows
+// that only 8, 4 or 2 bytes divide: 14288 rows of 1324 bf16 channels 27 us, of 1326 43, of
+// 1325 112.
 #include <algorithm>
 #include <type_traits>
 
@@ -41,33 +43,39 @@ struct ResidualParams {
     float inv_c, eps, scale;
 };
 
-// A 16-byte piece of a row.  VEC: rows are 16-byte aligned and whole pieces; else element
-// by element, n of the piece's N inside the row.
-template <typename T, bool VEC>
+template <int BYTES>
+struct Word;
+template <>
+struct Word<16> { using W = uint4; };
+template <>
+struct Word<8> { using W = uint2; };
+template <>
+struct Word<4> { using W = unsigned int; };
+template <>
+struct Word<2> { using W = unsigned short; };
+template <>
+struct Word<1> { using W = unsigned char; };
+
+// A 16-byte piece of a row, M elements at a time, of which the first n are inside the row: M
+// divides the channels, and M elements are what every row is aligned to.
+template <typename T, int M>
 __device__ __forceinline__ uint4 load_piece(const T* p, int n) {
-    if constexpr (VEC) {
-        return __ldcs(reinterpret_cast<const uint4*>(p));
-    } else {
-        constexpr int N = 16 / sizeof(T);
-        union { uint4 u; T e[N]; } r;
-        r.u = make_uint4(0, 0, 0, 0);
+    using W = typename Word<M * sizeof(T)>::W;
+    constexpr int N = 16 / sizeof(T);
+    union { uint4 u; W w[N / M]; } r;
+    r.u = make_uint4(0, 0, 0, 0);
 #pragma unroll
-        for (int e = 0; e < N; ++e)
-            if (e < n) r.e[e] = p[e];
-        return r.u;
-    }
+    for (int e = 0; e < N; e += M)
+        if (M == N || e < n) r.w[e / M] = __ldcs(reinterpret_cast<const W*>(p + e));
+    return r.u;
 }
-template <typename T, bool VEC>
-__device__ __forceinline__ void store_piece(T* p, int n, const uint4& u) {
-    if constexpr (VEC) {
-        *reinterpret_cast<uint4*>(p) = u;
-    } else {
-        constexpr int N = 16 / sizeof(T);
-        const T* q = reinterpret_cast<const T*>(&u);
+// B: bytes of an element in memory
+template <int B, int N, int M, typename U>
+__device__ __forceinline__ void store_piece(void* p, int n, const U& u) {
+    using W = typename Word<M * B>::W;
 #pragma unroll
-        for (int e = 0; e < N; ++e)
-            if (e < n) p[e] = q[e];
-    }
+    for (int e = 0; e < N; e += M)
+        if (M == N || e < n) reinterpret_cast<W*>(p)[e / M] = reinterpret_cast<const W*>(&u)[e / M];
 }
 
 // The larger of a (at least 0) and |b|; NaN if one of them is.
@@ -77,23 +85,24 @@ __device__ __forceinline__ float max_abs(float a, float b) {
     return r;
 }
 // The weights of a piece's N channels, of which the first n are there.
-template <bool VEC, int N>
+template <int M, int N>
 __device__ __forceinline__ void load_weights(const float* w, int n, float (&f)[N]) {
-    if constexpr (VEC) {
+    constexpr int F = M < 4 ? M : 4;
+    using W = typename Word<4 * F>::W;
 #pragma unroll
-        for (int e = 0; e < N; e += 4) {
-            const float4 u = __ldg(reinterpret_cast<const float4*>(w + e));
-            f[e] = u.x, f[e + 1] = u.y, f[e + 2] = u.z, f[e + 3] = u.w;
-        }
-    } else {
+    for (int e = 0; e < N; e += F) {
+        union { W u; float f[F]; } r;
 #pragma unroll
-        for (int e = 0; e < N; ++e) f[e] = e < n ? __ldg(w + e) : 0.0f;
+        for (int i = 0; i < F; ++i) r.f[i] = 0.0f;
+        if (M == N || e < n) r.u = __ldg(reinterpret_cast<const W*>(w + e));
+#pragma unroll
+        for (int i = 0; i < F; ++i) f[e + i] = r.f[i];
     }
 }
 
 // blockDim = 32 * wpr * (rows per block); lane l of a row's warp w holds pieces
 // (w * 32 + l) + k * 32 * wpr.  OUT8: the output in 8 bits.
-template <typename T, int NP, bool VEC, bool OUT8>
+template <typename T, int NP, int M, bool OUT8>
 __global__ void __launch_bounds__(512) residual_norm_kernel(const ResidualParams p) {
     using P = typename Ops<T>::P;
     constexpr int N = 16 / Ops<T>::BYTES;
@@ -110,7 +119,7 @@ __global__ void __launch_bounds__(512) residual_norm_kernel(const ResidualParams
     for (int k = 0; k < NP; ++k) {
         const int i = l0 + k * step;
         u[k] = v[k] = make_uint4(0, 0, 0, 0);
-        if (live && i < nvec) u[k] = load_piece<T, VEC>(x + i * N, p.C - i * N), v[k] = load_piece<T, VEC>(y + i * N, p.C - i * N);
+        if (live && i < nvec) u[k] = load_piece<T, M>(x + i * N, p.C - i * N), v[k] = load_piece<T, M>(y + i * N, p.C - i * N);
     }
     // the weights meanwhile, where a lane has at most 16: 64 rows of 832 fp32 channels 2.8 us,
     // 3.6 with them after the sum; at 32 of them they push rows out of the registers (16384
@@ -119,7 +128,7 @@ __global__ void __launch_bounds__(512) residual_norm_kernel(const ResidualParams
     float w[NP][N] = {};
     auto weights = [&](int k) {
         const int i = l0 + k * step;
-        if (live && i < nvec) load_weights<VEC>(p.w + i * N, p.C - i * N, w[k]);
+        if (live && i < nvec) load_weights<M>(p.w + i * N, p.C - i * N, w[k]);
     };
 #pragma unroll
     for (int k = 0; k < NP; ++k)
@@ -137,7 +146,7 @@ __global__ void __launch_bounds__(512) residual_norm_kernel(const ResidualParams
             ss2 = ffma2(f, f, ss2);
         }
         const int i = l0 + k * step;
-        if (live && i < nvec) store_piece<T, VEC>(static_cast<T*>(p.stream) + row * p.ss + i * N, p.C - i * N, u[k]);
+        if (live && i < nvec) store_piece<sizeof(T), N, M>(static_cast<T*>(p.stream) + row * p.ss + i * N, p.C - i * N, u[k]);
     }
     float ss = ss2.x + ss2.y;
 #pragma unroll
@@ -162,7 +171,7 @@ __global__ void __launch_bounds__(512) residual_norm_kernel(const ResidualParams
                 const float2 f = fmul2(fmul2(widen(a[e]), splat2(inv)), make_float2(w[k][2 * e], w[k][2 * e + 1]));
                 a[e] = Ops<T>::pack(f.x, f.y);
             }
-            store_piece<T, VEC>(static_cast<T*>(p.out) + row * p.os + i * N, p.C - i * N, u[k]);
+            store_piece<sizeof(T), N, M>(static_cast<T*>(p.out) + row * p.os + i * N, p.C - i * N, u[k]);
         }
     } else {
         // n in fp32, and the largest magnitudes (a NaN above an infinity).  Places outside the
@@ -204,28 +213,20 @@ __global__ void __launch_bounds__(512) residual_norm_kernel(const ResidualParams
             if (!live || i >= nvec) continue;
             const bool first = p.group != p.C ? (i & (lanes - 1)) == 0 : i == 0;
             if (first) p.scales[row * p.ngroups + (p.group != p.C ? i / lanes : 0)] = e4m3_scale(byte);
-            union { uint16_t h[N / 2]; uint2 w2; uint32_t w1; } q;
+            alignas(N) uint16_t q[N / 2];
 #pragma unroll
-            for (int e = 0; e < N / 2; ++e) q.h[e] = e4m3_pair(n[k][e], byte);
-            uint8_t* to = static_cast<uint8_t*>(p.out) + row * p.os + i * N;
-            if constexpr (VEC) {
-                if constexpr (N == 8) *reinterpret_cast<uint2*>(to) = q.w2;
-                else *reinterpret_cast<uint32_t*>(to) = q.w1;
-            } else {
-#pragma unroll
-                for (int e = 0; e < N; ++e)
-                    if (i * N + e < p.C) to[e] = static_cast<uint8_t>(q.h[e / 2] >> (8 * (e & 1)));
-            }
+            for (int e = 0; e < N / 2; ++e) q[e] = e4m3_pair(n[k][e], byte);
+            store_piece<1, N, M>(static_cast<uint8_t*>(p.out) + row * p.os + i * N, p.C - i * N, q);
         }
     }
 }
 
-template <typename T, int NP, bool VEC>
+template <typename T, int NP, int M>
 int launch(const ResidualParams& p, bool out8, cudaStream_t s) {
     const int warps = std::max(p.wpr, 4), rpb = warps / p.wpr;
     const int64_t blocks = (p.rows + rpb - 1) / rpb;
-    if (out8) residual_norm_kernel<T, NP, VEC, true><<<static_cast<unsigned>(blocks), 32 * warps, 0, s>>>(p);
-    else residual_norm_kernel<T, NP, VEC, false><<<static_cast<unsigned>(blocks), 32 * warps, 0, s>>>(p);
+    if (out8) residual_norm_kernel<T, NP, M, true><<<static_cast<unsigned>(blocks), 32 * warps, 0, s>>>(p);
+    else residual_norm_kernel<T, NP, M, false><<<static_cast<unsigned>(blocks), 32 * warps, 0, s>>>(p);
     const cudaError_t e = cudaGetLastError();
     return e == cudaSuccess ? NEED_OK : cuda_fail(e, "residual norm launch");
 }
@@ -259,23 +260,29 @@ extern "C" int need_residual_rms_norm(const need_residual_norm_args* a, need_str
     const int pieces = int64_t(a->rows) * a->C * es <= (2 << 20) ? 1 : kPieces;
     while (p.wpr * 32 * pieces < nvec && p.wpr < kMaxWarps) p.wpr *= 2;
     const int np = (nvec + 32 * p.wpr - 1) / (32 * p.wpr);
-    auto al = [&](const void* q, int64_t stride, int bytes) {
-        return reinterpret_cast<uintptr_t>(q) % bytes == 0 && (a->rows == 1 || stride * (q == a->out && a->out8 ? 1 : es) % bytes == 0);
+    // as many elements at a time as the channels divide into and every row is aligned to
+    auto al = [&](const void* q, int64_t stride, int bytes, int m) {
+        return reinterpret_cast<uintptr_t>(q) % (bytes * m) == 0 && (a->rows == 1 || stride % m == 0);
     };
-    const bool vec = a->C % n == 0 && aligned16(a->weight) && al(p.x, p.xs, 16) && al(p.y, p.ys, 16) && al(p.stream, p.ss, 16) &&
-                     al(p.out, p.os, a->out8 ? n : 16);
+    int m = n;
+    while (m > 1 && !(a->C % m == 0 && al(a->weight, 0, 4, std::min(m, 4)) && al(p.x, p.xs, es, m) && al(p.y, p.ys, es, m) &&
+                      al(p.stream, p.ss, es, m) && al(p.out, p.os, a->out8 ? 1 : es, m)))
+        m /= 2;
     auto run = [&](auto tag) {
         using T = decltype(tag);
         auto go = [&](auto v) {
-            constexpr bool V = decltype(v)::value;
+            constexpr int M = decltype(v)::value;
             switch (np) {
-                case 1: return launch<T, 1, V>(p, a->out8 != 0, stream);
-                case 2: return launch<T, 2, V>(p, a->out8 != 0, stream);
-                case 3: return launch<T, 3, V>(p, a->out8 != 0, stream);
-                default: return launch<T, 4, V>(p, a->out8 != 0, stream);
+                case 1: return launch<T, 1, M>(p, a->out8 != 0, stream);
+                case 2: return launch<T, 2, M>(p, a->out8 != 0, stream);
+                case 3: return launch<T, 3, M>(p, a->out8 != 0, stream);
+                default: return launch<T, 4, M>(p, a->out8 != 0, stream);
             }
         };
-        return vec ? go(std::true_type{}) : go(std::false_type{});
+        if constexpr (sizeof(T) == 2)
+            if (m == 8) return go(std::integral_constant<int, 8>{});
+        if (m == 4) return go(std::integral_constant<int, 4>{});
+        return m == 2 ? go(std::integral_constant<int, 2>{}) : go(std::integral_constant<int, 1>{});
     };
     const int rc = a->dtype == NEED_F32 ? run(float{}) : a->dtype == NEED_BF16 ? run(__nv_bfloat16{}) : run(__half{});
     return rc != NEED_OK ? rc : ok();

@@ -10,16 +10,20 @@
 // log1p(r / count), so that probabilities near 1 and small entropies keep their relative
 // precision (both terms of H are positive).
 //
-// The largest: the least of the warps' (k / 8)-th largest lanes' maxima is a bound that k
-// logits reach.  The first pass leaves the maxima of a thread's pieces, some 32 logits
-// each; only those that reach the bound are read again, and what they hold is put into
-// order by counting.  Keys order by value, then by the lower token.
+// The largest: the k-th of the lanes' maxima is a bound that k logits reach.  The first pass
+// leaves the maxima of a thread's pieces, some 32 logits each; only those that reach the
+// bound are read again, and what they hold is put into order by counting.  Keys order by
+// value, then by the lower token.
 //
-// Short rows take a warp each, longer ones 8; where there are few, rows are cut into parts
-// that a second launch joins, in order.  Rows of any alignment: the elements before the
-// first and after the last whole 16 bytes are taken one by one.  Per logit: 2 or 4 B, one
-// ex2 (16 a cycle and SM, which comes near HBM's rate for 16 bits) and some 6 other
-// instructions.
+// Short rows take a warp each, longer ones a block of 4; where there are few, rows are cut
+// into parts that a second launch joins, in order.  Rows of any alignment: the elements before
+// the first and after the last whole 16 bytes are taken one by one.  Per logit: 2 or 4 B, one
+// ex2 (16 a cycle and SM, three quarters of HBM's time for 16 bits) and some 7 other
+// instructions, half of them in packed pairs.  1024 rows of 50021 bf16 logits: 24 us (4.3
+// TB/s), with the 20 largest 31.6 -- all rows run side by side, so that what follows the
+// pass, some 7 us of waiting on one another, hides under nothing; fp32 34.6 us (5.9 TB/s).
+// 16384 rows of 784: 10 us, the gradient 14.  4 rows of 131072 fp32 logits, the 5 largest: 9
+// us, two launches.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <float.h>
