@@ -37,6 +37,10 @@
  *                                   GPU kernel need_kernels.py:99-107)
  *   need_ssd_scan_rms_norm       <- need_kernels.ssd_scan followed by the block's
  *                                   out_norm (need_core.py:1624-1643), one call
+ *   need_linear_attention, need_linear_attention_step, need_residual_rms_norm,
+ *   need_token_log_probs         <- no counterpart (operators of language models around the
+ *                                   block; the residual's scale and norm are
+ *                                   residual_scale_add and rms_norm, two calls there)
  *
  * Return codes: NEED_OK (0), or a need_status error; need_last_error() gives a
  * message for the calling thread's last failure.  All entry points are

@@ -8,9 +8,9 @@
 // 7 with 8 bits, so HBM bounds it.  A row lies in the registers of 1 to 16 warps, from the
 // addition to the output; its sum and the groups' largest values are taken by shuffles, a
 // group's pieces lying in neighbouring lanes.  16384 rows of 832 bf16 channels: 17.0 us, 6.4
-// TB/s; with 8 bits 20.3 us, 4.8 TB/s, by its instructions; 64 rows: 2.4 us, a launch and two round trips.  Rows
-// that only 8, 4 or 2 bytes divide: 14288 rows of 1324 bf16 channels 27 us, of 1326 43, of
-// 1325 112.
+// TB/s; with 8 bits 20.3 us, 4.8 TB/s, by its instructions; 64 rows: 2.4 us, a launch and two
+// round trips.  Rows that only 8, 4 or 2 bytes divide: 14288 rows of 1324 bf16 channels 27
+// us, of 1326 43, of 1325 112.
 #include <algorithm>
 #include <type_traits>
 
