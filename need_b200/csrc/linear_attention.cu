@@ -292,8 +292,10 @@ __device__ __forceinline__ bool make_decays(const TokenPair& tp, float scale, De
     return __any_sync(0xffffffffu, !(tp.ld[0] <= 1.0f && tp.ld[1] <= 1.0f));
 }
 // ------------------------------------------------------------------ the kernel
-// STATE: only the state of a segment of the sequence, from zero, and its decay.
-template <typename T, int DK, bool VEC, bool STATE>
+// What a launch's segments are run for.
+enum Kind { OUTPUTS, STATES, MIXED };
+
+template <typename T, int DK, bool VEC, int KIND>
 __global__ void __launch_bounds__(kThreads, DK == 64 && Split<T>::IN < 3 ? 3 : 2) attention_kernel(const AttnParams p) {
     using S = Split<T>;
     using L = Layout<T, DK, VEC>;
@@ -304,9 +306,9 @@ __global__ void __launch_bounds__(kThreads, DK == 64 && Split<T>::IN < 3 ? 3 : 2
     if (p.redo != nullptr && p.redo[blockIdx.x] == 0) return;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c2 = (lane & 3) * 2;
     int64_t id = blockIdx.x;
-    const int nseg = STATE ? p.nseg - 1 : p.nseg;
-    const int seg = static_cast<int>(id % nseg);
-    id /= nseg;
+    const int segs = p.launched(), seg = static_cast<int>(id % segs) + (p.ahead ? 0 : p.lead);
+    const bool state = KIND == MIXED ? seg >= p.lead : KIND == STATES;  // only the state
+    id /= segs;
     const int slice = static_cast<int>(id % p.slices);
     const int64_t chain = id / p.slices;
     const int64_t b = chain / p.H;
@@ -317,15 +319,14 @@ __global__ void __launch_bounds__(kThreads, DK == 64 && Split<T>::IN < 3 ? 3 : 2
     const float* ld = p.ld + b * p.lb + h * p.lh;
     const uint8_t* marks = p.seg == nullptr ? nullptr : p.seg + b * p.gb;
     T* out = static_cast<T*>(p.out) + b * p.ob + h * p.oh;
-    const int64_t chunks = (p.T + C - 1) / C, c0 = int64_t(seg) * p.seg_chunks;
-    const int64_t c1 = c0 + p.seg_chunks < chunks ? c0 + p.seg_chunks : chunks;
+    const int64_t chunks = (p.T + C - 1) / C, c0 = p.segment(seg), c1 = p.segment(seg + 1) < chunks ? p.segment(seg + 1) : chunks;
     Decays* const gates = reinterpret_cast<Decays*>(smem + L::G);
     const uint32_t sm = smem_addr(smem);
 
     // the state, transposed: rows j = jw + g and + 8, columns i = 8 n + c2 and + 1
     float s[NI][4];
     {
-        const float* from = STATE ? nullptr : seg > 0 ? p.part + (chain * (p.nseg - 1) + seg - 1) * p.dk * int64_t(p.dv)
+        const float* from = state ? nullptr : seg > 0 ? p.part + (chain * (p.nseg - 1) + seg - 1) * p.dk * int64_t(p.dv)
                                   : p.s0 != nullptr   ? p.s0 + chain * p.dk * int64_t(p.dv) : nullptr;
 #pragma unroll
         for (int n = 0; n < NI; ++n)
@@ -335,7 +336,7 @@ __global__ void __launch_bounds__(kThreads, DK == 64 && Split<T>::IN < 3 ? 3 : 2
                 s[n][e] = from != nullptr && i < p.dk && j < p.dv ? from[int64_t(i) * p.dv + j] : 0.0f;
             }
     }
-    float total = 1.0f;  // STATE: the segment's decay
+    float total = 1.0f;  // the segment's decay
 
     using B16 = __nv_bfloat16;
     const B16 *qc = reinterpret_cast<const B16*>(q), *kc = reinterpret_cast<const B16*>(k), *vc = reinterpret_cast<const B16*>(v);
@@ -344,7 +345,7 @@ __global__ void __launch_bounds__(kThreads, DK == 64 && Split<T>::IN < 3 ? 3 : 2
     auto issue = [&](int64_t c) {  // the asynchronous copies of a chunk, in turn
         if constexpr (L::STAGES == 2) {
             const uint32_t to = sm + (c & 1) * L::STAGE;
-            if (!STATE) copy_q.copy(to + L::Q, qc, p.T - c * C);
+            if (!state) copy_q.copy(to + L::Q, qc, p.T - c * C);
             copy_k.copy(to + L::K, kc, p.T - c * C);
             copy_v.copy(to + L::V, vc, p.T - c * C);
             cp_commit();
@@ -368,11 +369,11 @@ __global__ void __launch_bounds__(kThreads, DK == 64 && Split<T>::IN < 3 ? 3 : 2
             Loader<T, DK, VEC> lk, lq;
             Loader<T, DV, VEC> lv;
             lk.load(k, p.k.st, t0, p.T, 0, p.dk), lv.load(v, p.v.st, t0, p.T, col0, p.dv);
-            if (!STATE && ALL) lq.load(q, p.q.st, t0, p.T, 0, p.dk);
+            if (!state && ALL) lq.load(q, p.q.st, t0, p.T, 0, p.dk);
             __syncthreads();  // the chunk before this one has been read
             bad = lk.store(buf + L::K) | lv.store(buf + L::V);
-            if (!STATE && !ALL) lq.load(q, p.q.st, t0, p.T, 0, p.dk);
-            if (!STATE) lq.store(buf + L::Q);
+            if (!state && !ALL) lq.load(q, p.q.st, t0, p.T, 0, p.dk);
+            if (!state) lq.store(buf + L::Q);
         }
         bad = __syncthreads_or(bad | wild);  // the chunk and its decays are there
         const Decays& gt = gates[c & 1];
@@ -381,7 +382,7 @@ __global__ void __launch_bounds__(kThreads, DK == 64 && Split<T>::IN < 3 ? 3 : 2
             issue(c + 1);
             if (warp == 0) next = load_decays(p, ld, marks, t0 + C);
         }
-        if (STATE) total = total == -1.0f || gt.d == -1.0f ? -1.0f : total * gt.d;
+        if (KIND != OUTPUTS) total = total == -1.0f || gt.d == -1.0f ? -1.0f : total * gt.d;
 
         if (bad) {  // token by token, in fp32, from the inputs themselves
             const int n = static_cast<int>(p.T - t0 < C ? p.T - t0 : C);
@@ -403,13 +404,13 @@ __global__ void __launch_bounds__(kThreads, DK == 64 && Split<T>::IN < 3 ? 3 : 2
                             const float kk = to_float(k[t * p.k.st + i]);
                             s[m][e] = reset ? kk * v0 : fmaf(a, s[m][e], kk * v0);
                             s[m][2 + e] = reset ? kk * v1 : fmaf(a, s[m][2 + e], kk * v1);
-                            if (!STATE) {
+                            if (!state) {
                                 const float qq = to_float(q[t * p.q.st + i]);
                                 o0 = fmaf(qq, s[m][e], o0), o1 = fmaf(qq, s[m][2 + e], o1);
                             }
                         }
                     }
-                if (!STATE) {
+                if (!state) {
 #pragma unroll
                     for (int m = 1; m < 4; m <<= 1) {
                         o0 += __shfl_xor_sync(0xffffffffu, o0, m);
@@ -428,7 +429,7 @@ __global__ void __launch_bounds__(kThreads, DK == 64 && Split<T>::IN < 3 ? 3 : 2
         const int br = (lane & 7) + ((lane >> 4) << 3), bp = (lane >> 3) & 1;  // [n][k] tiles, and [k][m] ones transposed
         const bool resets = gt.d == -1.0f;
         float o[4][2][4] = {};
-        if constexpr (!STATE) {
+        if (!state) {
             // the scores on and below the diagonal, in blocks of 16 x 16: each warp the one on
             // the diagonal and one or two others
             for (int i = 0; i < (warp == 1 || warp == 2 ? 3 : 2); ++i) {
@@ -530,7 +531,7 @@ __global__ void __launch_bounds__(kThreads, DK == 64 && Split<T>::IN < 3 ? 3 : 2
                 }
         }
         if (warp == 0 && c + 1 < c1) wild = make_decays(next, p.scale, gates[(c + 1) & 1]);
-        if constexpr (!STATE) __syncthreads();  // the scores are there
+        if (!state) __syncthreads();  // the scores are there
 
         // the scores times v, and the state
         if (resets) {
@@ -549,7 +550,7 @@ __global__ void __launch_bounds__(kThreads, DK == 64 && Split<T>::IN < 3 ? 3 : 2
             uint32_t vf[S::IN][4];  // (tokens 0-7, columns 0-7), (0-7, 8-15), (8-15, 0-7), (8-15, 8-15)
 #pragma unroll
             for (int a = 0; a < S::IN; ++a) ldsm4_t(vf[a], sbuf + L::V + a * C * DV * 2 + at(16 * kb + br, 2 * warp + bp));
-            if constexpr (!STATE) {
+            if (!state) {
                 float t[4][2][4] = {};
                 products<S::OUT, S::SCORE, S::IN>([&](int a, int b2) {
 #pragma unroll
@@ -598,7 +599,7 @@ __global__ void __launch_bounds__(kThreads, DK == 64 && Split<T>::IN < 3 ? 3 : 2
                 for (int n = 0; n < 4; ++n) add4(s[n0 + n], t[n]);
             }
         }
-        if constexpr (!STATE) {
+        if (!state) {
             const int64_t rows = p.T - t0;
             T* const row0 = out + t0 * p.ot + jw + c2;
 #pragma unroll
@@ -627,7 +628,7 @@ __global__ void __launch_bounds__(kThreads, DK == 64 && Split<T>::IN < 3 ? 3 : 2
         }
     }
 
-    float* const to = STATE ? p.part + (chain * (p.nseg - 1) + seg) * p.dk * int64_t(p.dv)
+    float* const to = KIND != OUTPUTS ? p.part + (chain * (p.nseg - 1) + seg) * p.dk * int64_t(p.dv)
                             : seg == p.nseg - 1 && p.sT != nullptr ? p.sT + chain * p.dk * int64_t(p.dv) : nullptr;
     if (to != nullptr) {
 #pragma unroll
@@ -638,20 +639,20 @@ __global__ void __launch_bounds__(kThreads, DK == 64 && Split<T>::IN < 3 ? 3 : 2
                 if (i < p.dk && j < p.dv) to[int64_t(i) * p.dv + j] = s[n][e];
             }
     }
-    if (STATE && slice == 0 && threadIdx.x == 0) p.part_d[chain * (p.nseg - 1) + seg] = total;
+    if (KIND != OUTPUTS && slice == 0 && threadIdx.x == 0) p.part_d[chain * (p.nseg - 1) + seg] = total;
 }
 
 // The state that enters each segment after the first, in the place of the own state of
-// the one before it.
+// the one before it (lead: the second's lies there).
 __global__ void __launch_bounds__(256) enter_kernel(const AttnParams p) {
     const int64_t n = p.dk * int64_t(p.dv), chain = blockIdx.x;
     const int64_t i = blockIdx.y * int64_t(256) + threadIdx.x;
     if (i >= n) return;
     float* s = p.part + chain * (p.nseg - 1) * n + i;
     const float* d = p.part_d + chain * (p.nseg - 1);
-    float x = p.s0 != nullptr ? p.s0[chain * n + i] : 0.0f;
+    float x = p.lead ? s[0] : p.s0 != nullptr ? p.s0[chain * n + i] : 0.0f;
     constexpr int B = 8;  // loads in flight
-    for (int k0 = 0; k0 < p.nseg - 1; k0 += B) {
+    for (int k0 = p.lead; k0 < p.nseg - 1; k0 += B) {
         float own[B];
 #pragma unroll
         for (int e = 0; e < B; ++e) own[e] = k0 + e < p.nseg - 1 ? s[(k0 + e) * n] : 0.0f;
@@ -667,8 +668,9 @@ __global__ void __launch_bounds__(256) enter_kernel(const AttnParams p) {
 // ------------------------------------------------------------------ host
 struct Plan {
     bool umma;  // sm_100a's tensor cores take it, in chunks of 128
-    int64_t chains, chunks, blocks;
-    int32_t slices, nseg, seg_chunks;
+    int64_t chains, chunks;
+    int32_t slices, nseg, lead;
+    int64_t first_chunks, seg_chunks;  // of the first segment, of the others
 };
 // CTAs of attention_kernel that a multiprocessor holds (registers for 3, 227 KB).
 template <typename T>
@@ -677,13 +679,16 @@ constexpr int held(bool small) {
     return std::min(3, 227 * 1024 / bytes);
 }
 // Where there are few chains they are cut into segments, as many as the GPU holds at once (of
-// umma's CTAs one a multiprocessor): all but the last are run for the state that they leave
-// (four fifths of a chunk's time), a launch joins those, then all are run for the outputs.
-// That is worth it where it saves more chunks in a row than the two more launches cost (1.5
-// of attention_kernel's, five of umma's 128 tokens).  Uncut and cut: 4 bf16 chains of 64
-// features 14.3 and 18.2 us at 512 tokens, 22.3 and 18.8 at 1024; 52 in two segments 71 and
-// 74 at 4096; 64 fp16 ones 13.8 and 17.7 at 128 tokens, 24 and 21.6 at 256, 385 and 171 at
-// 4096; 104 fp32 ones of 64 features 521 and 475 at 4096.
+// umma's CTAs one a multiprocessor): all but the last are run for the state that they leave, a
+// launch joins those, then all are run for the outputs.  That is worth it where it saves more
+// chunks in a row than the two more launches cost (1.5 of attention_kernel's, five of umma's
+// 128 tokens; a chunk for the state alone counts as 0.8).  Uncut and cut: 4 bf16 chains of 64
+// features 14.3 and 18.2 us at 512 tokens, 22.3 and 18.8 at 1024; 64 fp16 ones 13.8 and 17.7
+// at 128 tokens, 24 and 21.6 at 256, 385 and 171 at 4096; 104 fp32 ones 521 and 475 at 4096.
+// umma may also run one segment more, the first for its outputs ahead (lead): of two places a
+// chain, 1x16384 32x128 takes 282 us, 347 without and 384 uncut, 52 chains of 64 features at
+// 4096 tokens 62, 74 and 71.  (In attention_kernel the choice at run time costs more: 16
+// x 2048, 8 heads of 128 x 128 in fp32 431 us, 391 without.)
 Plan plan(bool umma, int32_t dtype, int64_t nb, int64_t T, int64_t H, int64_t dk, int64_t dv) {
     Plan pl{};
     pl.umma = umma;
@@ -691,48 +696,55 @@ Plan plan(bool umma, int32_t dtype, int64_t nb, int64_t T, int64_t H, int64_t dk
     const bool small = dk <= 64;
     const int64_t ctas = std::max<int64_t>(1, pl.chains * pl.slices), unit = umma ? 2 : 1, chunks = (pl.chunks + unit - 1) / unit;
     const int64_t places = 148 * (umma ? 1 : dtype == NEED_F32 ? held<float>(small) : dtype == NEED_BF16 ? held<__nv_bfloat16>(small) : held<__half>(small));
-    const int64_t nseg = std::max<int64_t>(1, std::min(places / ctas, chunks)), seg = (chunks + nseg - 1) / nseg;
-    const bool cut = 18 * seg + (umma ? 50 : 15) <= 10 * chunks;
-    pl.seg_chunks = int32_t(cut ? seg * unit : chunks * unit);
-    pl.nseg = int32_t((pl.chunks + pl.seg_chunks - 1) / pl.seg_chunks);
-    pl.blocks = pl.chains * pl.slices * pl.nseg;
+    const int64_t most = std::max<int64_t>(1, places / ctas), nseg = std::min(most, chunks), len = (chunks + nseg - 1) / nseg;
+    int64_t cost = 18 * len + (umma ? 50 : 15);  // tenths of a chunk
+    pl.nseg = 1, pl.first_chunks = pl.seg_chunks = chunks * unit;
+    if (cost <= 10 * chunks) pl.nseg = int32_t((chunks + len - 1) / len), pl.first_chunks = pl.seg_chunks = len * unit;
+    else cost = 10 * chunks;
+    if (umma) {
+        const int64_t n = (10 * chunks + 10 * most + 6) / (10 * most + 7), others = std::min(most, (chunks - 1) / n), first = chunks - others * n;
+        if (others > 1 && std::max(10 * first, 8 * n) + 10 * n + 50 < cost)
+            pl.lead = 1, pl.nseg = int32_t(others) + 1, pl.first_chunks = first * unit, pl.seg_chunks = n * unit;
+    }
     return pl;
 }
 size_t workspace_of(const Plan& pl, int64_t dk, int64_t dv) {
-    return 16 + size_t(pl.chains) * size_t(pl.nseg - 1) * (size_t(dk) * size_t(dv) + 1) * 4 + (pl.umma ? size_t(pl.blocks) * 4 : 0);
+    return 16 + size_t(pl.chains) * size_t(pl.nseg - 1) * (size_t(dk) * size_t(dv) + 1) * 4 + (pl.umma ? size_t(pl.chains) * pl.slices * pl.nseg * 4 : 0);
 }
 
-template <typename T, int DK, bool VEC, bool STATE>
-int launch(const AttnParams& p, int64_t blocks, cudaStream_t s) {
+template <typename T, int DK, bool VEC, int KIND>
+int launch(const AttnParams& p, const Plan& pl, cudaStream_t s) {
     static std::atomic<uint64_t> done{0};
-    auto kern = attention_kernel<T, DK, VEC, STATE>;
+    auto kern = attention_kernel<T, DK, VEC, KIND>;
     constexpr int bytes = Layout<T, DK, VEC>::BYTES;
     cudaError_t e = ensure_smem(kern, bytes, done);
     if (e != cudaSuccess) return cuda_fail(e, "linear attention shared memory");
-    kern<<<static_cast<unsigned>(blocks), kThreads, bytes, s>>>(p);
+    kern<<<static_cast<unsigned>(pl.chains * pl.slices * p.launched()), kThreads, bytes, s>>>(p);
     e = cudaGetLastError();
     return e == cudaSuccess ? NEED_OK : cuda_fail(e, "linear attention launch");
 }
 
 template <typename T, int DK, bool VEC>
 int run(AttnParams p, const Plan& pl, int64_t nb, uint32_t* redo, cudaStream_t s) {
-    const int64_t per = pl.chains * pl.slices;
-    auto all = [&](auto state) {
-        constexpr bool STATE = decltype(state)::value;
+    auto part = [&](bool ahead) {
+        p.ahead = ahead;
         if (pl.umma) {
-            if (int rc = umma_run(p, nb, STATE, redo, s)) return rc;
+            if (int rc = umma_run(p, nb, redo, s)) return rc;
         }
-        return launch<T, DK, VEC, STATE>(p, per * (STATE ? pl.nseg - 1 : pl.nseg), s);  // or what umma has left
+        // or what umma has left
+        if constexpr (VEC && std::is_same<T, __nv_bfloat16>::value)
+            if (ahead && p.lead) return launch<T, DK, VEC, MIXED>(p, pl, s);
+        return ahead ? launch<T, DK, VEC, STATES>(p, pl, s) : launch<T, DK, VEC, OUTPUTS>(p, pl, s);
     };
     p.redo = pl.umma ? redo : nullptr;
     if (pl.nseg > 1) {
-        if (int rc = all(std::true_type{})) return rc;
+        if (int rc = part(true)) return rc;
         const dim3 grid(static_cast<unsigned>(pl.chains), static_cast<unsigned>((int64_t(p.dk) * p.dv + 255) / 256));
         enter_kernel<<<grid, 256, 0, s>>>(p);
         const cudaError_t e = cudaGetLastError();
         if (e != cudaSuccess) return cuda_fail(e, "linear attention launch");
     }
-    return all(std::false_type{});
+    return part(false);
 }
 
 }  // namespace
@@ -787,7 +799,7 @@ int need_linear_attention(const need_linear_attention_args* a, need_stream_t str
     if ((pl.nseg > 1 || pl.umma) && (a->workspace == nullptr || (reinterpret_cast<uintptr_t>(a->workspace) & 3u) != 0 ||
                                      a->workspace_bytes < workspace_of(pl, a->dk, a->dv)))
         return fail(NEED_ERR_WORKSPACE, "linear attention: workspace missing, misaligned or too small");
-    p.slices = pl.slices, p.nseg = pl.nseg, p.seg_chunks = pl.seg_chunks;
+    p.slices = pl.slices, p.nseg = pl.nseg, p.lead = pl.lead, p.first_chunks = pl.first_chunks, p.seg_chunks = pl.seg_chunks;
     p.part = static_cast<float*>(a->workspace);
     p.part_d = p.part + pl.chains * (pl.nseg - 1) * a->dk * a->dv;
     uint32_t* redo = reinterpret_cast<uint32_t*>(p.part_d + pl.chains * (pl.nseg - 1));

@@ -27,11 +27,17 @@ struct AttnParams {
     int64_t ob, ot, oh;
     int64_t T;
     int32_t H, dk, dv, slices, nseg;
-    int32_t seg_chunks;   // chunks of a segment of the sequence
+    int64_t first_chunks, seg_chunks;  // of 64 tokens: of the first segment of the sequence, of the others
+    // The launch ahead runs all segments but the last for the state that they leave (from
+    // none); the one after it runs them for their outputs.  lead: the first one's outputs come
+    // ahead, and its state with them.
+    int32_t ahead, lead;
     float scale;
-    float* part;          // [chain, nseg - 1, dk, dv]: segments' own states, then those that enter the next
+    float* part;          // [chain, nseg - 1, dk, dv]: the segments' own states, then those that enter the next
     float* part_d;        // [chain, nseg - 1]: their decays, below 0 where a reset lies in between
     const uint32_t* redo; // of each block, null for all: whether it has to run
+    __host__ __device__ int launched() const { return ahead ? nseg - 1 : nseg - lead; }  // segments of this launch
+    __host__ __device__ int64_t segment(int s) const { return s == 0 ? 0 : first_chunks + (s - 1) * seg_chunks; }  // its first chunk
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -68,7 +74,7 @@ __device__ __forceinline__ float times_state(float d, float s) { return d == -1.
 // tokens, bf16, up to 128 features.  `redo` [blocks] tells which of attention_kernel's
 // blocks it leaves to that.  state: only the segments' states.
 bool umma_takes(const AttnParams& p, int64_t nb);
-int umma_run(const AttnParams& p, int64_t nb, bool state, uint32_t* redo, cudaStream_t stream);
+int umma_run(const AttnParams& p, int64_t nb, uint32_t* redo, cudaStream_t stream);
 
 }  // namespace attention
 }  // namespace need

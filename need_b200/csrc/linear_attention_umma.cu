@@ -33,8 +33,8 @@
 //
 // Measured: 16 x 4096 tokens, 16 heads of 64 x 64, 157 us (3.4 TB/s of the 541 MB that go in
 // and out; attention_kernel 349); 8 x 2048, 13 heads of 64 x 64, 44 us (104 chains leave 44 of
-// the 148 multiprocessors idle); 1 x 16384, 32 heads of 128 x 128, 346 us, in two segments of
-// each chain, the first run twice.  A chunk takes 2.0 us at 64 features (the MMAs 1.1, the
+// the 148 multiprocessors idle); 1 x 16384, 32 heads of 128 x 128, 283 us, in three segments
+// of each chain, the middle one run twice.  A chunk takes 2.0 us at 64 features (the MMAs 1.1, the
 // warps' work on P', outputs and state beside them about the whole) and 3.0 at 128 (the
 // MMAs 1.9; one buffer of P and of Q fits, so that P' waits for the outputs before it).
 #include <cuda.h>
@@ -254,7 +254,7 @@ __device__ __noinline__ void load_rows(uint32_t full, const CUtensorMap* tm, uin
 }
 
 // ------------------------------------------------------------------ the kernel
-template <int DK, bool STATE, int VP>
+template <int DK, int VP>
 __global__ void __launch_bounds__(kThreads, 1) umma_attention_kernel(const __grid_constant__ UmmaParams up) {
     using M = Map<DK>;
     constexpr int NQ = M::NQ, NK = M::NK, NV = M::NV, NP = M::NP;
@@ -275,12 +275,12 @@ __global__ void __launch_bounds__(kThreads, 1) umma_attention_kernel(const __gri
     Gates* const gates = reinterpret_cast<Gates*>(base + M::G);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint32_t nseg = STATE ? p.nseg - 1 : p.nseg, rest = blockIdx.x / nseg;
-    const int seg = static_cast<int>(blockIdx.x % nseg), slice = static_cast<int>(rest % p.slices);
+    const uint32_t segs = p.launched(), rest = blockIdx.x / segs;
+    const int seg = static_cast<int>(blockIdx.x % segs) + (p.ahead ? 0 : p.lead), slice = static_cast<int>(rest % p.slices);
+    const bool state = p.ahead && seg >= p.lead;  // only the state
     const int64_t chain = rest / p.slices;
     const int b = static_cast<int>(static_cast<uint32_t>(chain) / p.H), h = static_cast<int>(static_cast<uint32_t>(chain) % p.H), col0 = slice * DVS;
-    const int64_t first = int64_t(seg) * p.seg_chunks * 64;
-    const int64_t last = first + int64_t(p.seg_chunks) * 64 < p.T ? first + int64_t(p.seg_chunks) * 64 : p.T;
+    const int64_t first = p.segment(seg) * 64, last = p.segment(seg + 1) * 64 < p.T ? p.segment(seg + 1) * 64 : p.T;
     const int n = static_cast<int>((last - first + CT - 1) / CT);
     const float* ld = p.ld + b * p.lb + h * p.lh;
     const uint8_t* marks = p.seg == nullptr ? nullptr : p.seg + b * p.gb;
@@ -290,8 +290,8 @@ __global__ void __launch_bounds__(kThreads, 1) umma_attention_kernel(const __gri
 #pragma unroll 1
             for (int i = 0; i < n; ++i) mbar_init(x + i, count);
         };
-        init(full_q, NQ + NK + NV + GR, 1), init(gates_free, GR, STATE ? 8 : 16), init(k_free, NK, STATE ? 1 : 2);
-        init(v_free, NV, STATE ? 8 : 9), init(s_ready, 2, 8), init(qk_done, 5, 1), init(ds_free, 1, 8), init(p_ready, 2, 8);
+        init(full_q, NQ + NK + NV + GR, 1), init(gates_free, GR, state ? 8 : 16), init(k_free, NK, state ? 1 : 2);
+        init(v_free, NV, state ? 8 : 9), init(s_ready, 2, 8), init(qk_done, 5, 1), init(ds_free, 1, 8), init(p_ready, 2, 8);
         init(o_done, 2, 1), init(o_free, 2, 8), init(drain, 3, 1);
         *dead = 0, *bad_word = 0;
         fence_barrier_init();
@@ -317,7 +317,7 @@ __global__ void __launch_bounds__(kThreads, 1) umma_attention_kernel(const __gri
 
     if (warp < 8) {
         // ---------------------------------------------------------------- P', outputs
-        if constexpr (!STATE) {
+        if (!state) {
             const int quad = warp & 3, half = warp >> 2, r = 32 * quad + lane;
             __nv_bfloat16* const out = static_cast<__nv_bfloat16*>(p.out) + b * p.ob + h * p.oh + col0 + 32 * half;
             const int cols = p.dv - col0 - 32 * half;
@@ -427,7 +427,7 @@ __global__ void __launch_bounds__(kThreads, 1) umma_attention_kernel(const __gri
         const int m0 = (warp >= 12 ? NH : 0);  // its first tile
         float s[NH][4];  // transposed: rows j0 and + 8, columns 8 (m0 + m) + c2 and + 1
         {
-            const float* from = STATE ? nullptr : seg > 0 ? p.part + (chain * (p.nseg - 1) + seg - 1) * p.dk * int64_t(p.dv)
+            const float* from = state ? nullptr : seg > 0 ? p.part + (chain * (p.nseg - 1) + seg - 1) * p.dk * int64_t(p.dv)
                                       : p.s0 != nullptr   ? p.s0 + chain * p.dk * int64_t(p.dv) : nullptr;
 #pragma unroll
             for (int m = 0; m < NH; ++m)
@@ -467,7 +467,7 @@ __global__ void __launch_bounds__(kThreads, 1) umma_attention_kernel(const __gri
             arrive(vw_ready);
             arrive(gates_free + c % GR);
             arrive(v_free + c % NV);
-            if constexpr (!STATE) {  // the planes of the state that enters, as the K-major B of Q S
+            if (!state) {  // the planes of the state that enters, as the K-major B of Q S
                 if (c > 0) wait(qs_done + ((c - 1) & 1), (c - 1) >> 1);  // the last ones have been read
                 const uint32_t row = sb + M::S + umma::sw128(16 * quad + gr, 0) + c2 * 2;  // and the one 8 below, 1024 bytes on
 #pragma unroll
@@ -509,7 +509,7 @@ __global__ void __launch_bounds__(kThreads, 1) umma_attention_kernel(const __gri
             bad |= !(chk.x == 0.0f && chk.y == 0.0f);
         }
         if (bad) *bad_word = 1;
-        float* const to = STATE ? p.part + (chain * (p.nseg - 1) + seg) * p.dk * int64_t(p.dv)
+        float* const to = p.ahead ? p.part + (chain * (p.nseg - 1) + seg) * p.dk * int64_t(p.dv)
                                 : seg == p.nseg - 1 && p.sT != nullptr ? p.sT + chain * p.dk * int64_t(p.dv) : nullptr;
         if (to != nullptr)
 #pragma unroll
@@ -519,7 +519,7 @@ __global__ void __launch_bounds__(kThreads, 1) umma_attention_kernel(const __gri
                     const int i = 8 * (m0 + m) + c2 + (e & 1), j = j0 + (e >> 1) * 8;
                     if (i < p.dk && j < p.dv) to[int64_t(i) * p.dv + j] = s[m][e];
                 }
-        if (STATE && slice == 0 && bt == 0) p.part_d[chain * (p.nseg - 1) + seg] = total;
+        if (p.ahead && slice == 0 && bt == 0) p.part_d[chain * (p.nseg - 1) + seg] = total;
     } else if (warp == 16) {
         // ---------------------------------------------------------------- decays
         const float* at = ld + (first + 4 * lane) * p.lt;
@@ -556,7 +556,7 @@ __global__ void __launch_bounds__(kThreads, 1) umma_attention_kernel(const __gri
         auto load_k = [&](int c) { load(full_k + c % NK, &up.k, sb + M::K + c % NK * M::QB, M::QB, 0, h / p.k.share, c); };
         auto load_v = [&](int c) { load(full_v + c % NV, &up.v, sb + M::V + c % NV * M::VB, M::VB, col0, h / p.v.share, c); };
         if (warp == 17) {  // P = Q K^T of the chunk ahead, O2 = Q S
-            if constexpr (!STATE) {
+            if (!state) {
                 constexpr uint32_t ID_QK = umma::idesc_bf16(128, 128, umma::K_MAJOR, umma::K_MAJOR);
                 constexpr uint32_t ID_QS = umma::idesc_bf16(128, DVS, umma::K_MAJOR, umma::K_MAJOR);
     #pragma unroll 1
@@ -609,13 +609,13 @@ __global__ void __launch_bounds__(kThreads, 1) umma_attention_kernel(const __gri
 #pragma unroll 1
             for (int c = 0; c < NK; ++c) {
                 load_k(c);
-                if (STATE) load_v(c);
+                if (state) load_v(c);
             }
             for (int c = 0; c < n; ++c) {
                 if (c > 0) {
                     wait(k_free + (c - 1) % NK, (c - 1) / NK);
                     load_k(c - 1 + NK);
-                    if (STATE) {
+                    if (state) {
                         wait(v_free + (c - 1) % NV, (c - 1) / NV);
                         load_v(c - 1 + NV);
                     }
@@ -636,7 +636,7 @@ __global__ void __launch_bounds__(kThreads, 1) umma_attention_kernel(const __gri
                 }
                 __syncwarp();
             }
-        } else if constexpr (!STATE) {  // O1 = P' V
+        } else if (!state) {  // O1 = P' V
             constexpr uint32_t ID_PV = umma::idesc_bf16(128, DVS, umma::K_MAJOR, umma::MN_MAJOR);
 #pragma unroll 1
             for (int c = 0; c < NV; ++c) load_v(c);
@@ -673,9 +673,9 @@ __global__ void __launch_bounds__(kThreads, 1) umma_attention_kernel(const __gri
                     for (uint32_t i = 0; i < kPolls && !mbar_try_wait(full + c % ring, (c / ring) & 1); ++i) {
                     }
             };
-            if (warp == 17 && !STATE) landed(full_q, NQ);
+            if (warp == 17 && !state) landed(full_q, NQ);
             if (warp == 18) landed(full_k, NK);
-            if (warp == (STATE ? 18 : 19)) landed(full_v, NV);
+            if (warp == (state ? 18 : 19)) landed(full_v, NV);
         }
         __syncwarp();
     }
@@ -704,10 +704,10 @@ int encode(CUtensorMap* tm, const Stream& x, int64_t nb, int64_t T, int64_t head
 
 std::atomic<uint32_t> umma_polls{kPolls};
 
-template <int DK, bool STATE, int VP>
+template <int DK, int VP>
 int launch(const UmmaParams& up, int64_t blocks, cudaStream_t s) {
     static std::atomic<uint64_t> done{0};
-    auto kern = umma_attention_kernel<DK, STATE, VP>;
+    auto kern = umma_attention_kernel<DK, VP>;
     cudaError_t e = ensure_smem(kern, Map<DK>::BYTES, done);
     if (e != cudaSuccess) return cuda_fail(e, "linear attention shared memory");
     kern<<<static_cast<unsigned>(blocks), kThreads, Map<DK>::BYTES, s>>>(up);
@@ -729,7 +729,7 @@ bool umma_takes(const AttnParams& p, int64_t nb) {
     return p.T < (int64_t(1) << 31) - 256 && nb < (int64_t(1) << 31) && p.ob % 8 == 0 && p.ot % 8 == 0 && p.oh % 8 == 0;
 }
 
-int umma_run(const AttnParams& p, int64_t nb, bool state, uint32_t* redo, cudaStream_t stream) {
+int umma_run(const AttnParams& p, int64_t nb, uint32_t* redo, cudaStream_t stream) {
     if (int rc = ensure_context()) return rc;
     UmmaParams up{};
     up.a = p, up.redo = redo, up.polls = umma_polls.load(std::memory_order_relaxed);
@@ -737,11 +737,10 @@ int umma_run(const AttnParams& p, int64_t nb, bool state, uint32_t* redo, cudaSt
     if (int rc = encode(&up.q, p.q, nb, p.T, p.H / p.q.share, p.dk)) return rc;
     if (int rc = encode(&up.k, p.k, nb, p.T, p.H / p.k.share, p.dk)) return rc;
     if (int rc = encode(&up.v, p.v, nb, p.T, p.H / p.v.share, p.dv)) return rc;
-    const int64_t blocks = nb * p.H * p.slices * (state ? p.nseg - 1 : p.nseg);
+    const int64_t blocks = nb * p.H * p.slices * p.launched();
     auto go = [&](auto dk) {
         constexpr int DK = decltype(dk)::value;
-        if (state) return p.sT != nullptr ? launch<DK, true, 3>(up, blocks, stream) : launch<DK, true, 2>(up, blocks, stream);
-        return p.sT != nullptr ? launch<DK, false, 3>(up, blocks, stream) : launch<DK, false, 2>(up, blocks, stream);
+        return p.sT != nullptr ? launch<DK, 3>(up, blocks, stream) : launch<DK, 2>(up, blocks, stream);
     };
     return p.dk <= 64 ? go(std::integral_constant<int, 64>{}) : go(std::integral_constant<int, 128>{});
 }

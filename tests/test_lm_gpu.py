@@ -126,6 +126,27 @@ def test_attention_short_parts(cuda, T, dtype):
     check_attention(q, k, v, ld, 0.125, seg, s0)
 
 
+@pytest.mark.parametrize("H,T,dk,dv", [(52, 4000, 64, 64), (30, 2200, 128, 128), (40, 2700, 40, 64)])
+@pytest.mark.parametrize("resets", [0, 500])
+def test_attention_some_chains(cuda, H, T, dk, dv, resets):
+    """Two or three parts side by side, the first one's outputs ahead of the others'."""
+    q, k, v, ld, seg, s0 = make(cuda, 1, T, H, dk, dv, BF, state=True, resets=resets)
+    out, fin = check_attention(q, k, v, ld, dk ** -0.5, seg, s0)
+    bad = [t.clone() for t in (k, v)]
+    bad[0][0, 20, 1, 3], bad[1][0, 2000, 2, 5] = math.inf, math.nan  # in the first part, in a later one
+    got, last = nk.linear_attention(q, *bad, ld, scale=dk ** -0.5, seg_start=seg, state=s0, return_final_state=True)
+    rest = [h for h in range(H) if h not in (1, 2)]
+    assert torch.equal(got[:, :, rest], out[:, :, rest]) and torch.equal(last[:, rest], fin[:, rest])
+    _, _, mag, _ = ref.attention(q, k, v, ld, dk ** -0.5, seg, s0)
+    for h, t in ((1, 20), (2, 2000)):  # another kernel's sums there
+        close(got[:, :t, h], out[:, :t, h].double(), mag[:, :t, h], 2 * SUMS[BF], 2 * ref.HALF_STEP[BF])
+        assert not torch.isfinite(got[:, t, h]).all()
+        later = [] if seg is None else (seg[0, t + 1:] != 0).nonzero().flatten().tolist()
+        if later:  # the next segment is free of it
+            after = t + 1 + later[0]
+            close(got[:, after:, h], out[:, after:, h].double(), mag[:, after:, h], 2 * SUMS[BF], 2 * ref.HALF_STEP[BF])
+
+
 def test_attention_parts_and_batches_agree(cuda):
     """One sequence alone (cut into parts) and among many (not cut): the same but for fp32 sums."""
     q, k, v, ld, _, _ = make(cuda, 1, 2048, 2, 64, 64, F32, decay="head")
@@ -234,6 +255,18 @@ def test_attention_waits_given_up(cuda):
             torch.cuda.synchronize()
         finally:
             abi.load().need_test_linear_attention_polls(0)
+
+
+def test_attention_waits_given_up_in_parts(cuda):
+    from need_b200 import abi
+    lib = abi.load()
+    q, k, v, ld, seg, s0 = make(cuda, 1, 4000, 52, 64, 64, BF, state=True, resets=500)
+    try:
+        lib.need_test_linear_attention_polls(1)
+        check_attention(q, k, v, ld, 0.125, seg, s0, twice=False)
+    finally:
+        lib.need_test_linear_attention_polls(0)
+    check_attention(q, k, v, ld, 0.125, seg, s0)
 
 
 def test_attention_empty(cuda):
