@@ -118,8 +118,8 @@ Tensor linear_attention_step(const Tensor& q_, const Tensor& k_, const Tensor& v
     a.log_decay = ptr<float>(ld), a.ld_stride_h = ld.stride(-1), a.ld_stride_n = ld.dim() == 2 ? ld.stride(0) : 0;
     a.state = ptr<float>(state), a.state_stride = state.stride(0), a.slots = S, a.slot = ptr<int32_t>(slot);
     a.out = out.data_ptr(), a.out_stride_n = out.stride(0), a.out_stride_h = out.stride(1);
+    state.unsafeGetTensorImpl()->bump_version();  // or raises: an inference tensor outside its mode
     check("need_linear_attention_step", need_linear_attention_step(&a, on.stream));
-    state.unsafeGetTensorImpl()->bump_version();
     return out;
 }
 

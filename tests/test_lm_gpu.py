@@ -451,6 +451,29 @@ def test_norm_shapes_and_strides(cuda):
     assert torch.equal(one[1], n[0, 0, 0])
 
 
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("C,stride,at", [(1324, 1324, 0), (1324, 1326, 0), (1324, 1328, 2), (1326, 1326, 0), (64, 64, 1), (60, 68, 4), (2052, 2056, 8)])
+def test_norm_alignments(cuda, C, stride, at, dtype):
+    """Rows, weights and channels that 8, 4 or 2 bytes divide."""
+    g = gen(C + at, cuda)
+    flat = [torch.randn(5 * stride + at, device=cuda, generator=g).to(dtype) for _ in range(2)]
+    x, y = (t[at:].unflatten(0, (5, stride))[:, :C] for t in flat)
+    w = (1 + 0.1 * torch.randn(C + at, device=cuda, generator=g))[at:]
+    r, n = nk.residual_rms_norm(x, y, w, 1e-6, scale=0.7)
+    # one fp32 rounding of the sum (torch's expression has two: a tie may fall the other way) before r's own
+    close(r, x.double() + float(torch.tensor(0.7)) * y.double(), x.double().abs() + y.double().abs(), 2.0 ** -24, ref.HALF_STEP[dtype])
+    f = r.double()
+    want = f / (f.square().mean(-1, keepdim=True) + 1e-6).sqrt() * w.double()
+    close(n, want, want.abs(), 2.0 ** -18, ref.HALF_STEP[dtype])
+    for group in (32, 128, None):
+        r8, q, s = nk.residual_rms_norm(x, y, w, 1e-6, scale=0.7, out_dtype=F8, group=group)
+        size = group or C
+        val = q.double() * s.double().repeat_interleave(size, -1)[:, :C]
+        # e4m3: half a step of the value, or of its least step under the scale
+        lim = want.abs() * 2.0 ** -4 * (1 + 2.0 ** -7) + s.double().repeat_interleave(size, -1)[:, :C] * 2.0 ** -10
+        assert torch.equal(r8, r) and ((val - want).abs() <= lim).all()
+
+
 @pytest.mark.parametrize("group", [32, None])
 def test_norm_special_values(cuda, group):
     """Rows of zeros, a NaN, an infinity; the others are left as they are."""
@@ -817,6 +840,55 @@ def test_graphs(cuda):
         assert all(same(o, w) for o, w in zip(outs, want))
     for gr in graphs:
         gr.reset()
+
+
+def test_first_call_captured():
+    """A process whose first calls are captured into a graph."""
+    code = """
+import torch
+from need_b200 import need_kernels as nk
+q = torch.randn(1, 300, 2, 64, device="cuda").bfloat16()
+ld = torch.full((2,), -0.1, device="cuda")
+x, t, w, pool = q.flatten(2), torch.zeros(1, 300, dtype=torch.long, device="cuda"), torch.ones(128, device="cuda"), torch.zeros(1, 2, 64, 64, device="cuda")
+def calls():
+    y = nk.linear_attention(q, q, q, ld, scale=0.125)
+    z = nk.linear_attention_step(q[:, 0], q[:, 0], q[:, 0], ld, pool)
+    r, n = nk.residual_rms_norm(x, y.flatten(2), w)
+    return [y, z, r, n, *nk.token_log_probs(n, t, top=3)]
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    got = calls()
+g.replay()
+torch.cuda.synchronize()
+pool.zero_()
+assert all(torch.equal(a, b) for a, b in zip(got, calls()))
+"""
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
+
+
+def test_step_under_inference_mode(cuda):
+    q, k, v, ld, _, _ = make(cuda, 2, 1, 2, 32, 32, BF)
+    with torch.inference_mode():
+        pool = torch.zeros(2, 2, 32, 32, device=cuda)
+        nk.linear_attention_step(q[:, 0], k[:, 0], v[:, 0], ld[:, 0], pool)
+    before = pool.clone()
+    with pytest.raises(RuntimeError, match="inference tensor"):
+        nk.linear_attention_step(q[:, 0], k[:, 0], v[:, 0], ld[:, 0], pool)
+    assert torch.equal(pool, before) and before.any()
+
+
+def test_attention_broadcast_batch(cuda):
+    """Strides of 0: one k and v for the whole batch."""
+    q, k, v, ld, _, _ = make(cuda, 3, 200, 4, 64, 64, BF)
+    k1, v1 = (t[:1].expand(3, -1, -1, -1) for t in (k, v))
+    check_attention(q, k1, v1, ld, 0.125)
+    one = q[:, :1].expand(-1, 200, -1, -1)
+    check_attention(one, k, v, ld, 0.125)
 
 
 def test_no_synchronisation(cuda):
