@@ -59,7 +59,7 @@ constexpr int DVS = 64;      // columns of v of a CTA
 constexpr int kThreads = 640;
 constexpr int GR = 4;        // chunks whose decays are held
 constexpr uint32_t kPolls = 1u << 16;  // of a wait before it is given up
-constexpr uint32_t kTmem = 512, T_O1 = 0, T_O2 = 64, T_DS = 192;  // tensor memory columns
+constexpr uint32_t kTmem = 512, T_O1 = 0;  // tensor memory columns
 
 struct alignas(16) Gates {
     float hi[CT], lo[CT], w[CT], eg[CT];  // as Decays
@@ -77,8 +77,8 @@ struct Map {  // shared memory, from a 1024-byte aligned base
     static constexpr int NQ = DK == 64 ? 2 : 1, NK = DK == 64 ? 3 : 2, NV = NK;  // chunks loaded ahead
     // buffers of P (tensor memory holds a second one at 64 features; at 128 in the place of O2's
     // second, which took longer: 1x16384 32x128 406 us against 343)
-    static constexpr int NP = DK == 64 ? 2 : 1;
-    static constexpr uint32_t T_P = T_DS + DK;
+    static constexpr int NP = DK == 64 ? 2 : 1, NO = 3 - NP;  // NO: of O1
+    static constexpr uint32_t T_O2 = T_O1 + NO * DVS, T_DS = T_O2 + 2 * DVS, T_P = T_DS + DK;
     static_assert(T_P + NP * 128 <= kTmem, "tensor memory");
     static constexpr int QB = CT * DK * 2, VB = CT * DVS * 2, SB = DVS * DK * 2;
     static constexpr int Q = 0, K = Q + NQ * QB, V = K + NK * QB, W = V + NV * VB, S = W + 3 * VB, G = S + 2 * SB;
@@ -165,20 +165,6 @@ __device__ __forceinline__ void tmem_ld_half(uint32_t taddr, float (&v)[16]) {
         : "r"(taddr));
 #pragma unroll
     for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
-}
-__device__ __forceinline__ void tmem_ld_half(uint32_t taddr, float (&v)[32]) {
-    uint32_t r[32];
-    asm volatile(
-        "tcgen05.ld.sync.aligned.16x256b.x8.b32 "
-        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
-          "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
-          "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
-          "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-        : "r"(taddr));
-#pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
 }
 
 // ------------------------------------------------------------------ decays
@@ -327,8 +313,8 @@ __global__ void __launch_bounds__(kThreads, 1) umma_attention_kernel(const __gri
                 wait(qs_done + (c & 1), c >> 1);
                 umma::fence_after_sync();
                 float x[32], y[32];
-                umma::tmem_ld32(tmem + T_O1 + 32 * half + lanes, x);
-                umma::tmem_ld32(tmem + T_O2 + 64 * (c & 1) + 32 * half + lanes, y);
+                umma::tmem_ld32(tmem + T_O1 + DVS * (c % M::NO) + 32 * half + lanes, x);
+                umma::tmem_ld32(tmem + M::T_O2 + DVS * (c & 1) + 32 * half + lanes, y);
                 umma::tmem_wait_ld();
                 umma::fence_before_sync();
                 arrive(o_free + (c & 1));
@@ -437,36 +423,43 @@ __global__ void __launch_bounds__(kThreads, 1) umma_attention_kernel(const __gri
                     s[m][e] = from != nullptr && i < p.dk && j < p.dv ? from[int64_t(i) * p.dv + j] : 0.0f;
                 }
         }
-        float total = 1.0f;
+        float total = 1.0f, d, d_next = 0.0f;
         bool bad = false;
-        for (int c = 0; c < n; ++c) {
+        float2 vw[16];  // of the next chunk, 4 rows 32 apart: made while its predecessor's dS is
+        auto fetch = [&](int c) {
             const Gates& g = gates[c % GR];
             wait(full_v + c % NV, c / NV);
             wait(gates_full + c % GR, c / GR);
-            const unsigned char *vt = base + M::V + (c % NV) * M::VB + umma::sw128(bt / 8, bt % 8);  // rows 32 apart: 4096 bytes
-            unsigned char* const wt = base + M::W + umma::sw128(bt / 8, bt % 8);
-            const float d = g.d;
-            bad |= g.wild != 0;
-            total = total == -1.0f || d == -1.0f ? -1.0f : total * d;
-            uint4 u[4];
-            float w[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) u[i] = *reinterpret_cast<const uint4*>(vt + 4096 * i), w[i] = g.w[bt / 8 + 32 * i];
-            // (the planes of the last chunk have been read: its dS is there)
+            const unsigned char* vt = base + M::V + (c % NV) * M::VB + umma::sw128(bt / 8, bt % 8);  // rows 32 apart: 4096 bytes
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const uint32_t x[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
+                const uint4 u = *reinterpret_cast<const uint4*>(vt + 4096 * i);
+                const float2 w = splat(g.w[bt / 8 + 32 * i]);
+                vw[4 * i] = __fmul2_rn(w, unpack_bf16(u.x)), vw[4 * i + 1] = __fmul2_rn(w, unpack_bf16(u.y));
+                vw[4 * i + 2] = __fmul2_rn(w, unpack_bf16(u.z)), vw[4 * i + 3] = __fmul2_rn(w, unpack_bf16(u.w));
+            }
+            d_next = g.d;
+            bad |= g.wild != 0;
+            total = total == -1.0f || d_next == -1.0f ? -1.0f : total * d_next;
+            arrive(gates_free + c % GR);
+            arrive(v_free + c % NV);
+        };
+        fetch(0);
+        for (int c = 0; c < n; ++c) {
+            // (the planes of the last chunk have been read: its dS is there)
+            unsigned char* const wt = base + M::W + umma::sw128(bt / 8, bt % 8);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
                 uint32_t pl[4][VP];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) split<VP>(__fmul2_rn(splat(w[i]), unpack_bf16(x[e])), pl[e]);
+                for (int e = 0; e < 4; ++e) split<VP>(vw[4 * i + e], pl[e]);
 #pragma unroll
                 for (int a = 0; a < VP; ++a)
                     *reinterpret_cast<uint4*>(wt + a * M::VB + 4096 * i) = make_uint4(pl[0][a], pl[1][a], pl[2][a], pl[3][a]);
             }
             fence_proxy_async_shared();
             arrive(vw_ready);
-            arrive(gates_free + c % GR);
-            arrive(v_free + c % NV);
+            d = d_next;
             if (!state) {  // the planes of the state that enters, as the K-major B of Q S
                 if (c > 0) wait(qs_done + ((c - 1) & 1), (c - 1) >> 1);  // the last ones have been read
                 const uint32_t row = sb + M::S + umma::sw128(16 * quad + gr, 0) + c2 * 2;  // and the one 8 below, 1024 bytes on
@@ -484,28 +477,34 @@ __global__ void __launch_bounds__(kThreads, 1) umma_attention_kernel(const __gri
                 fence_proxy_async_shared();
                 arrive(s_ready);
             }
+            if (c + 1 < n) fetch(c + 1);
             wait(ds_done, c);
             umma::fence_after_sync();
-            float x[NH * 4];
-            tmem_ld_half(tmem + T_DS + 8 * m0 + lanes, x);
-            umma::tmem_wait_ld();
-            umma::fence_before_sync();
-            arrive(ds_free);
             // an infinity or NaN of k or v leaves one here, under a weight of 0 too (V w is a NaN
             // then): a sum of 0 x is 0 otherwise
             float2 chk = splat(0.0f);
             const float2 dd = splat(d == -1.0f ? 0.0f : d);
 #pragma unroll
-            for (int m = 0; m < NH; ++m)
-#pragma unroll
-                for (int e = 0; e < 4; e += 2) {
-                    const float2 z = make_float2(x[4 * m + e], x[4 * m + e + 1]);
-                    float2 y = make_float2(s[m][e], s[m][e + 1]);
-                    if (d == -1.0f) y = splat(0.0f);  // whatever it holds
-                    chk = __ffma2_rn(z, splat(0.0f), chk);
-                    y = __ffma2_rn(dd, y, z);
-                    s[m][e] = y.x, s[m][e + 1] = y.y;
+            for (int m1 = 0; m1 < NH; m1 += 4) {
+                float x[16];
+                tmem_ld_half(tmem + M::T_DS + 8 * (m0 + m1) + lanes, x);
+                umma::tmem_wait_ld();
+                if (m1 + 4 == NH) {
+                    umma::fence_before_sync();
+                    arrive(ds_free);
                 }
+#pragma unroll
+                for (int m = 0; m < 4; ++m)
+#pragma unroll
+                    for (int e = 0; e < 4; e += 2) {
+                        const float2 z = make_float2(x[4 * m + e], x[4 * m + e + 1]);
+                        float2 y = make_float2(s[m1 + m][e], s[m1 + m][e + 1]);
+                        if (d == -1.0f) y = splat(0.0f);  // whatever it holds
+                        chk = __ffma2_rn(z, splat(0.0f), chk);
+                        y = __ffma2_rn(dd, y, z);
+                        s[m1 + m][e] = y.x, s[m1 + m][e + 1] = y.y;
+                    }
+            }
             bad |= !(chk.x == 0.0f && chk.y == 0.0f);
         }
         if (bad) *bad_word = 1;
@@ -591,7 +590,7 @@ __global__ void __launch_bounds__(kThreads, 1) umma_attention_kernel(const __gri
                             for (int a = 1; a >= 0; --a)
 #pragma unroll 4
                                 for (int k = 0; k < DK / 16; ++k)
-                                    umma::mma_bf16(tmem + T_O2 + 64 * (l & 1), q0 + (((k >> 2) * (CT * 128) + 32 * (k & 3)) >> 4),
+                                    umma::mma_bf16(tmem + M::T_O2 + DVS * (l & 1), q0 + (((k >> 2) * (CT * 128) + 32 * (k & 3)) >> 4),
                                                    s0 + ((a * M::SB + (k >> 2) * (DVS * 128) + 32 * (k & 3)) >> 4), ID_QS, a < 1 || k > 0);
                             umma::mma_commit(qs_done + (l & 1));
                         }
@@ -630,7 +629,7 @@ __global__ void __launch_bounds__(kThreads, 1) umma_attention_kernel(const __gri
                     for (int a = VP - 1; a >= 0; --a)  // the smallest products first
 #pragma unroll
                         for (int k = 0; k < CT / 16; ++k)
-                            umma::mma_bf16(tmem + T_DS, w0 + ((a * M::VB + 2048 * k) >> 4), k0 + (2048 * k >> 4), ID_VK, a < VP - 1 || k > 0);
+                            umma::mma_bf16(tmem + M::T_DS, w0 + ((a * M::VB + 2048 * k) >> 4), k0 + (2048 * k >> 4), ID_VK, a < VP - 1 || k > 0);
                     umma::mma_commit(ds_done);
                     umma::mma_commit(k_free + c % NK);
                 }
@@ -647,7 +646,7 @@ __global__ void __launch_bounds__(kThreads, 1) umma_attention_kernel(const __gri
                 }
                 wait(full_v + c % NV, c / NV);
                 wait(p_ready + (c & 1), c >> 1);
-                if (c > 0) wait(o_free + ((c - 1) & 1), (c - 1) >> 1);  // the last outputs have been read
+                if (c >= M::NO) wait(o_free + ((c - M::NO) & 1), (c - M::NO) >> 1);  // the outputs in O1's place have been read
                 umma::fence_after_sync();
                 if (elect_one()) {
                     const uint32_t tp = tmem + M::T_P + 128 * (c % NP);
@@ -656,7 +655,7 @@ __global__ void __launch_bounds__(kThreads, 1) umma_attention_kernel(const __gri
                     for (int a = 1; a >= 0; --a)
 #pragma unroll
                         for (int k = 0; k < CT / 16; ++k)
-                            mma_ts(tmem + T_O1, tp + 16 * k + 8 * a, v0 + (2048 * k >> 4), ID_PV, a < 1 || k > 0);
+                            mma_ts(tmem + T_O1 + DVS * (c % M::NO), tp + 16 * k + 8 * a, v0 + (2048 * k >> 4), ID_PV, a < 1 || k > 0);
                     umma::mma_commit(o_done + (c & 1));
                     umma::mma_commit(v_free + c % NV);
                 }
