@@ -239,6 +239,16 @@ __device__ __noinline__ void load_rows(uint32_t full, const CUtensorMap* tm, uin
     __syncwarp();
 }
 
+// The same rows into L2.
+__device__ __forceinline__ void prefetch_rows(const CUtensorMap* tm, int bytes, int head, int t, int b) {
+    if (elect_one())
+#pragma unroll 1
+        for (int j = 0; j < bytes; j += CT * 128)
+            asm volatile("cp.async.bulk.prefetch.tensor.4d.L2.global.tile [%0, {%1, %2, %3, %4}];" ::"l"(tm), "r"(j / 256), "r"(head), "r"(t), "r"(b)
+                         : "memory");
+    __syncwarp();
+}
+
 // ------------------------------------------------------------------ the kernel
 template <int DK, int VP>
 __global__ void __launch_bounds__(kThreads, 1) umma_attention_kernel(const __grid_constant__ UmmaParams up) {
@@ -600,6 +610,7 @@ __global__ void __launch_bounds__(kThreads, 1) umma_attention_kernel(const __gri
                             load_q(l + NQ);
                         }
                     }
+                    if (NQ == 1 && c + 1 < n) prefetch_rows(&up.q, M::QB, h / p.q.share, static_cast<int>(first) + (c + 1) * CT, b);
                     if (NQ == 1 && c < n) scores();
                 }
             }
