@@ -686,9 +686,9 @@ constexpr int held(bool small) {
 // features 14.3 and 18.2 us at 512 tokens, 22.3 and 18.8 at 1024; 64 fp16 ones 13.8 and 17.7
 // at 128 tokens, 24 and 21.6 at 256, 385 and 171 at 4096; 104 fp32 ones 521 and 475 at 4096.
 // umma may also run one segment more, the first for its outputs ahead (lead): of two places a
-// chain, 1x16384 32x128 takes 282 us, 347 without and 384 uncut, 52 chains of 64 features at
-// 4096 tokens 62, 74 and 71.  (In attention_kernel the choice at run time costs more: 16
-// x 2048, 8 heads of 128 x 128 in fp32 431 us, 391 without.)
+// chain, 1x16384 32x128 took 282 us, 347 without and 384 uncut, 52 chains of 64 features at
+// 4096 tokens 62, 74 and 71.  (In attention_kernel the choice at run time costs more: 8 x 1024
+// tokens, 13 heads of 128 x 128 in fp32, 431 us, 391 without.)
 Plan plan(bool umma, int32_t dtype, int64_t nb, int64_t T, int64_t H, int64_t dk, int64_t dv) {
     Plan pl{};
     pl.umma = umma;

@@ -8,7 +8,8 @@
 //
 //   P    = Q K^T                 128 x 128
 //   O2   = Q S                   128 x 64           S: 2 planes, shared memory; two buffers
-//   O1   = P' V                  128 x 64           P' = P with its decays, 2 planes, in P's place
+//   O1   = P' V                  128 x 64           P' = P with its decays, 2 planes, in P's place; two buffers at
+//                                                   128 features, where P has one
 //   dS^T = (V w)^T K             64 x features      V w: 3 planes, shared memory
 //   out  = O1 + e^G O2,  S' = e^{G_end} S + dS
 //
@@ -33,10 +34,11 @@
 //
 // Measured: 16 x 4096 tokens, 16 heads of 64 x 64, 157 us (3.4 TB/s of the 541 MB that go in
 // and out; attention_kernel 349); 8 x 2048, 13 heads of 64 x 64, 44 us (104 chains leave 44 of
-// the 148 multiprocessors idle); 1 x 16384, 32 heads of 128 x 128, 283 us, in three segments
+// the 148 multiprocessors idle); 1 x 16384, 32 heads of 128 x 128, 253 us, in three segments
 // of each chain, the middle one run twice.  A chunk takes 2.0 us at 64 features (the MMAs 1.1, the
-// warps' work on P', outputs and state beside them about the whole) and 3.0 at 128 (the
-// MMAs 1.9; one buffer of P and of Q fits, so that P' waits for the outputs before it).
+// warps' work on P', outputs and state beside them about the whole) and 2.9 at 128 (the
+// MMAs 1.9; one buffer of Q fits, which the products with K and S must have left before
+// the next chunk's 32 KB come, and those take a third of the time).
 #include <cuda.h>
 #include <cuda_bf16.h>
 
