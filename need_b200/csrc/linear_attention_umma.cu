@@ -625,12 +625,12 @@ __global__ void __launch_bounds__(kThreads, 1) umma_attention_kernel(const __gri
             }
             for (int c = 0; c < n; ++c) {
                 if (c > 0) {
-                    wait(k_free + (c - 1) % NK, (c - 1) / NK);
-                    load_k(c - 1 + NK);
                     if (state) {
                         wait(v_free + (c - 1) % NV, (c - 1) / NV);
                         load_v(c - 1 + NV);
                     }
+                    wait(k_free + (c - 1) % NK, (c - 1) / NK);
+                    load_k(c - 1 + NK);
                 }
                 wait(full_k + c % NK, c / NK);
                 wait(vw_ready, c);
