@@ -210,7 +210,7 @@ __device__ __forceinline__ void add(const float (&x)[K], float m, float c, float
 
 // ------------------------------------------------------------------ keys
 __device__ __forceinline__ u64 key_of(float x, int64_t i) {
-    const uint32_t v = x != x ? 0xffffffffu : static_cast<uint32_t>(order(x)) ^ 0x80000000u;
+    const uint32_t v = x != x ? 0xffffffffu : static_cast<uint32_t>(order(x + 0.0f)) ^ 0x80000000u;  // -0 as 0
     return (static_cast<u64>(v) << 32) | (0xffffffffu - static_cast<uint32_t>(i));
 }
 __device__ __forceinline__ float value_of(u64 k) {

@@ -612,6 +612,17 @@ def test_logp_ties(cuda, V):
     check_logp(y, torch.zeros(3, dtype=torch.long, device=cuda), top=32)
 
 
+@pytest.mark.parametrize("dtype", [BF, HF, F32])
+@pytest.mark.parametrize("V,top", [(50, 32), (700, 5), (30000, 20)])
+def test_logp_zeros_of_both_signs(cuda, V, top, dtype):
+    """-0 and 0 are equal: the lower token first."""
+    g = gen(V, cuda)
+    x = -torch.rand(5, V, device=cuda, generator=g)
+    x[torch.rand(5, V, device=cuda, generator=g) < 0.5] = 0.0
+    x[torch.rand(5, V, device=cuda, generator=g) < 0.4] = -0.0
+    check_logp(x.to(dtype), torch.zeros(5, dtype=torch.long, device=cuda), top=top)
+
+
 def test_logp_sure_of_it(cuda):
     """Probabilities near 1: log p and the entropy keep their relative precision."""
     for V in (784, 20000):
