@@ -320,6 +320,7 @@ __global__ void __launch_bounds__(kThreads, 1) umma_attention_kernel(const __gri
             __nv_bfloat16* const out = static_cast<__nv_bfloat16*>(p.out) + b * p.ob + h * p.oh + col0 + 32 * half;
             const int cols = p.dv - col0 - 32 * half;
             float eg_last = 0.0f, row_last = 0.0f;  // of the chunk whose outputs come next
+            bool reach_last = false;                // whether the entering state reaches its row
             auto outputs = [&](int c) {  // 32 columns of chunk c
                 wait(o_done + (c & 1), c >> 1);
                 wait(qs_done + (c & 1), c >> 1);
@@ -338,7 +339,7 @@ __global__ void __launch_bounds__(kThreads, 1) umma_attention_kernel(const __gri
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
                         float2 z = __fmul2_rn(splat(row_last), make_float2(x[e + 2 * i], x[e + 2 * i + 1]));
-                        if (eg_last >= 0.0f) z = __ffma2_rn(splat(eg_last), make_float2(y[e + 2 * i], y[e + 2 * i + 1]), z);
+                        if (reach_last) z = __ffma2_rn(splat(eg_last), make_float2(y[e + 2 * i], y[e + 2 * i + 1]), z);
                         w[i] = pack_bf16(z.x, z.y);
                     }
                     if (t >= p.T) continue;
@@ -354,11 +355,12 @@ __global__ void __launch_bounds__(kThreads, 1) umma_attention_kernel(const __gri
             };
 #pragma unroll 1
             for (int c = 0; c <= n; ++c) {  // P' of chunk c, the outputs of the one before it
-                float eg = 0.0f, row = 0.0f;  // of the chunk; eg below 0: the entering state does not reach the row
+                float eg = 0.0f, row = 0.0f;  // of the chunk
+                bool reach = false;
                 if (c < n) {
                 const Gates& g = gates[c % GR];
                 wait(gates_full + c % GR, c / GR);
-                eg = g.seg[r] == 0 ? g.eg[r] : -1.0f, row = g.row[r];
+                eg = g.eg[r], row = g.row[r], reach = g.seg[r] == 0;
                 const bool factors = g.factors != 0;
                 wait(qk_done + (c & 1), c >> 1);
                 umma::fence_after_sync();
@@ -414,7 +416,7 @@ __global__ void __launch_bounds__(kThreads, 1) umma_attention_kernel(const __gri
                 arrive(gates_free + c % GR);
                 }
                 if (c > 0) outputs(c - 1);
-                eg_last = eg, row_last = row;
+                eg_last = eg, row_last = row, reach_last = reach;
             }
         }
     } else if (warp < 16) {

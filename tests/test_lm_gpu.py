@@ -100,6 +100,16 @@ def test_attention_decays(cuda, decay, dtype):
     check_attention(q, k, v, ld, 1.0, (torch.arange(300, device=cuda) % 37 == 5).expand(2, 300), s0)
 
 
+@pytest.mark.parametrize("dtype", [BF, HF, F32])
+@pytest.mark.parametrize("scale", [-0.125, -3.0, 0.0])
+@pytest.mark.parametrize("B,T,H,dk,dv", [(2, 65, 3, 64, 64), (2, 300, 3, 64, 72), (1, 300, 2, 128, 64), (1, 3000, 2, 64, 64)])
+def test_attention_scales(cuda, B, T, H, dk, dv, scale, dtype):
+    """Of either sign and 0, with a state, whole and cut into parts."""
+    q, k, v, ld, seg, s0 = make(cuda, B, T, H, dk, dv, dtype, state=True, resets=170)
+    check_attention(q, k, v, ld, scale, None, s0)
+    check_attention(q, k, v, ld, scale, seg, s0)
+
+
 def test_attention_decay_strides(cuda):
     q, k, v, ld, _, _ = make(cuda, 2, 100, 4, 32, 32, BF)
     want = nk.linear_attention(q, k, v, ld)
