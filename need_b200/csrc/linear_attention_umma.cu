@@ -19,7 +19,7 @@
 //
 //   warps 0-7    P' and the outputs: two for each 32 rows, a row per thread.  A decay is a row's
 //                factor, which can wait for the outputs, times a column's -- but in a chunk that a
-//                segment starts in, or that decays by more than 2^-64
+//                segment starts in, or that decays by more than 2^-64 or grows by more than 2^32
 //   warps 8-15   V w, the check for infinities, the state and its planes
 //   warp 16      the decays of the chunks ahead
 //   warps 17-19  the MMAs, each with the loads (TMA, no multicast) whose place they free: P and
@@ -210,15 +210,23 @@ __device__ __forceinline__ void make_gates(const float (&x)[4], float scale, Gat
     Sum2 before = of((lane + 31) & 31);
     if (lane == 0) before = {0.0f, 0.0f};
     const Sum2 end = of(31);
-    // a row's factor is up to 2^64 then
-    const bool factors = send == 0 && end.hi > -64.0f;
+    // a row's factor is up to 2^64 then, a column's up to 2^32 (more than 1 only where states grow), and
+    // neither falls below what bf16 holds
+    bool near = send == 0 && end.hi > -64.0f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        G[e] = add(before, G[e]);
+        const float d = minus(G[e], end);
+        near = near && d < 64.0f && d > -32.0f;
+    }
+    const bool factors = __all_sync(0xffffffffu, near);
     float4 hi, lo, w, eg, be;
     int4 seg;
     float *ph = &hi.x, *pl = &lo.x, *pw = &w.x, *pe = &eg.x, *pb = &be.x;
     int* ps = &seg.x;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-        const Sum2 t = add(before, G[e]);
+        const Sum2 t = G[e];
         s += reset[e] ? 1 : 0;
         ph[e] = t.hi, pl[e] = t.lo, ps[e] = s;
         pw[e] = s == send ? ex2(minus(end, t)) : 0.0f;

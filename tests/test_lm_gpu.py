@@ -110,6 +110,30 @@ def test_attention_scales(cuda, B, T, H, dk, dv, scale, dtype):
     check_attention(q, k, v, ld, scale, seg, s0)
 
 
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("grow,n,then,m", [(0.5, 120, -100.0, 1), (0.5, 100, -90.0, 1), (0.4, 90, -90.0, 1), (0.5, 40, -20.0, 1),
+                                           (-1.0, 80, 0.5, 80), (0.5, 128, 0.0, 1)])
+def test_attention_grows_and_forgets(cuda, grow, n, then, m, dtype):
+    """`n` tokens of one log decay, `m` of another sign, then none; within a chunk, across two,
+    and with segments' starts between.  An exponent of 2 below 128 is off by 2^-18 as a float, so
+    that each of the three factors of a term (to a chunk's end, over a chunk, from its start) is
+    off by ln 2 2^-18 beside what the bounds count: under 2^-16 together."""
+    q, k, v, _, _, s0 = make(cuda, 2, 384, 2, 64, 64, dtype, state=True)
+    one = torch.zeros(384, device=cuda)
+    one[:n], one[n:n + m] = grow, then
+    ld = torch.zeros(2, 384, 2, device=cuda)
+    ld[0, :, 0] = ld[1, :, 1] = one
+    ld[0, 70:, 1], ld[1, 17:, 0] = one[:314], one[:367]
+    seg = torch.zeros(2, 384, dtype=torch.uint8, device=cuda)
+    seg[:, [60, 200]] = 1
+    for marks in (None, seg):
+        out, fin = nk.linear_attention(q, k, v, ld, scale=0.125, seg_start=marks, state=s0, return_final_state=True)
+        want, s, mag, ms = ref.attention(q, k, v, ld, 0.125, marks, s0)
+        close(out, want, mag, SUMS[dtype] + 2.0 ** -16, ref.HALF_STEP[dtype])
+        close(fin, s, ms, STATE + 2.0 ** -16)
+        close(nk.linear_attention(q, k, v, ld, scale=0.125, seg_start=marks, state=s0), want, mag, SUMS[dtype] + 2.0 ** -16, ref.HALF_STEP[dtype])
+
+
 def test_attention_decay_strides(cuda):
     q, k, v, ld, _, _ = make(cuda, 2, 100, 4, 32, 32, BF)
     want = nk.linear_attention(q, k, v, ld)
