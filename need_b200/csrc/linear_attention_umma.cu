@@ -445,7 +445,7 @@ __global__ void __launch_bounds__(kThreads, 1) umma_attention_kernel(const __gri
                     s[m][e] = from != nullptr && i < p.dk && j < p.dv ? from[int64_t(i) * p.dv + j] : 0.0f;
                 }
         }
-        float total = 1.0f, d, d_next = 0.0f;
+        float d, d_next = 0.0f;
         bool bad = false;
         float2 vw[16];  // of the next chunk, 4 rows 32 apart: made while its predecessor's dS is
         auto fetch = [&](int c) {
@@ -462,7 +462,6 @@ __global__ void __launch_bounds__(kThreads, 1) umma_attention_kernel(const __gri
             }
             d_next = g.d;
             bad |= g.wild != 0;
-            total = total == -1.0f || d_next == -1.0f ? -1.0f : total * d_next;
             arrive(gates_free + c % GR);
             arrive(v_free + c % NV);
         };
@@ -540,7 +539,6 @@ __global__ void __launch_bounds__(kThreads, 1) umma_attention_kernel(const __gri
                     const int i = 8 * (m0 + m) + c2 + (e & 1), j = j0 + (e >> 1) * 8;
                     if (i < p.dk && j < p.dv) to[int64_t(i) * p.dv + j] = s[m][e];
                 }
-        if (p.ahead && slice == 0 && bt == 0) p.part_d[chain * (p.nseg - 1) + seg] = total;
     } else if (warp == 16) {
         // ---------------------------------------------------------------- decays
         const float* at = ld + (first + 4 * lane) * p.lt;
@@ -557,6 +555,8 @@ __global__ void __launch_bounds__(kThreads, 1) umma_attention_kernel(const __gri
             if (marks != nullptr) mark += CT * p.gt;
         };
         fetch(0);
+        double* const total = reinterpret_cast<double*>(base + M::BAR + 504);  // the segment's decay, lane 0's: no registers for it
+        if (lane == 0) *total = 1.0;
 #pragma unroll 1
         for (int c = 0; c < n; ++c) {
             float now[4];
@@ -565,8 +565,10 @@ __global__ void __launch_bounds__(kThreads, 1) umma_attention_kernel(const __gri
             if (c + 1 < n) fetch(c + 1);
             if (c >= GR) wait(gates_free + c % GR, c / GR - 1);
             make_gates(now, p.scale, gates[c % GR]);
+            if (lane == 0) *total = *total == -1.0 || gates[c % GR].d == -1.0f ? -1.0 : *total * gates[c % GR].d;
             arrive(gates_full + c % GR);
         }
+        if (p.ahead && slice == 0 && lane == 0) put_decay(p.part_d + 2 * (chain * (p.nseg - 1) + seg), *total);
     } else {
         // ---------------------------------------------------------------- MMAs and loads
         const uint64_t desc_k = umma::smem_desc(sb, 16, 1024), desc_mn = umma::smem_desc(sb, CT * 128, 1024);  // + bytes / 16

@@ -193,6 +193,34 @@ def test_attention_parts_and_batches_agree(cuda):
 
 
 @pytest.mark.parametrize("dtype", [BF, HF, F32])
+def test_attention_parts_grow_from_nothing(cuda, dtype):
+    """A growing prefix of zero keys (padding on the left): a state of 0 stays 0, though what the
+    prefix would multiply it with is past fp32 (e^256 a part and more)."""
+    q, k, v, _, _, _ = make(cuda, 1, 2200, 30, 64, 64, dtype)
+    k[:, :1400] = 0
+    ld = torch.zeros(1, 2200, 30, device=cuda)
+    ld[:, :1400] = 0.5
+    out, fin = check_attention(q, k, v, ld, 0.125)
+    assert (out[:, :1400] == 0).all() and torch.isfinite(fin).all()
+
+
+@pytest.mark.parametrize("dtype,grow,start,n", [(BF, 0.2, 256, 700), (F32, 0.5, 0, 280)])
+def test_attention_parts_grow_from_little(cuda, dtype, grow, start, n):
+    """States of 1e-30 that grow by e^140, over e^88 of it in one part: 1e30 is left.  The chunks'
+    exponents (202 together, 2^-24 of each lost: ln 2 2^-16.3) and their ex2 (2^-22 each of 22) beside
+    what the bounds count: under 2^-15."""
+    q, k, v, _, _, s0 = make(cuda, 1, 2200, 30, 64, 64, dtype, state=True)
+    k[:, :start + n] = 0
+    ld = torch.zeros(1, 2200, 30, device=cuda)
+    ld[:, start:start + n] = grow
+    s0 = s0 * 1e-30
+    out, fin = nk.linear_attention(q, k, v, ld, scale=0.125, state=s0, return_final_state=True)
+    want, s, mag, m = ref.attention(q, k, v, ld, 0.125, None, s0)
+    close(out, want, mag, SUMS[dtype] + 2.0 ** -15, ref.HALF_STEP[dtype])
+    close(fin, s, m, STATE + 2.0 ** -15)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF, F32])
 def test_attention_views(cuda, dtype):
     """Chunks of a projection, heads before tokens, features apart, rows at odd offsets."""
     g = gen(3, cuda)
