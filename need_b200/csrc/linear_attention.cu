@@ -336,8 +336,7 @@ __global__ void __launch_bounds__(kThreads, DK == 64 && Split<T>::IN < 3 ? 3 : 2
                 s[n][e] = from != nullptr && i < p.dk && j < p.dv ? from[int64_t(i) * p.dv + j] : 0.0f;
             }
     }
-    __shared__ double s_total;  // the segment's decay: thread 0's, which has no registers for it
-    if (KIND != OUTPUTS && threadIdx.x == 0) s_total = 1.0;
+    double total = 1.0;  // the segment's decay
 
     using B16 = __nv_bfloat16;
     const B16 *qc = reinterpret_cast<const B16*>(q), *kc = reinterpret_cast<const B16*>(k), *vc = reinterpret_cast<const B16*>(v);
@@ -383,7 +382,7 @@ __global__ void __launch_bounds__(kThreads, DK == 64 && Split<T>::IN < 3 ? 3 : 2
             issue(c + 1);
             if (warp == 0) next = load_decays(p, ld, marks, t0 + C);
         }
-        if (KIND != OUTPUTS && threadIdx.x == 0) s_total = s_total == -1.0 || gt.d == -1.0f ? -1.0 : s_total * gt.d;
+        if (KIND != OUTPUTS) total = total == -1.0 || gt.d == -1.0f ? -1.0 : total * gt.d;
 
         if (bad) {  // token by token, in fp32, from the inputs themselves
             const int n = static_cast<int>(p.T - t0 < C ? p.T - t0 : C);
@@ -640,7 +639,7 @@ __global__ void __launch_bounds__(kThreads, DK == 64 && Split<T>::IN < 3 ? 3 : 2
                 if (i < p.dk && j < p.dv) to[int64_t(i) * p.dv + j] = s[n][e];
             }
     }
-    if (KIND != OUTPUTS && slice == 0 && threadIdx.x == 0) put_decay(p.part_d + 2 * (chain * (p.nseg - 1) + seg), s_total);
+    if (KIND != OUTPUTS && slice == 0 && threadIdx.x == 0) put_decay(p.part_d + 2 * (chain * (p.nseg - 1) + seg), total);
 }
 
 // The state that enters each segment after the first, in the place of the own state of
@@ -650,17 +649,21 @@ __global__ void __launch_bounds__(256) enter_kernel(const AttnParams p) {
     const int64_t i = blockIdx.y * int64_t(256) + threadIdx.x;
     if (i >= n) return;
     float* s = p.part + chain * (p.nseg - 1) * n + i;
-    const uint32_t* d = p.part_d + 2 * chain * (p.nseg - 1);
+    const float* d = p.part_d + 2 * chain * (p.nseg - 1);
     float x = p.lead ? s[0] : p.s0 != nullptr ? p.s0[chain * n + i] : 0.0f;
     constexpr int B = 8;  // loads in flight
     for (int k0 = p.lead; k0 < p.nseg - 1; k0 += B) {
         float own[B];
+        float2 by[B];
 #pragma unroll
-        for (int e = 0; e < B; ++e) own[e] = k0 + e < p.nseg - 1 ? s[(k0 + e) * n] : 0.0f;
+        for (int e = 0; e < B; ++e) {
+            const int k = k0 + e < p.nseg - 1 ? k0 + e : k0;
+            own[e] = s[k * n], by[e] = make_float2(d[2 * k], d[2 * k + 1]);
+        }
 #pragma unroll
         for (int e = 0; e < B; ++e)
             if (k0 + e < p.nseg - 1) {
-                x = times_state(d + 2 * (k0 + e), x) + own[e];
+                x = times_state(by[e], x) + own[e];
                 s[(k0 + e) * n] = x;
             }
     }
@@ -802,8 +805,8 @@ int need_linear_attention(const need_linear_attention_args* a, need_stream_t str
         return fail(NEED_ERR_WORKSPACE, "linear attention: workspace missing, misaligned or too small");
     p.slices = pl.slices, p.nseg = pl.nseg, p.lead = pl.lead, p.first_chunks = pl.first_chunks, p.seg_chunks = pl.seg_chunks;
     p.part = static_cast<float*>(a->workspace);
-    p.part_d = reinterpret_cast<uint32_t*>(p.part + pl.chains * (pl.nseg - 1) * a->dk * a->dv);
-    uint32_t* redo = p.part_d + 2 * pl.chains * (pl.nseg - 1);
+    p.part_d = p.part + pl.chains * (pl.nseg - 1) * a->dk * a->dv;
+    uint32_t* redo = reinterpret_cast<uint32_t*>(p.part_d + 2 * pl.chains * (pl.nseg - 1));
     auto go = [&](auto tag) {
         using T = decltype(tag);
         if (a->dk <= 64) return vec ? run<T, 64, true>(p, pl, a->nb, redo, stream) : run<T, 64, false>(p, pl, a->nb, redo, stream);

@@ -34,7 +34,7 @@ struct AttnParams {
     int32_t ahead, lead;
     float scale;
     float* part;          // [chain, nseg - 1, dk, dv]: the segments' own states, then those that enter the next
-    uint32_t* part_d;     // [chain, nseg - 1]: their decays (a double's two words), below 0 where a reset lies in between
+    float* part_d;        // [chain, nseg - 1, 2]: their decays as products of two, below 0 where a reset lies in between
     const uint32_t* redo; // of each block, null for all: whether it has to run
     __host__ __device__ int launched() const { return ahead ? nseg - 1 : nseg - lead; }  // segments of this launch
     __host__ __device__ int64_t segment(int s) const { return s == 0 ? 0 : first_chunks + (s - 1) * seg_chunks; }  // its first chunk
@@ -68,14 +68,17 @@ __device__ __forceinline__ void split(float2 x, uint32_t (&pl)[N]) {
     }
 }
 
-// A segment's decay is the product of its chunks' in fp64: a growing one passes fp32's range before the
-// states that it multiplies do.
-__device__ __forceinline__ void put_decay(uint32_t* to, double d) { to[0] = __double2loint(d), to[1] = __double2hiint(d); }
-// The state of a segment's start at its end: 0 and the infinities stay, however far the segment grows or decays.
-__device__ __forceinline__ float times_state(const uint32_t* decay, float s) {
-    const double d = __hiloint2double(decay[1], decay[0]);
-    return d == -1.0 ? 0.0f : s == 0.0f || isinf(s) ? s : static_cast<float>(d * s);
+// A segment's decay is the product of its chunks' in fp64, and kept as that of two floats: a growing one
+// passes fp32's range before the states that it multiplies do.  Neither float is 0 or infinite, so that
+// states of 0 and infinity stay.
+__device__ __forceinline__ void put_decay(float* to, double d) {
+    const bool plain = d == -1.0 || d != d;
+    const int h = plain ? 0 : max(-252, min(252, ilogb(d))) >> 1;
+    const float a = static_cast<float>(ldexp(d, -h));
+    to[0] = plain ? a : fminf(fmaxf(a, 0x1p-126f), 0x1p126f), to[1] = ldexpf(1.0f, h);
 }
+// The state of a segment's start at its end.
+__device__ __forceinline__ float times_state(float2 d, float s) { return d.x == -1.0f ? 0.0f : s * d.x * d.y; }
 
 // The kernel on the tensor cores of sm_100a (linear_attention_umma.cu): chunks of 128
 // tokens, bf16, up to 128 features.  `redo` [blocks] tells which of attention_kernel's

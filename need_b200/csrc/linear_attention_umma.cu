@@ -565,7 +565,7 @@ __global__ void __launch_bounds__(kThreads, 1) umma_attention_kernel(const __gri
             if (c + 1 < n) fetch(c + 1);
             if (c >= GR) wait(gates_free + c % GR, c / GR - 1);
             make_gates(now, p.scale, gates[c % GR]);
-            if (lane == 0) *total = *total == -1.0 || gates[c % GR].d == -1.0f ? -1.0 : *total * gates[c % GR].d;
+            if (p.ahead && lane == 0) *total = *total == -1.0 || gates[c % GR].d == -1.0f ? -1.0 : *total * gates[c % GR].d;
             arrive(gates_full + c % GR);
         }
         if (p.ahead && slice == 0 && lane == 0) put_decay(p.part_d + 2 * (chain * (p.nseg - 1) + seg), *total);
