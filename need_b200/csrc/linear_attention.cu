@@ -42,6 +42,7 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "host_common.h"
@@ -416,8 +417,8 @@ __global__ void __launch_bounds__(kThreads, DK == 64 && Split<T>::IN < 3 ? 3 : 2
                         o0 += __shfl_xor_sync(0xffffffffu, o0, m);
                         o1 += __shfl_xor_sync(0xffffffffu, o1, m);
                     }
-                    if (c2 == 0 && j < p.dv) out[t * p.ot + j] = static_cast<T>(p.scale * o0);
-                    if (c2 == 2 && j + 8 < p.dv) out[t * p.ot + j + 8] = static_cast<T>(p.scale * o1);
+                    if (c2 == 0 && j < p.dv) out[t * p.ot + j] = static_cast<T>(p.scale * p.late * o0);
+                    if (c2 == 2 && j + 8 < p.dv) out[t * p.ot + j + 8] = static_cast<T>(p.scale * p.late * o1);
                 }
             }
             if (warp == 0 && c + 1 < c1) wild = make_decays(next, p.scale, gates[(c + 1) & 1]);
@@ -602,6 +603,13 @@ __global__ void __launch_bounds__(kThreads, DK == 64 && Split<T>::IN < 3 ? 3 : 2
         if (!state) {
             const int64_t rows = p.T - t0;
             T* const row0 = out + t0 * p.ot + jw + c2;
+            if (p.late != 1.0f)
+#pragma unroll
+                for (int m = 0; m < 4; ++m)
+#pragma unroll
+                    for (int n = 0; n < 2; ++n)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) o[m][n][e] *= p.late;
 #pragma unroll
             for (int m = 0; m < 4; ++m)
 #pragma unroll
@@ -797,7 +805,8 @@ int need_linear_attention(const need_linear_attention_args* a, need_stream_t str
     p.s0 = a->state, p.sT = a->final_state;
     p.out = a->out, p.ob = a->out_stride_b, p.ot = a->out_stride_t, p.oh = a->out_stride_h;
     p.T = a->T, p.H = int32_t(a->H), p.dk = int32_t(a->dk), p.dv = int32_t(a->dv);
-    p.scale = a->scale;
+    const bool large = std::fabs(a->scale) > 0x1p32f;
+    p.scale = large ? 1.0f : a->scale, p.late = large ? a->scale : 1.0f;
     const Plan pl = plan(vec && a->dtype == NEED_BF16 && a->T > C && umma_takes(p, a->nb), a->dtype, a->nb, a->T, a->H,
                          a->dk, a->dv);
     if ((pl.nseg > 1 || pl.umma) && (a->workspace == nullptr || (reinterpret_cast<uintptr_t>(a->workspace) & 3u) != 0 ||

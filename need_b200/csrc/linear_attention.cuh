@@ -32,7 +32,8 @@ struct AttnParams {
     // none); the one after it runs them for their outputs.  lead: the first one's outputs come
     // ahead, and its state with them.
     int32_t ahead, lead;
-    float scale;
+    float scale;          // at most 2^32, so that no decay's product with it is past fp32
+    float late;           // a larger one, of the outputs (scale is 1 then); else 1
     float* part;          // [chain, nseg - 1, dk, dv]: the segments' own states, then those that enter the next
     float* part_d;        // [chain, nseg - 1, 2]: their decays as products of two, below 0 where a reset lies in between
     const uint32_t* redo; // of each block, null for all: whether it has to run

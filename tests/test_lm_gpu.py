@@ -111,6 +111,20 @@ def test_attention_scales(cuda, B, T, H, dk, dv, scale, dtype):
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("T", [64, 300])
+@pytest.mark.parametrize("decay", [-0.34, 0.5])
+def test_attention_large_scale(cuda, T, decay, dtype):
+    """A scale that no decay may be multiplied with first: small q and k, rows of no key among them."""
+    q, k, v, _, _, s0 = make(cuda, 2, T, 2, 64, 64, dtype, state=True)
+    q, k = q * 2.0 ** -36, k * 2.0 ** -34
+    k[:, 10:60] = 0
+    ld = torch.zeros(2, T, 2, device=cuda)
+    ld[:, 10:120] = decay
+    check_attention(q, k, v, ld, 2.0 ** 70, None, None)
+    check_attention(q, k, v, ld, -2.0 ** 70, None, s0 * 2.0 ** -34)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
 @pytest.mark.parametrize("grow,n,then,m", [(0.5, 120, -100.0, 1), (0.5, 100, -90.0, 1), (0.4, 90, -90.0, 1), (0.5, 40, -20.0, 1),
                                            (-1.0, 80, 0.5, 80), (0.5, 128, 0.0, 1)])
 def test_attention_grows_and_forgets(cuda, grow, n, then, m, dtype):
