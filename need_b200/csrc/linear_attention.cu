@@ -131,6 +131,7 @@ struct alignas(16) Decays {
     float end[C];        // from a token to the end of its block of 16
     int seg[C];          // segments started up to the token
     float d;             // over the chunk; -1 where a segment starts in it
+    int pairwise;        // scores take each pair's own decay
 };
 
 template <typename T, int DK, bool VEC>
@@ -289,7 +290,11 @@ __device__ __forceinline__ bool make_decays(const TokenPair& tp, float scale, De
         g.eg[i] = s[e] == 0 ? scale * ex2(hi) : 0.0f;
         g.end[i] = ex2(static_cast<float>(block_end - G[e]));
     }
-    if (lane == 0) g.d = send == 0 ? ex2(static_cast<float>(end)) : -1.0f;
+    // A block's column factor may fall to 0 where a pair's decay does not, if states grow after it: then
+    // (2^60 and more between two tokens' sums, one of them growing), and where a segment starts.
+    const bool grows = __any_sync(0xffffffffu, tp.ld[0] > 0.0f || tp.ld[1] > 0.0f);
+    const bool wide = __any_sync(0xffffffffu, fabs(G[0] - end) > 30.0 || fabs(G[1] - end) > 30.0);
+    if (lane == 0) g.d = send == 0 ? ex2(static_cast<float>(end)) : -1.0f, g.pairwise = send != 0 || (grows && wide) ? 1 : 0;
     return __any_sync(0xffffffffu, !(tp.ld[0] <= 1.0f && tp.ld[1] <= 1.0f));
 }
 // ------------------------------------------------------------------ the kernel
@@ -452,7 +457,7 @@ __global__ void __launch_bounds__(kThreads, DK == 64 && Split<T>::IN < 3 ? 3 : 2
                 }
                 const int r0 = 16 * rb + g;
                 const float h0 = gt.hi[r0], l0 = gt.lo[r0], h1 = gt.hi[r0 + 8], l1 = gt.lo[r0 + 8];
-                const bool pairwise = rb == cb || resets;
+                const bool pairwise = rb == cb || gt.pairwise != 0;
                 float f0 = 0.0f, f1 = 0.0f;  // of a block below the diagonal: from its columns' end on
                 if (!pairwise) {
                     const float he = gt.hi[16 * cb + 15], le = gt.lo[16 * cb + 15];

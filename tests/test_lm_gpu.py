@@ -148,6 +148,28 @@ def test_attention_grows_and_forgets(cuda, grow, n, then, m, dtype):
         close(nk.linear_attention(q, k, v, ld, scale=0.125, seg_start=marks, state=s0), want, mag, SUMS[dtype] + 2.0 ** -16, ref.HALF_STEP[dtype])
 
 
+@pytest.mark.parametrize("dtype", [BF, HF, F32])
+@pytest.mark.parametrize("T", [64, 128, 300])
+def test_attention_grows_back(cuda, T, dtype):
+    """Tokens forgotten to e^-100 that grow back to e^-52: all that the later rows hold is theirs.
+    Decays below 2^-126 (the first rows') may be taken for 0, which costs 2^-126 of a term without
+    its decay; three exponents below 256 a term lose ln 2 2^-17 each."""
+    q, k, v, _, _, _ = make(cuda, 1, T, 2, 32, 32, dtype)
+    k[:, 8:64] = 0
+    v[:, :8] = v[:, :8] * 2.0 ** 10  # with the scale the last rows' results are normal numbers in f16 too
+    ld = torch.zeros(1, T, 2, device=cuda)
+    ld[:, 8] = -100.0
+    ld[:, 16:64] = 1.0
+    scale = 2.0 ** 60
+    out, fin = nk.linear_attention(q, k, v, ld, scale=scale, return_final_state=True)
+    want, s, mag, m = ref.attention(q, k, v, ld, scale)
+    bare = ref.attention(q, k, v, 0 * ld, scale)[2:]
+    rows, sums = slice(20, 64), SUMS[dtype] + 2.0 ** -15
+    small = 2.0 ** -24 if dtype == HF else 0.0
+    close(out[:, rows], want[:, rows], mag[:, rows] + (small + 2.0 ** -126 * bare[0][:, rows]) / sums, sums, ref.HALF_STEP[dtype])
+    close(fin, s, m + 2.0 ** -126 * bare[1] / STATE, STATE + 2.0 ** -15)
+
+
 def test_attention_decay_strides(cuda):
     q, k, v, ld, _, _ = make(cuda, 2, 100, 4, 32, 32, BF)
     want = nk.linear_attention(q, k, v, ld)
