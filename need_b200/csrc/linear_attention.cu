@@ -27,10 +27,10 @@
 // running sums are fp64, kept as two floats: a difference of two of them is exact to
 // fp32 however far the chunk has decayed.
 //
-// A chunk whose k or v holds an infinity or NaN (or fp32 values that a bf16 rounding
-// would carry over the largest), or whose log decays hold a NaN or a value over 1, is
-// run token by token in fp32 instead: under a score of 0 it would reach the tokens
-// before it, and other segments.
+// A chunk whose q, k, v or entering state holds an infinity or NaN (or fp32 values that a
+// bf16 rounding would carry over the largest), or whose log decays hold a NaN or a value
+// over 1, is run token by token in fp32 instead: under a score of 0 it would reach the
+// tokens before it, and other segments, and planes of an infinity make a NaN of it.
 //
 // bf16 rows of whole 16 bytes and more than 64 tokens are linear_attention_umma.cu's (104
 // chains of 64 features: 128 tokens 9.0 us there and 11.0 here, 64 tokens 8.6 and 7.1).
@@ -168,7 +168,7 @@ struct Loader {
     }
     // true where a value is not finite (or too near the largest to be rounded)
     __device__ __forceinline__ bool store(char* dst) const {
-        float chk = 0.0f;
+        float2 chk = splat(0.0f);
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int n = i * kThreads + threadIdx.x, row = n / PIECES, piece = n % PIECES;
@@ -178,15 +178,14 @@ struct Loader {
             for (int e = 0; e < 4; ++e) {
                 split<IN>(make_float2(to_float(x[2 * e]), to_float(x[2 * e + 1])), pl[e]);
                 // of a value that rounds to an infinity the first plane is one
-                chk = fmaf(__uint_as_float(pl[e][0] << 16), 0.0f, chk);
-                chk = fmaf(__uint_as_float(pl[e][0] & 0xffff0000u), 0.0f, chk);
+                chk = __ffma2_rn(unpack_bf16(pl[e][0]), splat(0.0f), chk);
             }
 #pragma unroll
             for (int p = 0; p < IN; ++p)
                 *reinterpret_cast<uint4*>(dst + p * C * COLS * 2 + at(row, piece)) =
                     make_uint4(pl[0][p], pl[1][p], pl[2][p], pl[3][p]);
         }
-        return !(chk == 0.0f);
+        return !(chk.x == 0.0f && chk.y == 0.0f);
     }
 };
 
@@ -332,6 +331,7 @@ __global__ void __launch_bounds__(kThreads, DK == 64 && Split<T>::IN < 3 ? 3 : 2
     // the state, transposed: rows j = jw + g and + 8, columns i = 8 n + c2 and + 1
     float s[NI][4];
     {
+        const bool fresh = starts(ld, p.lt, marks, p.gt, c0 * C);
         const float* from = state ? nullptr : seg > 0 ? p.part + (chain * (p.nseg - 1) + seg - 1) * p.dk * int64_t(p.dv)
                                   : p.s0 != nullptr   ? p.s0 + chain * p.dk * int64_t(p.dv) : nullptr;
 #pragma unroll
@@ -341,7 +341,21 @@ __global__ void __launch_bounds__(kThreads, DK == 64 && Split<T>::IN < 3 ? 3 : 2
                 const int i = 8 * n + c2 + (e & 1), j = jw + g + (e >> 1) * 8;
                 s[n][e] = from != nullptr && i < p.dk && j < p.dv ? from[int64_t(i) * p.dv + j] : 0.0f;
             }
+        if (fresh)
+#pragma unroll
+            for (int n = 0; n < NI; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
     }
+    // Whether the state holds an infinity or NaN (2^-8 more of a value rounds to one): after finite
+    // chunks it does not.
+    auto not_finite = [&] {
+        float chk = 0.0f;
+#pragma unroll
+        for (int n = 0; n < NI; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) chk = fmaf((1.0f + 0x1p-8f) * s[n][e], 0.0f, chk);
+        return !(chk == 0.0f);
+    };
+    bool lost = not_finite();
     double total = 1.0;  // the segment's decay
 
     using B16 = __nv_bfloat16;
@@ -370,6 +384,7 @@ __global__ void __launch_bounds__(kThreads, DK == 64 && Split<T>::IN < 3 ? 3 : 2
         if constexpr (L::STAGES == 2) {
             cp_wait_all();
             bad = check_rows<DK>(buf + L::K) | check_rows<DV>(buf + L::V);
+            if (!state) bad |= check_rows<DK>(buf + L::Q);
         } else {
             constexpr bool ALL = DK == 64 || S::IN < 3;  // else the registers hold K and V only
             Loader<T, DK, VEC> lk, lq;
@@ -379,8 +394,9 @@ __global__ void __launch_bounds__(kThreads, DK == 64 && Split<T>::IN < 3 ? 3 : 2
             __syncthreads();  // the chunk before this one has been read
             bad = lk.store(buf + L::K) | lv.store(buf + L::V);
             if (!state && !ALL) lq.load(q, p.q.st, t0, p.T, 0, p.dk);
-            if (!state) lq.store(buf + L::Q);
+            if (!state) bad |= lq.store(buf + L::Q);
         }
+        bad |= lost;
         bad = __syncthreads_or(bad | wild);  // the chunk and its decays are there
         const Decays& gt = gates[c & 1];
         TokenPair next{};
@@ -426,6 +442,7 @@ __global__ void __launch_bounds__(kThreads, DK == 64 && Split<T>::IN < 3 ? 3 : 2
                     if (c2 == 2 && j + 8 < p.dv) out[t * p.ot + j + 8] = static_cast<T>(p.scale * p.late * o1);
                 }
             }
+            lost = not_finite();
             if (warp == 0 && c + 1 < c1) wild = make_decays(next, p.scale, gates[(c + 1) & 1]);
             continue;
         }

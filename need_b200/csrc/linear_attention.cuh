@@ -81,6 +81,11 @@ __device__ __forceinline__ void put_decay(float* to, double d) {
 // The state of a segment's start at its end.
 __device__ __forceinline__ float times_state(float2 d, float s) { return d.x == -1.0f ? 0.0f : s * d.x * d.y; }
 
+// Whether a segment starts at token t: the state before it is not read then, whatever it holds.
+__device__ __forceinline__ bool starts(const float* ld, int64_t lt, const uint8_t* marks, int64_t gt, int64_t t) {
+    return (marks != nullptr && marks[t * gt] != 0) || ld[t * lt] == -INFINITY;
+}
+
 // The kernel on the tensor cores of sm_100a (linear_attention_umma.cu): chunks of 128
 // tokens, bf16, up to 128 features.  `redo` [blocks] tells which of attention_kernel's
 // blocks it leaves to that.  state: only the segments' states.

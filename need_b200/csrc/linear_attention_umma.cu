@@ -28,7 +28,7 @@
 // All roles' code runs on every part of the multiprocessor, so that it is kept short: straight
 // code of the same work took twice the time, waiting for instructions.
 //
-// Every wait is bounded.  A block that gave one up, or met a value that is not finite (or
+// Every wait is bounded.  A block that gave one up, or has an output or a state that is not finite (or
 // a log decay that makes a chunk's products leave fp32's range), says so in `redo`:
 // attention_kernel, launched behind, then computes the block's whole segment.
 //
@@ -329,6 +329,7 @@ __global__ void __launch_bounds__(kThreads, 1) umma_attention_kernel(const __gri
             const int cols = p.dv - col0 - 32 * half;
             float eg_last = 0.0f, row_last = 0.0f;  // of the chunk whose outputs come next
             bool reach_last = false;                // whether the entering state reaches its row
+            float2 chk = splat(0.0f);               // 0 unless an output is no finite number
             auto outputs = [&](int c) {  // 32 columns of chunk c
                 wait(o_done + (c & 1), c >> 1);
                 wait(qs_done + (c & 1), c >> 1);
@@ -348,6 +349,7 @@ __global__ void __launch_bounds__(kThreads, 1) umma_attention_kernel(const __gri
                     for (int i = 0; i < 8; ++i) {
                         float2 z = __fmul2_rn(splat(row_last), make_float2(x[e + 2 * i], x[e + 2 * i + 1]));
                         if (reach_last) z = __ffma2_rn(splat(eg_last), make_float2(y[e + 2 * i], y[e + 2 * i + 1]), z);
+                        chk = __ffma2_rn(z, splat(0.0f), chk);
                         w[i] = pack_bf16(z.x, z.y);
                     }
                     if (t >= p.T) continue;
@@ -426,6 +428,7 @@ __global__ void __launch_bounds__(kThreads, 1) umma_attention_kernel(const __gri
                 if (c > 0) outputs(c - 1);
                 eg_last = eg, row_last = row, reach_last = reach;
             }
+            if (!(chk.x == 0.0f && chk.y == 0.0f)) *bad_word = 1;
         }
     } else if (warp < 16) {
         // ---------------------------------------------------------------- V w, the state
@@ -437,6 +440,7 @@ __global__ void __launch_bounds__(kThreads, 1) umma_attention_kernel(const __gri
         {
             const float* from = state ? nullptr : seg > 0 ? p.part + (chain * (p.nseg - 1) + seg - 1) * p.dk * int64_t(p.dv)
                                       : p.s0 != nullptr   ? p.s0 + chain * p.dk * int64_t(p.dv) : nullptr;
+            if (from != nullptr && starts(ld, p.lt, marks, p.gt, first)) from = nullptr;  // nothing of it is seen
 #pragma unroll
             for (int m = 0; m < NH; ++m)
 #pragma unroll
@@ -444,6 +448,14 @@ __global__ void __launch_bounds__(kThreads, 1) umma_attention_kernel(const __gri
                     const int i = 8 * (m0 + m) + c2 + (e & 1), j = j0 + (e >> 1) * 8;
                     s[m][e] = from != nullptr && i < p.dk && j < p.dv ? from[int64_t(i) * p.dv + j] : 0.0f;
                 }
+            if (from != nullptr) {
+                float chk = 0.0f;
+#pragma unroll
+                for (int m = 0; m < NH; ++m)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) chk = fmaf(s[m][e], 0.0f, chk);
+                if (!(chk == 0.0f)) *bad_word = 1;
+            }
         }
         float d, d_next = 0.0f;
         bool bad = false;
@@ -501,8 +513,8 @@ __global__ void __launch_bounds__(kThreads, 1) umma_attention_kernel(const __gri
             if (c + 1 < n) fetch(c + 1);
             wait(ds_done, c);
             umma::fence_after_sync();
-            // an infinity or NaN of k or v leaves one here, under a weight of 0 too (V w is a NaN
-            // then): a sum of 0 x is 0 otherwise
+            // an infinity or NaN of k, v or the state leaves one here, under a weight of 0 too (V w is a
+            // NaN then): a sum of 0 x is 0 otherwise
             float2 chk = splat(0.0f);
             const float2 dd = splat(d == -1.0f ? 0.0f : d);
 #pragma unroll
@@ -521,8 +533,8 @@ __global__ void __launch_bounds__(kThreads, 1) umma_attention_kernel(const __gri
                         const float2 z = make_float2(x[4 * m + e], x[4 * m + e + 1]);
                         float2 y = make_float2(s[m1 + m][e], s[m1 + m][e + 1]);
                         if (d == -1.0f) y = splat(0.0f);  // whatever it holds
-                        chk = __ffma2_rn(z, splat(0.0f), chk);
                         y = __ffma2_rn(dd, y, z);
+                        chk = __ffma2_rn(y, splat(0.0f), chk);
                         s[m1 + m][e] = y.x, s[m1 + m][e + 1] = y.y;
                     }
             }

@@ -313,6 +313,40 @@ def test_attention_infinities_stay(cuda, where, bad, dtype):
         assert torch.isfinite(out[0, t + 1:140, 0]).all()
 
 
+@pytest.mark.parametrize("dtype", [BF, HF, F32])
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
+@pytest.mark.parametrize("where", ["q", "k", "v", "state"])
+@pytest.mark.parametrize("B,T,H,dk,dv", [(2, 64, 2, 32, 40), (2, 300, 2, 64, 72), (1, 900, 2, 128, 64)])
+def test_attention_infinities_are_the_definition_s(cuda, B, T, H, dk, dv, where, bad, dtype):
+    """Infinities stay infinities, with their signs, and NaN what is NaN in the recurrence: in the
+    rows that see them, in the chunks and parts that follow, in the final state."""
+    q, k, v, ld, _, s0 = make(cuda, B, T, H, dk, dv, dtype, state=True)
+    if where == "state":
+        s0[0, 1, 3, 5] = bad
+        s0[-1, 0, 7, 1] = -bad
+    else:
+        x = {"q": q, "k": k, "v": v}[where]
+        x[0, 20, 0, 5], x[-1, T - 40, 1, 9] = bad, -bad
+    seg = torch.zeros(B, T, dtype=torch.uint8, device=cuda)
+    seg[0, T - 20] = 1
+    small = 2.0 ** -24 if dtype == HF else 0.0
+    for marks in (None, seg):
+        out, fin = nk.linear_attention(q, k, v, ld, scale=0.125, seg_start=marks, state=s0, return_final_state=True)
+        alone = nk.linear_attention(q, k, v, ld, scale=0.125, seg_start=marks, state=s0)
+        want, s, mag, m = ref.attention(q, k, v, ld, 0.125, marks, s0)
+        for got, exact, terms, sums, half in ((out, want, mag, SUMS[dtype], ref.HALF_STEP[dtype]), (fin, s, m, STATE, 0.0),
+                                              (alone, want, mag, SUMS[dtype], ref.HALF_STEP[dtype])):
+            assert torch.equal(torch.isnan(got), torch.isnan(exact))
+            assert torch.equal(torch.isposinf(got), torch.isposinf(exact)) and torch.equal(torch.isneginf(got), torch.isneginf(exact))
+            fine = torch.isfinite(exact)
+            close(got[fine], exact[fine], terms[fine] + small / sums, sums, half)
+    # a state that a segment's start at the first token drops is not looked at
+    if where == "state":
+        seg[:, 0] = 1
+        a, b = (nk.linear_attention(q, k, v, ld, seg_start=seg, state=x, return_final_state=True) for x in (s0, None))
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
 def test_attention_large_values(cuda):
     """Values whose bf16 rounding would be infinite, and products past 65504 in f16."""
     q, k, v, ld, _, _ = make(cuda, 1, 100, 1, 8, 8, F32)
