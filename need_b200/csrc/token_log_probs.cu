@@ -466,7 +466,7 @@ __global__ void __launch_bounds__(kThreads) logp_kernel(const LogpParams p) {
                 u64 best = 0;
                 each([&](float x, int i) {
                     const u64 key = x == -INFINITY ? 0 : key_of(x, first + i);
-                    if (key < below && key > best) best = key;
+                    if ((k == 0 || key < below) && key > best) best = key;  // a NaN at token 0 has the largest key there is
                 });
 #pragma unroll
                 for (int m = 16; m >= 1; m >>= 1) {

@@ -724,6 +724,25 @@ def test_logp_infinities(cuda, V):
         assert torch.equal(a[[0, 4, 5]], b[[0, 4, 5]])
 
 
+@pytest.mark.parametrize("dtype", [BF, HF, F32])
+@pytest.mark.parametrize("V,top", [(300, 5), (784, 16), (784, 32), (3000, 5), (131072, 20)])
+def test_logp_rows_of_nan(cuda, V, top, dtype):
+    """NaN are the largest, the lower token first: rows of nothing else, and one at token 0 of a row
+    of equal logits (more than are put into order at once)."""
+    x = torch.full((4, V), math.nan, device=cuda, dtype=dtype)
+    x[1] = 0.5
+    x[1, 0] = math.nan
+    x[2] = 0.5
+    x[2, V - 1] = math.nan
+    x[3] = 0.5
+    r = nk.token_log_probs(x, torch.zeros(4, dtype=torch.long, device=cuda), top=top)
+    lowest = torch.arange(top, device=cuda)
+    assert torch.equal(r.top_tokens[0], lowest) and torch.equal(r.top_tokens[1], lowest) and torch.equal(r.top_tokens[3], lowest)
+    assert r.top_tokens[2, 0] == V - 1 and torch.equal(r.top_tokens[2, 1:], lowest[:-1])
+    assert torch.isnan(r.top_log_probs[:3]).all() and torch.isnan(r.log_prob[:3]).all() and torch.isnan(r.entropy[:3]).all()
+    assert torch.allclose(r.top_log_probs[3], torch.full((top,), -math.log(V), device=cuda), rtol=1e-6)
+
+
 def test_logp_tokens(cuda):
     """None given, and past the vocabulary."""
     x, t = logits_of(cuda, 4, 784, BF)
