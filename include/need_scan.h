@@ -333,7 +333,7 @@ typedef struct {
     const float* log_decay; int64_t ld_stride_b, ld_stride_t, ld_stride_h; /* [nb, T, H]; strides may be 0 */
     const uint8_t* seg_start; int64_t seg_stride_b, seg_stride_t;          /* optional [nb, T] */
     const float* state;    /* optional [nb, H, dk, dv] contiguous: before the first token */
-    float* final_state;    /* optional, likewise: after the last */
+    float* final_state;    /* optional, likewise: after the last; not in state's place */
     void* out; int64_t out_stride_b, out_stride_t, out_stride_h;           /* [nb, T, H, dv] */
     void* workspace; size_t workspace_bytes;
 } need_linear_attention_args;
@@ -637,7 +637,8 @@ NEED_API size_t need_linear_attention_workspace_size(int32_t dtype, int64_t nb, 
  *     S_t = exp(log_decay_t) S_{t-1} + k_t^T v_t,   out_t = scale q_t S_t,
  * sums and states in fp32, out rounded once.  At a marked token, or one whose log
  * decay is -infinity, the state before it is dropped, whatever it holds.  At most
- * NEED_LINEAR_ATTENTION_MAX_DK features a head. */
+ * NEED_LINEAR_ATTENTION_MAX_DK features a head.  out and final_state overlap no input:
+ * a block may be run a second time (final_state over state is refused). */
 NEED_API int need_linear_attention(const need_linear_attention_args* args, need_stream_t stream);
 
 /* Test hook, no counterpart in the reference: the waits inside need_linear_attention's

@@ -810,6 +810,11 @@ int need_linear_attention(const need_linear_attention_args* a, need_stream_t str
     if (a->T > 1 && a->out_stride_t < a->dv) return fail(NEED_ERR_INVALID, "linear attention: the output's rows overlap");
     if (a->nb > (int64_t(1) << 30) / a->H / ((a->dv + DV - 1) / DV))
         return fail(NEED_ERR_UNSUPPORTED, "linear attention: too many sequences and heads");
+    // parts, and blocks that are run again, read the state after final_state has been written
+    const uintptr_t before = reinterpret_cast<uintptr_t>(a->state), after = reinterpret_cast<uintptr_t>(a->final_state);
+    const size_t bytes = size_t(a->nb) * a->H * a->dk * a->dv * sizeof(float);
+    if (before != 0 && after != 0 && before < after + bytes && after < before + bytes)
+        return fail(NEED_ERR_INVALID, "linear attention: state and final_state overlap");
     const int es = dtype_bytes(a->dtype), per = 16 / es;
     AttnParams p{};
     Stream* to[3] = {&p.q, &p.k, &p.v};

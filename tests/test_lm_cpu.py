@@ -71,6 +71,22 @@ def test_attention_refuses(lib, change, code):
     assert lib.need_last_error()
 
 
+@pytest.mark.parametrize("T,dtype", [(1, abi.F32), (100, abi.BF16), (4096, abi.F16)])
+@pytest.mark.parametrize("shift", [0, 4, 2 * 4 * 64 * 64 * 4 - 4, -4])
+def test_attention_refuses_a_state_in_place(lib, T, dtype, shift):
+    """Blocks may read it again after the final one has been written."""
+    a = attention_args(T=T, dtype=dtype, state=P, final_state=P + shift)
+    assert lib.need_linear_attention(ctypes.byref(a), None) == abi.ERR_INVALID
+    assert b"overlap" in lib.need_last_error()
+
+
+def test_attention_takes_states_side_by_side(lib):
+    """Next to each other they are taken: what is refused here is the workspace."""
+    for shift in (2 * 4 * 64 * 64 * 4, -2 * 4 * 64 * 64 * 4):
+        a = attention_args(T=4096, state=P, final_state=P + shift, workspace=None)
+        assert lib.need_linear_attention(ctypes.byref(a), None) == abi.ERR_WORKSPACE
+
+
 def step_args(**kw):
     a = abi.NeedLinearAttentionStepArgs()
     a.dtype, a.scale, a.n, a.H, a.dk, a.dv = abi.BF16, 1.0, 10, 4, 64, 64
