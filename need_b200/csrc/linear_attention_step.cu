@@ -144,7 +144,7 @@ extern "C" int need_linear_attention_step(const need_linear_attention_step_args*
         if (x->heads < 1 || a->H % x->heads != 0)
             return fail(NEED_ERR_INVALID, "linear attention step: heads must divide H = %lld", static_cast<long long>(a->H));
     }
-    if (a->log_decay == nullptr || a->state == nullptr || a->out == nullptr)
+    if (a->log_decay == nullptr || (a->state == nullptr && a->slots > 0) || a->out == nullptr)
         return fail(NEED_ERR_INVALID, "linear attention step: log_decay, state and out are required");
     if (a->slot == nullptr && a->slots < a->n) return fail(NEED_ERR_INVALID, "linear attention step: fewer states than tokens");
     if (a->slots > 1 && a->state_stride < a->H * a->dk * a->dv)

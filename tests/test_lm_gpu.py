@@ -490,6 +490,16 @@ def test_step_slots(cuda):
     assert torch.equal(pool[[1, 2, 4]], before[[1, 2, 4]])
 
 
+def test_step_empty_pool(cuda):
+    """No state at all: rows without a sequence are 0, the others NaN."""
+    q, k, v, ld, _, _ = make(cuda, 4, 1, 2, 16, 24, BF)
+    slot = torch.tensor([-1, 0, -5, 3], dtype=torch.int32, device=cuda)
+    out = nk.linear_attention_step(q[:, 0], k[:, 0], v[:, 0], ld[:, 0], torch.zeros(0, 2, 16, 24, device=cuda), slot=slot)
+    assert (out[[0, 2]] == 0).all() and torch.isnan(out[[1, 3]]).all()
+    with pytest.raises(ValueError):
+        nk.linear_attention_step(q[:, 0], k[:, 0], v[:, 0], ld[:, 0], torch.zeros(0, 2, 16, 24, device=cuda))
+
+
 def test_step_decays(cuda):
     """A log decay of -infinity drops the state, whatever it holds; pool rows apart."""
     q, k, v, _, _, _ = make(cuda, 2, 1, 2, 16, 16, F32)
