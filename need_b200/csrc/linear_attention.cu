@@ -406,53 +406,13 @@ __global__ void __launch_bounds__(kThreads, DK == 64 && Split<T>::IN < 3 ? 3 : 2
         }
         if (KIND != OUTPUTS) total = total == -1.0 || gt.d == -1.0f ? -1.0 : total * gt.d;
 
-        if (bad) {  // token by token, in fp32, from the inputs themselves
-            const int n = static_cast<int>(p.T - t0 < C ? p.T - t0 : C);
-            for (int r = 0; r < n; ++r) {
-                const int64_t t = t0 + r;
-                const float x = ld[t * p.lt];
-                const bool reset = (marks != nullptr && marks[t * p.gt] != 0) || x == -INFINITY;
-                const float a = expf(x);
-                const int j = jw + g;
-                const float v0 = j < p.dv ? to_float(v[t * p.v.st + j]) : 0.0f;
-                const float v1 = j + 8 < p.dv ? to_float(v[t * p.v.st + j + 8]) : 0.0f;
-                float o0 = 0.0f, o1 = 0.0f;
-#pragma unroll
-                for (int m = 0; m < NI; ++m)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const int i = 8 * m + c2 + e;
-                        if (i < p.dk) {
-                            const float kk = to_float(k[t * p.k.st + i]);
-                            s[m][e] = reset ? kk * v0 : fmaf(a, s[m][e], kk * v0);
-                            s[m][2 + e] = reset ? kk * v1 : fmaf(a, s[m][2 + e], kk * v1);
-                            if (!state) {
-                                const float qq = to_float(q[t * p.q.st + i]);
-                                o0 = fmaf(qq, s[m][e], o0), o1 = fmaf(qq, s[m][2 + e], o1);
-                            }
-                        }
-                    }
-                if (!state) {
-#pragma unroll
-                    for (int m = 1; m < 4; m <<= 1) {
-                        o0 += __shfl_xor_sync(0xffffffffu, o0, m);
-                        o1 += __shfl_xor_sync(0xffffffffu, o1, m);
-                    }
-                    if (c2 == 0 && j < p.dv) out[t * p.ot + j] = static_cast<T>(p.scale * p.late * o0);
-                    if (c2 == 2 && j + 8 < p.dv) out[t * p.ot + j + 8] = static_cast<T>(p.scale * p.late * o1);
-                }
-            }
-            lost = not_finite();
-            if (warp == 0 && c + 1 < c1) wild = make_decays(next, p.scale, gates[(c + 1) & 1]);
-            continue;
-        }
-
         // rows and pieces of this lane's ldmatrix addresses: 16 rows x 16 columns a load
         const int lr = lane & 15, lp = lane >> 4;                              // [m][k] tiles, and [k][n] ones transposed
         const int br = (lane & 7) + ((lane >> 4) << 3), bp = (lane >> 3) & 1;  // [n][k] tiles, and [k][m] ones transposed
         const bool resets = gt.d == -1.0f;
         float o[4][2][4] = {};
-        if (!state) {
+        float2 over = splat(0.0f);  // 0 unless a score is past fp32 (an infinity or NaN)
+        if (!state && !bad) {
             // the scores on and below the diagonal, in blocks of 16 x 16: each warp the one on
             // the diagonal and one or two others
             for (int i = 0; i < (warp == 1 || warp == 2 ? 3 : 2); ++i) {
@@ -498,6 +458,7 @@ __global__ void __launch_bounds__(kThreads, DK == 64 && Split<T>::IN < 3 ? 3 : 2
                         x1.x = ss.x == s1 && col <= r0 + 8 ? x1.x * (p.scale * ex2((h1 - hs.x) + (l1 - ls.x))) : 0.0f;
                         x1.y = ss.y == s1 && col + 1 <= r0 + 8 ? x1.y * (p.scale * ex2((h1 - hs.y) + (l1 - ls.y))) : 0.0f;
                     }
+                    over = __ffma2_rn(x0, splat(0.0f), over), over = __ffma2_rn(x1, splat(0.0f), over);
                     uint32_t p0[S::SCORE], p1[S::SCORE];
                     split<S::SCORE>(x0, p0);
                     split<S::SCORE>(x1, p1);
@@ -554,7 +515,46 @@ __global__ void __launch_bounds__(kThreads, DK == 64 && Split<T>::IN < 3 ? 3 : 2
                 }
         }
         if (warp == 0 && c + 1 < c1) wild = make_decays(next, p.scale, gates[(c + 1) & 1]);
-        if (!state) __syncthreads();  // the scores are there
+        if (!state) bad |= __syncthreads_or(!(over.x == 0.0f && over.y == 0.0f));  // the scores are there
+        if (bad) {  // token by token, in fp32, from the inputs themselves
+            const int n = static_cast<int>(p.T - t0 < C ? p.T - t0 : C);
+            for (int r = 0; r < n; ++r) {
+                const int64_t t = t0 + r;
+                const float x = ld[t * p.lt];
+                const bool reset = (marks != nullptr && marks[t * p.gt] != 0) || x == -INFINITY;
+                const float a = expf(x);
+                const int j = jw + g;
+                const float v0 = j < p.dv ? to_float(v[t * p.v.st + j]) : 0.0f;
+                const float v1 = j + 8 < p.dv ? to_float(v[t * p.v.st + j + 8]) : 0.0f;
+                float o0 = 0.0f, o1 = 0.0f;
+#pragma unroll
+                for (int m = 0; m < NI; ++m)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const int i = 8 * m + c2 + e;
+                        if (i < p.dk) {
+                            const float kk = to_float(k[t * p.k.st + i]);
+                            s[m][e] = reset ? kk * v0 : fmaf(a, s[m][e], kk * v0);
+                            s[m][2 + e] = reset ? kk * v1 : fmaf(a, s[m][2 + e], kk * v1);
+                            if (!state) {
+                                const float qq = to_float(q[t * p.q.st + i]);
+                                o0 = fmaf(qq, s[m][e], o0), o1 = fmaf(qq, s[m][2 + e], o1);
+                            }
+                        }
+                    }
+                if (!state) {
+#pragma unroll
+                    for (int m = 1; m < 4; m <<= 1) {
+                        o0 += __shfl_xor_sync(0xffffffffu, o0, m);
+                        o1 += __shfl_xor_sync(0xffffffffu, o1, m);
+                    }
+                    if (c2 == 0 && j < p.dv) out[t * p.ot + j] = static_cast<T>(p.scale * p.late * o0);
+                    if (c2 == 2 && j + 8 < p.dv) out[t * p.ot + j + 8] = static_cast<T>(p.scale * p.late * o1);
+                }
+            }
+            lost = not_finite();
+            continue;
+        }
 
         // the scores times v, and the state
         if (resets) {

@@ -347,6 +347,24 @@ def test_attention_infinities_are_the_definition_s(cuda, B, T, H, dk, dv, where,
         assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
 
 
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("B,T,H,dk,dv", [(2, 64, 2, 32, 40), (2, 300, 2, 64, 72), (1, 900, 2, 128, 64)])
+def test_attention_scores_past_fp32(cuda, B, T, H, dk, dv, dtype):
+    """q . k past fp32 where the states and the results are not.  Such chunks run token by token: two
+    roundings of the state (2^-24 of its terms) a token, dk of the product with q."""
+    q, k, v, ld, seg, s0 = make(cuda, B, T, H, dk, dv, dtype, state=True, resets=100)
+    q, k, v = q * 2.0 ** 66, k * 2.0 ** 64, v * 2.0 ** -66
+    q[:, T // 2:T // 2 + 70] *= 2.0 ** -66  # and some where they are in range
+    more = (2 * T + dk) * 2.0 ** -24
+    for marks in (None, seg):
+        out, fin = nk.linear_attention(q, k, v, ld, scale=0.125, seg_start=marks, state=s0, return_final_state=True)
+        alone = nk.linear_attention(q, k, v, ld, scale=0.125, seg_start=marks, state=s0)
+        want, s, mag, m = ref.attention(q, k, v, ld, 0.125, marks, s0)
+        for got in (out, alone):
+            close(got, want, mag, SUMS[dtype] + more, ref.HALF_STEP[dtype])
+        close(fin, s, m, STATE + more)
+
+
 def test_attention_large_values(cuda):
     """Values whose bf16 rounding would be infinite, and products past 65504 in f16."""
     q, k, v, ld, _, _ = make(cuda, 1, 100, 1, 8, 8, F32)
