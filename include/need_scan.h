@@ -635,7 +635,9 @@ NEED_API size_t need_linear_attention_workspace_size(int32_t dtype, int64_t nb, 
  * retention scan: need_core.py:1590-1592 keeps k v by element where this keeps
  * k^T v), over whole prompts:
  *     S_t = exp(log_decay_t) S_{t-1} + k_t^T v_t,   out_t = scale q_t S_t,
- * sums and states in fp32, out rounded once.  At a marked token, or one whose log
+ * sums and states in fp32, out rounded once; on the tensor cores scores and entering
+ * states are sums of 2 bf16 values under 16-bit results (2^-17), of 3 under fp32 ones and
+ * for final_state (2^-25).  At a marked token, or one whose log
  * decay is -infinity, the state before it is dropped, whatever it holds.  At most
  * NEED_LINEAR_ATTENTION_MAX_DK features a head.  out and final_state overlap no input:
  * a block may be run a second time (final_state over state is refused). */

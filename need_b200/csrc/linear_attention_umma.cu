@@ -170,7 +170,7 @@ __device__ __forceinline__ void tmem_ld_half(uint32_t taddr, float (&v)[16]) {
 }
 
 // ------------------------------------------------------------------ decays
-// A sum as two floats: a + b with what rounding left of it.
+// A sum as two floats: a + b with what rounding left of it (Knuth's two-sum).
 struct Sum2 {
     float hi, lo;
 };
@@ -368,62 +368,62 @@ __global__ void __launch_bounds__(kThreads, 1) umma_attention_kernel(const __gri
                 float eg = 0.0f, row = 0.0f;  // of the chunk
                 bool reach = false;
                 if (c < n) {
-                const Gates& g = gates[c % GR];
-                wait(gates_full + c % GR, c / GR);
-                eg = g.eg[r], row = g.row[r], reach = g.seg[r] == 0;
-                const bool factors = g.factors != 0;
-                wait(qk_done + (c & 1), c >> 1);
-                umma::fence_after_sync();
-                const uint32_t tp = tmem + M::T_P + 128 * (c % NP) + lanes;
-                // 16 columns at a time, every other one, two of them in flight; after the diagonal's they are 0
-                auto scores = [&](int cb, float (&x)[16]) {
-                    uint32_t pl[16];  // the first planes of 16 scores, then the second
-                    if (cb < 2 * quad + 2) {
-                        if (factors) {
+                    const Gates& g = gates[c % GR];
+                    wait(gates_full + c % GR, c / GR);
+                    eg = g.eg[r], row = g.row[r], reach = g.seg[r] == 0;
+                    const bool factors = g.factors != 0;
+                    wait(qk_done + (c & 1), c >> 1);
+                    umma::fence_after_sync();
+                    const uint32_t tp = tmem + M::T_P + 128 * (c % NP) + lanes;
+                    // 16 columns at a time, every other one, two of them in flight; after the diagonal's they are 0
+                    auto scores = [&](int cb, float (&x)[16]) {
+                        uint32_t pl[16];  // the first planes of 16 scores, then the second
+                        if (cb < 2 * quad + 2) {
+                            if (factors) {
 #pragma unroll
-                            for (int e = 0; e < 16; e += 4) {
-                                const float4 w = *reinterpret_cast<const float4*>(&g.w[16 * cb + e]);
-                                const float2 u = __fmul2_rn(make_float2(x[e], x[e + 1]), make_float2(w.x, w.y));
-                                const float2 d = __fmul2_rn(make_float2(x[e + 2], x[e + 3]), make_float2(w.z, w.w));
-                                x[e] = u.x, x[e + 1] = u.y, x[e + 2] = d.x, x[e + 3] = d.y;
+                                for (int e = 0; e < 16; e += 4) {
+                                    const float4 w = *reinterpret_cast<const float4*>(&g.w[16 * cb + e]);
+                                    const float2 u = __fmul2_rn(make_float2(x[e], x[e + 1]), make_float2(w.x, w.y));
+                                    const float2 d = __fmul2_rn(make_float2(x[e + 2], x[e + 3]), make_float2(w.z, w.w));
+                                    x[e] = u.x, x[e + 1] = u.y, x[e + 2] = d.x, x[e + 3] = d.y;
+                                }
+                                if (cb >= 2 * quad)
+#pragma unroll
+                                    for (int e = 0; e < 16; ++e) x[e] = 16 * cb + e <= r ? x[e] : 0.0f;
+                            } else {
+                                const float hr = g.hi[r], lr = g.lo[r];
+                                const int sr = g.seg[r];
+#pragma unroll
+                                for (int e = 0; e < 16; ++e) {
+                                    const int i = 16 * cb + e;
+                                    x[e] = g.seg[i] == sr && i <= r ? x[e] * (p.scale * ex2((hr - g.hi[i]) + (lr - g.lo[i]))) : 0.0f;
+                                }
                             }
-                            if (cb >= 2 * quad)
 #pragma unroll
-                                for (int e = 0; e < 16; ++e) x[e] = 16 * cb + e <= r ? x[e] : 0.0f;
+                            for (int e = 0; e < 8; ++e) {
+                                uint32_t two[2];
+                                split<2>(make_float2(x[2 * e], x[2 * e + 1]), two);
+                                pl[e] = two[0], pl[8 + e] = two[1];
+                            }
                         } else {
-                            const float hr = g.hi[r], lr = g.lo[r];
-                            const int sr = g.seg[r];
 #pragma unroll
-                            for (int e = 0; e < 16; ++e) {
-                                const int i = 16 * cb + e;
-                                x[e] = g.seg[i] == sr && i <= r ? x[e] * (p.scale * ex2((hr - g.hi[i]) + (lr - g.lo[i]))) : 0.0f;
-                            }
+                            for (int e = 0; e < 16; ++e) pl[e] = 0u;
                         }
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) {
-                            uint32_t two[2];
-                            split<2>(make_float2(x[2 * e], x[2 * e + 1]), two);
-                            pl[e] = two[0], pl[8 + e] = two[1];
-                        }
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) pl[e] = 0u;
-                    }
-                    tmem_st16(tp + 16 * cb, pl);
-                };
+                        tmem_st16(tp + 16 * cb, pl);
+                    };
 #pragma unroll 1
-                for (int cb = half; cb < 8; cb += 4) {
-                    float x[16], y[16];
-                    tmem_ld16(tp + 16 * cb, x);
-                    tmem_ld16(tp + 16 * cb + 32, y);
-                    umma::tmem_wait_ld();
-                    scores(cb, x);
-                    scores(cb + 2, y);
-                }
-                umma::tmem_wait_st();
-                umma::fence_before_sync();
-                arrive(p_ready + (c & 1));
-                arrive(gates_free + c % GR);
+                    for (int cb = half; cb < 8; cb += 4) {
+                        float x[16], y[16];
+                        tmem_ld16(tp + 16 * cb, x);
+                        tmem_ld16(tp + 16 * cb + 32, y);
+                        umma::tmem_wait_ld();
+                        scores(cb, x);
+                        scores(cb + 2, y);
+                    }
+                    umma::tmem_wait_st();
+                    umma::fence_before_sync();
+                    arrive(p_ready + (c & 1));
+                    arrive(gates_free + c % GR);
                 }
                 if (c > 0) outputs(c - 1);
                 eg_last = eg, row_last = row, reach_last = reach;
@@ -594,8 +594,8 @@ __global__ void __launch_bounds__(kThreads, 1) umma_attention_kernel(const __gri
             if (!state) {
                 constexpr uint32_t ID_QK = umma::idesc_bf16(128, 128, umma::K_MAJOR, umma::K_MAJOR);
                 constexpr uint32_t ID_QS = umma::idesc_bf16(128, DVS, umma::K_MAJOR, umma::K_MAJOR);
-    #pragma unroll 1
-            for (int c = 0; c < NQ; ++c) load_q(c);
+#pragma unroll 1
+                for (int c = 0; c < NQ; ++c) load_q(c);
                 for (int c = 0; c <= n; ++c) {  // P of chunk c, O2 of the one before it
                     auto scores = [&] {
                         wait(full_q + c % NQ, c / NQ);
