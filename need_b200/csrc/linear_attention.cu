@@ -28,16 +28,17 @@
 // fp32 however far the chunk has decayed.
 //
 // A chunk whose q, k, v or entering state holds an infinity or NaN (or fp32 values that a
-// bf16 rounding would carry over the largest), or whose log decays hold a NaN or a value
-// over 1, is run token by token in fp32 instead: under a score of 0 it would reach the
-// tokens before it, and other segments, and planes of an infinity make a NaN of it.
+// bf16 rounding would carry over the largest), whose scores pass fp32, or whose log decays
+// hold a NaN or a value over 1, is run token by token in fp32 instead: under a score of 0
+// it would reach the tokens before it, and other segments, and planes of an infinity make
+// a NaN of it.
 //
 // bf16 rows of whole 16 bytes and more than 64 tokens are linear_attention_umma.cu's (104
-// chains of 64 features: 128 tokens 9.0 us there and 11.0 here, 64 tokens 8.6 and 7.1).
+// chains of 64 features: 128 tokens 9.6 us there and 12.0 here, 64 tokens 9.0 and 7.6).
 // Here the tensor pipe is busy a third of the time: the loads, the split into planes, the
 // scores and the products with them follow one another in a chunk, some 5 us.  3 x 777
-// tokens, 6 heads of 40 x 72 in fp16, in 7 segments: 30 us; 16 x 2048 tokens, 16 heads of
-// 64 x 64: fp16 250 us, fp32 360 (0.5 and 0.8 TB/s).
+// tokens, 6 heads of 40 x 72 in fp16, in 7 segments: 32 us; 16 x 2048 tokens, 16 heads of
+// 64 x 64: fp16 260 us, fp32 362 (0.5 and 0.8 TB/s).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -372,10 +373,12 @@ __global__ void __launch_bounds__(kThreads, DK == 64 && Split<T>::IN < 3 ? 3 : 2
 
     // the state, transposed: rows j = jw + g and + 8, columns i = 8 n + c2 and + 1
     float s[NI][4];
+    bool entered;
     {
-        const bool fresh = starts(ld, p.lt, marks, p.gt, c0 * C);
         const float* from = state ? nullptr : seg > 0 ? p.part + (chain * (p.nseg - 1) + seg - 1) * p.dk * int64_t(p.dv)
                                   : p.s0 != nullptr   ? p.s0 + chain * p.dk * int64_t(p.dv) : nullptr;
+        const bool fresh = from != nullptr && starts(ld, p.lt, marks, p.gt, c0 * C);  // nothing of it is seen
+        entered = from != nullptr;
 #pragma unroll
         for (int n = 0; n < NI; ++n)
 #pragma unroll
@@ -397,7 +400,7 @@ __global__ void __launch_bounds__(kThreads, DK == 64 && Split<T>::IN < 3 ? 3 : 2
             for (int e = 0; e < 4; ++e) chk = fmaf((1.0f + 0x1p-8f) * s[n][e], 0.0f, chk);
         return !(chk == 0.0f);
     };
-    bool lost = not_finite();
+    bool lost = entered && not_finite();
     double total = 1.0;  // the segment's decay
 
     using B16 = __nv_bfloat16;
@@ -415,6 +418,8 @@ __global__ void __launch_bounds__(kThreads, DK == 64 && Split<T>::IN < 3 ? 3 : 2
     };
     issue(c0);
     bool wild = false;  // warp 0: of the next chunk's decays
+    bool again = false;  // the chunk is run a second time, token by token
+    TokenPair next{};
     if (warp == 0) wild = make_decays(load_decays(p, ld, marks, c0 * C), p.scale, gates[c0 & 1]);
 
     for (int64_t c = c0; c < c1; ++c) {
@@ -426,7 +431,6 @@ __global__ void __launch_bounds__(kThreads, DK == 64 && Split<T>::IN < 3 ? 3 : 2
         if constexpr (L::STAGES == 2) {
             cp_wait_all();
             bad = check_rows<DK>(buf + L::K) | check_rows<DV>(buf + L::V);
-            if (!state) bad |= check_rows<DK>(buf + L::Q);
         } else {
             constexpr bool ALL = DK == 64 || S::IN < 3;  // else the registers hold K and V only
             Loader<T, DK, VEC> lk, lq;
@@ -436,13 +440,12 @@ __global__ void __launch_bounds__(kThreads, DK == 64 && Split<T>::IN < 3 ? 3 : 2
             __syncthreads();  // the chunk before this one has been read
             bad = lk.store(buf + L::K) | lv.store(buf + L::V);
             if (!state && !ALL) lq.load(q, p.q.st, t0, p.T, 0, p.dk);
-            if (!state) bad |= lq.store(buf + L::Q);
+            if (!state) lq.store(buf + L::Q);
         }
         bad |= lost;
         bad = __syncthreads_or(bad | wild);  // the chunk and its decays are there
         const Decays& gt = gates[c & 1];
-        TokenPair next{};
-        if (c + 1 < c1) {
+        if (c + 1 < c1 && !again) {
             issue(c + 1);
             if (warp == 0) next = load_decays(p, ld, marks, t0 + C);
         }
@@ -459,11 +462,12 @@ __global__ void __launch_bounds__(kThreads, DK == 64 && Split<T>::IN < 3 ? 3 : 2
                 for (int e = 0; e < 4; ++e) s[n][e] = x[n][e];
             lost = not_finite();
         };
-        if (KIND != OUTPUTS) total = total == -1.0 || gt.d == -1.0f ? -1.0 : total * gt.d;
+        if (KIND != OUTPUTS && !again) total = total == -1.0 || gt.d == -1.0f ? -1.0 : total * gt.d;
 
-        if (bad) {
+        if (bad || again) {
             by_token();
-            if (warp == 0 && c + 1 < c1) wild = make_decays(next, p.scale, gates[(c + 1) & 1]);
+            if (warp == 0 && c + 1 < c1 && !again) wild = make_decays(next, p.scale, gates[(c + 1) & 1]);
+            again = false;
             continue;
         }
 
@@ -472,7 +476,7 @@ __global__ void __launch_bounds__(kThreads, DK == 64 && Split<T>::IN < 3 ? 3 : 2
         const int br = (lane & 7) + ((lane >> 4) << 3), bp = (lane >> 3) & 1;  // [n][k] tiles, and [k][m] ones transposed
         const bool resets = gt.d == -1.0f;
         float o[4][2][4] = {};
-        float2 over = splat(0.0f);  // 0 unless a score is past fp32 (an infinity or NaN)
+        float2 over = splat(0.0f);  // 0 unless a score is no finite number (one past fp32, or q holds none)
         if (!state) {
             // the scores on and below the diagonal, in blocks of 16 x 16: each warp the one on
             // the diagonal and one or two others
@@ -577,7 +581,7 @@ __global__ void __launch_bounds__(kThreads, DK == 64 && Split<T>::IN < 3 ? 3 : 2
         }
         if (warp == 0 && c + 1 < c1) wild = make_decays(next, p.scale, gates[(c + 1) & 1]);
         if (!state && __syncthreads_or(!(over.x == 0.0f && over.y == 0.0f))) {  // the scores are there
-            by_token();
+            again = true, --c;
             continue;
         }
 
@@ -650,13 +654,6 @@ __global__ void __launch_bounds__(kThreads, DK == 64 && Split<T>::IN < 3 ? 3 : 2
         if (!state) {
             const int64_t rows = p.T - t0;
             T* const row0 = out + t0 * p.ot + jw + c2;
-            if (p.late != 1.0f)
-#pragma unroll
-                for (int m = 0; m < 4; ++m)
-#pragma unroll
-                    for (int n = 0; n < 2; ++n)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) o[m][n][e] *= p.late;
 #pragma unroll
             for (int m = 0; m < 4; ++m)
 #pragma unroll
@@ -666,7 +663,7 @@ __global__ void __launch_bounds__(kThreads, DK == 64 && Split<T>::IN < 3 ? 3 : 2
 #pragma unroll
                         for (int n = 0; n < 2; ++n) {
                             const int j = jw + 8 * n + c2;
-                            const float x = o[m][n][2 * r], y = o[m][n][2 * r + 1];
+                            const float x = p.late * o[m][n][2 * r], y = p.late * o[m][n][2 * r + 1];
                             T* const to = row0 + row * p.ot + 8 * n;
                             if (VEC) {  // whole pairs, aligned
                                 if (j < p.dv) {
@@ -742,12 +739,12 @@ constexpr int held(bool small) {
 // launch joins those, then all are run for the outputs.  That is worth it where it saves more
 // chunks in a row than the two more launches cost (1.5 of attention_kernel's, five of umma's
 // 128 tokens; a chunk for the state alone counts as 0.8).  Uncut and cut: 4 bf16 chains of 64
-// features 14.3 and 18.2 us at 512 tokens, 22.3 and 18.8 at 1024; 64 fp16 ones 13.8 and 17.7
-// at 128 tokens, 24 and 21.6 at 256, 385 and 171 at 4096; 104 fp32 ones 521 and 475 at 4096.
+// features 13.8 and 17.7 us at 512 tokens, 20.7 and 17.8 at 1024; 64 fp16 ones 14.2 and 17.8
+// at 128 tokens, 24.8 and 22.3 at 256, 401 and 181 at 4096; 104 fp32 ones 540 and 482 at 4096.
 // umma may also run one segment more, the first for its outputs ahead (lead): of two places a
-// chain, 1x16384 32x128 took 282 us, 347 without and 384 uncut, 52 chains of 64 features at
-// 4096 tokens 62, 74 and 71.  (In attention_kernel the choice at run time costs more: 8 x 1024
-// tokens, 13 heads of 128 x 128 in fp32, 431 us, 391 without.)
+// chain, 1x16384 32x128 takes 264 us, 341 without and 350 uncut, 52 chains of 64 features at
+// 4096 tokens 67, 73 without (and uncut).  (In attention_kernel the choice at run time cost more:
+// 8 x 1024 tokens, 13 heads of 128 x 128 in fp32, 431 us, 391 without.)
 Plan plan(bool umma, int32_t dtype, int64_t nb, int64_t T, int64_t H, int64_t dk, int64_t dv) {
     Plan pl{};
     pl.umma = umma;
