@@ -32,9 +32,9 @@
 // a log decay that makes a chunk's products leave fp32's range), says so in `redo`:
 // attention_kernel, launched behind, then computes the block's whole segment.
 //
-// Measured: 16 x 4096 tokens, 16 heads of 64 x 64, 157 us (3.4 TB/s of the 541 MB that go in
-// and out; attention_kernel 349); 8 x 2048, 13 heads of 64 x 64, 44 us (104 chains leave 44 of
-// the 148 multiprocessors idle); 1 x 16384, 32 heads of 128 x 128, 253 us, in three segments
+// Measured: 16 x 4096 tokens, 16 heads of 64 x 64, 161 us (3.4 TB/s of the 541 MB that go in
+// and out; attention_kernel 390); 8 x 2048, 13 heads of 64 x 64, 44 us (104 chains leave 44 of
+// the 148 multiprocessors idle); 1 x 16384, 32 heads of 128 x 128, 254-264 us, in three segments
 // of each chain, the middle one run twice.  A chunk takes 2.0 us at 64 features (the MMAs 1.1, the
 // warps' work on P', outputs and state beside them about the whole) and 2.9 at 128 (the
 // MMAs 1.9; one buffer of Q fits, which the products with K and S must have left before
@@ -73,7 +73,7 @@ struct alignas(16) Gates {
 };
 
 // VP: planes of V w.  3 where the state itself is a result; where only outputs of bf16 come
-// of it, 2 as of the other operands (16x4096 16x64 157 us, 165 with 3).
+// of it, 2 as of the other operands (16x4096 16x64 157 us, 165 with 3, when it was chosen).
 template <int DK>
 struct Map {  // shared memory, from a 1024-byte aligned base
     static constexpr int NQ = DK == 64 ? 2 : 1, NK = DK == 64 ? 3 : 2, NV = NK;  // chunks loaded ahead
